@@ -1,0 +1,581 @@
+// mm_linattn.hip -- gfx950 linear attention with one decay for each head: chunked forward and backward
+// (mm_linattn_dev.h has the mathematics and the operands' layouts), and the single-token step.
+//
+// A walk takes one (batch row, head), or a segment of it, through its chunks in order, the state in the
+// accumulators of its waves: every tensor is read once and every output written once. Rows with too few
+// (batch row, head) pairs for the card are cut into segments; a first pass then gathers what each segment
+// adds to the state, a second joins those, and the walks start from the joined states.
+//
+// Built once per input type: this file for float32, mm_linattn_f16.hip / mm_linattn_bf16.hip, which set
+// MM_LINATTN_TYPE, for the 16-bit types.
+#ifndef MM_LINATTN_TYPE
+#define MM_LINATTN_TYPE float
+#define MM_LINATTN_COMMON
+#endif
+
+#include "mm_linattn_dev.h"
+#include "mm_linattn_host.h"
+
+namespace mm {
+namespace la {
+
+constexpr int kWaves = 4, kThreads = 64 * kWaves;
+
+template <typename T>
+__device__ __forceinline__ Rows<T> rows_of(const View &v, int64_t b, int64_t h, int d, int col0) {
+    return Rows<T>{reinterpret_cast<const T *>(v.p) + b * v.batch + (h / v.share) * v.head + col0, v.seq, d - col0, v.vec != 0};
+}
+
+// Forward walk: out = scale (masked X Y^T) V + ..., KD the padded length of X's rows, 64 NC columns of V per
+// workgroup, 16 NC per wave. DOT: also e[t] = (the product with the state alone) . Z_t, and the state at every
+// kBlock-th token into ck (the decays' gradient).
+template <typename T, int KD, int NC, bool DOT>
+__global__ void __launch_bounds__(kThreads) la_walk(const WalkArgs a) {
+    constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, PS = Cfg<T>::st, W = 64 * NC;
+    constexpr int LDX = KD + kPad, LDV = W + kPad, LDM = C + kPad;
+    constexpr int NT = C / 16 * (C / 16 + 1) / 2;   // score tiles
+    typedef Stage<T, C, KD, kThreads> SX;
+    typedef Stage<T, C, W, kThreads> SV;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    u16 *X = reinterpret_cast<u16 *>(smem), *Y = X + PI * C * LDX, *V = Y + PI * C * LDX;
+    u16 *M = V + PI * C * LDV, *Z = M + PS * C * LDM;
+    Decays<C> *dec = reinterpret_cast<Decays<C> *>(Z + (DOT ? PI * C * LDV : 0));
+    float *part = reinterpret_cast<float *>(dec + 2);
+
+    const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64;
+    int64_t id = blockIdx.x;
+    const int slice = id % a.slices; id /= a.slices;
+    const int seg = id % a.segs; id /= a.segs;
+    const int64_t h = id % a.heads, b = id / a.heads, bh = b * a.heads + h;
+    const int64_t tbeg = int64_t(seg) * a.seg_len, tend = min(a.seqlen, tbeg + a.seg_len);
+    const int col0 = slice * W, col = wave * 16 * NC;
+
+    const Rows<T> rx = rows_of<T>(a.x, b, h, a.kdim, 0), ry = rows_of<T>(a.y, b, h, a.kdim, 0);
+    const Rows<T> rv = rows_of<T>(a.v, b, h, a.cdim, col0), rz = rows_of<T>(a.z, b, h, a.cdim, col0);
+    const int64_t g0 = b * a.g_batch + h * a.g_head;
+
+    f32x4 S[KD / 16][NC];
+    load_state<KD, NC>(S, Mat{a.s0.p ? a.s0.p + (bh * a.segs + seg) * a.s0_step : nullptr, a.s0.row, a.s0.col}, a.kdim, a.cdim,
+                       col0 + col, lane);
+    zero_masked_scores<C, PS>(M, false, tid, kThreads);
+
+    SX sx, sy;
+    SV sv, sz;
+    auto load = [&](int64_t t0) {
+        const int rows = int(min(int64_t(C), tend - t0));
+        sx.load(rx, t0, rows, tid);
+        sy.load(ry, t0, rows, tid);
+        sv.load(rv, t0, rows, tid);
+        if constexpr (DOT) sz.load(rz, t0, rows, tid);
+    };
+    auto decay = [&](int64_t t0) {
+        const int64_t t = t0 + lane;
+        return lane < C && t < tend ? load_g(a.g, a.gtype, g0 + t * a.g_seq) : 0.f;
+    };
+    const int dwave = kWaves - 1;
+    float gnext = 0.f;
+    load(tbeg);
+    if (wave == dwave) {
+        make_decays<C>(dec[0], decay(tbeg), lane);
+        if (tbeg + C < tend) gnext = decay(tbeg + C);
+    }
+    int buf = 0;
+    for (int64_t t0 = tbeg; t0 < tend; t0 += C, buf ^= 1) {
+        const int rows = int(min(int64_t(C), tend - t0));
+        if constexpr (DOT) {
+            if (a.ck && t0 > 0 && t0 % kBlock == 0)
+                store_state<KD, NC>(S, Mat{a.ck + (bh * a.blocks + t0 / kBlock - 1) * a.kdim * a.cdim, a.cdim, 1}, a.kdim, a.cdim,
+                                    col0 + col, lane);
+        }
+        __syncthreads();
+        sx.store(X, tid);
+        sy.store(Y, tid);
+        sv.store(V, tid);
+        if constexpr (DOT) sz.store(Z, tid);
+        const bool more = t0 + C < tend;
+        if (more) load(t0 + C);
+        __syncthreads();
+        const Decays<C> &d = dec[buf];
+        for (int t = wave; t < NT; t += kWaves) {
+            int o = 0, n = t;
+            while (n > o) n -= ++o;
+            f32x4 s = score_tile<T, C, KD>(X, Y, o, n, lane);
+            const f32x4 f = tile_decay<C, false>(d, o, n, a.scale, lane);
+            float x[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[r] = f[r] == 0.f && o == n ? 0.f : s[r] * f[r];
+            store_scores<C, PS>(M, x, o, n, lane);
+        }
+        f32x4 O[C / 16][NC];
+        inter<T, C, KD, NC>(O, S, X, d.in, a.scale, lane);
+        if constexpr (DOT) dot_rows<T, C, NC, LDV>(O, Z, col, part + wave * C, lane);
+        if (wave == dwave && more) {
+            make_decays<C>(dec[buf ^ 1], gnext, lane);
+            if (t0 + 2 * C < tend) gnext = decay(t0 + 2 * C);
+        }
+        __syncthreads();
+        if constexpr (DOT) {
+            if (tid < rows) {
+                float e = 0.f;
+#pragma unroll
+                for (int w = 0; w < kWaves; ++w) e += part[w * C + tid];
+                a.e[bh * a.seqlen + t0 + tid] = e;
+            }
+        }
+        bf16x8 v[C / 32][NC][PI];
+        load_v<T, C, NC, LDV>(v, V, col, lane);
+        intra<T, C, NC, LDV, false>(O, v, M, V, col, lane);
+        update<T, C, KD, NC>(S, v, Y, d.out, 1.f, d.all, lane);
+        store_out<T, C, NC>(O, a.out_f32 ? static_cast<void *>(reinterpret_cast<float *>(a.out) + b * a.out_batch + h * a.out_head)
+                                         : static_cast<void *>(reinterpret_cast<T *>(a.out) + b * a.out_batch + h * a.out_head),
+                            a.out_f32, a.out_seq, t0, rows, a.cdim, col0 + col, lane);
+    }
+    if (a.s1.p && seg == a.segs - 1)
+        store_state<KD, NC>(S, Mat{a.s1.p + bh * a.kdim * a.cdim, a.s1.row, a.s1.col}, a.kdim, a.cdim, col0 + col, lane);
+    if constexpr (DOT) {
+        // The state after the last token, for the product with the last state's gradient.
+        if (a.ck && a.ck_last && seg == a.segs - 1)
+            store_state<KD, NC>(S, Mat{a.ck + (bh * a.blocks + a.blocks - 1) * a.kdim * a.cdim, a.cdim, 1}, a.kdim, a.cdim, col0 + col, lane);
+    }
+}
+
+// What each segment but the last one (REV: the first one) of a row adds to the state: sum of y_t (decay to the
+// segment's end) v_t^T into st[bh][seg], and the segment's own decay into decay[bh][seg].
+template <typename T, int KD, bool REV>
+__global__ void __launch_bounds__(kThreads) la_segments(const WalkArgs a) {
+    constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, W = 64;
+    constexpr int LDX = KD + kPad, LDV = W + kPad;
+    typedef Stage<T, C, KD, kThreads> SX;
+    typedef Stage<T, C, W, kThreads> SV;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    u16 *Y = reinterpret_cast<u16 *>(smem), *V = Y + PI * C * LDX;
+    Decays<C> *dec = reinterpret_cast<Decays<C> *>(V + PI * C * LDV);
+    const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64;
+    int64_t id = blockIdx.x;
+    const int slice = id % a.slices; id /= a.slices;
+    const int seg = id % a.segs; id /= a.segs;
+    const int64_t h = id % a.heads, b = id / a.heads, bh = b * a.heads + h;
+    if (seg == (REV ? 0 : a.segs - 1)) return;
+    const int64_t tbeg = int64_t(seg) * a.seg_len, tend = min(a.seqlen, tbeg + a.seg_len);
+    const int64_t chunks = (tend - tbeg + C - 1) / C;
+    const int col0 = slice * W, col = wave * 16;
+    const Rows<T> ry = rows_of<T>(a.y, b, h, a.kdim, 0), rv = rows_of<T>(a.v, b, h, a.cdim, col0);
+    const int64_t g0 = b * a.g_batch + h * a.g_head;
+    f32x4 S[KD / 16][1];
+    load_state<KD, 1>(S, Mat{nullptr, 0, 0}, 0, 0, 0, lane);
+    SX sy;
+    SV sv;
+    float g = 0.f;
+    double total = 0.0;
+    auto load = [&](int64_t n) {
+        const int64_t t0 = tbeg + (REV ? chunks - 1 - n : n) * C;
+        const int rows = int(min(int64_t(C), tend - t0));
+        sy.load(ry, t0, rows, tid);
+        sv.load(rv, t0, rows, tid);
+        if (wave == 0) g = lane < rows ? load_g(a.g, a.gtype, g0 + (t0 + lane) * a.g_seq) : 0.f;
+    };
+    load(0);
+    for (int64_t n = 0; n < chunks; ++n) {
+        __syncthreads();
+        sy.store(Y, tid);
+        sv.store(V, tid);
+        if (wave == 0) {
+            make_decays<C>(*dec, g, lane);
+            total += double(dec->hi[C - 1]) + double(dec->lo[C - 1]);
+        }
+        if (n + 1 < chunks) load(n + 1);
+        __syncthreads();
+        bf16x8 v[C / 32][1][PI];
+        load_v<T, C, 1, LDV>(v, V, col, lane);
+        update<T, C, KD, 1>(S, v, Y, REV ? dec->in : dec->out, a.scale, dec->all, lane);
+    }
+    store_state<KD, 1>(S, Mat{a.st + (bh * a.segs + seg) * a.kdim * a.cdim, a.cdim, 1}, a.kdim, a.cdim, col0 + col, lane);
+    if (slice == 0 && tid == 0) a.seg_decay[bh * a.segs + seg] = expf(float(total));
+}
+
+// Backward walk from the end: dv, dk, the scores' part of the decays' gradient (a), the state's part (f), and at
+// every kBlock-th token the product of the state there with its gradient (y). Waves 0 to 3 hold the gradient R of the
+// state for dv (rows dk, columns dv), waves 4 to 7 its transpose for dk.
+template <typename T, int KD, int VD>
+__global__ void __launch_bounds__(2 * kThreads) la_bwd(const BwdArgs a) {
+    constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, PS = Cfg<T>::st, NT2 = 2 * kThreads;
+    constexpr int LDK = KD + kPad, LDV = VD + kPad, LDM = C + kPad, CT = C / 16;
+    constexpr int NT = CT * (CT + 1) / 2, NV = VD / 64, NK = KD / 64;
+    typedef Stage<T, C, KD, NT2> SK;
+    typedef Stage<T, C, VD, NT2> SV;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    u16 *Q = reinterpret_cast<u16 *>(smem), *K = Q + PI * C * LDK, *V = K + PI * C * LDK, *G = V + PI * C * LDV;
+    u16 *M1 = G + PI * C * LDV, *M2 = M1 + PS * C * LDM;
+    Decays<C> *dec = reinterpret_cast<Decays<C> *>(M2 + PS * C * LDM);
+    float *rowp = reinterpret_cast<float *>(dec + 2), *colp = rowp + CT * C, *part = colp + CT * C;
+
+    const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64;
+    int64_t id = blockIdx.x;
+    const int seg = id % a.segs; id /= a.segs;
+    const int64_t h = id % a.heads, b = id / a.heads, bh = b * a.heads + h;
+    const int64_t tbeg = int64_t(seg) * a.seg_len, tend = min(a.seqlen, tbeg + a.seg_len);
+    const int64_t chunks = (tend - tbeg + C - 1) / C;
+    const Rows<T> rq = rows_of<T>(a.q, b, h, a.dk, 0), rk = rows_of<T>(a.k, b, h, a.dk, 0);
+    const Rows<T> rv = rows_of<T>(a.v, b, h, a.dv, 0), rd = rows_of<T>(a.dout, b, h, a.dv, 0);
+    const int64_t g0 = b * a.g_batch + h * a.g_head;
+    const bool for_v = wave < kWaves;
+    const int col = (wave % kWaves) * 16 * (for_v ? NV : NK);
+
+    // R at the segment's end.
+    const float *r0 = a.r0 ? a.r0 + (bh * a.segs + seg) * int64_t(a.dk) * a.dv : nullptr;
+    f32x4 SV_[KD / 16][NV], SK_[VD / 16][NK];
+    if (for_v) {
+        load_state<KD, NV>(SV_, Mat{const_cast<float *>(r0), a.dv, 1}, a.dk, a.dv, col, lane);
+    } else {
+        load_state<VD, NK>(SK_, Mat{const_cast<float *>(r0), 1, a.dv}, a.dv, a.dk, col, lane);
+    }
+    // <R, state> at a kept boundary, each wave's share.
+    auto boundary = [&](int64_t m) {
+        const float *s = a.ck + (bh * a.blocks + m) * int64_t(a.dk) * a.dv;   // rows dv, columns dk
+        const int g = lane / 16, i = lane % 16;
+        float sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < VD / 16; ++k)
+#pragma unroll
+            for (int c = 0; c < NK; ++c)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int y = 16 * k + 4 * g + r, x = col + 16 * c + i;
+                    if (y < a.dv && x < a.dk) sum = __builtin_fmaf(SK_[k][c][r], s[int64_t(y) * a.dk + x], sum);
+                }
+        sum = wave_sum(sum);
+        if (lane == 0) a.y[(bh * a.blocks + m) * kWaves + wave - kWaves] = sum;
+    };
+    if (!for_v && a.ck && a.has_last && seg == a.segs - 1) boundary(a.blocks - 1);
+
+    zero_masked_scores<C, PS>(M1, true, tid, NT2);
+    zero_masked_scores<C, PS>(M2, true, tid, NT2);
+    SK sq, sk;
+    SV sv, sd;
+    auto start = [&](int64_t n) { return tbeg + (chunks - 1 - n) * C; };
+    auto load = [&](int64_t n) {
+        const int64_t t0 = start(n);
+        const int rows = int(min(int64_t(C), tend - t0));
+        sq.load(rq, t0, rows, tid);
+        sk.load(rk, t0, rows, tid);
+        sv.load(rv, t0, rows, tid);
+        sd.load(rd, t0, rows, tid);
+    };
+    auto decay = [&](int64_t n) {
+        const int64_t t = start(n) + lane;
+        return lane < C && t < tend ? load_g(a.g, a.gtype, g0 + t * a.g_seq) : 0.f;
+    };
+    const int dwave = 2 * kWaves - 1;
+    float gnext = 0.f;
+    load(0);
+    if (wave == dwave) {
+        make_decays<C>(dec[0], decay(0), lane);
+        if (chunks > 1) gnext = decay(1);
+    }
+    int buf = 0;
+    for (int64_t n = 0; n < chunks; ++n, buf ^= 1) {
+        const int64_t t0 = start(n);
+        const int rows = int(min(int64_t(C), tend - t0));
+        __syncthreads();
+        sq.store(Q, tid);
+        sk.store(K, tid);
+        sv.store(V, tid);
+        sd.store(G, tid);
+        const bool more = n + 1 < chunks;
+        if (more) load(n + 1);
+        __syncthreads();
+        const Decays<C> &d = dec[buf];
+        for (int t = wave; t < NT; t += 2 * kWaves) {
+            int x = 0, y = t;
+            while (y > x) y -= ++x;
+            const int o = y, m = x;   // row token tile o sees tile m >= o
+            const f32x4 p = score_tile<T, C, KD>(K, Q, o, m, lane), dp = score_tile<T, C, VD>(V, G, o, m, lane);
+            const f32x4 f = tile_decay<C, true>(d, o, m, a.scale, lane);
+            float s1[4], s2[4], w[4], cs = 0.f;
+            const int jj = 16 * o + lane % 16, ii = 16 * m + 4 * (lane / 16);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const bool sees = ii + r >= jj;
+                s1[r] = sees ? p[r] * f[r] : 0.f;
+                s2[r] = sees ? dp[r] * f[r] : 0.f;
+                w[r] = ii + r > jj ? p[r] * dp[r] * f[r] : 0.f;
+                cs += w[r];
+            }
+            store_scores<C, PS>(M1, s1, o, m, lane);
+            store_scores<C, PS>(M2, s2, o, m, lane);
+            if (a.a) {
+                // Sums over the seen tokens j (for each i) and over the seeing tokens i (for each j) of the tile.
+                f32x4 rs;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) rs[r] = group_sum<16>(w[r]);
+                cs += __shfl_xor(cs, 16);
+                cs += __shfl_xor(cs, 32);
+                if (lane % 16 == 0) *reinterpret_cast<f32x4 *>(&rowp[o * C + ii]) = rs;
+                if (lane < 16) colp[m * C + jj] = cs;
+            }
+        }
+        f32x4 OV[CT][NV], OK[CT][NK];
+        if (for_v) {
+            inter<T, C, KD, NV>(OV, SV_, K, d.out, 1.f, lane);
+        } else {
+            inter<T, C, VD, NK>(OK, SK_, V, d.out, 1.f, lane);
+            if (a.a) dot_rows<T, C, NK, LDK>(OK, K, col, part + (wave - kWaves) * C, lane);
+        }
+        if (wave == dwave && more) {
+            make_decays<C>(dec[buf ^ 1], gnext, lane);
+            if (n + 2 < chunks) gnext = decay(n + 2);
+        }
+        __syncthreads();
+        if (a.a && tid < rows) {
+            const int t = tid / 16;
+            float sum = 0.f, f = 0.f;
+            for (int o = 0; o <= t; ++o) sum += rowp[o * C + tid];
+            for (int m = t; m < CT; ++m) sum -= colp[m * C + tid];
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) f += part[w * C + tid];
+            a.a[bh * a.seqlen + t0 + tid] = sum;
+            a.f[bh * a.seqlen + t0 + tid] = f;
+        }
+        if (for_v) {
+            bf16x8 v[C / 32][NV][PI];
+            load_v<T, C, NV, LDV>(v, G, col, lane);
+            intra<T, C, NV, LDV, true>(OV, v, M1, G, col, lane);
+            update<T, C, KD, NV>(SV_, v, Q, d.in, a.scale, d.all, lane);
+            store_out<T, C, NV>(OV, reinterpret_cast<T *>(a.dv_out) + (b * a.seqlen * a.heads + h) * a.dv, false, a.heads * a.dv, t0, rows,
+                                a.dv, col, lane);
+        } else {
+            bf16x8 v[C / 32][NK][PI];
+            load_v<T, C, NK, LDK>(v, Q, col, lane);
+            intra<T, C, NK, LDK, true>(OK, v, M2, Q, col, lane);
+            update<T, C, VD, NK>(SK_, v, G, d.in, a.scale, d.all, lane);
+            const int64_t at = (b * a.seqlen * a.heads + h) * a.dk;
+            store_out<T, C, NK>(OK, a.dk_f32 ? static_cast<void *>(reinterpret_cast<float *>(a.dk_out) + at)
+                                             : static_cast<void *>(reinterpret_cast<T *>(a.dk_out) + at),
+                                a.dk_f32, a.heads * a.dk, t0, rows, a.dk, col, lane);
+            if (a.ck && t0 > 0 && t0 % kBlock == 0) boundary(t0 / kBlock - 1);
+        }
+    }
+    if (a.dr && seg == 0 && for_v)
+        store_state<KD, NV>(SV_, Mat{a.dr + bh * int64_t(a.dk) * a.dv, a.dv, 1}, a.dk, a.dv, col, lane);
+}
+
+template <typename T, int KD, int NC, bool DOT>
+static int launch_walk_t(const WalkArgs &a, hipStream_t s) {
+    constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, PS = Cfg<T>::st;
+    constexpr int bytes = 2 * (2 * PI * C * (KD + kPad) + (DOT ? 2 : 1) * PI * C * (64 * NC + kPad) + PS * C * (C + kPad)) +
+                          2 * int(sizeof(Decays<C>)) + (DOT ? 4 * kWaves * C : 0);
+    static_assert(bytes <= 160 * 1024, "LDS");
+    static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void *>(la_walk<T, KD, NC, DOT>),
+                                                      hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (set != hipSuccess) return set_error(int(set), "linear attention: hipFuncSetAttribute failed");
+    const int64_t grid = a.batch * a.heads * a.segs * a.slices;
+    hipLaunchKernelGGL((la_walk<T, KD, NC, DOT>), dim3(unsigned(grid)), dim3(kThreads), bytes, s, a);
+    return launch_status("la_walk");
+}
+
+template <typename T, int KD, bool REV>
+static int launch_segments_t(const WalkArgs &a0, hipStream_t s) {
+    constexpr int C = Cfg<T>::C, PI = Cfg<T>::in;
+    constexpr int bytes = 2 * (PI * C * (KD + kPad) + PI * C * (64 + kPad)) + int(sizeof(Decays<C>));
+    static_assert(bytes <= 160 * 1024, "LDS");
+    static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void *>(la_segments<T, KD, REV>),
+                                                      hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (set != hipSuccess) return set_error(int(set), "linear attention: hipFuncSetAttribute failed");
+    WalkArgs a = a0;
+    a.slices = (a.cdim + 63) / 64;
+    const int64_t grid = a.batch * a.heads * a.segs * a.slices;
+    hipLaunchKernelGGL((la_segments<T, KD, REV>), dim3(unsigned(grid)), dim3(kThreads), bytes, s, a);
+    return launch_status("la_segments");
+}
+
+template <typename T, int KD, int VD>
+static int launch_bwd_t(const BwdArgs &a, hipStream_t s) {
+    constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, PS = Cfg<T>::st;
+    constexpr int bytes = 2 * (2 * PI * C * (KD + kPad) + 2 * PI * C * (VD + kPad) + 2 * PS * C * (C + kPad)) +
+                          2 * int(sizeof(Decays<C>)) + 4 * (2 * (C / 16) * C + kWaves * C);
+    static_assert(bytes <= 160 * 1024, "LDS");
+    static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void *>(la_bwd<T, KD, VD>),
+                                                      hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (set != hipSuccess) return set_error(int(set), "linear attention: hipFuncSetAttribute failed");
+    const int64_t grid = a.batch * a.heads * a.segs;
+    hipLaunchKernelGGL((la_bwd<T, KD, VD>), dim3(unsigned(grid)), dim3(2 * kThreads), bytes, s, a);
+    return launch_status("la_bwd");
+}
+
+template <typename T>
+int launch_walk(const WalkArgs &a, bool dot, hipStream_t s) {
+    const bool wide = a.cdim > 64;
+    if (dot) {
+        if (a.kdim <= 64) return wide ? launch_walk_t<T, 64, 2, true>(a, s) : launch_walk_t<T, 64, 1, true>(a, s);
+        return wide ? launch_walk_t<T, 128, 2, true>(a, s) : launch_walk_t<T, 128, 1, true>(a, s);
+    }
+    if (a.kdim <= 32) return wide ? launch_walk_t<T, 32, 2, false>(a, s) : launch_walk_t<T, 32, 1, false>(a, s);
+    if (a.kdim <= 64) return wide ? launch_walk_t<T, 64, 2, false>(a, s) : launch_walk_t<T, 64, 1, false>(a, s);
+    return wide ? launch_walk_t<T, 128, 2, false>(a, s) : launch_walk_t<T, 128, 1, false>(a, s);
+}
+
+template <typename T>
+int launch_segments(const WalkArgs &a, bool rev, hipStream_t s) {
+    if (a.kdim <= 64) return rev ? launch_segments_t<T, 64, true>(a, s) : launch_segments_t<T, 64, false>(a, s);
+    return rev ? launch_segments_t<T, 128, true>(a, s) : launch_segments_t<T, 128, false>(a, s);
+}
+
+template <typename T>
+int launch_bwd(const BwdArgs &a, hipStream_t s) {
+    if (a.dk <= 64) return a.dv <= 64 ? launch_bwd_t<T, 64, 64>(a, s) : launch_bwd_t<T, 64, 128>(a, s);
+    return a.dv <= 64 ? launch_bwd_t<T, 128, 64>(a, s) : launch_bwd_t<T, 128, 128>(a, s);
+}
+
+template int launch_walk<MM_LINATTN_TYPE>(const WalkArgs &, bool, hipStream_t);
+template int launch_segments<MM_LINATTN_TYPE>(const WalkArgs &, bool, hipStream_t);
+template int launch_bwd<MM_LINATTN_TYPE>(const BwdArgs &, hipStream_t);
+
+#ifdef MM_LINATTN_COMMON
+// ---- joins and sums ------------------------------------------------------------------------------
+
+// The segments' shares in st[bh][seg] become the states the segments start from (rev: end with).
+__global__ void __launch_bounds__(256) la_join(float *st, const float *decay, const float *edge, int segs, int64_t size, bool rev) {
+    const int64_t bh = blockIdx.y, x = int64_t(blockIdx.x) * 256 + threadIdx.x;
+    if (x >= size) return;
+    float cur = edge ? edge[bh * size + x] : 0.f;
+    float *p = st + bh * segs * size + x;
+    for (int n = 0; n < segs; ++n) {
+        const int seg = rev ? segs - 1 - n : n;
+        const float add = n + 1 < segs ? p[seg * size] : 0.f;
+        p[seg * size] = cur;
+        if (n + 1 < segs) cur = __builtin_fmaf(decay[bh * segs + seg], cur, add);
+    }
+}
+
+// out[row][x] = sum over the group's heads of part[row][head][x], in order.
+template <typename T>
+__global__ void __launch_bounds__(256) la_head_sum(const float *part, T *out, int64_t n, int heads, int share, int d) {
+    const int64_t at = int64_t(blockIdx.x) * 256 + threadIdx.x;
+    if (at >= n) return;
+    const int64_t x = at % d, rg = at / d, groups = heads / share, row = rg / groups, grp = rg % groups;
+    const float *p = part + (row * heads + grp * share) * d + x;
+    float s = 0.f;
+    for (int r = 0; r < share; ++r) s += p[int64_t(r) * d];
+    out[at] = from_f32<T>(s);
+}
+
+__device__ __forceinline__ void store_g(void *p, mm_dtype t, int64_t i, float x) {
+    switch (t) {
+        case MM_FLOAT32: reinterpret_cast<float *>(p)[i] = x; break;
+        case MM_FLOAT16: reinterpret_cast<f16_t *>(p)[i] = from_f32<f16_t>(x); break;
+        default: reinterpret_cast<bf16_t *>(p)[i] = from_f32<bf16_t>(x);
+    }
+}
+
+// The gradient of a log decay is the sum of W_ij = scale exp(c_i - c_j) (q_i . k_j) (do_i . v_j) over the pairs that it
+// lies between, j < t <= i. Cut at t's chunk, with S the state before and R the state's gradient after the chunk: pairs
+// inside it (a holds each token's row sum less its column sum, the diagonal left out), pairs from before into it (e_i),
+// pairs from it to behind (f_j), and pairs around it, Z = exp(c_end) <R, S>. No part is a difference of larger ones but
+// Z, which is <R, S'> less the chunk's f; <R, S'> is taken from the states themselves every kBlock tokens. One workgroup
+// per block and (batch row, head); C: the chunk's tokens.
+__global__ void __launch_bounds__(kBlock) la_decay_grad(const float *a, const float *e, const float *f, const float *y, int64_t seqlen,
+                                                        int64_t blocks, int heads, int C, bool has_last, const void *g, int64_t g_batch,
+                                                        int64_t g_seq, int64_t g_head, float *tmp, void *out, mm_dtype gtype) {
+    __shared__ float sa[kBlock], sf[kBlock], se[kBlock], zc[kBlock / 16];
+    const int64_t blk = blockIdx.x, bh = blockIdx.y, t = blk * kBlock + threadIdx.x;
+    const int tid = threadIdx.x, chunks = kBlock / C;
+    const bool live = t < seqlen;
+    const float ae = live ? e[bh * seqlen + t] : 0.f;
+    sa[tid] = (live ? a[bh * seqlen + t] : 0.f) + ae;
+    sf[tid] = live ? f[bh * seqlen + t] : 0.f;
+    se[tid] = ae;
+    __syncthreads();
+    if (tid < chunks) {   // the chunks' totals
+        float E = 0.f, F = 0.f;
+        for (int n = 0; n < C; ++n) {
+            E += se[tid * C + n];
+            F += sf[tid * C + n];
+        }
+        zc[tid] = E;
+        zc[chunks + tid] = F;
+    }
+    __syncthreads();
+    if (tid == 0) {
+        float Y = 0.f;
+        if (blk + 1 < blocks || has_last)
+            for (int w = 0; w < 4; ++w) Y += y[(bh * blocks + blk) * 4 + w];
+        for (int c = chunks - 1; c >= 0; --c) {
+            const float Z = Y - zc[chunks + c];
+            Y = Z + zc[c];
+            zc[c] = Z;
+        }
+    }
+    __syncthreads();
+    if (!live) return;
+    const int c0 = tid / C * C;
+    float s = zc[tid / C];
+    for (int n = c0; n < tid; ++n) s += sf[n];
+    for (int n = c0 + C - 1; n >= tid; --n) s += sa[n];
+    // A forgotten state has no gradient; the sums above are of terms that cancel.
+    if (load_g(g, gtype, bh / heads * g_batch + t * g_seq + bh % heads * g_head) == -128.f) s = 0.f;
+    if (tmp) tmp[bh * seqlen + t] = s;
+    else store_g(out, gtype, (bh / heads * seqlen + t) * heads + bh % heads, s);
+}
+
+// dlog_decay[h] = sum over batch rows and tokens, one workgroup per head.
+__global__ void __launch_bounds__(256) la_decay_sum(const float *tmp, int64_t batch, int64_t heads, int64_t seqlen, void *out, mm_dtype gtype) {
+    __shared__ float part[256];
+    const int64_t h = blockIdx.x;
+    float s = 0.f;
+    for (int64_t b = 0; b < batch; ++b)
+        for (int64_t t = threadIdx.x; t < seqlen; t += 256) s += tmp[(b * heads + h) * seqlen + t];
+    part[threadIdx.x] = s;
+    for (int n = 128; n > 0; n /= 2) {
+        __syncthreads();
+        if (int(threadIdx.x) < n) part[threadIdx.x] += part[threadIdx.x + n];
+    }
+    if (threadIdx.x == 0) store_g(out, gtype, h, part[0]);
+}
+
+__global__ void __launch_bounds__(256) la_copy(float *dst, const float *src, int64_t n) {
+    const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
+    if (i < n) dst[i] = src ? src[i] : 0.f;
+}
+__global__ void __launch_bounds__(256) la_zero_g(void *dst, mm_dtype t, int64_t n) {
+    const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
+    if (i < n) store_g(dst, t, i, 0.f);
+}
+
+static unsigned blocks_of(int64_t n) { return unsigned((n + 255) / 256); }
+
+int launch_join(float *st, const float *decay, const float *edge, int segs, int64_t size, int64_t bh, bool rev, hipStream_t s) {
+    hipLaunchKernelGGL(la_join, dim3(blocks_of(size), unsigned(bh)), dim3(256), 0, s, st, decay, edge, segs, size, rev);
+    return launch_status("la_join");
+}
+
+int launch_head_sum(const float *part, void *out, mm_dtype t, int64_t rows, int heads, int share, int d, hipStream_t s) {
+    const int64_t n = rows * (heads / share) * d;
+    const dim3 grid(blocks_of(n)), blk(256);
+    if (t == MM_FLOAT32) hipLaunchKernelGGL(la_head_sum<float>, grid, blk, 0, s, part, static_cast<float *>(out), n, heads, share, d);
+    else if (t == MM_FLOAT16) hipLaunchKernelGGL(la_head_sum<f16_t>, grid, blk, 0, s, part, static_cast<f16_t *>(out), n, heads, share, d);
+    else hipLaunchKernelGGL(la_head_sum<bf16_t>, grid, blk, 0, s, part, static_cast<bf16_t *>(out), n, heads, share, d);
+    return launch_status("la_head_sum");
+}
+
+int launch_decay_grad(const BwdArgs &a, const float *e, int C, bool per_head, void *out, mm_dtype gtype, hipStream_t s) {
+    // The sums over a head's tokens go through f's place, which a block reads before it writes.
+    hipLaunchKernelGGL(la_decay_grad, dim3(unsigned(a.blocks), unsigned(a.batch * a.heads)), dim3(kBlock), 0, s, a.a, e, a.f, a.y, a.seqlen,
+                       a.blocks, int(a.heads), C, a.has_last != 0, a.g, a.g_batch, a.g_seq, a.g_head, per_head ? a.f : nullptr, out, gtype);
+    if (const int rc = launch_status("la_decay_grad")) return rc;
+    if (!per_head) return MM_OK;
+    hipLaunchKernelGGL(la_decay_sum, dim3(unsigned(a.heads)), dim3(256), 0, s, a.f, a.batch, a.heads, a.seqlen, out, gtype);
+    return launch_status("la_decay_sum");
+}
+
+int launch_copy(float *dst, const float *src, int64_t n, hipStream_t s) {
+    hipLaunchKernelGGL(la_copy, dim3(blocks_of(n)), dim3(256), 0, s, dst, src, n);
+    return launch_status("la_copy");
+}
+int launch_zero_g(void *dst, mm_dtype t, int64_t n, hipStream_t s) {
+    hipLaunchKernelGGL(la_zero_g, dim3(blocks_of(n)), dim3(256), 0, s, dst, t, n);
+    return launch_status("la_zero_g");
+}
+#endif  // MM_LINATTN_COMMON
+
+}  // namespace la
+}  // namespace mm

@@ -1,0 +1,617 @@
+// mm_linattn_dev.h -- device pieces of the chunked linear attention with one decay for each head
+// (mm_linattn.hip): the operand planes, the tiles' staging, and a chunk's steps.
+//
+// The mathematics. With c_i the sum of log_decay over a chunk's tokens up to i (c_end its total), a chunk
+// of C tokens that starts from the state S (dk x dv) gives
+//     o_i  = exp(c_i) q_i S + sum_{j <= i} exp(c_i - c_j) (q_i . k_j) v_j
+//     S'   = exp(c_end) S + sum_j k_j (exp(c_end - c_j) v_j)^T
+// and each of the three gradients of q, k and v is a walk of the same form: dq_i the forward one with
+// (do, v, k) in the place of (q, k, v), dv_j and dk_j the one from the end with (k, q, do) and (v, do, q),
+// whose row factor is exp(c_end - c_j) and whose update factor exp(c_i). A walk is named here by its
+// tiles: X (C x KD, the rows' factor), Y (C x KD, what the state is built from), V (C x columns).
+//
+// Exactness. Products run on v_mfma_f32_16x16x32_bf16, which multiplies bfloat16 exactly and adds in
+// float32. Every other number is carried as a sum of bfloat16 planes: float16 inputs as two and float32
+// inputs as three (both exact), the state and the decayed scores as two (relative error 2^-17, three for
+// float32 inputs), the decayed rows the state is built from as three (2^-25). So the state itself is
+// float32 from end to end and 16-bit outputs are rounded once.
+//
+// Lane layouts (l the lane, g = l / 16, i = l % 16; checked on the card): an accumulator tile holds column
+// i, rows 4g .. 4g + 3. An operand holds row (A) or column (B) i and eight of 32 contraction indices; the
+// order of those is free as long as A and B agree, and here it is {4g .. 4g + 3, 16 + 4g .. 16 + 4g + 3}:
+// two accumulator tiles, one below the other, ARE a B operand, so the state goes from the accumulators of
+// its update into the product with X without leaving the registers.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include "mm_common.h"
+#include "mm_internal.h"
+#include "mm_linattn.h"
+
+namespace mm {
+namespace la {
+
+typedef uint16_t u16;
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+// Planes of an input, of the state and the scores, of the update's rows; tokens of a chunk.
+template <typename T> struct Cfg;
+template <> struct Cfg<bf16_t> { static constexpr int in = 1, st = 2, up = 3, C = 64; };
+template <> struct Cfg<f16_t> { static constexpr int in = 2, st = 2, up = 3, C = 32; };
+template <> struct Cfg<float> { static constexpr int in = 3, st = 3, up = 3, C = 32; };
+
+constexpr int kBlock = 256;      // tokens between two kept states (see the decays' gradient)
+constexpr int kPad = 8;          // elements after an LDS row: 16 rows then start in 16 different bank groups
+
+__device__ __forceinline__ float load_g(const void *p, mm_dtype t, int64_t i) {
+    float x;
+    switch (t) {
+        case MM_FLOAT32: x = reinterpret_cast<const float *>(p)[i]; break;
+        case MM_FLOAT16: x = to_f32(reinterpret_cast<const f16_t *>(p)[i]); break;
+        default: x = to_f32(reinterpret_cast<const bf16_t *>(p)[i]);
+    }
+    // exp(-128) is 0 in float32 as every smaller decay is; a finite sum keeps the differences of two
+    // sums defined. The comparison is false for NaN, which stays.
+    return x < -128.f ? -128.f : x;
+}
+
+// ---- planes --------------------------------------------------------------------------------------
+
+// x as a sum of N bfloat16 planes, each the nearest of what is left.
+template <int N>
+__device__ __forceinline__ void split8(const float *x, bf16x8 *out) {
+    float r[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = x[i];
+#pragma unroll
+    for (int p = 0; p < N; ++p) {
+        u32x4 w;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = pack_bf16x2(r[2 * i], r[2 * i + 1]);
+        out[p] = __builtin_bit_cast(bf16x8, w);
+        if (p + 1 < N) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                r[2 * i] -= __uint_as_float(w[i] << 16);
+                r[2 * i + 1] -= __uint_as_float(w[i] & 0xffff0000u);
+            }
+        }
+    }
+}
+
+// acc += A B over the pairs of planes whose ranks sum below MAXS (the others are below the last plane).
+template <int NA, int NB, int MAXS>
+__device__ __forceinline__ f32x4 mma(f32x4 acc, const bf16x8 *a, const bf16x8 *b) {
+#pragma unroll
+    for (int i = 0; i < NA; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+            if (i + j < MAXS) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[j], acc, 0, 0, 0);
+    return acc;
+}
+
+__device__ __forceinline__ bf16x8 join(uint2 a, uint2 b) {
+    return __builtin_bit_cast(bf16x8, u32x4{a.x, a.y, b.x, b.y});
+}
+// Operand with its row in `row` (an LDS row's start), contraction columns col .. col + 31.
+__device__ __forceinline__ bf16x8 frag_row(const u16 *row, int col, int g) {
+    return join(*reinterpret_cast<const uint2 *>(row + col + 4 * g), *reinterpret_cast<const uint2 *>(row + col + 16 + 4 * g));
+}
+// Operand whose row or column is tile column col + i and whose contraction runs over tile rows r0 .. r0 + 31.
+template <int LD>
+__device__ __forceinline__ bf16x8 frag_tr(const u16 *tile, int r0, int col, int g, int i) {
+    const u16 *a = tile + (r0 + 4 * g + i / 4) * LD + col + 4 * (i % 4);
+    typedef __attribute__((address_space(3))) s16x4 *lds_ptr;
+    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)a);
+    const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(a + 16 * LD));
+    return join(__builtin_bit_cast(uint2, x), __builtin_bit_cast(uint2, y));
+}
+
+__device__ __forceinline__ void unpack_frag(const bf16x8 &f, float *x) {
+    const u32x4 w = __builtin_bit_cast(u32x4, f);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        x[2 * k] = __uint_as_float(w[k] << 16);
+        x[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+    }
+}
+
+// ---- staging -------------------------------------------------------------------------------------
+
+// A tensor's rows of one (batch row, head): token t at p + t * stride.
+template <typename T> struct Rows {
+    const T *p;
+    int64_t stride;
+    int d;           // elements of a row that exist
+    bool vec;        // 16-byte accesses (rows and d are multiples of 16 bytes)
+};
+
+// A C x D tile on its way from memory to LDS, 16 bytes per thread and step, in registers.
+template <typename T, int C, int D, int NT>
+struct Stage {
+    static constexpr int VE = 16 / sizeof(T), VR = D / VE, N = (C * VR + NT - 1) / NT;
+    static constexpr int LD = D + kPad, PLANE = C * LD;
+    static constexpr bool kEven = C * VR % NT == 0;
+    uint4 r[N];
+
+    __device__ __forceinline__ void load(const Rows<T> &s, int64_t t0, int rows, int tid) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int idx = tid + n * NT, row = idx / VR, col = idx % VR * VE;
+            uint4 x = make_uint4(0, 0, 0, 0);
+            if ((kEven || idx < C * VR) && row < rows && col < s.d) {
+                const T *src = s.p + (t0 + row) * s.stride + col;
+                if (s.vec) {
+                    x = *reinterpret_cast<const uint4 *>(src);
+                } else {
+                    uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+                    for (int e = 0; e < VE; ++e)
+                        if (col + e < s.d) {
+                            if constexpr (sizeof(T) == 4) w[e] = *reinterpret_cast<const uint32_t *>(src + e);
+                            else w[e / 2] |= uint32_t(*reinterpret_cast<const u16 *>(src + e)) << (16 * (e % 2));
+                        }
+                    x = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            }
+            r[n] = x;
+        }
+    }
+
+    // Into the tile's planes. float16 and float32 are cut after 8 significant bits per plane, which is exact;
+    // an infinity or NaN stands in the first plane alone.
+    __device__ __forceinline__ void store(u16 *tile, int tid) const {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int idx = tid + n * NT, row = idx / VR, col = idx % VR * VE;
+            if (!kEven && idx >= C * VR) break;
+            u16 *dst = tile + row * LD + col;
+            const uint32_t w[4] = {r[n].x, r[n].y, r[n].z, r[n].w};
+            if constexpr (std::is_same_v<T, bf16_t>) {
+                *reinterpret_cast<uint4 *>(dst) = r[n];
+            } else {
+                constexpr int P = Cfg<T>::in;
+                uint32_t o[P][VE / 2];
+                float x[VE];
+#pragma unroll
+                for (int e = 0; e < VE; ++e) x[e] = elem_f32<T>(sizeof(T) == 4 ? w[e] : (w[e / 2] >> (16 * (e % 2))) & 0xffffu);
+#pragma unroll
+                for (int e = 0; e < VE; ++e) {
+                    const uint32_t b = __float_as_uint(x[e]);
+                    const bool fin = (b & 0x7f800000u) != 0x7f800000u;
+                    uint32_t h = b & 0xffff0000u;
+                    if (!fin && (b & 0x007fffffu)) h |= 0x00400000u;   // NaN whatever its payload
+                    float rest = fin ? x[e] - __uint_as_float(h) : 0.f;
+#pragma unroll
+                    for (int p = 0; p < P; ++p) {
+                        if (e % 2 == 0) o[p][e / 2] = h >> 16;
+                        else o[p][e / 2] |= h;
+                        h = __float_as_uint(rest) & 0xffff0000u;
+                        rest -= __uint_as_float(h);
+                    }
+                }
+#pragma unroll
+                for (int p = 0; p < P; ++p) {
+                    if constexpr (VE == 8) *reinterpret_cast<uint4 *>(dst + p * PLANE) = make_uint4(o[p][0], o[p][1], o[p][2], o[p][3]);
+                    else *reinterpret_cast<uint2 *>(dst + p * PLANE) = make_uint2(o[p][0], o[p][1]);
+                }
+            }
+        }
+    }
+};
+
+// ---- decays of a chunk ---------------------------------------------------------------------------
+
+// All from sums taken in float64 over the chunk's tokens, so that a difference of two sums is as good as
+// its own sum: scores of 16-token tiles off the diagonal take the product of three factors, each the
+// exponential of a sum of log decays (at most 1 where those are at most 0: nothing overflows, and a
+// forgotten state gives 0, never 0 times infinity), tiles on the diagonal exp(c_i - c_j) itself.
+template <int C>
+struct __attribute__((aligned(16))) Decays {
+    float in[C];           // exp(c_t): from the chunk's start, t's own decay included
+    float out[C];          // exp(c_end - c_t)
+    float from[C];         // exp(c_t - the sum before t's tile)
+    float to[C];           // exp(the sum up to the end of t's tile - c_t)
+    float hi[C], lo[C];    // c_t
+    float mid[C / 16][C / 16];   // [I][J], J < I: from the end of tile J to the start of tile I
+    float all;             // exp(c_end)
+};
+
+template <int CTRL>
+__device__ __forceinline__ double dpp_add_f64(double x, int row_mask) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, x);
+    uint32_t lo, hi;
+    if (row_mask == 0xf) {
+        lo = __builtin_amdgcn_update_dpp(0, int(uint32_t(b)), CTRL, 0xf, 0xf, false);
+        hi = __builtin_amdgcn_update_dpp(0, int(uint32_t(b >> 32)), CTRL, 0xf, 0xf, false);
+    } else if (row_mask == 0xa) {
+        lo = __builtin_amdgcn_update_dpp(0, int(uint32_t(b)), CTRL, 0xa, 0xf, false);
+        hi = __builtin_amdgcn_update_dpp(0, int(uint32_t(b >> 32)), CTRL, 0xa, 0xf, false);
+    } else {
+        lo = __builtin_amdgcn_update_dpp(0, int(uint32_t(b)), CTRL, 0xc, 0xf, false);
+        hi = __builtin_amdgcn_update_dpp(0, int(uint32_t(b >> 32)), CTRL, 0xc, 0xf, false);
+    }
+    return x + __builtin_bit_cast(double, uint64_t(lo) | uint64_t(hi) << 32);
+}
+__device__ __forceinline__ double readlane_f64(double x, int lane) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = __builtin_amdgcn_readlane(int(uint32_t(b)), lane);
+    const uint32_t hi = __builtin_amdgcn_readlane(int(uint32_t(b >> 32)), lane);
+    return __builtin_bit_cast(double, uint64_t(lo) | uint64_t(hi) << 32);
+}
+// Sum over the lanes up to and including this one.
+__device__ __forceinline__ double prefix_f64(double x) {
+    x = dpp_add_f64<0x111>(x, 0xf);   // row_shr 1, 2, 4, 8: within 16 lanes
+    x = dpp_add_f64<0x112>(x, 0xf);
+    x = dpp_add_f64<0x114>(x, 0xf);
+    x = dpp_add_f64<0x118>(x, 0xf);
+    x = dpp_add_f64<0x142>(x, 0xa);   // row_bcast 15 into rows 1 and 3
+    x = dpp_add_f64<0x143>(x, 0xc);   // row_bcast 31 into rows 2 and 3
+    return x;
+}
+
+// One wave; g: the lane's token's log decay, 0 behind the last token and in lanes past C.
+template <int C>
+__device__ __forceinline__ void make_decays(Decays<C> &d, float g, int lane) {
+    const double c = prefix_f64(double(g));
+    double end[C / 16], mine_end = 0.0, mine_start = 0.0;
+#pragma unroll
+    for (int t = 0; t < C / 16; ++t) {
+        end[t] = readlane_f64(c, 16 * t + 15);
+        if (lane / 16 == t) mine_end = end[t];
+        if (lane / 16 == t + 1) mine_start = end[t];
+    }
+    const double all = end[C / 16 - 1];
+    if (lane < C) {
+        d.in[lane] = expf(float(c));
+        d.out[lane] = expf(float(all - c));
+        d.from[lane] = expf(float(c - mine_start));
+        d.to[lane] = expf(float(mine_end - c));
+        const float hi = float(c);
+        d.hi[lane] = hi;
+        d.lo[lane] = float(c - double(hi));
+    }
+    if (lane == 0) d.all = expf(float(all));
+#pragma unroll
+    for (int I = 1; I < C / 16; ++I)
+#pragma unroll
+        for (int J = 0; J < I; ++J)
+            if (lane == I * 4 + J) d.mid[I][J] = expf(float(end[I - 1] - end[J]));
+}
+
+// ---- a chunk's steps -----------------------------------------------------------------------------
+
+// Scores of one 16 x 16 tile: column i the row token 16 ot + i of X, rows 4g + r the tokens 16 nt + 4g + r of Y.
+template <typename T, int C, int KD>
+__device__ __forceinline__ f32x4 score_tile(const u16 *X, const u16 *Y, int ot, int nt, int lane) {
+    constexpr int LD = KD + kPad, PL = C * LD, P = Cfg<T>::in;
+    const int g = lane / 16, i = lane % 16;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < KD / 32; ++k) {
+        bf16x8 a[P], b[P];
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            a[p] = frag_row(Y + p * PL + (16 * nt + i) * LD, 32 * k, g);
+            b[p] = frag_row(X + p * PL + (16 * ot + i) * LD, 32 * k, g);
+        }
+        acc = mma<P, P, 3>(acc, a, b);
+    }
+    return acc;
+}
+
+// The decay factors of that tile times `scale`, 0 where the token does not see the other. REV: row tokens
+// see later ones. f32x4: one factor per accumulator element.
+template <int C, bool REV>
+__device__ __forceinline__ f32x4 tile_decay(const Decays<C> &d, int ot, int nt, float scale, int lane) {
+    const int g = lane / 16, i = lane % 16;
+    const int o = 16 * ot + i, n = 16 * nt + 4 * g;
+    f32x4 f;
+    if (ot != nt) {
+        const float row = scale * (REV ? d.to[o] * d.mid[nt][ot] : d.from[o] * d.mid[ot][nt]);
+        const f32x4 col = *reinterpret_cast<const f32x4 *>(REV ? &d.from[n] : &d.to[n]);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) f[r] = row * col[r];
+    } else {
+        const f32x4 hi = *reinterpret_cast<const f32x4 *>(&d.hi[n]), lo = *reinterpret_cast<const f32x4 *>(&d.lo[n]);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const float x = (d.hi[o] - hi[r]) + (d.lo[o] - lo[r]);
+            const bool sees = REV ? n + r >= o : n + r <= o;
+            f[r] = sees ? expf(REV ? -x : x) * scale : 0.f;
+        }
+    }
+    return f;
+}
+
+// Four consecutive scores of row token 16 ot + i into the score tile's planes ([row token][other token]).
+template <int C, int P>
+__device__ __forceinline__ void store_scores(u16 *M, const float *x, int ot, int nt, int lane) {
+    constexpr int LD = C + kPad, PL = C * LD;
+    u16 *dst = M + (16 * ot + lane % 16) * LD + 16 * nt + 4 * (lane / 16);
+    float r[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+        const uint2 w = make_uint2(pack_bf16x2(r[0], r[1]), pack_bf16x2(r[2], r[3]));
+        *reinterpret_cast<uint2 *>(dst + p * PL) = w;
+        r[0] -= __uint_as_float(w.x << 16);
+        r[1] -= __uint_as_float(w.x & 0xffff0000u);
+        r[2] -= __uint_as_float(w.y << 16);
+        r[3] -= __uint_as_float(w.y & 0xffff0000u);
+    }
+}
+
+// The tiles on the masked side of the diagonal that share a 32-wide contraction with a diagonal tile are 0
+// (written once; the chunks write the other tiles only).
+template <int C, int P>
+__device__ __forceinline__ void zero_masked_scores(u16 *M, bool rev, int tid, int nt) {
+    constexpr int LD = C + kPad, PL = C * LD;
+    for (int x = tid; x < C / 32 * 16 * 16 * P; x += nt) {
+        const int p = x / (C / 32 * 256), y = x % (C / 32 * 256), pair = y / 256, r = y % 256 / 16, c = y % 16;
+        const int row = 32 * pair + (rev ? 16 : 0) + r, col = 32 * pair + (rev ? 0 : 16) + c;
+        M[p * PL + row * LD + col] = 0;
+    }
+}
+
+// O = diag(row) X S for the wave's columns, from the state S before (after, REV) the chunk.
+template <typename T, int C, int KD, int NC>
+__device__ __forceinline__ void inter(f32x4 (&O)[C / 16][NC], const f32x4 (&S)[KD / 16][NC], const u16 *X, const float *row,
+                                      float scale, int lane) {
+    constexpr int LD = KD + kPad, PL = C * LD, PI = Cfg<T>::in, PS = Cfg<T>::st;
+    const int g = lane / 16, i = lane % 16;
+#pragma unroll
+    for (int t = 0; t < C / 16; ++t)
+#pragma unroll
+        for (int c = 0; c < NC; ++c) O[t][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < KD / 32; ++k) {
+        bf16x8 s[NC][PS];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            float x[8];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                x[r] = S[2 * k][c][r];
+                x[4 + r] = S[2 * k + 1][c][r];
+            }
+            split8<PS>(x, s[c]);
+        }
+#pragma unroll
+        for (int t = 0; t < C / 16; ++t) {
+            bf16x8 a[PI];
+#pragma unroll
+            for (int p = 0; p < PI; ++p) a[p] = frag_row(X + p * PL + (16 * t + i) * LD, 32 * k, g);
+#pragma unroll
+            for (int c = 0; c < NC; ++c) O[t][c] = mma<PI, PS, PS>(O[t][c], a, s[c]);
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < C / 16; ++t) {
+        const f32x4 f = *reinterpret_cast<const f32x4 *>(row + 16 * t + 4 * g);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int c = 0; c < NC; ++c) O[t][c][r] *= f[r] * scale;
+    }
+}
+
+// S = all S + Y^T diag(w) V for the wave's columns (V's operands in v).
+template <typename T, int C, int KD, int NC>
+__device__ __forceinline__ void update(f32x4 (&S)[KD / 16][NC], const bf16x8 (&v)[C / 32][NC][Cfg<T>::in], const u16 *Y,
+                                       const float *w, float scale, float all, int lane) {
+    constexpr int LD = KD + kPad, PL = C * LD, PI = Cfg<T>::in, PU = Cfg<T>::up;
+    const int g = lane / 16, i = lane % 16;
+#pragma unroll
+    for (int k = 0; k < KD / 16; ++k)
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) S[k][c][r] *= all;
+#pragma unroll
+    for (int j = 0; j < C / 32; ++j) {
+        const f32x4 w0 = *reinterpret_cast<const f32x4 *>(w + 32 * j + 4 * g);
+        const f32x4 w1 = *reinterpret_cast<const f32x4 *>(w + 32 * j + 16 + 4 * g);
+        bf16x8 u[NC][PU];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            float x[8], y[8];
+            unpack_frag(v[j][c][PI - 1], x);
+#pragma unroll
+            for (int p = PI - 2; p >= 0; --p) {
+                unpack_frag(v[j][c][p], y);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] += y[e];
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                x[e] *= w0[e] * scale;
+                x[4 + e] *= w1[e] * scale;
+            }
+            split8<PU>(x, u[c]);
+        }
+#pragma unroll
+        for (int k = 0; k < KD / 16; ++k) {
+            bf16x8 a[PI];
+#pragma unroll
+            for (int p = 0; p < PI; ++p) a[p] = frag_tr<LD>(Y + p * PL, 32 * j, 16 * k, g, i);
+#pragma unroll
+            for (int c = 0; c < NC; ++c) S[k][c] = mma<PI, PU, PU>(S[k][c], a, u[c]);
+        }
+    }
+}
+
+template <typename T, int C, int NC, int LDV>
+__device__ __forceinline__ void load_v(bf16x8 (&v)[C / 32][NC][Cfg<T>::in], const u16 *V, int col, int lane) {
+    constexpr int PL = C * LDV;
+#pragma unroll
+    for (int j = 0; j < C / 32; ++j)
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int p = 0; p < Cfg<T>::in; ++p)
+                v[j][c][p] = frag_tr<LDV>(V + p * PL, 32 * j, col + 16 * c, lane / 16, lane % 16);
+}
+
+// O += M V, M the masked scores. A masked score is 0, and 0 times an infinity or NaN of a token that the row
+// does not see would be NaN: where V holds one, its elements leave the product and are added one by one.
+template <typename T, int C, int NC, int LDV, bool REV>
+__device__ __forceinline__ void intra(f32x4 (&O)[C / 16][NC], const bf16x8 (&v0)[C / 32][NC][Cfg<T>::in], const u16 *M,
+                                      const u16 *V, int col, int lane) {
+    constexpr int LD = C + kPad, PL = C * LD, PI = Cfg<T>::in, PS = Cfg<T>::st;
+    const int g = lane / 16, i = lane % 16;
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+    u16x2 most = {0, 0};
+#pragma unroll
+    for (int j = 0; j < C / 32; ++j)
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const u32x4 w = __builtin_bit_cast(u32x4, v0[j][c][0]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, w[k] & 0x7fff7fffu));
+        }
+    const bool odd = most[0] >= 0x7f80 || most[1] >= 0x7f80;
+    auto product = [&](const bf16x8 (&v)[C / 32][NC][PI]) {
+#pragma unroll
+        for (int t = 0; t < C / 16; ++t)
+#pragma unroll
+            for (int j = 0; j < C / 32; ++j) {
+                if (REV ? 2 * j + 1 < t : 2 * j > t) continue;
+                bf16x8 a[PS];
+#pragma unroll
+                for (int p = 0; p < PS; ++p) a[p] = frag_row(M + p * PL + (16 * t + i) * LD, 32 * j, g);
+#pragma unroll
+                for (int c = 0; c < NC; ++c) O[t][c] = mma<PS, PI, PS>(O[t][c], a, v[j][c]);
+            }
+    };
+    if (!__any(odd)) {
+        product(v0);
+        return;
+    }
+    bf16x8 v[C / 32][NC][PI];
+#pragma unroll
+    for (int j = 0; j < C / 32; ++j)
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            u32x4 w = __builtin_bit_cast(u32x4, v0[j][c][0]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if ((w[k] & 0x7f80u) == 0x7f80u) w[k] &= 0xffff0000u;
+                if ((w[k] & 0x7f800000u) == 0x7f800000u) w[k] &= 0xffffu;
+            }
+            v[j][c][0] = __builtin_bit_cast(bf16x8, w);
+#pragma unroll
+            for (int p = 1; p < PI; ++p) v[j][c][p] = v0[j][c][p];
+        }
+    product(v);
+    for (int n = 0; n < C; ++n)
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const float x = __uint_as_float(uint32_t(V[n * LDV + col + 16 * c + i]) << 16);
+            const bool bad = (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u;
+            if (!__any(bad)) continue;
+#pragma unroll
+            for (int t = 0; t < C / 16; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int o = 16 * t + 4 * g + r;
+                    if (!bad || (REV ? n < o : n > o)) continue;
+                    float m = 0.f;
+#pragma unroll
+                    for (int p = PS - 1; p >= 0; --p) m += __uint_as_float(uint32_t(M[p * PL + o * LD + n]) << 16);
+                    O[t][c][r] += m * x;
+                }
+        }
+}
+
+// A float32 matrix of a (batch row, head): rows x cols, with its strides.
+struct Mat {
+    float *p;
+    int64_t row, col;
+};
+template <int KD, int NC>
+__device__ __forceinline__ void load_state(f32x4 (&S)[KD / 16][NC], const Mat &m, int rows, int cols, int col, int lane) {
+    const int g = lane / 16, i = lane % 16;
+#pragma unroll
+    for (int k = 0; k < KD / 16; ++k)
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int y = 16 * k + 4 * g + r, x = col + 16 * c + i;
+                S[k][c][r] = m.p && y < rows && x < cols ? m.p[y * m.row + x * m.col] : 0.f;
+            }
+}
+template <int KD, int NC>
+__device__ __forceinline__ void store_state(const f32x4 (&S)[KD / 16][NC], const Mat &m, int rows, int cols, int col, int lane) {
+    const int g = lane / 16, i = lane % 16;
+#pragma unroll
+    for (int k = 0; k < KD / 16; ++k)
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int y = 16 * k + 4 * g + r, x = col + 16 * c + i;
+                if (y < rows && x < cols) m.p[y * m.row + x * m.col] = S[k][c][r];
+            }
+}
+
+// The wave's C x 16 NC outputs to T or float32 rows.
+template <typename T, int C, int NC>
+__device__ __forceinline__ void store_out(const f32x4 (&O)[C / 16][NC], void *out, bool f32, int64_t stride, int64_t t0, int rows,
+                                          int cols, int col, int lane) {
+    const int g = lane / 16, i = lane % 16;
+#pragma unroll
+    for (int t = 0; t < C / 16; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int n = 16 * t + 4 * g + r;
+            if (n >= rows) continue;
+            const int64_t at = (t0 + n) * stride;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const int x = col + 16 * c + i;
+                if (x >= cols) continue;
+                if (f32) reinterpret_cast<float *>(out)[at + x] = O[t][c][r];
+                else reinterpret_cast<T *>(out)[at + x] = from_f32<T>(O[t][c][r]);
+            }
+        }
+}
+
+// dot[n] = sum over the wave's columns of O[n][x] Z[n][x], into part[n] (lanes i == 0 write).
+template <typename T, int C, int NC, int LDZ>
+__device__ __forceinline__ void dot_rows(const f32x4 (&O)[C / 16][NC], const u16 *Z, int col, float *part, int lane) {
+    constexpr int PL = C * LDZ, PI = Cfg<T>::in;
+    const int g = lane / 16, i = lane % 16;
+#pragma unroll
+    for (int t = 0; t < C / 16; ++t) {
+        f32x4 s;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            float x = 0.f;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const u16 *z = Z + (16 * t + 4 * g + r) * LDZ + col + 16 * c + i;
+                float y = 0.f;
+#pragma unroll
+                for (int p = PI - 1; p >= 0; --p) y += __uint_as_float(uint32_t(z[p * PL]) << 16);
+                x = __builtin_fmaf(O[t][c][r], y, x);
+            }
+            s[r] = group_sum<16>(x);
+        }
+        if (i == 0) *reinterpret_cast<f32x4 *>(part + 16 * t + 4 * g) = s;
+    }
+}
+
+__device__ __forceinline__ float wave_sum(float x) {
+    x = group_sum<16>(x);
+    x += __shfl_xor(x, 16);
+    x += __shfl_xor(x, 32);
+    return x;
+}
+
+}  // namespace la
+}  // namespace mm

@@ -20,6 +20,8 @@
 #include <vector>
 
 #include "mm_conv1d.h"
+#include "mm_group_norm.h"
+#include "mm_linattn.h"
 #include "mm_norm.h"
 #include "mm_scan.h"
 
@@ -763,6 +765,248 @@ at::Tensor state_update(const at::Tensor &state, const at::Tensor &x, const at::
     return out;
 }
 
+// ---- linear attention and group norm --------------------------------------------------------------
+
+mm_dtype float_dtype(const at::Tensor &t, const char *name) {
+    const auto st = t.scalar_type();
+    TORCH_CHECK(st == at::ScalarType::Float || st == at::ScalarType::Half || st == at::ScalarType::BFloat16, name,
+                " must be float32, float16 or bfloat16");
+    return to_mm(st);
+}
+
+// q, k (lead..., groups, dk) and v (lead..., heads, dv), on one device and of one dtype, rows contiguous.
+void check_qkv(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, int64_t rank) {
+    TORCH_CHECK(q.is_cuda() && k.is_cuda() && v.is_cuda(), "q, k and v must be on the GPU");
+    TORCH_CHECK(q.device() == v.device() && k.device() == v.device(), "q, k and v must be on one device");
+    TORCH_CHECK(q.dim() == rank && v.dim() == rank, "q, k and v must have ", rank, " dimensions");
+    TORCH_CHECK(q.sizes() == k.sizes(), "q and k must have the same shape");
+    for (int64_t i = 0; i < rank - 2; ++i) TORCH_CHECK(q.size(i) == v.size(i), "q, k and v must agree in batch and seqlen");
+    TORCH_CHECK(q.scalar_type() == v.scalar_type() && k.scalar_type() == v.scalar_type(), "q, k and v must have one dtype");
+    float_dtype(v, "v");
+    for (const auto *t : {&q, &k, &v}) TORCH_CHECK(t->stride(-1) == 1 || t->size(-1) == 1, "q, k and v must be contiguous along their last dimension");
+    const int64_t groups = q.size(-2), heads = v.size(-2);
+    TORCH_CHECK(groups >= 1 && heads % groups == 0, "the heads of v must be a multiple of those of q and k");
+    TORCH_CHECK(q.size(-1) >= 1 && v.size(-1) >= 1, "q, k and v must have at least one element per head");
+}
+
+void check_decay(const at::Tensor &g, at::IntArrayRef sizes, const at::Tensor &v) {
+    TORCH_CHECK(g.is_cuda() && g.device() == v.device(), "log_decay must be on the device of v");
+    TORCH_CHECK(g.sizes() == sizes, "log_decay must have the shape of v without its last dimension, or (nheads,)");
+    float_dtype(g, "log_decay");
+}
+
+void check_state(const at::Tensor &s, const at::Tensor &v, int64_t batch, int64_t heads, int64_t dk, int64_t dv, const char *name) {
+    TORCH_CHECK(s.is_cuda() && s.device() == v.device(), name, " must be on the device of v");
+    TORCH_CHECK(s.scalar_type() == at::ScalarType::Float, name, " must be float32");
+    TORCH_CHECK(s.sizes() == torch::IntArrayRef({batch, heads, dk, dv}), name, " must have shape (batch, nheads, dk, dv)");
+}
+
+void *workspace_of(at::Tensor &keep, int64_t bytes, const at::Tensor &like) {
+    if (bytes <= 0) return nullptr;
+    keep = torch::empty({bytes}, like.options().dtype(at::ScalarType::Byte));
+    return keep.data_ptr();
+}
+
+std::vector<at::Tensor> linattn_fwd(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &g,
+                                    double scale, const c10::optional<at::Tensor> &initial_, bool return_last_state) {
+    check_qkv(q, k, v, 4);
+    const int64_t batch = v.size(0), seqlen = v.size(1), heads = v.size(2), dv = v.size(3), dk = q.size(3);
+    check_decay(g, {batch, seqlen, heads}, v);
+    at::Tensor initial;
+    if (initial_.has_value()) {
+        check_state(initial_.value(), v, batch, heads, dk, dv, "initial_state");
+        initial = initial_.value().contiguous();
+    }
+    const c10::DeviceGuard device_guard{v.device()};
+    at::Tensor out = torch::empty({batch, seqlen, heads, dv}, v.options());
+    at::Tensor last;
+    if (return_last_state) last = torch::empty({batch, heads, dk, dv}, v.options().dtype(at::ScalarType::Float));
+    mm_linattn_fwd_params p;
+    std::memset(&p, 0, sizeof(p));
+    p.batch = batch; p.seqlen = seqlen; p.n_groups = q.size(2); p.nheads = heads; p.dk = dk; p.dv = dv;
+    p.itype = to_mm(v.scalar_type());
+    p.gtype = to_mm(g.scalar_type());
+    p.scale = static_cast<float>(scale);
+    p.q = q.data_ptr(); p.k = k.data_ptr(); p.v = v.data_ptr(); p.log_decay = g.data_ptr();
+    p.initial_state = initial.defined() ? initial.data_ptr<float>() : nullptr;
+    p.out = out.data_ptr();
+    p.last_state = last.defined() ? last.data_ptr<float>() : nullptr;
+    p.q_batch_stride = q.stride(0); p.q_seq_stride = q.stride(1); p.q_group_stride = q.stride(2);
+    p.k_batch_stride = k.stride(0); p.k_seq_stride = k.stride(1); p.k_group_stride = k.stride(2);
+    p.v_batch_stride = v.stride(0); p.v_seq_stride = v.stride(1); p.v_head_stride = v.stride(2);
+    p.g_batch_stride = g.stride(0); p.g_seq_stride = g.stride(1); p.g_head_stride = g.stride(2);
+    p.out_batch_stride = out.stride(0); p.out_seq_stride = out.stride(1); p.out_head_stride = out.stride(2);
+    at::Tensor ws;
+    p.workspace_bytes = mm_linattn_fwd_workspace_size(&p);
+    p.workspace = workspace_of(ws, p.workspace_bytes, v);
+    check_rc(mm_linattn_fwd(&p, c10::hip::getCurrentHIPStream().stream()), "mm_linattn_fwd");
+    std::vector<at::Tensor> res{out};
+    if (return_last_state) res.push_back(last);
+    return res;
+}
+
+// Gradients [dq, dk, dv, dlog_decay | None, dinitial_state | None]; dlog_decay has the shape of log_decay, or
+// (nheads,) with decay_per_head.
+std::vector<c10::optional<at::Tensor>> linattn_bwd(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &g,
+                                                   double scale, const c10::optional<at::Tensor> &initial_, const at::Tensor &dout,
+                                                   const c10::optional<at::Tensor> &dlast_, bool decay_per_head, bool want_decay,
+                                                   bool want_initial) {
+    check_qkv(q, k, v, 4);
+    const int64_t batch = v.size(0), seqlen = v.size(1), heads = v.size(2), dv = v.size(3), dk = q.size(3);
+    check_decay(g, {batch, seqlen, heads}, v);
+    TORCH_CHECK(dout.is_cuda() && dout.sizes() == v.sizes() && dout.scalar_type() == v.scalar_type(), "dout must have the shape and dtype of v");
+    TORCH_CHECK(dout.stride(-1) == 1 || dout.size(-1) == 1, "dout must be contiguous along its last dimension");
+    at::Tensor initial, dlast;
+    if (initial_.has_value()) {
+        check_state(initial_.value(), v, batch, heads, dk, dv, "initial_state");
+        initial = initial_.value().contiguous();
+    }
+    if (dlast_.has_value()) {
+        check_state(dlast_.value(), v, batch, heads, dk, dv, "dlast_state");
+        dlast = dlast_.value().contiguous();
+    }
+    const c10::DeviceGuard device_guard{v.device()};
+    at::Tensor dq = torch::empty(q.sizes(), q.options()), dkk = torch::empty(k.sizes(), k.options()), dvv = torch::empty(v.sizes(), v.options());
+    at::Tensor dg, ds;
+    if (want_decay) dg = decay_per_head ? torch::empty({heads}, g.options()) : torch::empty({batch, seqlen, heads}, g.options());
+    if (want_initial) ds = torch::empty({batch, heads, dk, dv}, v.options().dtype(at::ScalarType::Float));
+    mm_linattn_bwd_params p;
+    std::memset(&p, 0, sizeof(p));
+    p.batch = batch; p.seqlen = seqlen; p.n_groups = q.size(2); p.nheads = heads; p.dk = dk; p.dv = dv;
+    p.itype = to_mm(v.scalar_type());
+    p.gtype = to_mm(g.scalar_type());
+    p.scale = static_cast<float>(scale);
+    p.q = q.data_ptr(); p.k = k.data_ptr(); p.v = v.data_ptr(); p.log_decay = g.data_ptr();
+    p.initial_state = initial.defined() ? initial.data_ptr<float>() : nullptr;
+    p.dout = dout.data_ptr();
+    p.dlast_state = dlast.defined() ? dlast.data_ptr<float>() : nullptr;
+    p.dq = dq.data_ptr(); p.dk_out = dkk.data_ptr(); p.dv_out = dvv.data_ptr();
+    p.dlog_decay = dg.defined() ? dg.data_ptr() : nullptr;
+    p.dinitial_state = ds.defined() ? ds.data_ptr<float>() : nullptr;
+    p.decay_per_head = decay_per_head;
+    p.q_batch_stride = q.stride(0); p.q_seq_stride = q.stride(1); p.q_group_stride = q.stride(2);
+    p.k_batch_stride = k.stride(0); p.k_seq_stride = k.stride(1); p.k_group_stride = k.stride(2);
+    p.v_batch_stride = v.stride(0); p.v_seq_stride = v.stride(1); p.v_head_stride = v.stride(2);
+    p.g_batch_stride = g.stride(0); p.g_seq_stride = g.stride(1); p.g_head_stride = g.stride(2);
+    p.do_batch_stride = dout.stride(0); p.do_seq_stride = dout.stride(1); p.do_head_stride = dout.stride(2);
+    at::Tensor ws;
+    p.workspace_bytes = mm_linattn_bwd_workspace_size(&p);
+    p.workspace = workspace_of(ws, p.workspace_bytes, v);
+    check_rc(mm_linattn_bwd(&p, c10::hip::getCurrentHIPStream().stream()), "mm_linattn_bwd");
+    std::vector<c10::optional<at::Tensor>> res{dq, dkk, dvv, c10::nullopt, c10::nullopt};
+    if (want_decay) res[3] = dg;
+    if (want_initial) res[4] = ds;
+    return res;
+}
+
+at::Tensor linattn_update(const at::Tensor &state, const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &g,
+                          double scale) {
+    check_qkv(q, k, v, 3);
+    const int64_t batch = v.size(0), heads = v.size(1), dv = v.size(2), dk = q.size(2);
+    check_decay(g, {batch, heads}, v);
+    check_state(state, v, batch, heads, dk, dv, "state");
+    TORCH_CHECK(state.stride(-1) == 1 || dv == 1, "state must be contiguous along its last dimension");
+    const c10::DeviceGuard device_guard{v.device()};
+    at::Tensor out = torch::empty({batch, heads, dv}, v.options());
+    mm_linattn_update_params p;
+    std::memset(&p, 0, sizeof(p));
+    p.batch = batch; p.n_groups = q.size(1); p.nheads = heads; p.dk = dk; p.dv = dv;
+    p.itype = to_mm(v.scalar_type());
+    p.gtype = to_mm(g.scalar_type());
+    p.scale = static_cast<float>(scale);
+    p.state = state.data_ptr<float>();
+    p.q = q.data_ptr(); p.k = k.data_ptr(); p.v = v.data_ptr(); p.log_decay = g.data_ptr();
+    p.out = out.data_ptr();
+    p.state_batch_stride = state.stride(0); p.state_head_stride = state.stride(1); p.state_dk_stride = state.stride(2);
+    p.q_batch_stride = q.stride(0); p.q_group_stride = q.stride(1);
+    p.k_batch_stride = k.stride(0); p.k_group_stride = k.stride(1);
+    p.v_batch_stride = v.stride(0); p.v_head_stride = v.stride(1);
+    p.g_batch_stride = g.stride(0); p.g_head_stride = g.stride(1);
+    check_rc(mm_linattn_update(&p, c10::hip::getCurrentHIPStream().stream()), "mm_linattn_update");
+    return out;
+}
+
+mm_group_norm_params norm_params(const at::Tensor &x, int64_t n_groups, const c10::optional<at::Tensor> &weight_,
+                                 const c10::optional<at::Tensor> &bias_, const c10::optional<at::Tensor> &z_, double eps, bool is_rms,
+                                 int64_t gate) {
+    TORCH_CHECK(x.is_cuda() && x.dim() == 2, "x must be a (rows, channels) tensor on the GPU");
+    const int64_t rows = x.size(0), channels = x.size(1);
+    auto row_ok = [&](const at::Tensor &t) { return t.stride(1) == 1 || channels == 1; };
+    TORCH_CHECK(row_ok(x), "x must be contiguous along its channels");
+    TORCH_CHECK(n_groups >= 1 && channels % n_groups == 0, "the channels must be a multiple of n_groups");
+    mm_group_norm_params p;
+    std::memset(&p, 0, sizeof(p));
+    p.rows = rows; p.channels = channels; p.n_groups = n_groups;
+    p.itype = float_dtype(x, "x");
+    p.wtype = MM_FLOAT32;
+    p.eps = static_cast<float>(eps);
+    p.is_rms = is_rms;
+    p.gate = static_cast<mm_gate>(gate);
+    p.x = x.data_ptr();
+    p.x_row_stride = x.stride(0);
+    for (const auto *t : {&weight_, &bias_})
+        if (t->has_value()) {
+            const at::Tensor &w = t->value();
+            TORCH_CHECK(w.is_cuda() && w.device() == x.device() && w.dim() == 1 && w.size(0) == channels && w.is_contiguous(),
+                        "weight and bias must be contiguous (channels,) tensors on the device of x");
+            p.wtype = float_dtype(w, "weight");
+        }
+    if (weight_.has_value() && bias_.has_value())
+        TORCH_CHECK(weight_.value().scalar_type() == bias_.value().scalar_type(), "weight and bias must have one dtype");
+    p.weight = weight_.has_value() ? weight_.value().data_ptr() : nullptr;
+    p.bias = bias_.has_value() ? bias_.value().data_ptr() : nullptr;
+    if (z_.has_value()) {
+        const at::Tensor &z = z_.value();
+        TORCH_CHECK(z.is_cuda() && z.device() == x.device() && z.sizes() == x.sizes() && z.scalar_type() == x.scalar_type(),
+                    "z must have the shape, dtype and device of x");
+        TORCH_CHECK(row_ok(z), "z must be contiguous along its channels");
+        p.z = z.data_ptr();
+        p.z_row_stride = z.stride(0);
+    }
+    return p;
+}
+
+at::Tensor group_norm_fwd(const at::Tensor &x, int64_t n_groups, const c10::optional<at::Tensor> &weight, const c10::optional<at::Tensor> &bias,
+                          const c10::optional<at::Tensor> &z, double eps, bool is_rms, int64_t gate) {
+    mm_group_norm_params p = norm_params(x, n_groups, weight, bias, z, eps, is_rms, gate);
+    const c10::DeviceGuard device_guard{x.device()};
+    at::Tensor out = torch::empty({p.rows, p.channels}, x.options());
+    p.out = out.data_ptr();
+    check_rc(mm_group_norm_fwd(&p, c10::hip::getCurrentHIPStream().stream()), "mm_group_norm_fwd");
+    return out;
+}
+
+// [dx, dweight | None, dbias | None, dz | None]
+std::vector<c10::optional<at::Tensor>> group_norm_bwd(const at::Tensor &x, int64_t n_groups, const c10::optional<at::Tensor> &weight,
+                                                      const c10::optional<at::Tensor> &bias, const c10::optional<at::Tensor> &z, double eps,
+                                                      bool is_rms, int64_t gate, const at::Tensor &dout, bool want_weights) {
+    mm_group_norm_params p = norm_params(x, n_groups, weight, bias, z, eps, is_rms, gate);
+    TORCH_CHECK(dout.is_cuda() && dout.sizes() == x.sizes() && dout.scalar_type() == x.scalar_type(), "dout must have the shape and dtype of x");
+    TORCH_CHECK(dout.stride(1) == 1 || p.channels == 1, "dout must be contiguous along its channels");
+    const c10::DeviceGuard device_guard{x.device()};
+    std::vector<c10::optional<at::Tensor>> res{torch::empty({p.rows, p.channels}, x.options()), c10::nullopt, c10::nullopt, c10::nullopt};
+    p.dout = dout.data_ptr();
+    p.dout_row_stride = dout.stride(0);
+    p.dx = res[0].value().data_ptr();
+    if (want_weights && weight.has_value()) {
+        res[1] = torch::empty_like(weight.value());
+        p.dweight = res[1].value().data_ptr();
+    }
+    if (want_weights && bias.has_value()) {
+        res[2] = torch::empty_like(bias.value());
+        p.dbias = res[2].value().data_ptr();
+    }
+    if (z.has_value()) {
+        res[3] = torch::empty({p.rows, p.channels}, x.options());
+        p.dz = res[3].value().data_ptr();
+    }
+    at::Tensor ws;
+    p.workspace_bytes = mm_group_norm_bwd_workspace_size(&p);
+    p.workspace = workspace_of(ws, p.workspace_bytes, x);
+    check_rc(mm_group_norm_bwd(&p, c10::hip::getCurrentHIPStream().stream()), "mm_group_norm_bwd");
+    return res;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -803,5 +1047,20 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("rms_norm_fwd", &rms_norm_fwd, "Row RMSNorm over dim 1 of a 3-D tensor",
           pybind11::arg("x"), pybind11::arg("weight"), pybind11::arg("eps") = 1e-6,
           pybind11::arg("out") = pybind11::none());
+    m.def("linattn_fwd", &linattn_fwd, "Linear attention forward [out, last_state?]", pybind11::arg("q"), pybind11::arg("k"),
+          pybind11::arg("v"), pybind11::arg("log_decay"), pybind11::arg("scale"), pybind11::arg("initial_state") = pybind11::none(),
+          pybind11::arg("return_last_state") = false);
+    m.def("linattn_bwd", &linattn_bwd, "Linear attention backward [dq, dk, dv, dlog_decay?, dinitial_state?]", pybind11::arg("q"),
+          pybind11::arg("k"), pybind11::arg("v"), pybind11::arg("log_decay"), pybind11::arg("scale"), pybind11::arg("initial_state"),
+          pybind11::arg("dout"), pybind11::arg("dlast_state"), pybind11::arg("decay_per_head"), pybind11::arg("want_decay"),
+          pybind11::arg("want_initial"));
+    m.def("linattn_update", &linattn_update, "Linear attention, one token (in place on state)", pybind11::arg("state"), pybind11::arg("q"),
+          pybind11::arg("k"), pybind11::arg("v"), pybind11::arg("log_decay"), pybind11::arg("scale"));
+    m.def("group_norm_fwd", &group_norm_fwd, "Gated group norm forward", pybind11::arg("x"), pybind11::arg("n_groups"),
+          pybind11::arg("weight"), pybind11::arg("bias"), pybind11::arg("z"), pybind11::arg("eps"), pybind11::arg("is_rms"),
+          pybind11::arg("gate"));
+    m.def("group_norm_bwd", &group_norm_bwd, "Gated group norm backward [dx, dweight?, dbias?, dz?]", pybind11::arg("x"),
+          pybind11::arg("n_groups"), pybind11::arg("weight"), pybind11::arg("bias"), pybind11::arg("z"), pybind11::arg("eps"),
+          pybind11::arg("is_rms"), pybind11::arg("gate"), pybind11::arg("dout"), pybind11::arg("want_weights"));
     m.def("abi_version", []() { return mm_abi_version(); });
 }

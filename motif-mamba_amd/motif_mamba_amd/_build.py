@@ -27,11 +27,13 @@ PROBE_NAME = "libmm_probe.so"
 EXT_NAME = "mm_scan_torch"
 ARCH = "gfx950"
 
-# mm_scan_{tiled,pq,bwd_lanes}_{f16,bf16}.hip include mm_scan_{tiled,pq,bwd_lanes}.hip for their input type
+# mm_scan_{tiled,pq,bwd_lanes}_{f16,bf16}.hip include mm_scan_{tiled,pq,bwd_lanes}.hip for their input type, and
+# mm_linattn_{f16,bf16}.hip mm_linattn.hip
 # (parallel builds).
 HIP_SOURCES = ["mm_scan.hip", "mm_scan_tiled.hip", "mm_scan_tiled_f16.hip", "mm_scan_tiled_bf16.hip",
                "mm_scan_pq.hip", "mm_scan_pq_f16.hip", "mm_scan_pq_bf16.hip", "mm_scan_bwd.hip", "mm_scan_pq_bwd.hip", "mm_scan_bwd_lanes.hip",
-               "mm_scan_bwd_lanes_f16.hip", "mm_scan_bwd_lanes_bf16.hip", "mm_conv1d.hip", "mm_norm.hip"]
+               "mm_scan_bwd_lanes_f16.hip", "mm_scan_bwd_lanes_bf16.hip", "mm_conv1d.hip", "mm_norm.hip",
+               "mm_linattn.hip", "mm_linattn_f16.hip", "mm_linattn_bf16.hip", "mm_linattn_api.hip", "mm_group_norm.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # Packed fp32 VALU ops are disabled: the compiler would otherwise form v_pk_{add,mul,fma}_f32
 # from scalar float code, and those have given silent wrong results on these GPUs.
