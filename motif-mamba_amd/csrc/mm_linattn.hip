@@ -23,26 +23,26 @@ constexpr int kWaves = 4, kThreads = 64 * kWaves;
 
 template <typename T>
 __device__ __forceinline__ Rows<T> rows_of(const View &v, int64_t b, int64_t h, int d, int col0) {
-    return Rows<T>{reinterpret_cast<const T *>(v.p) + b * v.batch + (h / v.share) * v.head + col0, v.seq, d - col0, v.vec != 0};
+    return Rows<T>{reinterpret_cast<const T *>(v.p) + b * v.batch + (h / v.share) * v.head + col0, v.seq, d - col0};
 }
 
 // Forward walk: out = scale (masked X Y^T) V + ..., KD the padded length of X's rows, 64 NC columns of V per
 // workgroup, 16 NC per wave. DOT: also e[t] = (the product with the state alone) . Z_t, and the state at every
 // kBlock-th token into ck (the decays' gradient).
-template <typename T, int KD, int NC, bool DOT>
-__global__ void __launch_bounds__(kThreads) la_walk(const WalkArgs a) {
+template <typename T, int KD, int NC, bool DOT, bool VEC, bool F32>
+__global__ void __launch_bounds__(kThreads, 2) la_walk(const WalkArgs a) {
     constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, PS = Cfg<T>::st, W = 64 * NC;
     constexpr int LDX = KD + kPad, LDV = W + kPad, LDM = C + kPad;
     constexpr int NT = C / 16 * (C / 16 + 1) / 2;   // score tiles
-    typedef Stage<T, C, KD, kThreads> SX;
-    typedef Stage<T, C, W, kThreads> SV;
+    typedef Stage<T, C, KD, kThreads, VEC> SX;
+    typedef Stage<T, C, W, kThreads, VEC> SV;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     u16 *X = reinterpret_cast<u16 *>(smem), *Y = X + PI * C * LDX, *V = Y + PI * C * LDX;
     u16 *M = V + PI * C * LDV, *Z = M + PS * C * LDM;
     Decays<C> *dec = reinterpret_cast<Decays<C> *>(Z + (DOT ? PI * C * LDV : 0));
     float *part = reinterpret_cast<float *>(dec + 2);
 
-    const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64;
     int64_t id = blockIdx.x;
     const int slice = id % a.slices; id /= a.slices;
     const int seg = id % a.segs; id /= a.segs;
@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(kThreads) la_walk(const WalkArgs a) {
             store_scores<C, PS>(M, x, o, n, lane);
         }
         f32x4 O[C / 16][NC];
-        inter<T, C, KD, NC>(O, S, X, d.in, a.scale, lane);
+        inter<T, C, KD, NC, DOT ? 3 : PS>(O, S, X, d.in, a.scale, lane);
         if constexpr (DOT) dot_rows<T, C, NC, LDV>(O, Z, col, part + wave * C, lane);
         if (wave == dwave && more) {
             make_decays<C>(dec[buf ^ 1], gnext, lane);
@@ -126,9 +126,8 @@ __global__ void __launch_bounds__(kThreads) la_walk(const WalkArgs a) {
         load_v<T, C, NC, LDV>(v, V, col, lane);
         intra<T, C, NC, LDV, false>(O, v, M, V, col, lane);
         update<T, C, KD, NC>(S, v, Y, d.out, 1.f, d.all, lane);
-        store_out<T, C, NC>(O, a.out_f32 ? static_cast<void *>(reinterpret_cast<float *>(a.out) + b * a.out_batch + h * a.out_head)
-                                         : static_cast<void *>(reinterpret_cast<T *>(a.out) + b * a.out_batch + h * a.out_head),
-                            a.out_f32, a.out_seq, t0, rows, a.cdim, col0 + col, lane);
+        store_out<T, C, NC, LDV, VEC, F32>(O, static_cast<char *>(a.out) + (b * a.out_batch + h * a.out_head) * int64_t(F32 ? 4 : sizeof(T)),
+                                           a.out_seq, t0, rows, a.cdim, col0, V, col, lane);
     }
     if (a.s1.p && seg == a.segs - 1)
         store_state<KD, NC>(S, Mat{a.s1.p + bh * a.kdim * a.cdim, a.s1.row, a.s1.col}, a.kdim, a.cdim, col0 + col, lane);
@@ -141,16 +140,16 @@ __global__ void __launch_bounds__(kThreads) la_walk(const WalkArgs a) {
 
 // What each segment but the last one (REV: the first one) of a row adds to the state: sum of y_t (decay to the
 // segment's end) v_t^T into st[bh][seg], and the segment's own decay into decay[bh][seg].
-template <typename T, int KD, bool REV>
+template <typename T, int KD, bool REV, bool VEC>
 __global__ void __launch_bounds__(kThreads) la_segments(const WalkArgs a) {
     constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, W = 64;
     constexpr int LDX = KD + kPad, LDV = W + kPad;
-    typedef Stage<T, C, KD, kThreads> SX;
-    typedef Stage<T, C, W, kThreads> SV;
+    typedef Stage<T, C, KD, kThreads, VEC> SX;
+    typedef Stage<T, C, W, kThreads, VEC> SV;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     u16 *Y = reinterpret_cast<u16 *>(smem), *V = Y + PI * C * LDX;
     Decays<C> *dec = reinterpret_cast<Decays<C> *>(V + PI * C * LDV);
-    const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64;
     int64_t id = blockIdx.x;
     const int slice = id % a.slices; id /= a.slices;
     const int seg = id % a.segs; id /= a.segs;
@@ -196,20 +195,20 @@ __global__ void __launch_bounds__(kThreads) la_segments(const WalkArgs a) {
 // Backward walk from the end: dv, dk, the scores' part of the decays' gradient (a), the state's part (f), and at
 // every kBlock-th token the product of the state there with its gradient (y). Waves 0 to 3 hold the gradient R of the
 // state for dv (rows dk, columns dv), waves 4 to 7 its transpose for dk.
-template <typename T, int KD, int VD>
+template <typename T, int KD, int VD, bool VEC, bool F32>
 __global__ void __launch_bounds__(2 * kThreads) la_bwd(const BwdArgs a) {
     constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, PS = Cfg<T>::st, NT2 = 2 * kThreads;
     constexpr int LDK = KD + kPad, LDV = VD + kPad, LDM = C + kPad, CT = C / 16;
     constexpr int NT = CT * (CT + 1) / 2, NV = VD / 64, NK = KD / 64;
-    typedef Stage<T, C, KD, NT2> SK;
-    typedef Stage<T, C, VD, NT2> SV;
+    typedef Stage<T, C, KD, NT2, VEC> SK;
+    typedef Stage<T, C, VD, NT2, VEC> SV;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     u16 *Q = reinterpret_cast<u16 *>(smem), *K = Q + PI * C * LDK, *V = K + PI * C * LDK, *G = V + PI * C * LDV;
     u16 *M1 = G + PI * C * LDV, *M2 = M1 + PS * C * LDM;
     Decays<C> *dec = reinterpret_cast<Decays<C> *>(M2 + PS * C * LDM);
     float *rowp = reinterpret_cast<float *>(dec + 2), *colp = rowp + CT * C, *part = colp + CT * C;
 
-    const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64;
     int64_t id = blockIdx.x;
     const int seg = id % a.segs; id /= a.segs;
     const int64_t h = id % a.heads, b = id / a.heads, bh = b * a.heads + h;
@@ -316,9 +315,9 @@ __global__ void __launch_bounds__(2 * kThreads) la_bwd(const BwdArgs a) {
         }
         f32x4 OV[CT][NV], OK[CT][NK];
         if (for_v) {
-            inter<T, C, KD, NV>(OV, SV_, K, d.out, 1.f, lane);
+            inter<T, C, KD, NV, PS>(OV, SV_, K, d.out, 1.f, lane);
         } else {
-            inter<T, C, VD, NK>(OK, SK_, V, d.out, 1.f, lane);
+            inter<T, C, VD, NK, 3>(OK, SK_, V, d.out, 1.f, lane);
             if (a.a) dot_rows<T, C, NK, LDK>(OK, K, col, part + (wave - kWaves) * C, lane);
         }
         if (wave == dwave && more) {
@@ -341,17 +340,15 @@ __global__ void __launch_bounds__(2 * kThreads) la_bwd(const BwdArgs a) {
             load_v<T, C, NV, LDV>(v, G, col, lane);
             intra<T, C, NV, LDV, true>(OV, v, M1, G, col, lane);
             update<T, C, KD, NV>(SV_, v, Q, d.in, a.scale, d.all, lane);
-            store_out<T, C, NV>(OV, reinterpret_cast<T *>(a.dv_out) + (b * a.seqlen * a.heads + h) * a.dv, false, a.heads * a.dv, t0, rows,
-                                a.dv, col, lane);
+            store_out<T, C, NV, LDV, VEC, false>(OV, reinterpret_cast<T *>(a.dv_out) + (b * a.seqlen * a.heads + h) * a.dv, a.heads * a.dv, t0,
+                                                 rows, a.dv, 0, V, col, lane);
         } else {
             bf16x8 v[C / 32][NK][PI];
             load_v<T, C, NK, LDK>(v, Q, col, lane);
             intra<T, C, NK, LDK, true>(OK, v, M2, Q, col, lane);
             update<T, C, VD, NK>(SK_, v, G, d.in, a.scale, d.all, lane);
-            const int64_t at = (b * a.seqlen * a.heads + h) * a.dk;
-            store_out<T, C, NK>(OK, a.dk_f32 ? static_cast<void *>(reinterpret_cast<float *>(a.dk_out) + at)
-                                             : static_cast<void *>(reinterpret_cast<T *>(a.dk_out) + at),
-                                a.dk_f32, a.heads * a.dk, t0, rows, a.dk, col, lane);
+            store_out<T, C, NK, LDK, VEC, F32>(OK, static_cast<char *>(a.dk_out) + (b * a.seqlen * a.heads + h) * a.dk * int64_t(F32 ? 4 : sizeof(T)),
+                                               a.heads * a.dk, t0, rows, a.dk, 0, K, col, lane);
             if (a.ck && t0 > 0 && t0 % kBlock == 0) boundary(t0 / kBlock - 1);
         }
     }
@@ -359,71 +356,93 @@ __global__ void __launch_bounds__(2 * kThreads) la_bwd(const BwdArgs a) {
         store_state<KD, NV>(SV_, Mat{a.dr + bh * int64_t(a.dk) * a.dv, a.dv, 1}, a.dk, a.dv, col, lane);
 }
 
-template <typename T, int KD, int NC, bool DOT>
+template <typename K, typename A>
+static int launch_kernel(K kernel, int bytes, hipError_t set, int64_t grid, int threads, const A &a, hipStream_t s, const char *what) {
+    if (set != hipSuccess) return set_error(int(set), "linear attention: hipFuncSetAttribute failed");
+    hipLaunchKernelGGL(kernel, dim3(unsigned(grid)), dim3(unsigned(threads)), bytes, s, a);
+    return launch_status(what);
+}
+
+template <typename T, int KD, int NC, bool DOT, bool VEC, bool F32>
 static int launch_walk_t(const WalkArgs &a, hipStream_t s) {
     constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, PS = Cfg<T>::st;
     constexpr int bytes = 2 * (2 * PI * C * (KD + kPad) + (DOT ? 2 : 1) * PI * C * (64 * NC + kPad) + PS * C * (C + kPad)) +
                           2 * int(sizeof(Decays<C>)) + (DOT ? 4 * kWaves * C : 0);
     static_assert(bytes <= 160 * 1024, "LDS");
-    static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void *>(la_walk<T, KD, NC, DOT>),
-                                                      hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (set != hipSuccess) return set_error(int(set), "linear attention: hipFuncSetAttribute failed");
-    const int64_t grid = a.batch * a.heads * a.segs * a.slices;
-    hipLaunchKernelGGL((la_walk<T, KD, NC, DOT>), dim3(unsigned(grid)), dim3(kThreads), bytes, s, a);
-    return launch_status("la_walk");
+    const auto kernel = la_walk<T, KD, NC, DOT, VEC, F32>;
+    static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    return launch_kernel(kernel, bytes, set, a.batch * a.heads * a.segs * a.slices, kThreads, a, s, "la_walk");
+}
+template <typename T, int KD, int NC, bool DOT>
+static int launch_walk_k(const WalkArgs &a, hipStream_t s) {
+    const bool vec = a.x.vec && a.y.vec && a.v.vec && (!DOT || a.z.vec) && a.out_vec;
+    if constexpr (sizeof(T) == 4) {
+        return vec ? launch_walk_t<T, KD, NC, DOT, true, true>(a, s) : launch_walk_t<T, KD, NC, DOT, false, true>(a, s);
+    } else {
+        if (a.out_f32) return vec ? launch_walk_t<T, KD, NC, DOT, true, true>(a, s) : launch_walk_t<T, KD, NC, DOT, false, true>(a, s);
+        return vec ? launch_walk_t<T, KD, NC, DOT, true, false>(a, s) : launch_walk_t<T, KD, NC, DOT, false, false>(a, s);
+    }
 }
 
-template <typename T, int KD, bool REV>
+template <typename T, int KD, bool REV, bool VEC>
 static int launch_segments_t(const WalkArgs &a0, hipStream_t s) {
     constexpr int C = Cfg<T>::C, PI = Cfg<T>::in;
     constexpr int bytes = 2 * (PI * C * (KD + kPad) + PI * C * (64 + kPad)) + int(sizeof(Decays<C>));
     static_assert(bytes <= 160 * 1024, "LDS");
-    static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void *>(la_segments<T, KD, REV>),
-                                                      hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (set != hipSuccess) return set_error(int(set), "linear attention: hipFuncSetAttribute failed");
+    const auto kernel = la_segments<T, KD, REV, VEC>;
+    static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
     WalkArgs a = a0;
     a.slices = (a.cdim + 63) / 64;
-    const int64_t grid = a.batch * a.heads * a.segs * a.slices;
-    hipLaunchKernelGGL((la_segments<T, KD, REV>), dim3(unsigned(grid)), dim3(kThreads), bytes, s, a);
-    return launch_status("la_segments");
+    return launch_kernel(kernel, bytes, set, a.batch * a.heads * a.segs * a.slices, kThreads, a, s, "la_segments");
+}
+template <typename T, int KD>
+static int launch_segments_k(const WalkArgs &a, bool rev, hipStream_t s) {
+    if (a.y.vec && a.v.vec) return rev ? launch_segments_t<T, KD, true, true>(a, s) : launch_segments_t<T, KD, false, true>(a, s);
+    return rev ? launch_segments_t<T, KD, true, false>(a, s) : launch_segments_t<T, KD, false, false>(a, s);
 }
 
-template <typename T, int KD, int VD>
+template <typename T, int KD, int VD, bool VEC, bool F32>
 static int launch_bwd_t(const BwdArgs &a, hipStream_t s) {
     constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, PS = Cfg<T>::st;
     constexpr int bytes = 2 * (2 * PI * C * (KD + kPad) + 2 * PI * C * (VD + kPad) + 2 * PS * C * (C + kPad)) +
                           2 * int(sizeof(Decays<C>)) + 4 * (2 * (C / 16) * C + kWaves * C);
     static_assert(bytes <= 160 * 1024, "LDS");
-    static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void *>(la_bwd<T, KD, VD>),
-                                                      hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (set != hipSuccess) return set_error(int(set), "linear attention: hipFuncSetAttribute failed");
-    const int64_t grid = a.batch * a.heads * a.segs;
-    hipLaunchKernelGGL((la_bwd<T, KD, VD>), dim3(unsigned(grid)), dim3(2 * kThreads), bytes, s, a);
-    return launch_status("la_bwd");
+    const auto kernel = la_bwd<T, KD, VD, VEC, F32>;
+    static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    return launch_kernel(kernel, bytes, set, a.batch * a.heads * a.segs, 2 * kThreads, a, s, "la_bwd");
+}
+template <typename T, int KD, int VD>
+static int launch_bwd_k(const BwdArgs &a, hipStream_t s) {
+    const bool vec = a.q.vec && a.k.vec && a.v.vec && a.dout.vec && a.out_vec;
+    if constexpr (sizeof(T) == 4) {
+        return vec ? launch_bwd_t<T, KD, VD, true, true>(a, s) : launch_bwd_t<T, KD, VD, false, true>(a, s);
+    } else {
+        if (a.dk_f32) return vec ? launch_bwd_t<T, KD, VD, true, true>(a, s) : launch_bwd_t<T, KD, VD, false, true>(a, s);
+        return vec ? launch_bwd_t<T, KD, VD, true, false>(a, s) : launch_bwd_t<T, KD, VD, false, false>(a, s);
+    }
 }
 
 template <typename T>
 int launch_walk(const WalkArgs &a, bool dot, hipStream_t s) {
     const bool wide = a.cdim > 64;
     if (dot) {
-        if (a.kdim <= 64) return wide ? launch_walk_t<T, 64, 2, true>(a, s) : launch_walk_t<T, 64, 1, true>(a, s);
-        return wide ? launch_walk_t<T, 128, 2, true>(a, s) : launch_walk_t<T, 128, 1, true>(a, s);
+        if (a.kdim <= 64) return wide ? launch_walk_k<T, 64, 2, true>(a, s) : launch_walk_k<T, 64, 1, true>(a, s);
+        return wide ? launch_walk_k<T, 128, 2, true>(a, s) : launch_walk_k<T, 128, 1, true>(a, s);
     }
-    if (a.kdim <= 32) return wide ? launch_walk_t<T, 32, 2, false>(a, s) : launch_walk_t<T, 32, 1, false>(a, s);
-    if (a.kdim <= 64) return wide ? launch_walk_t<T, 64, 2, false>(a, s) : launch_walk_t<T, 64, 1, false>(a, s);
-    return wide ? launch_walk_t<T, 128, 2, false>(a, s) : launch_walk_t<T, 128, 1, false>(a, s);
+    if (a.kdim <= 32) return wide ? launch_walk_k<T, 32, 2, false>(a, s) : launch_walk_k<T, 32, 1, false>(a, s);
+    if (a.kdim <= 64) return wide ? launch_walk_k<T, 64, 2, false>(a, s) : launch_walk_k<T, 64, 1, false>(a, s);
+    return wide ? launch_walk_k<T, 128, 2, false>(a, s) : launch_walk_k<T, 128, 1, false>(a, s);
 }
 
 template <typename T>
 int launch_segments(const WalkArgs &a, bool rev, hipStream_t s) {
-    if (a.kdim <= 64) return rev ? launch_segments_t<T, 64, true>(a, s) : launch_segments_t<T, 64, false>(a, s);
-    return rev ? launch_segments_t<T, 128, true>(a, s) : launch_segments_t<T, 128, false>(a, s);
+    return a.kdim <= 64 ? launch_segments_k<T, 64>(a, rev, s) : launch_segments_k<T, 128>(a, rev, s);
 }
 
 template <typename T>
 int launch_bwd(const BwdArgs &a, hipStream_t s) {
-    if (a.dk <= 64) return a.dv <= 64 ? launch_bwd_t<T, 64, 64>(a, s) : launch_bwd_t<T, 64, 128>(a, s);
-    return a.dv <= 64 ? launch_bwd_t<T, 128, 64>(a, s) : launch_bwd_t<T, 128, 128>(a, s);
+    if (a.dk <= 64) return a.dv <= 64 ? launch_bwd_k<T, 64, 64>(a, s) : launch_bwd_k<T, 64, 128>(a, s);
+    return a.dv <= 64 ? launch_bwd_k<T, 128, 64>(a, s) : launch_bwd_k<T, 128, 128>(a, s);
 }
 
 template int launch_walk<MM_LINATTN_TYPE>(const WalkArgs &, bool, hipStream_t);

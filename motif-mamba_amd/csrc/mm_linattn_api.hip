@@ -3,6 +3,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <initializer_list>
 
 #include "mm_common.h"
 #include "mm_internal.h"
@@ -156,6 +157,13 @@ static int check(int64_t batch, int64_t seqlen, int64_t groups, int64_t heads, i
     return MM_OK;
 }
 
+// A tile's 64 rows are addressed with 32-bit offsets.
+static bool near(std::initializer_list<int64_t> strides) {
+    for (const int64_t s : strides)
+        if (s < 0 || s >= (int64_t(1) << 22)) return false;
+    return true;
+}
+
 static int64_t fwd_bytes(const mm_linattn_fwd_params &p, int segs) {
     return segs > 1 ? pad16(p.batch * p.nheads * segs * p.dk * p.dv * 4) + pad16(p.batch * p.nheads * segs * 4) : 0;
 }
@@ -193,6 +201,7 @@ static int run_fwd(const mm_linattn_fwd_params &p, hipStream_t s) {
     a.s1 = State{p.last_state, p.dv, 1};
     a.scale = p.scale;
     a.out = p.out;
+    a.out_vec = view(p.out, p.itype, p.out_batch_stride, p.out_seq_stride, p.out_head_stride, 1, p.dv).vec;
     a.out_batch = p.out_batch_stride; a.out_seq = p.out_seq_stride; a.out_head = p.out_head_stride;
     return launch_walk<T>(a, false, s);
 }
@@ -269,6 +278,7 @@ static int run_bwd(const mm_linattn_bwd_params &p, hipStream_t s) {
     a.s0_step = size;
     a.out = shared ? static_cast<void *>(f32(w.part)) : p.dq;
     a.out_f32 = shared;
+    a.out_vec = view(p.dq, p.itype, 0, 0, 0, 1, p.dk).vec;
     a.out_batch = p.seqlen * p.nheads * p.dk; a.out_seq = p.nheads * p.dk; a.out_head = p.dk;
     if (want_g) {
         a.e = f32(w.e);
@@ -291,6 +301,7 @@ static int run_bwd(const mm_linattn_bwd_params &p, hipStream_t s) {
     r.dv_out = p.dv_out;
     r.dk_out = shared ? static_cast<void *>(f32(w.part)) : p.dk_out;
     r.dk_f32 = shared;
+    r.out_vec = view(p.dv_out, p.itype, 0, 0, 0, 1, p.dv).vec && view(p.dk_out, p.itype, 0, 0, 0, 1, p.dk).vec;
     r.blocks = w.blocks;
     r.has_last = p.dlast_state != nullptr;
     if (want_g) {
@@ -334,6 +345,8 @@ extern "C" int mm_linattn_fwd(const mm_linattn_fwd_params *params, void *stream)
     if (p.seqlen == 0) return p.last_state ? la::launch_copy(p.last_state, p.initial_state, bh * p.dk * p.dv, s) : MM_OK;
     if (!p.q || !p.k || !p.v || !p.log_decay || !p.out)
         return set_error(MM_ERR_INVALID_ARGUMENT, "mm_linattn_fwd: q, k, v, log_decay and out are required");
+    if (!la::near({p.q_seq_stride, p.k_seq_stride, p.v_seq_stride, p.out_seq_stride}))
+        return set_error(MM_ERR_UNSUPPORTED, "mm_linattn_fwd: sequence strides must be between 0 and 2^22 - 1 elements");
     switch (p.itype) {
         case MM_FLOAT32: return la::run_fwd<float>(p, s);
         case MM_FLOAT16: return la::run_fwd<f16_t>(p, s);
@@ -358,6 +371,8 @@ extern "C" int mm_linattn_bwd(const mm_linattn_bwd_params *params, void *stream)
     const int64_t need = la::plan_bwd(p).bytes;
     if (need > 0 && (!p.workspace || p.workspace_bytes < need))
         return set_error(MM_ERR_INVALID_ARGUMENT, "mm_linattn_bwd: the workspace is smaller than mm_linattn_bwd_workspace_size()");
+    if (!la::near({p.q_seq_stride, p.k_seq_stride, p.v_seq_stride, p.do_seq_stride, p.nheads * p.dk, p.nheads * p.dv}))
+        return set_error(MM_ERR_UNSUPPORTED, "mm_linattn_bwd: sequence strides must be between 0 and 2^22 - 1 elements");
     switch (p.itype) {
         case MM_FLOAT32: return la::run_bwd<float>(p, s);
         case MM_FLOAT16: return la::run_bwd<f16_t>(p, s);

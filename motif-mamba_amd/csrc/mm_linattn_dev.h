@@ -122,53 +122,62 @@ __device__ __forceinline__ void unpack_frag(const bf16x8 &f, float *x) {
 
 // ---- staging -------------------------------------------------------------------------------------
 
-// A tensor's rows of one (batch row, head): token t at p + t * stride.
+// Buffer accesses: offsets below 2^31 from a uniform base; kNone reads 0 and drops a store.
+constexpr uint32_t kNone = 0x80000000u;
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void *base) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), (short)0, int(kNone), 0x00020000);
+}
+
+// A tensor's rows of one (batch row, head): token t at p + t * stride. The host takes care that 64 rows span less
+// than 2^31 bytes.
 template <typename T> struct Rows {
     const T *p;
     int64_t stride;
     int d;           // elements of a row that exist
-    bool vec;        // 16-byte accesses (rows and d are multiples of 16 bytes)
 };
 
-// A C x D tile on its way from memory to LDS, 16 bytes per thread and step, in registers.
-template <typename T, int C, int D, int NT>
+// A C x D tile on its way from memory to LDS, 16 bytes per thread and step, in registers. VEC: rows and d are
+// multiples of 16 bytes; else element by element. Rows and columns that do not exist are 0.
+template <typename T, int C, int D, int NT, bool VEC>
 struct Stage {
-    static constexpr int VE = 16 / sizeof(T), VR = D / VE, N = (C * VR + NT - 1) / NT;
+    static constexpr int VE = 16 / sizeof(T), VR = D / VE, RS = NT / VR, N = (C + RS - 1) / RS;
     static constexpr int LD = D + kPad, PLANE = C * LD;
-    static constexpr bool kEven = C * VR % NT == 0;
+    static_assert(NT % VR == 0, "a row's threads");
+    static constexpr bool kEven = C % RS == 0;
     uint4 r[N];
 
     __device__ __forceinline__ void load(const Rows<T> &s, int64_t t0, int rows, int tid) {
+        const __amdgpu_buffer_rsrc_t buf = buffer(s.p + t0 * s.stride);
+        const int row = tid / VR, col = tid % VR * VE;
+        const uint32_t stride = uint32_t(s.stride) * uint32_t(sizeof(T));
+        const uint32_t off = uint32_t(row) * stride + uint32_t(col) * uint32_t(sizeof(T));
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const int idx = tid + n * NT, row = idx / VR, col = idx % VR * VE;
-            uint4 x = make_uint4(0, 0, 0, 0);
-            if ((kEven || idx < C * VR) && row < rows && col < s.d) {
-                const T *src = s.p + (t0 + row) * s.stride + col;
-                if (s.vec) {
-                    x = *reinterpret_cast<const uint4 *>(src);
-                } else {
-                    uint32_t w[4] = {0, 0, 0, 0};
+            const bool live = row + n * RS < (kEven ? rows : min(rows, C));
+            const uint32_t at = off + uint32_t(n * RS) * stride;
+            if constexpr (VEC) {
+                r[n] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(buf, live && col < s.d ? at : kNone, 0, 0));
+            } else {
+                uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
-                    for (int e = 0; e < VE; ++e)
-                        if (col + e < s.d) {
-                            if constexpr (sizeof(T) == 4) w[e] = *reinterpret_cast<const uint32_t *>(src + e);
-                            else w[e / 2] |= uint32_t(*reinterpret_cast<const u16 *>(src + e)) << (16 * (e % 2));
-                        }
-                    x = make_uint4(w[0], w[1], w[2], w[3]);
+                for (int e = 0; e < VE; ++e) {
+                    const uint32_t a = live && col + e < s.d ? at + e * uint32_t(sizeof(T)) : kNone;
+                    if constexpr (sizeof(T) == 4) w[e] = __builtin_amdgcn_raw_buffer_load_b32(buf, a, 0, 0);
+                    else w[e / 2] |= uint32_t(u16(__builtin_amdgcn_raw_buffer_load_b16(buf, a, 0, 0))) << (16 * (e % 2));
                 }
+                r[n] = make_uint4(w[0], w[1], w[2], w[3]);
             }
-            r[n] = x;
         }
     }
 
     // Into the tile's planes. float16 and float32 are cut after 8 significant bits per plane, which is exact;
     // an infinity or NaN stands in the first plane alone.
     __device__ __forceinline__ void store(u16 *tile, int tid) const {
+        const int row0 = tid / VR, col = tid % VR * VE;
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const int idx = tid + n * NT, row = idx / VR, col = idx % VR * VE;
-            if (!kEven && idx >= C * VR) break;
+            const int row = row0 + n * RS;
+            if (!kEven && row >= C) break;
             u16 *dst = tile + row * LD + col;
             const uint32_t w[4] = {r[n].x, r[n].y, r[n].z, r[n].w};
             if constexpr (std::is_same_v<T, bf16_t>) {
@@ -358,10 +367,11 @@ __device__ __forceinline__ void zero_masked_scores(u16 *M, bool rev, int tid, in
 }
 
 // O = diag(row) X S for the wave's columns, from the state S before (after, REV) the chunk.
-template <typename T, int C, int KD, int NC>
+// PS: the state's planes.
+template <typename T, int C, int KD, int NC, int PS>
 __device__ __forceinline__ void inter(f32x4 (&O)[C / 16][NC], const f32x4 (&S)[KD / 16][NC], const u16 *X, const float *row,
                                       float scale, int lane) {
-    constexpr int LD = KD + kPad, PL = C * LD, PI = Cfg<T>::in, PS = Cfg<T>::st;
+    constexpr int LD = KD + kPad, PL = C * LD, PI = Cfg<T>::in;
     const int g = lane / 16, i = lane % 16;
 #pragma unroll
     for (int t = 0; t < C / 16; ++t)
@@ -559,26 +569,51 @@ __device__ __forceinline__ void store_state(const f32x4 (&S)[KD / 16][NC], const
             }
 }
 
-// The wave's C x 16 NC outputs to T or float32 rows.
-template <typename T, int C, int NC>
-__device__ __forceinline__ void store_out(const f32x4 (&O)[C / 16][NC], void *out, bool f32, int64_t stride, int64_t t0, int rows,
-                                          int cols, int col, int lane) {
+// The wave's C x 16 NC outputs to rows of T, or of float32 (F32). Rows of 16-bit types in 16-byte pieces go through the
+// wave's own columns of a tile that no other wave reads any more.
+template <typename T, int C, int NC, int LDV, bool VEC, bool F32>
+__device__ __forceinline__ void store_out(const f32x4 (&O)[C / 16][NC], void *out, int64_t stride, int64_t t0, int rows, int cols, int col0,
+                                          u16 *tile, int col, int lane) {
     const int g = lane / 16, i = lane % 16;
+    constexpr uint32_t ES = F32 ? 4 : sizeof(T);
+    const __amdgpu_buffer_rsrc_t buf = buffer(static_cast<char *>(out) + t0 * stride * ES);
+    const uint32_t step = uint32_t(stride) * ES;
+    if constexpr (VEC && !F32 && sizeof(T) == 2) {
 #pragma unroll
-    for (int t = 0; t < C / 16; ++t)
+        for (int t = 0; t < C / 16; ++t)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int n = 16 * t + 4 * g + r;
-            if (n >= rows) continue;
-            const int64_t at = (t0 + n) * stride;
+            for (int c = 0; c < NC; ++c)
 #pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                const int x = col + 16 * c + i;
-                if (x >= cols) continue;
-                if (f32) reinterpret_cast<float *>(out)[at + x] = O[t][c][r];
-                else reinterpret_cast<T *>(out)[at + x] = from_f32<T>(O[t][c][r]);
-            }
+                for (int r = 0; r < 4; r += 2) {
+                    const uint32_t w = std::is_same_v<T, bf16_t> ? pack_bf16x2(O[t][c][r], O[t][c][r + 1]) : pack_f16x2(O[t][c][r], O[t][c][r + 1]);
+                    u16 *dst = tile + (16 * t + 4 * g + r) * LDV + col + 16 * c + i;
+                    dst[0] = u16(w);
+                    dst[LDV] = u16(w >> 16);
+                }
+        constexpr int PR = 2 * NC;   // pieces of a row
+#pragma unroll
+        for (int n = 0; n < C * PR / 64; ++n) {
+            const int x = n * 64 + lane, row = x / PR, c = x % PR * 8;
+            const u32x4 w = *reinterpret_cast<const u32x4 *>(tile + row * LDV + col + c);
+            const bool live = row < rows && col0 + col + c < cols;
+            __builtin_amdgcn_raw_buffer_store_b128(w, buf, live ? uint32_t(row) * step + uint32_t(col0 + col + c) * 2 : kNone, 0, 0);
         }
+    } else {
+#pragma unroll
+        for (int t = 0; t < C / 16; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int n = 16 * t + 4 * g + r;
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    const int x = col0 + col + 16 * c + i;
+                    const uint32_t at = n < rows && x < cols ? uint32_t(n) * step + uint32_t(x) * ES : kNone;
+                    if constexpr (ES == 4) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(O[t][c][r]), buf, at, 0, 0);
+                    else if constexpr (std::is_same_v<T, bf16_t>) __builtin_amdgcn_raw_buffer_store_b16(short(pack_bf16x2(O[t][c][r], 0.f)), buf, at, 0, 0);
+                    else __builtin_amdgcn_raw_buffer_store_b16(short(pack_f16x2(O[t][c][r], 0.f)), buf, at, 0, 0);
+                }
+            }
+    }
 }
 
 // dot[n] = sum over the wave's columns of O[n][x] Z[n][x], into part[n] (lanes i == 0 write).

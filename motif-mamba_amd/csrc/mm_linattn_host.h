@@ -34,7 +34,7 @@ struct WalkArgs {
     int64_t s0_step;
     State s1;              // state after the last token
     void *out;             // T, or float32 with out_f32
-    int out_f32;
+    int out_f32, out_vec;  // out_vec: 16-byte stores
     int64_t out_batch, out_seq, out_head;
     float *e;              // [bh][seqlen]
     float *ck;             // [bh][blocks][kdim][cdim]: states before token (i + 1) kBlock; the last one after the last token
@@ -55,7 +55,7 @@ struct BwdArgs {
     const float *r0;       // [bh][segs][dk][dv]: the state's gradient at each segment's end; NULL: zeros
     float *dr;             // [bh][dk][dv]: at the first token
     void *dv_out, *dk_out; // [batch][seqlen][heads][dv], [batch][seqlen][heads][dk] (float32 with dk_f32)
-    int dk_f32;
+    int dk_f32, out_vec;
     float *a, *f;          // [bh][seqlen] each, or NULL: no gradient of the decays
     const float *ck;       // [bh][blocks][dv][dk]
     float *y;              // [bh][blocks][4]
