@@ -30,7 +30,7 @@ __device__ __forceinline__ Rows<T> rows_of(const View &v, int64_t b, int64_t h, 
 // workgroup, 16 NC per wave. DOT: also e[t] = (the product with the state alone) . Z_t, and the state at every
 // kBlock-th token into ck (the decays' gradient).
 template <typename T, int KD, int NC, bool DOT, bool VEC, bool F32>
-__global__ void __launch_bounds__(kThreads, 2) la_walk(const WalkArgs a) {
+__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) la_walk(const WalkArgs a) {
     constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, PS = Cfg<T>::st, W = 64 * NC;
     constexpr int LDX = KD + kPad, LDV = W + kPad, LDM = C + kPad;
     constexpr int NT = C / 16 * (C / 16 + 1) / 2;   // score tiles
@@ -70,13 +70,13 @@ __global__ void __launch_bounds__(kThreads, 2) la_walk(const WalkArgs a) {
     };
     auto decay = [&](int64_t t0) {
         const int64_t t = t0 + lane;
-        return lane < C && t < tend ? load_g(a.g, a.gtype, g0 + t * a.g_seq) : 0.f;
+        return lane < C && t < tend ? load_g_raw(a.g, a.gtype, g0 + t * a.g_seq) : 0u;
     };
     const int dwave = kWaves - 1;
-    float gnext = 0.f;
+    uint32_t gnext = 0;
     load(tbeg);
     if (wave == dwave) {
-        make_decays<C>(dec[0], decay(tbeg), lane);
+        make_decays<C>(dec[0], decode_g(decay(tbeg), a.gtype), lane);
         if (tbeg + C < tend) gnext = decay(tbeg + C);
     }
     int buf = 0;
@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(kThreads, 2) la_walk(const WalkArgs a) {
         inter<T, C, KD, NC, DOT ? 3 : PS>(O, S, X, d.in, a.scale, lane);
         if constexpr (DOT) dot_rows<T, C, NC, LDV>(O, Z, col, part + wave * C, lane);
         if (wave == dwave && more) {
-            make_decays<C>(dec[buf ^ 1], gnext, lane);
+            make_decays<C>(dec[buf ^ 1], decode_g(gnext, a.gtype), lane);
             if (t0 + 2 * C < tend) gnext = decay(t0 + 2 * C);
         }
         __syncthreads();
@@ -164,14 +164,14 @@ __global__ void __launch_bounds__(kThreads) la_segments(const WalkArgs a) {
     load_state<KD, 1>(S, Mat{nullptr, 0, 0}, 0, 0, 0, lane);
     SX sy;
     SV sv;
-    float g = 0.f;
+    uint32_t g = 0;
     double total = 0.0;
     auto load = [&](int64_t n) {
         const int64_t t0 = tbeg + (REV ? chunks - 1 - n : n) * C;
         const int rows = int(min(int64_t(C), tend - t0));
         sy.load(ry, t0, rows, tid);
         sv.load(rv, t0, rows, tid);
-        if (wave == 0) g = lane < rows ? load_g(a.g, a.gtype, g0 + (t0 + lane) * a.g_seq) : 0.f;
+        if (wave == 0) g = lane < rows ? load_g_raw(a.g, a.gtype, g0 + (t0 + lane) * a.g_seq) : 0u;
     };
     load(0);
     for (int64_t n = 0; n < chunks; ++n) {
@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(kThreads) la_segments(const WalkArgs a) {
         sy.store(Y, tid);
         sv.store(V, tid);
         if (wave == 0) {
-            make_decays<C>(*dec, g, lane);
+            make_decays<C>(*dec, decode_g(g, a.gtype), lane);
             total += double(dec->hi[C - 1]) + double(dec->lo[C - 1]);
         }
         if (n + 1 < chunks) load(n + 1);
@@ -189,26 +189,28 @@ __global__ void __launch_bounds__(kThreads) la_segments(const WalkArgs a) {
         update<T, C, KD, 1>(S, v, Y, REV ? dec->in : dec->out, a.scale, dec->all, lane);
     }
     store_state<KD, 1>(S, Mat{a.st + (bh * a.segs + seg) * a.kdim * a.cdim, a.cdim, 1}, a.kdim, a.cdim, col0 + col, lane);
-    if (slice == 0 && tid == 0) a.seg_decay[bh * a.segs + seg] = expf(float(total));
+    if (slice == 0 && tid == 0) a.seg_decay[bh * a.segs + seg] = exp_f32(float(total));
 }
 
 // Backward walk from the end: dv, dk, the scores' part of the decays' gradient (a), the state's part (f), and at
 // every kBlock-th token the product of the state there with its gradient (y). Waves 0 to 3 hold the gradient R of the
-// state for dv (rows dk, columns dv), waves 4 to 7 its transpose for dk.
-template <typename T, int KD, int VD, bool VEC, bool F32>
-__global__ void __launch_bounds__(2 * kThreads) la_bwd(const BwdArgs a) {
+// state for dv (rows dk, columns dv), waves 4 to 7 its transpose for dk: two walks over the same tiles, each in code of
+// its own with the same barriers.
+//
+// FOR_K: the walk of dk, X = v, Y = do, V = q; else that of dv, X = k, Y = q, V = do. KX: X's padded row length, KV: V's.
+template <typename T, int KD, int VD, bool VEC, bool F32, bool FOR_K>
+__device__ __forceinline__ void bwd_walk(const BwdArgs &a, char *smem, int tid, int wave, int lane) {
     constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, PS = Cfg<T>::st, NT2 = 2 * kThreads;
     constexpr int LDK = KD + kPad, LDV = VD + kPad, LDM = C + kPad, CT = C / 16;
-    constexpr int NT = CT * (CT + 1) / 2, NV = VD / 64, NK = KD / 64;
+    constexpr int NT = CT * (CT + 1) / 2;
+    constexpr int KX = FOR_K ? VD : KD, NC = (FOR_K ? KD : VD) / 64, LDC = FOR_K ? LDK : LDV;
     typedef Stage<T, C, KD, NT2, VEC> SK;
     typedef Stage<T, C, VD, NT2, VEC> SV;
-    extern __shared__ __attribute__((aligned(16))) char smem[];
     u16 *Q = reinterpret_cast<u16 *>(smem), *K = Q + PI * C * LDK, *V = K + PI * C * LDK, *G = V + PI * C * LDV;
     u16 *M1 = G + PI * C * LDV, *M2 = M1 + PS * C * LDM;
     Decays<C> *dec = reinterpret_cast<Decays<C> *>(M2 + PS * C * LDM);
     float *rowp = reinterpret_cast<float *>(dec + 2), *colp = rowp + CT * C, *part = colp + CT * C;
 
-    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64;
     int64_t id = blockIdx.x;
     const int seg = id % a.segs; id /= a.segs;
     const int64_t h = id % a.heads, b = id / a.heads, bh = b * a.heads + h;
@@ -217,35 +219,32 @@ __global__ void __launch_bounds__(2 * kThreads) la_bwd(const BwdArgs a) {
     const Rows<T> rq = rows_of<T>(a.q, b, h, a.dk, 0), rk = rows_of<T>(a.k, b, h, a.dk, 0);
     const Rows<T> rv = rows_of<T>(a.v, b, h, a.dv, 0), rd = rows_of<T>(a.dout, b, h, a.dv, 0);
     const int64_t g0 = b * a.g_batch + h * a.g_head;
-    const bool for_v = wave < kWaves;
-    const int col = (wave % kWaves) * 16 * (for_v ? NV : NK);
+    const int col = (wave % kWaves) * 16 * NC, rows_s = FOR_K ? a.dv : a.dk, cols_s = FOR_K ? a.dk : a.dv;
 
-    // R at the segment's end.
-    const float *r0 = a.r0 ? a.r0 + (bh * a.segs + seg) * int64_t(a.dk) * a.dv : nullptr;
-    f32x4 SV_[KD / 16][NV], SK_[VD / 16][NK];
-    if (for_v) {
-        load_state<KD, NV>(SV_, Mat{const_cast<float *>(r0), a.dv, 1}, a.dk, a.dv, col, lane);
-    } else {
-        load_state<VD, NK>(SK_, Mat{const_cast<float *>(r0), 1, a.dv}, a.dv, a.dk, col, lane);
-    }
+    // R (or its transpose) at the segment's end.
+    f32x4 S[KX / 16][NC];
+    load_state<KX, NC>(S, Mat{a.r0 ? const_cast<float *>(a.r0) + (bh * a.segs + seg) * int64_t(a.dk) * a.dv : nullptr, FOR_K ? 1 : a.dv,
+                              FOR_K ? a.dv : 1}, rows_s, cols_s, col, lane);
     // <R, state> at a kept boundary, each wave's share.
     auto boundary = [&](int64_t m) {
         const float *s = a.ck + (bh * a.blocks + m) * int64_t(a.dk) * a.dv;   // rows dv, columns dk
-        const int g = lane / 16, i = lane % 16;
+        const int g = lane / 16, i = lane % 16, rows = afresh(rows_s), cols = afresh(cols_s);
         float sum = 0.f;
 #pragma unroll
-        for (int k = 0; k < VD / 16; ++k)
+        for (int k = 0; k < KX / 16; ++k)
 #pragma unroll
-            for (int c = 0; c < NK; ++c)
+            for (int c = 0; c < NC; ++c)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int y = 16 * k + 4 * g + r, x = col + 16 * c + i;
-                    if (y < a.dv && x < a.dk) sum = __builtin_fmaf(SK_[k][c][r], s[int64_t(y) * a.dk + x], sum);
+                    if (y < rows && x < cols) sum = __builtin_fmaf(S[k][c][r], s[int64_t(y) * cols + x], sum);
                 }
         sum = wave_sum(sum);
         if (lane == 0) a.y[(bh * a.blocks + m) * kWaves + wave - kWaves] = sum;
     };
-    if (!for_v && a.ck && a.has_last && seg == a.segs - 1) boundary(a.blocks - 1);
+    if constexpr (FOR_K) {
+        if (a.ck && a.has_last && seg == a.segs - 1) boundary(a.blocks - 1);
+    }
 
     zero_masked_scores<C, PS>(M1, true, tid, NT2);
     zero_masked_scores<C, PS>(M2, true, tid, NT2);
@@ -262,13 +261,13 @@ __global__ void __launch_bounds__(2 * kThreads) la_bwd(const BwdArgs a) {
     };
     auto decay = [&](int64_t n) {
         const int64_t t = start(n) + lane;
-        return lane < C && t < tend ? load_g(a.g, a.gtype, g0 + t * a.g_seq) : 0.f;
+        return lane < C && t < tend ? load_g_raw(a.g, a.gtype, g0 + t * a.g_seq) : 0u;
     };
-    const int dwave = 2 * kWaves - 1;
-    float gnext = 0.f;
+    const bool dwave = !FOR_K && wave == kWaves - 1;
+    uint32_t gnext = 0;
     load(0);
-    if (wave == dwave) {
-        make_decays<C>(dec[0], decay(0), lane);
+    if (dwave) {
+        make_decays<C>(dec[0], decode_g(decay(0), a.gtype), lane);
         if (chunks > 1) gnext = decay(1);
     }
     int buf = 0;
@@ -313,47 +312,53 @@ __global__ void __launch_bounds__(2 * kThreads) la_bwd(const BwdArgs a) {
                 if (lane < 16) colp[m * C + jj] = cs;
             }
         }
-        f32x4 OV[CT][NV], OK[CT][NK];
-        if (for_v) {
-            inter<T, C, KD, NV, PS>(OV, SV_, K, d.out, 1.f, lane);
-        } else {
-            inter<T, C, VD, NK, 3>(OK, SK_, V, d.out, 1.f, lane);
-            if (a.a) dot_rows<T, C, NK, LDK>(OK, K, col, part + (wave - kWaves) * C, lane);
+        f32x4 O[CT][NC];
+        inter<T, C, KX, NC, FOR_K ? 3 : PS>(O, S, FOR_K ? V : K, d.out, 1.f, lane);
+        if constexpr (FOR_K) {
+            if (a.a) dot_rows<T, C, NC, LDK>(O, K, col, part + (wave - kWaves) * C, lane);
         }
-        if (wave == dwave && more) {
-            make_decays<C>(dec[buf ^ 1], gnext, lane);
+        if (dwave && more) {
+            make_decays<C>(dec[buf ^ 1], decode_g(gnext, a.gtype), lane);
             if (n + 2 < chunks) gnext = decay(n + 2);
         }
         __syncthreads();
-        if (a.a && tid < rows) {
-            const int t = tid / 16;
-            float sum = 0.f, f = 0.f;
-            for (int o = 0; o <= t; ++o) sum += rowp[o * C + tid];
-            for (int m = t; m < CT; ++m) sum -= colp[m * C + tid];
+        if constexpr (!FOR_K) {
+            if (a.a && tid < rows) {
+                const int t = tid / 16;
+                float sum = 0.f, f = 0.f;
+                for (int o = 0; o <= t; ++o) sum += rowp[o * C + tid];
+                for (int m = t; m < CT; ++m) sum -= colp[m * C + tid];
 #pragma unroll
-            for (int w = 0; w < kWaves; ++w) f += part[w * C + tid];
-            a.a[bh * a.seqlen + t0 + tid] = sum;
-            a.f[bh * a.seqlen + t0 + tid] = f;
+                for (int w = 0; w < kWaves; ++w) f += part[w * C + tid];
+                a.a[bh * a.seqlen + t0 + tid] = sum;
+                a.f[bh * a.seqlen + t0 + tid] = f;
+            }
         }
-        if (for_v) {
-            bf16x8 v[C / 32][NV][PI];
-            load_v<T, C, NV, LDV>(v, G, col, lane);
-            intra<T, C, NV, LDV, true>(OV, v, M1, G, col, lane);
-            update<T, C, KD, NV>(SV_, v, Q, d.in, a.scale, d.all, lane);
-            store_out<T, C, NV, LDV, VEC, false>(OV, reinterpret_cast<T *>(a.dv_out) + (b * a.seqlen * a.heads + h) * a.dv, a.heads * a.dv, t0,
-                                                 rows, a.dv, 0, V, col, lane);
-        } else {
-            bf16x8 v[C / 32][NK][PI];
-            load_v<T, C, NK, LDK>(v, Q, col, lane);
-            intra<T, C, NK, LDK, true>(OK, v, M2, Q, col, lane);
-            update<T, C, VD, NK>(SK_, v, G, d.in, a.scale, d.all, lane);
-            store_out<T, C, NK, LDK, VEC, F32>(OK, static_cast<char *>(a.dk_out) + (b * a.seqlen * a.heads + h) * a.dk * int64_t(F32 ? 4 : sizeof(T)),
+        const u16 *VT = FOR_K ? Q : G;
+        bf16x8 v[C / 32][NC][PI];
+        load_v<T, C, NC, LDC>(v, VT, col, lane);
+        intra<T, C, NC, LDC, true>(O, v, FOR_K ? M2 : M1, VT, col, lane);
+        update<T, C, KX, NC>(S, v, FOR_K ? G : Q, d.in, a.scale, d.all, lane);
+        if constexpr (FOR_K) {
+            store_out<T, C, NC, LDC, VEC, F32>(O, static_cast<char *>(a.dk_out) + (b * a.seqlen * a.heads + h) * a.dk * int64_t(F32 ? 4 : sizeof(T)),
                                                a.heads * a.dk, t0, rows, a.dk, 0, K, col, lane);
             if (a.ck && t0 > 0 && t0 % kBlock == 0) boundary(t0 / kBlock - 1);
+        } else {
+            store_out<T, C, NC, LDC, VEC, false>(O, reinterpret_cast<T *>(a.dv_out) + (b * a.seqlen * a.heads + h) * a.dv, a.heads * a.dv, t0, rows,
+                                                 a.dv, 0, V, col, lane);
         }
     }
-    if (a.dr && seg == 0 && for_v)
-        store_state<KD, NV>(SV_, Mat{a.dr + bh * int64_t(a.dk) * a.dv, a.dv, 1}, a.dk, a.dv, col, lane);
+    if constexpr (!FOR_K) {
+        if (a.dr && seg == 0) store_state<KX, NC>(S, Mat{a.dr + bh * int64_t(a.dk) * a.dv, a.dv, 1}, a.dk, a.dv, col, lane);
+    }
+}
+
+template <typename T, int KD, int VD, bool VEC, bool F32>
+__global__ void __launch_bounds__(2 * kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) la_bwd(const BwdArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64;
+    if (wave < kWaves) bwd_walk<T, KD, VD, VEC, F32, false>(a, smem, tid, wave, lane);
+    else bwd_walk<T, KD, VD, VEC, F32, true>(a, smem, tid, wave, lane);
 }
 
 template <typename K, typename A>
@@ -531,7 +536,7 @@ __global__ void __launch_bounds__(kBlock) la_decay_grad(const float *a, const fl
     for (int n = c0; n < tid; ++n) s += sf[n];
     for (int n = c0 + C - 1; n >= tid; --n) s += sa[n];
     // A forgotten state has no gradient; the sums above are of terms that cancel.
-    if (load_g(g, gtype, bh / heads * g_batch + t * g_seq + bh % heads * g_head) == -128.f) s = 0.f;
+    if (decode_g(load_g_raw(g, gtype, bh / heads * g_batch + t * g_seq + bh % heads * g_head), gtype) == -128.f) s = 0.f;
     if (tmp) tmp[bh * seqlen + t] = s;
     else store_g(out, gtype, (bh / heads * seqlen + t) * heads + bh % heads, s);
 }

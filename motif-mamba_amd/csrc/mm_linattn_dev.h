@@ -47,16 +47,24 @@ template <> struct Cfg<float> { static constexpr int in = 3, st = 3, up = 3, C =
 constexpr int kBlock = 256;      // tokens between two kept states (see the decays' gradient)
 constexpr int kPad = 8;          // elements after an LDS row: 16 rows then start in 16 different bank groups
 
-__device__ __forceinline__ float load_g(const void *p, mm_dtype t, int64_t i) {
-    float x;
-    switch (t) {
-        case MM_FLOAT32: x = reinterpret_cast<const float *>(p)[i]; break;
-        case MM_FLOAT16: x = to_f32(reinterpret_cast<const f16_t *>(p)[i]); break;
-        default: x = to_f32(reinterpret_cast<const bf16_t *>(p)[i]);
-    }
+// A log decay's bits (converted when used, so that the load is waited for there).
+__device__ __forceinline__ uint32_t load_g_raw(const void *p, mm_dtype t, int64_t i) {
+    if (t == MM_FLOAT32) return reinterpret_cast<const uint32_t *>(p)[i];
+    return reinterpret_cast<const u16 *>(p)[i];
+}
+__device__ __forceinline__ float decode_g(uint32_t w, mm_dtype t) {
+    const float x = t == MM_FLOAT32 ? __uint_as_float(w) : t == MM_BFLOAT16 ? __uint_as_float(w << 16) : elem_f32<f16_t>(w);
     // exp(-128) is 0 in float32 as every smaller decay is; a finite sum keeps the differences of two
     // sums defined. The comparison is false for NaN, which stays.
     return x < -128.f ? -128.f : x;
+}
+
+// exp(x): 2^(x log2 e) with the product's rounding error and log2 e's own taken back in (v_exp_f32 is within 1 ulp).
+__device__ __forceinline__ float exp_f32(float x) {
+    const float p = x * kLog2e;
+    const float e = __builtin_fmaf(x, 1.925963033e-8f, __builtin_fmaf(x, kLog2e, -p));
+    const float r = __builtin_amdgcn_exp2f(p);
+    return __builtin_fmaf(r, e * kLn2, r);
 }
 
 // ---- planes --------------------------------------------------------------------------------------
@@ -263,33 +271,35 @@ __device__ __forceinline__ double prefix_f64(double x) {
     return x;
 }
 
+__device__ __forceinline__ double shfl_f64(double x, int lane) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = __builtin_amdgcn_ds_bpermute(lane * 4, int(uint32_t(b))), hi = __builtin_amdgcn_ds_bpermute(lane * 4, int(uint32_t(b >> 32)));
+    return __builtin_bit_cast(double, uint64_t(lo) | uint64_t(hi) << 32);
+}
+
 // One wave; g: the lane's token's log decay, 0 behind the last token and in lanes past C.
 template <int C>
 __device__ __forceinline__ void make_decays(Decays<C> &d, float g, int lane) {
     const double c = prefix_f64(double(g));
-    double end[C / 16], mine_end = 0.0, mine_start = 0.0;
-#pragma unroll
-    for (int t = 0; t < C / 16; ++t) {
-        end[t] = readlane_f64(c, 16 * t + 15);
-        if (lane / 16 == t) mine_end = end[t];
-        if (lane / 16 == t + 1) mine_start = end[t];
-    }
-    const double all = end[C / 16 - 1];
-    if (lane < C) {
-        d.in[lane] = expf(float(c));
-        d.out[lane] = expf(float(all - c));
-        d.from[lane] = expf(float(c - mine_start));
-        d.to[lane] = expf(float(mine_end - c));
-        const float hi = float(c);
+    const double all = readlane_f64(c, C - 1);
+    const int tile = lane / 16;
+    const double end = shfl_f64(c, 16 * tile + 15), before = shfl_f64(c, 16 * tile - 1 & 63);
+    // lane 4 I + J of the first 16: from the end of tile J to the start of tile I (J < I)
+    const int I = lane / 4 % 4, J = lane % 4;
+    const double mid = shfl_f64(c, 16 * I - 1 & 63) - shfl_f64(c, 16 * J + 15);
+    const float hi = float(c);
+    const float in = exp_f32(hi + float(c - double(hi))), out = exp_f32(float(all - c)), from = exp_f32(float(c - (tile ? before : 0.0))),
+                to = exp_f32(float(end - c)), m = exp_f32(float(mid));
+    if (C == 64 || lane < C) {
+        d.in[lane] = in;
+        d.out[lane] = out;
+        d.from[lane] = from;
+        d.to[lane] = to;
         d.hi[lane] = hi;
         d.lo[lane] = float(c - double(hi));
+        if (lane == C - 1) d.all = in;
     }
-    if (lane == 0) d.all = expf(float(all));
-#pragma unroll
-    for (int I = 1; I < C / 16; ++I)
-#pragma unroll
-        for (int J = 0; J < I; ++J)
-            if (lane == I * 4 + J) d.mid[I][J] = expf(float(end[I - 1] - end[J]));
+    if (lane < 16 && I < C / 16 && J < I) d.mid[I][J] = m;
 }
 
 // ---- a chunk's steps -----------------------------------------------------------------------------
@@ -299,17 +309,17 @@ template <typename T, int C, int KD>
 __device__ __forceinline__ f32x4 score_tile(const u16 *X, const u16 *Y, int ot, int nt, int lane) {
     constexpr int LD = KD + kPad, PL = C * LD, P = Cfg<T>::in;
     const int g = lane / 16, i = lane % 16;
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    bf16x8 a[KD / 32][P], b[KD / 32][P];
 #pragma unroll
-    for (int k = 0; k < KD / 32; ++k) {
-        bf16x8 a[P], b[P];
+    for (int k = 0; k < KD / 32; ++k)
 #pragma unroll
         for (int p = 0; p < P; ++p) {
-            a[p] = frag_row(Y + p * PL + (16 * nt + i) * LD, 32 * k, g);
-            b[p] = frag_row(X + p * PL + (16 * ot + i) * LD, 32 * k, g);
+            a[k][p] = frag_row(Y + p * PL + (16 * nt + i) * LD, 32 * k, g);
+            b[k][p] = frag_row(X + p * PL + (16 * ot + i) * LD, 32 * k, g);
         }
-        acc = mma<P, P, 3>(acc, a, b);
-    }
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < KD / 32; ++k) acc = mma<P, P, 3>(acc, a[k], b[k]);
     return acc;
 }
 
@@ -331,7 +341,7 @@ __device__ __forceinline__ f32x4 tile_decay(const Decays<C> &d, int ot, int nt, 
         for (int r = 0; r < 4; ++r) {
             const float x = (d.hi[o] - hi[r]) + (d.lo[o] - lo[r]);
             const bool sees = REV ? n + r >= o : n + r <= o;
-            f[r] = sees ? expf(REV ? -x : x) * scale : 0.f;
+            f[r] = sees ? exp_f32(REV ? -x : x) * scale : 0.f;
         }
     }
     return f;
@@ -377,8 +387,19 @@ __device__ __forceinline__ void inter(f32x4 (&O)[C / 16][NC], const f32x4 (&S)[K
     for (int t = 0; t < C / 16; ++t)
 #pragma unroll
         for (int c = 0; c < NC; ++c) O[t][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+    // The rows of the next 32 columns are read while the products of these run.
+    bf16x8 a[2][C / 16][PI];
+    auto read = [&](int k) {
+#pragma unroll
+        for (int t = 0; t < C / 16; ++t)
+#pragma unroll
+            for (int p = 0; p < PI; ++p) a[k % 2][t][p] = frag_row(X + p * PL + (16 * t + i) * LD, 32 * k, g);
+    };
+    read(0);
 #pragma unroll
     for (int k = 0; k < KD / 32; ++k) {
+        if (k + 1 < KD / 32) read(k + 1);
+        __builtin_amdgcn_sched_barrier(0);
         bf16x8 s[NC][PS];
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
@@ -391,13 +412,15 @@ __device__ __forceinline__ void inter(f32x4 (&O)[C / 16][NC], const f32x4 (&S)[K
             split8<PS>(x, s[c]);
         }
 #pragma unroll
-        for (int t = 0; t < C / 16; ++t) {
-            bf16x8 a[PI];
+        for (int p = 0; p < PI; ++p)
 #pragma unroll
-            for (int p = 0; p < PI; ++p) a[p] = frag_row(X + p * PL + (16 * t + i) * LD, 32 * k, g);
+            for (int q = 0; q < PS; ++q)
+                if (p + q < PS)
 #pragma unroll
-            for (int c = 0; c < NC; ++c) O[t][c] = mma<PI, PS, PS>(O[t][c], a, s[c]);
-        }
+                    for (int t = 0; t < C / 16; ++t)
+#pragma unroll
+                        for (int c = 0; c < NC; ++c)
+                            O[t][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[k % 2][t][p], s[c][q], O[t][c], 0, 0, 0);
     }
 #pragma unroll
     for (int t = 0; t < C / 16; ++t) {
@@ -443,13 +466,31 @@ __device__ __forceinline__ void update(f32x4 (&S)[KD / 16][NC], const bf16x8 (&v
             }
             split8<PU>(x, u[c]);
         }
+        constexpr int KB = PI > 1 ? 2 : 4;   // rows of tiles read ahead
+        bf16x8 a[2][KB][PI];
+        auto read = [&](int b) {
 #pragma unroll
-        for (int k = 0; k < KD / 16; ++k) {
-            bf16x8 a[PI];
+            for (int k = 0; k < KB; ++k)
 #pragma unroll
-            for (int p = 0; p < PI; ++p) a[p] = frag_tr<LD>(Y + p * PL, 32 * j, 16 * k, g, i);
+                for (int p = 0; p < PI; ++p)
+                    if (b * KB + k < KD / 16) a[b % 2][k][p] = frag_tr<LD>(Y + p * PL, 32 * j, 16 * (b * KB + k), g, i);
+        };
+        read(0);
 #pragma unroll
-            for (int c = 0; c < NC; ++c) S[k][c] = mma<PI, PU, PU>(S[k][c], a, u[c]);
+        for (int b = 0; b * KB < KD / 16; ++b) {
+            if ((b + 1) * KB < KD / 16) read(b + 1);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int p = 0; p < PI; ++p)
+#pragma unroll
+                for (int q = 0; q < PU; ++q)
+                    if (p + q < PU)
+#pragma unroll
+                        for (int k = 0; k < KB; ++k)
+#pragma unroll
+                            for (int c = 0; c < NC; ++c)
+                                if (b * KB + k < KD / 16)
+                                    S[b * KB + k][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[b % 2][k][p], u[c][q], S[b * KB + k][c], 0, 0, 0);
         }
     }
 }
@@ -486,16 +527,26 @@ __device__ __forceinline__ void intra(f32x4 (&O)[C / 16][NC], const bf16x8 (&v0)
     const bool odd = most[0] >= 0x7f80 || most[1] >= 0x7f80;
     auto product = [&](const bf16x8 (&v)[C / 32][NC][PI]) {
 #pragma unroll
-        for (int t = 0; t < C / 16; ++t)
+        for (int j = 0; j < C / 32; ++j) {
+            bf16x8 a[C / 16][PS];
 #pragma unroll
-            for (int j = 0; j < C / 32; ++j) {
-                if (REV ? 2 * j + 1 < t : 2 * j > t) continue;
-                bf16x8 a[PS];
+            for (int t = 0; t < C / 16; ++t)
+                if (REV ? 2 * j + 1 >= t : 2 * j <= t)
 #pragma unroll
-                for (int p = 0; p < PS; ++p) a[p] = frag_row(M + p * PL + (16 * t + i) * LD, 32 * j, g);
+                    for (int p = 0; p < PS; ++p) a[t][p] = frag_row(M + p * PL + (16 * t + i) * LD, 32 * j, g);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int c = 0; c < NC; ++c) O[t][c] = mma<PS, PI, PS>(O[t][c], a, v[j][c]);
-            }
+            for (int p = 0; p < PS; ++p)
+#pragma unroll
+                for (int q = 0; q < PI; ++q)
+                    if (p + q < PS)
+#pragma unroll
+                        for (int t = 0; t < C / 16; ++t)
+#pragma unroll
+                            for (int c = 0; c < NC; ++c)
+                                if (REV ? 2 * j + 1 >= t : 2 * j <= t)
+                                    O[t][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[t][p], v[j][c][q], O[t][c], 0, 0, 0);
+        }
     };
     if (!__any(odd)) {
         product(v0);
@@ -537,6 +588,13 @@ __device__ __forceinline__ void intra(f32x4 (&O)[C / 16][NC], const bf16x8 (&v0)
         }
 }
 
+// A number that the compiler does not know to be the one it was: keeps the bounds of the states' loads and stores from
+// being computed once and held through the walk.
+__device__ __forceinline__ int afresh(int x) {
+    asm volatile("" : "+s"(x));
+    return x;
+}
+
 // A float32 matrix of a (batch row, head): rows x cols, with its strides.
 struct Mat {
     float *p;
@@ -545,6 +603,8 @@ struct Mat {
 template <int KD, int NC>
 __device__ __forceinline__ void load_state(f32x4 (&S)[KD / 16][NC], const Mat &m, int rows, int cols, int col, int lane) {
     const int g = lane / 16, i = lane % 16;
+    rows = afresh(rows);
+    cols = afresh(cols);
 #pragma unroll
     for (int k = 0; k < KD / 16; ++k)
 #pragma unroll
@@ -558,6 +618,8 @@ __device__ __forceinline__ void load_state(f32x4 (&S)[KD / 16][NC], const Mat &m
 template <int KD, int NC>
 __device__ __forceinline__ void store_state(const f32x4 (&S)[KD / 16][NC], const Mat &m, int rows, int cols, int col, int lane) {
     const int g = lane / 16, i = lane % 16;
+    rows = afresh(rows);
+    cols = afresh(cols);
 #pragma unroll
     for (int k = 0; k < KD / 16; ++k)
 #pragma unroll
