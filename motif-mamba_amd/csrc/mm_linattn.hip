@@ -32,7 +32,7 @@ __device__ __forceinline__ Rows<T> rows_of(const View &v, int64_t b, int64_t h, 
 template <typename T, int KD, int NC, bool DOT, bool VEC, bool F32>
 __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) la_walk(const WalkArgs a) {
     constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, PS = Cfg<T>::st, W = 64 * NC;
-    constexpr int LDX = KD + kPad, LDV = W + kPad, LDM = C + kPad;
+    constexpr int LDX = KD, LDV = W, LDM = kScoreRow;
     constexpr int NT = C / 16 * (C / 16 + 1) / 2;   // score tiles
     typedef Stage<T, C, KD, kThreads, VEC> SX;
     typedef Stage<T, C, W, kThreads, VEC> SV;
@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
 template <typename T, int KD, bool REV, bool VEC>
 __global__ void __launch_bounds__(kThreads) la_segments(const WalkArgs a) {
     constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, W = 64;
-    constexpr int LDX = KD + kPad, LDV = W + kPad;
+    constexpr int LDX = KD, LDV = W;
     typedef Stage<T, C, KD, kThreads, VEC> SX;
     typedef Stage<T, C, W, kThreads, VEC> SV;
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -201,7 +201,7 @@ __global__ void __launch_bounds__(kThreads) la_segments(const WalkArgs a) {
 template <typename T, int KD, int VD, bool VEC, bool F32, bool FOR_K>
 __device__ __forceinline__ void bwd_walk(const BwdArgs &a, char *smem, int tid, int wave, int lane) {
     constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, PS = Cfg<T>::st, NT2 = 2 * kThreads;
-    constexpr int LDK = KD + kPad, LDV = VD + kPad, LDM = C + kPad, CT = C / 16;
+    constexpr int LDK = KD, LDV = VD, LDM = kScoreRow, CT = C / 16;
     constexpr int NT = CT * (CT + 1) / 2;
     constexpr int KX = FOR_K ? VD : KD, NC = (FOR_K ? KD : VD) / 64, LDC = FOR_K ? LDK : LDV;
     typedef Stage<T, C, KD, NT2, VEC> SK;
@@ -371,7 +371,7 @@ static int launch_kernel(K kernel, int bytes, hipError_t set, int64_t grid, int 
 template <typename T, int KD, int NC, bool DOT, bool VEC, bool F32>
 static int launch_walk_t(const WalkArgs &a, hipStream_t s) {
     constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, PS = Cfg<T>::st;
-    constexpr int bytes = 2 * (2 * PI * C * (KD + kPad) + (DOT ? 2 : 1) * PI * C * (64 * NC + kPad) + PS * C * (C + kPad)) +
+    constexpr int bytes = 2 * (2 * PI * C * KD + (DOT ? 2 : 1) * PI * C * 64 * NC + PS * C * kScoreRow) +
                           2 * int(sizeof(Decays<C>)) + (DOT ? 4 * kWaves * C : 0);
     static_assert(bytes <= 160 * 1024, "LDS");
     const auto kernel = la_walk<T, KD, NC, DOT, VEC, F32>;
@@ -392,7 +392,7 @@ static int launch_walk_k(const WalkArgs &a, hipStream_t s) {
 template <typename T, int KD, bool REV, bool VEC>
 static int launch_segments_t(const WalkArgs &a0, hipStream_t s) {
     constexpr int C = Cfg<T>::C, PI = Cfg<T>::in;
-    constexpr int bytes = 2 * (PI * C * (KD + kPad) + PI * C * (64 + kPad)) + int(sizeof(Decays<C>));
+    constexpr int bytes = 2 * (PI * C * KD + PI * C * 64) + int(sizeof(Decays<C>));
     static_assert(bytes <= 160 * 1024, "LDS");
     const auto kernel = la_segments<T, KD, REV, VEC>;
     static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
@@ -409,7 +409,7 @@ static int launch_segments_k(const WalkArgs &a, bool rev, hipStream_t s) {
 template <typename T, int KD, int VD, bool VEC, bool F32>
 static int launch_bwd_t(const BwdArgs &a, hipStream_t s) {
     constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, PS = Cfg<T>::st;
-    constexpr int bytes = 2 * (2 * PI * C * (KD + kPad) + 2 * PI * C * (VD + kPad) + 2 * PS * C * (C + kPad)) +
+    constexpr int bytes = 2 * (2 * PI * C * KD + 2 * PI * C * VD + 2 * PS * C * kScoreRow) +
                           2 * int(sizeof(Decays<C>)) + 4 * (2 * (C / 16) * C + kWaves * C);
     static_assert(bytes <= 160 * 1024, "LDS");
     const auto kernel = la_bwd<T, KD, VD, VEC, F32>;
@@ -434,7 +434,6 @@ int launch_walk(const WalkArgs &a, bool dot, hipStream_t s) {
         if (a.kdim <= 64) return wide ? launch_walk_k<T, 64, 2, true>(a, s) : launch_walk_k<T, 64, 1, true>(a, s);
         return wide ? launch_walk_k<T, 128, 2, true>(a, s) : launch_walk_k<T, 128, 1, true>(a, s);
     }
-    if (a.kdim <= 32) return wide ? launch_walk_k<T, 32, 2, false>(a, s) : launch_walk_k<T, 32, 1, false>(a, s);
     if (a.kdim <= 64) return wide ? launch_walk_k<T, 64, 2, false>(a, s) : launch_walk_k<T, 64, 1, false>(a, s);
     return wide ? launch_walk_k<T, 128, 2, false>(a, s) : launch_walk_k<T, 128, 1, false>(a, s);
 }

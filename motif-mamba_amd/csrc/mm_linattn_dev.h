@@ -45,7 +45,17 @@ template <> struct Cfg<f16_t> { static constexpr int in = 2, st = 2, up = 3, C =
 template <> struct Cfg<float> { static constexpr int in = 3, st = 3, up = 3, C = 32; };
 
 constexpr int kBlock = 256;      // tokens between two kept states (see the decays' gradient)
-constexpr int kPad = 8;          // elements after an LDS row: 16 rows then start in 16 different bank groups
+
+// Tiles in LDS are rows of D elements (64 or 128; 64 scores), cut into units of 4 (8 bytes). Both ways that operands
+// are read, 16 rows of one unit (frag_row) and 4 rows of 4 units (frag_tr), should touch the 16 units of a 128-byte
+// line each once, so unit u of row r lies at u ^ swizzle(r): r's low two bits move a unit between the line's quarters,
+// its next two within one. Rows padded by 16 bytes instead cost 42 % of all LDS cycles in bank conflicts.
+__device__ __forceinline__ constexpr int swizzle(int row) { return (row & 3) << 2 | (row >> 2 & 3); }
+template <int D>
+__device__ __forceinline__ constexpr int at(int row, int col) {
+    return row * D + (((col >> 2) ^ swizzle(row)) << 2) + (col & 3);
+}
+constexpr int kScoreRow = 64;
 
 // A log decay's bits (converted when used, so that the load is waited for there).
 __device__ __forceinline__ uint32_t load_g_raw(const void *p, mm_dtype t, int64_t i) {
@@ -65,6 +75,17 @@ __device__ __forceinline__ float exp_f32(float x) {
     const float e = __builtin_fmaf(x, 1.925963033e-8f, __builtin_fmaf(x, kLog2e, -p));
     const float r = __builtin_amdgcn_exp2f(p);
     return __builtin_fmaf(r, e * kLn2, r);
+}
+
+// A number that the compiler does not know to be the one it was: what is computed from it is computed where it is used,
+// not once and held in registers through the walk (the walks would not fit their registers otherwise).
+__device__ __forceinline__ int afresh(int x) {
+    asm volatile("" : "+s"(x));
+    return x;
+}
+__device__ __forceinline__ int afresh_lane(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
 }
 
 // ---- planes --------------------------------------------------------------------------------------
@@ -105,17 +126,22 @@ __device__ __forceinline__ f32x4 mma(f32x4 acc, const bf16x8 *a, const bf16x8 *b
 __device__ __forceinline__ bf16x8 join(uint2 a, uint2 b) {
     return __builtin_bit_cast(bf16x8, u32x4{a.x, a.y, b.x, b.y});
 }
-// Operand with its row in `row` (an LDS row's start), contraction columns col .. col + 31.
-__device__ __forceinline__ bf16x8 frag_row(const u16 *row, int col, int g) {
-    return join(*reinterpret_cast<const uint2 *>(row + col + 4 * g), *reinterpret_cast<const uint2 *>(row + col + 16 + 4 * g));
+// Operand whose row or column is tile row r0 + i and whose contraction runs over tile columns 32 k .. 32 k + 31.
+template <int D>
+__device__ __forceinline__ bf16x8 frag_row(const u16 *tile, int r0, int k, int g, int i) {
+    const u16 *row = tile + (r0 + i) * D + (k / 2) * 64;
+    const int u = (8 * (k % 2) + g) ^ swizzle(i);
+    return join(*reinterpret_cast<const uint2 *>(row + 4 * u), *reinterpret_cast<const uint2 *>(row + 4 * (u ^ 4)));
 }
-// Operand whose row or column is tile column col + i and whose contraction runs over tile rows r0 .. r0 + 31.
-template <int LD>
+// Operand whose row or column is tile column col + i and whose contraction runs over tile rows r0 .. r0 + 31
+// (r0 and col multiples of 16).
+template <int D>
 __device__ __forceinline__ bf16x8 frag_tr(const u16 *tile, int r0, int col, int g, int i) {
-    const u16 *a = tile + (r0 + 4 * g + i / 4) * LD + col + 4 * (i % 4);
+    const int u = ((col / 16 % 4) ^ (i / 4)) << 2 | ((i % 4) ^ g);
+    const u16 *a = tile + (r0 + 4 * g + i / 4) * D + col / 64 * 64 + 4 * u;
     typedef __attribute__((address_space(3))) s16x4 *lds_ptr;
     const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)a);
-    const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(a + 16 * LD));
+    const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(a + 16 * D));
     return join(__builtin_bit_cast(uint2, x), __builtin_bit_cast(uint2, y));
 }
 
@@ -149,12 +175,13 @@ template <typename T> struct Rows {
 template <typename T, int C, int D, int NT, bool VEC>
 struct Stage {
     static constexpr int VE = 16 / sizeof(T), VR = D / VE, RS = NT / VR, N = (C + RS - 1) / RS;
-    static constexpr int LD = D + kPad, PLANE = C * LD;
+    static constexpr int PLANE = C * D;
     static_assert(NT % VR == 0, "a row's threads");
     static constexpr bool kEven = C % RS == 0;
     uint4 r[N];
 
     __device__ __forceinline__ void load(const Rows<T> &s, int64_t t0, int rows, int tid) {
+        tid = afresh_lane(tid);
         const __amdgpu_buffer_rsrc_t buf = buffer(s.p + t0 * s.stride);
         const int row = tid / VR, col = tid % VR * VE;
         const uint32_t stride = uint32_t(s.stride) * uint32_t(sizeof(T));
@@ -181,15 +208,19 @@ struct Stage {
     // Into the tile's planes. float16 and float32 are cut after 8 significant bits per plane, which is exact;
     // an infinity or NaN stands in the first plane alone.
     __device__ __forceinline__ void store(u16 *tile, int tid) const {
+        tid = afresh_lane(tid);
         const int row0 = tid / VR, col = tid % VR * VE;
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             const int row = row0 + n * RS;
             if (!kEven && row >= C) break;
-            u16 *dst = tile + row * LD + col;
+            // Two units of 4 elements (one of float32), next to each other but in the order of the row's swizzle.
+            const int sw = swizzle(row);
+            const bool flip = VE == 8 && (sw & 1);
+            u16 *dst = tile + row * D + ((((col >> 2) ^ sw) & (VE == 8 ? ~1 : ~0)) << 2);
             const uint32_t w[4] = {r[n].x, r[n].y, r[n].z, r[n].w};
             if constexpr (std::is_same_v<T, bf16_t>) {
-                *reinterpret_cast<uint4 *>(dst) = r[n];
+                *reinterpret_cast<uint4 *>(dst) = flip ? make_uint4(w[2], w[3], w[0], w[1]) : r[n];
             } else {
                 constexpr int P = Cfg<T>::in;
                 uint32_t o[P][VE / 2];
@@ -213,7 +244,7 @@ struct Stage {
                 }
 #pragma unroll
                 for (int p = 0; p < P; ++p) {
-                    if constexpr (VE == 8) *reinterpret_cast<uint4 *>(dst + p * PLANE) = make_uint4(o[p][0], o[p][1], o[p][2], o[p][3]);
+                    if constexpr (VE == 8) *reinterpret_cast<uint4 *>(dst + p * PLANE) = flip ? make_uint4(o[p][2], o[p][3], o[p][0], o[p][1]) : make_uint4(o[p][0], o[p][1], o[p][2], o[p][3]);
                     else *reinterpret_cast<uint2 *>(dst + p * PLANE) = make_uint2(o[p][0], o[p][1]);
                 }
             }
@@ -307,15 +338,16 @@ __device__ __forceinline__ void make_decays(Decays<C> &d, float g, int lane) {
 // Scores of one 16 x 16 tile: column i the row token 16 ot + i of X, rows 4g + r the tokens 16 nt + 4g + r of Y.
 template <typename T, int C, int KD>
 __device__ __forceinline__ f32x4 score_tile(const u16 *X, const u16 *Y, int ot, int nt, int lane) {
-    constexpr int LD = KD + kPad, PL = C * LD, P = Cfg<T>::in;
+    constexpr int PL = C * KD, P = Cfg<T>::in;
+    lane = afresh_lane(lane);
     const int g = lane / 16, i = lane % 16;
     bf16x8 a[KD / 32][P], b[KD / 32][P];
 #pragma unroll
     for (int k = 0; k < KD / 32; ++k)
 #pragma unroll
         for (int p = 0; p < P; ++p) {
-            a[k][p] = frag_row(Y + p * PL + (16 * nt + i) * LD, 32 * k, g);
-            b[k][p] = frag_row(X + p * PL + (16 * ot + i) * LD, 32 * k, g);
+            a[k][p] = frag_row<KD>(Y + p * PL, 16 * nt, k, g, i);
+            b[k][p] = frag_row<KD>(X + p * PL, 16 * ot, k, g, i);
         }
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -327,6 +359,7 @@ __device__ __forceinline__ f32x4 score_tile(const u16 *X, const u16 *Y, int ot, 
 // see later ones. f32x4: one factor per accumulator element.
 template <int C, bool REV>
 __device__ __forceinline__ f32x4 tile_decay(const Decays<C> &d, int ot, int nt, float scale, int lane) {
+    lane = afresh_lane(lane);
     const int g = lane / 16, i = lane % 16;
     const int o = 16 * ot + i, n = 16 * nt + 4 * g;
     f32x4 f;
@@ -350,8 +383,9 @@ __device__ __forceinline__ f32x4 tile_decay(const Decays<C> &d, int ot, int nt, 
 // Four consecutive scores of row token 16 ot + i into the score tile's planes ([row token][other token]).
 template <int C, int P>
 __device__ __forceinline__ void store_scores(u16 *M, const float *x, int ot, int nt, int lane) {
-    constexpr int LD = C + kPad, PL = C * LD;
-    u16 *dst = M + (16 * ot + lane % 16) * LD + 16 * nt + 4 * (lane / 16);
+    lane = afresh_lane(lane);
+    constexpr int PL = C * kScoreRow;
+    u16 *dst = M + 16 * ot * kScoreRow + at<kScoreRow>(lane % 16, 16 * nt + 4 * (lane / 16));
     float r[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
     for (int p = 0; p < P; ++p) {
@@ -368,11 +402,11 @@ __device__ __forceinline__ void store_scores(u16 *M, const float *x, int ot, int
 // (written once; the chunks write the other tiles only).
 template <int C, int P>
 __device__ __forceinline__ void zero_masked_scores(u16 *M, bool rev, int tid, int nt) {
-    constexpr int LD = C + kPad, PL = C * LD;
+    constexpr int PL = C * kScoreRow;
     for (int x = tid; x < C / 32 * 16 * 16 * P; x += nt) {
         const int p = x / (C / 32 * 256), y = x % (C / 32 * 256), pair = y / 256, r = y % 256 / 16, c = y % 16;
         const int row = 32 * pair + (rev ? 16 : 0) + r, col = 32 * pair + (rev ? 0 : 16) + c;
-        M[p * PL + row * LD + col] = 0;
+        M[p * PL + at<kScoreRow>(row, col)] = 0;
     }
 }
 
@@ -381,7 +415,8 @@ __device__ __forceinline__ void zero_masked_scores(u16 *M, bool rev, int tid, in
 template <typename T, int C, int KD, int NC, int PS>
 __device__ __forceinline__ void inter(f32x4 (&O)[C / 16][NC], const f32x4 (&S)[KD / 16][NC], const u16 *X, const float *row,
                                       float scale, int lane) {
-    constexpr int LD = KD + kPad, PL = C * LD, PI = Cfg<T>::in;
+    constexpr int PL = C * KD, PI = Cfg<T>::in;
+    lane = afresh_lane(lane);
     const int g = lane / 16, i = lane % 16;
 #pragma unroll
     for (int t = 0; t < C / 16; ++t)
@@ -393,7 +428,7 @@ __device__ __forceinline__ void inter(f32x4 (&O)[C / 16][NC], const f32x4 (&S)[K
 #pragma unroll
         for (int t = 0; t < C / 16; ++t)
 #pragma unroll
-            for (int p = 0; p < PI; ++p) a[k % 2][t][p] = frag_row(X + p * PL + (16 * t + i) * LD, 32 * k, g);
+            for (int p = 0; p < PI; ++p) a[k % 2][t][p] = frag_row<KD>(X + p * PL, 16 * t, k, g, i);
     };
     read(0);
 #pragma unroll
@@ -436,7 +471,8 @@ __device__ __forceinline__ void inter(f32x4 (&O)[C / 16][NC], const f32x4 (&S)[K
 template <typename T, int C, int KD, int NC>
 __device__ __forceinline__ void update(f32x4 (&S)[KD / 16][NC], const bf16x8 (&v)[C / 32][NC][Cfg<T>::in], const u16 *Y,
                                        const float *w, float scale, float all, int lane) {
-    constexpr int LD = KD + kPad, PL = C * LD, PI = Cfg<T>::in, PU = Cfg<T>::up;
+    constexpr int PL = C * KD, PI = Cfg<T>::in, PU = Cfg<T>::up;
+    lane = afresh_lane(lane);
     const int g = lane / 16, i = lane % 16;
 #pragma unroll
     for (int k = 0; k < KD / 16; ++k)
@@ -473,7 +509,7 @@ __device__ __forceinline__ void update(f32x4 (&S)[KD / 16][NC], const bf16x8 (&v
             for (int k = 0; k < KB; ++k)
 #pragma unroll
                 for (int p = 0; p < PI; ++p)
-                    if (b * KB + k < KD / 16) a[b % 2][k][p] = frag_tr<LD>(Y + p * PL, 32 * j, 16 * (b * KB + k), g, i);
+                    if (b * KB + k < KD / 16) a[b % 2][k][p] = frag_tr<KD>(Y + p * PL, 32 * j, 16 * (b * KB + k), g, i);
         };
         read(0);
 #pragma unroll
@@ -497,6 +533,7 @@ __device__ __forceinline__ void update(f32x4 (&S)[KD / 16][NC], const bf16x8 (&v
 
 template <typename T, int C, int NC, int LDV>
 __device__ __forceinline__ void load_v(bf16x8 (&v)[C / 32][NC][Cfg<T>::in], const u16 *V, int col, int lane) {
+    lane = afresh_lane(lane);
     constexpr int PL = C * LDV;
 #pragma unroll
     for (int j = 0; j < C / 32; ++j)
@@ -512,7 +549,8 @@ __device__ __forceinline__ void load_v(bf16x8 (&v)[C / 32][NC][Cfg<T>::in], cons
 template <typename T, int C, int NC, int LDV, bool REV>
 __device__ __forceinline__ void intra(f32x4 (&O)[C / 16][NC], const bf16x8 (&v0)[C / 32][NC][Cfg<T>::in], const u16 *M,
                                       const u16 *V, int col, int lane) {
-    constexpr int LD = C + kPad, PL = C * LD, PI = Cfg<T>::in, PS = Cfg<T>::st;
+    constexpr int PL = C * kScoreRow, PI = Cfg<T>::in, PS = Cfg<T>::st;
+    lane = afresh_lane(lane);
     const int g = lane / 16, i = lane % 16;
     typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
     u16x2 most = {0, 0};
@@ -533,7 +571,7 @@ __device__ __forceinline__ void intra(f32x4 (&O)[C / 16][NC], const bf16x8 (&v0)
             for (int t = 0; t < C / 16; ++t)
                 if (REV ? 2 * j + 1 >= t : 2 * j <= t)
 #pragma unroll
-                    for (int p = 0; p < PS; ++p) a[t][p] = frag_row(M + p * PL + (16 * t + i) * LD, 32 * j, g);
+                    for (int p = 0; p < PS; ++p) a[t][p] = frag_row<kScoreRow>(M + p * PL, 16 * t, j, g, i);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int p = 0; p < PS; ++p)
@@ -571,7 +609,7 @@ __device__ __forceinline__ void intra(f32x4 (&O)[C / 16][NC], const bf16x8 (&v0)
     for (int n = 0; n < C; ++n)
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            const float x = __uint_as_float(uint32_t(V[n * LDV + col + 16 * c + i]) << 16);
+            const float x = __uint_as_float(uint32_t(V[at<LDV>(n, col + 16 * c + i)]) << 16);
             const bool bad = (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u;
             if (!__any(bad)) continue;
 #pragma unroll
@@ -582,17 +620,10 @@ __device__ __forceinline__ void intra(f32x4 (&O)[C / 16][NC], const bf16x8 (&v0)
                     if (!bad || (REV ? n < o : n > o)) continue;
                     float m = 0.f;
 #pragma unroll
-                    for (int p = PS - 1; p >= 0; --p) m += __uint_as_float(uint32_t(M[p * PL + o * LD + n]) << 16);
+                    for (int p = PS - 1; p >= 0; --p) m += __uint_as_float(uint32_t(M[p * PL + at<kScoreRow>(o, n)]) << 16);
                     O[t][c][r] += m * x;
                 }
         }
-}
-
-// A number that the compiler does not know to be the one it was: keeps the bounds of the states' loads and stores from
-// being computed once and held through the walk.
-__device__ __forceinline__ int afresh(int x) {
-    asm volatile("" : "+s"(x));
-    return x;
 }
 
 // A float32 matrix of a (batch row, head): rows x cols, with its strides.
@@ -602,6 +633,7 @@ struct Mat {
 };
 template <int KD, int NC>
 __device__ __forceinline__ void load_state(f32x4 (&S)[KD / 16][NC], const Mat &m, int rows, int cols, int col, int lane) {
+    lane = afresh_lane(lane);
     const int g = lane / 16, i = lane % 16;
     rows = afresh(rows);
     cols = afresh(cols);
@@ -617,6 +649,7 @@ __device__ __forceinline__ void load_state(f32x4 (&S)[KD / 16][NC], const Mat &m
 }
 template <int KD, int NC>
 __device__ __forceinline__ void store_state(const f32x4 (&S)[KD / 16][NC], const Mat &m, int rows, int cols, int col, int lane) {
+    lane = afresh_lane(lane);
     const int g = lane / 16, i = lane % 16;
     rows = afresh(rows);
     cols = afresh(cols);
@@ -636,6 +669,7 @@ __device__ __forceinline__ void store_state(const f32x4 (&S)[KD / 16][NC], const
 template <typename T, int C, int NC, int LDV, bool VEC, bool F32>
 __device__ __forceinline__ void store_out(const f32x4 (&O)[C / 16][NC], void *out, int64_t stride, int64_t t0, int rows, int cols, int col0,
                                           u16 *tile, int col, int lane) {
+    lane = afresh_lane(lane);
     const int g = lane / 16, i = lane % 16;
     constexpr uint32_t ES = F32 ? 4 : sizeof(T);
     const __amdgpu_buffer_rsrc_t buf = buffer(static_cast<char *>(out) + t0 * stride * ES);
@@ -648,15 +682,17 @@ __device__ __forceinline__ void store_out(const f32x4 (&O)[C / 16][NC], void *ou
 #pragma unroll
                 for (int r = 0; r < 4; r += 2) {
                     const uint32_t w = std::is_same_v<T, bf16_t> ? pack_bf16x2(O[t][c][r], O[t][c][r + 1]) : pack_f16x2(O[t][c][r], O[t][c][r + 1]);
-                    u16 *dst = tile + (16 * t + 4 * g + r) * LDV + col + 16 * c + i;
-                    dst[0] = u16(w);
-                    dst[LDV] = u16(w >> 16);
+                    tile[16 * t * LDV + at<LDV>(4 * g + r, col + 16 * c + i)] = u16(w);
+                    tile[16 * t * LDV + at<LDV>(4 * g + r + 1, col + 16 * c + i)] = u16(w >> 16);
                 }
         constexpr int PR = 2 * NC;   // pieces of a row
 #pragma unroll
         for (int n = 0; n < C * PR / 64; ++n) {
-            const int x = n * 64 + lane, row = x / PR, c = x % PR * 8;
-            const u32x4 w = *reinterpret_cast<const u32x4 *>(tile + row * LDV + col + c);
+            const int row = n * (64 / PR) + lane / PR, c = lane % PR * 8;
+            const u16 *src = tile + n * (64 / PR) * LDV;   // whole tiles of 16 rows down
+            const uint2 w0 = *reinterpret_cast<const uint2 *>(src + at<LDV>(lane / PR, col + c)),
+                        w1 = *reinterpret_cast<const uint2 *>(src + at<LDV>(lane / PR, col + c + 4));
+            const u32x4 w = {w0.x, w0.y, w1.x, w1.y};
             const bool live = row < rows && col0 + col + c < cols;
             __builtin_amdgcn_raw_buffer_store_b128(w, buf, live ? uint32_t(row) * step + uint32_t(col0 + col + c) * 2 : kNone, 0, 0);
         }
@@ -682,6 +718,7 @@ __device__ __forceinline__ void store_out(const f32x4 (&O)[C / 16][NC], void *ou
 template <typename T, int C, int NC, int LDZ>
 __device__ __forceinline__ void dot_rows(const f32x4 (&O)[C / 16][NC], const u16 *Z, int col, float *part, int lane) {
     constexpr int PL = C * LDZ, PI = Cfg<T>::in;
+    lane = afresh_lane(lane);
     const int g = lane / 16, i = lane % 16;
 #pragma unroll
     for (int t = 0; t < C / 16; ++t) {
@@ -691,7 +728,7 @@ __device__ __forceinline__ void dot_rows(const f32x4 (&O)[C / 16][NC], const u16
             float x = 0.f;
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
-                const u16 *z = Z + (16 * t + 4 * g + r) * LDZ + col + 16 * c + i;
+                const u16 *z = Z + 16 * t * LDZ + at<LDZ>(4 * g + r, col + 16 * c + i);
                 float y = 0.f;
 #pragma unroll
                 for (int p = PI - 1; p >= 0; --p) y += __uint_as_float(uint32_t(z[p * PL]) << 16);
