@@ -42,7 +42,15 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
     Decays<C> *dec = reinterpret_cast<Decays<C> *>(Z + (DOT ? PI * C * LDV : 0));
     float *part = reinterpret_cast<float *>(dec + 2);
 
-    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64;
+    constexpr bool kTight = DOT || NC > 1;   // registers
+    int tid = threadIdx.x, lane = tid % 64;
+    const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
+    auto fresh = [&] {
+        if constexpr (kTight) {
+            tid = afresh_lane(tid);
+            lane = tid % 64;
+        }
+    };
     int64_t id = blockIdx.x;
     const int slice = id % a.slices; id /= a.slices;
     const int seg = id % a.segs; id /= a.segs;
@@ -88,6 +96,7 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
                                     col0 + col, lane);
         }
         __syncthreads();
+        fresh();
         sx.store(X, tid);
         sy.store(Y, tid);
         sv.store(V, tid);
@@ -95,6 +104,7 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
         const bool more = t0 + C < tend;
         if (more) load(t0 + C);
         __syncthreads();
+        fresh();
         const Decays<C> &d = dec[buf];
         for (int t = wave; t < NT; t += kWaves) {
             int o = 0, n = t;
@@ -107,6 +117,7 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
             store_scores<C, PS>(M, x, o, n, lane);
         }
         f32x4 O[C / 16][NC];
+        fresh();
         inter<T, C, KD, NC, DOT ? 3 : PS>(O, S, X, d.in, a.scale, lane);
         if constexpr (DOT) dot_rows<T, C, NC, LDV>(O, Z, col, part + wave * C, lane);
         if (wave == dwave && more) {
@@ -114,6 +125,7 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
             if (t0 + 2 * C < tend) gnext = decay(t0 + 2 * C);
         }
         __syncthreads();
+        fresh();
         if constexpr (DOT) {
             if (tid < rows) {
                 float e = 0.f;
@@ -126,6 +138,7 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
         load_v<T, C, NC, LDV>(v, V, col, lane);
         intra<T, C, NC, LDV, false>(O, v, M, V, col, lane);
         update<T, C, KD, NC>(S, v, Y, d.out, 1.f, d.all, lane);
+        fresh();
         store_out<T, C, NC, LDV, VEC, F32>(O, static_cast<char *>(a.out) + (b * a.out_batch + h * a.out_head) * int64_t(F32 ? 4 : sizeof(T)),
                                            a.out_seq, t0, rows, a.cdim, col0, V, col, lane);
     }
@@ -200,6 +213,13 @@ __global__ void __launch_bounds__(kThreads) la_segments(const WalkArgs a) {
 // FOR_K: the walk of dk, X = v, Y = do, V = q; else that of dv, X = k, Y = q, V = do. KX: X's padded row length, KV: V's.
 template <typename T, int KD, int VD, bool VEC, bool F32, bool FOR_K>
 __device__ __forceinline__ void bwd_walk(const BwdArgs &a, char *smem, int tid, int wave, int lane) {
+    constexpr bool kTight = KD + VD > 128;   // registers
+    auto fresh = [&] {
+        if constexpr (kTight) {
+            tid = afresh_lane(tid);
+            lane = tid % 64;
+        }
+    };
     constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, PS = Cfg<T>::st, NT2 = 2 * kThreads;
     constexpr int LDK = KD, LDV = VD, LDM = kScoreRow, CT = C / 16;
     constexpr int NT = CT * (CT + 1) / 2;
@@ -275,6 +295,7 @@ __device__ __forceinline__ void bwd_walk(const BwdArgs &a, char *smem, int tid, 
         const int64_t t0 = start(n);
         const int rows = int(min(int64_t(C), tend - t0));
         __syncthreads();
+        fresh();
         sq.store(Q, tid);
         sk.store(K, tid);
         sv.store(V, tid);
@@ -282,6 +303,7 @@ __device__ __forceinline__ void bwd_walk(const BwdArgs &a, char *smem, int tid, 
         const bool more = n + 1 < chunks;
         if (more) load(n + 1);
         __syncthreads();
+        fresh();
         const Decays<C> &d = dec[buf];
         for (int t = wave; t < NT; t += 2 * kWaves) {
             int x = 0, y = t;
@@ -313,6 +335,7 @@ __device__ __forceinline__ void bwd_walk(const BwdArgs &a, char *smem, int tid, 
             }
         }
         f32x4 O[CT][NC];
+        fresh();
         inter<T, C, KX, NC, FOR_K ? 3 : PS>(O, S, FOR_K ? V : K, d.out, 1.f, lane);
         if constexpr (FOR_K) {
             if (a.a) dot_rows<T, C, NC, LDK>(O, K, col, part + (wave - kWaves) * C, lane);
@@ -322,6 +345,7 @@ __device__ __forceinline__ void bwd_walk(const BwdArgs &a, char *smem, int tid, 
             if (n + 2 < chunks) gnext = decay(n + 2);
         }
         __syncthreads();
+        fresh();
         if constexpr (!FOR_K) {
             if (a.a && tid < rows) {
                 const int t = tid / 16;
@@ -339,6 +363,7 @@ __device__ __forceinline__ void bwd_walk(const BwdArgs &a, char *smem, int tid, 
         load_v<T, C, NC, LDC>(v, VT, col, lane);
         intra<T, C, NC, LDC, true>(O, v, FOR_K ? M2 : M1, VT, col, lane);
         update<T, C, KX, NC>(S, v, FOR_K ? G : Q, d.in, a.scale, d.all, lane);
+        fresh();
         if constexpr (FOR_K) {
             store_out<T, C, NC, LDC, VEC, F32>(O, static_cast<char *>(a.dk_out) + (b * a.seqlen * a.heads + h) * a.dk * int64_t(F32 ? 4 : sizeof(T)),
                                                a.heads * a.dk, t0, rows, a.dk, 0, K, col, lane);

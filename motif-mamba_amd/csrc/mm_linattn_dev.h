@@ -181,7 +181,6 @@ struct Stage {
     uint4 r[N];
 
     __device__ __forceinline__ void load(const Rows<T> &s, int64_t t0, int rows, int tid) {
-        tid = afresh_lane(tid);
         const __amdgpu_buffer_rsrc_t buf = buffer(s.p + t0 * s.stride);
         const int row = tid / VR, col = tid % VR * VE;
         const uint32_t stride = uint32_t(s.stride) * uint32_t(sizeof(T));
@@ -208,7 +207,6 @@ struct Stage {
     // Into the tile's planes. float16 and float32 are cut after 8 significant bits per plane, which is exact;
     // an infinity or NaN stands in the first plane alone.
     __device__ __forceinline__ void store(u16 *tile, int tid) const {
-        tid = afresh_lane(tid);
         const int row0 = tid / VR, col = tid % VR * VE;
 #pragma unroll
         for (int n = 0; n < N; ++n) {
@@ -339,7 +337,6 @@ __device__ __forceinline__ void make_decays(Decays<C> &d, float g, int lane) {
 template <typename T, int C, int KD>
 __device__ __forceinline__ f32x4 score_tile(const u16 *X, const u16 *Y, int ot, int nt, int lane) {
     constexpr int PL = C * KD, P = Cfg<T>::in;
-    lane = afresh_lane(lane);
     const int g = lane / 16, i = lane % 16;
     bf16x8 a[KD / 32][P], b[KD / 32][P];
 #pragma unroll
@@ -359,7 +356,6 @@ __device__ __forceinline__ f32x4 score_tile(const u16 *X, const u16 *Y, int ot, 
 // see later ones. f32x4: one factor per accumulator element.
 template <int C, bool REV>
 __device__ __forceinline__ f32x4 tile_decay(const Decays<C> &d, int ot, int nt, float scale, int lane) {
-    lane = afresh_lane(lane);
     const int g = lane / 16, i = lane % 16;
     const int o = 16 * ot + i, n = 16 * nt + 4 * g;
     f32x4 f;
@@ -383,7 +379,6 @@ __device__ __forceinline__ f32x4 tile_decay(const Decays<C> &d, int ot, int nt, 
 // Four consecutive scores of row token 16 ot + i into the score tile's planes ([row token][other token]).
 template <int C, int P>
 __device__ __forceinline__ void store_scores(u16 *M, const float *x, int ot, int nt, int lane) {
-    lane = afresh_lane(lane);
     constexpr int PL = C * kScoreRow;
     u16 *dst = M + 16 * ot * kScoreRow + at<kScoreRow>(lane % 16, 16 * nt + 4 * (lane / 16));
     float r[4] = {x[0], x[1], x[2], x[3]};
@@ -416,7 +411,6 @@ template <typename T, int C, int KD, int NC, int PS>
 __device__ __forceinline__ void inter(f32x4 (&O)[C / 16][NC], const f32x4 (&S)[KD / 16][NC], const u16 *X, const float *row,
                                       float scale, int lane) {
     constexpr int PL = C * KD, PI = Cfg<T>::in;
-    lane = afresh_lane(lane);
     const int g = lane / 16, i = lane % 16;
 #pragma unroll
     for (int t = 0; t < C / 16; ++t)
@@ -472,7 +466,6 @@ template <typename T, int C, int KD, int NC>
 __device__ __forceinline__ void update(f32x4 (&S)[KD / 16][NC], const bf16x8 (&v)[C / 32][NC][Cfg<T>::in], const u16 *Y,
                                        const float *w, float scale, float all, int lane) {
     constexpr int PL = C * KD, PI = Cfg<T>::in, PU = Cfg<T>::up;
-    lane = afresh_lane(lane);
     const int g = lane / 16, i = lane % 16;
 #pragma unroll
     for (int k = 0; k < KD / 16; ++k)
@@ -533,7 +526,6 @@ __device__ __forceinline__ void update(f32x4 (&S)[KD / 16][NC], const bf16x8 (&v
 
 template <typename T, int C, int NC, int LDV>
 __device__ __forceinline__ void load_v(bf16x8 (&v)[C / 32][NC][Cfg<T>::in], const u16 *V, int col, int lane) {
-    lane = afresh_lane(lane);
     constexpr int PL = C * LDV;
 #pragma unroll
     for (int j = 0; j < C / 32; ++j)
@@ -550,7 +542,6 @@ template <typename T, int C, int NC, int LDV, bool REV>
 __device__ __forceinline__ void intra(f32x4 (&O)[C / 16][NC], const bf16x8 (&v0)[C / 32][NC][Cfg<T>::in], const u16 *M,
                                       const u16 *V, int col, int lane) {
     constexpr int PL = C * kScoreRow, PI = Cfg<T>::in, PS = Cfg<T>::st;
-    lane = afresh_lane(lane);
     const int g = lane / 16, i = lane % 16;
     typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
     u16x2 most = {0, 0};
@@ -633,7 +624,6 @@ struct Mat {
 };
 template <int KD, int NC>
 __device__ __forceinline__ void load_state(f32x4 (&S)[KD / 16][NC], const Mat &m, int rows, int cols, int col, int lane) {
-    lane = afresh_lane(lane);
     const int g = lane / 16, i = lane % 16;
     rows = afresh(rows);
     cols = afresh(cols);
@@ -649,7 +639,6 @@ __device__ __forceinline__ void load_state(f32x4 (&S)[KD / 16][NC], const Mat &m
 }
 template <int KD, int NC>
 __device__ __forceinline__ void store_state(const f32x4 (&S)[KD / 16][NC], const Mat &m, int rows, int cols, int col, int lane) {
-    lane = afresh_lane(lane);
     const int g = lane / 16, i = lane % 16;
     rows = afresh(rows);
     cols = afresh(cols);
@@ -669,7 +658,6 @@ __device__ __forceinline__ void store_state(const f32x4 (&S)[KD / 16][NC], const
 template <typename T, int C, int NC, int LDV, bool VEC, bool F32>
 __device__ __forceinline__ void store_out(const f32x4 (&O)[C / 16][NC], void *out, int64_t stride, int64_t t0, int rows, int cols, int col0,
                                           u16 *tile, int col, int lane) {
-    lane = afresh_lane(lane);
     const int g = lane / 16, i = lane % 16;
     constexpr uint32_t ES = F32 ? 4 : sizeof(T);
     const __amdgpu_buffer_rsrc_t buf = buffer(static_cast<char *>(out) + t0 * stride * ES);
@@ -718,7 +706,6 @@ __device__ __forceinline__ void store_out(const f32x4 (&O)[C / 16][NC], void *ou
 template <typename T, int C, int NC, int LDZ>
 __device__ __forceinline__ void dot_rows(const f32x4 (&O)[C / 16][NC], const u16 *Z, int col, float *part, int lane) {
     constexpr int PL = C * LDZ, PI = Cfg<T>::in;
-    lane = afresh_lane(lane);
     const int g = lane / 16, i = lane % 16;
 #pragma unroll
     for (int t = 0; t < C / 16; ++t) {
