@@ -30,25 +30,24 @@ __device__ __forceinline__ Rows<T> rows_of(const View &v, int64_t b, int64_t h, 
 // workgroup, 16 NC per wave. DOT: also e[t] = (the product with the state alone) . Z_t, and the state at every
 // kBlock-th token into ck (the decays' gradient).
 template <typename T, int KD, int NC, bool DOT, bool VEC, bool F32>
-__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) la_walk(const WalkArgs a) {
+__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(KD * NC == 64 ? 3 : 2, KD * NC == 64 ? 3 : 2))) la_walk(const WalkArgs a) {
     constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, PS = Cfg<T>::st, W = 64 * NC;
     constexpr int LDX = KD, LDV = W, LDM = kScoreRow;
-    constexpr int NT = C / 16 * (C / 16 + 1) / 2;   // score tiles
     typedef Stage<T, C, KD, kThreads, VEC> SX;
     typedef Stage<T, C, W, kThreads, VEC> SV;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    u16 *X = reinterpret_cast<u16 *>(smem), *Y = X + PI * C * LDX, *V = Y + PI * C * LDX;
-    u16 *M = V + PI * C * LDV, *Z = M + PS * C * LDM;
-    Decays<C> *dec = reinterpret_cast<Decays<C> *>(Z + (DOT ? PI * C * LDV : 0));
+    u16 *X = reinterpret_cast<u16 *>(smem), *Y = X + PI * kTile<C, LDX>, *V = Y + PI * kTile<C, LDX>;
+    u16 *M = V + PI * kTile<C, LDV>, *Z = M + PS * kTile<C, LDM>;
+    Decays<C> *dec = reinterpret_cast<Decays<C> *>(Z + (DOT ? PI * kTile<C, LDV> : 0));
     float *part = reinterpret_cast<float *>(dec + 2);
 
-    constexpr bool kTight = DOT || NC > 1;   // registers
-    int tid = threadIdx.x, lane = tid % 64;
+    constexpr bool kTight = true;
+    int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
     auto fresh = [&] {
         if constexpr (kTight) {
             tid = afresh_lane(tid);
-            lane = tid % 64;
+            lane = tid & 63;
         }
     };
     int64_t id = blockIdx.x;
@@ -84,7 +83,7 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
     uint32_t gnext = 0;
     load(tbeg);
     if (wave == dwave) {
-        make_decays<C>(dec[0], decode_g(decay(tbeg), a.gtype), lane);
+        make_decays<C>(dec[0], decode_g(decay(tbeg), a.gtype), a.scale, lane);
         if (tbeg + C < tend) gnext = decay(tbeg + C);
     }
     int buf = 0;
@@ -106,22 +105,28 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
         __syncthreads();
         fresh();
         const Decays<C> &d = dec[buf];
-        for (int t = wave; t < NT; t += kWaves) {
-            int o = 0, n = t;
-            while (n > o) n -= ++o;
-            f32x4 s = score_tile<T, C, KD>(X, Y, o, n, lane);
-            const f32x4 f = tile_decay<C, false>(d, o, n, a.scale, lane);
-            float x[4];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) x[r] = f[r] == 0.f && o == n ? 0.f : s[r] * f[r];
-            store_scores<C, PS>(M, x, o, n, lane);
+        // The score tiles, static for each wave; the last one, which also makes the next chunk's decays, has the fewest.
+        auto tiles = [&](auto L) { scores<T, C, KD, decltype(L)>(d, X, Y, M, a.scale, lane); };
+        if constexpr (C == 64) {
+            switch (wave) {
+                case 0: tiles(Tiles<3, 0, 3, 1, 3, 2>{}); break;
+                case 1: tiles(Tiles<2, 0, 2, 1, 2, 2>{}); break;
+                case 2: tiles(Tiles<1, 0, 1, 1, 3, 3>{}); break;
+                default: tiles(Tiles<0, 0>{});
+            }
+        } else {
+            switch (wave) {
+                case 0: tiles(Tiles<1, 0>{}); break;
+                case 1: tiles(Tiles<1, 1>{}); break;
+                case 2: tiles(Tiles<0, 0>{});
+            }
         }
         f32x4 O[C / 16][NC];
         fresh();
-        inter<T, C, KD, NC, DOT ? 3 : PS>(O, S, X, d.in, a.scale, lane);
+        inter<T, C, KD, NC, DOT ? 3 : PS>(O, S, X, d.in, lane);
         if constexpr (DOT) dot_rows<T, C, NC, LDV>(O, Z, col, part + wave * C, lane);
         if (wave == dwave && more) {
-            make_decays<C>(dec[buf ^ 1], decode_g(gnext, a.gtype), lane);
+            make_decays<C>(dec[buf ^ 1], decode_g(gnext, a.gtype), a.scale, lane);
             if (t0 + 2 * C < tend) gnext = decay(t0 + 2 * C);
         }
         __syncthreads();
@@ -137,7 +142,7 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
         bf16x8 v[C / 32][NC][PI];
         load_v<T, C, NC, LDV>(v, V, col, lane);
         intra<T, C, NC, LDV, false>(O, v, M, V, col, lane);
-        update<T, C, KD, NC>(S, v, Y, d.out, 1.f, d.all, lane);
+        update<T, C, KD, NC>(S, v, Y, d.out, d.all, lane);
         fresh();
         store_out<T, C, NC, LDV, VEC, F32>(O, static_cast<char *>(a.out) + (b * a.out_batch + h * a.out_head) * int64_t(F32 ? 4 : sizeof(T)),
                                            a.out_seq, t0, rows, a.cdim, col0, V, col, lane);
@@ -160,9 +165,9 @@ __global__ void __launch_bounds__(kThreads) la_segments(const WalkArgs a) {
     typedef Stage<T, C, KD, kThreads, VEC> SX;
     typedef Stage<T, C, W, kThreads, VEC> SV;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    u16 *Y = reinterpret_cast<u16 *>(smem), *V = Y + PI * C * LDX;
-    Decays<C> *dec = reinterpret_cast<Decays<C> *>(V + PI * C * LDV);
-    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64;
+    u16 *Y = reinterpret_cast<u16 *>(smem), *V = Y + PI * kTile<C, LDX>;
+    Decays<C> *dec = reinterpret_cast<Decays<C> *>(V + PI * kTile<C, LDV>);
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid & 63;
     int64_t id = blockIdx.x;
     const int slice = id % a.slices; id /= a.slices;
     const int seg = id % a.segs; id /= a.segs;
@@ -192,14 +197,14 @@ __global__ void __launch_bounds__(kThreads) la_segments(const WalkArgs a) {
         sy.store(Y, tid);
         sv.store(V, tid);
         if (wave == 0) {
-            make_decays<C>(*dec, decode_g(g, a.gtype), lane);
+            make_decays<C>(*dec, decode_g(g, a.gtype), a.scale, lane);
             total += double(dec->hi[C - 1]) + double(dec->lo[C - 1]);
         }
         if (n + 1 < chunks) load(n + 1);
         __syncthreads();
         bf16x8 v[C / 32][1][PI];
         load_v<T, C, 1, LDV>(v, V, col, lane);
-        update<T, C, KD, 1>(S, v, Y, REV ? dec->in : dec->out, a.scale, dec->all, lane);
+        update<T, C, KD, 1>(S, v, Y, REV ? dec->in : dec->out, dec->all, lane);
     }
     store_state<KD, 1>(S, Mat{a.st + (bh * a.segs + seg) * a.kdim * a.cdim, a.cdim, 1}, a.kdim, a.cdim, col0 + col, lane);
     if (slice == 0 && tid == 0) a.seg_decay[bh * a.segs + seg] = exp_f32(float(total));
@@ -217,18 +222,17 @@ __device__ __forceinline__ void bwd_walk(const BwdArgs &a, char *smem, int tid, 
     auto fresh = [&] {
         if constexpr (kTight) {
             tid = afresh_lane(tid);
-            lane = tid % 64;
+            lane = tid & 63;
         }
     };
     constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, PS = Cfg<T>::st, NT2 = 2 * kThreads;
     constexpr int LDK = KD, LDV = VD, LDM = kScoreRow, CT = C / 16;
-    constexpr int NT = CT * (CT + 1) / 2;
     constexpr int KX = FOR_K ? VD : KD, NC = (FOR_K ? KD : VD) / 64, LDC = FOR_K ? LDK : LDV;
     typedef Stage<T, C, KD, NT2, VEC> SK;
     typedef Stage<T, C, VD, NT2, VEC> SV;
-    u16 *Q = reinterpret_cast<u16 *>(smem), *K = Q + PI * C * LDK, *V = K + PI * C * LDK, *G = V + PI * C * LDV;
-    u16 *M1 = G + PI * C * LDV, *M2 = M1 + PS * C * LDM;
-    Decays<C> *dec = reinterpret_cast<Decays<C> *>(M2 + PS * C * LDM);
+    u16 *Q = reinterpret_cast<u16 *>(smem), *K = Q + PI * kTile<C, LDK>, *V = K + PI * kTile<C, LDK>, *G = V + PI * kTile<C, LDV>;
+    u16 *M1 = G + PI * kTile<C, LDV>, *M2 = M1 + PS * kTile<C, LDM>;
+    Decays<C> *dec = reinterpret_cast<Decays<C> *>(M2 + PS * kTile<C, LDM>);
     float *rowp = reinterpret_cast<float *>(dec + 2), *colp = rowp + CT * C, *part = colp + CT * C;
 
     int64_t id = blockIdx.x;
@@ -248,7 +252,7 @@ __device__ __forceinline__ void bwd_walk(const BwdArgs &a, char *smem, int tid, 
     // <R, state> at a kept boundary, each wave's share.
     auto boundary = [&](int64_t m) {
         const float *s = a.ck + (bh * a.blocks + m) * int64_t(a.dk) * a.dv;   // rows dv, columns dk
-        const int g = lane / 16, i = lane % 16, rows = afresh(rows_s), cols = afresh(cols_s);
+        const int g = (lane >> 4), i = (lane & 15), rows = afresh(rows_s), cols = afresh(cols_s);
         float sum = 0.f;
 #pragma unroll
         for (int k = 0; k < KX / 16; ++k)
@@ -283,11 +287,11 @@ __device__ __forceinline__ void bwd_walk(const BwdArgs &a, char *smem, int tid, 
         const int64_t t = start(n) + lane;
         return lane < C && t < tend ? load_g_raw(a.g, a.gtype, g0 + t * a.g_seq) : 0u;
     };
-    const bool dwave = !FOR_K && wave == kWaves - 1;
+    const bool dwave = FOR_K && wave == 2 * kWaves - 1;
     uint32_t gnext = 0;
     load(0);
     if (dwave) {
-        make_decays<C>(dec[0], decode_g(decay(0), a.gtype), lane);
+        make_decays<C>(dec[0], decode_g(decay(0), a.gtype), a.scale, lane);
         if (chunks > 1) gnext = decay(1);
     }
     int buf = 0;
@@ -305,43 +309,34 @@ __device__ __forceinline__ void bwd_walk(const BwdArgs &a, char *smem, int tid, 
         __syncthreads();
         fresh();
         const Decays<C> &d = dec[buf];
-        for (int t = wave; t < NT; t += 2 * kWaves) {
-            int x = 0, y = t;
-            while (y > x) y -= ++x;
-            const int o = y, m = x;   // row token tile o sees tile m >= o
-            const f32x4 p = score_tile<T, C, KD>(K, Q, o, m, lane), dp = score_tile<T, C, VD>(V, G, o, m, lane);
-            const f32x4 f = tile_decay<C, true>(d, o, m, a.scale, lane);
-            float s1[4], s2[4], w[4], cs = 0.f;
-            const int jj = 16 * o + lane % 16, ii = 16 * m + 4 * (lane / 16);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const bool sees = ii + r >= jj;
-                s1[r] = sees ? p[r] * f[r] : 0.f;
-                s2[r] = sees ? dp[r] * f[r] : 0.f;
-                w[r] = ii + r > jj ? p[r] * dp[r] * f[r] : 0.f;
-                cs += w[r];
+        auto tiles = [&](auto L) {
+            scores_bwd<T, C, KD, VD, decltype(L)>(d, Q, K, V, G, M1, M2, a.scale, a.a != nullptr, rowp, colp, lane);
+        };
+        if constexpr (C == 64) {
+            switch (wave) {
+                case 0: tiles(Tiles<0, 0, 0, 1>{}); break;
+                case 1: tiles(Tiles<0, 2, 0, 3>{}); break;
+                case 2: tiles(Tiles<1, 1, 1, 2>{}); break;
+                case 3: tiles(Tiles<3, 3>{}); break;
+                case 4: tiles(Tiles<1, 3>{}); break;
+                case 5: tiles(Tiles<2, 2>{}); break;
+                case 6: tiles(Tiles<2, 3>{});
             }
-            store_scores<C, PS>(M1, s1, o, m, lane);
-            store_scores<C, PS>(M2, s2, o, m, lane);
-            if (a.a) {
-                // Sums over the seen tokens j (for each i) and over the seeing tokens i (for each j) of the tile.
-                f32x4 rs;
-#pragma unroll
-                for (int r = 0; r < 4; ++r) rs[r] = group_sum<16>(w[r]);
-                cs += __shfl_xor(cs, 16);
-                cs += __shfl_xor(cs, 32);
-                if (lane % 16 == 0) *reinterpret_cast<f32x4 *>(&rowp[o * C + ii]) = rs;
-                if (lane < 16) colp[m * C + jj] = cs;
+        } else {
+            switch (wave) {
+                case 0: tiles(Tiles<0, 0>{}); break;
+                case 1: tiles(Tiles<0, 1>{}); break;
+                case kWaves: tiles(Tiles<1, 1>{});
             }
         }
         f32x4 O[CT][NC];
         fresh();
-        inter<T, C, KX, NC, FOR_K ? 3 : PS>(O, S, FOR_K ? V : K, d.out, 1.f, lane);
+        inter<T, C, KX, NC, FOR_K ? 3 : PS>(O, S, FOR_K ? V : K, d.out, lane);
         if constexpr (FOR_K) {
             if (a.a) dot_rows<T, C, NC, LDK>(O, K, col, part + (wave - kWaves) * C, lane);
         }
         if (dwave && more) {
-            make_decays<C>(dec[buf ^ 1], decode_g(gnext, a.gtype), lane);
+            make_decays<C>(dec[buf ^ 1], decode_g(gnext, a.gtype), a.scale, lane);
             if (n + 2 < chunks) gnext = decay(n + 2);
         }
         __syncthreads();
@@ -362,7 +357,7 @@ __device__ __forceinline__ void bwd_walk(const BwdArgs &a, char *smem, int tid, 
         bf16x8 v[C / 32][NC][PI];
         load_v<T, C, NC, LDC>(v, VT, col, lane);
         intra<T, C, NC, LDC, true>(O, v, FOR_K ? M2 : M1, VT, col, lane);
-        update<T, C, KX, NC>(S, v, FOR_K ? G : Q, d.in, a.scale, d.all, lane);
+        update<T, C, KX, NC>(S, v, FOR_K ? G : Q, d.in, d.all, lane);
         fresh();
         if constexpr (FOR_K) {
             store_out<T, C, NC, LDC, VEC, F32>(O, static_cast<char *>(a.dk_out) + (b * a.seqlen * a.heads + h) * a.dk * int64_t(F32 ? 4 : sizeof(T)),
@@ -381,7 +376,7 @@ __device__ __forceinline__ void bwd_walk(const BwdArgs &a, char *smem, int tid, 
 template <typename T, int KD, int VD, bool VEC, bool F32>
 __global__ void __launch_bounds__(2 * kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) la_bwd(const BwdArgs a) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid & 63;
     if (wave < kWaves) bwd_walk<T, KD, VD, VEC, F32, false>(a, smem, tid, wave, lane);
     else bwd_walk<T, KD, VD, VEC, F32, true>(a, smem, tid, wave, lane);
 }
@@ -396,7 +391,7 @@ static int launch_kernel(K kernel, int bytes, hipError_t set, int64_t grid, int 
 template <typename T, int KD, int NC, bool DOT, bool VEC, bool F32>
 static int launch_walk_t(const WalkArgs &a, hipStream_t s) {
     constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, PS = Cfg<T>::st;
-    constexpr int bytes = 2 * (2 * PI * C * KD + (DOT ? 2 : 1) * PI * C * 64 * NC + PS * C * kScoreRow) +
+    constexpr int bytes = 2 * (2 * PI * kTile<C, KD> + (DOT ? 2 : 1) * PI * kTile<C, 64 * NC> + PS * kTile<C, kScoreRow>) +
                           2 * int(sizeof(Decays<C>)) + (DOT ? 4 * kWaves * C : 0);
     static_assert(bytes <= 160 * 1024, "LDS");
     const auto kernel = la_walk<T, KD, NC, DOT, VEC, F32>;
@@ -417,7 +412,7 @@ static int launch_walk_k(const WalkArgs &a, hipStream_t s) {
 template <typename T, int KD, bool REV, bool VEC>
 static int launch_segments_t(const WalkArgs &a0, hipStream_t s) {
     constexpr int C = Cfg<T>::C, PI = Cfg<T>::in;
-    constexpr int bytes = 2 * (PI * C * KD + PI * C * 64) + int(sizeof(Decays<C>));
+    constexpr int bytes = 2 * (PI * kTile<C, KD> + PI * kTile<C, 64>) + int(sizeof(Decays<C>));
     static_assert(bytes <= 160 * 1024, "LDS");
     const auto kernel = la_segments<T, KD, REV, VEC>;
     static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
@@ -434,7 +429,7 @@ static int launch_segments_k(const WalkArgs &a, bool rev, hipStream_t s) {
 template <typename T, int KD, int VD, bool VEC, bool F32>
 static int launch_bwd_t(const BwdArgs &a, hipStream_t s) {
     constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, PS = Cfg<T>::st;
-    constexpr int bytes = 2 * (2 * PI * C * KD + 2 * PI * C * VD + 2 * PS * C * kScoreRow) +
+    constexpr int bytes = 2 * (2 * PI * kTile<C, KD> + 2 * PI * kTile<C, VD> + 2 * PS * kTile<C, kScoreRow>) +
                           2 * int(sizeof(Decays<C>)) + 4 * (2 * (C / 16) * C + kWaves * C);
     static_assert(bytes <= 160 * 1024, "LDS");
     const auto kernel = la_bwd<T, KD, VD, VEC, F32>;

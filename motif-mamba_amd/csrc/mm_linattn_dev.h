@@ -51,10 +51,16 @@ constexpr int kBlock = 256;      // tokens between two kept states (see the deca
 // line each once, so unit u of row r lies at u ^ swizzle(r): r's low two bits move a unit between the line's quarters,
 // its next two within one. Rows padded by 16 bytes instead cost 42 % of all LDS cycles in bank conflicts.
 __device__ __forceinline__ constexpr int swizzle(int row) { return (row & 3) << 2 | (row >> 2 & 3); }
+// 16 bytes stand between blocks of 16 rows: two blocks' reads at one lane's address are then no constant distance apart that one
+// instruction could span. (The compiler would join them, and move every half into its operand afterwards.)
+template <int D>
+__device__ __forceinline__ constexpr int block(int row) { return row * D + row / 16 * 8; }   // row: a multiple of 16
 template <int D>
 __device__ __forceinline__ constexpr int at(int row, int col) {
-    return row * D + (((col >> 2) ^ swizzle(row)) << 2) + (col & 3);
+    return row * D + (row >> 4) * 8 + (((col >> 2) ^ swizzle(row)) << 2) + (col & 3);
 }
+template <int C, int D>
+constexpr int kTile = C * D + C / 16 * 8;   // elements of a tile's plane
 constexpr int kScoreRow = 64;
 
 // A log decay's bits (converted when used, so that the load is waited for there).
@@ -112,24 +118,13 @@ __device__ __forceinline__ void split8(const float *x, bf16x8 *out) {
     }
 }
 
-// acc += A B over the pairs of planes whose ranks sum below MAXS (the others are below the last plane).
-template <int NA, int NB, int MAXS>
-__device__ __forceinline__ f32x4 mma(f32x4 acc, const bf16x8 *a, const bf16x8 *b) {
-#pragma unroll
-    for (int i = 0; i < NA; ++i)
-#pragma unroll
-        for (int j = 0; j < NB; ++j)
-            if (i + j < MAXS) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[j], acc, 0, 0, 0);
-    return acc;
-}
-
 __device__ __forceinline__ bf16x8 join(uint2 a, uint2 b) {
     return __builtin_bit_cast(bf16x8, u32x4{a.x, a.y, b.x, b.y});
 }
-// Operand whose row or column is tile row r0 + i and whose contraction runs over tile columns 32 k .. 32 k + 31.
+// Operand whose row or column is tile row r0 + i (r0 a multiple of 16) and whose contraction runs over tile columns 32 k .. 32 k + 31.
 template <int D>
 __device__ __forceinline__ bf16x8 frag_row(const u16 *tile, int r0, int k, int g, int i) {
-    const u16 *row = tile + (r0 + i) * D + (k / 2) * 64;
+    const u16 *row = tile + block<D>(r0) + i * D + (k / 2) * 64;
     const int u = (8 * (k % 2) + g) ^ swizzle(i);
     return join(*reinterpret_cast<const uint2 *>(row + 4 * u), *reinterpret_cast<const uint2 *>(row + 4 * (u ^ 4)));
 }
@@ -137,11 +132,11 @@ __device__ __forceinline__ bf16x8 frag_row(const u16 *tile, int r0, int k, int g
 // (r0 and col multiples of 16).
 template <int D>
 __device__ __forceinline__ bf16x8 frag_tr(const u16 *tile, int r0, int col, int g, int i) {
-    const int u = ((col / 16 % 4) ^ (i / 4)) << 2 | ((i % 4) ^ g);
-    const u16 *a = tile + (r0 + 4 * g + i / 4) * D + col / 64 * 64 + 4 * u;
+    const int u = ((col / 16 % 4) ^ (i >> 2)) << 2 | ((i & 3) ^ g);
+    const u16 *a = tile + block<D>(r0) + (4 * g + (i >> 2)) * D + col / 64 * 64 + 4 * u;
     typedef __attribute__((address_space(3))) s16x4 *lds_ptr;
     const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)a);
-    const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(a + 16 * D));
+    const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(a + block<D>(16)));
     return join(__builtin_bit_cast(uint2, x), __builtin_bit_cast(uint2, y));
 }
 
@@ -175,14 +170,14 @@ template <typename T> struct Rows {
 template <typename T, int C, int D, int NT, bool VEC>
 struct Stage {
     static constexpr int VE = 16 / sizeof(T), VR = D / VE, RS = NT / VR, N = (C + RS - 1) / RS;
-    static constexpr int PLANE = C * D;
+    static constexpr int PLANE = kTile<C, D>;
     static_assert(NT % VR == 0, "a row's threads");
     static constexpr bool kEven = C % RS == 0;
     uint4 r[N];
 
     __device__ __forceinline__ void load(const Rows<T> &s, int64_t t0, int rows, int tid) {
         const __amdgpu_buffer_rsrc_t buf = buffer(s.p + t0 * s.stride);
-        const int row = tid / VR, col = tid % VR * VE;
+        const int row = unsigned(tid) / VR, col = unsigned(tid) % VR * VE;
         const uint32_t stride = uint32_t(s.stride) * uint32_t(sizeof(T));
         const uint32_t off = uint32_t(row) * stride + uint32_t(col) * uint32_t(sizeof(T));
 #pragma unroll
@@ -190,7 +185,9 @@ struct Stage {
             const bool live = row + n * RS < (kEven ? rows : min(rows, C));
             const uint32_t at = off + uint32_t(n * RS) * stride;
             if constexpr (VEC) {
-                r[n] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(buf, live && col < s.d ? at : kNone, 0, 0));
+                uint32_t a = live && col < s.d ? at : kNone;
+                asm("" : "+v"(a));   // the offset is selected, the load not branched over
+                r[n] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(buf, a, 0, 0));
             } else {
                 uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
@@ -207,7 +204,7 @@ struct Stage {
     // Into the tile's planes. float16 and float32 are cut after 8 significant bits per plane, which is exact;
     // an infinity or NaN stands in the first plane alone.
     __device__ __forceinline__ void store(u16 *tile, int tid) const {
-        const int row0 = tid / VR, col = tid % VR * VE;
+        const int row0 = unsigned(tid) / VR, col = unsigned(tid) % VR * VE;
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             const int row = row0 + n * RS;
@@ -215,7 +212,7 @@ struct Stage {
             // Two units of 4 elements (one of float32), next to each other but in the order of the row's swizzle.
             const int sw = swizzle(row);
             const bool flip = VE == 8 && (sw & 1);
-            u16 *dst = tile + row * D + ((((col >> 2) ^ sw) & (VE == 8 ? ~1 : ~0)) << 2);
+            u16 *dst = tile + row * D + (row >> 4) * 8 + ((((col >> 2) ^ sw) & (VE == 8 ? ~1 : ~0)) << 2);
             const uint32_t w[4] = {r[n].x, r[n].y, r[n].z, r[n].w};
             if constexpr (std::is_same_v<T, bf16_t>) {
                 *reinterpret_cast<uint4 *>(dst) = flip ? make_uint4(w[2], w[3], w[0], w[1]) : r[n];
@@ -258,9 +255,9 @@ struct Stage {
 // forgotten state gives 0, never 0 times infinity), tiles on the diagonal exp(c_i - c_j) itself.
 template <int C>
 struct __attribute__((aligned(16))) Decays {
-    float in[C];           // exp(c_t): from the chunk's start, t's own decay included
+    float in[C];           // scale exp(c_t): from the chunk's start, t's own decay included
     float out[C];          // exp(c_end - c_t)
-    float from[C];         // exp(c_t - the sum before t's tile)
+    float from[C];         // scale exp(c_t - the sum before t's tile)
     float to[C];           // exp(the sum up to the end of t's tile - c_t)
     float hi[C], lo[C];    // c_t
     float mid[C / 16][C / 16];   // [I][J], J < I: from the end of tile J to the start of tile I
@@ -308,21 +305,21 @@ __device__ __forceinline__ double shfl_f64(double x, int lane) {
 
 // One wave; g: the lane's token's log decay, 0 behind the last token and in lanes past C.
 template <int C>
-__device__ __forceinline__ void make_decays(Decays<C> &d, float g, int lane) {
+__device__ __forceinline__ void make_decays(Decays<C> &d, float g, float scale, int lane) {
     const double c = prefix_f64(double(g));
     const double all = readlane_f64(c, C - 1);
-    const int tile = lane / 16;
+    const int tile = (lane >> 4);
     const double end = shfl_f64(c, 16 * tile + 15), before = shfl_f64(c, 16 * tile - 1 & 63);
     // lane 4 I + J of the first 16: from the end of tile J to the start of tile I (J < I)
-    const int I = lane / 4 % 4, J = lane % 4;
+    const int I = lane >> 2 & 3, J = lane & 3;
     const double mid = shfl_f64(c, 16 * I - 1 & 63) - shfl_f64(c, 16 * J + 15);
     const float hi = float(c);
     const float in = exp_f32(hi + float(c - double(hi))), out = exp_f32(float(all - c)), from = exp_f32(float(c - (tile ? before : 0.0))),
                 to = exp_f32(float(end - c)), m = exp_f32(float(mid));
     if (C == 64 || lane < C) {
-        d.in[lane] = in;
+        d.in[lane] = in * scale;
         d.out[lane] = out;
-        d.from[lane] = from;
+        d.from[lane] = from * scale;
         d.to[lane] = to;
         d.hi[lane] = hi;
         d.lo[lane] = float(c - double(hi));
@@ -333,44 +330,67 @@ __device__ __forceinline__ void make_decays(Decays<C> &d, float g, int lane) {
 
 // ---- a chunk's steps -----------------------------------------------------------------------------
 
-// Scores of one 16 x 16 tile: column i the row token 16 ot + i of X, rows 4g + r the tokens 16 nt + 4g + r of Y.
-template <typename T, int C, int KD>
-__device__ __forceinline__ f32x4 score_tile(const u16 *X, const u16 *Y, int ot, int nt, int lane) {
-    constexpr int PL = C * KD, P = Cfg<T>::in;
-    const int g = lane / 16, i = lane % 16;
-    bf16x8 a[KD / 32][P], b[KD / 32][P];
+// A list of 16 x 16 score tiles: row token tiles O and tiles n of the tokens they see.
+template <int... ON>
+struct Tiles {
+    static constexpr int N = sizeof...(ON) / 2;
+    static constexpr int on[2 * N] = {ON...};
+    static constexpr int O(int j) { return on[2 * j]; }
+    static constexpr int n(int j) { return on[2 * j + 1]; }
+};
+
+// Their scores, side by side: column i the row token 16 O + i of X, rows 4g + r the tokens 16 n + 4g + r of Y.
+template <typename T, int C, int KD, typename L>
+__device__ __forceinline__ void score_tiles(f32x4 (&s)[L::N], const u16 *X, const u16 *Y, int lane) {
+    constexpr int PL = kTile<C, KD>, P = Cfg<T>::in, N = L::N;
+    const int g = (lane >> 4), i = (lane & 15);
 #pragma unroll
-    for (int k = 0; k < KD / 32; ++k)
+    for (int j = 0; j < N; ++j) s[j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int p = 0; p < P; ++p) {
-            a[k][p] = frag_row<KD>(Y + p * PL, 16 * nt, k, g, i);
-            b[k][p] = frag_row<KD>(X + p * PL, 16 * ot, k, g, i);
-        }
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    for (int k = 0; k < KD / 32; k += 2) {
+        bf16x8 a[2][N][P], b[2][N][P];
 #pragma unroll
-    for (int k = 0; k < KD / 32; ++k) acc = mma<P, P, 3>(acc, a[k], b[k]);
-    return acc;
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int p = 0; p < P; ++p)
+#pragma unroll
+                for (int j = 0; j < N; ++j) {
+                    if (j > 0 && L::O(j) == L::O(j - 1)) b[h][j][p] = b[h][j - 1][p];
+                    else b[h][j][p] = frag_row<KD>(X + p * PL, 16 * L::O(j), k + h, g, i);
+                    a[h][j][p] = frag_row<KD>(Y + p * PL, 16 * L::n(j), k + h, g, i);
+                }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int p = 0; p < P; ++p)
+#pragma unroll
+                for (int q = 0; q < P; ++q)
+                    if (p + q < 3)
+#pragma unroll
+                        for (int j = 0; j < N; ++j) s[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[h][j][p], b[h][j][q], s[j], 0, 0, 0);
+    }
 }
 
-// The decay factors of that tile times `scale`, 0 where the token does not see the other. REV: row tokens
-// see later ones. f32x4: one factor per accumulator element.
-template <int C, bool REV>
-__device__ __forceinline__ f32x4 tile_decay(const Decays<C> &d, int ot, int nt, float scale, int lane) {
-    const int g = lane / 16, i = lane % 16;
-    const int o = 16 * ot + i, n = 16 * nt + 4 * g;
+// The decay factors of the tile (O, n) times `scale`, 0 where the token does not see the other. REV: row tokens see later
+// ones. One factor per accumulator element.
+template <int C, bool REV, int O, int n>
+__device__ __forceinline__ f32x4 tile_decay(const Decays<C> &d, float scale, int lane) {
+    const int g = (lane >> 4), i = (lane & 15);
+    constexpr int o = 16 * O, m = 16 * n;
     f32x4 f;
-    if (ot != nt) {
-        const float row = scale * (REV ? d.to[o] * d.mid[nt][ot] : d.from[o] * d.mid[ot][nt]);
-        const f32x4 col = *reinterpret_cast<const f32x4 *>(REV ? &d.from[n] : &d.to[n]);
+    if constexpr (O != n) {
+        const float row = REV ? d.to[o + i] * d.mid[n][O] : d.from[o + i] * d.mid[O][n];
+        const f32x4 col = *reinterpret_cast<const f32x4 *>(REV ? &d.from[m + 4 * g] : &d.to[m + 4 * g]);
 #pragma unroll
         for (int r = 0; r < 4; ++r) f[r] = row * col[r];
     } else {
-        const f32x4 hi = *reinterpret_cast<const f32x4 *>(&d.hi[n]), lo = *reinterpret_cast<const f32x4 *>(&d.lo[n]);
+        const f32x4 hi = *reinterpret_cast<const f32x4 *>(&d.hi[m + 4 * g]), lo = *reinterpret_cast<const f32x4 *>(&d.lo[m + 4 * g]);
+        const float h = d.hi[o + i], l = d.lo[o + i];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const float x = (d.hi[o] - hi[r]) + (d.lo[o] - lo[r]);
-            const bool sees = REV ? n + r >= o : n + r <= o;
-            f[r] = sees ? exp_f32(REV ? -x : x) * scale : 0.f;
+            float x = (h - hi[r]) + (l - lo[r]);
+            if (REV) x = -x;
+            f[r] = exp_f32((REV ? 4 * g + r >= i : 4 * g + r <= i) ? x : -1e30f) * scale;
         }
     }
     return f;
@@ -379,8 +399,8 @@ __device__ __forceinline__ f32x4 tile_decay(const Decays<C> &d, int ot, int nt, 
 // Four consecutive scores of row token 16 ot + i into the score tile's planes ([row token][other token]).
 template <int C, int P>
 __device__ __forceinline__ void store_scores(u16 *M, const float *x, int ot, int nt, int lane) {
-    constexpr int PL = C * kScoreRow;
-    u16 *dst = M + 16 * ot * kScoreRow + at<kScoreRow>(lane % 16, 16 * nt + 4 * (lane / 16));
+    constexpr int PL = kTile<C, kScoreRow>;
+    u16 *dst = M + block<kScoreRow>(16 * ot) + at<kScoreRow>((lane & 15), 16 * nt + 4 * ((lane >> 4)));
     float r[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
     for (int p = 0; p < P; ++p) {
@@ -393,11 +413,62 @@ __device__ __forceinline__ void store_scores(u16 *M, const float *x, int ot, int
     }
 }
 
+// The forward walk's decayed, masked scores of the tiles L into M.
+template <typename T, int C, int KD, typename L>
+__device__ __forceinline__ void scores(const Decays<C> &d, const u16 *X, const u16 *Y, u16 *M, float scale, int lane) {
+    f32x4 s[L::N];
+    score_tiles<T, C, KD, L>(s, X, Y, lane);
+    static_for<0, L::N>([&](auto Nc) {
+        constexpr int j = decltype(Nc)::value, O = L::O(j), n = L::n(j);
+        const f32x4 f = tile_decay<C, false, O, n>(d, scale, lane);
+        float x[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r] = n == O && 4 * ((lane >> 4)) + r > (lane & 15) ? 0.f : s[j][r] * f[r];
+        store_scores<C, Cfg<T>::st>(M, x, O, n, lane);
+    });
+}
+
+// The backward walk's, of both products (K Q^T into M1, V dO^T into M2, row token tile O), and with `sums` the tiles' sums of
+// w = both scores times the decay, the diagonal left out: over the seen tokens for each seeing one (rowp) and over the seeing
+// tokens for each seen one (colp).
+template <typename T, int C, int KD, int VD, typename L>
+__device__ __forceinline__ void scores_bwd(const Decays<C> &d, const u16 *Q, const u16 *K, const u16 *V, const u16 *G, u16 *M1, u16 *M2, float scale,
+                                           bool sums, float *rowp, float *colp, int lane) {
+    f32x4 p[L::N], dp[L::N];
+    score_tiles<T, C, KD, L>(p, K, Q, lane);
+    score_tiles<T, C, VD, L>(dp, V, G, lane);
+    static_for<0, L::N>([&](auto Nc) {
+        constexpr int j = decltype(Nc)::value, O = L::O(j), m = L::n(j);
+        const f32x4 f = tile_decay<C, true, O, m>(d, scale, lane);
+        const int i = (lane & 15), ii = 4 * ((lane >> 4));
+        float s1[4], s2[4], w[4], cs = 0.f;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const bool sees = m != O || ii + r >= i;
+            s1[r] = sees ? p[j][r] * f[r] : 0.f;
+            s2[r] = sees ? dp[j][r] * f[r] : 0.f;
+            w[r] = m != O || ii + r > i ? p[j][r] * s2[r] : 0.f;
+            cs += w[r];
+        }
+        store_scores<C, Cfg<T>::st>(M1, s1, O, m, lane);
+        store_scores<C, Cfg<T>::st>(M2, s2, O, m, lane);
+        if (sums) {
+            f32x4 rs;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) rs[r] = group_sum<16>(w[r]);
+            cs += __shfl_xor(cs, 16);
+            cs += __shfl_xor(cs, 32);
+            if (i == 0) *reinterpret_cast<f32x4 *>(&rowp[O * C + 16 * m + ii]) = rs;
+            if (lane < 16) colp[m * C + 16 * O + i] = cs;
+        }
+    });
+}
+
 // The tiles on the masked side of the diagonal that share a 32-wide contraction with a diagonal tile are 0
 // (written once; the chunks write the other tiles only).
 template <int C, int P>
 __device__ __forceinline__ void zero_masked_scores(u16 *M, bool rev, int tid, int nt) {
-    constexpr int PL = C * kScoreRow;
+    constexpr int PL = kTile<C, kScoreRow>;
     for (int x = tid; x < C / 32 * 16 * 16 * P; x += nt) {
         const int p = x / (C / 32 * 256), y = x % (C / 32 * 256), pair = y / 256, r = y % 256 / 16, c = y % 16;
         const int row = 32 * pair + (rev ? 16 : 0) + r, col = 32 * pair + (rev ? 0 : 16) + c;
@@ -409,9 +480,9 @@ __device__ __forceinline__ void zero_masked_scores(u16 *M, bool rev, int tid, in
 // PS: the state's planes.
 template <typename T, int C, int KD, int NC, int PS>
 __device__ __forceinline__ void inter(f32x4 (&O)[C / 16][NC], const f32x4 (&S)[KD / 16][NC], const u16 *X, const float *row,
-                                      float scale, int lane) {
-    constexpr int PL = C * KD, PI = Cfg<T>::in;
-    const int g = lane / 16, i = lane % 16;
+                                      int lane) {
+    constexpr int PL = kTile<C, KD>, PI = Cfg<T>::in;
+    const int g = (lane >> 4), i = (lane & 15);
 #pragma unroll
     for (int t = 0; t < C / 16; ++t)
 #pragma unroll
@@ -457,16 +528,16 @@ __device__ __forceinline__ void inter(f32x4 (&O)[C / 16][NC], const f32x4 (&S)[K
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int c = 0; c < NC; ++c) O[t][c][r] *= f[r] * scale;
+            for (int c = 0; c < NC; ++c) O[t][c][r] *= f[r];
     }
 }
 
 // S = all S + Y^T diag(w) V for the wave's columns (V's operands in v).
 template <typename T, int C, int KD, int NC>
 __device__ __forceinline__ void update(f32x4 (&S)[KD / 16][NC], const bf16x8 (&v)[C / 32][NC][Cfg<T>::in], const u16 *Y,
-                                       const float *w, float scale, float all, int lane) {
-    constexpr int PL = C * KD, PI = Cfg<T>::in, PU = Cfg<T>::up;
-    const int g = lane / 16, i = lane % 16;
+                                       const float *w, float all, int lane) {
+    constexpr int PL = kTile<C, KD>, PI = Cfg<T>::in, PU = Cfg<T>::up;
+    const int g = (lane >> 4), i = (lane & 15);
 #pragma unroll
     for (int k = 0; k < KD / 16; ++k)
 #pragma unroll
@@ -490,8 +561,8 @@ __device__ __forceinline__ void update(f32x4 (&S)[KD / 16][NC], const bf16x8 (&v
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                x[e] *= w0[e] * scale;
-                x[4 + e] *= w1[e] * scale;
+                x[e] *= w0[e];
+                x[4 + e] *= w1[e];
             }
             split8<PU>(x, u[c]);
         }
@@ -526,14 +597,14 @@ __device__ __forceinline__ void update(f32x4 (&S)[KD / 16][NC], const bf16x8 (&v
 
 template <typename T, int C, int NC, int LDV>
 __device__ __forceinline__ void load_v(bf16x8 (&v)[C / 32][NC][Cfg<T>::in], const u16 *V, int col, int lane) {
-    constexpr int PL = C * LDV;
+    constexpr int PL = kTile<C, LDV>;
 #pragma unroll
     for (int j = 0; j < C / 32; ++j)
 #pragma unroll
         for (int c = 0; c < NC; ++c)
 #pragma unroll
             for (int p = 0; p < Cfg<T>::in; ++p)
-                v[j][c][p] = frag_tr<LDV>(V + p * PL, 32 * j, col + 16 * c, lane / 16, lane % 16);
+                v[j][c][p] = frag_tr<LDV>(V + p * PL, 32 * j, col + 16 * c, (lane >> 4), (lane & 15));
 }
 
 // O += M V, M the masked scores. A masked score is 0, and 0 times an infinity or NaN of a token that the row
@@ -541,8 +612,8 @@ __device__ __forceinline__ void load_v(bf16x8 (&v)[C / 32][NC][Cfg<T>::in], cons
 template <typename T, int C, int NC, int LDV, bool REV>
 __device__ __forceinline__ void intra(f32x4 (&O)[C / 16][NC], const bf16x8 (&v0)[C / 32][NC][Cfg<T>::in], const u16 *M,
                                       const u16 *V, int col, int lane) {
-    constexpr int PL = C * kScoreRow, PI = Cfg<T>::in, PS = Cfg<T>::st;
-    const int g = lane / 16, i = lane % 16;
+    constexpr int PL = kTile<C, kScoreRow>, PI = Cfg<T>::in, PS = Cfg<T>::st;
+    const int g = (lane >> 4), i = (lane & 15);
     typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
     u16x2 most = {0, 0};
 #pragma unroll
@@ -624,7 +695,7 @@ struct Mat {
 };
 template <int KD, int NC>
 __device__ __forceinline__ void load_state(f32x4 (&S)[KD / 16][NC], const Mat &m, int rows, int cols, int col, int lane) {
-    const int g = lane / 16, i = lane % 16;
+    const int g = (lane >> 4), i = (lane & 15);
     rows = afresh(rows);
     cols = afresh(cols);
 #pragma unroll
@@ -639,7 +710,7 @@ __device__ __forceinline__ void load_state(f32x4 (&S)[KD / 16][NC], const Mat &m
 }
 template <int KD, int NC>
 __device__ __forceinline__ void store_state(const f32x4 (&S)[KD / 16][NC], const Mat &m, int rows, int cols, int col, int lane) {
-    const int g = lane / 16, i = lane % 16;
+    const int g = (lane >> 4), i = (lane & 15);
     rows = afresh(rows);
     cols = afresh(cols);
 #pragma unroll
@@ -658,7 +729,7 @@ __device__ __forceinline__ void store_state(const f32x4 (&S)[KD / 16][NC], const
 template <typename T, int C, int NC, int LDV, bool VEC, bool F32>
 __device__ __forceinline__ void store_out(const f32x4 (&O)[C / 16][NC], void *out, int64_t stride, int64_t t0, int rows, int cols, int col0,
                                           u16 *tile, int col, int lane) {
-    const int g = lane / 16, i = lane % 16;
+    const int g = (lane >> 4), i = (lane & 15);
     constexpr uint32_t ES = F32 ? 4 : sizeof(T);
     const __amdgpu_buffer_rsrc_t buf = buffer(static_cast<char *>(out) + t0 * stride * ES);
     const uint32_t step = uint32_t(stride) * ES;
@@ -670,16 +741,16 @@ __device__ __forceinline__ void store_out(const f32x4 (&O)[C / 16][NC], void *ou
 #pragma unroll
                 for (int r = 0; r < 4; r += 2) {
                     const uint32_t w = std::is_same_v<T, bf16_t> ? pack_bf16x2(O[t][c][r], O[t][c][r + 1]) : pack_f16x2(O[t][c][r], O[t][c][r + 1]);
-                    tile[16 * t * LDV + at<LDV>(4 * g + r, col + 16 * c + i)] = u16(w);
-                    tile[16 * t * LDV + at<LDV>(4 * g + r + 1, col + 16 * c + i)] = u16(w >> 16);
+                    tile[block<LDV>(16 * t) + at<LDV>(4 * g + r, col + 16 * c + i)] = u16(w);
+                    tile[block<LDV>(16 * t) + at<LDV>(4 * g + r + 1, col + 16 * c + i)] = u16(w >> 16);
                 }
         constexpr int PR = 2 * NC;   // pieces of a row
 #pragma unroll
         for (int n = 0; n < C * PR / 64; ++n) {
-            const int row = n * (64 / PR) + lane / PR, c = lane % PR * 8;
-            const u16 *src = tile + n * (64 / PR) * LDV;   // whole tiles of 16 rows down
-            const uint2 w0 = *reinterpret_cast<const uint2 *>(src + at<LDV>(lane / PR, col + c)),
-                        w1 = *reinterpret_cast<const uint2 *>(src + at<LDV>(lane / PR, col + c + 4));
+            const int row = n * (64 / PR) + int(unsigned(lane) / PR), c = int(unsigned(lane) % PR) * 8;
+            const u16 *src = tile + block<LDV>(n * (64 / PR));   // whole tiles of 16 rows down
+            const uint2 w0 = *reinterpret_cast<const uint2 *>(src + at<LDV>(int(unsigned(lane) / PR), col + c)),
+                        w1 = *reinterpret_cast<const uint2 *>(src + at<LDV>(int(unsigned(lane) / PR), col + c + 4));
             const u32x4 w = {w0.x, w0.y, w1.x, w1.y};
             const bool live = row < rows && col0 + col + c < cols;
             __builtin_amdgcn_raw_buffer_store_b128(w, buf, live ? uint32_t(row) * step + uint32_t(col0 + col + c) * 2 : kNone, 0, 0);
@@ -705,8 +776,8 @@ __device__ __forceinline__ void store_out(const f32x4 (&O)[C / 16][NC], void *ou
 // dot[n] = sum over the wave's columns of O[n][x] Z[n][x], into part[n] (lanes i == 0 write).
 template <typename T, int C, int NC, int LDZ>
 __device__ __forceinline__ void dot_rows(const f32x4 (&O)[C / 16][NC], const u16 *Z, int col, float *part, int lane) {
-    constexpr int PL = C * LDZ, PI = Cfg<T>::in;
-    const int g = lane / 16, i = lane % 16;
+    constexpr int PL = kTile<C, LDZ>, PI = Cfg<T>::in;
+    const int g = (lane >> 4), i = (lane & 15);
 #pragma unroll
     for (int t = 0; t < C / 16; ++t) {
         f32x4 s;
@@ -715,7 +786,7 @@ __device__ __forceinline__ void dot_rows(const f32x4 (&O)[C / 16][NC], const u16
             float x = 0.f;
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
-                const u16 *z = Z + 16 * t * LDZ + at<LDZ>(4 * g + r, col + 16 * c + i);
+                const u16 *z = Z + block<LDZ>(16 * t) + at<LDZ>(4 * g + r, col + 16 * c + i);
                 float y = 0.f;
 #pragma unroll
                 for (int p = PI - 1; p >= 0; --p) y += __uint_as_float(uint32_t(z[p * PL]) << 16);
