@@ -37,18 +37,30 @@ __device__ __forceinline__ float sigmoid(float x) {
     return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-x * kLog2e));
 }
 
-// VE consecutive elements (16 bytes, or 1).
-template <typename T, int VE>
-__device__ __forceinline__ void load(const T *p, float *x) {
-    if constexpr (VE == 1) {
-        x[0] = to_f32(p[0]);
-    } else {
-        const uint4 v = *reinterpret_cast<const uint4 *>(p);
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+// NV pieces of VE consecutive elements (16 bytes, or 1) on their way from memory, one every `lanes` pieces.
+template <typename T, int VE, int NV>
+struct Raw {
+    typedef typename std::conditional<VE == 1, T, uint4>::type V;
+    V v[NV];
+
+    __device__ __forceinline__ void load(const T *p, int lane, int lanes, int size, bool live) {
 #pragma unroll
-        for (int e = 0; e < VE; ++e) x[e] = elem_f32<T>(sizeof(T) == 4 ? w[e] : (w[e / 2] >> (16 * (e % 2))) & 0xffffu);
+        for (int n = 0; n < NV; ++n) {
+            const int c = (n * lanes + lane) * VE;
+            v[n] = V{};
+            if (live && c < size) v[n] = *reinterpret_cast<const V *>(p + c);
+        }
     }
-}
+    __device__ __forceinline__ void get(int n, float *x) const {
+        if constexpr (VE == 1) {
+            x[0] = to_f32(v[n]);
+        } else {
+            const uint32_t w[4] = {v[n].x, v[n].y, v[n].z, v[n].w};
+#pragma unroll
+            for (int e = 0; e < VE; ++e) x[e] = elem_f32<T>(sizeof(T) == 4 ? w[e] : (w[e / 2] >> (16 * (e % 2))) & 0xffffu);
+        }
+    }
+};
 template <typename T, int VE>
 __device__ __forceinline__ void store(T *p, const float *x) {
     if constexpr (VE == 1) {
@@ -64,26 +76,31 @@ __device__ __forceinline__ void store(T *p, const float *x) {
     }
 }
 
-// Sums of N values over a group's `lanes` threads (a power of two). Past one wave through `buf`, the same
-// order in every thread; `buf` alternates between two halves so that one barrier per sum is enough.
+// Sums of N values over a group's `lanes` threads (a power of two up to 64, then whole waves), by lane swaps in a wave and
+// through `buf` past it, in the same order in every thread; `buf` alternates between two halves so that one barrier per sum
+// is enough.
 template <int N>
 __device__ __forceinline__ void group_sums(float (&x)[N], int lanes, float *buf, int &half) {
-    for (int d = 1; d < lanes && d < 64; d *= 2)
 #pragma unroll
-        for (int i = 0; i < N; ++i) x[i] += __shfl_xor(x[i], d);
+    for (int i = 0; i < N; ++i) {
+        if (lanes > 1) x[i] = dpp_add<0xB1>(x[i]);    // quad_perm [1,0,3,2]
+        if (lanes > 2) x[i] = dpp_add<0x4E>(x[i]);    // quad_perm [2,3,0,1]
+        if (lanes > 4) x[i] = dpp_add<0x141>(x[i]);   // row_half_mirror: the other quad of 8 lanes
+        if (lanes > 8) x[i] = dpp_add<0x140>(x[i]);   // row_mirror: the other half of 16 lanes
+        if (lanes > 16) x[i] += __shfl_xor(x[i], 16);
+        if (lanes > 32) x[i] += __shfl_xor(x[i], 32);
+    }
     if (lanes <= 64) return;
-    const int waves = lanes / 64, wave = threadIdx.x / 64;
     float *b = buf + half * 32;
     half ^= 1;
     if (threadIdx.x % 64 == 0)
 #pragma unroll
-        for (int i = 0; i < N; ++i) b[wave * N + i] = x[i];
+        for (int i = 0; i < N; ++i) b[threadIdx.x / 64 * N + i] = x[i];
     __syncthreads();
-    const int w0 = wave / waves * waves;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         float s = 0.f;
-        for (int w = 0; w < waves; ++w) s += b[(w0 + w) * N + i];
+        for (int w = 0; w < lanes / 64; ++w) s += b[w * N + i];
         x[i] = s;
     }
 }
@@ -102,18 +119,11 @@ struct Group {
     __device__ __forceinline__ float h(int v, int e, bool before) const {
         return before ? x[v][e] * (z[v][e] * s[v][e]) : x[v][e];
     }
-    __device__ __forceinline__ void read(const mm_group_norm_params &p, int64_t row, int64_t c0, int lane, int lanes, int size, bool live) {
-        const T *xr = reinterpret_cast<const T *>(p.x) + row * p.x_row_stride + c0;
-        const T *zr = reinterpret_cast<const T *>(p.z) + (p.z ? row * p.z_row_stride + c0 : 0);
+    __device__ __forceinline__ void take(const Raw<T, VE, NV> &rx, const Raw<T, VE, NV> &rz) {
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            const int c = (v * lanes + lane) * VE;
-#pragma unroll
-            for (int e = 0; e < VE; ++e) x[v][e] = z[v][e] = 0.f;
-            if (live && c < size) {
-                load<T, VE>(xr + c, x[v]);
-                if (p.z) load<T, VE>(zr + c, z[v]);
-            }
+            rx.get(v, x[v]);
+            rz.get(v, z[v]);
         }
     }
     __device__ __forceinline__ void stats(const mm_group_norm_params &p, int lane, int lanes, int size, float *buf, int &half) {
@@ -170,9 +180,17 @@ __global__ void __launch_bounds__(NT) gn_fwd(const mm_group_norm_params p, const
     read_weights<VE, NV>(p, w, b, c0, lane, k.lanes, size, live);
     int half = 0;
     const int64_t r0 = int64_t(blockIdx.y) * k.per, r1 = min(p.rows, r0 + k.per);
+    // The next row is on its way while a row is worked on.
+    Raw<T, VE, NV> rx, rz = {};
+    auto read = [&](int64_t row) {
+        rx.load(reinterpret_cast<const T *>(p.x) + row * p.x_row_stride + c0, lane, k.lanes, size, live);
+        if (p.z) rz.load(reinterpret_cast<const T *>(p.z) + row * p.z_row_stride + c0, lane, k.lanes, size, live);
+    };
+    if (r0 < r1) read(r0);
     for (int64_t row = r0; row < r1; ++row) {
         Group<T, VE, NV> g;
-        g.read(p, row, c0, lane, k.lanes, size, live);
+        g.take(rx, rz);
+        if (row + 1 < r1) read(row + 1);
         g.stats(p, lane, k.lanes, size, buf, half);
         T *out = reinterpret_cast<T *>(p.out) + row * p.channels + c0;
 #pragma unroll
@@ -206,18 +224,20 @@ __global__ void __launch_bounds__(NT) gn_bwd(const mm_group_norm_params p, const
         for (int e = 0; e < VE; ++e) dw[v][e] = db[v][e] = 0.f;
     int half = 0;
     const int64_t r0 = int64_t(blockIdx.y) * k.per, r1 = min(p.rows, r0 + k.per);
+    Raw<T, VE, NV> rx, rd, rz = {};
+    auto read = [&](int64_t row) {
+        rx.load(reinterpret_cast<const T *>(p.x) + row * p.x_row_stride + c0, lane, k.lanes, size, live);
+        rd.load(reinterpret_cast<const T *>(p.dout) + row * p.dout_row_stride + c0, lane, k.lanes, size, live);
+        if (p.z) rz.load(reinterpret_cast<const T *>(p.z) + row * p.z_row_stride + c0, lane, k.lanes, size, live);
+    };
+    if (r0 < r1) read(r0);
     for (int64_t row = r0; row < r1; ++row) {
         Group<T, VE, NV> g;
         float d[NV][VE];
-        g.read(p, row, c0, lane, k.lanes, size, live);
-        const T *dr = reinterpret_cast<const T *>(p.dout) + row * p.dout_row_stride + c0;
+        g.take(rx, rz);
 #pragma unroll
-        for (int v = 0; v < NV; ++v) {
-            const int c = (v * k.lanes + lane) * VE;
-#pragma unroll
-            for (int e = 0; e < VE; ++e) d[v][e] = 0.f;
-            if (live && c < size) load<T, VE>(dr + c, d[v]);
-        }
+        for (int v = 0; v < NV; ++v) rd.get(v, d[v]);
+        if (row + 1 < r1) read(row + 1);
         g.stats(p, lane, k.lanes, size, buf, half);
         float sum[2] = {0.f, 0.f};
 #pragma unroll
@@ -284,27 +304,32 @@ __global__ void __launch_bounds__(NT) gn_bwd(const mm_group_norm_params p, const
         }
 }
 
-// dweight and dbias: the blocks' partial rows summed in order, 32 columns and 8 runs of rows per block.
-__global__ void __launch_bounds__(256) gn_sum(const mm_group_norm_params p, const float *part, int64_t n) {
-    __shared__ float buf[2][8][32];
+// dweight and dbias: the blocks' partial rows summed in order, 32 columns and 32 runs of rows per block.
+__global__ void __launch_bounds__(1024) gn_sum(const mm_group_norm_params p, const float *part, int64_t n) {
+    __shared__ float buf[2][32][33];
     const int x = threadIdx.x % 32, run = threadIdx.x / 32;
     const int64_t c = int64_t(blockIdx.x) * 32 + x;
     float w = 0.f, b = 0.f;
     if (c < p.channels)
-        for (int64_t r = run; r < n; r += 8) {
+#pragma unroll 4
+        for (int64_t r = run; r < n; r += 32) {
             w += part[2 * r * p.channels + c];
             b += part[(2 * r + 1) * p.channels + c];
         }
     buf[0][run][x] = w;
     buf[1][run][x] = b;
     __syncthreads();
-    if (run == 0 && c < p.channels) {
-        for (int r = 1; r < 8; ++r) {
-            w += buf[0][r][x];
-            b += buf[1][r][x];
-        }
-        if (p.dweight) store_w(p.dweight, p.wtype, c, w);
-        if (p.dbias) store_w(p.dbias, p.wtype, c, b);
+    // The runs' sums of a column by 32 lanes of one wave.
+    w = buf[0][x][run];
+    b = buf[1][x][run];
+    for (int d = 16; d > 0; d /= 2) {
+        w += __shfl_xor(w, d);
+        b += __shfl_xor(b, d);
+    }
+    const int64_t out = int64_t(blockIdx.x) * 32 + run;
+    if (x == 0 && out < p.channels) {
+        if (p.dweight) store_w(p.dweight, p.wtype, out, w);
+        if (p.dbias) store_w(p.dbias, p.wtype, out, b);
     }
 }
 
@@ -323,18 +348,20 @@ static bool vectors(const mm_group_norm_params &p, bool bwd) {
 static Plan plan(const mm_group_norm_params &p, bool bwd) {
     Plan k = {};
     const int64_t size = p.channels / p.n_groups, ve = vectors(p, bwd) ? 16 / elem(p.itype) : 1, vecs = (size + ve - 1) / ve;
-    k.lanes = 1;
-    while (k.lanes < vecs && k.lanes < 64) k.lanes *= 2;
-    k.nv = int((vecs + k.lanes - 1) / k.lanes);
-    const int most = ve == 1 ? 4 : 2;          // vectors per thread before a group takes more than a wave
-    while (k.nv > most && k.lanes < 1024) {
-        k.lanes *= k.lanes == 64 ? 4 : 2;
-        k.nv = int((vecs + k.lanes - 1) / k.lanes);
+    // A wave or less per group while that takes at most `most` pieces per thread, else as many waves as that takes, up to 16.
+    const int most = ve == 1 ? 4 : 2, all = ve == 1 ? 16 : 4;
+    if (vecs <= 64 * most) {
+        k.lanes = 1;
+        while (k.lanes < vecs && k.lanes < 64) k.lanes *= 2;
+    } else {
+        const int per = vecs <= 1024 * most ? most : all;
+        k.lanes = int((vecs + 64 * per - 1) / (64 * per)) * 64;
     }
-    k.threads = std::max(256, k.lanes);
+    k.nv = int((vecs + k.lanes - 1) / k.lanes);
+    k.threads = k.lanes > 64 ? k.lanes : 256;
     k.col_blocks = (p.n_groups + k.threads / k.lanes - 1) / (k.threads / k.lanes);
     // Blocks for about 8 waves per SIMD and two rounds; the backward writes a partial row per block, so fewer.
-    const int64_t want = std::max<int64_t>(1, device_simds() * 16 / (k.threads / 64) / k.col_blocks / (bwd ? 4 : 1));
+    const int64_t want = std::max<int64_t>(1, device_simds() * 16 / ((k.threads + 63) / 64) / k.col_blocks / (bwd ? 4 : 1));
     k.per = std::max<int64_t>(1, (p.rows + std::min<int64_t>(want, 65535) - 1) / std::min<int64_t>(want, 65535));
     k.row_blocks = (p.rows + k.per - 1) / k.per;
     return k;
@@ -352,13 +379,15 @@ static int launch_nt(const mm_group_norm_params &p, const Plan &k, bool bwd, hip
     hipLaunchKernelGGL((gn_bwd<T, VE, NV, NT>), grid, block, 0, s, p, k, part);
     if (const int rc = launch_status("gn_bwd")) return rc;
     if (!part) return MM_OK;
-    hipLaunchKernelGGL(gn_sum, dim3(unsigned((p.channels + 31) / 32)), dim3(256), 0, s, p, part, k.row_blocks);
+    hipLaunchKernelGGL(gn_sum, dim3(unsigned((p.channels + 31) / 32)), dim3(1024), 0, s, p, part, k.row_blocks);
     return launch_status("gn_sum");
 }
 
 template <typename T, int VE, int NV>
 static int launch(const mm_group_norm_params &p, const Plan &k, bool bwd, hipStream_t s) {
-    return k.threads == 256 ? launch_nt<T, VE, NV, 256>(p, k, bwd, s) : launch_nt<T, VE, NV, 1024>(p, k, bwd, s);
+    if (k.threads <= 256) return launch_nt<T, VE, NV, 256>(p, k, bwd, s);
+    if (k.threads <= 512) return launch_nt<T, VE, NV, 512>(p, k, bwd, s);
+    return launch_nt<T, VE, NV, 1024>(p, k, bwd, s);
 }
 
 template <typename T>
@@ -370,6 +399,7 @@ static int run(const mm_group_norm_params &p, bool bwd, hipStream_t s) {
         if (k.nv == 2) return launch<T, V, 2>(p, k, bwd, s);
         return launch<T, V, 4>(p, k, bwd, s);
     }
+    if (k.nv <= 2) return launch<T, 1, 2>(p, k, bwd, s);
     if (k.nv <= 4) return launch<T, 1, 4>(p, k, bwd, s);
     return launch<T, 1, 16>(p, k, bwd, s);
 }
@@ -423,7 +453,7 @@ extern "C" int mm_group_norm_bwd(const mm_group_norm_params *params, void *strea
     if (p.channels == 0) return MM_OK;
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     if (p.rows == 0) {   // empty sums
-        if (p.dweight || p.dbias) hipLaunchKernelGGL(gn::gn_sum, dim3(unsigned((p.channels + 31) / 32)), dim3(256), 0, s, p, nullptr, int64_t(0));
+        if (p.dweight || p.dbias) hipLaunchKernelGGL(gn::gn_sum, dim3(unsigned((p.channels + 31) / 32)), dim3(1024), 0, s, p, nullptr, int64_t(0));
         return p.dweight || p.dbias ? launch_status("gn_sum") : MM_OK;
     }
     if (!p.x || !p.dout || !p.dx || (p.z && !p.dz)) return set_error(MM_ERR_INVALID_ARGUMENT, "mm_group_norm_bwd: x, dout, dx and, with z, dz are required");

@@ -21,16 +21,22 @@ def _flat(t):
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
+def _forward(x, n_groups, weight, bias, z, eps, is_rms_norm, gate):
+    xf, zf = _flat(x), None if z is None else _flat(z)
+    weight = None if weight is None else weight.contiguous()
+    bias = None if bias is None else bias.contiguous()
+    out = ext().group_norm_fwd(xf, n_groups, weight, bias, zf, eps, is_rms_norm, gate)
+    return xf, weight, bias, zf, out.view(x.shape)
+
+
 class GroupNormFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, n_groups, weight, bias, z, eps, is_rms_norm, gate):
-        xf, zf = _flat(x), None if z is None else _flat(z)
-        weight = None if weight is None else weight.contiguous()
-        bias = None if bias is None else bias.contiguous()
+        xf, weight, bias, zf, out = _forward(x, n_groups, weight, bias, z, eps, is_rms_norm, gate)
         ctx.args = (n_groups, eps, is_rms_norm, gate)
         ctx.save_for_backward(xf, weight, bias, zf)
-        return ext().group_norm_fwd(xf, n_groups, weight, bias, zf, eps, is_rms_norm, gate).view(x.shape)
+        return out
 
     @staticmethod
     def backward(ctx, dout):
@@ -54,4 +60,7 @@ def group_norm_fn(x, n_groups, weight=None, bias=None, z=None, eps=1e-5, activat
     if x.dim() < 1 or (z is not None and z.shape != x.shape):
         raise ValueError("x must be (..., channels), and z must have its shape")
     gate = (_AFTER if norm_before_gate else _BEFORE) if z is not None else _ACT if activation else _NONE
-    return GroupNormFn.apply(x, int(n_groups), weight, bias, z, float(eps), bool(is_rms_norm), gate)
+    args = (x, int(n_groups), weight, bias, z, float(eps), bool(is_rms_norm), gate)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, z)):
+        return GroupNormFn.apply(*args)
+    return _forward(*args)[4]

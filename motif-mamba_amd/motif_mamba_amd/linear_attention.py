@@ -41,17 +41,22 @@ def _scale(scale, q):
     return q.shape[-1] ** -0.5 if scale is None else float(scale)
 
 
+def _forward(q, k, v, log_decay, scale, initial_state, return_last_state):
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    g, per_head = _spread(log_decay, v.shape[:2], v)
+    res = ext().linattn_fwd(q, k, v, g, scale, initial_state, return_last_state)
+    return q, k, v, per_head, tuple(res) if return_last_state else res[0]
+
+
 class LinearAttentionFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, log_decay, scale, initial_state, return_last_state):
-        q, k, v = _rows(q), _rows(k), _rows(v)
-        g, ctx.per_head = _spread(log_decay, v.shape[:2], v)
-        res = ext().linattn_fwd(q, k, v, g, scale, initial_state, return_last_state)
+        q, k, v, ctx.per_head, out = _forward(q, k, v, log_decay, scale, initial_state, return_last_state)
         ctx.scale = scale
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(q, k, v, log_decay, initial_state)
-        return tuple(res) if return_last_state else res[0]
+        return out
 
     @staticmethod
     def backward(ctx, dout, dlast=None):
@@ -74,7 +79,10 @@ def linear_attention_fn(q, k, v, log_decay, scale=None, initial_state=None, retu
     (batch, nheads, dk, dv) float32, the state linear_attention_update continues from]."""
     if v.dim() != 4:
         raise ValueError("v must have shape (batch, seqlen, nheads, dv)")
-    return LinearAttentionFn.apply(q, k, v, log_decay, _scale(scale, q), initial_state, return_last_state)
+    args = (q, k, v, log_decay, _scale(scale, q), initial_state, return_last_state)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, log_decay, initial_state)):
+        return LinearAttentionFn.apply(*args)
+    return _forward(*args)[4]
 
 
 def linear_attention_update(state, q, k, v, log_decay, scale=None):
