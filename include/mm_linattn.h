@@ -42,7 +42,8 @@ typedef struct mm_linattn_fwd_params {
     const float *initial_state;  /* (batch, nheads, dk, dv) or NULL (zeros) */
     void *out;                   /* (batch, seqlen, nheads, dv) */
     float *last_state;           /* (batch, nheads, dk, dv) or NULL */
-    void *workspace;             /* mm_linattn_fwd_workspace_size() bytes, 16-byte aligned; NULL: one pass per row */
+    void *workspace;             /* mm_linattn_fwd_workspace_size() bytes, 16-byte aligned; NULL: one pass per row.
+                                  * Afterwards it holds the states that the row's segments start from. */
     int64_t workspace_bytes;
     int64_t q_batch_stride, q_seq_stride, q_group_stride;
     int64_t k_batch_stride, k_seq_stride, k_group_stride;
@@ -64,6 +65,7 @@ typedef struct mm_linattn_bwd_params {
     void *dv_out;                /* contiguous (batch, seqlen, nheads, dv) */
     void *dlog_decay;            /* contiguous (batch, seqlen, nheads), or (nheads,) with decay_per_head; or NULL */
     float *dinitial_state;       /* (batch, nheads, dk, dv) or NULL */
+    const void *segment_states;  /* the forward's workspace after the same call, or NULL (computed again) */
     int32_t decay_per_head;      /* log_decay is one value per head: dlog_decay is summed over batch and seqlen */
     void *workspace;             /* mm_linattn_bwd_workspace_size() bytes, 16-byte aligned (required) */
     int64_t workspace_bytes;

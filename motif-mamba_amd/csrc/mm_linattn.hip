@@ -182,29 +182,44 @@ __global__ void __launch_bounds__(kThreads) la_segments(const WalkArgs a) {
     load_state<KD, 1>(S, Mat{nullptr, 0, 0}, 0, 0, 0, lane);
     SX sy;
     SV sv;
-    uint32_t g = 0;
-    double total = 0.0;
+    auto start = [&](int64_t n) { return tbeg + (REV ? chunks - 1 - n : n) * C; };
     auto load = [&](int64_t n) {
-        const int64_t t0 = tbeg + (REV ? chunks - 1 - n : n) * C;
+        const int64_t t0 = start(n);
         const int rows = int(min(int64_t(C), tend - t0));
         sy.load(ry, t0, rows, tid);
         sv.load(rv, t0, rows, tid);
-        if (wave == 0) g = lane < rows ? load_g_raw(a.g, a.gtype, g0 + (t0 + lane) * a.g_seq) : 0u;
     };
+    auto decay = [&](int64_t n) {
+        const int64_t t = start(n) + lane;
+        return lane < C && t < tend ? load_g_raw(a.g, a.gtype, g0 + t * a.g_seq) : 0u;
+    };
+    // The next chunk's decays are made by one wave while the others work on this one's state.
+    double total = 0.0;
+    auto decays = [&](int buf, uint32_t w) {
+        make_decays<C>(dec[buf], decode_g(w, a.gtype), a.scale, lane);
+        total += double(dec[buf].hi[C - 1]) + double(dec[buf].lo[C - 1]);
+    };
+    uint32_t gnext = 0;
     load(0);
-    for (int64_t n = 0; n < chunks; ++n) {
+    if (wave == 0) {
+        decays(0, decay(0));
+        if (chunks > 1) gnext = decay(1);
+    }
+    int buf = 0;
+    for (int64_t n = 0; n < chunks; ++n, buf ^= 1) {
         __syncthreads();
         sy.store(Y, tid);
         sv.store(V, tid);
-        if (wave == 0) {
-            make_decays<C>(*dec, decode_g(g, a.gtype), a.scale, lane);
-            total += double(dec->hi[C - 1]) + double(dec->lo[C - 1]);
-        }
         if (n + 1 < chunks) load(n + 1);
         __syncthreads();
+        const Decays<C> &d = dec[buf];
         bf16x8 v[C / 32][1][PI];
         load_v<T, C, 1, LDV>(v, V, col, lane);
-        update<T, C, KD, 1>(S, v, Y, REV ? dec->in : dec->out, dec->all, lane);
+        update<T, C, KD, 1>(S, v, Y, REV ? d.in : d.out, d.all, lane);
+        if (wave == 0 && n + 1 < chunks) {
+            decays(buf ^ 1, gnext);
+            if (n + 2 < chunks) gnext = decay(n + 2);
+        }
     }
     store_state<KD, 1>(S, Mat{a.st + (bh * a.segs + seg) * a.kdim * a.cdim, a.cdim, 1}, a.kdim, a.cdim, col0 + col, lane);
     if (slice == 0 && tid == 0) a.seg_decay[bh * a.segs + seg] = exp_f32(float(total));
@@ -412,7 +427,7 @@ static int launch_walk_k(const WalkArgs &a, hipStream_t s) {
 template <typename T, int KD, bool REV, bool VEC>
 static int launch_segments_t(const WalkArgs &a0, hipStream_t s) {
     constexpr int C = Cfg<T>::C, PI = Cfg<T>::in;
-    constexpr int bytes = 2 * (PI * kTile<C, KD> + PI * kTile<C, 64>) + int(sizeof(Decays<C>));
+    constexpr int bytes = 2 * (PI * kTile<C, KD> + PI * kTile<C, 64>) + 2 * int(sizeof(Decays<C>));
     static_assert(bytes <= 160 * 1024, "LDS");
     const auto kernel = la_segments<T, KD, REV, VEC>;
     static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
@@ -490,16 +505,26 @@ __global__ void __launch_bounds__(256) la_join(float *st, const float *decay, co
     }
 }
 
-// out[row][x] = sum over the group's heads of part[row][head][x], in order.
-template <typename T>
+// out[row][x] = sum over the group's heads of part[row][head][x], in order; W consecutive x per thread.
+template <typename T, int W>
 __global__ void __launch_bounds__(256) la_head_sum(const float *part, T *out, int64_t n, int heads, int share, int d) {
-    const int64_t at = int64_t(blockIdx.x) * 256 + threadIdx.x;
-    if (at >= n) return;
-    const int64_t x = at % d, rg = at / d, groups = heads / share, row = rg / groups, grp = rg % groups;
+    const int64_t id = (int64_t(blockIdx.x) * 256 + threadIdx.x) * W;
+    if (id >= n) return;
+    const int64_t x = id % d, rg = id / d, groups = heads / share, row = rg / groups, grp = rg % groups;
     const float *p = part + (row * heads + grp * share) * d + x;
-    float s = 0.f;
-    for (int r = 0; r < share; ++r) s += p[int64_t(r) * d];
-    out[at] = from_f32<T>(s);
+    float s[W] = {};
+#pragma unroll 8
+    for (int r = 0; r < share; ++r) {
+        if constexpr (W == 4) {
+            const f32x4 y = *reinterpret_cast<const f32x4 *>(p + int64_t(r) * d);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[e] += y[e];
+        } else {
+            s[0] += p[int64_t(r) * d];
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < W; ++e) out[id + e] = from_f32<T>(s[e]);
 }
 
 __device__ __forceinline__ void store_g(void *p, mm_dtype t, int64_t i, float x) {
@@ -593,10 +618,16 @@ int launch_join(float *st, const float *decay, const float *edge, int segs, int6
 
 int launch_head_sum(const float *part, void *out, mm_dtype t, int64_t rows, int heads, int share, int d, hipStream_t s) {
     const int64_t n = rows * (heads / share) * d;
-    const dim3 grid(blocks_of(n)), blk(256);
-    if (t == MM_FLOAT32) hipLaunchKernelGGL(la_head_sum<float>, grid, blk, 0, s, part, static_cast<float *>(out), n, heads, share, d);
-    else if (t == MM_FLOAT16) hipLaunchKernelGGL(la_head_sum<f16_t>, grid, blk, 0, s, part, static_cast<f16_t *>(out), n, heads, share, d);
-    else hipLaunchKernelGGL(la_head_sum<bf16_t>, grid, blk, 0, s, part, static_cast<bf16_t *>(out), n, heads, share, d);
+    const bool vec = d % 4 == 0;
+    const dim3 grid(blocks_of(vec ? n / 4 : n)), blk(256);
+    auto go = [&](auto *to) {
+        typedef std::remove_pointer_t<decltype(to)> O;
+        if (vec) hipLaunchKernelGGL((la_head_sum<O, 4>), grid, blk, 0, s, part, to, n, heads, share, d);
+        else hipLaunchKernelGGL((la_head_sum<O, 1>), grid, blk, 0, s, part, to, n, heads, share, d);
+    };
+    if (t == MM_FLOAT32) go(static_cast<float *>(out));
+    else if (t == MM_FLOAT16) go(static_cast<f16_t *>(out));
+    else go(static_cast<bf16_t *>(out));
     return launch_status("la_head_sum");
 }
 

@@ -126,15 +126,28 @@ static int chunk_of(mm_dtype t) { return t == MM_BFLOAT16 ? 64 : 32; }
 
 constexpr int kBlockTokens = 256;
 
-// Segments of a row: one where the (batch row, head) pairs give every CU a workgroup, else enough for two per CU, of
-// two blocks at least.
-static void segments(int64_t pairs, int64_t seqlen, int *segs, int64_t *len) {
-    const int64_t cus = device_simds() / 4, blocks = (seqlen + kBlockTokens - 1) / kBlockTokens;
-    int64_t n = pairs >= cus ? 1 : (2 * cus + pairs - 1) / std::max<int64_t>(pairs, 1);
-    n = std::max<int64_t>(1, std::min(n, blocks / 2));
-    const int64_t per = (blocks + n - 1) / std::max<int64_t>(n, 1);
-    *len = std::max<int64_t>(1, per) * kBlockTokens;
-    *segs = int(std::max<int64_t>(1, (seqlen + *len - 1) / *len));
+// Segments of a row, by the time that a call takes with n of them, in steps of a chunk of one workgroup alone on its CU
+// (about 3.7 us at dk 128, dv 64, bfloat16). Two workgroups on a CU take 1.45 steps per chunk of both. With n > 1 a pass over
+// k and v before (0.9 of a step per chunk, four workgroups per CU), its join (about 2 steps), and the states' traffic, 16 bytes
+// per element and segment at some 4.5 TB/s. Measured: 320 pairs (4 x 80 heads), L 4,096: one segment 322 us, two 274 + 128;
+// 192 pairs, L 2,048: one 103 us, three 86 + 45; 64 pairs (dk = dv = 128), L 4,096: 100 + 70 us with eight, 240 with one.
+static void segments(int64_t pairs, int64_t seqlen, int64_t size, int *segs, int64_t *len) {
+    const int64_t cus = device_simds() / 4, blocks = std::max<int64_t>(1, (seqlen + kBlockTokens - 1) / kBlockTokens);
+    double best = 0.0;
+    for (int64_t n = 1; n <= std::min<int64_t>(blocks, 64); ++n) {
+        const int64_t per = (blocks + n - 1) / n, w = (blocks + per - 1) / per;   // blocks per segment, segments
+        if (w != n) continue;
+        const double steps = double(per) * 4.0;
+        const int64_t r = (pairs * n + cus - 1) / cus;
+        double t = steps * (1.45 * double(r / 2) + double(r % 2));
+        if (n > 1)
+            t += 0.9 * steps * double((pairs * (n - 1) + 4 * cus - 1) / (4 * cus)) + 2.0 + double(n * pairs * size) * 16.0 / 4.5e12 / 3.7e-6;
+        if (n == 1 || t < best) {
+            best = t;
+            *segs = int(n);
+            *len = per * kBlockTokens;
+        }
+    }
 }
 
 static int64_t pad16(int64_t n) { return (n + 15) / 16 * 16; }
@@ -181,7 +194,7 @@ static int run_fwd(const mm_linattn_fwd_params &p, hipStream_t s) {
     a.g_batch = p.g_batch_stride; a.g_seq = p.g_seq_stride; a.g_head = p.g_head_stride;
     a.batch = p.batch; a.seqlen = p.seqlen; a.heads = p.nheads;
     a.kdim = int(p.dk); a.cdim = int(p.dv); a.slices = 1;
-    segments(p.batch * p.nheads, p.seqlen, &a.segs, &a.seg_len);
+    segments(p.batch * p.nheads, p.seqlen, p.dk * p.dv, &a.segs, &a.seg_len);
     if (a.segs > 1 && (!p.workspace || p.workspace_bytes < fwd_bytes(p, a.segs))) {
         a.segs = 1;
         a.seg_len = (p.seqlen + kBlockTokens - 1) / kBlockTokens * kBlockTokens;
@@ -215,7 +228,7 @@ struct BwdPlan {
 
 static BwdPlan plan_bwd(const mm_linattn_bwd_params &p) {
     BwdPlan w = {};
-    segments(p.batch * p.nheads, p.seqlen, &w.segs, &w.seg_len);
+    segments(p.batch * p.nheads, p.seqlen, p.dk * p.dv, &w.segs, &w.seg_len);
     w.blocks = (p.seqlen + kBlockTokens - 1) / kBlockTokens;
     const int64_t bh = p.batch * p.nheads, size = p.dk * p.dv, tok = bh * p.seqlen;
     int64_t at = 0;
@@ -225,7 +238,7 @@ static BwdPlan plan_bwd(const mm_linattn_bwd_params &p) {
         return o;
     };
     if (w.segs > 1) {
-        w.st = take(bh * w.segs * size);
+        if (!p.segment_states) w.st = take(bh * w.segs * size);
         w.rt = take(bh * w.segs * size);
         w.decay = take(bh * w.segs);
     }
@@ -263,9 +276,11 @@ static int run_bwd(const mm_linattn_bwd_params &p, hipStream_t s) {
         // The states the segments start from, and the states' gradients at their ends.
         a.seg_decay = f32(w.decay);
         a.kdim = int(p.dk); a.cdim = int(p.dv);
-        a.y = k; a.v = v; a.st = f32(w.st); a.scale = 1.f;
-        if (const int rc = launch_segments<T>(a, false, s)) return rc;
-        if (const int rc = launch_join(a.st, a.seg_decay, p.initial_state, a.segs, size, bh, false, s)) return rc;
+        if (!p.segment_states) {
+            a.y = k; a.v = v; a.st = f32(w.st); a.scale = 1.f;
+            if (const int rc = launch_segments<T>(a, false, s)) return rc;
+            if (const int rc = launch_join(a.st, a.seg_decay, p.initial_state, a.segs, size, bh, false, s)) return rc;
+        }
         a.y = q; a.v = d; a.st = f32(w.rt); a.scale = p.scale;
         if (const int rc = launch_segments<T>(a, true, s)) return rc;
         if (const int rc = launch_join(a.st, a.seg_decay, p.dlast_state, a.segs, size, bh, true, s)) return rc;
@@ -274,7 +289,8 @@ static int run_bwd(const mm_linattn_bwd_params &p, hipStream_t s) {
     a.x = d; a.y = v; a.v = k; a.z = q;
     a.kdim = int(p.dv); a.cdim = int(p.dk); a.slices = 1;
     a.scale = p.scale;
-    a.s0 = State{w.segs > 1 ? f32(w.st) : const_cast<float *>(p.initial_state), 1, p.dv};
+    const float *start = w.segs == 1 ? p.initial_state : p.segment_states ? static_cast<const float *>(p.segment_states) : f32(w.st);
+    a.s0 = State{const_cast<float *>(start), 1, p.dv};
     a.s0_step = size;
     a.out = shared ? static_cast<void *>(f32(w.part)) : p.dq;
     a.out_f32 = shared;
@@ -326,7 +342,7 @@ extern "C" int64_t mm_linattn_fwd_workspace_size(const mm_linattn_fwd_params *p)
     if (!p || p->batch <= 0 || p->seqlen <= 0 || p->nheads <= 0) return 0;
     int segs;
     int64_t len;
-    la::segments(p->batch * p->nheads, p->seqlen, &segs, &len);
+    la::segments(p->batch * p->nheads, p->seqlen, p->dk * p->dv, &segs, &len);
     return la::fwd_bytes(*p, segs);
 }
 

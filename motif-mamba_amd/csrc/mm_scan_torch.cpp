@@ -808,7 +808,7 @@ void *workspace_of(at::Tensor &keep, int64_t bytes, const at::Tensor &like) {
 }
 
 std::vector<at::Tensor> linattn_fwd(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &g,
-                                    double scale, const c10::optional<at::Tensor> &initial_, bool return_last_state) {
+                                    double scale, const c10::optional<at::Tensor> &initial_, bool return_last_state, bool keep_states) {
     check_qkv(q, k, v, 4);
     const int64_t batch = v.size(0), seqlen = v.size(1), heads = v.size(2), dv = v.size(3), dk = q.size(3);
     check_decay(g, {batch, seqlen, heads}, v);
@@ -842,6 +842,7 @@ std::vector<at::Tensor> linattn_fwd(const at::Tensor &q, const at::Tensor &k, co
     check_rc(mm_linattn_fwd(&p, c10::hip::getCurrentHIPStream().stream()), "mm_linattn_fwd");
     std::vector<at::Tensor> res{out};
     if (return_last_state) res.push_back(last);
+    if (keep_states) res.push_back(ws);   // undefined where a row is one segment
     return res;
 }
 
@@ -849,8 +850,8 @@ std::vector<at::Tensor> linattn_fwd(const at::Tensor &q, const at::Tensor &k, co
 // (nheads,) with decay_per_head.
 std::vector<c10::optional<at::Tensor>> linattn_bwd(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &g,
                                                    double scale, const c10::optional<at::Tensor> &initial_, const at::Tensor &dout,
-                                                   const c10::optional<at::Tensor> &dlast_, bool decay_per_head, bool want_decay,
-                                                   bool want_initial) {
+                                                   const c10::optional<at::Tensor> &dlast_, const c10::optional<at::Tensor> &states_,
+                                                   bool decay_per_head, bool want_decay, bool want_initial) {
     check_qkv(q, k, v, 4);
     const int64_t batch = v.size(0), seqlen = v.size(1), heads = v.size(2), dv = v.size(3), dk = q.size(3);
     check_decay(g, {batch, seqlen, heads}, v);
@@ -884,6 +885,7 @@ std::vector<c10::optional<at::Tensor>> linattn_bwd(const at::Tensor &q, const at
     p.dlog_decay = dg.defined() ? dg.data_ptr() : nullptr;
     p.dinitial_state = ds.defined() ? ds.data_ptr<float>() : nullptr;
     p.decay_per_head = decay_per_head;
+    p.segment_states = states_.has_value() && states_.value().defined() ? states_.value().data_ptr() : nullptr;
     p.q_batch_stride = q.stride(0); p.q_seq_stride = q.stride(1); p.q_group_stride = q.stride(2);
     p.k_batch_stride = k.stride(0); p.k_seq_stride = k.stride(1); p.k_group_stride = k.stride(2);
     p.v_batch_stride = v.stride(0); p.v_seq_stride = v.stride(1); p.v_head_stride = v.stride(2);
@@ -1047,12 +1049,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("rms_norm_fwd", &rms_norm_fwd, "Row RMSNorm over dim 1 of a 3-D tensor",
           pybind11::arg("x"), pybind11::arg("weight"), pybind11::arg("eps") = 1e-6,
           pybind11::arg("out") = pybind11::none());
-    m.def("linattn_fwd", &linattn_fwd, "Linear attention forward [out, last_state?]", pybind11::arg("q"), pybind11::arg("k"),
+    m.def("linattn_fwd", &linattn_fwd, "Linear attention forward [out, last_state?, states of the segments?]", pybind11::arg("q"), pybind11::arg("k"),
           pybind11::arg("v"), pybind11::arg("log_decay"), pybind11::arg("scale"), pybind11::arg("initial_state") = pybind11::none(),
-          pybind11::arg("return_last_state") = false);
+          pybind11::arg("return_last_state") = false, pybind11::arg("keep_states") = false);
     m.def("linattn_bwd", &linattn_bwd, "Linear attention backward [dq, dk, dv, dlog_decay?, dinitial_state?]", pybind11::arg("q"),
           pybind11::arg("k"), pybind11::arg("v"), pybind11::arg("log_decay"), pybind11::arg("scale"), pybind11::arg("initial_state"),
-          pybind11::arg("dout"), pybind11::arg("dlast_state"), pybind11::arg("decay_per_head"), pybind11::arg("want_decay"),
+          pybind11::arg("dout"), pybind11::arg("dlast_state"), pybind11::arg("states"), pybind11::arg("decay_per_head"), pybind11::arg("want_decay"),
           pybind11::arg("want_initial"));
     m.def("linattn_update", &linattn_update, "Linear attention, one token (in place on state)", pybind11::arg("state"), pybind11::arg("q"),
           pybind11::arg("k"), pybind11::arg("v"), pybind11::arg("log_decay"), pybind11::arg("scale"));

@@ -41,33 +41,35 @@ def _scale(scale, q):
     return q.shape[-1] ** -0.5 if scale is None else float(scale)
 
 
-def _forward(q, k, v, log_decay, scale, initial_state, return_last_state):
+def _forward(q, k, v, log_decay, scale, initial_state, return_last_state, keep_states=False):
     q, k, v = _rows(q), _rows(k), _rows(v)
     g, per_head = _spread(log_decay, v.shape[:2], v)
-    res = ext().linattn_fwd(q, k, v, g, scale, initial_state, return_last_state)
-    return q, k, v, per_head, tuple(res) if return_last_state else res[0]
+    res = ext().linattn_fwd(q, k, v, g, scale, initial_state, return_last_state, keep_states)
+    states = res.pop() if keep_states else None
+    return q, k, v, per_head, states, tuple(res) if return_last_state else res[0]
 
 
 class LinearAttentionFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, log_decay, scale, initial_state, return_last_state):
-        q, k, v, ctx.per_head, out = _forward(q, k, v, log_decay, scale, initial_state, return_last_state)
+        # Long rows of few heads run in segments; the states those start from serve the backward too.
+        q, k, v, ctx.per_head, states, out = _forward(q, k, v, log_decay, scale, initial_state, return_last_state, True)
         ctx.scale = scale
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(q, k, v, log_decay, initial_state)
+        ctx.save_for_backward(q, k, v, log_decay, initial_state, states)
         return out
 
     @staticmethod
     def backward(ctx, dout, dlast=None):
-        q, k, v, log_decay, initial_state = ctx.saved_tensors
+        q, k, v, log_decay, initial_state, states = ctx.saved_tensors
         if dout is None:
             if dlast is None:
                 return None, None, None, None, None, None, None
             dout = torch.zeros_like(v, memory_format=torch.contiguous_format)
         g, _ = _spread(log_decay, v.shape[:2], v)
         want = ctx.needs_input_grad
-        dq, dk, dv, dg, ds = ext().linattn_bwd(q, k, v, g, ctx.scale, initial_state, _rows(dout), dlast, ctx.per_head, want[3],
+        dq, dk, dv, dg, ds = ext().linattn_bwd(q, k, v, g, ctx.scale, initial_state, _rows(dout), dlast, states, ctx.per_head, want[3],
                                                want[5] and initial_state is not None)
         return dq, dk, dv, dg, None, ds, None
 
@@ -82,7 +84,7 @@ def linear_attention_fn(q, k, v, log_decay, scale=None, initial_state=None, retu
     args = (q, k, v, log_decay, _scale(scale, q), initial_state, return_last_state)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, log_decay, initial_state)):
         return LinearAttentionFn.apply(*args)
-    return _forward(*args)[4]
+    return _forward(*args)[5]
 
 
 def linear_attention_update(state, q, k, v, log_decay, scale=None):
