@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(K
         sv.store(V, tid);
         if constexpr (DOT) sz.store(Z, tid);
         const bool more = t0 + C < tend;
-        if (more) load(t0 + C);
+        const int next = int(min(int64_t(C), tend - t0 - C));
         __syncthreads();
         fresh();
         const Decays<C> &d = dec[buf];
@@ -121,10 +121,13 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(K
                 case 2: tiles(Tiles<0, 0>{});
             }
         }
+        // The next chunk's loads go out between the steps, a tensor at a time.
+        if (more) sx.load(rx, t0 + C, next, tid);
         f32x4 O[C / 16][NC];
         fresh();
         inter<T, C, KD, NC, DOT ? 3 : PS>(O, S, X, d.in, lane);
         if constexpr (DOT) dot_rows<T, C, NC, LDV>(O, Z, col, part + wave * C, lane);
+        if (more) sy.load(ry, t0 + C, next, tid);
         if (wave == dwave && more) {
             make_decays<C>(dec[buf ^ 1], decode_g(gnext, a.gtype), a.scale, lane);
             if (t0 + 2 * C < tend) gnext = decay(t0 + 2 * C);
@@ -138,6 +141,10 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(K
                 for (int w = 0; w < kWaves; ++w) e += part[w * C + tid];
                 a.e[bh * a.seqlen + t0 + tid] = e;
             }
+        }
+        if (more) {
+            sv.load(rv, t0 + C, next, tid);
+            if constexpr (DOT) sz.load(rz, t0 + C, next, tid);
         }
         bf16x8 v[C / 32][NC][PI];
         load_v<T, C, NC, LDV>(v, V, col, lane);
@@ -320,7 +327,7 @@ __device__ __forceinline__ void bwd_walk(const BwdArgs &a, char *smem, int tid, 
         sv.store(V, tid);
         sd.store(G, tid);
         const bool more = n + 1 < chunks;
-        if (more) load(n + 1);
+        const int64_t tn = t0 - C;   // the next chunk is a whole one
         __syncthreads();
         fresh();
         const Decays<C> &d = dec[buf];
@@ -344,12 +351,14 @@ __device__ __forceinline__ void bwd_walk(const BwdArgs &a, char *smem, int tid, 
                 case kWaves: tiles(Tiles<1, 1>{});
             }
         }
+        if (more) sq.load(rq, tn, C, tid);
         f32x4 O[CT][NC];
         fresh();
         inter<T, C, KX, NC, FOR_K ? 3 : PS>(O, S, FOR_K ? V : K, d.out, lane);
         if constexpr (FOR_K) {
             if (a.a) dot_rows<T, C, NC, LDK>(O, K, col, part + (wave - kWaves) * C, lane);
         }
+        if (more) sk.load(rk, tn, C, tid);
         if (dwave && more) {
             make_decays<C>(dec[buf ^ 1], decode_g(gnext, a.gtype), a.scale, lane);
             if (n + 2 < chunks) gnext = decay(n + 2);
@@ -367,6 +376,10 @@ __device__ __forceinline__ void bwd_walk(const BwdArgs &a, char *smem, int tid, 
                 a.a[bh * a.seqlen + t0 + tid] = sum;
                 a.f[bh * a.seqlen + t0 + tid] = f;
             }
+        }
+        if (more) {
+            sv.load(rv, tn, C, tid);
+            sd.load(rd, tn, C, tid);
         }
         const u16 *VT = FOR_K ? Q : G;
         bf16x8 v[C / 32][NC][PI];
