@@ -17,6 +17,8 @@ _NONE, _AFTER, _BEFORE, _ACT = 0, 1, 2, 3
 
 def _flat(t):
     """(rows, channels), a view where there is one."""
+    if t.dim() == 2 and t.stride(1) == 1:
+        return t
     t = t.reshape(-1, t.shape[-1]) if t.shape[-1] else t.reshape(t[..., 0:0].numel(), 0)
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
