@@ -166,7 +166,7 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(K
 // What each segment but the last one (REV: the first one) of a row adds to the state: sum of y_t (decay to the
 // segment's end) v_t^T into st[bh][seg], and the segment's own decay into decay[bh][seg].
 template <typename T, int KD, bool REV, bool VEC>
-__global__ void __launch_bounds__(kThreads) la_segments(const WalkArgs a) {
+__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 2 ? 3 : 2, sizeof(T) == 2 ? 3 : 2))) la_segments(const WalkArgs a) {
     constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, W = 64;
     constexpr int LDX = KD, LDV = W;
     typedef Stage<T, C, KD, kThreads, VEC> SX;
@@ -174,7 +174,8 @@ __global__ void __launch_bounds__(kThreads) la_segments(const WalkArgs a) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     u16 *Y = reinterpret_cast<u16 *>(smem), *V = Y + PI * kTile<C, LDX>;
     Decays<C> *dec = reinterpret_cast<Decays<C> *>(V + PI * kTile<C, LDV>);
-    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid & 63;
+    int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
     int64_t id = blockIdx.x;
     const int slice = id % a.slices; id /= a.slices;
     const int seg = id % a.segs; id /= a.segs;
@@ -215,6 +216,8 @@ __global__ void __launch_bounds__(kThreads) la_segments(const WalkArgs a) {
     int buf = 0;
     for (int64_t n = 0; n < chunks; ++n, buf ^= 1) {
         __syncthreads();
+        tid = afresh_lane(tid);
+        lane = tid & 63;
         sy.store(Y, tid);
         sv.store(V, tid);
         if (n + 1 < chunks) load(n + 1);

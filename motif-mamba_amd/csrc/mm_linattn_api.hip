@@ -128,8 +128,8 @@ constexpr int kBlockTokens = 256;
 
 // Segments of a row, by the time that a call takes with n of them, in steps of a chunk of one workgroup alone on its CU
 // (about 3.7 us at dk 128, dv 64, bfloat16). Two workgroups on a CU take 1.45 steps per chunk of both. With n > 1 a pass over
-// k and v before (0.9 of a step per chunk, four workgroups per CU), its join (about 2 steps), and the states' traffic, 16 bytes
-// per element and segment at some 4.5 TB/s. Measured: 320 pairs (4 x 80 heads), L 4,096: one segment 322 us, two 274 + 128;
+// k and v before (0.9 of a step per chunk for few workgroups, 0.5 of one per chunk and CU for many), its join (about 2 steps),
+// and the states' traffic, 16 bytes per element and segment at some 4.5 TB/s. Measured: 320 pairs (4 x 80 heads), L 4,096: one segment 322 us, two 274 + 128;
 // 192 pairs, L 2,048: one 103 us, three 86 + 45; 64 pairs (dk = dv = 128), L 4,096: 100 + 70 us with eight, 240 with one.
 static void segments(int64_t pairs, int64_t seqlen, int64_t size, int *segs, int64_t *len) {
     const int64_t cus = device_simds() / 4, blocks = std::max<int64_t>(1, (seqlen + kBlockTokens - 1) / kBlockTokens);
@@ -141,7 +141,7 @@ static void segments(int64_t pairs, int64_t seqlen, int64_t size, int *segs, int
         const int64_t r = (pairs * n + cus - 1) / cus;
         double t = steps * (1.45 * double(r / 2) + double(r % 2));
         if (n > 1)
-            t += 0.9 * steps * double((pairs * (n - 1) + 4 * cus - 1) / (4 * cus)) + 2.0 + double(n * pairs * size) * 16.0 / 4.5e12 / 3.7e-6;
+            t += steps * std::max(0.9, 0.5 * double(pairs * (n - 1)) / double(cus)) + 2.0 + double(n * pairs * size) * 16.0 / 4.5e12 / 3.7e-6;
         if (n == 1 || t < best) {
             best = t;
             *segs = int(n);
