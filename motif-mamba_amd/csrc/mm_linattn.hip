@@ -13,6 +13,8 @@
 #define MM_LINATTN_COMMON
 #endif
 
+#include <atomic>
+
 #include "mm_linattn_dev.h"
 #include "mm_linattn_host.h"
 
@@ -29,6 +31,14 @@ __device__ __forceinline__ Rows<T> rows_of(const View &v, int64_t b, int64_t h, 
 // Forward walk: out = scale (masked X Y^T) V + ..., KD the padded length of X's rows, 64 NC columns of V per
 // workgroup, 16 NC per wave. DOT: also e[t] = (the product with the state alone) . Z_t, and the state at every
 // kBlock-th token into ck (the decays' gradient).
+//
+// Per chunk: stage X, Y and V; scores (each wave its tiles, into M) and the product with the state; the product of M and V,
+// the state's update, the outputs. The waves share X, Y and M through LDS and split V's columns, so that a wave's part of the
+// state never leaves its accumulators. At dk 128, dv 64, bfloat16 a wave issues 102 matrix and some 510 other vector
+// instructions per 64 tokens and the LDS works 2,900 cycles; with 2 workgroups on a CU (202 registers, 61 KB) a chunk of both
+// takes some 5.7 us, of one alone 4.0: latency between the three barriers bounds it, no unit is busy more than 60 %.
+// 4 x 4,096 tokens, 80 heads: 319 us, 1.1 TB/s of its 360 MB and 400 TFLOP/s on the matrix cores, split planes counted.
+// Three workgroups at 168 registers spill (457 us for 128 heads against 365), chunks of 32 tokens gain nothing (394).
 template <typename T, int KD, int NC, bool DOT, bool VEC, bool F32>
 __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(KD * NC == 64 ? 3 : 2, KD * NC == 64 ? 3 : 2))) la_walk(const WalkArgs a) {
     constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, PS = Cfg<T>::st, W = 64 * NC;
@@ -164,7 +174,8 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(K
 }
 
 // What each segment but the last one (REV: the first one) of a row adds to the state: sum of y_t (decay to the
-// segment's end) v_t^T into st[bh][seg], and the segment's own decay into decay[bh][seg].
+// segment's end) v_t^T into st[bh][seg], and the segment's own decay into decay[bh][seg]. About 2 us per chunk and CU at
+// dk 128 (7 of 8 segments of 64 pairs, dv 128, L 4,096: 55 us).
 template <typename T, int KD, bool REV, bool VEC>
 __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 2 ? 3 : 2, sizeof(T) == 2 ? 3 : 2))) la_segments(const WalkArgs a) {
     constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, W = 64;
@@ -239,6 +250,10 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(s
 // every kBlock-th token the product of the state there with its gradient (y). Waves 0 to 3 hold the gradient R of the
 // state for dv (rows dk, columns dv), waves 4 to 7 its transpose for dk: two walks over the same tiles, each in code of
 // its own with the same barriers.
+//
+// Every q, k, v and dout row is read once for both. One workgroup of 8 waves per CU (90 KB of LDS and 200 to 250 registers at
+// dk 128), 9 us per 64 tokens with dv 64, half of the waves' time waiting: 8 x 2,048 tokens, 24 heads, 291 us; 4 x 4,096 tokens,
+// 16 heads with dv 128, 181 us.
 //
 // FOR_K: the walk of dk, X = v, Y = do, V = q; else that of dv, X = k, Y = q, V = do. KX: X's padded row length, KV: V's.
 template <typename T, int KD, int VD, bool VEC, bool F32, bool FOR_K>
@@ -412,9 +427,18 @@ __global__ void __launch_bounds__(2 * kThreads) __attribute__((amdgpu_waves_per_
     else bwd_walk<T, KD, VD, VEC, F32, true>(a, smem, tid, wave, lane);
 }
 
+// Launches with `bytes` of dynamic LDS, which a kernel is allowed once per device (`done`: a bit per device).
 template <typename K, typename A>
-static int launch_kernel(K kernel, int bytes, hipError_t set, int64_t grid, int threads, const A &a, hipStream_t s, const char *what) {
-    if (set != hipSuccess) return set_error(int(set), "linear attention: hipFuncSetAttribute failed");
+static int launch_kernel(K kernel, int bytes, std::atomic<uint64_t> &done, int64_t grid, int threads, const A &a, hipStream_t s,
+                         const char *what) {
+    int dev = 0;
+    if (const hipError_t e = hipGetDevice(&dev)) return set_error(int(e), "linear attention: hipGetDevice failed");
+    const uint64_t bit = uint64_t(1) << (dev & 63);
+    if (!(done.load(std::memory_order_relaxed) & bit)) {
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e != hipSuccess) return set_error(int(e), "linear attention: hipFuncSetAttribute failed");
+        done.fetch_or(bit, std::memory_order_relaxed);
+    }
     hipLaunchKernelGGL(kernel, dim3(unsigned(grid)), dim3(unsigned(threads)), bytes, s, a);
     return launch_status(what);
 }
@@ -426,8 +450,8 @@ static int launch_walk_t(const WalkArgs &a, hipStream_t s) {
                           2 * int(sizeof(Decays<C>)) + (DOT ? 4 * kWaves * C : 0);
     static_assert(bytes <= 160 * 1024, "LDS");
     const auto kernel = la_walk<T, KD, NC, DOT, VEC, F32>;
-    static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    return launch_kernel(kernel, bytes, set, a.batch * a.heads * a.segs * a.slices, kThreads, a, s, "la_walk");
+    static std::atomic<uint64_t> done{0};
+    return launch_kernel(kernel, bytes, done, a.batch * a.heads * a.segs * a.slices, kThreads, a, s, "la_walk");
 }
 template <typename T, int KD, int NC, bool DOT>
 static int launch_walk_k(const WalkArgs &a, hipStream_t s) {
@@ -446,10 +470,10 @@ static int launch_segments_t(const WalkArgs &a0, hipStream_t s) {
     constexpr int bytes = 2 * (PI * kTile<C, KD> + PI * kTile<C, 64>) + 2 * int(sizeof(Decays<C>));
     static_assert(bytes <= 160 * 1024, "LDS");
     const auto kernel = la_segments<T, KD, REV, VEC>;
-    static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    static std::atomic<uint64_t> done{0};
     WalkArgs a = a0;
     a.slices = (a.cdim + 63) / 64;
-    return launch_kernel(kernel, bytes, set, a.batch * a.heads * a.segs * a.slices, kThreads, a, s, "la_segments");
+    return launch_kernel(kernel, bytes, done, a.batch * a.heads * a.segs * a.slices, kThreads, a, s, "la_segments");
 }
 template <typename T, int KD>
 static int launch_segments_k(const WalkArgs &a, bool rev, hipStream_t s) {
@@ -464,8 +488,8 @@ static int launch_bwd_t(const BwdArgs &a, hipStream_t s) {
                           2 * int(sizeof(Decays<C>)) + 4 * (2 * (C / 16) * C + kWaves * C);
     static_assert(bytes <= 160 * 1024, "LDS");
     const auto kernel = la_bwd<T, KD, VD, VEC, F32>;
-    static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    return launch_kernel(kernel, bytes, set, a.batch * a.heads * a.segs, 2 * kThreads, a, s, "la_bwd");
+    static std::atomic<uint64_t> done{0};
+    return launch_kernel(kernel, bytes, done, a.batch * a.heads * a.segs, 2 * kThreads, a, s, "la_bwd");
 }
 template <typename T, int KD, int VD>
 static int launch_bwd_k(const BwdArgs &a, hipStream_t s) {
@@ -509,7 +533,7 @@ template int launch_bwd<MM_LINATTN_TYPE>(const BwdArgs &, hipStream_t);
 
 // The segments' shares in st[bh][seg] become the states the segments start from (rev: end with).
 __global__ void __launch_bounds__(256) la_join(float *st, const float *decay, const float *edge, int segs, int64_t size, bool rev) {
-    const int64_t bh = blockIdx.y, x = int64_t(blockIdx.x) * 256 + threadIdx.x;
+    const int64_t bh = blockIdx.x, x = int64_t(blockIdx.y) * 256 + threadIdx.x;
     if (x >= size) return;
     float cur = edge ? edge[bh * size + x] : 0.f;
     float *p = st + bh * segs * size + x;
@@ -521,7 +545,8 @@ __global__ void __launch_bounds__(256) la_join(float *st, const float *decay, co
     }
 }
 
-// out[row][x] = sum over the group's heads of part[row][head][x], in order; W consecutive x per thread.
+// out[row][x] = sum over the group's heads of part[row][head][x], in order; W consecutive x per thread. HBM-bound: 201 MB of
+// 24 heads' gradients in 31 us (6.5 TB/s, part of them from the last-level cache), 59 with one element per thread.
 template <typename T, int W>
 __global__ void __launch_bounds__(256) la_head_sum(const float *part, T *out, int64_t n, int heads, int share, int d) {
     const int64_t id = (int64_t(blockIdx.x) * 256 + threadIdx.x) * W;
@@ -561,7 +586,7 @@ __global__ void __launch_bounds__(kBlock) la_decay_grad(const float *a, const fl
                                                         int64_t blocks, int heads, int C, bool has_last, const void *g, int64_t g_batch,
                                                         int64_t g_seq, int64_t g_head, float *tmp, void *out, mm_dtype gtype) {
     __shared__ float sa[kBlock], sf[kBlock], se[kBlock], zc[kBlock / 16];
-    const int64_t blk = blockIdx.x, bh = blockIdx.y, t = blk * kBlock + threadIdx.x;
+    const int64_t blk = blockIdx.y, bh = blockIdx.x, t = blk * kBlock + threadIdx.x;
     const int tid = threadIdx.x, chunks = kBlock / C;
     const bool live = t < seqlen;
     const float ae = live ? e[bh * seqlen + t] : 0.f;
@@ -628,7 +653,7 @@ __global__ void __launch_bounds__(256) la_zero_g(void *dst, mm_dtype t, int64_t 
 static unsigned blocks_of(int64_t n) { return unsigned((n + 255) / 256); }
 
 int launch_join(float *st, const float *decay, const float *edge, int segs, int64_t size, int64_t bh, bool rev, hipStream_t s) {
-    hipLaunchKernelGGL(la_join, dim3(blocks_of(size), unsigned(bh)), dim3(256), 0, s, st, decay, edge, segs, size, rev);
+    hipLaunchKernelGGL(la_join, dim3(unsigned(bh), blocks_of(size)), dim3(256), 0, s, st, decay, edge, segs, size, rev);
     return launch_status("la_join");
 }
 
@@ -649,7 +674,7 @@ int launch_head_sum(const float *part, void *out, mm_dtype t, int64_t rows, int 
 
 int launch_decay_grad(const BwdArgs &a, const float *e, int C, bool per_head, void *out, mm_dtype gtype, hipStream_t s) {
     // The sums over a head's tokens go through f's place, which a block reads before it writes.
-    hipLaunchKernelGGL(la_decay_grad, dim3(unsigned(a.blocks), unsigned(a.batch * a.heads)), dim3(kBlock), 0, s, a.a, e, a.f, a.y, a.seqlen,
+    hipLaunchKernelGGL(la_decay_grad, dim3(unsigned(a.batch * a.heads), unsigned(a.blocks)), dim3(kBlock), 0, s, a.a, e, a.f, a.y, a.seqlen,
                        a.blocks, int(a.heads), C, a.has_last != 0, a.g, a.g_batch, a.g_seq, a.g_head, per_head ? a.f : nullptr, out, gtype);
     if (const int rc = launch_status("la_decay_grad")) return rc;
     if (!per_head) return MM_OK;

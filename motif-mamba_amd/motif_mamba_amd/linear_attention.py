@@ -20,6 +20,7 @@ dk and dv up to 128 (else NotImplementedError).
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from ._native import ext
 
@@ -61,6 +62,7 @@ class LinearAttentionFn(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout, dlast=None):
         q, k, v, log_decay, initial_state, states = ctx.saved_tensors
         if dout is None:

@@ -365,3 +365,32 @@ def test_refusals():
         linear_attention_update(t["initial_state"].transpose(2, 3), **u)
     with pytest.raises(ValueError):
         linear_attention_update(t["initial_state"], u["q"], u["k"], t["v"], u["log_decay"])
+
+
+def test_many_short_rows():
+    """More (batch row, head) pairs than one grid dimension of 65,535 holds."""
+    _say("linear attention 70,000 pairs")
+    from motif_mamba_amd import linear_attention_fn, linear_attention_update
+    t = _inputs(1500, 17500, 3, 1, 4, 8, 8, BF16)
+    d = {n: x.to(DEV).requires_grad_(True) for n, x in t.items()}
+    dout = torch.randn(t["v"].shape, generator=torch.Generator().manual_seed(16)).to(BF16)
+    out = linear_attention_fn(**d, scale=0.4)
+    got = dict(zip(["d" + n for n in d], torch.autograd.grad(out, list(d.values()), dout.to(DEV))), out=out)
+    _check_all(got, t, 0.4, dout, None, BF16)
+    state = torch.zeros(17500, 4, 8, 8, device=DEV)
+    y = linear_attention_update(state, *(d[n].detach()[:, 0] for n in ("q", "k", "v", "log_decay")), scale=0.4)
+    exact, size = ref.with_grads({n: x[:, :1] for n, x in t.items()}, 0.4), ref.magnitudes({n: x[:, :1] for n, x in t.items()}, 0.4)
+    ref.check(y, exact["out"][:, 0], size["out"][:, 0], F32, "out")
+
+
+def test_no_second_derivative():
+    _say("linear attention, group norm: second derivatives refused")
+    from motif_mamba_amd import group_norm_fn, linear_attention_fn
+    t = {n: x.to(DEV).requires_grad_(True) for n, x in _inputs(1600, 1, 4, 1, 1, 8, 8, F32).items()}
+    (g,) = torch.autograd.grad(linear_attention_fn(**t).sum(), [t["q"]], create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+    x = torch.randn(4, 8, device=DEV, requires_grad=True)
+    (g,) = torch.autograd.grad(group_norm_fn(x, 2).square().sum(), [x], create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()

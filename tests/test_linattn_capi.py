@@ -80,7 +80,7 @@ PTRS = dict(q=4096, k=4096, v=4096, log_decay=4096)
 @pytest.mark.parametrize("change,code,needle", [
     (dict(itype=7), -1, "dtype"), (dict(gtype=9), -1, "dtype"), (dict(seqlen=-1), -1, "negative"), (dict(n_groups=0), -1, "multiple"),
     (dict(nheads=3, n_groups=2), -1, "multiple"), (dict(dk=0), -1, "at least 1"), (dict(dk=129), -2, "128"), (dict(dv=200), -2, "128"),
-    (dict(batch=40000), -2, "too large"), (dict(q=0), -1, "required"), (dict(out=0), -1, "required"),
+    (dict(batch=1 << 23), -2, "too large"), (dict(seqlen=1 << 24), -2, "2^23"), (dict(q=0), -1, "required"), (dict(out=0), -1, "required"),
     (dict(q_seq_stride=1 << 23), -2, "strides"), (dict(v_seq_stride=-4), -2, "strides")])
 def test_fwd_refusals(blocks, change, code, needle):
     rc, msg = _call("mm_linattn_fwd", _fill(blocks, "mm_linattn_fwd_params", **{**SIZES, **PTRS, "out": 4096, **change}))
