@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(K
         bf16x8 v[C / 32][NC][PI];
         load_v<T, C, NC, LDV>(v, V, col, lane);
         intra<T, C, NC, LDV, false>(O, v, M, V, col, lane);
-        update<T, C, KD, NC>(S, v, Y, d.out, d.all, lane);
+        update<T, C, KD, NC, Cfg<T>::up>(S, v, Y, d.out, d.all, lane);
         fresh();
         store_out<T, C, NC, LDV, VEC, F32>(O, static_cast<char *>(a.out) + (b * a.out_batch + h * a.out_head) * int64_t(F32 ? 4 : sizeof(T)),
                                            a.out_seq, t0, rows, a.cdim, col0, V, col, lane);
@@ -236,7 +236,7 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(s
         const Decays<C> &d = dec[buf];
         bf16x8 v[C / 32][1][PI];
         load_v<T, C, 1, LDV>(v, V, col, lane);
-        update<T, C, KD, 1>(S, v, Y, REV ? d.in : d.out, d.all, lane);
+        update<T, C, KD, 1, Cfg<T>::up>(S, v, Y, REV ? d.in : d.out, d.all, lane);
         if (wave == 0 && n + 1 < chunks) {
             decays(buf ^ 1, gnext);
             if (n + 2 < chunks) gnext = decay(n + 2);
@@ -255,8 +255,9 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(s
 // dk 128), 9 us per 64 tokens with dv 64, half of the waves' time waiting: 8 x 2,048 tokens, 24 heads, 291 us; 4 x 4,096 tokens,
 // 16 heads with dv 128, 181 us.
 //
-// FOR_K: the walk of dk, X = v, Y = do, V = q; else that of dv, X = k, Y = q, V = do. KX: X's padded row length, KV: V's.
-template <typename T, int KD, int VD, bool VEC, bool F32, bool FOR_K>
+// PREC: float32 results come from the state too (the decays' gradient, the initial state's): three planes where 16-bit
+// gradients alone need two. FOR_K: the walk of dk, X = v, Y = do, V = q; else that of dv, X = k, Y = q, V = do. KX: X's padded row length, KV: V's.
+template <typename T, int KD, int VD, bool VEC, bool F32, bool PREC, bool FOR_K>
 __device__ __forceinline__ void bwd_walk(const BwdArgs &a, char *smem, int tid, int wave, int lane) {
     constexpr bool kTight = KD + VD > 128;   // registers
     auto fresh = [&] {
@@ -291,22 +292,12 @@ __device__ __forceinline__ void bwd_walk(const BwdArgs &a, char *smem, int tid, 
                               FOR_K ? a.dv : 1}, rows_s, cols_s, col, lane);
     // <R, state> at a kept boundary, each wave's share.
     auto boundary = [&](int64_t m) {
-        const float *s = a.ck + (bh * a.blocks + m) * int64_t(a.dk) * a.dv;   // rows dv, columns dk
-        const int g = (lane >> 4), i = (lane & 15), rows = afresh(rows_s), cols = afresh(cols_s);
-        float sum = 0.f;
-#pragma unroll
-        for (int k = 0; k < KX / 16; ++k)
-#pragma unroll
-            for (int c = 0; c < NC; ++c)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int y = 16 * k + 4 * g + r, x = col + 16 * c + i;
-                    if (y < rows && x < cols) sum = __builtin_fmaf(S[k][c][r], s[int64_t(y) * cols + x], sum);
-                }
+        const Mat at{const_cast<float *>(a.ck) + (bh * a.blocks + m) * int64_t(a.dk) * a.dv, a.dk, 1};   // rows dv, columns dk
+        float sum = dot_state<KX, NC>(S, at, rows_s, cols_s, col, lane);
         sum = wave_sum(sum);
         if (lane == 0) a.y[(bh * a.blocks + m) * kWaves + wave - kWaves] = sum;
     };
-    if constexpr (FOR_K) {
+    if constexpr (FOR_K && PREC) {
         if (a.ck && a.has_last && seg == a.segs - 1) boundary(a.blocks - 1);
     }
 
@@ -350,7 +341,7 @@ __device__ __forceinline__ void bwd_walk(const BwdArgs &a, char *smem, int tid, 
         fresh();
         const Decays<C> &d = dec[buf];
         auto tiles = [&](auto L) {
-            scores_bwd<T, C, KD, VD, decltype(L)>(d, Q, K, V, G, M1, M2, a.scale, a.a != nullptr, rowp, colp, lane);
+            scores_bwd<T, C, KD, VD, decltype(L)>(d, Q, K, V, G, M1, M2, a.scale, PREC && a.a != nullptr, rowp, colp, lane);
         };
         if constexpr (C == 64) {
             switch (wave) {
@@ -372,8 +363,8 @@ __device__ __forceinline__ void bwd_walk(const BwdArgs &a, char *smem, int tid, 
         if (more) sq.load(rq, tn, C, tid);
         f32x4 O[CT][NC];
         fresh();
-        inter<T, C, KX, NC, FOR_K ? 3 : PS>(O, S, FOR_K ? V : K, d.out, lane);
-        if constexpr (FOR_K) {
+        inter<T, C, KX, NC, FOR_K && PREC ? 3 : PS>(O, S, FOR_K ? V : K, d.out, lane);
+        if constexpr (FOR_K && PREC) {
             if (a.a) dot_rows<T, C, NC, LDK>(O, K, col, part + (wave - kWaves) * C, lane);
         }
         if (more) sk.load(rk, tn, C, tid);
@@ -383,7 +374,7 @@ __device__ __forceinline__ void bwd_walk(const BwdArgs &a, char *smem, int tid, 
         }
         __syncthreads();
         fresh();
-        if constexpr (!FOR_K) {
+        if constexpr (!FOR_K && PREC) {
             if (a.a && tid < rows) {
                 const int t = tid / 16;
                 float sum = 0.f, f = 0.f;
@@ -403,12 +394,14 @@ __device__ __forceinline__ void bwd_walk(const BwdArgs &a, char *smem, int tid, 
         bf16x8 v[C / 32][NC][PI];
         load_v<T, C, NC, LDC>(v, VT, col, lane);
         intra<T, C, NC, LDC, true>(O, v, FOR_K ? M2 : M1, VT, col, lane);
-        update<T, C, KX, NC>(S, v, FOR_K ? G : Q, d.in, d.all, lane);
+        update<T, C, KX, NC, PREC ? Cfg<T>::up : PS>(S, v, FOR_K ? G : Q, d.in, d.all, lane);
         fresh();
         if constexpr (FOR_K) {
             store_out<T, C, NC, LDC, VEC, F32>(O, static_cast<char *>(a.dk_out) + (b * a.seqlen * a.heads + h) * a.dk * int64_t(F32 ? 4 : sizeof(T)),
                                                a.heads * a.dk, t0, rows, a.dk, 0, K, col, lane);
-            if (a.ck && t0 > 0 && t0 % kBlock == 0) boundary(t0 / kBlock - 1);
+            if constexpr (PREC) {
+                if (a.ck && t0 > 0 && t0 % kBlock == 0) boundary(t0 / kBlock - 1);
+            }
         } else {
             store_out<T, C, NC, LDC, VEC, false>(O, reinterpret_cast<T *>(a.dv_out) + (b * a.seqlen * a.heads + h) * a.dv, a.heads * a.dv, t0, rows,
                                                  a.dv, 0, V, col, lane);
@@ -419,12 +412,12 @@ __device__ __forceinline__ void bwd_walk(const BwdArgs &a, char *smem, int tid, 
     }
 }
 
-template <typename T, int KD, int VD, bool VEC, bool F32>
+template <typename T, int KD, int VD, bool VEC, bool F32, bool PREC>
 __global__ void __launch_bounds__(2 * kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) la_bwd(const BwdArgs a) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid & 63;
-    if (wave < kWaves) bwd_walk<T, KD, VD, VEC, F32, false>(a, smem, tid, wave, lane);
-    else bwd_walk<T, KD, VD, VEC, F32, true>(a, smem, tid, wave, lane);
+    if (wave < kWaves) bwd_walk<T, KD, VD, VEC, F32, PREC, false>(a, smem, tid, wave, lane);
+    else bwd_walk<T, KD, VD, VEC, F32, PREC, true>(a, smem, tid, wave, lane);
 }
 
 // Launches with `bytes` of dynamic LDS, which a kernel is allowed once per device (`done`: a bit per device).
@@ -481,25 +474,30 @@ static int launch_segments_k(const WalkArgs &a, bool rev, hipStream_t s) {
     return rev ? launch_segments_t<T, KD, true, false>(a, s) : launch_segments_t<T, KD, false, false>(a, s);
 }
 
-template <typename T, int KD, int VD, bool VEC, bool F32>
+template <typename T, int KD, int VD, bool VEC, bool F32, bool PREC>
 static int launch_bwd_t(const BwdArgs &a, hipStream_t s) {
     constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, PS = Cfg<T>::st;
     constexpr int bytes = 2 * (2 * PI * kTile<C, KD> + 2 * PI * kTile<C, VD> + 2 * PS * kTile<C, kScoreRow>) +
                           2 * int(sizeof(Decays<C>)) + 4 * (2 * (C / 16) * C + kWaves * C);
     static_assert(bytes <= 160 * 1024, "LDS");
-    const auto kernel = la_bwd<T, KD, VD, VEC, F32>;
+    const auto kernel = la_bwd<T, KD, VD, VEC, F32, PREC>;
     static std::atomic<uint64_t> done{0};
     return launch_kernel(kernel, bytes, done, a.batch * a.heads * a.segs, 2 * kThreads, a, s, "la_bwd");
 }
+template <typename T, int KD, int VD, bool F32>
+static int launch_bwd_f(const BwdArgs &a, hipStream_t s) {
+    const bool vec = a.q.vec && a.k.vec && a.v.vec && a.dout.vec && a.out_vec;
+    // float32 inputs take three planes everywhere.
+    const bool prec = sizeof(T) == 4 || a.a || a.dr;
+    if constexpr (sizeof(T) == 2) {
+        if (!prec) return vec ? launch_bwd_t<T, KD, VD, true, F32, false>(a, s) : launch_bwd_t<T, KD, VD, false, F32, false>(a, s);
+    }
+    return vec ? launch_bwd_t<T, KD, VD, true, F32, true>(a, s) : launch_bwd_t<T, KD, VD, false, F32, true>(a, s);
+}
 template <typename T, int KD, int VD>
 static int launch_bwd_k(const BwdArgs &a, hipStream_t s) {
-    const bool vec = a.q.vec && a.k.vec && a.v.vec && a.dout.vec && a.out_vec;
-    if constexpr (sizeof(T) == 4) {
-        return vec ? launch_bwd_t<T, KD, VD, true, true>(a, s) : launch_bwd_t<T, KD, VD, false, true>(a, s);
-    } else {
-        if (a.dk_f32) return vec ? launch_bwd_t<T, KD, VD, true, true>(a, s) : launch_bwd_t<T, KD, VD, false, true>(a, s);
-        return vec ? launch_bwd_t<T, KD, VD, true, false>(a, s) : launch_bwd_t<T, KD, VD, false, false>(a, s);
-    }
+    if constexpr (sizeof(T) == 4) return launch_bwd_f<T, KD, VD, true>(a, s);
+    else return a.dk_f32 ? launch_bwd_f<T, KD, VD, true>(a, s) : launch_bwd_f<T, KD, VD, false>(a, s);
 }
 
 template <typename T>

@@ -532,11 +532,11 @@ __device__ __forceinline__ void inter(f32x4 (&O)[C / 16][NC], const f32x4 (&S)[K
     }
 }
 
-// S = all S + Y^T diag(w) V for the wave's columns (V's operands in v).
-template <typename T, int C, int KD, int NC>
+// S = all S + Y^T diag(w) V for the wave's columns (V's operands in v). PU: the planes of diag(w) V.
+template <typename T, int C, int KD, int NC, int PU>
 __device__ __forceinline__ void update(f32x4 (&S)[KD / 16][NC], const bf16x8 (&v)[C / 32][NC][Cfg<T>::in], const u16 *Y,
                                        const float *w, float all, int lane) {
-    constexpr int PL = kTile<C, KD>, PI = Cfg<T>::in, PU = Cfg<T>::up;
+    constexpr int PL = kTile<C, KD>, PI = Cfg<T>::in;
     const int g = (lane >> 4), i = (lane & 15);
 #pragma unroll
     for (int k = 0; k < KD / 16; ++k)
@@ -688,24 +688,30 @@ __device__ __forceinline__ void intra(f32x4 (&O)[C / 16][NC], const bf16x8 (&v0)
         }
 }
 
-// A float32 matrix of a (batch row, head): rows x cols, with its strides.
+// A float32 matrix of a (batch row, head): rows x cols, with its strides (spans less than 2^31 bytes).
 struct Mat {
     float *p;
     int64_t row, col;
 };
+// Byte offset of the state's element (16 k + 4 g + r, col + 16 c + i), kNone outside.
+__device__ __forceinline__ uint32_t state_at(const Mat &m, int rows, int cols, int y, int x) {
+    return y < rows && x < cols ? (uint32_t(y) * uint32_t(m.row) + uint32_t(x) * uint32_t(m.col)) * 4 : kNone;
+}
 template <int KD, int NC>
 __device__ __forceinline__ void load_state(f32x4 (&S)[KD / 16][NC], const Mat &m, int rows, int cols, int col, int lane) {
     const int g = (lane >> 4), i = (lane & 15);
-    rows = afresh(rows);
+    rows = m.p ? afresh(rows) : 0;
     cols = afresh(cols);
+    const __amdgpu_buffer_rsrc_t buf = buffer(m.p);
 #pragma unroll
     for (int k = 0; k < KD / 16; ++k)
 #pragma unroll
         for (int c = 0; c < NC; ++c)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int y = 16 * k + 4 * g + r, x = col + 16 * c + i;
-                S[k][c][r] = m.p && y < rows && x < cols ? m.p[y * m.row + x * m.col] : 0.f;
+                uint32_t at = state_at(m, rows, cols, 16 * k + 4 * g + r, col + 16 * c + i);
+                asm("" : "+v"(at));
+                S[k][c][r] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(buf, at, 0, 0));
             }
 }
 template <int KD, int NC>
@@ -713,19 +719,51 @@ __device__ __forceinline__ void store_state(const f32x4 (&S)[KD / 16][NC], const
     const int g = (lane >> 4), i = (lane & 15);
     rows = afresh(rows);
     cols = afresh(cols);
+    const __amdgpu_buffer_rsrc_t buf = buffer(m.p);
 #pragma unroll
     for (int k = 0; k < KD / 16; ++k)
 #pragma unroll
         for (int c = 0; c < NC; ++c)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int y = 16 * k + 4 * g + r, x = col + 16 * c + i;
-                if (y < rows && x < cols) m.p[y * m.row + x * m.col] = S[k][c][r];
+                uint32_t at = state_at(m, rows, cols, 16 * k + 4 * g + r, col + 16 * c + i);
+                asm("" : "+v"(at));
+                __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(S[k][c][r]), buf, at, 0, 0);
             }
 }
+// The wave's share of <S, m>.
+template <int KD, int NC>
+__device__ __forceinline__ float dot_state(const f32x4 (&S)[KD / 16][NC], const Mat &m, int rows, int cols, int col, int lane) {
+    const int g = (lane >> 4), i = (lane & 15);
+    rows = afresh(rows);
+    cols = afresh(cols);
+    const __amdgpu_buffer_rsrc_t buf = buffer(m.p);
+    float sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < KD / 16; ++k)
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            float w[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                uint32_t at = state_at(m, rows, cols, 16 * k + 4 * g + r, col + 16 * c + i);
+                asm("" : "+v"(at));
+                w[r] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(buf, at, 0, 0));
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                // Outside the matrix the state is 0, whatever its accumulator holds.
+                const bool in = 16 * k + 4 * g + r < rows && col + 16 * c + i < cols;
+                sum = __builtin_fmaf(in ? S[k][c][r] : 0.f, w[r], sum);
+            }
+        }
+    return sum;
+}
 
-// The wave's C x 16 NC outputs to rows of T, or of float32 (F32). Rows of 16-bit types in 16-byte pieces go through the
-// wave's own columns of a tile that no other wave reads any more.
+// The wave's C x 16 NC outputs to rows of T, or of float32 (F32). In 16-byte pieces (VEC) they go
+// through the wave's own columns of a tile that no other wave reads any more: 16-bit rows as they lie there, float32 rows half a
+// chunk at a time, each in the place of two rows of the tile. (float32 by the lane instead cost dk's walk 5,000 of 21,000 cycles
+// per chunk.)
 template <typename T, int C, int NC, int LDV, bool VEC, bool F32>
 __device__ __forceinline__ void store_out(const f32x4 (&O)[C / 16][NC], void *out, int64_t stride, int64_t t0, int rows, int cols, int col0,
                                           u16 *tile, int col, int lane) {
@@ -755,6 +793,32 @@ __device__ __forceinline__ void store_out(const f32x4 (&O)[C / 16][NC], void *ou
             const bool live = row < rows && col0 + col + c < cols;
             __builtin_amdgcn_raw_buffer_store_b128(w, buf, live ? uint32_t(row) * step + uint32_t(col0 + col + c) * 2 : kNone, 0, 0);
         }
+    } else if constexpr (VEC) {
+        constexpr int PR = 4 * NC, TH = C / 32;   // pieces of a row, row tiles of half a chunk
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int t = 0; t < TH; ++t)
+#pragma unroll
+                for (int c = 0; c < NC; ++c)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        // element x of row n: row 2 n + x / (8 NC), column 2 (x mod 8 NC) of the tile
+                        const int n = 4 * g + r, x = 16 * c + i;
+                        *reinterpret_cast<float *>(tile + block<LDV>(32 * t) + at<LDV>(2 * n + x / (8 * NC), col + x % (8 * NC) * 2)) =
+                            O[h * TH + t][c][r];
+                    }
+#pragma unroll
+            for (int m = 0; m < C / 2 * PR / 64; ++m) {
+                const int q = m * 64 + lane, n = q / PR, x = q % PR * 4;
+                const int row = 2 * n + x / (8 * NC), cc = col + x % (8 * NC) * 2;
+                const uint2 w0 = *reinterpret_cast<const uint2 *>(tile + at<LDV>(row, cc)), w1 = *reinterpret_cast<const uint2 *>(tile + at<LDV>(row, cc + 4));
+                const u32x4 w = {w0.x, w0.y, w1.x, w1.y};
+                const int to = h * (C / 2) + n;
+                const bool live = to < rows && col0 + col + x < cols;
+                __builtin_amdgcn_raw_buffer_store_b128(w, buf, live ? uint32_t(to) * step + uint32_t(col0 + col + x) * 4 : kNone, 0, 0);
+            }
+        }
     } else {
 #pragma unroll
         for (int t = 0; t < C / 16; ++t)
@@ -773,28 +837,33 @@ __device__ __forceinline__ void store_out(const f32x4 (&O)[C / 16][NC], void *ou
     }
 }
 
-// dot[n] = sum over the wave's columns of O[n][x] Z[n][x], into part[n] (lanes i == 0 write).
+// dot[n] = sum over the wave's columns of O[n][x] Z[n][x], into part[n] (lanes i == 0 write). A transposed read of Z has O's layout.
 template <typename T, int C, int NC, int LDZ>
 __device__ __forceinline__ void dot_rows(const f32x4 (&O)[C / 16][NC], const u16 *Z, int col, float *part, int lane) {
     constexpr int PL = kTile<C, LDZ>, PI = Cfg<T>::in;
     const int g = (lane >> 4), i = (lane & 15);
 #pragma unroll
-    for (int t = 0; t < C / 16; ++t) {
-        f32x4 s;
+    for (int j = 0; j < C / 32; ++j) {
+        float s[8] = {};
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            float x = 0.f;
+        for (int c = 0; c < NC; ++c) {
+            float z[8], y[8];
+            unpack_frag(frag_tr<LDZ>(Z + (PI - 1) * PL, 32 * j, col + 16 * c, g, i), z);
 #pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                const u16 *z = Z + block<LDZ>(16 * t) + at<LDZ>(4 * g + r, col + 16 * c + i);
-                float y = 0.f;
+            for (int p = PI - 2; p >= 0; --p) {
+                unpack_frag(frag_tr<LDZ>(Z + p * PL, 32 * j, col + 16 * c, g, i), y);
 #pragma unroll
-                for (int p = PI - 1; p >= 0; --p) y += __uint_as_float(uint32_t(z[p * PL]) << 16);
-                x = __builtin_fmaf(O[t][c][r], y, x);
+                for (int e = 0; e < 8; ++e) z[e] += y[e];
             }
-            s[r] = group_sum<16>(x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[e] = __builtin_fmaf(O[2 * j + e / 4][c][e % 4], z[e], s[e]);
         }
-        if (i == 0) *reinterpret_cast<f32x4 *>(part + 16 * t + 4 * g) = s;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[e] = group_sum<16>(s[e]);
+        if (i == 0) {
+            *reinterpret_cast<f32x4 *>(part + 32 * j + 4 * g) = f32x4{s[0], s[1], s[2], s[3]};
+            *reinterpret_cast<f32x4 *>(part + 32 * j + 16 + 4 * g) = f32x4{s[4], s[5], s[6], s[7]};
+        }
     }
 }
 
