@@ -112,6 +112,9 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(K
         if constexpr (DOT) sz.store(Z, tid);
         const bool more = t0 + C < tend;
         const int next = int(min(int64_t(C), tend - t0 - C));
+        // The next chunk's loads go out between the steps, a tensor at a time (float32: at once, its walk is bound elsewhere).
+        constexpr bool kSpread = sizeof(T) == 2;
+        if (!kSpread && more) load(t0 + C);
         __syncthreads();
         fresh();
         const Decays<C> &d = dec[buf];
@@ -131,13 +134,12 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(K
                 case 2: tiles(Tiles<0, 0>{});
             }
         }
-        // The next chunk's loads go out between the steps, a tensor at a time.
-        if (more) sx.load(rx, t0 + C, next, tid);
+        if (kSpread && more) sx.load(rx, t0 + C, next, tid);
         f32x4 O[C / 16][NC];
         fresh();
         inter<T, C, KD, NC, DOT ? 3 : PS>(O, S, X, d.in, lane);
         if constexpr (DOT) dot_rows<T, C, NC, LDV>(O, Z, col, part + wave * C, lane);
-        if (more) sy.load(ry, t0 + C, next, tid);
+        if (kSpread && more) sy.load(ry, t0 + C, next, tid);
         if (wave == dwave && more) {
             make_decays<C>(dec[buf ^ 1], decode_g(gnext, a.gtype), a.scale, lane);
             if (t0 + 2 * C < tend) gnext = decay(t0 + 2 * C);
@@ -152,7 +154,7 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(K
                 a.e[bh * a.seqlen + t0 + tid] = e;
             }
         }
-        if (more) {
+        if (kSpread && more) {
             sv.load(rv, t0 + C, next, tid);
             if constexpr (DOT) sz.load(rz, t0 + C, next, tid);
         }
