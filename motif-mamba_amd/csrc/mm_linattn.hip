@@ -254,8 +254,8 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(s
 // its own with the same barriers.
 //
 // Every q, k, v and dout row is read once for both. One workgroup of 8 waves per CU (90 KB of LDS and 200 to 250 registers at
-// dk 128), 9 us per 64 tokens with dv 64, half of the waves' time waiting: 8 x 2,048 tokens, 24 heads, 291 us; 4 x 4,096 tokens,
-// 16 heads with dv 128, 181 us.
+// dk 128), 7.5 us per 64 tokens with dv 64, bound by vector instructions (some 1,050 per wave and chunk, two waves per SIMD):
+// 8 x 2,048 tokens, 24 heads, 242 us; 4 x 4,096 tokens, 16 heads with dv 128, 161 us.
 //
 // PREC: float32 results come from the state too (the decays' gradient, the initial state's): three planes where 16-bit
 // gradients alone need two. FOR_K: the walk of dk, X = v, Y = do, V = q; else that of dv, X = k, Y = q, V = do. KX: X's padded row length, KV: V's.

@@ -760,6 +760,13 @@ __device__ __forceinline__ float dot_state(const f32x4 (&S)[KD / 16][NC], const 
     return sum;
 }
 
+// Orders a wave's LDS accesses of different types around it (they are in order in the hardware; the compiler may take a store
+// of one type and a load of another for independent).
+__device__ __forceinline__ void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // The wave's C x 16 NC outputs to rows of T, or of float32 (F32). In 16-byte pieces (VEC) they go
 // through the wave's own columns of a tile that no other wave reads any more: 16-bit rows as they lie there, the 16-bit types'
 // float32 shares half a chunk at a time, each row in the place of two rows of the tile. float32 tensors' rows go out by the lane, in
@@ -771,6 +778,7 @@ __device__ __forceinline__ void store_out(const f32x4 (&O)[C / 16][NC], void *ou
     constexpr uint32_t ES = F32 ? 4 : sizeof(T);
     const __amdgpu_buffer_rsrc_t buf = buffer(static_cast<char *>(out) + t0 * stride * ES);
     const uint32_t step = uint32_t(stride) * ES;
+    if constexpr (VEC && sizeof(T) == 2) wave_fence();
     if constexpr (VEC && !F32 && sizeof(T) == 2) {
 #pragma unroll
         for (int t = 0; t < C / 16; ++t)
@@ -782,6 +790,7 @@ __device__ __forceinline__ void store_out(const f32x4 (&O)[C / 16][NC], void *ou
                     tile[block<LDV>(16 * t) + at<LDV>(4 * g + r, col + 16 * c + i)] = u16(w);
                     tile[block<LDV>(16 * t) + at<LDV>(4 * g + r + 1, col + 16 * c + i)] = u16(w >> 16);
                 }
+        wave_fence();
         constexpr int PR = 2 * NC;   // pieces of a row
 #pragma unroll
         for (int n = 0; n < C * PR / 64; ++n) {
@@ -808,6 +817,7 @@ __device__ __forceinline__ void store_out(const f32x4 (&O)[C / 16][NC], void *ou
                         *reinterpret_cast<float *>(tile + block<LDV>(32 * t) + at<LDV>(2 * n + x / (8 * NC), col + x % (8 * NC) * 2)) =
                             O[h * TH + t][c][r];
                     }
+            wave_fence();
 #pragma unroll
             for (int m = 0; m < C / 2 * PR / 64; ++m) {
                 const int q = m * 64 + lane, n = q / PR, x = q % PR * 4;
@@ -818,6 +828,7 @@ __device__ __forceinline__ void store_out(const f32x4 (&O)[C / 16][NC], void *ou
                 const bool live = to < rows && col0 + col + x < cols;
                 __builtin_amdgcn_raw_buffer_store_b128(w, buf, live ? uint32_t(to) * step + uint32_t(col0 + col + x) * 4 : kNone, 0, 0);
             }
+            wave_fence();
         }
     } else {
 #pragma unroll
