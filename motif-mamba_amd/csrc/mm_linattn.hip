@@ -41,13 +41,13 @@ __device__ __forceinline__ Rows<T> rows_of(const View &v, int64_t b, int64_t h, 
 // Three workgroups at 168 registers spill (457 us for 128 heads against 365), chunks of 32 tokens gain nothing (394).
 template <typename T, int KD, int NC, bool DOT, bool VEC, bool F32>
 __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(KD * NC == 64 ? 3 : 2, KD * NC == 64 ? 3 : 2))) la_walk(const WalkArgs a) {
-    constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, PS = Cfg<T>::st, W = 64 * NC;
+    constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, W = 64 * NC;
     constexpr int LDX = KD, LDV = W, LDM = kScoreRow;
     typedef Stage<T, C, KD, kThreads, VEC> SX;
     typedef Stage<T, C, W, kThreads, VEC> SV;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     u16 *X = reinterpret_cast<u16 *>(smem), *Y = X + PI * kTile<C, LDX>, *V = Y + PI * kTile<C, LDX>;
-    u16 *M = V + PI * kTile<C, LDV>, *Z = M + PS * kTile<C, LDM>;
+    u16 *M = V + PI * kTile<C, LDV>, *Z = M + kPlanes * kTile<C, LDM>;
     Decays<C> *dec = reinterpret_cast<Decays<C> *>(Z + (DOT ? PI * kTile<C, LDV> : 0));
     float *part = reinterpret_cast<float *>(dec + 2);
 
@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(K
     f32x4 S[KD / 16][NC];
     load_state<KD, NC>(S, Mat{a.s0.p ? a.s0.p + (bh * a.segs + seg) * a.s0_step : nullptr, a.s0.row, a.s0.col}, a.kdim, a.cdim,
                        col0 + col, lane);
-    zero_masked_scores<C, PS>(M, false, tid, kThreads);
+    zero_masked_scores<C>(M, false, tid, kThreads);
 
     SX sx, sy;
     SV sv, sz;
@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(K
         if (kSpread && more) sx.load(rx, t0 + C, next, tid);
         f32x4 O[C / 16][NC];
         fresh();
-        inter<T, C, KD, NC, DOT ? 3 : PS>(O, S, X, d.in, lane);
+        inter<T, C, KD, NC>(O, S, X, d.in, lane);
         if constexpr (DOT) dot_rows<T, C, NC, LDV>(O, Z, col, part + wave * C, lane);
         if (kSpread && more) sy.load(ry, t0 + C, next, tid);
         if (wave == dwave && more) {
@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(K
         bf16x8 v[C / 32][NC][PI];
         load_v<T, C, NC, LDV>(v, V, col, lane);
         intra<T, C, NC, LDV, false>(O, v, M, V, col, lane);
-        update<T, C, KD, NC, Cfg<T>::up>(S, v, Y, d.out, d.all, lane);
+        update<T, C, KD, NC>(S, v, Y, d.out, d.all, lane);
         fresh();
         store_out<T, C, NC, LDV, VEC, F32>(O, static_cast<char *>(a.out) + (b * a.out_batch + h * a.out_head) * int64_t(F32 ? 4 : sizeof(T)),
                                            a.out_seq, t0, rows, a.cdim, col0, V, col, lane);
@@ -238,7 +238,7 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(s
         const Decays<C> &d = dec[buf];
         bf16x8 v[C / 32][1][PI];
         load_v<T, C, 1, LDV>(v, V, col, lane);
-        update<T, C, KD, 1, Cfg<T>::up>(S, v, Y, REV ? d.in : d.out, d.all, lane);
+        update<T, C, KD, 1>(S, v, Y, REV ? d.in : d.out, d.all, lane);
         if (wave == 0 && n + 1 < chunks) {
             decays(buf ^ 1, gnext);
             if (n + 2 < chunks) gnext = decay(n + 2);
@@ -257,9 +257,8 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(s
 // dk 128), 7.5 us per 64 tokens with dv 64, bound by vector instructions (some 1,050 per wave and chunk, two waves per SIMD):
 // 8 x 2,048 tokens, 24 heads, 242 us; 4 x 4,096 tokens, 16 heads with dv 128, 161 us.
 //
-// PREC: float32 results come from the state too (the decays' gradient, the initial state's): three planes where 16-bit
-// gradients alone need two. FOR_K: the walk of dk, X = v, Y = do, V = q; else that of dv, X = k, Y = q, V = do. KX: X's padded row length, KV: V's.
-template <typename T, int KD, int VD, bool VEC, bool F32, bool PREC, bool FOR_K>
+// FOR_K: the walk of dk, X = v, Y = do, V = q; else that of dv, X = k, Y = q, V = do. KX: X's padded row length, KV: V's.
+template <typename T, int KD, int VD, bool VEC, bool F32, bool FOR_K>
 __device__ __forceinline__ void bwd_walk(const BwdArgs &a, char *smem, int tid, int wave, int lane) {
     constexpr bool kTight = KD + VD > 128;   // registers
     auto fresh = [&] {
@@ -268,14 +267,14 @@ __device__ __forceinline__ void bwd_walk(const BwdArgs &a, char *smem, int tid, 
             lane = tid & 63;
         }
     };
-    constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, PS = Cfg<T>::st, NT2 = 2 * kThreads;
+    constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, NT2 = 2 * kThreads;
     constexpr int LDK = KD, LDV = VD, LDM = kScoreRow, CT = C / 16;
     constexpr int KX = FOR_K ? VD : KD, NC = (FOR_K ? KD : VD) / 64, LDC = FOR_K ? LDK : LDV;
     typedef Stage<T, C, KD, NT2, VEC> SK;
     typedef Stage<T, C, VD, NT2, VEC> SV;
     u16 *Q = reinterpret_cast<u16 *>(smem), *K = Q + PI * kTile<C, LDK>, *V = K + PI * kTile<C, LDK>, *G = V + PI * kTile<C, LDV>;
-    u16 *M1 = G + PI * kTile<C, LDV>, *M2 = M1 + PS * kTile<C, LDM>;
-    Decays<C> *dec = reinterpret_cast<Decays<C> *>(M2 + PS * kTile<C, LDM>);
+    u16 *M1 = G + PI * kTile<C, LDV>, *M2 = M1 + kPlanes * kTile<C, LDM>;
+    Decays<C> *dec = reinterpret_cast<Decays<C> *>(M2 + kPlanes * kTile<C, LDM>);
     float *rowp = reinterpret_cast<float *>(dec + 2), *colp = rowp + CT * C, *part = colp + CT * C;
 
     int64_t id = blockIdx.x;
@@ -299,12 +298,12 @@ __device__ __forceinline__ void bwd_walk(const BwdArgs &a, char *smem, int tid, 
         sum = wave_sum(sum);
         if (lane == 0) a.y[(bh * a.blocks + m) * kWaves + wave - kWaves] = sum;
     };
-    if constexpr (FOR_K && PREC) {
+    if constexpr (FOR_K) {
         if (a.ck && a.has_last && seg == a.segs - 1) boundary(a.blocks - 1);
     }
 
-    zero_masked_scores<C, PS>(M1, true, tid, NT2);
-    zero_masked_scores<C, PS>(M2, true, tid, NT2);
+    zero_masked_scores<C>(M1, true, tid, NT2);
+    zero_masked_scores<C>(M2, true, tid, NT2);
     SK sq, sk;
     SV sv, sd;
     auto start = [&](int64_t n) { return tbeg + (chunks - 1 - n) * C; };
@@ -343,7 +342,7 @@ __device__ __forceinline__ void bwd_walk(const BwdArgs &a, char *smem, int tid, 
         fresh();
         const Decays<C> &d = dec[buf];
         auto tiles = [&](auto L) {
-            scores_bwd<T, C, KD, VD, decltype(L)>(d, Q, K, V, G, M1, M2, a.scale, PREC && a.a != nullptr, rowp, colp, lane);
+            scores_bwd<T, C, KD, VD, decltype(L)>(d, Q, K, V, G, M1, M2, a.scale, a.a != nullptr, rowp, colp, lane);
         };
         if constexpr (C == 64) {
             switch (wave) {
@@ -365,8 +364,8 @@ __device__ __forceinline__ void bwd_walk(const BwdArgs &a, char *smem, int tid, 
         if (more) sq.load(rq, tn, C, tid);
         f32x4 O[CT][NC];
         fresh();
-        inter<T, C, KX, NC, FOR_K && PREC ? 3 : PS>(O, S, FOR_K ? V : K, d.out, lane);
-        if constexpr (FOR_K && PREC) {
+        inter<T, C, KX, NC>(O, S, FOR_K ? V : K, d.out, lane);
+        if constexpr (FOR_K) {
             if (a.a) dot_rows<T, C, NC, LDK>(O, K, col, part + (wave - kWaves) * C, lane);
         }
         if (more) sk.load(rk, tn, C, tid);
@@ -376,7 +375,7 @@ __device__ __forceinline__ void bwd_walk(const BwdArgs &a, char *smem, int tid, 
         }
         __syncthreads();
         fresh();
-        if constexpr (!FOR_K && PREC) {
+        if constexpr (!FOR_K) {
             if (a.a && tid < rows) {
                 const int t = tid / 16;
                 float sum = 0.f, f = 0.f;
@@ -396,14 +395,12 @@ __device__ __forceinline__ void bwd_walk(const BwdArgs &a, char *smem, int tid, 
         bf16x8 v[C / 32][NC][PI];
         load_v<T, C, NC, LDC>(v, VT, col, lane);
         intra<T, C, NC, LDC, true>(O, v, FOR_K ? M2 : M1, VT, col, lane);
-        update<T, C, KX, NC, PREC ? Cfg<T>::up : PS>(S, v, FOR_K ? G : Q, d.in, d.all, lane);
+        update<T, C, KX, NC>(S, v, FOR_K ? G : Q, d.in, d.all, lane);
         fresh();
         if constexpr (FOR_K) {
             store_out<T, C, NC, LDC, VEC, F32>(O, static_cast<char *>(a.dk_out) + (b * a.seqlen * a.heads + h) * a.dk * int64_t(F32 ? 4 : sizeof(T)),
                                                a.heads * a.dk, t0, rows, a.dk, 0, K, col, lane);
-            if constexpr (PREC) {
-                if (a.ck && t0 > 0 && t0 % kBlock == 0) boundary(t0 / kBlock - 1);
-            }
+            if (a.ck && t0 > 0 && t0 % kBlock == 0) boundary(t0 / kBlock - 1);
         } else {
             store_out<T, C, NC, LDC, VEC, false>(O, reinterpret_cast<T *>(a.dv_out) + (b * a.seqlen * a.heads + h) * a.dv, a.heads * a.dv, t0, rows,
                                                  a.dv, 0, V, col, lane);
@@ -414,12 +411,12 @@ __device__ __forceinline__ void bwd_walk(const BwdArgs &a, char *smem, int tid, 
     }
 }
 
-template <typename T, int KD, int VD, bool VEC, bool F32, bool PREC>
+template <typename T, int KD, int VD, bool VEC, bool F32>
 __global__ void __launch_bounds__(2 * kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) la_bwd(const BwdArgs a) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid & 63;
-    if (wave < kWaves) bwd_walk<T, KD, VD, VEC, F32, PREC, false>(a, smem, tid, wave, lane);
-    else bwd_walk<T, KD, VD, VEC, F32, PREC, true>(a, smem, tid, wave, lane);
+    if (wave < kWaves) bwd_walk<T, KD, VD, VEC, F32, false>(a, smem, tid, wave, lane);
+    else bwd_walk<T, KD, VD, VEC, F32, true>(a, smem, tid, wave, lane);
 }
 
 // Launches with `bytes` of dynamic LDS, which a kernel is allowed once per device (`done`: a bit per device).
@@ -440,8 +437,8 @@ static int launch_kernel(K kernel, int bytes, std::atomic<uint64_t> &done, int64
 
 template <typename T, int KD, int NC, bool DOT, bool VEC, bool F32>
 static int launch_walk_t(const WalkArgs &a, hipStream_t s) {
-    constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, PS = Cfg<T>::st;
-    constexpr int bytes = 2 * (2 * PI * kTile<C, KD> + (DOT ? 2 : 1) * PI * kTile<C, 64 * NC> + PS * kTile<C, kScoreRow>) +
+    constexpr int C = Cfg<T>::C, PI = Cfg<T>::in;
+    constexpr int bytes = 2 * (2 * PI * kTile<C, KD> + (DOT ? 2 : 1) * PI * kTile<C, 64 * NC> + kPlanes * kTile<C, kScoreRow>) +
                           2 * int(sizeof(Decays<C>)) + (DOT ? 4 * kWaves * C : 0);
     static_assert(bytes <= 160 * 1024, "LDS");
     const auto kernel = la_walk<T, KD, NC, DOT, VEC, F32>;
@@ -476,25 +473,20 @@ static int launch_segments_k(const WalkArgs &a, bool rev, hipStream_t s) {
     return rev ? launch_segments_t<T, KD, true, false>(a, s) : launch_segments_t<T, KD, false, false>(a, s);
 }
 
-template <typename T, int KD, int VD, bool VEC, bool F32, bool PREC>
+template <typename T, int KD, int VD, bool VEC, bool F32>
 static int launch_bwd_t(const BwdArgs &a, hipStream_t s) {
-    constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, PS = Cfg<T>::st;
-    constexpr int bytes = 2 * (2 * PI * kTile<C, KD> + 2 * PI * kTile<C, VD> + 2 * PS * kTile<C, kScoreRow>) +
+    constexpr int C = Cfg<T>::C, PI = Cfg<T>::in;
+    constexpr int bytes = 2 * (2 * PI * kTile<C, KD> + 2 * PI * kTile<C, VD> + 2 * kPlanes * kTile<C, kScoreRow>) +
                           2 * int(sizeof(Decays<C>)) + 4 * (2 * (C / 16) * C + kWaves * C);
     static_assert(bytes <= 160 * 1024, "LDS");
-    const auto kernel = la_bwd<T, KD, VD, VEC, F32, PREC>;
+    const auto kernel = la_bwd<T, KD, VD, VEC, F32>;
     static std::atomic<uint64_t> done{0};
     return launch_kernel(kernel, bytes, done, a.batch * a.heads * a.segs, 2 * kThreads, a, s, "la_bwd");
 }
 template <typename T, int KD, int VD, bool F32>
 static int launch_bwd_f(const BwdArgs &a, hipStream_t s) {
     const bool vec = a.q.vec && a.k.vec && a.v.vec && a.dout.vec && a.out_vec;
-    // float32 inputs take three planes everywhere.
-    const bool prec = sizeof(T) == 4 || a.a || a.dr;
-    if constexpr (sizeof(T) == 2) {
-        if (!prec) return vec ? launch_bwd_t<T, KD, VD, true, F32, false>(a, s) : launch_bwd_t<T, KD, VD, false, F32, false>(a, s);
-    }
-    return vec ? launch_bwd_t<T, KD, VD, true, F32, true>(a, s) : launch_bwd_t<T, KD, VD, false, F32, true>(a, s);
+    return vec ? launch_bwd_t<T, KD, VD, true, F32>(a, s) : launch_bwd_t<T, KD, VD, false, F32>(a, s);
 }
 template <typename T, int KD, int VD>
 static int launch_bwd_k(const BwdArgs &a, hipStream_t s) {

@@ -12,9 +12,11 @@
 //
 // Exactness. Products run on v_mfma_f32_16x16x32_bf16, which multiplies bfloat16 exactly and adds in
 // float32. Every other number is carried as a sum of bfloat16 planes: float16 inputs as two and float32
-// inputs as three (both exact), the state and the decayed scores as two (relative error 2^-17, three for
-// float32 inputs), the decayed rows the state is built from as three (2^-25). So the state itself is
-// float32 from end to end and 16-bit outputs are rounded once.
+// inputs as three (both exact), and every float32 factor, the state, the decayed scores and the decayed rows
+// that the state is built from, as three (relative error 2^-25, for every input type). So all of them are
+// float32 from end to end and 16-bit outputs are rounded once. (Two planes, 2^-17, for the state and the scores of 16-bit
+// inputs took 316 us where three take 358, 4 x 4,096 tokens of 80 heads at 128 x 64 in bfloat16, and moved outputs near the
+// middle of two 16-bit numbers to the wrong one.)
 //
 // Lane layouts (l the lane, g = l / 16, i = l % 16; checked on the card): an accumulator tile holds column
 // i, rows 4g .. 4g + 3. An operand holds row (A) or column (B) i and eight of 32 contraction indices; the
@@ -38,11 +40,12 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
-// Planes of an input, of the state and the scores, of the update's rows; tokens of a chunk.
+// Planes of an input; tokens of a chunk.
 template <typename T> struct Cfg;
-template <> struct Cfg<bf16_t> { static constexpr int in = 1, st = 2, up = 3, C = 64; };
-template <> struct Cfg<f16_t> { static constexpr int in = 2, st = 2, up = 3, C = 32; };
-template <> struct Cfg<float> { static constexpr int in = 3, st = 3, up = 3, C = 32; };
+template <> struct Cfg<bf16_t> { static constexpr int in = 1, C = 64; };
+template <> struct Cfg<f16_t> { static constexpr int in = 2, C = 32; };
+template <> struct Cfg<float> { static constexpr int in = 3, C = 32; };
+constexpr int kPlanes = 3;       // of a float32 factor
 
 constexpr int kBlock = 256;      // tokens between two kept states (see the decays' gradient)
 
@@ -96,19 +99,18 @@ __device__ __forceinline__ int afresh_lane(int x) {
 
 // ---- planes --------------------------------------------------------------------------------------
 
-// x as a sum of N bfloat16 planes, each the nearest of what is left.
-template <int N>
+// x as a sum of bfloat16 planes, each the nearest of what is left.
 __device__ __forceinline__ void split8(const float *x, bf16x8 *out) {
     float r[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) r[i] = x[i];
 #pragma unroll
-    for (int p = 0; p < N; ++p) {
+    for (int p = 0; p < kPlanes; ++p) {
         u32x4 w;
 #pragma unroll
         for (int i = 0; i < 4; ++i) w[i] = pack_bf16x2(r[2 * i], r[2 * i + 1]);
         out[p] = __builtin_bit_cast(bf16x8, w);
-        if (p + 1 < N) {
+        if (p + 1 < kPlanes) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 r[2 * i] -= __uint_as_float(w[i] << 16);
@@ -397,13 +399,13 @@ __device__ __forceinline__ f32x4 tile_decay(const Decays<C> &d, float scale, int
 }
 
 // Four consecutive scores of row token 16 ot + i into the score tile's planes ([row token][other token]).
-template <int C, int P>
+template <int C>
 __device__ __forceinline__ void store_scores(u16 *M, const float *x, int ot, int nt, int lane) {
     constexpr int PL = kTile<C, kScoreRow>;
     u16 *dst = M + block<kScoreRow>(16 * ot) + at<kScoreRow>((lane & 15), 16 * nt + 4 * ((lane >> 4)));
     float r[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-    for (int p = 0; p < P; ++p) {
+    for (int p = 0; p < kPlanes; ++p) {
         const uint2 w = make_uint2(pack_bf16x2(r[0], r[1]), pack_bf16x2(r[2], r[3]));
         *reinterpret_cast<uint2 *>(dst + p * PL) = w;
         r[0] -= __uint_as_float(w.x << 16);
@@ -424,7 +426,7 @@ __device__ __forceinline__ void scores(const Decays<C> &d, const u16 *X, const u
         float x[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) x[r] = n == O && 4 * ((lane >> 4)) + r > (lane & 15) ? 0.f : s[j][r] * f[r];
-        store_scores<C, Cfg<T>::st>(M, x, O, n, lane);
+        store_scores<C>(M, x, O, n, lane);
     });
 }
 
@@ -450,8 +452,8 @@ __device__ __forceinline__ void scores_bwd(const Decays<C> &d, const u16 *Q, con
             w[r] = m != O || ii + r > i ? p[j][r] * s2[r] : 0.f;
             cs += w[r];
         }
-        store_scores<C, Cfg<T>::st>(M1, s1, O, m, lane);
-        store_scores<C, Cfg<T>::st>(M2, s2, O, m, lane);
+        store_scores<C>(M1, s1, O, m, lane);
+        store_scores<C>(M2, s2, O, m, lane);
         if (sums) {
             f32x4 rs;
 #pragma unroll
@@ -466,10 +468,10 @@ __device__ __forceinline__ void scores_bwd(const Decays<C> &d, const u16 *Q, con
 
 // The tiles on the masked side of the diagonal that share a 32-wide contraction with a diagonal tile are 0
 // (written once; the chunks write the other tiles only).
-template <int C, int P>
+template <int C>
 __device__ __forceinline__ void zero_masked_scores(u16 *M, bool rev, int tid, int nt) {
     constexpr int PL = kTile<C, kScoreRow>;
-    for (int x = tid; x < C / 32 * 16 * 16 * P; x += nt) {
+    for (int x = tid; x < C / 32 * 16 * 16 * kPlanes; x += nt) {
         const int p = x / (C / 32 * 256), y = x % (C / 32 * 256), pair = y / 256, r = y % 256 / 16, c = y % 16;
         const int row = 32 * pair + (rev ? 16 : 0) + r, col = 32 * pair + (rev ? 0 : 16) + c;
         M[p * PL + at<kScoreRow>(row, col)] = 0;
@@ -477,8 +479,7 @@ __device__ __forceinline__ void zero_masked_scores(u16 *M, bool rev, int tid, in
 }
 
 // O = diag(row) X S for the wave's columns, from the state S before (after, REV) the chunk.
-// PS: the state's planes.
-template <typename T, int C, int KD, int NC, int PS>
+template <typename T, int C, int KD, int NC>
 __device__ __forceinline__ void inter(f32x4 (&O)[C / 16][NC], const f32x4 (&S)[KD / 16][NC], const u16 *X, const float *row,
                                       int lane) {
     constexpr int PL = kTile<C, KD>, PI = Cfg<T>::in;
@@ -500,7 +501,7 @@ __device__ __forceinline__ void inter(f32x4 (&O)[C / 16][NC], const f32x4 (&S)[K
     for (int k = 0; k < KD / 32; ++k) {
         if (k + 1 < KD / 32) read(k + 1);
         __builtin_amdgcn_sched_barrier(0);
-        bf16x8 s[NC][PS];
+        bf16x8 s[NC][kPlanes];
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             float x[8];
@@ -509,13 +510,13 @@ __device__ __forceinline__ void inter(f32x4 (&O)[C / 16][NC], const f32x4 (&S)[K
                 x[r] = S[2 * k][c][r];
                 x[4 + r] = S[2 * k + 1][c][r];
             }
-            split8<PS>(x, s[c]);
+            split8(x, s[c]);
         }
 #pragma unroll
         for (int p = 0; p < PI; ++p)
 #pragma unroll
-            for (int q = 0; q < PS; ++q)
-                if (p + q < PS)
+            for (int q = 0; q < kPlanes; ++q)
+                if (p + q < kPlanes)
 #pragma unroll
                     for (int t = 0; t < C / 16; ++t)
 #pragma unroll
@@ -532,8 +533,8 @@ __device__ __forceinline__ void inter(f32x4 (&O)[C / 16][NC], const f32x4 (&S)[K
     }
 }
 
-// S = all S + Y^T diag(w) V for the wave's columns (V's operands in v). PU: the planes of diag(w) V.
-template <typename T, int C, int KD, int NC, int PU>
+// S = all S + Y^T diag(w) V for the wave's columns (V's operands in v).
+template <typename T, int C, int KD, int NC>
 __device__ __forceinline__ void update(f32x4 (&S)[KD / 16][NC], const bf16x8 (&v)[C / 32][NC][Cfg<T>::in], const u16 *Y,
                                        const float *w, float all, int lane) {
     constexpr int PL = kTile<C, KD>, PI = Cfg<T>::in;
@@ -548,7 +549,7 @@ __device__ __forceinline__ void update(f32x4 (&S)[KD / 16][NC], const bf16x8 (&v
     for (int j = 0; j < C / 32; ++j) {
         const f32x4 w0 = *reinterpret_cast<const f32x4 *>(w + 32 * j + 4 * g);
         const f32x4 w1 = *reinterpret_cast<const f32x4 *>(w + 32 * j + 16 + 4 * g);
-        bf16x8 u[NC][PU];
+        bf16x8 u[NC][kPlanes];
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             float x[8], y[8];
@@ -564,7 +565,7 @@ __device__ __forceinline__ void update(f32x4 (&S)[KD / 16][NC], const bf16x8 (&v
                 x[e] *= w0[e];
                 x[4 + e] *= w1[e];
             }
-            split8<PU>(x, u[c]);
+            split8(x, u[c]);
         }
         constexpr int KB = PI > 1 ? 2 : 4;   // rows of tiles read ahead
         bf16x8 a[2][KB][PI];
@@ -583,8 +584,8 @@ __device__ __forceinline__ void update(f32x4 (&S)[KD / 16][NC], const bf16x8 (&v
 #pragma unroll
             for (int p = 0; p < PI; ++p)
 #pragma unroll
-                for (int q = 0; q < PU; ++q)
-                    if (p + q < PU)
+                for (int q = 0; q < kPlanes; ++q)
+                    if (p + q < kPlanes)
 #pragma unroll
                         for (int k = 0; k < KB; ++k)
 #pragma unroll
@@ -612,7 +613,7 @@ __device__ __forceinline__ void load_v(bf16x8 (&v)[C / 32][NC][Cfg<T>::in], cons
 template <typename T, int C, int NC, int LDV, bool REV>
 __device__ __forceinline__ void intra(f32x4 (&O)[C / 16][NC], const bf16x8 (&v0)[C / 32][NC][Cfg<T>::in], const u16 *M,
                                       const u16 *V, int col, int lane) {
-    constexpr int PL = kTile<C, kScoreRow>, PI = Cfg<T>::in, PS = Cfg<T>::st;
+    constexpr int PL = kTile<C, kScoreRow>, PI = Cfg<T>::in;
     const int g = (lane >> 4), i = (lane & 15);
     typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
     u16x2 most = {0, 0};
@@ -628,18 +629,18 @@ __device__ __forceinline__ void intra(f32x4 (&O)[C / 16][NC], const bf16x8 (&v0)
     auto product = [&](const bf16x8 (&v)[C / 32][NC][PI]) {
 #pragma unroll
         for (int j = 0; j < C / 32; ++j) {
-            bf16x8 a[C / 16][PS];
+            bf16x8 a[C / 16][kPlanes];
 #pragma unroll
             for (int t = 0; t < C / 16; ++t)
                 if (REV ? 2 * j + 1 >= t : 2 * j <= t)
 #pragma unroll
-                    for (int p = 0; p < PS; ++p) a[t][p] = frag_row<kScoreRow>(M + p * PL, 16 * t, j, g, i);
+                    for (int p = 0; p < kPlanes; ++p) a[t][p] = frag_row<kScoreRow>(M + p * PL, 16 * t, j, g, i);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int p = 0; p < PS; ++p)
+            for (int p = 0; p < kPlanes; ++p)
 #pragma unroll
                 for (int q = 0; q < PI; ++q)
-                    if (p + q < PS)
+                    if (p + q < kPlanes)
 #pragma unroll
                         for (int t = 0; t < C / 16; ++t)
 #pragma unroll
@@ -682,7 +683,7 @@ __device__ __forceinline__ void intra(f32x4 (&O)[C / 16][NC], const bf16x8 (&v0)
                     if (!bad || (REV ? n < o : n > o)) continue;
                     float m = 0.f;
 #pragma unroll
-                    for (int p = PS - 1; p >= 0; --p) m += __uint_as_float(uint32_t(M[p * PL + at<kScoreRow>(o, n)]) << 16);
+                    for (int p = kPlanes - 1; p >= 0; --p) m += __uint_as_float(uint32_t(M[p * PL + at<kScoreRow>(o, n)]) << 16);
                     O[t][c][r] += m * x;
                 }
         }

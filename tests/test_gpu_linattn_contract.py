@@ -1,0 +1,76 @@
+"""GPU tests of what the linear attention's texts promise beyond its results' bounds (tests/test_gpu_linattn.py): 16-bit results
+are float32 ones rounded once."""
+import sys
+
+import pytest
+import torch
+
+from tests import linattn_ref as ref
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def _say(msg):
+    print(f"\n[gpu-case] {msg}", flush=True)
+    sys.stdout.flush()
+
+
+def _randn(r, *shape):
+    return torch.randn(*shape, generator=r)
+
+
+def _rounded_once(got, exact, size, what):
+    """|got - exact| within half a unit of got's type at the exact value, and 2^-19 of the terms: each is a product of up to
+    three factors within 2^-25 of their values, and of three exponentials of arguments up to 10 or so, 2^-24 (1 + 10 / 8) each
+    at most; the sums' own roundings are smaller. A factor in 17 bits moves every few hundredth result past it."""
+    g, e = got.detach().cpu().double(), exact.double()
+    least, half = {BF16: (-126, -8), F16: (-14, -11)}[got.dtype]
+    unit = torch.exp2(torch.floor(torch.log2(e.abs().clamp_min(2.0 ** least))) + half)
+    bad = (g - e).abs() > unit + 2.0 ** -19 * size
+    assert not bool(bad.any()), f"{what}: {int(bad.sum())} of {bad.numel()}"
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_scores_are_float32(dtype):
+    """Decays of e^-2 or so: every output is little more than its own token's score times v."""
+    _say(f"linear attention scores {dtype}")
+    from motif_mamba_amd import linear_attention_fn
+    r = torch.Generator().manual_seed(1)
+    t = {"q": _randn(r, 64, 64, 1, 1).to(dtype), "k": _randn(r, 64, 64, 1, 1).to(dtype), "v": _randn(r, 64, 64, 4, 64).to(dtype),
+         "log_decay": -2 - torch.rand(64, 64, 4, generator=r)}
+    out = linear_attention_fn(**{n: x.to(DEV) for n, x in t.items()}, scale=0.3)
+    _rounded_once(out, ref.with_grads(t, 0.3)["out"], ref.magnitudes(t, 0.3)["out"], "out")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_states_are_float32(dtype):
+    """Nothing but the state that was handed in."""
+    _say(f"linear attention states {dtype}")
+    from motif_mamba_amd import linear_attention_fn
+    r = torch.Generator().manual_seed(2)
+    t = {"q": _randn(r, 64, 64, 1, 1).to(dtype), "k": torch.zeros(64, 64, 1, 1, dtype=dtype), "v": _randn(r, 64, 64, 4, 64).to(dtype),
+         "log_decay": -0.1 * torch.rand(64, 64, 4, generator=r), "initial_state": _randn(r, 64, 4, 1, 64)}
+    out = linear_attention_fn(**{n: x.to(DEV) for n, x in t.items()}, scale=0.3)
+    _rounded_once(out, ref.with_grads(t, 0.3)["out"], ref.magnitudes(t, 0.3)["out"], "out")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("dk,dv", [(1, 64), (64, 1)])
+def test_gradients_are_float32(dtype, dk, dv):
+    """Without a gradient of the decays or of a state, the states' gradient too is float32: few terms, most of them from behind
+    the token's chunk."""
+    _say(f"linear attention gradients {dk} {dv} {dtype}")
+    from motif_mamba_amd import linear_attention_fn
+    r = torch.Generator().manual_seed(3)
+    b, L, H = 16, 130, 4
+    t = {"q": _randn(r, b, L, H, dk).to(dtype), "k": _randn(r, b, L, H, dk).to(dtype), "v": _randn(r, b, L, H, dv).to(dtype)}
+    dout = _randn(r, b, L, H, dv).to(dtype)
+    dout[:, torch.arange(L) % 65 != 64] = 0
+    g = {"log_decay": -0.02 * torch.rand(b, L, H, generator=r)}
+    leaves = {n: x.to(DEV).requires_grad_(True) for n, x in t.items()}
+    got = torch.autograd.grad(linear_attention_fn(**leaves, log_decay=g["log_decay"].to(DEV), scale=0.3), list(leaves.values()), dout.to(DEV))
+    exact, size = ref.with_grads({**t, **g}, 0.3, dout), ref.magnitudes({**t, **g}, 0.3, dout)
+    for n, x in zip(leaves, got):
+        _rounded_once(x, exact["d" + n], size["d" + n], "d" + n)
