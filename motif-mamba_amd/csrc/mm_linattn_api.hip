@@ -381,6 +381,13 @@ extern "C" int mm_linattn_bwd(const mm_linattn_bwd_params *params, void *stream)
         if (bh > 0 && p.dinitial_state)
             if (const int rc = la::launch_copy(p.dinitial_state, p.dlast_state, bh * p.dk * p.dv, s)) return rc;
         if (p.dlog_decay && p.decay_per_head && p.nheads > 0) return la::launch_zero_g(p.dlog_decay, p.gtype, p.nheads, s);
+        // Without heads nothing reaches q and k, which still have rows: empty sums.
+        const int64_t n = p.nheads == 0 ? p.batch * p.seqlen * p.n_groups * p.dk : 0;
+        if (n > 0) {
+            if (!p.dq || !p.dk_out) return set_error(MM_ERR_INVALID_ARGUMENT, "mm_linattn_bwd: dq and dk_out are required");
+            if (const int rc = la::launch_zero_g(p.dq, p.itype, n, s)) return rc;
+            return la::launch_zero_g(p.dk_out, p.itype, n, s);
+        }
         return MM_OK;
     }
     if (!p.q || !p.k || !p.v || !p.log_decay || !p.dout || !p.dq || !p.dk_out || !p.dv_out)

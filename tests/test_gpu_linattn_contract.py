@@ -74,3 +74,18 @@ def test_gradients_are_float32(dtype, dk, dv):
     exact, size = ref.with_grads({**t, **g}, 0.3, dout), ref.magnitudes({**t, **g}, 0.3, dout)
     for n, x in zip(leaves, got):
         _rounded_once(x, exact["d" + n], size["d" + n], "d" + n)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_no_heads(dtype):
+    """No head uses q and k: their gradients are empty sums, 0, whatever stood in the memory they get."""
+    _say(f"linear attention without heads {dtype}")
+    from motif_mamba_amd import linear_attention_fn
+    q, k = (torch.randn(2, 300, 1, 16, device=DEV).to(dtype).requires_grad_(True) for _ in range(2))
+    v = torch.zeros(2, 300, 0, 8, device=DEV, dtype=dtype, requires_grad=True)
+    out, last = linear_attention_fn(q, k, v, torch.zeros(2, 300, 0, device=DEV), return_last_state=True)
+    assert out.shape == (2, 300, 0, 8) and last.shape == (2, 0, 16, 8)
+    junk = [torch.full((2, 300, 1, 16), float("nan"), device=DEV, dtype=dtype) for _ in range(8)]
+    del junk
+    dq, dk, dv = torch.autograd.grad(out, [q, k, v], torch.zeros_like(out))
+    assert dq.shape == q.shape and not dq.any() and not dk.any() and dv.shape == v.shape
