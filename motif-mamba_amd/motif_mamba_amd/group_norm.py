@@ -11,6 +11,7 @@ from __future__ import annotations
 import torch
 from torch.autograd.function import once_differentiable
 
+from ._autograd import differentiated
 from ._native import ext
 
 _NONE, _AFTER, _BEFORE, _ACT = 0, 1, 2, 3
@@ -65,6 +66,6 @@ def group_norm_fn(x, n_groups, weight=None, bias=None, z=None, eps=1e-5, activat
         raise ValueError("x must be (..., channels), and z must have its shape")
     gate = (_AFTER if norm_before_gate else _BEFORE) if z is not None else _ACT if activation else _NONE
     args = (x, int(n_groups), weight, bias, z, float(eps), bool(is_rms_norm), gate)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, z)):
+    if differentiated(x, weight, bias, z):
         return GroupNormFn.apply(*args)
     return _forward(*args)[4]

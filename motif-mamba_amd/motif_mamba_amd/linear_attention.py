@@ -22,6 +22,7 @@ from __future__ import annotations
 import torch
 from torch.autograd.function import once_differentiable
 
+from ._autograd import differentiated
 from ._native import ext
 
 
@@ -84,7 +85,7 @@ def linear_attention_fn(q, k, v, log_decay, scale=None, initial_state=None, retu
     if v.dim() != 4:
         raise ValueError("v must have shape (batch, seqlen, nheads, dv)")
     args = (q, k, v, log_decay, _scale(scale, q), initial_state, return_last_state)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, log_decay, initial_state)):
+    if differentiated(q, k, v, log_decay, initial_state):
         return LinearAttentionFn.apply(*args)
     return _forward(*args)[5]
 

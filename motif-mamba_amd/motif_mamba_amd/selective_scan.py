@@ -41,6 +41,7 @@ import os
 import torch
 from einops import rearrange
 
+from ._autograd import differentiated
 from ._native import ext
 
 
@@ -287,11 +288,11 @@ def selective_scan_fn(u, delta, A, B, C, D=None, z=None, delta_bias=None, delta_
     pq = P is not None or Q is not None or gamma is not None
     if pq:
         _check_pq(u, delta, A, B, C, P, Q)
-    # Without a gradient to take (grad mode off, or no input that requires one) the inference
+    # Without a derivative to take (grad mode off, or no input that requires one; no tangent) the inference
     # forward runs directly, without the autograd Function's own host cost (~5 us per call; the
     # Motif decode step calls the P/Q scan once per layer and token, mamba_simplemotif.py:378-396).
     grads = (u, delta, A, B, C, D, z, delta_bias) + ((P, Q) if pq else ())
-    if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in grads):
+    if not differentiated(*grads):
         return _infer(u, delta, A, B, C, D, z, delta_bias, delta_softplus, return_last_state,
                       *((P, Q, gamma) if pq else ()))
     if pq:

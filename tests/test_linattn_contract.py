@@ -1,0 +1,60 @@
+"""CPU tests of how the linear attention's and the group norm's entry points treat autograd, with a stand-in for the extension
+where a call would reach it."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+
+class _Ext:
+    """Outputs of the right shapes."""
+
+    def linattn_fwd(self, q, k, v, g, scale, initial, last, keep):
+        return [torch.zeros_like(v), *([torch.zeros(v.shape[0], v.shape[2], q.shape[3], v.shape[3])] if last else []),
+                *([None] if keep else [])]
+
+    def group_norm_fwd(self, x, *rest):
+        return torch.zeros_like(x)
+
+
+def _calls(monkeypatch):
+    from motif_mamba_amd import group_norm, linear_attention, selective_scan
+    monkeypatch.setattr(linear_attention, "ext", _Ext)
+    monkeypatch.setattr(group_norm, "ext", _Ext)
+
+    monkeypatch.setattr(selective_scan, "_infer", lambda u, *rest: torch.zeros_like(u))
+    x, s = torch.randn(1, 4, 2, 8), torch.randn(1, 2, 8, 8)
+    g = -torch.rand(1, 4, 2)
+    at = [dict(q=x, k=x, v=x, log_decay=g, initial_state=s)] * 5
+    for n, t in zip(("q", "k", "v", "log_decay", "initial_state"), at):
+        yield f"linear attention {n}", t[n], lambda y, n=n, t=t: linear_attention.linear_attention_fn(**{**t, n: y})
+    r, w = torch.randn(3, 8), torch.randn(8)
+    for n, y in (("x", r), ("weight", w), ("bias", w), ("z", r)):
+        args = dict(x=r, n_groups=2, weight=w, bias=w, z=r)
+        yield f"group norm {n}", y, lambda y, n=n, args=args: group_norm.group_norm_fn(**{**args, n: y})
+    u, A, B = torch.randn(1, 2, 4), -torch.rand(2, 3), torch.randn(1, 3, 4)
+    yield "scan u", u, lambda y: selective_scan.selective_scan_fn(y, u, A, B, B)
+
+
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_derivatives_are_refused(monkeypatch, grad):
+    """A tangent needs no requires_grad: without this the call returned outputs that had none."""
+    for what, x, call in _calls(monkeypatch):
+        with torch.set_grad_enabled(grad), forward_ad.dual_level():
+            dual = forward_ad.make_dual(x, torch.ones_like(x))
+            try:
+                call(dual)
+            except (RuntimeError, NotImplementedError):
+                continue
+            pytest.fail(what)
+
+
+def test_without_derivatives_the_call_goes_past_autograd(monkeypatch):
+    for what, x, call in _calls(monkeypatch):
+        if what.startswith("scan"):
+            continue
+        assert call(x).grad_fn is None, what
+        with forward_ad.dual_level():
+            assert call(x).grad_fn is None, what
+        with torch.no_grad():
+            assert call(x.clone().requires_grad_(True)).grad_fn is None, what
+        assert call(x.clone().requires_grad_(True)).grad_fn is not None, what
