@@ -81,7 +81,8 @@ typedef struct mm_linattn_update_params {
     mm_dtype itype;              /* q, k, v, out */
     mm_dtype gtype;              /* log_decay */
     float scale;
-    float *state;                /* (batch, nheads, dk, dv), read and written; the last dimension contiguous */
+    float *state;                /* (batch, nheads, dk, dv), read and written; the last dimension contiguous, no two
+                                  * elements in one place */
     const void *q, *k;           /* (batch, n_groups, dk) */
     const void *v;               /* (batch, nheads, dv) */
     const void *log_decay;       /* (batch, nheads); strides may be 0 */

@@ -178,6 +178,22 @@ static bool near(std::initializer_list<int64_t> strides) {
     return true;
 }
 
+// No two elements of a state lie in one place: workgroups write them in any order. Each dimension has to step over all that the
+// smaller ones span, as views of a contiguous tensor by slices and transposes do.
+static bool apart(const mm_linattn_update_params &p) {
+    int64_t size[4] = {p.batch, p.nheads, p.dk, p.dv}, step[4] = {p.state_batch_stride, p.state_head_stride, p.state_dk_stride, 1};
+    int order[4] = {0, 1, 2, 3};
+    for (int64_t &s : step) s = s < 0 ? -s : s;
+    std::sort(order, order + 4, [&](int a, int b) { return step[a] < step[b]; });
+    int64_t span = 0;
+    for (const int d : order) {
+        if (size[d] <= 1) continue;
+        if (step[d] <= span) return false;
+        span += (size[d] - 1) * step[d];
+    }
+    return true;
+}
+
 static int64_t fwd_bytes(const mm_linattn_fwd_params &p, int segs) {
     return segs > 1 ? pad16(p.batch * p.nheads * segs * p.dk * p.dv * 4) + pad16(p.batch * p.nheads * segs * 4) : 0;
 }
@@ -411,6 +427,7 @@ extern "C" int mm_linattn_update(const mm_linattn_update_params *params, void *s
     if (p.batch * p.nheads == 0) return MM_OK;
     if (!p.state || !p.q || !p.k || !p.v || !p.log_decay || !p.out)
         return set_error(MM_ERR_INVALID_ARGUMENT, "mm_linattn_update: state, q, k, v, log_decay and out are required");
+    if (!la::apart(p)) return set_error(MM_ERR_INVALID_ARGUMENT, "mm_linattn_update: elements of the state overlap");
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     switch (p.itype) {
         case MM_FLOAT32: return la::launch_update<float>(p, s);

@@ -908,6 +908,9 @@ at::Tensor linattn_update(const at::Tensor &state, const at::Tensor &q, const at
     check_decay(g, {batch, heads}, v);
     check_state(state, v, batch, heads, dk, dv, "state");
     TORCH_CHECK(state.stride(-1) == 1 || dv == 1, "state must be contiguous along its last dimension");
+    for (const auto *t : {&state, &q, &k, &v, &g})
+        TORCH_CHECK(!(at::GradMode::is_enabled() && t->requires_grad()) && !t->_fw_grad(0).defined(),
+                    "linear_attention_update has no derivatives: call it under torch.no_grad() or on detached tensors");
     const c10::DeviceGuard device_guard{v.device()};
     at::Tensor out = torch::empty({batch, heads, dv}, v.options());
     mm_linattn_update_params p;
@@ -925,6 +928,8 @@ at::Tensor linattn_update(const at::Tensor &state, const at::Tensor &q, const at
     p.v_batch_stride = v.stride(0); p.v_head_stride = v.stride(1);
     p.g_batch_stride = g.stride(0); p.g_head_stride = g.stride(1);
     check_rc(mm_linattn_update(&p, c10::hip::getCurrentHIPStream().stream()), "mm_linattn_update");
+    // The state is not what an autograd node may have saved any more.
+    if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();
     return out;
 }
 

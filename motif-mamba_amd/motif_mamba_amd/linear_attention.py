@@ -93,7 +93,8 @@ def linear_attention_fn(q, k, v, log_decay, scale=None, initial_state=None, retu
 def linear_attention_update(state, q, k, v, log_decay, scale=None):
     """One token. state: (batch, nheads, dk, dv) float32, updated in place (its last dimension contiguous);
     q, k: (batch, n_groups, dk); v: (batch, nheads, dv); log_decay: (batch, nheads) or (nheads,). Returns
-    out (batch, nheads, dv) in v's dtype. Calls on one state must be ordered."""
+    out (batch, nheads, dv) in v's dtype. Calls on one state must be ordered. No derivatives: inputs that require a gradient are
+    refused in grad mode, and the state's version counts the update, so that a backward which needs what stood there raises."""
     if v.dim() != 3:
         raise ValueError("v must have shape (batch, nheads, dv)")
     g, _ = _spread(log_decay, v.shape[:1], v)

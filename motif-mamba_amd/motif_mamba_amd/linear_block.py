@@ -10,6 +10,7 @@ import torch
 from torch import nn
 from torch.nn import functional as F
 
+from ._autograd import differentiated
 from .causal_conv1d import causal_conv1d_fn, causal_conv1d_update
 from .group_norm import group_norm_fn
 from .linear_attention import linear_attention_fn, linear_attention_update
@@ -71,7 +72,10 @@ class LinearAttentionBlock(nn.Module):
         return self._finish(y, z)
 
     def step(self, hidden, cache):
-        """hidden: (batch, d_model), one token; the cache is updated in place."""
+        """hidden: (batch, d_model), one token; the cache is updated in place. Not differentiable: under torch.no_grad()."""
+        # Before anything is written.
+        if differentiated(hidden, *self.parameters()):
+            raise RuntimeError("step has no derivatives: call it under torch.no_grad()")
         conv_state, state = cache
         z, xbc, dt = self._split(self.in_proj(hidden))
         conv = causal_conv1d_update(xbc.contiguous(), conv_state, self.conv_weight, self.conv_bias, activation="silu")

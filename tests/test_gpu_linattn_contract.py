@@ -89,3 +89,61 @@ def test_no_heads(dtype):
     del junk
     dq, dk, dv = torch.autograd.grad(out, [q, k, v], torch.zeros_like(out))
     assert dq.shape == q.shape and not dq.any() and not dk.any() and dv.shape == v.shape
+
+
+def _token(seed=4):
+    r = torch.Generator().manual_seed(seed)
+    t = {"q": _randn(r, 2, 5, 1, 16), "k": _randn(r, 2, 5, 1, 16), "v": _randn(r, 2, 5, 2, 8), "log_decay": -torch.rand(2, 5, 2, generator=r)}
+    return {n: x.to(DEV) for n, x in t.items()}, _randn(r, 2, 2, 16, 8).to(DEV)
+
+
+def test_update_counts_as_a_change_of_the_state():
+    """A state that a backward still needs is updated: an error, as with torch's own in-place operations."""
+    _say("linear attention update: version")
+    from motif_mamba_amd import linear_attention_fn, linear_attention_update
+    t, state = _token()
+    q = t["q"].clone().requires_grad_(True)
+    out = linear_attention_fn(q, t["k"], t["v"], t["log_decay"], initial_state=state)
+    before = state._version
+    linear_attention_update(state, *(t[n][:, 0] for n in ("q", "k", "v", "log_decay")))
+    assert state._version == before + 1
+    with pytest.raises(RuntimeError, match="inplace"):
+        out.sum().backward()
+    with torch.inference_mode():
+        s = torch.zeros_like(state)
+        linear_attention_update(s, *(t[n][:, 0] for n in ("q", "k", "v", "log_decay")))
+        assert s.any()
+
+
+@pytest.mark.parametrize("which", ["state", "q", "k", "v", "log_decay"])
+def test_update_refuses_derivatives(which):
+    _say(f"linear attention update: {which} with a derivative")
+    from torch.autograd import forward_ad
+    from motif_mamba_amd import linear_attention_update
+    t, state = _token()
+    args = {"state": state, **{n: x[:, 0].clone() for n, x in t.items()}}
+    leaf = {**args, which: args[which].clone().requires_grad_(True)}
+    with pytest.raises(RuntimeError, match="derivatives"):
+        linear_attention_update(**leaf)
+    with torch.no_grad():
+        assert not linear_attention_update(**leaf).requires_grad
+    with forward_ad.dual_level(), pytest.raises(RuntimeError, match="derivatives"):
+        linear_attention_update(**{**args, which: forward_ad.make_dual(args[which], torch.ones_like(args[which]))})
+
+
+def test_block_step_refuses_derivatives():
+    """In grad mode, before the cache is touched: the operators of one token have no derivatives."""
+    _say("linear attention block: step in grad mode")
+    from motif_mamba_amd import LinearAttentionBlock
+    torch.manual_seed(5)
+    b = LinearAttentionBlock(32, nheads=2, headdim=16, d_state=16).to(DEV)
+    cache = b.allocate_inference_cache(2)
+    with pytest.raises(RuntimeError, match="derivatives"):
+        b.step(torch.randn(2, 32, device=DEV), cache)
+    assert not cache[0].any() and not cache[1].any()
+    with torch.no_grad():
+        b.step(torch.randn(2, 32, device=DEV), cache)
+    assert cache[0].any() and cache[1].any()
+    for p in b.parameters():
+        p.requires_grad_(False)
+    b.step(torch.randn(2, 32, device=DEV), cache)

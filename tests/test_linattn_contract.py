@@ -1,8 +1,10 @@
 """CPU tests of how the linear attention's and the group norm's entry points treat autograd, with a stand-in for the extension
-where a call would reach it."""
+where a call would reach it, and of requests that their C entries refuse."""
 import pytest
 import torch
 from torch.autograd import forward_ad
+
+from tests.test_linattn_capi import PTRS, SIZES, _call, _fill, blocks  # noqa: F401
 
 
 class _Ext:
@@ -58,3 +60,15 @@ def test_without_derivatives_the_call_goes_past_autograd(monkeypatch):
         with torch.no_grad():
             assert call(x.clone().requires_grad_(True)).grad_fn is None, what
         assert call(x.clone().requires_grad_(True)).grad_fn is not None, what
+
+
+TOKEN = {**{n: x for n, x in {**SIZES, **PTRS}.items() if n != "seqlen"}, "state": 4096, "out": 4096}
+
+
+@pytest.mark.parametrize("strides", [(0, 256, 16), (512, 0, 16), (512, 256, 0), (512, 256, 15), (512, 255, 16), (256, 512, 8), (500, 256, 16),
+                                     (-256, 256, 16)])
+def test_update_refuses_states_that_overlap(blocks, strides):
+    """batch 2, 2 heads, 16 x 16: an expanded state would be written by several workgroups at once."""
+    names = ("state_batch_stride", "state_head_stride", "state_dk_stride")
+    rc, msg = _call("mm_linattn_update", _fill(blocks, "mm_linattn_update_params", **TOKEN, **dict(zip(names, strides))))
+    assert rc == -1 and "overlap" in msg, (rc, msg)
