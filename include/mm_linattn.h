@@ -10,7 +10,8 @@
  * the single-token form on a kept state.
  *
  * log_decay is meant to be <= 0. -inf forgets the state (a document's first token); values below -128
- * count as -128, whose exponential is 0 in float32. NaN stays NaN.
+ * count as -128, whose exponential is 0 in float32, values above 128 as 128, whose exponential is infinite. NaN stays
+ * NaN.
  *
  * Conventions as in mm_scan.h: device pointers, element strides, outputs allocated by the caller, nothing
  * is synchronised or allocated, 0 or a code of mm_scan.h is returned and mm_last_error() has the text. The

@@ -73,17 +73,18 @@ __device__ __forceinline__ uint32_t load_g_raw(const void *p, mm_dtype t, int64_
 }
 __device__ __forceinline__ float decode_g(uint32_t w, mm_dtype t) {
     const float x = t == MM_FLOAT32 ? __uint_as_float(w) : t == MM_BFLOAT16 ? __uint_as_float(w << 16) : elem_f32<f16_t>(w);
-    // exp(-128) is 0 in float32 as every smaller decay is; a finite sum keeps the differences of two
-    // sums defined. The comparison is false for NaN, which stays.
-    return x < -128.f ? -128.f : x;
+    // exp(-128) is 0 in float32 as every smaller decay is, and exp(128) infinite; a finite sum keeps the
+    // differences of two sums defined. The comparisons are false for NaN, which stays.
+    return x < -128.f ? -128.f : x > 128.f ? 128.f : x;
 }
 
-// exp(x): 2^(x log2 e) with the product's rounding error and log2 e's own taken back in (v_exp_f32 is within 1 ulp).
+// exp(x): 2^(x log2 e) with the product's rounding error and log2 e's own taken back in (v_exp_f32 is within 1 ulp). An infinite
+// result has no correction: infinity less a part of itself is NaN.
 __device__ __forceinline__ float exp_f32(float x) {
     const float p = x * kLog2e;
     const float e = __builtin_fmaf(x, 1.925963033e-8f, __builtin_fmaf(x, kLog2e, -p));
     const float r = __builtin_amdgcn_exp2f(p);
-    return __builtin_fmaf(r, e * kLn2, r);
+    return p < 128.f ? __builtin_fmaf(r, e * kLn2, r) : r;
 }
 
 // A number that the compiler does not know to be the one it was: what is computed from it is computed where it is used,
@@ -316,7 +317,7 @@ __device__ __forceinline__ void make_decays(Decays<C> &d, float g, float scale, 
     const int I = lane >> 2 & 3, J = lane & 3;
     const double mid = shfl_f64(c, 16 * I - 1 & 63) - shfl_f64(c, 16 * J + 15);
     const float hi = float(c);
-    const float in = exp_f32(hi + float(c - double(hi))), out = exp_f32(float(all - c)), from = exp_f32(float(c - (tile ? before : 0.0))),
+    const float in = exp_f32(hi), out = exp_f32(float(all - c)), from = exp_f32(float(c - (tile ? before : 0.0))),
                 to = exp_f32(float(end - c)), m = exp_f32(float(mid));
     if (C == 64 || lane < C) {
         d.in[lane] = in * scale;

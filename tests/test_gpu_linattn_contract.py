@@ -147,3 +147,20 @@ def test_block_step_refuses_derivatives():
     for p in b.parameters():
         p.requires_grad_(False)
     b.step(torch.randn(2, 32, device=DEV), cache)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("grow", [88.8, 90.0, 1000.0, float("inf")])
+def test_growing_states(dtype, grow):
+    """A log decay whose exponential is infinite makes the state infinite, not NaN."""
+    _say(f"linear attention log decay {grow} {dtype}")
+    from motif_mamba_amd import linear_attention_fn, linear_attention_update
+    r = torch.Generator().manual_seed(6)
+    t = {"q": _randn(r, 1, 1, 1, 1).abs().to(dtype), "k": _randn(r, 1, 1, 1, 1).to(dtype), "v": _randn(r, 1, 1, 2, 16).to(dtype),
+         "log_decay": torch.full((1, 1, 2), grow), "initial_state": 1 + torch.rand(1, 2, 1, 16, generator=r)}
+    d = {n: x.to(DEV) for n, x in t.items()}
+    out, last = linear_attention_fn(**d, return_last_state=True)
+    assert torch.isposinf(out).all() and torch.isposinf(last).all()
+    state = d["initial_state"].clone()
+    out = linear_attention_update(state, *(d[n][:, 0] for n in ("q", "k", "v", "log_decay")))
+    assert torch.isposinf(out).all() and torch.isposinf(state).all()
