@@ -13,6 +13,10 @@
  * count as -128, whose exponential is 0 in float32, values above 128 as 128, whose exponential is infinite. NaN stays
  * NaN.
  *
+ * Infinities: the outputs and states of mm_linattn_fwd and mm_linattn_update, and dq, are what the recurrence makes of them,
+ * +-infinity or NaN; in the other gradients what they reach is NaN or infinite. Rows that hold one take some six times as long
+ * in mm_linattn_fwd.
+ *
  * Conventions as in mm_scan.h: device pointers, element strides, outputs allocated by the caller, nothing
  * is synchronised or allocated, 0 or a code of mm_scan.h is returned and mm_last_error() has the text. The
  * innermost dimension (dk or dv) of q, k, v, dout and of every output is contiguous; states are contiguous

@@ -24,12 +24,92 @@ namespace la {
 constexpr int kWaves = 4, kThreads = 64 * kWaves;
 
 template <typename T>
-__device__ __forceinline__ Rows<T> rows_of(const View &v, int64_t b, int64_t h, int d, int col0) {
+__device__ __forceinline__ Rows<T> rows_of(const View &v, int64_t b, int64_t h, int d, int col0 = 0) {
     return Rows<T>{reinterpret_cast<const T *>(v.p) + b * v.batch + (h / v.share) * v.head + col0, v.seq, d - col0};
 }
 
-// Forward walk: out = scale (masked X Y^T) V + ..., KD the padded length of X's rows, 64 NC columns of V per
-// workgroup, 16 NC per wave. DOT: also e[t] = (the product with the state alone) . Z_t, and the state at every
+// The walk once more by the recurrence, for what is not finite in it (see mm_linattn_dev.h). Its arguments are read again, so that
+// nothing of it takes registers while the products run.
+template <typename T, int KD, int NC, bool DOT, bool VEC, bool F32>
+__device__ __forceinline__ void infinite_rows(char *smem) {
+    constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, W = 64 * NC, ES = F32 ? 4 : sizeof(T);
+    typedef const __attribute__((address_space(4))) WalkArgs *Args;
+    Args args = (Args)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(args));
+    const WalkArgs a = *(const WalkArgs *)args;
+    u16 *X = reinterpret_cast<u16 *>(smem), *Y = X + PI * kTile<C, KD>, *V = Y + PI * kTile<C, KD>;
+    Decays<C> *dec = reinterpret_cast<Decays<C> *>(V + (DOT ? 2 : 1) * PI * kTile<C, W> + kPlanes * kTile<C, kScoreRow>);
+    const int tid = afresh_lane(threadIdx.x), wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid & 63, col = wave * 16 * NC;
+    int64_t id = afresh(blockIdx.x);
+    const int seg = id % a.segs; id /= a.segs;
+    const int64_t h = id % a.heads, b = id / a.heads, bh = b * a.heads + h;
+    const int64_t tbeg = int64_t(seg) * a.seg_len, tend = min(a.seqlen, tbeg + a.seg_len);
+    const Rows<T> rx = rows_of<T>(a.x, b, h, a.kdim), ry = rows_of<T>(a.y, b, h, a.kdim), rv = rows_of<T>(a.v, b, h, a.cdim);
+    f32x4 S[KD / 16][NC];
+    auto begin = [&] {
+        load_state<KD, NC>(S, Mat{a.s0.p ? a.s0.p + (bh * a.segs + seg) * a.s0_step : nullptr, a.s0.row, a.s0.col}, a.kdim, a.cdim, col, lane);
+    };
+    auto stage = [&](int64_t t0, int rows) {
+        __syncthreads();
+        {
+            Stage<T, C, KD, kThreads, VEC> s;
+            s.load(rx, t0, rows, tid);
+            s.store(X, tid);
+            s.load(ry, t0, rows, tid);
+            s.store(Y, tid);
+        }
+        {
+            Stage<T, C, W, kThreads, VEC> s;
+            s.load(rv, t0, rows, tid);
+            s.store(V, tid);
+        }
+        if (wave == 0) {
+            const int64_t t = t0 + lane;
+            const uint32_t g = lane < C && t < tend ? load_g_raw(a.g, a.gtype, b * a.g_batch + h * a.g_head + t * a.g_seq) : 0u;
+            make_decays<C>(dec[0], decode_g(g, a.gtype), a.scale, lane);
+        }
+        __syncthreads();
+    };
+    // NaN alone needs no second look.
+    begin();
+    Kinds seen = kinds<KD, NC>(S);
+#pragma unroll 1
+    for (int64_t t0 = tbeg; t0 < tend; t0 += C) {
+        stage(t0, int(min(int64_t(C), tend - t0)));
+        seen.tile<C, KD>(X, lane);
+        seen.tile<C, KD>(Y, lane);
+        seen.tile<C, W>(V, lane);
+        seen.add(dec[0].hi[C - 1]);
+    }
+    const bool inf = __syncthreads_or(seen.inf), nan = __syncthreads_or(seen.nan);
+    if (nan && !inf) return;
+    begin();
+    auto keep = [&](int64_t block) {
+        store_state<KD, NC, true>(S, Mat{a.ck + (bh * a.blocks + block) * a.kdim * a.cdim, a.cdim, 1}, a.kdim, a.cdim, col, lane);
+    };
+#pragma unroll 1
+    for (int64_t t0 = tbeg; t0 < tend; t0 += C) {
+        const int rows = int(min(int64_t(C), tend - t0));
+        if constexpr (DOT) {
+            if (a.ck && t0 > 0 && t0 % kBlock == 0) keep(t0 / kBlock - 1);
+        }
+        stage(t0, rows);
+        const __amdgpu_buffer_rsrc_t to = buffer(static_cast<char *>(a.out) + (b * a.out_batch + h * a.out_head + t0 * a.out_seq) * ES);
+        recur<T, C, KD, NC, W, true>(S, X, Y, V, dec[0], rows, a.kdim, col, lane, [&](int t, int c, float x) {
+            x *= a.scale;
+            const int at = col + 16 * c + (lane & 15);
+            store_element<T, F32>(x, to, !finite(x) && lane < 16 && at < a.cdim ? uint32_t(t) * uint32_t(a.out_seq) + uint32_t(at) : kNone);
+        });
+    }
+    if (a.s1.p && seg == a.segs - 1)
+        store_state<KD, NC, true>(S, Mat{a.s1.p + bh * a.kdim * a.cdim, a.s1.row, a.s1.col}, a.kdim, a.cdim, col, lane);
+    if constexpr (DOT) {
+        if (a.ck && a.ck_last && seg == a.segs - 1) keep(a.blocks - 1);
+    }
+}
+
+// Forward walk: out = scale (masked X Y^T) V + ..., KD the padded length of X's rows, 64 NC that of V's,
+// 16 NC columns per wave. DOT: also e[t] = (the product with the state alone) . Z_t, and the state at every
 // kBlock-th token into ck (the decays' gradient).
 //
 // Per chunk: stage X, Y and V; scores (each wave its tiles, into M) and the product with the state; the product of M and V,
@@ -51,30 +131,27 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(K
     Decays<C> *dec = reinterpret_cast<Decays<C> *>(Z + (DOT ? PI * kTile<C, LDV> : 0));
     float *part = reinterpret_cast<float *>(dec + 2);
 
-    constexpr bool kTight = true;
     int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
     auto fresh = [&] {
-        if constexpr (kTight) {
-            tid = afresh_lane(tid);
-            lane = tid & 63;
-        }
+        tid = afresh_lane(tid);
+        lane = tid & 63;
     };
     int64_t id = blockIdx.x;
-    const int slice = id % a.slices; id /= a.slices;
     const int seg = id % a.segs; id /= a.segs;
     const int64_t h = id % a.heads, b = id / a.heads, bh = b * a.heads + h;
     const int64_t tbeg = int64_t(seg) * a.seg_len, tend = min(a.seqlen, tbeg + a.seg_len);
-    const int col0 = slice * W, col = wave * 16 * NC;
+    const int col = wave * 16 * NC;
 
-    const Rows<T> rx = rows_of<T>(a.x, b, h, a.kdim, 0), ry = rows_of<T>(a.y, b, h, a.kdim, 0);
-    const Rows<T> rv = rows_of<T>(a.v, b, h, a.cdim, col0), rz = rows_of<T>(a.z, b, h, a.cdim, col0);
+    const Rows<T> rx = rows_of<T>(a.x, b, h, a.kdim), ry = rows_of<T>(a.y, b, h, a.kdim);
+    const Rows<T> rv = rows_of<T>(a.v, b, h, a.cdim), rz = rows_of<T>(a.z, b, h, a.cdim);
     const int64_t g0 = b * a.g_batch + h * a.g_head;
 
     f32x4 S[KD / 16][NC];
     load_state<KD, NC>(S, Mat{a.s0.p ? a.s0.p + (bh * a.segs + seg) * a.s0_step : nullptr, a.s0.row, a.s0.col}, a.kdim, a.cdim,
-                       col0 + col, lane);
+                       col, lane);
     zero_masked_scores<C>(M, false, tid, kThreads);
+    bool special = false;   // something in X or Y was not finite
 
     SX sx, sy;
     SV sv, sz;
@@ -102,7 +179,7 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(K
         if constexpr (DOT) {
             if (a.ck && t0 > 0 && t0 % kBlock == 0)
                 store_state<KD, NC>(S, Mat{a.ck + (bh * a.blocks + t0 / kBlock - 1) * a.kdim * a.cdim, a.cdim, 1}, a.kdim, a.cdim,
-                                    col0 + col, lane);
+                                    col, lane);
         }
         __syncthreads();
         fresh();
@@ -119,7 +196,7 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(K
         fresh();
         const Decays<C> &d = dec[buf];
         // The score tiles, static for each wave; the last one, which also makes the next chunk's decays, has the fewest.
-        auto tiles = [&](auto L) { scores<T, C, KD, decltype(L)>(d, X, Y, M, a.scale, lane); };
+        auto tiles = [&](auto L) { special |= scores<T, C, KD, decltype(L)>(d, X, Y, M, a.scale, lane); };
         if constexpr (C == 64) {
             switch (wave) {
                 case 0: tiles(Tiles<3, 0, 3, 1, 3, 2>{}); break;
@@ -164,15 +241,18 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(K
         update<T, C, KD, NC>(S, v, Y, d.out, d.all, lane);
         fresh();
         store_out<T, C, NC, LDV, VEC, F32>(O, static_cast<char *>(a.out) + (b * a.out_batch + h * a.out_head) * int64_t(F32 ? 4 : sizeof(T)),
-                                           a.out_seq, t0, rows, a.cdim, col0, V, col, lane);
+                                           a.out_seq, t0, rows, a.cdim, V, col, lane);
     }
     if (a.s1.p && seg == a.segs - 1)
-        store_state<KD, NC>(S, Mat{a.s1.p + bh * a.kdim * a.cdim, a.s1.row, a.s1.col}, a.kdim, a.cdim, col0 + col, lane);
+        store_state<KD, NC>(S, Mat{a.s1.p + bh * a.kdim * a.cdim, a.s1.row, a.s1.col}, a.kdim, a.cdim, col, lane);
     if constexpr (DOT) {
         // The state after the last token, for the product with the last state's gradient.
         if (a.ck && a.ck_last && seg == a.segs - 1)
-            store_state<KD, NC>(S, Mat{a.ck + (bh * a.blocks + a.blocks - 1) * a.kdim * a.cdim, a.cdim, 1}, a.kdim, a.cdim, col0 + col, lane);
+            store_state<KD, NC>(S, Mat{a.ck + (bh * a.blocks + a.blocks - 1) * a.kdim * a.cdim, a.cdim, 1}, a.kdim, a.cdim, col, lane);
     }
+
+    // A state that is not finite stays so: what made it so is seen at the end.
+    if (__syncthreads_or(special || !finite_state<KD, NC>(S))) infinite_rows<T, KD, NC, DOT, VEC, F32>(smem);
 }
 
 // What each segment but the last one (REV: the first one) of a row adds to the state: sum of y_t (decay to the
@@ -216,9 +296,11 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(s
     };
     // The next chunk's decays are made by one wave while the others work on this one's state.
     double total = 0.0;
+    bool cut = false;   // a token's own decay is 0
     auto decays = [&](int buf, uint32_t w) {
-        make_decays<C>(dec[buf], decode_g(w, a.gtype), a.scale, lane);
-        total += double(dec[buf].hi[C - 1]) + double(dec[buf].lo[C - 1]);
+        const float g = decode_g(w, a.gtype);
+        total += make_decays<C>(dec[buf], g, a.scale, lane);
+        cut |= exp_f32(g) == 0.f;
     };
     uint32_t gnext = 0;
     load(0);
@@ -244,8 +326,51 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(s
             if (n + 2 < chunks) gnext = decay(n + 2);
         }
     }
+    if constexpr (!REV) {
+        // What an infinity reached, by the recurrence, as behind the walk.
+        if (__syncthreads_or(!finite_state<KD, 1>(S))) {
+            auto again = [&](int64_t n) {
+                __syncthreads();
+                load(n);
+                sy.store(Y, tid);
+                sv.store(V, tid);
+                if (wave == 0) make_decays<C>(dec[0], decode_g(decay(n), a.gtype), a.scale, lane);
+                __syncthreads();
+            };
+            Kinds seen = {false, false};
+#pragma unroll 1
+            for (int64_t n = 0; n < chunks; ++n) {
+                again(n);
+                seen.tile<C, KD>(Y, lane);
+                seen.tile<C, W>(V, lane);
+                seen.add(dec[0].hi[C - 1]);
+            }
+            const bool inf = __syncthreads_or(seen.inf), nan = __syncthreads_or(seen.nan);
+            if (inf || !nan) {
+                f32x4 R[KD / 16][1];
+                load_state<KD, 1>(R, Mat{nullptr, 0, 0}, 0, 0, 0, lane);
+#pragma unroll 1
+                for (int64_t n = 0; n < chunks; ++n) {
+                    again(n);
+                    recur<T, C, KD, 1, LDV, false>(R, nullptr, Y, V, dec[0], int(min(int64_t(C), tend - start(n))), a.kdim, col, lane,
+                                                   [](int, int, float) {});
+                }
+#pragma unroll
+                for (int k = 0; k < KD / 16; ++k)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (!finite(S[k][0][r])) S[k][0][r] = R[k][0][r];
+            }
+        }
+    }
     store_state<KD, 1>(S, Mat{a.st + (bh * a.segs + seg) * a.kdim * a.cdim, a.cdim, 1}, a.kdim, a.cdim, col0 + col, lane);
-    if (slice == 0 && tid == 0) a.seg_decay[bh * a.segs + seg] = exp_f32(float(total));
+    // A decay that no token's own makes 0 is not 0: an infinite state stays infinite in any number of segments. (Nothing finite
+    // changes by 2^-126 of a state.)
+    cut = __any(cut);
+    if (slice == 0 && tid == 0) {
+        const float d = exp_f32(float(total));
+        a.seg_decay[bh * a.segs + seg] = !cut && d < 1.17549435e-38f ? 1.17549435e-38f : d;
+    }
 }
 
 // Backward walk from the end: dv, dk, the scores' part of the decays' gradient (a), the state's part (f), and at
@@ -282,8 +407,8 @@ __device__ __forceinline__ void bwd_walk(const BwdArgs &a, char *smem, int tid, 
     const int64_t h = id % a.heads, b = id / a.heads, bh = b * a.heads + h;
     const int64_t tbeg = int64_t(seg) * a.seg_len, tend = min(a.seqlen, tbeg + a.seg_len);
     const int64_t chunks = (tend - tbeg + C - 1) / C;
-    const Rows<T> rq = rows_of<T>(a.q, b, h, a.dk, 0), rk = rows_of<T>(a.k, b, h, a.dk, 0);
-    const Rows<T> rv = rows_of<T>(a.v, b, h, a.dv, 0), rd = rows_of<T>(a.dout, b, h, a.dv, 0);
+    const Rows<T> rq = rows_of<T>(a.q, b, h, a.dk), rk = rows_of<T>(a.k, b, h, a.dk);
+    const Rows<T> rv = rows_of<T>(a.v, b, h, a.dv), rd = rows_of<T>(a.dout, b, h, a.dv);
     const int64_t g0 = b * a.g_batch + h * a.g_head;
     const int col = (wave % kWaves) * 16 * NC, rows_s = FOR_K ? a.dv : a.dk, cols_s = FOR_K ? a.dk : a.dv;
 
@@ -399,11 +524,11 @@ __device__ __forceinline__ void bwd_walk(const BwdArgs &a, char *smem, int tid, 
         fresh();
         if constexpr (FOR_K) {
             store_out<T, C, NC, LDC, VEC, F32>(O, static_cast<char *>(a.dk_out) + (b * a.seqlen * a.heads + h) * a.dk * int64_t(F32 ? 4 : sizeof(T)),
-                                               a.heads * a.dk, t0, rows, a.dk, 0, K, col, lane);
+                                               a.heads * a.dk, t0, rows, a.dk, K, col, lane);
             if (a.ck && t0 > 0 && t0 % kBlock == 0) boundary(t0 / kBlock - 1);
         } else {
             store_out<T, C, NC, LDC, VEC, false>(O, reinterpret_cast<T *>(a.dv_out) + (b * a.seqlen * a.heads + h) * a.dv, a.heads * a.dv, t0, rows,
-                                                 a.dv, 0, V, col, lane);
+                                                 a.dv, V, col, lane);
         }
     }
     if constexpr (!FOR_K) {
@@ -443,7 +568,7 @@ static int launch_walk_t(const WalkArgs &a, hipStream_t s) {
     static_assert(bytes <= 160 * 1024, "LDS");
     const auto kernel = la_walk<T, KD, NC, DOT, VEC, F32>;
     static std::atomic<uint64_t> done{0};
-    return launch_kernel(kernel, bytes, done, a.batch * a.heads * a.segs * a.slices, kThreads, a, s, "la_walk");
+    return launch_kernel(kernel, bytes, done, a.batch * a.heads * a.segs, kThreads, a, s, "la_walk");
 }
 template <typename T, int KD, int NC, bool DOT>
 static int launch_walk_k(const WalkArgs &a, hipStream_t s) {

@@ -210,7 +210,7 @@ static int run_fwd(const mm_linattn_fwd_params &p, hipStream_t s) {
     a.gtype = p.gtype;
     a.g_batch = p.g_batch_stride; a.g_seq = p.g_seq_stride; a.g_head = p.g_head_stride;
     a.batch = p.batch; a.seqlen = p.seqlen; a.heads = p.nheads;
-    a.kdim = int(p.dk); a.cdim = int(p.dv); a.slices = 1;
+    a.kdim = int(p.dk); a.cdim = int(p.dv);
     segments(p.batch * p.nheads, p.seqlen, p.dk * p.dv, &a.segs, &a.seg_len);
     if (a.segs > 1 && (!p.workspace || p.workspace_bytes < fwd_bytes(p, a.segs))) {
         a.segs = 1;
@@ -304,7 +304,7 @@ static int run_bwd(const mm_linattn_bwd_params &p, hipStream_t s) {
     }
     // dq: the forward walk with (do, v, k), its state the transposed one.
     a.x = d; a.y = v; a.v = k; a.z = q;
-    a.kdim = int(p.dv); a.cdim = int(p.dk); a.slices = 1;
+    a.kdim = int(p.dv); a.cdim = int(p.dk);
     a.scale = p.scale;
     const float *start = w.segs == 1 ? p.initial_state : p.segment_states ? static_cast<const float *>(p.segment_states) : f32(w.st);
     a.s0 = State{const_cast<float *>(start), 1, p.dv};

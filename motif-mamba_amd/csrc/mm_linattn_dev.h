@@ -78,6 +78,8 @@ __device__ __forceinline__ float decode_g(uint32_t w, mm_dtype t) {
     return x < -128.f ? -128.f : x > 128.f ? 128.f : x;
 }
 
+__device__ __forceinline__ bool finite(float x) { return __builtin_fabsf(x) <= 3.402823466e38f; }
+
 // exp(x): 2^(x log2 e) with the product's rounding error and log2 e's own taken back in (v_exp_f32 is within 1 ulp). An infinite
 // result has no correction: infinity less a part of itself is NaN.
 __device__ __forceinline__ float exp_f32(float x) {
@@ -306,9 +308,9 @@ __device__ __forceinline__ double shfl_f64(double x, int lane) {
     return __builtin_bit_cast(double, uint64_t(lo) | uint64_t(hi) << 32);
 }
 
-// One wave; g: the lane's token's log decay, 0 behind the last token and in lanes past C.
+// One wave; g: the lane's token's log decay, 0 behind the last token and in lanes past C. Returns the chunk's total.
 template <int C>
-__device__ __forceinline__ void make_decays(Decays<C> &d, float g, float scale, int lane) {
+__device__ __forceinline__ double make_decays(Decays<C> &d, float g, float scale, int lane) {
     const double c = prefix_f64(double(g));
     const double all = readlane_f64(c, C - 1);
     const int tile = (lane >> 4);
@@ -329,6 +331,7 @@ __device__ __forceinline__ void make_decays(Decays<C> &d, float g, float scale, 
         if (lane == C - 1) d.all = in;
     }
     if (lane < 16 && I < C / 16 && J < I) d.mid[I][J] = m;
+    return all;
 }
 
 // ---- a chunk's steps -----------------------------------------------------------------------------
@@ -416,19 +419,23 @@ __device__ __forceinline__ void store_scores(u16 *M, const float *x, int ot, int
     }
 }
 
-// The forward walk's decayed, masked scores of the tiles L into M.
+// The forward walk's decayed, masked scores of the tiles L into M. True where a row of X or Y holds an infinity or NaN: the
+// product of a token's own two rows then is neither finite, and the tiles on the diagonal hold those.
 template <typename T, int C, int KD, typename L>
-__device__ __forceinline__ void scores(const Decays<C> &d, const u16 *X, const u16 *Y, u16 *M, float scale, int lane) {
+__device__ __forceinline__ bool scores(const Decays<C> &d, const u16 *X, const u16 *Y, u16 *M, float scale, int lane) {
     f32x4 s[L::N];
     score_tiles<T, C, KD, L>(s, X, Y, lane);
+    bool special = false;
     static_for<0, L::N>([&](auto Nc) {
         constexpr int j = decltype(Nc)::value, O = L::O(j), n = L::n(j);
+        if constexpr (O == n) special |= !finite((s[j][0] + s[j][1]) + (s[j][2] + s[j][3]));
         const f32x4 f = tile_decay<C, false, O, n>(d, scale, lane);
         float x[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) x[r] = n == O && 4 * ((lane >> 4)) + r > (lane & 15) ? 0.f : s[j][r] * f[r];
         store_scores<C>(M, x, O, n, lane);
     });
+    return special;
 }
 
 // The backward walk's, of both products (K Q^T into M1, V dO^T into M2, row token tile O), and with `sums` the tiles' sums of
@@ -690,6 +697,113 @@ __device__ __forceinline__ void intra(f32x4 (&O)[C / 16][NC], const bf16x8 (&v0)
         }
 }
 
+// ---- infinite values -----------------------------------------------------------------------------
+
+// An infinity has no planes behind the first (their rest would be infinity - infinity), and a plane that is 0 times an infinity
+// is NaN. So the products above make NaN of every output and state element that an infinity reaches, and of those alone. Which of
+// them the recurrence makes +-infinity is found by running it, token by token in float32, behind the walk over a row that holds
+// one, and what is not finite there is written over the NaN. The finite results stay as they are, and so does a row of finite
+// values and NaN. Such a row takes some six times as long.
+
+// Whether there are infinities and NaNs among the values that this lane was shown.
+struct Kinds {
+    bool inf, nan;
+
+    __device__ __forceinline__ void add(float x) {
+        inf |= __builtin_fabsf(x) == __builtin_inff();
+        nan |= x != x;
+    }
+    template <int C, int D>
+    __device__ __forceinline__ void tile(const u16 *tile, int lane) {   // the first plane; the lane's share
+        for (int x = lane; x < C * D / 4; x += 64) {
+            const int row = x / (D / 4);
+            const uint2 w = *reinterpret_cast<const uint2 *>(tile + row * D + row / 16 * 8 + x % (D / 4) * 4);
+            add(__uint_as_float(w.x << 16));
+            add(__uint_as_float(w.x & 0xffff0000u));
+            add(__uint_as_float(w.y << 16));
+            add(__uint_as_float(w.y & 0xffff0000u));
+        }
+    }
+};
+template <int KD, int NC>
+__device__ __forceinline__ Kinds kinds(const f32x4 (&S)[KD / 16][NC]) {
+    Kinds k = {false, false};
+#pragma unroll
+    for (int y = 0; y < KD / 16; ++y)
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) k.add(S[y][c][r]);
+    return k;
+}
+template <int KD, int NC>
+__device__ __forceinline__ bool finite_state(const f32x4 (&S)[KD / 16][NC]) {
+    const Kinds k = kinds<KD, NC>(S);
+    return !k.inf && !k.nan;
+}
+// Four consecutive elements of a tile's row, and one.
+template <typename T, int C, int D>
+__device__ __forceinline__ void tile_row4(float (&x)[4], const u16 *tile, int row, int col) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = 0.f;
+#pragma unroll
+    for (int p = Cfg<T>::in - 1; p >= 0; --p) {
+        const uint2 w = *reinterpret_cast<const uint2 *>(tile + p * kTile<C, D> + at<D>(row, col));
+        x[0] += __uint_as_float(w.x << 16);
+        x[1] += __uint_as_float(w.x & 0xffff0000u);
+        x[2] += __uint_as_float(w.y << 16);
+        x[3] += __uint_as_float(w.y & 0xffff0000u);
+    }
+}
+template <typename T, int C, int D>
+__device__ __forceinline__ float tile_at(const u16 *tile, int row, int col) {
+    float x = 0.f;
+#pragma unroll
+    for (int p = Cfg<T>::in - 1; p >= 0; --p) x += __uint_as_float(uint32_t(tile[p * kTile<C, D> + at<D>(row, col)]) << 16);
+    return x;
+}
+
+// A chunk's first `rows` tokens one by one: S = exp(g) S + y v^T; out(t, c, the column's x S without the scale) in every lane (OUT).
+// kdim: the rows' length; beyond it S stays 0.
+template <typename T, int C, int KD, int NC, int LDV, bool OUT, typename F>
+__device__ __forceinline__ void recur(f32x4 (&S)[KD / 16][NC], const u16 *X, const u16 *Y, const u16 *V, const Decays<C> &d, int rows, int kdim,
+                                      int col, int lane, F &&out) {
+    const int g = (lane >> 4), i = (lane & 15);
+#pragma unroll 1
+    for (int t = 0; t < rows; ++t) {
+        const float e = exp_f32(t ? (d.hi[t] - d.hi[t - 1]) + (d.lo[t] - d.lo[t - 1]) : d.hi[0] + d.lo[0]);
+        float v[NC], o[NC];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            v[c] = tile_at<T, C, LDV>(V, t, col + 16 * c + i);
+            o[c] = 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < KD / 16; ++k) {
+            float y[4], x[4];
+            tile_row4<T, C, KD>(y, Y, t, 16 * k + 4 * g);
+            if constexpr (OUT) tile_row4<T, C, KD>(x, X, t, 16 * k + 4 * g);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const bool in = 16 * k + 4 * g + r < kdim;
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    S[k][c][r] = in ? __builtin_fmaf(e, S[k][c][r], y[r] * v[c]) : 0.f;
+                    if constexpr (OUT) o[c] += in ? x[r] * S[k][c][r] : 0.f;
+                }
+            }
+        }
+        if constexpr (OUT) {
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                o[c] += __shfl_xor(o[c], 16);
+                o[c] += __shfl_xor(o[c], 32);
+                out(t, c, o[c]);
+            }
+        }
+    }
+}
+
 // A float32 matrix of a (batch row, head): rows x cols, with its strides (spans less than 2^31 bytes).
 struct Mat {
     float *p;
@@ -716,7 +830,8 @@ __device__ __forceinline__ void load_state(f32x4 (&S)[KD / 16][NC], const Mat &m
                 S[k][c][r] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(buf, at, 0, 0));
             }
 }
-template <int KD, int NC>
+// ODD: only the elements that are not finite.
+template <int KD, int NC, bool ODD = false>
 __device__ __forceinline__ void store_state(const f32x4 (&S)[KD / 16][NC], const Mat &m, int rows, int cols, int col, int lane) {
     const int g = (lane >> 4), i = (lane & 15);
     rows = afresh(rows);
@@ -729,6 +844,7 @@ __device__ __forceinline__ void store_state(const f32x4 (&S)[KD / 16][NC], const
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 uint32_t at = state_at(m, rows, cols, 16 * k + 4 * g + r, col + 16 * c + i);
+                if (ODD && finite(S[k][c][r])) at = kNone;
                 asm("" : "+v"(at));
                 __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(S[k][c][r]), buf, at, 0, 0);
             }
@@ -769,12 +885,22 @@ __device__ __forceinline__ void wave_fence() {
     __builtin_amdgcn_wave_barrier();
 }
 
+// One output element; `at` counts elements, kNone drops it.
+template <typename T, bool F32>
+__device__ __forceinline__ void store_element(float x, const __amdgpu_buffer_rsrc_t &buf, uint32_t at) {
+    constexpr uint32_t ES = F32 ? 4 : sizeof(T);
+    at = at == kNone ? kNone : at * ES;
+    if constexpr (ES == 4) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(x), buf, at, 0, 0);
+    else if constexpr (std::is_same_v<T, bf16_t>) __builtin_amdgcn_raw_buffer_store_b16(short(pack_bf16x2(x, 0.f)), buf, at, 0, 0);
+    else __builtin_amdgcn_raw_buffer_store_b16(short(pack_f16x2(x, 0.f)), buf, at, 0, 0);
+}
+
 // The wave's C x 16 NC outputs to rows of T, or of float32 (F32). In 16-byte pieces (VEC) they go
 // through the wave's own columns of a tile that no other wave reads any more: 16-bit rows as they lie there, the 16-bit types'
 // float32 shares half a chunk at a time, each row in the place of two rows of the tile. float32 tensors' rows go out by the lane, in
 // 64-byte runs (through LDS: 1,025 us against 990 for 65,536 tokens of 40 heads).
 template <typename T, int C, int NC, int LDV, bool VEC, bool F32>
-__device__ __forceinline__ void store_out(const f32x4 (&O)[C / 16][NC], void *out, int64_t stride, int64_t t0, int rows, int cols, int col0,
+__device__ __forceinline__ void store_out(const f32x4 (&O)[C / 16][NC], void *out, int64_t stride, int64_t t0, int rows, int cols,
                                           u16 *tile, int col, int lane) {
     const int g = (lane >> 4), i = (lane & 15);
     constexpr uint32_t ES = F32 ? 4 : sizeof(T);
@@ -801,8 +927,8 @@ __device__ __forceinline__ void store_out(const f32x4 (&O)[C / 16][NC], void *ou
             const uint2 w0 = *reinterpret_cast<const uint2 *>(src + at<LDV>(int(unsigned(lane) / PR), col + c)),
                         w1 = *reinterpret_cast<const uint2 *>(src + at<LDV>(int(unsigned(lane) / PR), col + c + 4));
             const u32x4 w = {w0.x, w0.y, w1.x, w1.y};
-            const bool live = row < rows && col0 + col + c < cols;
-            __builtin_amdgcn_raw_buffer_store_b128(w, buf, live ? uint32_t(row) * step + uint32_t(col0 + col + c) * 2 : kNone, 0, 0);
+            const bool live = row < rows && col + c < cols;
+            __builtin_amdgcn_raw_buffer_store_b128(w, buf, live ? uint32_t(row) * step + uint32_t(col + c) * 2 : kNone, 0, 0);
         }
     } else if constexpr (VEC && sizeof(T) == 2) {
         constexpr int PR = 4 * NC, TH = C / 32;   // pieces of a row, row tiles of half a chunk
@@ -827,8 +953,8 @@ __device__ __forceinline__ void store_out(const f32x4 (&O)[C / 16][NC], void *ou
                 const uint2 w0 = *reinterpret_cast<const uint2 *>(tile + at<LDV>(row, cc)), w1 = *reinterpret_cast<const uint2 *>(tile + at<LDV>(row, cc + 4));
                 const u32x4 w = {w0.x, w0.y, w1.x, w1.y};
                 const int to = h * (C / 2) + n;
-                const bool live = to < rows && col0 + col + x < cols;
-                __builtin_amdgcn_raw_buffer_store_b128(w, buf, live ? uint32_t(to) * step + uint32_t(col0 + col + x) * 4 : kNone, 0, 0);
+                const bool live = to < rows && col + x < cols;
+                __builtin_amdgcn_raw_buffer_store_b128(w, buf, live ? uint32_t(to) * step + uint32_t(col + x) * 4 : kNone, 0, 0);
             }
             wave_fence();
         }
@@ -840,11 +966,8 @@ __device__ __forceinline__ void store_out(const f32x4 (&O)[C / 16][NC], void *ou
                 const int n = 16 * t + 4 * g + r;
 #pragma unroll
                 for (int c = 0; c < NC; ++c) {
-                    const int x = col0 + col + 16 * c + i;
-                    const uint32_t at = n < rows && x < cols ? uint32_t(n) * step + uint32_t(x) * ES : kNone;
-                    if constexpr (ES == 4) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(O[t][c][r]), buf, at, 0, 0);
-                    else if constexpr (std::is_same_v<T, bf16_t>) __builtin_amdgcn_raw_buffer_store_b16(short(pack_bf16x2(O[t][c][r], 0.f)), buf, at, 0, 0);
-                    else __builtin_amdgcn_raw_buffer_store_b16(short(pack_f16x2(O[t][c][r], 0.f)), buf, at, 0, 0);
+                    const int x = col + 16 * c + i;
+                    store_element<T, F32>(O[t][c][r], buf, n < rows && x < cols ? uint32_t(n) * uint32_t(stride) + uint32_t(x) : kNone);
                 }
             }
     }

@@ -27,7 +27,8 @@ struct WalkArgs {
     mm_dtype gtype;
     int64_t g_batch, g_seq, g_head;
     int64_t batch, seqlen, heads;
-    int kdim, cdim, slices, segs;
+    int kdim, cdim, segs;
+    int slices;            // the segments' pass: workgroups over V's columns
     int64_t seg_len;       // tokens, a multiple of kBlock
     float scale;
     State s0;              // state the first token (or each segment) starts from, s0_step elements apart

@@ -164,3 +164,73 @@ def test_growing_states(dtype, grow):
     state = d["initial_state"].clone()
     out = linear_attention_update(state, *(d[n][:, 0] for n in ("q", "k", "v", "log_decay")))
     assert torch.isposinf(out).all() and torch.isposinf(state).all()
+
+
+def _infinite(dtype, L, dk, dv, which, bad, at, forget=(), states=True):
+    """Inputs with one infinity (or a token of them) and what the definition makes of it, in float64."""
+    r = torch.Generator().manual_seed(7 + L + dk)
+    t = {"q": _randn(r, 1, L, 1, dk).to(dtype), "k": _randn(r, 1, L, 1, dk).to(dtype), "v": _randn(r, 1, L, 2, dv).to(dtype),
+         "log_decay": -0.5 * torch.rand(1, L, 2, generator=r)}
+    if states:
+        t["initial_state"] = _randn(r, 1, 2, dk, dv)
+    clean = {n: x.clone() for n, x in t.items()}
+    for f in forget:
+        t["log_decay"][:, f] = clean["log_decay"][:, f] = float("-inf")
+    if which == "initial_state":
+        t[which][0, 0, dk // 2, dv // 3] = bad
+    elif which == "v":
+        t[which][0, at, 1, dv // 2] = bad
+    else:
+        t[which][0, at, 0, dk // 3] = bad
+    return t, clean
+
+
+def _same_kinds(got, exact, what):
+    g, e = got.cpu().double(), exact
+    for kind in (torch.isnan, torch.isposinf, torch.isneginf):
+        assert torch.equal(kind(g), kind(e)), (what, kind.__name__, int((kind(g) != kind(e)).sum()))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("which", ["q", "k", "v", "initial_state"])
+@pytest.mark.parametrize("L,dk,dv", [(1, 16, 16), (90, 64, 64), (150, 128, 128), (70, 37, 50), (1100, 64, 64), (1100, 128, 100)])
+def test_infinite_values(L, dk, dv, which, dtype):
+    """An infinity becomes what the recurrence makes of it, infinity or NaN, in outputs and states, in one segment and in several,
+    and everything that it does not reach keeps its bits."""
+    _say(f"linear attention infinite {which} {L} {dk} {dv} {dtype}")
+    from motif_mamba_amd import linear_attention_fn
+    for bad, at in ((float("inf"), 0), (float("-inf"), L // 3)):
+        t, clean = _infinite(dtype, L, dk, dv, which, bad, at)
+        out, last = linear_attention_fn(**{n: x.to(DEV) for n, x in t.items()}, scale=0.25, return_last_state=True)
+        exact = ref.recurrence(*(t[n].double() for n in ("q", "k", "v", "log_decay")), 0.25, t["initial_state"].double())
+        _same_kinds(out, exact[0], "out")
+        _same_kinds(last, exact[1], "last_state")
+        want = linear_attention_fn(**{n: x.to(DEV) for n, x in clean.items()}, scale=0.25, return_last_state=True)
+        for x, y, e in zip((out, last), want, exact):
+            assert torch.equal(x[e.isfinite().to(DEV)], y[e.isfinite().to(DEV)])
+
+
+@pytest.mark.parametrize("L", [150, 1100])
+def test_infinite_values_and_forgotten_states(L):
+    """0 times infinity is NaN in the recurrence too: -inf does not forget an infinity."""
+    _say(f"linear attention infinite v, -inf {L}")
+    from motif_mamba_amd import linear_attention_fn
+    t, _ = _infinite(BF16, L, 64, 64, "v", float("inf"), 40, forget=(20, 100))
+    out, last = linear_attention_fn(**{n: x.to(DEV) for n, x in t.items()}, return_last_state=True)
+    exact = ref.recurrence(*(t[n].double() for n in ("q", "k", "v", "log_decay")), 0.125, t["initial_state"].double())
+    _same_kinds(out, exact[0], "out")
+    _same_kinds(last, exact[1], "last_state")
+
+
+def test_infinite_values_then_tokens():
+    """The prompt and its tokens one by one agree."""
+    _say("linear attention infinite v, tokens")
+    from motif_mamba_amd import linear_attention_fn, linear_attention_update
+    t, _ = _infinite(F32, 40, 32, 32, "v", float("inf"), 10)
+    d = {n: x.to(DEV) for n, x in t.items()}
+    out, last = linear_attention_fn(**d, return_last_state=True)
+    state = d["initial_state"].clone()
+    for n in range(40):
+        y = linear_attention_update(state, *(d[m][:, n] for m in ("q", "k", "v", "log_decay")))
+        _same_kinds(out[:, n], y.cpu().double(), n)
+    _same_kinds(last, state.cpu().double(), "state")
