@@ -23,9 +23,55 @@ namespace la {
 
 constexpr int kWaves = 4, kThreads = 64 * kWaves;
 
+// The kernel's only argument, read where this stands. A walk keeps the few numbers that every chunk needs (a tensor's first
+// row and stride, 3 scalars each) and reads the others when it needs them: all of them, some 60, do not fit the scalar registers, and a
+// build that spilled them lost the low word of an output's address (a tuple of arguments was overwritten in part before it was
+// spilled; one instance of 144 stored to wrong addresses).
+template <typename A>
+__device__ __forceinline__ A own_args() {
+    typedef const __attribute__((address_space(4))) A *Args;
+    Args args = (Args)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(args));
+    return *(const A *)args;
+}
+
 template <typename T>
-__device__ __forceinline__ Rows<T> rows_of(const View &v, int64_t b, int64_t h, int d, int col0 = 0) {
-    return Rows<T>{reinterpret_cast<const T *>(v.p) + b * v.batch + (h / v.share) * v.head + col0, v.seq, d - col0};
+__device__ __forceinline__ Rows<T> rows_of(const View &v, int b, int h, int d, int col0 = 0) {
+    return Rows<T>{afresh(reinterpret_cast<const T *>(v.p) + b * v.batch + int64_t(unsigned(h) / unsigned(v.share)) * v.head + col0), uint32_t(afresh(int(v.seq) * int(sizeof(T)))), afresh(d - col0)};
+}
+// A workgroup's place: its batch row, head and segment, and the segment's tokens.
+struct Place {
+    int slice, seg, b, h, beg, end;
+};
+template <typename A>
+__device__ __forceinline__ Place place_of(const A &a, int slices) {
+    const unsigned id = unsigned(afresh(int(blockIdx.x))), seg = id / unsigned(slices), pair = seg / unsigned(a.segs);
+    Place p;
+    p.slice = afresh(int(id % unsigned(slices)));
+    p.seg = afresh(int(seg % unsigned(a.segs)));
+    p.h = afresh(int(pair % unsigned(a.heads)));
+    p.b = afresh(int(pair / unsigned(a.heads)));
+    p.beg = afresh(p.seg * int(a.seg_len));
+    p.end = afresh(min(int(a.seqlen), p.beg + int(a.seg_len)));
+    return p;
+}
+// The log decays of a (batch row, head).
+struct Gates {
+    const char *p;
+    int64_t stride;   // bytes
+    mm_dtype type;
+
+    // A lane's token's bits in the chunk at t0, 0 past `end`; see decode_g.
+    template <int C>
+    __device__ __forceinline__ uint32_t load(int t0, int end, int lane) const {
+        const int t = t0 + lane;
+        return lane < C && t < end ? load_g_raw(p + t * stride, type, 0) : 0u;
+    }
+};
+template <typename A>
+__device__ __forceinline__ Gates gates_of(const A &a, const Place &p) {
+    const int64_t size = a.gtype == MM_FLOAT32 ? 4 : 2;
+    return Gates{afresh(static_cast<const char *>(a.g) + (p.b * a.g_batch + p.h * a.g_head) * size), afresh(a.g_seq * size), mm_dtype(afresh(int(a.gtype)))};
 }
 
 // The walk once more by the recurrence, for what is not finite in it (see mm_linattn_dev.h). Its arguments are read again, so that
@@ -33,49 +79,42 @@ __device__ __forceinline__ Rows<T> rows_of(const View &v, int64_t b, int64_t h, 
 template <typename T, int KD, int NC, bool DOT, bool VEC, bool F32>
 __device__ __forceinline__ void infinite_rows(char *smem) {
     constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, W = 64 * NC, ES = F32 ? 4 : sizeof(T);
-    typedef const __attribute__((address_space(4))) WalkArgs *Args;
-    Args args = (Args)__builtin_amdgcn_kernarg_segment_ptr();
-    asm volatile("" : "+s"(args));
-    const WalkArgs a = *(const WalkArgs *)args;
+    auto args = [] { return own_args<WalkArgs>(); };
     u16 *X = reinterpret_cast<u16 *>(smem), *Y = X + PI * kTile<C, KD>, *V = Y + PI * kTile<C, KD>;
     Decays<C> *dec = reinterpret_cast<Decays<C> *>(V + (DOT ? 2 : 1) * PI * kTile<C, W> + kPlanes * kTile<C, kScoreRow>);
     const int tid = afresh_lane(threadIdx.x), wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid & 63, col = wave * 16 * NC;
-    int64_t id = afresh(blockIdx.x);
-    const int seg = id % a.segs; id /= a.segs;
-    const int64_t h = id % a.heads, b = id / a.heads, bh = b * a.heads + h;
-    const int64_t tbeg = int64_t(seg) * a.seg_len, tend = min(a.seqlen, tbeg + a.seg_len);
-    const Rows<T> rx = rows_of<T>(a.x, b, h, a.kdim), ry = rows_of<T>(a.y, b, h, a.kdim), rv = rows_of<T>(a.v, b, h, a.cdim);
+    const Place p = place_of(args(), 1);
     f32x4 S[KD / 16][NC];
     auto begin = [&] {
-        load_state<KD, NC>(S, Mat{a.s0.p ? a.s0.p + (bh * a.segs + seg) * a.s0_step : nullptr, a.s0.row, a.s0.col}, a.kdim, a.cdim, col, lane);
+        const WalkArgs a = args();
+        const int64_t bh = int64_t(p.b) * a.heads + p.h;
+        load_state<KD, NC>(S, Mat{a.s0.p ? a.s0.p + (bh * a.segs + p.seg) * a.s0_step : nullptr, a.s0.row, a.s0.col}, a.kdim, a.cdim, col, lane);
     };
-    auto stage = [&](int64_t t0, int rows) {
+    auto stage = [&](int t0) {
+        const WalkArgs a = args();
+        const int rows = min(C, p.end - t0);
         __syncthreads();
         {
             Stage<T, C, KD, kThreads, VEC> s;
-            s.load(rx, t0, rows, tid);
+            s.load(rows_of<T>(a.x, p.b, p.h, a.kdim), t0, rows, tid);
             s.store(X, tid);
-            s.load(ry, t0, rows, tid);
+            s.load(rows_of<T>(a.y, p.b, p.h, a.kdim), t0, rows, tid);
             s.store(Y, tid);
         }
         {
             Stage<T, C, W, kThreads, VEC> s;
-            s.load(rv, t0, rows, tid);
+            s.load(rows_of<T>(a.v, p.b, p.h, a.cdim), t0, rows, tid);
             s.store(V, tid);
         }
-        if (wave == 0) {
-            const int64_t t = t0 + lane;
-            const uint32_t g = lane < C && t < tend ? load_g_raw(a.g, a.gtype, b * a.g_batch + h * a.g_head + t * a.g_seq) : 0u;
-            make_decays<C>(dec[0], decode_g(g, a.gtype), a.scale, lane);
-        }
+        if (wave == 0) make_decays<C>(dec[0], decode_g(gates_of(a, p).template load<C>(t0, p.end, lane), a.gtype), a.scale, lane);
         __syncthreads();
     };
     // NaN alone needs no second look.
     begin();
     Kinds seen = kinds<KD, NC>(S);
 #pragma unroll 1
-    for (int64_t t0 = tbeg; t0 < tend; t0 += C) {
-        stage(t0, int(min(int64_t(C), tend - t0)));
+    for (int t0 = p.beg; t0 < p.end; t0 += C) {
+        stage(t0);
         seen.tile<C, KD>(X, lane);
         seen.tile<C, KD>(Y, lane);
         seen.tile<C, W>(V, lane);
@@ -84,27 +123,30 @@ __device__ __forceinline__ void infinite_rows(char *smem) {
     const bool inf = __syncthreads_or(seen.inf), nan = __syncthreads_or(seen.nan);
     if (nan && !inf) return;
     begin();
-    auto keep = [&](int64_t block) {
+    auto keep = [&](const WalkArgs &a, int64_t block) {
+        const int64_t bh = int64_t(p.b) * a.heads + p.h;
         store_state<KD, NC, true>(S, Mat{a.ck + (bh * a.blocks + block) * a.kdim * a.cdim, a.cdim, 1}, a.kdim, a.cdim, col, lane);
     };
 #pragma unroll 1
-    for (int64_t t0 = tbeg; t0 < tend; t0 += C) {
-        const int rows = int(min(int64_t(C), tend - t0));
+    for (int t0 = p.beg; t0 < p.end; t0 += C) {
         if constexpr (DOT) {
-            if (a.ck && t0 > 0 && t0 % kBlock == 0) keep(t0 / kBlock - 1);
+            const WalkArgs a = args();
+            if (a.ck && t0 > 0 && t0 % kBlock == 0) keep(a, t0 / kBlock - 1);
         }
-        stage(t0, rows);
-        const __amdgpu_buffer_rsrc_t to = buffer(static_cast<char *>(a.out) + (b * a.out_batch + h * a.out_head + t0 * a.out_seq) * ES);
-        recur<T, C, KD, NC, W, true>(S, X, Y, V, dec[0], rows, a.kdim, col, lane, [&](int t, int c, float x) {
+        stage(t0);
+        const WalkArgs a = args();
+        const __amdgpu_buffer_rsrc_t to = buffer(static_cast<char *>(a.out) + (p.b * a.out_batch + p.h * a.out_head + t0 * a.out_seq) * ES);
+        recur<T, C, KD, NC, W, true>(S, X, Y, V, dec[0], min(C, p.end - t0), a.kdim, col, lane, [&](int t, int c, float x) {
             x *= a.scale;
             const int at = col + 16 * c + (lane & 15);
             store_element<T, F32>(x, to, !finite(x) && lane < 16 && at < a.cdim ? uint32_t(t) * uint32_t(a.out_seq) + uint32_t(at) : kNone);
         });
     }
-    if (a.s1.p && seg == a.segs - 1)
-        store_state<KD, NC, true>(S, Mat{a.s1.p + bh * a.kdim * a.cdim, a.s1.row, a.s1.col}, a.kdim, a.cdim, col, lane);
+    const WalkArgs a = args();
+    if (a.s1.p && p.seg == a.segs - 1)
+        store_state<KD, NC, true>(S, Mat{a.s1.p + (int64_t(p.b) * a.heads + p.h) * a.kdim * a.cdim, a.s1.row, a.s1.col}, a.kdim, a.cdim, col, lane);
     if constexpr (DOT) {
-        if (a.ck && a.ck_last && seg == a.segs - 1) keep(a.blocks - 1);
+        if (a.ck && a.ck_last && p.seg == a.segs - 1) keep(a, a.blocks - 1);
     }
 }
 
@@ -120,7 +162,7 @@ __device__ __forceinline__ void infinite_rows(char *smem) {
 // 4 x 4,096 tokens, 80 heads: 319 us, 1.1 TB/s of its 360 MB and 400 TFLOP/s on the matrix cores, split planes counted.
 // Three workgroups at 168 registers spill (457 us for 128 heads against 365), chunks of 32 tokens gain nothing (394).
 template <typename T, int KD, int NC, bool DOT, bool VEC, bool F32>
-__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(KD * NC == 64 ? 3 : 2, KD * NC == 64 ? 3 : 2))) la_walk(const WalkArgs a) {
+__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(KD * NC == 64 ? 3 : 2, KD * NC == 64 ? 3 : 2))) la_walk(const WalkArgs) {
     constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, W = 64 * NC;
     constexpr int LDX = KD, LDV = W, LDM = kScoreRow;
     typedef Stage<T, C, KD, kThreads, VEC> SX;
@@ -137,49 +179,61 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(K
         tid = afresh_lane(tid);
         lane = tid & 63;
     };
-    int64_t id = blockIdx.x;
-    const int seg = id % a.segs; id /= a.segs;
-    const int64_t h = id % a.heads, b = id / a.heads, bh = b * a.heads + h;
-    const int64_t tbeg = int64_t(seg) * a.seg_len, tend = min(a.seqlen, tbeg + a.seg_len);
+    auto args = [] { return own_args<WalkArgs>(); };
+    const Place p = place_of(args(), 1);
     const int col = wave * 16 * NC;
 
-    const Rows<T> rx = rows_of<T>(a.x, b, h, a.kdim), ry = rows_of<T>(a.y, b, h, a.kdim);
-    const Rows<T> rv = rows_of<T>(a.v, b, h, a.cdim), rz = rows_of<T>(a.z, b, h, a.cdim);
-    const int64_t g0 = b * a.g_batch + h * a.g_head;
-
     f32x4 S[KD / 16][NC];
-    load_state<KD, NC>(S, Mat{a.s0.p ? a.s0.p + (bh * a.segs + seg) * a.s0_step : nullptr, a.s0.row, a.s0.col}, a.kdim, a.cdim,
-                       col, lane);
+    {
+        const WalkArgs a = args();
+        const int64_t bh = int64_t(p.b) * a.heads + p.h;
+        load_state<KD, NC>(S, Mat{a.s0.p ? a.s0.p + (bh * a.segs + p.seg) * a.s0_step : nullptr, a.s0.row, a.s0.col}, a.kdim, a.cdim, col, lane);
+    }
     zero_masked_scores<C>(M, false, tid, kThreads);
     bool special = false;   // something in X or Y was not finite
+    // One after the other: arguments that are read together are held together.
+    auto tensor = [&](auto of) { const WalkArgs a = args(); return of(a); };
+    const Rows<T> rx = tensor([&](const WalkArgs &a) { return rows_of<T>(a.x, p.b, p.h, a.kdim); });
+    const Rows<T> ry = tensor([&](const WalkArgs &a) { return rows_of<T>(a.y, p.b, p.h, a.kdim); });
+    const Rows<T> rv = tensor([&](const WalkArgs &a) { return rows_of<T>(a.v, p.b, p.h, a.cdim); });
+    const Rows<T> rz = DOT ? tensor([&](const WalkArgs &a) { return rows_of<T>(a.z, p.b, p.h, a.cdim); }) : rv;
+    const Gates gates = tensor([&](const WalkArgs &a) { return gates_of(a, p); });
+    const float scale = afresh(args().scale);
+    char *const out = tensor([&](const WalkArgs &a) {
+        return afresh(static_cast<char *>(a.out) + (p.b * a.out_batch + p.h * a.out_head) * int64_t(F32 ? 4 : sizeof(T)));
+    });
+    const uint32_t out_stride = uint32_t(afresh(int(args().out_seq)));
+    float *const e_out = DOT ? tensor([&](const WalkArgs &a) { return afresh(a.e + (int64_t(p.b) * a.heads + p.h) * a.seqlen); }) : nullptr;
 
     SX sx, sy;
     SV sv, sz;
-    auto load = [&](int64_t t0) {
-        const int rows = int(min(int64_t(C), tend - t0));
+    auto load = [&](int t0) {
+        const int rows = min(C, p.end - t0);
         sx.load(rx, t0, rows, tid);
         sy.load(ry, t0, rows, tid);
         sv.load(rv, t0, rows, tid);
         if constexpr (DOT) sz.load(rz, t0, rows, tid);
     };
-    auto decay = [&](int64_t t0) {
-        const int64_t t = t0 + lane;
-        return lane < C && t < tend ? load_g_raw(a.g, a.gtype, g0 + t * a.g_seq) : 0u;
+    auto make = [&](int buf, uint32_t g) { make_decays<C>(dec[buf], decode_g(g, gates.type), scale, lane); };
+    auto keep = [&](const WalkArgs &a, int64_t block) {
+        const int64_t bh = int64_t(p.b) * a.heads + p.h;
+        store_state<KD, NC>(S, Mat{a.ck + (bh * a.blocks + block) * a.kdim * a.cdim, a.cdim, 1}, a.kdim, a.cdim, col, lane);
     };
     const int dwave = kWaves - 1;
     uint32_t gnext = 0;
-    load(tbeg);
+    load(p.beg);
     if (wave == dwave) {
-        make_decays<C>(dec[0], decode_g(decay(tbeg), a.gtype), a.scale, lane);
-        if (tbeg + C < tend) gnext = decay(tbeg + C);
+        make(0, gates.template load<C>(p.beg, p.end, lane));
+        if (p.beg + C < p.end) gnext = gates.template load<C>(p.beg + C, p.end, lane);
     }
     int buf = 0;
-    for (int64_t t0 = tbeg; t0 < tend; t0 += C, buf ^= 1) {
-        const int rows = int(min(int64_t(C), tend - t0));
+    for (int t0 = p.beg; t0 < p.end; t0 += C, buf ^= 1) {
+        const int rows = min(C, p.end - t0);
         if constexpr (DOT) {
-            if (a.ck && t0 > 0 && t0 % kBlock == 0)
-                store_state<KD, NC>(S, Mat{a.ck + (bh * a.blocks + t0 / kBlock - 1) * a.kdim * a.cdim, a.cdim, 1}, a.kdim, a.cdim,
-                                    col, lane);
+            if (t0 > 0 && t0 % kBlock == 0) {
+                const WalkArgs a = args();
+                if (a.ck) keep(a, t0 / kBlock - 1);
+            }
         }
         __syncthreads();
         fresh();
@@ -187,8 +241,8 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(K
         sy.store(Y, tid);
         sv.store(V, tid);
         if constexpr (DOT) sz.store(Z, tid);
-        const bool more = t0 + C < tend;
-        const int next = int(min(int64_t(C), tend - t0 - C));
+        const bool more = t0 + C < p.end;
+        const int next = min(C, p.end - t0 - C);
         // The next chunk's loads go out between the steps, a tensor at a time (float32: at once, its walk is bound elsewhere).
         constexpr bool kSpread = sizeof(T) == 2;
         if (!kSpread && more) load(t0 + C);
@@ -196,7 +250,7 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(K
         fresh();
         const Decays<C> &d = dec[buf];
         // The score tiles, static for each wave; the last one, which also makes the next chunk's decays, has the fewest.
-        auto tiles = [&](auto L) { special |= scores<T, C, KD, decltype(L)>(d, X, Y, M, a.scale, lane); };
+        auto tiles = [&](auto L) { special |= scores<T, C, KD, decltype(L)>(d, X, Y, M, scale, lane); };
         if constexpr (C == 64) {
             switch (wave) {
                 case 0: tiles(Tiles<3, 0, 3, 1, 3, 2>{}); break;
@@ -218,8 +272,8 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(K
         if constexpr (DOT) dot_rows<T, C, NC, LDV>(O, Z, col, part + wave * C, lane);
         if (kSpread && more) sy.load(ry, t0 + C, next, tid);
         if (wave == dwave && more) {
-            make_decays<C>(dec[buf ^ 1], decode_g(gnext, a.gtype), a.scale, lane);
-            if (t0 + 2 * C < tend) gnext = decay(t0 + 2 * C);
+            make(buf ^ 1, gnext);
+            if (t0 + 2 * C < p.end) gnext = gates.template load<C>(t0 + 2 * C, p.end, lane);
         }
         __syncthreads();
         fresh();
@@ -228,7 +282,7 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(K
                 float e = 0.f;
 #pragma unroll
                 for (int w = 0; w < kWaves; ++w) e += part[w * C + tid];
-                a.e[bh * a.seqlen + t0 + tid] = e;
+                e_out[t0 + tid] = e;
             }
         }
         if (kSpread && more) {
@@ -240,15 +294,16 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(K
         intra<T, C, NC, LDV, false>(O, v, M, V, col, lane);
         update<T, C, KD, NC>(S, v, Y, d.out, d.all, lane);
         fresh();
-        store_out<T, C, NC, LDV, VEC, F32>(O, static_cast<char *>(a.out) + (b * a.out_batch + h * a.out_head) * int64_t(F32 ? 4 : sizeof(T)),
-                                           a.out_seq, t0, rows, a.cdim, V, col, lane);
+        store_out<T, C, NC, LDV, VEC, F32>(O, out, out_stride, t0, rows, rv.d, V, col, lane);
     }
-    if (a.s1.p && seg == a.segs - 1)
-        store_state<KD, NC>(S, Mat{a.s1.p + bh * a.kdim * a.cdim, a.s1.row, a.s1.col}, a.kdim, a.cdim, col, lane);
-    if constexpr (DOT) {
-        // The state after the last token, for the product with the last state's gradient.
-        if (a.ck && a.ck_last && seg == a.segs - 1)
-            store_state<KD, NC>(S, Mat{a.ck + (bh * a.blocks + a.blocks - 1) * a.kdim * a.cdim, a.cdim, 1}, a.kdim, a.cdim, col, lane);
+    {
+        const WalkArgs a = args();
+        if (a.s1.p && p.seg == a.segs - 1)
+            store_state<KD, NC>(S, Mat{a.s1.p + (int64_t(p.b) * a.heads + p.h) * a.kdim * a.cdim, a.s1.row, a.s1.col}, a.kdim, a.cdim, col, lane);
+        if constexpr (DOT) {
+            // The state after the last token, for the product with the last state's gradient.
+            if (a.ck && a.ck_last && p.seg == a.segs - 1) keep(a, a.blocks - 1);
+        }
     }
 
     // A state that is not finite stays so: what made it so is seen at the end.
@@ -259,7 +314,7 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(K
 // segment's end) v_t^T into st[bh][seg], and the segment's own decay into decay[bh][seg]. About 2 us per chunk and CU at
 // dk 128 (7 of 8 segments of 64 pairs, dv 128, L 4,096: 55 us).
 template <typename T, int KD, bool REV, bool VEC>
-__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 2 ? 3 : 2, sizeof(T) == 2 ? 3 : 2))) la_segments(const WalkArgs a) {
+__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 2 ? 3 : 2, sizeof(T) == 2 ? 3 : 2))) la_segments(const WalkArgs) {
     constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, W = 64;
     constexpr int LDX = KD, LDV = W;
     typedef Stage<T, C, KD, kThreads, VEC> SX;
@@ -269,37 +324,33 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(s
     Decays<C> *dec = reinterpret_cast<Decays<C> *>(V + PI * kTile<C, LDV>);
     int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
-    int64_t id = blockIdx.x;
-    const int slice = id % a.slices; id /= a.slices;
-    const int seg = id % a.segs; id /= a.segs;
-    const int64_t h = id % a.heads, b = id / a.heads, bh = b * a.heads + h;
-    if (seg == (REV ? 0 : a.segs - 1)) return;
-    const int64_t tbeg = int64_t(seg) * a.seg_len, tend = min(a.seqlen, tbeg + a.seg_len);
-    const int64_t chunks = (tend - tbeg + C - 1) / C;
-    const int col0 = slice * W, col = wave * 16;
-    const Rows<T> ry = rows_of<T>(a.y, b, h, a.kdim, 0), rv = rows_of<T>(a.v, b, h, a.cdim, col0);
-    const int64_t g0 = b * a.g_batch + h * a.g_head;
+    auto args = [] { return own_args<WalkArgs>(); };
+    const Place p = place_of(args(), args().slices);
+    if (p.seg == (REV ? 0 : args().segs - 1)) return;
+    const int chunks = (p.end - p.beg + C - 1) / C;
+    const int col0 = p.slice * W, col = wave * 16;
+    auto tensor = [&](auto of) { const WalkArgs a = args(); return of(a); };
+    const Rows<T> ry = tensor([&](const WalkArgs &a) { return rows_of<T>(a.y, p.b, p.h, a.kdim); });
+    const Rows<T> rv = tensor([&](const WalkArgs &a) { return rows_of<T>(a.v, p.b, p.h, a.cdim, col0); });
+    const Gates gates = tensor([&](const WalkArgs &a) { return gates_of(a, p); });
+    const float scale = afresh(args().scale);
     f32x4 S[KD / 16][1];
     load_state<KD, 1>(S, Mat{nullptr, 0, 0}, 0, 0, 0, lane);
     SX sy;
     SV sv;
-    auto start = [&](int64_t n) { return tbeg + (REV ? chunks - 1 - n : n) * C; };
-    auto load = [&](int64_t n) {
-        const int64_t t0 = start(n);
-        const int rows = int(min(int64_t(C), tend - t0));
+    auto start = [&](int n) { return p.beg + (REV ? chunks - 1 - n : n) * C; };
+    auto load = [&](int n) {
+        const int t0 = start(n), rows = min(C, p.end - t0);
         sy.load(ry, t0, rows, tid);
         sv.load(rv, t0, rows, tid);
     };
-    auto decay = [&](int64_t n) {
-        const int64_t t = start(n) + lane;
-        return lane < C && t < tend ? load_g_raw(a.g, a.gtype, g0 + t * a.g_seq) : 0u;
-    };
+    auto decay = [&](int n) { return gates.template load<C>(start(n), p.end, lane); };
     // The next chunk's decays are made by one wave while the others work on this one's state.
     double total = 0.0;
     bool cut = false;   // a token's own decay is 0
     auto decays = [&](int buf, uint32_t w) {
-        const float g = decode_g(w, a.gtype);
-        total += make_decays<C>(dec[buf], g, a.scale, lane);
+        const float g = decode_g(w, gates.type);
+        total += make_decays<C>(dec[buf], g, scale, lane);
         cut |= exp_f32(g) == 0.f;
     };
     uint32_t gnext = 0;
@@ -309,7 +360,7 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(s
         if (chunks > 1) gnext = decay(1);
     }
     int buf = 0;
-    for (int64_t n = 0; n < chunks; ++n, buf ^= 1) {
+    for (int n = 0; n < chunks; ++n, buf ^= 1) {
         __syncthreads();
         tid = afresh_lane(tid);
         lane = tid & 63;
@@ -329,17 +380,17 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(s
     if constexpr (!REV) {
         // What an infinity reached, by the recurrence, as behind the walk.
         if (__syncthreads_or(!finite_state<KD, 1>(S))) {
-            auto again = [&](int64_t n) {
+            auto again = [&](int n) {
                 __syncthreads();
                 load(n);
                 sy.store(Y, tid);
                 sv.store(V, tid);
-                if (wave == 0) make_decays<C>(dec[0], decode_g(decay(n), a.gtype), a.scale, lane);
+                if (wave == 0) make_decays<C>(dec[0], decode_g(decay(n), gates.type), scale, lane);
                 __syncthreads();
             };
             Kinds seen = {false, false};
 #pragma unroll 1
-            for (int64_t n = 0; n < chunks; ++n) {
+            for (int n = 0; n < chunks; ++n) {
                 again(n);
                 seen.tile<C, KD>(Y, lane);
                 seen.tile<C, W>(V, lane);
@@ -350,9 +401,9 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(s
                 f32x4 R[KD / 16][1];
                 load_state<KD, 1>(R, Mat{nullptr, 0, 0}, 0, 0, 0, lane);
 #pragma unroll 1
-                for (int64_t n = 0; n < chunks; ++n) {
+                for (int n = 0; n < chunks; ++n) {
                     again(n);
-                    recur<T, C, KD, 1, LDV, false>(R, nullptr, Y, V, dec[0], int(min(int64_t(C), tend - start(n))), a.kdim, col, lane,
+                    recur<T, C, KD, 1, LDV, false>(R, nullptr, Y, V, dec[0], min(C, p.end - start(n)), args().kdim, col, lane,
                                                    [](int, int, float) {});
                 }
 #pragma unroll
@@ -363,13 +414,15 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(s
             }
         }
     }
-    store_state<KD, 1>(S, Mat{a.st + (bh * a.segs + seg) * a.kdim * a.cdim, a.cdim, 1}, a.kdim, a.cdim, col0 + col, lane);
+    const WalkArgs a = args();
+    const int64_t at = (int64_t(p.b) * a.heads + p.h) * a.segs + p.seg;
+    store_state<KD, 1>(S, Mat{a.st + at * a.kdim * a.cdim, a.cdim, 1}, a.kdim, a.cdim, col0 + col, lane);
     // A decay that no token's own makes 0 is not 0: an infinite state stays infinite in any number of segments. (Nothing finite
     // changes by 2^-126 of a state.)
     cut = __any(cut);
-    if (slice == 0 && tid == 0) {
+    if (p.slice == 0 && tid == 0) {
         const float d = exp_f32(float(total));
-        a.seg_decay[bh * a.segs + seg] = !cut && d < 1.17549435e-38f ? 1.17549435e-38f : d;
+        a.seg_decay[at] = !cut && d < 1.17549435e-38f ? 1.17549435e-38f : d;
     }
 }
 
@@ -384,7 +437,8 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(s
 //
 // FOR_K: the walk of dk, X = v, Y = do, V = q; else that of dv, X = k, Y = q, V = do. KX: X's padded row length, KV: V's.
 template <typename T, int KD, int VD, bool VEC, bool F32, bool FOR_K>
-__device__ __forceinline__ void bwd_walk(const BwdArgs &a, char *smem, int tid, int wave, int lane) {
+__device__ __forceinline__ void bwd_walk(char *smem, int tid, int wave, int lane) {
+    auto args = [] { return own_args<BwdArgs>(); };
     constexpr bool kTight = KD + VD > 128;   // registers
     auto fresh = [&] {
         if constexpr (kTight) {
@@ -402,59 +456,67 @@ __device__ __forceinline__ void bwd_walk(const BwdArgs &a, char *smem, int tid, 
     Decays<C> *dec = reinterpret_cast<Decays<C> *>(M2 + kPlanes * kTile<C, LDM>);
     float *rowp = reinterpret_cast<float *>(dec + 2), *colp = rowp + CT * C, *part = colp + CT * C;
 
-    int64_t id = blockIdx.x;
-    const int seg = id % a.segs; id /= a.segs;
-    const int64_t h = id % a.heads, b = id / a.heads, bh = b * a.heads + h;
-    const int64_t tbeg = int64_t(seg) * a.seg_len, tend = min(a.seqlen, tbeg + a.seg_len);
-    const int64_t chunks = (tend - tbeg + C - 1) / C;
-    const Rows<T> rq = rows_of<T>(a.q, b, h, a.dk), rk = rows_of<T>(a.k, b, h, a.dk);
-    const Rows<T> rv = rows_of<T>(a.v, b, h, a.dv), rd = rows_of<T>(a.dout, b, h, a.dv);
-    const int64_t g0 = b * a.g_batch + h * a.g_head;
-    const int col = (wave % kWaves) * 16 * NC, rows_s = FOR_K ? a.dv : a.dk, cols_s = FOR_K ? a.dk : a.dv;
+    const Place p = place_of(args(), 1);
+    const int chunks = (p.end - p.beg + C - 1) / C, col = (wave % kWaves) * 16 * NC;
+    auto pair = [&](const BwdArgs &a) { return int64_t(p.b) * a.heads + p.h; };
 
     // R (or its transpose) at the segment's end.
     f32x4 S[KX / 16][NC];
-    load_state<KX, NC>(S, Mat{a.r0 ? const_cast<float *>(a.r0) + (bh * a.segs + seg) * int64_t(a.dk) * a.dv : nullptr, FOR_K ? 1 : a.dv,
-                              FOR_K ? a.dv : 1}, rows_s, cols_s, col, lane);
+    {
+        const BwdArgs a = args();
+        load_state<KX, NC>(S, Mat{a.r0 ? const_cast<float *>(a.r0) + (pair(a) * a.segs + p.seg) * a.dk * a.dv : nullptr, FOR_K ? 1 : a.dv,
+                                  FOR_K ? a.dv : 1}, FOR_K ? a.dv : a.dk, FOR_K ? a.dk : a.dv, col, lane);
+    }
     // <R, state> at a kept boundary, each wave's share.
-    auto boundary = [&](int64_t m) {
-        const Mat at{const_cast<float *>(a.ck) + (bh * a.blocks + m) * int64_t(a.dk) * a.dv, a.dk, 1};   // rows dv, columns dk
-        float sum = dot_state<KX, NC>(S, at, rows_s, cols_s, col, lane);
+    auto boundary = [&](const BwdArgs &a, int m) {
+        const int64_t at = pair(a) * a.blocks + m;
+        const Mat ck{const_cast<float *>(a.ck) + at * a.dk * a.dv, a.dk, 1};   // rows dv, columns dk
+        float sum = dot_state<KX, NC>(S, ck, a.dv, a.dk, col, lane);
         sum = wave_sum(sum);
-        if (lane == 0) a.y[(bh * a.blocks + m) * kWaves + wave - kWaves] = sum;
+        if (lane == 0) a.y[at * kWaves + wave - kWaves] = sum;
     };
     if constexpr (FOR_K) {
-        if (a.ck && a.has_last && seg == a.segs - 1) boundary(a.blocks - 1);
+        const BwdArgs a = args();
+        if (a.ck && a.has_last && p.seg == a.segs - 1) boundary(a, int(a.blocks) - 1);
     }
 
+    // One after the other: arguments that are read together are held together.
+    auto tensor = [&](auto of) { const BwdArgs a = args(); return of(a); };
+    const Rows<T> rq = tensor([&](const BwdArgs &a) { return rows_of<T>(a.q, p.b, p.h, a.dk); });
+    const Rows<T> rk = tensor([&](const BwdArgs &a) { return rows_of<T>(a.k, p.b, p.h, a.dk); });
+    const Rows<T> rv = tensor([&](const BwdArgs &a) { return rows_of<T>(a.v, p.b, p.h, a.dv); });
+    const Rows<T> rd = tensor([&](const BwdArgs &a) { return rows_of<T>(a.dout, p.b, p.h, a.dv); });
+    const float scale = afresh(args().scale);
+    const bool want_g = args().a != nullptr;
+    char *const out = tensor([&](const BwdArgs &a) {
+        return afresh(static_cast<char *>(FOR_K ? a.dk_out : a.dv_out) +
+                      (p.b * a.seqlen * a.heads + p.h) * (FOR_K ? a.dk : a.dv) * int64_t(FOR_K && F32 ? 4 : sizeof(T)));
+    });
+    const uint32_t out_stride = tensor([&](const BwdArgs &a) { return uint32_t(afresh(int(a.heads) * (FOR_K ? a.dk : a.dv))); });
     zero_masked_scores<C>(M1, true, tid, NT2);
     zero_masked_scores<C>(M2, true, tid, NT2);
     SK sq, sk;
     SV sv, sd;
-    auto start = [&](int64_t n) { return tbeg + (chunks - 1 - n) * C; };
-    auto load = [&](int64_t n) {
-        const int64_t t0 = start(n);
-        const int rows = int(min(int64_t(C), tend - t0));
+    auto start = [&](int n) { return p.beg + (chunks - 1 - n) * C; };
+    // (dk's walk alone makes the decays.)
+    const Gates gates = FOR_K ? tensor([&](const BwdArgs &a) { return gates_of(a, p); }) : Gates{nullptr, 0, MM_FLOAT32};
+    auto make = [&](int buf, uint32_t g) { make_decays<C>(dec[buf], decode_g(g, gates.type), scale, lane); };
+    const bool dwave = FOR_K && wave == 2 * kWaves - 1;
+    uint32_t gnext = 0;
+    {
+        const int t0 = start(0), rows = min(C, p.end - t0);
         sq.load(rq, t0, rows, tid);
         sk.load(rk, t0, rows, tid);
         sv.load(rv, t0, rows, tid);
         sd.load(rd, t0, rows, tid);
-    };
-    auto decay = [&](int64_t n) {
-        const int64_t t = start(n) + lane;
-        return lane < C && t < tend ? load_g_raw(a.g, a.gtype, g0 + t * a.g_seq) : 0u;
-    };
-    const bool dwave = FOR_K && wave == 2 * kWaves - 1;
-    uint32_t gnext = 0;
-    load(0);
+    }
     if (dwave) {
-        make_decays<C>(dec[0], decode_g(decay(0), a.gtype), a.scale, lane);
-        if (chunks > 1) gnext = decay(1);
+        make(0, gates.template load<C>(start(0), p.end, lane));
+        if (chunks > 1) gnext = gates.template load<C>(start(1), p.end, lane);
     }
     int buf = 0;
-    for (int64_t n = 0; n < chunks; ++n, buf ^= 1) {
-        const int64_t t0 = start(n);
-        const int rows = int(min(int64_t(C), tend - t0));
+    for (int n = 0; n < chunks; ++n, buf ^= 1) {
+        const int t0 = start(n), rows = min(C, p.end - t0);
         __syncthreads();
         fresh();
         sq.store(Q, tid);
@@ -462,13 +524,11 @@ __device__ __forceinline__ void bwd_walk(const BwdArgs &a, char *smem, int tid, 
         sv.store(V, tid);
         sd.store(G, tid);
         const bool more = n + 1 < chunks;
-        const int64_t tn = t0 - C;   // the next chunk is a whole one
+        const int tn = t0 - C;   // the next chunk is a whole one
         __syncthreads();
         fresh();
         const Decays<C> &d = dec[buf];
-        auto tiles = [&](auto L) {
-            scores_bwd<T, C, KD, VD, decltype(L)>(d, Q, K, V, G, M1, M2, a.scale, a.a != nullptr, rowp, colp, lane);
-        };
+        auto tiles = [&](auto L) { scores_bwd<T, C, KD, VD, decltype(L)>(d, Q, K, V, G, M1, M2, scale, want_g, rowp, colp, lane); };
         if constexpr (C == 64) {
             switch (wave) {
                 case 0: tiles(Tiles<0, 0, 0, 1>{}); break;
@@ -491,25 +551,27 @@ __device__ __forceinline__ void bwd_walk(const BwdArgs &a, char *smem, int tid, 
         fresh();
         inter<T, C, KX, NC>(O, S, FOR_K ? V : K, d.out, lane);
         if constexpr (FOR_K) {
-            if (a.a) dot_rows<T, C, NC, LDK>(O, K, col, part + (wave - kWaves) * C, lane);
+            if (want_g) dot_rows<T, C, NC, LDK>(O, K, col, part + (wave - kWaves) * C, lane);
         }
         if (more) sk.load(rk, tn, C, tid);
         if (dwave && more) {
-            make_decays<C>(dec[buf ^ 1], decode_g(gnext, a.gtype), a.scale, lane);
-            if (n + 2 < chunks) gnext = decay(n + 2);
+            make(buf ^ 1, gnext);
+            if (n + 2 < chunks) gnext = gates.template load<C>(start(n + 2), p.end, lane);
         }
         __syncthreads();
         fresh();
         if constexpr (!FOR_K) {
-            if (a.a && tid < rows) {
+            if (want_g && tid < rows) {
                 const int t = tid / 16;
                 float sum = 0.f, f = 0.f;
                 for (int o = 0; o <= t; ++o) sum += rowp[o * C + tid];
                 for (int m = t; m < CT; ++m) sum -= colp[m * C + tid];
 #pragma unroll
                 for (int w = 0; w < kWaves; ++w) f += part[w * C + tid];
-                a.a[bh * a.seqlen + t0 + tid] = sum;
-                a.f[bh * a.seqlen + t0 + tid] = f;
+                const BwdArgs a = args();
+                const int64_t at = pair(a) * a.seqlen + t0 + tid;
+                a.a[at] = sum;
+                a.f[at] = f;
             }
         }
         if (more) {
@@ -522,26 +584,23 @@ __device__ __forceinline__ void bwd_walk(const BwdArgs &a, char *smem, int tid, 
         intra<T, C, NC, LDC, true>(O, v, FOR_K ? M2 : M1, VT, col, lane);
         update<T, C, KX, NC>(S, v, FOR_K ? G : Q, d.in, d.all, lane);
         fresh();
+        store_out<T, C, NC, LDC, VEC, FOR_K && F32>(O, out, out_stride, t0, rows, FOR_K ? rk.d : rv.d, FOR_K ? K : V, col, lane);
         if constexpr (FOR_K) {
-            store_out<T, C, NC, LDC, VEC, F32>(O, static_cast<char *>(a.dk_out) + (b * a.seqlen * a.heads + h) * a.dk * int64_t(F32 ? 4 : sizeof(T)),
-                                               a.heads * a.dk, t0, rows, a.dk, K, col, lane);
-            if (a.ck && t0 > 0 && t0 % kBlock == 0) boundary(t0 / kBlock - 1);
-        } else {
-            store_out<T, C, NC, LDC, VEC, false>(O, reinterpret_cast<T *>(a.dv_out) + (b * a.seqlen * a.heads + h) * a.dv, a.heads * a.dv, t0, rows,
-                                                 a.dv, V, col, lane);
+            if (want_g && t0 > 0 && t0 % kBlock == 0) boundary(args(), t0 / kBlock - 1);
         }
     }
     if constexpr (!FOR_K) {
-        if (a.dr && seg == 0) store_state<KX, NC>(S, Mat{a.dr + bh * int64_t(a.dk) * a.dv, a.dv, 1}, a.dk, a.dv, col, lane);
+        const BwdArgs a = args();
+        if (a.dr && p.seg == 0) store_state<KX, NC>(S, Mat{a.dr + pair(a) * a.dk * a.dv, a.dv, 1}, a.dk, a.dv, col, lane);
     }
 }
 
 template <typename T, int KD, int VD, bool VEC, bool F32>
-__global__ void __launch_bounds__(2 * kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) la_bwd(const BwdArgs a) {
+__global__ void __launch_bounds__(2 * kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) la_bwd(const BwdArgs) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid & 63;
-    if (wave < kWaves) bwd_walk<T, KD, VD, VEC, F32, false>(a, smem, tid, wave, lane);
-    else bwd_walk<T, KD, VD, VEC, F32, true>(a, smem, tid, wave, lane);
+    if (wave < kWaves) bwd_walk<T, KD, VD, VEC, F32, false>(smem, tid, wave, lane);
+    else bwd_walk<T, KD, VD, VEC, F32, true>(smem, tid, wave, lane);
 }
 
 // Launches with `bytes` of dynamic LDS, which a kernel is allowed once per device (`done`: a bit per device).

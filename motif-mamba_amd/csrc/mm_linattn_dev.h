@@ -95,6 +95,21 @@ __device__ __forceinline__ int afresh(int x) {
     asm volatile("" : "+s"(x));
     return x;
 }
+__device__ __forceinline__ int64_t afresh(int64_t x) {
+    asm volatile("" : "+s"(x));
+    return x;
+}
+__device__ __forceinline__ float afresh(float x) {
+    asm volatile("" : "+s"(x));
+    return x;
+}
+template <typename T>
+__device__ __forceinline__ T *afresh(T *p) {
+    typedef __attribute__((address_space(1))) T *Global;
+    Global x = (Global)p;
+    asm volatile("" : "+s"(x));
+    return (T *)x;
+}
 __device__ __forceinline__ int afresh_lane(int x) {
     asm volatile("" : "+v"(x));
     return x;
@@ -166,7 +181,7 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void *base) {
 // than 2^31 bytes.
 template <typename T> struct Rows {
     const T *p;
-    int64_t stride;
+    uint32_t stride; // bytes
     int d;           // elements of a row that exist
 };
 
@@ -180,11 +195,10 @@ struct Stage {
     static constexpr bool kEven = C % RS == 0;
     uint4 r[N];
 
-    __device__ __forceinline__ void load(const Rows<T> &s, int64_t t0, int rows, int tid) {
-        const __amdgpu_buffer_rsrc_t buf = buffer(s.p + t0 * s.stride);
+    __device__ __forceinline__ void load(const Rows<T> &s, int t0, int rows, int tid) {
+        const __amdgpu_buffer_rsrc_t buf = buffer(reinterpret_cast<const char *>(s.p) + uint64_t(unsigned(t0)) * s.stride);
         const int row = unsigned(tid) / VR, col = unsigned(tid) % VR * VE;
-        const uint32_t stride = uint32_t(s.stride) * uint32_t(sizeof(T));
-        const uint32_t off = uint32_t(row) * stride + uint32_t(col) * uint32_t(sizeof(T));
+        const uint32_t stride = s.stride, off = uint32_t(row) * stride + uint32_t(col) * uint32_t(sizeof(T));
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             const bool live = row + n * RS < (kEven ? rows : min(rows, C));
@@ -900,12 +914,12 @@ __device__ __forceinline__ void store_element(float x, const __amdgpu_buffer_rsr
 // float32 shares half a chunk at a time, each row in the place of two rows of the tile. float32 tensors' rows go out by the lane, in
 // 64-byte runs (through LDS: 1,025 us against 990 for 65,536 tokens of 40 heads).
 template <typename T, int C, int NC, int LDV, bool VEC, bool F32>
-__device__ __forceinline__ void store_out(const f32x4 (&O)[C / 16][NC], void *out, int64_t stride, int64_t t0, int rows, int cols,
+__device__ __forceinline__ void store_out(const f32x4 (&O)[C / 16][NC], void *out, uint32_t stride, int t0, int rows, int cols,
                                           u16 *tile, int col, int lane) {
     const int g = (lane >> 4), i = (lane & 15);
     constexpr uint32_t ES = F32 ? 4 : sizeof(T);
-    const __amdgpu_buffer_rsrc_t buf = buffer(static_cast<char *>(out) + t0 * stride * ES);
-    const uint32_t step = uint32_t(stride) * ES;
+    const __amdgpu_buffer_rsrc_t buf = buffer(static_cast<char *>(out) + uint64_t(unsigned(t0)) * stride * ES);
+    const uint32_t step = stride * ES;
     if constexpr (VEC && sizeof(T) == 2) wave_fence();
     if constexpr (VEC && !F32 && sizeof(T) == 2) {
 #pragma unroll
@@ -967,7 +981,7 @@ __device__ __forceinline__ void store_out(const f32x4 (&O)[C / 16][NC], void *ou
 #pragma unroll
                 for (int c = 0; c < NC; ++c) {
                     const int x = col + 16 * c + i;
-                    store_element<T, F32>(O[t][c][r], buf, n < rows && x < cols ? uint32_t(n) * uint32_t(stride) + uint32_t(x) : kNone);
+                    store_element<T, F32>(O[t][c][r], buf, n < rows && x < cols ? uint32_t(n) * stride + uint32_t(x) : kNone);
                 }
             }
     }

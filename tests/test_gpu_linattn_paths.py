@@ -100,3 +100,16 @@ def test_segments_of_slices(off, dtype):
     assert _segmented(t)
     dout, _ = _dout(t, 5)
     _check(t, 0.1, dout, None, ["q", "k", "v", "log_decay"], views)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("wanted", [["q", "k", "v", "log_decay", "initial_state"], ["q", "k", "v"]])
+@pytest.mark.parametrize("heads", [1, 2])
+@pytest.mark.parametrize("dk,dv", [(48, 40), (48, 104), (112, 40), (112, 104), (37, 33), (37, 101), (107, 33), (107, 101)])
+def test_every_kernel(dk, dv, heads, wanted, dtype):
+    """The kernels are built for dk and dv up to 64 and up to 128, aligned rows and others, heads of their own and shared q and k,
+    and with and without the decays' gradient: each of them."""
+    _say(f"linear attention {dk} {dv} {heads} heads {len(wanted)} {dtype}")
+    t = _inputs(2500 + dk + dv, 1, 150, 1, heads, dk, dv, dtype, states=True)
+    dout, r = _dout(t, 6)
+    _check(t, dk ** -0.5, dout, torch.randn(t["initial_state"].shape, generator=r), wanted)
