@@ -754,14 +754,18 @@ __device__ __forceinline__ void store_g(void *p, mm_dtype t, int64_t i, float x)
 
 // The gradient of a log decay is the sum of W_ij = scale exp(c_i - c_j) (q_i . k_j) (do_i . v_j) over the pairs that it
 // lies between, j < t <= i. Cut at t's chunk, with S the state before and R the state's gradient after the chunk: pairs
-// inside it (a holds each token's row sum less its column sum, the diagonal left out), pairs from before into it (e_i),
-// pairs from it to behind (f_j), and pairs around it, Z = exp(c_end) <R, S>. No part is a difference of larger ones but
-// Z, which is <R, S'> less the chunk's f; <R, S'> is taken from the states themselves every kBlock tokens. One workgroup
-// per block and (batch row, head); C: the chunk's tokens.
+// inside it (a holds each token's row sum less its column sum, the diagonal left out; summed from t on), pairs from before into
+// it (e_i), pairs from it to behind (f_j), and pairs around it, Z = exp(c_end) <R, S>, which is <R, S'> less the chunk's f; <R, S'>
+// is taken from the states themselves every kBlock tokens. Two of these are differences: a pair that lies wholly behind t is in
+// a's sum once with each sign, and Z is what is left of <R, S'>. So a result's error is a fraction (2^-24 and the sums' depth) of the
+// terms of its chunk's tokens behind it and of its block's. A forgotten state (-inf) ends both: no pair crosses it, so a's sum stops
+// there and Z is 0, and a document's results have nothing of another one's rounding. One workgroup per block and
+// (batch row, head); C: the chunk's tokens.
 __global__ void __launch_bounds__(kBlock) la_decay_grad(const float *a, const float *e, const float *f, const float *y, int64_t seqlen,
                                                         int64_t blocks, int heads, int C, bool has_last, const void *g, int64_t g_batch,
                                                         int64_t g_seq, int64_t g_head, float *tmp, void *out, mm_dtype gtype) {
     __shared__ float sa[kBlock], sf[kBlock], se[kBlock], zc[kBlock / 16];
+    __shared__ int forgets[kBlock], chunk_forgets[kBlock / 32];
     const int64_t blk = blockIdx.y, bh = blockIdx.x, t = blk * kBlock + threadIdx.x;
     const int tid = threadIdx.x, chunks = kBlock / C;
     const bool live = t < seqlen;
@@ -769,15 +773,19 @@ __global__ void __launch_bounds__(kBlock) la_decay_grad(const float *a, const fl
     sa[tid] = (live ? a[bh * seqlen + t] : 0.f) + ae;
     sf[tid] = live ? f[bh * seqlen + t] : 0.f;
     se[tid] = ae;
+    forgets[tid] = live && decode_g(load_g_raw(g, gtype, bh / heads * g_batch + t * g_seq + bh % heads * g_head), gtype) == -128.f;
     __syncthreads();
     if (tid < chunks) {   // the chunks' totals
         float E = 0.f, F = 0.f;
+        int any = 0;
         for (int n = 0; n < C; ++n) {
             E += se[tid * C + n];
             F += sf[tid * C + n];
+            any |= forgets[tid * C + n];
         }
         zc[tid] = E;
         zc[chunks + tid] = F;
+        chunk_forgets[tid] = any;
     }
     __syncthreads();
     if (tid == 0) {
@@ -785,7 +793,7 @@ __global__ void __launch_bounds__(kBlock) la_decay_grad(const float *a, const fl
         if (blk + 1 < blocks || has_last)
             for (int w = 0; w < 4; ++w) Y += y[(bh * blocks + blk) * 4 + w];
         for (int c = chunks - 1; c >= 0; --c) {
-            const float Z = Y - zc[chunks + c];
+            const float Z = chunk_forgets[c] ? 0.f : Y - zc[chunks + c];
             Y = Z + zc[c];
             zc[c] = Z;
         }
@@ -795,9 +803,10 @@ __global__ void __launch_bounds__(kBlock) la_decay_grad(const float *a, const fl
     const int c0 = tid / C * C;
     float s = zc[tid / C];
     for (int n = c0; n < tid; ++n) s += sf[n];
-    for (int n = c0 + C - 1; n >= tid; --n) s += sa[n];
-    // A forgotten state has no gradient; the sums above are of terms that cancel.
-    if (decode_g(load_g_raw(g, gtype, bh / heads * g_batch + t * g_seq + bh % heads * g_head), gtype) == -128.f) s = 0.f;
+    int end = tid + 1;
+    while (end < c0 + C && !forgets[end]) ++end;
+    for (int n = end - 1; n >= tid; --n) s += sa[n];
+    if (forgets[tid]) s = 0.f;
     if (tmp) tmp[bh * seqlen + t] = s;
     else store_g(out, gtype, (bh / heads * seqlen + t) * heads + bh % heads, s);
 }

@@ -234,3 +234,37 @@ def test_infinite_values_then_tokens():
         y = linear_attention_update(state, *(d[m][:, n] for m in ("q", "k", "v", "log_decay")))
         _same_kinds(out[:, n], y.cpu().double(), n)
     _same_kinds(last, state.cpu().double(), "state")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("cuts", [(7,), (40, 90), (130, 300), (256,), (100, 101, 480)])
+def test_documents_do_not_share_rounding(cuts, dtype):
+    """Documents apart by -inf, every other one 30 times as large (its decays' gradients some 10^6 times): each one's results within
+    the bound of its own terms. (Gradients of 30^3 and more pass float16's range.)"""
+    _say(f"linear attention documents {cuts} {dtype}")
+    from motif_mamba_amd import linear_attention_fn
+    L, edges = 520, (0, *cuts, 520)
+    r = torch.Generator().manual_seed(8)
+    t = {"q": _randn(r, 1, L, 1, 32), "k": _randn(r, 1, L, 1, 32), "v": _randn(r, 1, L, 2, 32), "log_decay": -0.05 * torch.rand(1, L, 2, generator=r)}
+    dout = _randn(r, 1, L, 2, 32)
+    for n, (a, b) in enumerate(zip(edges, edges[1:])):
+        for x in (t["q"], t["k"], t["v"], dout):
+            x[:, a:b] *= 30.0 if n % 2 else 1.0
+        if n:
+            t["log_decay"][:, a] = float("-inf")
+    t = {n: x if n == "log_decay" else x.to(dtype) for n, x in t.items()}
+    dout = dout.to(dtype)
+    leaves = {n: x.to(DEV).requires_grad_(True) for n, x in t.items()}
+    got = torch.autograd.grad(linear_attention_fn(**leaves, scale=0.2), list(leaves.values()), dout.to(DEV))
+    for a, b in zip(edges, edges[1:]):
+        part = {n: x[:, a:b].clone() for n, x in t.items()}
+        part["log_decay"][:, 0] = 0.0   # nothing stands before it
+        exact, size = ref.with_grads(part, 0.2, dout[:, a:b]), ref.magnitudes(part, 0.2, dout[:, a:b])
+        for n, x in zip(leaves, got):
+            x, e, z = x[:, a:b], exact["d" + n], size["d" + n]
+            if n == "log_decay" and a:
+                assert not x[:, 0].any()
+                x, e, z = x[:, 1:], e[:, 1:], z[:, 1:]
+                if not e.numel():
+                    continue
+            ref.check(x, e, z, F32, f"d{n} of {a} .. {b}", whole_row=n == "log_decay")
