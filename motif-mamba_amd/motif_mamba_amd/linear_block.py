@@ -49,7 +49,7 @@ class LinearAttentionBlock(nn.Module):
     def _operands(self, xbc, dt):
         v, q, k = xbc.split([self.d_inner, self.d_qk, self.d_qk], -1)
         dt = F.softplus(dt.float() + self.dt_bias)
-        v = v.unflatten(-1, (self.nheads, self.headdim)) * dt.unsqueeze(-1).to(v.dtype)
+        v = (v.unflatten(-1, (self.nheads, self.headdim)) * dt.unsqueeze(-1)).to(v.dtype)   # dt stays float32: rounded once
         return q.unflatten(-1, (self.n_groups, self.d_state)), k.unflatten(-1, (self.n_groups, self.d_state)), v, -torch.exp(self.A_log) * dt
 
     def _finish(self, y, z):

@@ -72,3 +72,22 @@ def test_update_refuses_states_that_overlap(blocks, strides):
     names = ("state_batch_stride", "state_head_stride", "state_dk_stride")
     rc, msg = _call("mm_linattn_update", _fill(blocks, "mm_linattn_update_params", **TOKEN, **dict(zip(names, strides))))
     assert rc == -1 and "overlap" in msg, (rc, msg)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_block_rounds_a_value_once(dtype):
+    """A token's value enters as v dt with the dt that its decay uses, in float32, rounded once."""
+    from motif_mamba_amd import LinearAttentionBlock
+    torch.manual_seed(2)
+    b = LinearAttentionBlock(32, nheads=4, headdim=16, d_state=8)
+    xbc, dt = torch.randn(3, 50, b.d_xbc).to(dtype), torch.randn(3, 50, 4).to(dtype)
+    with torch.no_grad():
+        _, _, v, g = b._operands(xbc, dt)
+    exact_dt = torch.nn.functional.softplus(dt.double() + b.dt_bias.double())
+    exact = xbc[..., :64].double().unflatten(-1, (4, 16)) * exact_dt.unsqueeze(-1)
+    assert v.dtype == dtype and g.dtype == torch.float32
+    half = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}[dtype]
+    unit = torch.exp2(torch.floor(torch.log2(exact.detach().abs().clamp_min(2.0 ** -14)))) * half
+    # softplus and the product in float32: a few 2^-24
+    assert ((v.double() - exact).abs() <= unit + 2.0 ** -21 * exact.abs()).all()
+    assert torch.allclose(g.double(), -torch.exp(b.A_log.double()) * exact_dt, rtol=2.0 ** -20)
