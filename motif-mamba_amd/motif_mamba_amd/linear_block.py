@@ -66,9 +66,10 @@ class LinearAttentionBlock(nn.Module):
         if cache is None:
             return self._finish(linear_attention_fn(q, k, v, g, scale=1.0), z)
         conv_state, state = cache
-        conv_state.copy_(F.pad(x, (self.d_conv, 0))[..., x.shape[-1]:])
+        # The cache holds values: it is no part of the graph.
+        conv_state.copy_(F.pad(x.detach(), (self.d_conv, 0))[..., x.shape[-1]:])
         y, last = linear_attention_fn(q, k, v, g, scale=1.0, return_last_state=True)
-        state.copy_(last)
+        state.copy_(last.detach())
         return self._finish(y, z)
 
     def step(self, hidden, cache):

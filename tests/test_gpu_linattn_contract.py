@@ -268,3 +268,22 @@ def test_documents_do_not_share_rounding(cuts, dtype):
                 if not e.numel():
                     continue
             ref.check(x, e, z, F32, f"d{n} of {a} .. {b}", whole_row=n == "log_decay")
+
+
+def test_block_cache_is_no_part_of_the_graph():
+    """A prompt in grad mode fills the cache with values; the outputs still have their gradients."""
+    _say("linear attention block: cache in grad mode")
+    from motif_mamba_amd import LinearAttentionBlock
+    torch.manual_seed(9)
+    b = LinearAttentionBlock(32, nheads=2, headdim=16, d_state=16).to(DEV)
+    hidden = torch.randn(2, 20, 32, device=DEV)
+    cache, plain = b.allocate_inference_cache(2), b.allocate_inference_cache(2)
+    out = b(hidden, cache)
+    for x in cache:
+        assert not x.requires_grad and x.grad_fn is None
+    with torch.no_grad():
+        assert torch.equal(b(hidden, plain), out)
+        b.step(torch.randn(2, 32, device=DEV), cache)   # in place, while the graph is alive
+    grads = torch.autograd.grad(out.sum(), list(b.parameters()))
+    assert all(torch.isfinite(g).all() and g.any() for g in grads)
+    assert torch.equal(b(hidden), out)
