@@ -20,7 +20,8 @@
  * Conventions as in mm_scan.h: device pointers, element strides, outputs allocated by the caller, nothing
  * is synchronised or allocated, 0 or a code of mm_scan.h is returned and mm_last_error() has the text. The
  * innermost dimension (dk or dv) of q, k, v, dout and of every output is contiguous; states are contiguous
- * (batch, nheads, dk, dv).
+ * (batch, nheads, dk, dv). Sequence strides are 0 to 2^22 - 1 elements (nheads * dk and nheads * dv too in the backward), seqlen is at
+ * most 2^23, batch * nheads at most 2^23 - 1 (mm_linattn_update: 2^24 - 1); else MM_ERR_UNSUPPORTED.
  */
 #ifndef MM_LINATTN_H_
 #define MM_LINATTN_H_

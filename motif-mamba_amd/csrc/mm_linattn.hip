@@ -13,6 +13,7 @@
 #define MM_LINATTN_COMMON
 #endif
 
+#include <algorithm>
 #include <atomic>
 
 #include "mm_linattn_dev.h"
@@ -725,23 +726,23 @@ __global__ void __launch_bounds__(256) la_join(float *st, const float *decay, co
 // 24 heads' gradients in 31 us (6.5 TB/s, part of them from the last-level cache), 59 with one element per thread.
 template <typename T, int W>
 __global__ void __launch_bounds__(256) la_head_sum(const float *part, T *out, int64_t n, int heads, int share, int d) {
-    const int64_t id = (int64_t(blockIdx.x) * 256 + threadIdx.x) * W;
-    if (id >= n) return;
-    const int64_t x = id % d, rg = id / d, groups = heads / share, row = rg / groups, grp = rg % groups;
-    const float *p = part + (row * heads + grp * share) * d + x;
-    float s[W] = {};
+    for (int64_t id = (int64_t(blockIdx.x) * 256 + threadIdx.x) * W; id < n; id += int64_t(gridDim.x) * 256 * W) {
+        const int64_t x = id % d, rg = id / d, groups = heads / share, row = rg / groups, grp = rg % groups;
+        const float *p = part + (row * heads + grp * share) * d + x;
+        float s[W] = {};
 #pragma unroll 8
-    for (int r = 0; r < share; ++r) {
-        if constexpr (W == 4) {
-            const f32x4 y = *reinterpret_cast<const f32x4 *>(p + int64_t(r) * d);
+        for (int r = 0; r < share; ++r) {
+            if constexpr (W == 4) {
+                const f32x4 y = *reinterpret_cast<const f32x4 *>(p + int64_t(r) * d);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[e] += y[e];
-        } else {
-            s[0] += p[int64_t(r) * d];
+                for (int e = 0; e < 4; ++e) s[e] += y[e];
+            } else {
+                s[0] += p[int64_t(r) * d];
+            }
         }
-    }
 #pragma unroll
-    for (int e = 0; e < W; ++e) out[id + e] = from_f32<T>(s[e]);
+        for (int e = 0; e < W; ++e) out[id + e] = from_f32<T>(s[e]);
+    }
 }
 
 __device__ __forceinline__ void store_g(void *p, mm_dtype t, int64_t i, float x) {
@@ -827,15 +828,14 @@ __global__ void __launch_bounds__(256) la_decay_sum(const float *tmp, int64_t ba
 }
 
 __global__ void __launch_bounds__(256) la_copy(float *dst, const float *src, int64_t n) {
-    const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
-    if (i < n) dst[i] = src ? src[i] : 0.f;
+    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < n; i += int64_t(gridDim.x) * 256) dst[i] = src ? src[i] : 0.f;
 }
 __global__ void __launch_bounds__(256) la_zero_g(void *dst, mm_dtype t, int64_t n) {
-    const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
-    if (i < n) store_g(dst, t, i, 0.f);
+    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < n; i += int64_t(gridDim.x) * 256) store_g(dst, t, i, 0.f);
 }
 
-static unsigned blocks_of(int64_t n) { return unsigned((n + 255) / 256); }
+// Blocks of 256 for n elements, each thread taking one at a time until none is left: a launch holds less than 2^32 threads.
+static unsigned blocks_of(int64_t n) { return unsigned(std::min<int64_t>((n + 255) / 256, 1 << 23)); }
 
 int launch_join(float *st, const float *decay, const float *edge, int segs, int64_t size, int64_t bh, bool rev, hipStream_t s) {
     hipLaunchKernelGGL(la_join, dim3(unsigned(bh), blocks_of(size)), dim3(256), 0, s, st, decay, edge, segs, size, rev);

@@ -127,6 +127,9 @@ static int chunk_of(mm_dtype t) { return t == MM_BFLOAT16 ? 64 : 32; }
 
 constexpr int kBlockTokens = 256;
 
+// A launch takes less than 2^32 threads; a pair has a workgroup of up to 512 (the backward), for one token 256.
+constexpr int64_t kMostPairs = (int64_t(1) << 23) - 1, kMostTokenPairs = (int64_t(1) << 24) - 1;
+
 // Segments of a row, by the time that a call takes with n of them, in steps of a chunk of one workgroup alone on its CU
 // (about 3.7 us at dk 128, dv 64, bfloat16). Two workgroups on a CU take 1.45 steps per chunk of both. With n > 1 a pass over
 // k and v before (0.9 of a step per chunk for few workgroups, 0.5 of one per chunk and CU for many), its join (about 2 steps),
@@ -166,7 +169,7 @@ static int check(int64_t batch, int64_t seqlen, int64_t groups, int64_t heads, i
     if (groups < 1 || heads % groups) return set_error(MM_ERR_INVALID_ARGUMENT, "linear attention: nheads must be a multiple of n_groups");
     if (dk < 1 || dv < 1) return set_error(MM_ERR_INVALID_ARGUMENT, "linear attention: dk and dv must be at least 1");
     if (dk > MM_LINATTN_MAX_DIM || dv > MM_LINATTN_MAX_DIM) return set_error(MM_ERR_UNSUPPORTED, "linear attention: dk and dv must be <= 128");
-    if (batch * heads > pairs) return set_error(MM_ERR_UNSUPPORTED, "linear attention: batch * nheads is too large (2^23; one token: 2^31 - 1)");
+    if (batch > pairs || heads > pairs || batch * heads > pairs) return set_error(MM_ERR_UNSUPPORTED, "linear attention: batch * nheads is too large (at most 2^23 - 1, for one token 2^24 - 1)");
     if (seqlen > (int64_t(1) << 23)) return set_error(MM_ERR_UNSUPPORTED, "linear attention: seqlen must be <= 2^23");
     return MM_OK;
 }
@@ -371,7 +374,7 @@ extern "C" int64_t mm_linattn_bwd_workspace_size(const mm_linattn_bwd_params *p)
 extern "C" int mm_linattn_fwd(const mm_linattn_fwd_params *params, void *stream) {
     if (!params) return set_error(MM_ERR_INVALID_ARGUMENT, "mm_linattn_fwd: params is NULL");
     const mm_linattn_fwd_params &p = *params;
-    if (const int rc = la::check(p.batch, p.seqlen, p.n_groups, p.nheads, p.dk, p.dv, p.itype, p.gtype, int64_t(1) << 23)) return rc;
+    if (const int rc = la::check(p.batch, p.seqlen, p.n_groups, p.nheads, p.dk, p.dv, p.itype, p.gtype, la::kMostPairs)) return rc;
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     const int64_t bh = p.batch * p.nheads;
     if (bh == 0) return MM_OK;
@@ -390,7 +393,7 @@ extern "C" int mm_linattn_fwd(const mm_linattn_fwd_params *params, void *stream)
 extern "C" int mm_linattn_bwd(const mm_linattn_bwd_params *params, void *stream) {
     if (!params) return set_error(MM_ERR_INVALID_ARGUMENT, "mm_linattn_bwd: params is NULL");
     const mm_linattn_bwd_params &p = *params;
-    if (const int rc = la::check(p.batch, p.seqlen, p.n_groups, p.nheads, p.dk, p.dv, p.itype, p.gtype, int64_t(1) << 23)) return rc;
+    if (const int rc = la::check(p.batch, p.seqlen, p.n_groups, p.nheads, p.dk, p.dv, p.itype, p.gtype, la::kMostPairs)) return rc;
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     const int64_t bh = p.batch * p.nheads;
     if (bh == 0 || p.seqlen == 0) {
@@ -423,7 +426,7 @@ extern "C" int mm_linattn_bwd(const mm_linattn_bwd_params *params, void *stream)
 extern "C" int mm_linattn_update(const mm_linattn_update_params *params, void *stream) {
     if (!params) return set_error(MM_ERR_INVALID_ARGUMENT, "mm_linattn_update: params is NULL");
     const mm_linattn_update_params &p = *params;
-    if (const int rc = la::check(p.batch, 1, p.n_groups, p.nheads, p.dk, p.dv, p.itype, p.gtype, 2147483647)) return rc;
+    if (const int rc = la::check(p.batch, 1, p.n_groups, p.nheads, p.dk, p.dv, p.itype, p.gtype, la::kMostTokenPairs)) return rc;
     if (p.batch * p.nheads == 0) return MM_OK;
     if (!p.state || !p.q || !p.k || !p.v || !p.log_decay || !p.out)
         return set_error(MM_ERR_INVALID_ARGUMENT, "mm_linattn_update: state, q, k, v, log_decay and out are required");

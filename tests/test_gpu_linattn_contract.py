@@ -287,3 +287,42 @@ def test_block_cache_is_no_part_of_the_graph():
     grads = torch.autograd.grad(out.sum(), list(b.parameters()))
     assert all(torch.isfinite(g).all() and g.any() for g in grads)
     assert torch.equal(b(hidden), out)
+
+
+def test_most_pairs():
+    """As many (batch row, head) pairs as the texts allow: prompts and their gradients, one token."""
+    _say("linear attention most pairs")
+    from motif_mamba_amd import linear_attention_fn, linear_attention_update
+    n = (1 << 23) - 1
+    r = torch.Generator(device=DEV).manual_seed(10)
+    q, k, v = (torch.randn(n, 1, 1, 1, generator=r, device=DEV).requires_grad_(True) for _ in range(3))
+    g = -torch.rand(n, 1, 1, generator=r, device=DEV)
+    out = linear_attention_fn(q, k, v, g, scale=0.5)
+    torch.testing.assert_close(out, 0.5 * q * k * v, rtol=1e-6, atol=1e-30)
+    got = torch.autograd.grad(out, [q, k, v], torch.ones_like(out))
+    for x, y in zip(got, (k * v, q * v, q * k)):
+        torch.testing.assert_close(x, 0.5 * y, rtol=1e-6, atol=1e-30)
+    n = (1 << 24) - 1
+    state, q, k, v = (torch.randn(n, 1, 1, generator=r, device=DEV) for _ in range(4))
+    g = -torch.rand(n, 1, generator=r, device=DEV)
+    want = g.exp()[..., None] * state + k * v
+    y = linear_attention_update(state.unsqueeze(-1), q, k, v, g, scale=2.0)
+    torch.testing.assert_close(state, want, rtol=1e-6, atol=1e-6)
+    torch.testing.assert_close(y, 2 * q * want, rtol=1e-6, atol=1e-5)
+
+
+def test_states_of_more_than_2_to_the_32_elements():
+    """No tokens: the states are handed on, 17 GB of them."""
+    _say("linear attention 2^32 elements of states")
+    from motif_mamba_amd import linear_attention_fn
+    heads = (1 << 18) + 3
+    initial = torch.zeros(1, heads, 128, 128, device=DEV)
+    for at in (0, heads // 2, heads - 1):
+        initial[0, at] = torch.randn(128, 128, device=DEV)
+    x = torch.zeros(1, 0, 1, 128, device=DEV)
+    _, last = linear_attention_fn(x, x, torch.zeros(1, 0, heads, 128, device=DEV), torch.zeros(1, 0, heads, device=DEV), initial_state=initial,
+                                  return_last_state=True)
+    for at in (0, 1, heads // 2, heads - 2, heads - 1):
+        assert torch.equal(last[0, at], initial[0, at]), at
+    del initial, last
+    torch.cuda.empty_cache()

@@ -91,3 +91,12 @@ def test_block_rounds_a_value_once(dtype):
     # softplus and the product in float32: a few 2^-24
     assert ((v.double() - exact).abs() <= unit + 2.0 ** -21 * exact.abs()).all()
     assert torch.allclose(g.double(), -torch.exp(b.A_log.double()) * exact_dt, rtol=2.0 ** -20)
+
+
+@pytest.mark.parametrize("name,change", [("mm_linattn_fwd", dict(batch=1 << 23, nheads=1)), ("mm_linattn_bwd", dict(batch=1 << 23, nheads=1)),
+                                         ("mm_linattn_update", dict(batch=1 << 24, nheads=1))])
+def test_more_pairs_than_a_launch_takes(blocks, name, change):
+    base = {"mm_linattn_fwd": {**SIZES, **PTRS, "out": 4096}, "mm_linattn_update": {**TOKEN, "state_batch_stride": 256, "state_dk_stride": 16},
+            "mm_linattn_bwd": {**SIZES, **PTRS, "dout": 4096, "dq": 4096, "dk_out": 4096, "dv_out": 4096}}[name]
+    rc, msg = _call(name, _fill(blocks, name + "_params", **{**base, **change}))
+    assert rc == -2 and "too large" in msg, (rc, msg)
