@@ -801,6 +801,9 @@ void check_state(const at::Tensor &s, const at::Tensor &v, int64_t batch, int64_
     TORCH_CHECK(s.sizes() == torch::IntArrayRef({batch, heads, dk, dv}), name, " must have shape (batch, nheads, dk, dv)");
 }
 
+// The stride between tokens; a single token has none, whatever its tensor says.
+int64_t seq_stride(const at::Tensor &t) { return t.size(1) > 1 ? t.stride(1) : 0; }
+
 void *workspace_of(at::Tensor &keep, int64_t bytes, const at::Tensor &like) {
     if (bytes <= 0) return nullptr;
     keep = torch::empty({bytes}, like.options().dtype(at::ScalarType::Byte));
@@ -831,11 +834,11 @@ std::vector<at::Tensor> linattn_fwd(const at::Tensor &q, const at::Tensor &k, co
     p.initial_state = initial.defined() ? initial.data_ptr<float>() : nullptr;
     p.out = out.data_ptr();
     p.last_state = last.defined() ? last.data_ptr<float>() : nullptr;
-    p.q_batch_stride = q.stride(0); p.q_seq_stride = q.stride(1); p.q_group_stride = q.stride(2);
-    p.k_batch_stride = k.stride(0); p.k_seq_stride = k.stride(1); p.k_group_stride = k.stride(2);
-    p.v_batch_stride = v.stride(0); p.v_seq_stride = v.stride(1); p.v_head_stride = v.stride(2);
+    p.q_batch_stride = q.stride(0); p.q_seq_stride = seq_stride(q); p.q_group_stride = q.stride(2);
+    p.k_batch_stride = k.stride(0); p.k_seq_stride = seq_stride(k); p.k_group_stride = k.stride(2);
+    p.v_batch_stride = v.stride(0); p.v_seq_stride = seq_stride(v); p.v_head_stride = v.stride(2);
     p.g_batch_stride = g.stride(0); p.g_seq_stride = g.stride(1); p.g_head_stride = g.stride(2);
-    p.out_batch_stride = out.stride(0); p.out_seq_stride = out.stride(1); p.out_head_stride = out.stride(2);
+    p.out_batch_stride = out.stride(0); p.out_seq_stride = seq_stride(out); p.out_head_stride = out.stride(2);
     at::Tensor ws;
     p.workspace_bytes = mm_linattn_fwd_workspace_size(&p);
     p.workspace = workspace_of(ws, p.workspace_bytes, v);
@@ -886,11 +889,11 @@ std::vector<c10::optional<at::Tensor>> linattn_bwd(const at::Tensor &q, const at
     p.dinitial_state = ds.defined() ? ds.data_ptr<float>() : nullptr;
     p.decay_per_head = decay_per_head;
     p.segment_states = states_.has_value() && states_.value().defined() ? states_.value().data_ptr() : nullptr;
-    p.q_batch_stride = q.stride(0); p.q_seq_stride = q.stride(1); p.q_group_stride = q.stride(2);
-    p.k_batch_stride = k.stride(0); p.k_seq_stride = k.stride(1); p.k_group_stride = k.stride(2);
-    p.v_batch_stride = v.stride(0); p.v_seq_stride = v.stride(1); p.v_head_stride = v.stride(2);
+    p.q_batch_stride = q.stride(0); p.q_seq_stride = seq_stride(q); p.q_group_stride = q.stride(2);
+    p.k_batch_stride = k.stride(0); p.k_seq_stride = seq_stride(k); p.k_group_stride = k.stride(2);
+    p.v_batch_stride = v.stride(0); p.v_seq_stride = seq_stride(v); p.v_head_stride = v.stride(2);
     p.g_batch_stride = g.stride(0); p.g_seq_stride = g.stride(1); p.g_head_stride = g.stride(2);
-    p.do_batch_stride = dout.stride(0); p.do_seq_stride = dout.stride(1); p.do_head_stride = dout.stride(2);
+    p.do_batch_stride = dout.stride(0); p.do_seq_stride = seq_stride(dout); p.do_head_stride = dout.stride(2);
     at::Tensor ws;
     p.workspace_bytes = mm_linattn_bwd_workspace_size(&p);
     p.workspace = workspace_of(ws, p.workspace_bytes, v);

@@ -26,8 +26,15 @@ from ._autograd import differentiated
 from ._native import ext
 
 
+# The kernels address 64 tokens of a tensor with 32 bits.
+_SEQ_STRIDE = 1 << 22
+
+
 def _rows(t):
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+    """t with contiguous rows, and tokens less than 2^22 elements apart; copied where it is not so."""
+    if t.stride(-1) != 1 and t.shape[-1] != 1:
+        return t.contiguous()
+    return t.contiguous() if t.dim() == 4 and t.shape[1] > 1 and t.stride(1) >= _SEQ_STRIDE else t
 
 
 def _spread(log_decay, lead, v):

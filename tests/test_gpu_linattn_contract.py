@@ -326,3 +326,23 @@ def test_states_of_more_than_2_to_the_32_elements():
         assert torch.equal(last[0, at], initial[0, at]), at
     del initial, last
     torch.cuda.empty_cache()
+
+
+def test_tokens_far_apart():
+    """A layout with the tokens outermost, 2^22 elements and more from one to the next, and a single token with any stride."""
+    _say("linear attention tokens far apart")
+    from motif_mamba_amd import linear_attention_fn
+    r = torch.Generator(device=DEV).manual_seed(11)
+    for wide in (1 << 22, (1 << 22) - 1):
+        buf = torch.randn(5, 1, wide, generator=r, device=DEV).to(BF16).transpose(0, 1)
+        q, k, v, dout = (buf[..., n:n + 64].unflatten(-1, (2, 32)) for n in (0, 64, 128, 192))
+        g = -torch.rand(1, 5, 2, generator=r, device=DEV)
+        res = []
+        for copy in (False, True):
+            leaves = [(x.contiguous() if copy else x).detach().requires_grad_(True) for x in (q, k, v)]
+            out = linear_attention_fn(*leaves, g)
+            res.append((out, *torch.autograd.grad(out, leaves, dout.contiguous() if copy else dout)))
+        for x, y in zip(*res):
+            assert torch.equal(x, y)
+        one = [x[:, :1] for x in (q, k, v)]
+        assert torch.equal(linear_attention_fn(*one, g[:, :1]), res[0][0][:, :1])
