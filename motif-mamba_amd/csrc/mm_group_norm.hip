@@ -386,11 +386,12 @@ static int launch_nt(const mm_group_norm_params &p, const Plan &k, bool bwd, hip
     return launch_status("gn_sum");
 }
 
-template <typename T, int VE, int NV>
+// NT: the block sizes that plan() takes with these pieces, ascending.
+template <typename T, int VE, int NV, int... NT>
 static int launch(const mm_group_norm_params &p, const Plan &k, bool bwd, hipStream_t s) {
-    if (k.threads <= 256) return launch_nt<T, VE, NV, 256>(p, k, bwd, s);
-    if (k.threads <= 512) return launch_nt<T, VE, NV, 512>(p, k, bwd, s);
-    return launch_nt<T, VE, NV, 1024>(p, k, bwd, s);
+    int rc = MM_OK;
+    (void)((k.threads <= NT && (rc = launch_nt<T, VE, NV, NT>(p, k, bwd, s), true)) || ...);
+    return rc;
 }
 
 template <typename T>
@@ -398,13 +399,14 @@ static int run(const mm_group_norm_params &p, bool bwd, hipStream_t s) {
     const Plan k = plan(p, bwd);
     constexpr int V = 16 / sizeof(T);
     if (vectors(p, bwd)) {
-        if (k.nv == 1) return launch<T, V, 1>(p, k, bwd, s);
-        if (k.nv == 2) return launch<T, V, 2>(p, k, bwd, s);
-        return launch<T, V, 4>(p, k, bwd, s);
+        if (k.nv == 1) return launch<T, V, 1, 256>(p, k, bwd, s);
+        if constexpr (sizeof(T) == 4)   // 16,384 16-bit channels are two pieces of 1,024 threads
+            if (k.nv > 2) return launch<T, V, 4, 1024>(p, k, bwd, s);
+        return launch<T, V, 2, 256, 512, 1024>(p, k, bwd, s);
     }
-    if (k.nv <= 2) return launch<T, 1, 2>(p, k, bwd, s);
-    if (k.nv <= 4) return launch<T, 1, 4>(p, k, bwd, s);
-    return launch<T, 1, 16>(p, k, bwd, s);
+    if (k.nv <= 2) return launch<T, 1, 2, 256>(p, k, bwd, s);
+    if (k.nv <= 4) return launch<T, 1, 4, 256, 512, 1024>(p, k, bwd, s);
+    return launch<T, 1, 16, 512, 1024>(p, k, bwd, s);
 }
 
 static int64_t bwd_bytes(const mm_group_norm_params &p) {
