@@ -766,7 +766,7 @@ __global__ void __launch_bounds__(kBlock) la_decay_grad(const float *a, const fl
                                                         int64_t blocks, int heads, int C, bool has_last, const void *g, int64_t g_batch,
                                                         int64_t g_seq, int64_t g_head, float *tmp, void *out, mm_dtype gtype) {
     __shared__ float sa[kBlock], sf[kBlock], se[kBlock], zc[kBlock / 16];
-    __shared__ int forgets[kBlock], chunk_forgets[kBlock / 32];
+    __shared__ int chunk_forgets[kBlock / 32];
     const int64_t blk = blockIdx.y, bh = blockIdx.x, t = blk * kBlock + threadIdx.x;
     const int tid = threadIdx.x, chunks = kBlock / C;
     const bool live = t < seqlen;
@@ -774,19 +774,18 @@ __global__ void __launch_bounds__(kBlock) la_decay_grad(const float *a, const fl
     sa[tid] = (live ? a[bh * seqlen + t] : 0.f) + ae;
     sf[tid] = live ? f[bh * seqlen + t] : 0.f;
     se[tid] = ae;
-    forgets[tid] = live && decode_g(load_g_raw(g, gtype, bh / heads * g_batch + t * g_seq + bh % heads * g_head), gtype) == -128.f;
+    const bool forgets = live && decode_g(load_g_raw(g, gtype, bh / heads * g_batch + t * g_seq + bh % heads * g_head), gtype) == -128.f;
+    const uint64_t all_forgets = __ballot(forgets);   // of 64 tokens: one chunk or two
+    if (tid % C == 0) chunk_forgets[tid / C] = (all_forgets >> tid % 64 & (C == 64 ? ~uint64_t(0) : (uint64_t(1) << C) - 1)) != 0;
     __syncthreads();
     if (tid < chunks) {   // the chunks' totals
         float E = 0.f, F = 0.f;
-        int any = 0;
         for (int n = 0; n < C; ++n) {
             E += se[tid * C + n];
             F += sf[tid * C + n];
-            any |= forgets[tid * C + n];
         }
         zc[tid] = E;
         zc[chunks + tid] = F;
-        chunk_forgets[tid] = any;
     }
     __syncthreads();
     if (tid == 0) {
@@ -804,10 +803,10 @@ __global__ void __launch_bounds__(kBlock) la_decay_grad(const float *a, const fl
     const int c0 = tid / C * C;
     float s = zc[tid / C];
     for (int n = c0; n < tid; ++n) s += sf[n];
-    int end = tid + 1;
-    while (end < c0 + C && !forgets[end]) ++end;
+    const uint64_t behind = all_forgets >> tid % 64 >> 1;
+    const int end = min(c0 + C, tid + 1 + (behind ? __builtin_ctzll(behind) : 64));
     for (int n = end - 1; n >= tid; --n) s += sa[n];
-    if (forgets[tid]) s = 0.f;
+    if (forgets) s = 0.f;
     if (tmp) tmp[bh * seqlen + t] = s;
     else store_g(out, gtype, (bh / heads * seqlen + t) * heads + bh % heads, s);
 }
