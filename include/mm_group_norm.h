@@ -54,6 +54,8 @@ typedef struct mm_group_norm_params {
 } mm_group_norm_params;
 
 int mm_group_norm_fwd(const mm_group_norm_params *params, void *stream);
+/* Workspace bytes (0: none needed). They depend on which pointers are set, on the alignment of the tensors' and on their row
+ * strides, and on the current device's compute-unit count: query with the call's own parameters, its device current. */
 int64_t mm_group_norm_bwd_workspace_size(const mm_group_norm_params *params);
 int mm_group_norm_bwd(const mm_group_norm_params *params, void *stream);
 

@@ -48,8 +48,9 @@ typedef struct mm_linattn_fwd_params {
     const float *initial_state;  /* (batch, nheads, dk, dv) or NULL (zeros) */
     void *out;                   /* (batch, seqlen, nheads, dv) */
     float *last_state;           /* (batch, nheads, dk, dv) or NULL */
-    void *workspace;             /* mm_linattn_fwd_workspace_size() bytes, 16-byte aligned; NULL: one pass per row.
-                                  * Afterwards it holds the states that the row's segments start from. */
+    void *workspace;             /* mm_linattn_fwd_workspace_size() bytes, 16-byte aligned. Afterwards it holds the states that
+                                  * the row's segments start from. NULL, or fewer bytes: one pass per row, nothing is kept
+                                  * (and nothing of it may be handed to the backward as segment_states). */
     int64_t workspace_bytes;
     int64_t q_batch_stride, q_seq_stride, q_group_stride;
     int64_t k_batch_stride, k_seq_stride, k_group_stride;
@@ -71,7 +72,8 @@ typedef struct mm_linattn_bwd_params {
     void *dv_out;                /* contiguous (batch, seqlen, nheads, dv) */
     void *dlog_decay;            /* contiguous (batch, seqlen, nheads), or (nheads,) with decay_per_head; or NULL */
     float *dinitial_state;       /* (batch, nheads, dk, dv) or NULL */
-    const void *segment_states;  /* the forward's workspace after the same call, or NULL (computed again) */
+    const void *segment_states;  /* the forward's workspace, of the full size, after a call with the same sizes, inputs and
+                                  * device, or NULL (computed again) */
     int32_t decay_per_head;      /* log_decay is one value per head: dlog_decay is summed over batch and seqlen */
     void *workspace;             /* mm_linattn_bwd_workspace_size() bytes, 16-byte aligned (required) */
     int64_t workspace_bytes;
@@ -100,8 +102,9 @@ typedef struct mm_linattn_update_params {
     int64_t g_batch_stride, g_head_stride;
 } mm_linattn_update_params;
 
-/* Workspace bytes (0: none needed). They depend on the current device's compute-unit count: query with
- * the device of the call current. */
+/* Workspace bytes (0: none needed). They depend on the sizes and on the current device's compute-unit count: query with
+ * the device of the call current. The backward's also depend on whether dlog_decay and segment_states are NULL: query with
+ * those pointers set as in the call. */
 int64_t mm_linattn_fwd_workspace_size(const mm_linattn_fwd_params *params);
 int64_t mm_linattn_bwd_workspace_size(const mm_linattn_bwd_params *params);
 

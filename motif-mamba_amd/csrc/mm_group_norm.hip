@@ -1,14 +1,17 @@
 // mm_group_norm.hip -- gfx950 group norm of a row's channel groups with a gate or an activation, channels
 // last, forward and backward (mm_group_norm.h has the formulas).
 //
-// HBM-bound: every tensor is read once and written once. A group's elements lie in the registers of `lanes`
-// threads from the load to the store, so that the mean, the squares of the differences from it and the outputs
-// need no second read; sums over a group's threads are taken by lane swaps, past 64 threads through LDS. A thread
-// keeps its columns over the rows of its block: it reads weight and bias once, and the backward adds its rows'
-// dweight and dbias in registers, one partial row per block, which a second kernel sums in order (no atomics:
-// the same bits on every call).
-// Measured, bfloat16 (a large copy reaches 4.9 TB/s): 16,384 x 5,120 in one group, gated, forward 139 us (3.6 TB/s); 16,384 x
-// 1,536 in 24 groups, forward 40 us (3.8 TB/s), backward 86 us + 7 us for the sums (2.9 TB/s).
+// HBM-bound: every tensor is read once and written once. A group's elements stay with the `lanes` threads that
+// loaded them until the store, so that the mean, the squares of the differences from it and the outputs
+// need no second read. They lie in registers, but for large groups: a block of 1,024 threads has 128 for each and spills
+// the rest to scratch (backward: 16-bit groups past 8,192 channels some 290, float32 past 4,096 39 and past 8,192 327, element
+// by element up to 395; forward: float32 past 8,192 36, element by element up to 157). Sums over a group's threads
+// are taken by lane swaps, past 64 threads through LDS. A thread keeps its columns over the rows of its block: it
+// reads weight and bias once, and the backward adds its rows' dweight and dbias in registers, one partial row per
+// block, which a second kernel sums in order (no atomics: the same bits on every call).
+// Measured, bfloat16 (a large copy reaches 4.9 TB/s): 16,384 x 5,120 in one group, gated, forward 140 us (3.6 TB/s); 16,384 x
+// 1,536 in 24 groups, forward 36 us (4.2 TB/s), backward 84 us + 7 us for the sums (2.8 TB/s; blocks of 32 groups, so that a
+// quarter of their lanes have none).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

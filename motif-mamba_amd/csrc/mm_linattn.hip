@@ -1,5 +1,6 @@
 // mm_linattn.hip -- gfx950 linear attention with one decay for each head: chunked forward and backward
-// (mm_linattn_dev.h has the mathematics and the operands' layouts), and the single-token step.
+// (mm_linattn_dev.h has the mathematics and the operands' layouts). The single-token step and the plan of a call are
+// in mm_linattn_api.hip.
 //
 // A walk takes one (batch row, head), or a segment of it, through its chunks in order, the state in the
 // accumulators of its waves: every tensor is read once and every output written once. Rows with too few
@@ -157,11 +158,14 @@ __device__ __forceinline__ void infinite_rows(char *smem) {
 //
 // Per chunk: stage X, Y and V; scores (each wave its tiles, into M) and the product with the state; the product of M and V,
 // the state's update, the outputs. The waves share X, Y and M through LDS and split V's columns, so that a wave's part of the
-// state never leaves its accumulators. At dk 128, dv 64, bfloat16 a wave issues 102 matrix and some 510 other vector
-// instructions per 64 tokens and the LDS works 2,900 cycles; with 2 workgroups on a CU (202 registers, 61 KB) a chunk of both
-// takes some 5.7 us, of one alone 4.0: latency between the three barriers bounds it, no unit is busy more than 60 %.
-// 4 x 4,096 tokens, 80 heads: 319 us, 1.1 TB/s of its 360 MB and 400 TFLOP/s on the matrix cores, split planes counted.
-// Three workgroups at 168 registers spill (457 us for 128 heads against 365), chunks of 32 tokens gain nothing (394).
+// state never leaves its accumulators. At dk 128, dv 64, bfloat16 a wave issues 124 matrix and some 940 other vector
+// instructions per 64 tokens and the LDS works 3,200 cycles, a third of them bank conflicts; with 2 workgroups on a CU (203
+// registers, 69 KB) a chunk of both takes 5.6 us, of one alone 4.2. While a CU has work its vector units are busy 44 % of the
+// time, its matrix cores 23 %, its LDS 38 %: with one or two waves per SIMD nothing covers a wave's latencies between the three
+// barriers. 4 x 4,096 tokens, 80 heads: 361 us, 1.0 TB/s of its 360 MB and 460 TFLOP/s on the matrix cores, split planes counted.
+// With two planes of the state, three workgroups at 168 registers spilled (457 us for 128 heads against 365) and chunks of 32
+// tokens gained nothing (394). Rows of 128 x 128 spill 8 to 13 registers, with DOT 38 to 43.
+// 64 x 64 has the registers and the LDS of three workgroups on a CU (with DOT the LDS of two, but for float16).
 template <typename T, int KD, int NC, bool DOT, bool VEC, bool F32>
 __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(KD * NC == 64 ? 3 : 2, KD * NC == 64 ? 3 : 2))) la_walk(const WalkArgs) {
     constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, W = 64 * NC;
@@ -313,7 +317,7 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(K
 
 // What each segment but the last one (REV: the first one) of a row adds to the state: sum of y_t (decay to the
 // segment's end) v_t^T into st[bh][seg], and the segment's own decay into decay[bh][seg]. About 2 us per chunk and CU at
-// dk 128 (7 of 8 segments of 64 pairs, dv 128, L 4,096: 55 us).
+// dk 128 (7 of 8 segments of 64 pairs, dv 128, L 4,096: 52 us).
 template <typename T, int KD, bool REV, bool VEC>
 __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 2 ? 3 : 2, sizeof(T) == 2 ? 3 : 2))) la_segments(const WalkArgs) {
     constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, W = 64;
@@ -432,9 +436,11 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(s
 // state for dv (rows dk, columns dv), waves 4 to 7 its transpose for dk: two walks over the same tiles, each in code of
 // its own with the same barriers.
 //
-// Every q, k, v and dout row is read once for both. One workgroup of 8 waves per CU (90 KB of LDS and 200 to 250 registers at
-// dk 128), 7.5 us per 64 tokens with dv 64, bound by vector instructions (some 1,050 per wave and chunk, two waves per SIMD):
-// 8 x 2,048 tokens, 24 heads, 242 us; 4 x 4,096 tokens, 16 heads with dv 128, 161 us.
+// Every q, k, v and dout row is read once for both. One workgroup of 8 waves per CU (102 KB of LDS and 224 registers at dk 128,
+// dv 64; 118 KB, 256 registers and 6 to 12 spilled at 128 x 128), 7.2 us per 64 tokens with dv 64. A wave issues 130 matrix and some 1,135
+// other vector instructions per chunk, two waves per SIMD: the vector units are busy 55 % of the time, the matrix cores 25 %, the LDS
+// 38 % (a third of it conflicts), and a wave waits a third of its own. 8 x 2,048 tokens, 24 heads, 229 us; 4 x 4,096 tokens, 16 heads
+// with dv 128, 181 us.
 //
 // FOR_K: the walk of dk, X = v, Y = do, V = q; else that of dv, X = k, Y = q, V = do. KX: X's padded row length, KV: V's.
 template <typename T, int KD, int VD, bool VEC, bool F32, bool FOR_K>

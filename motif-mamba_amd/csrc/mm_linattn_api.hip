@@ -133,8 +133,12 @@ constexpr int64_t kMostPairs = (int64_t(1) << 23) - 1, kMostTokenPairs = (int64_
 // Segments of a row, by the time that a call takes with n of them, in steps of a chunk of one workgroup alone on its CU
 // (about 3.7 us at dk 128, dv 64, bfloat16). Two workgroups on a CU take 1.45 steps per chunk of both. With n > 1 a pass over
 // k and v before (0.9 of a step per chunk for few workgroups, 0.5 of one per chunk and CU for many), its join (about 2 steps),
-// and the states' traffic, 16 bytes per element and segment at some 4.5 TB/s. Measured: 320 pairs (4 x 80 heads), L 4,096: one segment 322 us, two 274 + 128;
-// 192 pairs, L 2,048: one 103 us, three 86 + 45; 64 pairs (dk = dv = 128), L 4,096: 100 + 70 us with eight, 240 with one.
+// and the states' traffic, 16 bytes per element and segment at some 4.5 TB/s. Fitted, before the state had its third plane, to: 320 pairs
+// (4 x 80 heads), L 4,096: one segment 322 us, two 274 + 128; 192 pairs, L 2,048: one 103 us, three 86 + 45; 64 pairs (dk = dv = 128),
+// L 4,096: 100 + 70 us with eight, 240 with one. The same rule serves the other types and sizes, for which nothing was fitted: at
+// dk and dv up to 64 a CU holds three workgroups, and float16 and float32 have twice the chunks per token (both sides'
+// counts in steps grow alike; the states' traffic then weighs too much). 64 segments at most: the join reads a row's segments one after
+// another (64 of 65,536 tokens of 40 heads: 43 us of 1,043, in float32).
 static void segments(int64_t pairs, int64_t seqlen, int64_t size, int *segs, int64_t *len) {
     const int64_t cus = device_simds() / 4, blocks = std::max<int64_t>(1, (seqlen + kBlockTokens - 1) / kBlockTokens);
     double best = 0.0;

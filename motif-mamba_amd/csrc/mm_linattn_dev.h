@@ -15,7 +15,7 @@
 // inputs as three (both exact), and every float32 factor, the state, the decayed scores and the decayed rows
 // that the state is built from, as three (relative error 2^-25, for every input type). So all of them are
 // float32 from end to end and 16-bit outputs are rounded once. (Two planes, 2^-17, for the state and the scores of 16-bit
-// inputs took 316 us where three take 358, 4 x 4,096 tokens of 80 heads at 128 x 64 in bfloat16, and moved outputs near the
+// inputs took 316 us where three take 361, 4 x 4,096 tokens of 80 heads at 128 x 64 in bfloat16, and moved outputs near the
 // middle of two 16-bit numbers to the wrong one.)
 //
 // Lane layouts (l the lane, g = l / 16, i = l % 16; checked on the card): an accumulator tile holds column
@@ -52,7 +52,8 @@ constexpr int kBlock = 256;      // tokens between two kept states (see the deca
 // Tiles in LDS are rows of D elements (64 or 128; 64 scores), cut into units of 4 (8 bytes). Both ways that operands
 // are read, 16 rows of one unit (frag_row) and 4 rows of 4 units (frag_tr), should touch the 16 units of a 128-byte
 // line each once, so unit u of row r lies at u ^ swizzle(r): r's low two bits move a unit between the line's quarters,
-// its next two within one. Rows padded by 16 bytes instead cost 42 % of all LDS cycles in bank conflicts.
+// its next two within one. Bank conflicts are still 31 % of the walks' LDS cycles (rows padded by 16 bytes instead: 42 %); which
+// access makes them has not been told apart.
 __device__ __forceinline__ constexpr int swizzle(int row) { return (row & 3) << 2 | (row >> 2 & 3); }
 // 16 bytes stand between blocks of 16 rows: two blocks' reads at one lane's address are then no constant distance apart that one
 // instruction could span. (The compiler would join them, and move every half into its operand afterwards.)
@@ -912,7 +913,7 @@ __device__ __forceinline__ void store_element(float x, const __amdgpu_buffer_rsr
 // The wave's C x 16 NC outputs to rows of T, or of float32 (F32). In 16-byte pieces (VEC) they go
 // through the wave's own columns of a tile that no other wave reads any more: 16-bit rows as they lie there, the 16-bit types'
 // float32 shares half a chunk at a time, each row in the place of two rows of the tile. float32 tensors' rows go out by the lane, in
-// 64-byte runs (through LDS: 1,025 us against 990 for 65,536 tokens of 40 heads).
+// 64-byte runs (through LDS 3 % slower on one card, 65,536 tokens of 40 heads; cards differ by as much).
 template <typename T, int C, int NC, int LDV, bool VEC, bool F32>
 __device__ __forceinline__ void store_out(const f32x4 (&O)[C / 16][NC], void *out, uint32_t stride, int t0, int rows, int cols,
                                           u16 *tile, int col, int lane) {

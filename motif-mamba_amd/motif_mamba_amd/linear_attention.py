@@ -13,7 +13,8 @@ decays by ``exp(dt_t A_h)`` (the state-space dual of the scan) passes ``q=C, k=B
 float32, float16 and bfloat16; log_decay may have a dtype of its own (float32 is advised: a decay's
 error is raised to the power of its memory). Sums, scores and states are float32 from end to end; 16-bit
 outputs are rounded once. log_decay is meant to be at most 0; -inf forgets the state, so a packed batch
-marks each document's first token with it.
+marks each document's first token with it (below -128 counts as that, above 128 as an infinite growth).
+Infinite inputs give the outputs and states of the recurrence, slowly.
 
 dk and dv up to 128 (else NotImplementedError).
 """
