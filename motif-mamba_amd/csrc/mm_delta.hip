@@ -1,0 +1,1244 @@
+// mm_delta.hip -- gfx950 gated delta rule: chunked forward and backward on the matrix cores. The single-token step and the plan of
+// a call are in mm_delta_api.hip; operand layouts, planes and decays are the linear attention's (mm_linattn_dev.h).
+//
+// The mathematics. A chunk of C tokens starts from the state S (dk x dv). With c_i the sum of log_decay up to token i, c_end its
+// total, D_ij = exp(c_i - c_j) for i >= j, B = diag(beta), N the strict lower triangle of K K^T . D and M the lower one of
+// scale Q K^T . D:
+//     X = V - diag(e^c) K S            what the tokens would correct if they did not see each other
+//     (I + N B) Z = X,  U = B Z        z_i = v_i - S'^T k_i
+//     O = scale diag(e^c) Q S + M U,   S' = e^c_end S + K^T diag(e^(c_end - c)) U
+// P = -(I + N B)^-1 N is strictly lower triangular and gives Z = X + P B X, without a division by beta, and the gradient's
+// transposed system as well: with R the gradient of S',
+//     dU = M^T dO + diag(e^(c_end - c)) K R,   G = dU + P^T B dU,   dV = dX = B G,   dbeta_i = G_i . Z_i
+//     R' = e^c_end R + scale Q^T diag(e^c) dO - K^T diag(e^c) dV
+//     dQ = scale diag(e^c) dO S^T + A K,                    A = the lower triangle of scale dO U^T . D
+//     dK = A^T Q + E K + E^T K - diag(e^c) dV S^T + diag(e^(c_end - c)) U R^T,   E = minus the strict one of dV U^T . D
+// P and M need no state: dr_prep makes them for all chunks at once, dr_walk carries the state through a row's chunks, dr_back the
+// state's gradient back, and dr_grad takes dQ and dK chunk by chunk from the kept S, R, Z and dV, again all chunks at once.
+//
+// Exactness: as in the linear attention, every float32 factor (S, R, P, M, U, dV and the decayed scores) enters its product as
+// three bfloat16 planes (2^-25), for every input type; 16-bit results are rounded once.
+//
+// Built once per input type: this file for float32, mm_delta_f16.hip / mm_delta_bf16.hip, which set MM_DELTA_TYPE.
+#ifndef MM_DELTA_TYPE
+#define MM_DELTA_TYPE float
+#endif
+
+#include <algorithm>
+
+#include "mm_delta_host.h"
+#include "mm_linattn_dev.h"
+
+namespace mm {
+namespace dr {
+
+using namespace la;
+
+constexpr int kWaves = 4, kThreads = 64 * kWaves;
+
+// ---- triangles as operands -----------------------------------------------------------------------
+
+// The 32-wide A operands of a triangle of 16 x 16 tiles: row tile t, columns 32 j .. 32 j + 31, those that hold a tile of it. LOWER:
+// 2 j <= t, its transpose 2 j + 1 >= t.
+template <int C> constexpr int kFrags = C == 64 ? 6 : 2;
+template <int C, bool LOWER>
+constexpr bool has_frag(int t, int j) { return LOWER ? 2 * j <= t : 2 * j + 1 >= t; }
+template <int C, bool LOWER>
+constexpr int frag_at(int t, int j) { return LOWER ? (t < 2 ? t : 2 * t - 2 + j) : (C == 32 ? t : t < 2 ? 2 * t + j : t + 2); }
+template <int C> constexpr int kImage = kFrags<C> * kPlanes * 512;   // elements
+
+__device__ __forceinline__ bf16x8 image_frag(const u16 *img, int frag, int plane, int lane) {
+    return *reinterpret_cast<const bf16x8 *>(img + (frag * kPlanes + plane) * 512 + lane * 8);
+}
+
+// ---- a workgroup's place -------------------------------------------------------------------------
+
+struct Spot {
+    int b, h, bh;
+};
+template <typename A>
+__device__ __forceinline__ Spot spot_of(const A &a, unsigned pair) {
+    Spot p;
+    p.bh = afresh(int(pair));
+    p.h = afresh(int(pair % unsigned(a.heads)));
+    p.b = afresh(int(pair / unsigned(a.heads)));
+    return p;
+}
+__device__ __forceinline__ Gates gates_of(const Gate &g, const Spot &p) {
+    const int64_t size = g.type == MM_FLOAT32 ? 4 : 2;
+    return Gates{g.p ? afresh(static_cast<const char *>(g.p) + (p.b * g.batch + p.h * g.head) * size) : nullptr, afresh(g.seq * size), mm_dtype(afresh(int(g.type)))};
+}
+template <int C>
+__device__ __forceinline__ uint32_t load_gate(const Gates &g, int t0, int end, int lane) {
+    return g.p ? g.template load<C>(t0, end, lane) : 0u;
+}
+__device__ __forceinline__ float decode_beta(uint32_t w, mm_dtype t) {
+    return t == MM_FLOAT32 ? __uint_as_float(w) : t == MM_BFLOAT16 ? __uint_as_float(w << 16) : elem_f32<f16_t>(w);
+}
+
+// A chunk's decays (without the scale), beta, and scale e^c.
+template <int C>
+struct Chunk {
+    Decays<C> d;
+    float beta[C], inq[C];
+};
+// One wave makes them; g and b: the lane's token's bits.
+template <int C>
+__device__ __forceinline__ void make_chunk(Chunk<C> &k, uint32_t g, mm_dtype gtype, uint32_t b, mm_dtype btype, float scale, int lane) {
+    make_decays<C>(k.d, decode_g(g, gtype), 1.f, lane);
+    if (C == 64 || lane < C) {
+        k.beta[lane] = decode_beta(b, btype);
+        k.inq[lane] = k.d.in[lane] * scale;
+    }
+}
+
+// What a walk needs of it: no factors between two tokens.
+template <int C>
+struct __attribute__((aligned(16))) Steps {
+    float in[C], out[C], beta[C], inq[C];   // e^c, e^(c_end - c), beta, scale e^c
+    float hi[C], lo[C];                     // c
+    float all;                              // e^c_end
+};
+template <int C>
+__device__ __forceinline__ void make_steps(Steps<C> &k, uint32_t g, mm_dtype gtype, uint32_t b, mm_dtype btype, float scale, int lane) {
+    const double c = prefix_f64(double(decode_g(g, gtype))), all = readlane_f64(c, C - 1);
+    const float hi = float(c), in = exp_f32(hi);
+    if (C == 64 || lane < C) {
+        k.in[lane] = in;
+        k.out[lane] = exp_f32(float(all - c));
+        k.beta[lane] = decode_beta(b, btype);
+        k.inq[lane] = in * scale;
+        k.hi[lane] = hi;
+        k.lo[lane] = float(c - double(hi));
+        if (lane == C - 1) k.all = in;
+    }
+}
+
+// ---- products ------------------------------------------------------------------------------------
+
+// s += the tiles L of X Y^T, X in PX planes and Y in PY: column i the row token 16 O + i of X, rows 4g + r the tokens of Y.
+template <int PX, int PY, int C, int D, typename L>
+__device__ __forceinline__ void tile_products(f32x4 *s, const u16 *X, const u16 *Y, int lane) {
+    constexpr int PL = kTile<C, D>;
+    const int g = lane >> 4, i = lane & 15;
+#pragma unroll
+    for (int k = 0; k < D / 32; ++k) {
+        bf16x8 a[L::N][PY], b[L::N][PX];
+#pragma unroll
+        for (int j = 0; j < L::N; ++j) {
+#pragma unroll
+            for (int p = 0; p < PX; ++p) {
+                if (j > 0 && L::O(j) == L::O(j - 1)) b[j][p] = b[j - 1][p];
+                else b[j][p] = frag_row<D>(X + p * PL, 16 * L::O(j), k, g, i);
+            }
+#pragma unroll
+            for (int p = 0; p < PY; ++p) a[j][p] = frag_row<D>(Y + p * PL, 16 * L::n(j), k, g, i);
+        }
+#pragma unroll
+        for (int p = 0; p < PY; ++p)
+#pragma unroll
+            for (int q = 0; q < PX; ++q)
+                if (p + q < kPlanes)
+#pragma unroll
+                    for (int j = 0; j < L::N; ++j) s[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[j][p], b[j][q], s[j], 0, 0, 0);
+    }
+}
+// The waves' shares of a chunk's lower triangle of tiles.
+template <int C, typename F>
+__device__ __forceinline__ void each_tile(int wave, F &&f) {
+    if constexpr (C == 64) {
+        switch (wave) {
+            case 0: f(Tiles<3, 0, 3, 1, 3, 2>{}); break;
+            case 1: f(Tiles<2, 0, 2, 1, 2, 2>{}); break;
+            case 2: f(Tiles<1, 0, 1, 1, 3, 3>{}); break;
+            default: f(Tiles<0, 0>{});
+        }
+    } else {
+        switch (wave) {
+            case 0: f(Tiles<1, 0>{}); break;
+            case 1: f(Tiles<1, 1>{}); break;
+            case 2: f(Tiles<0, 0>{});
+        }
+    }
+}
+
+// Rows of accumulators times w as B operands in three planes: f[j] holds the tokens 32 j .. 32 j + 31.
+template <int C, int NC>
+__device__ __forceinline__ void split_rows(bf16x8 (&f)[C / 32][NC][kPlanes], const f32x4 (&x)[C / 16][NC], const float *w, int lane) {
+    const int g = lane >> 4;
+#pragma unroll
+    for (int j = 0; j < C / 32; ++j) {
+        const f32x4 w0 = *reinterpret_cast<const f32x4 *>(w + 32 * j + 4 * g), w1 = *reinterpret_cast<const f32x4 *>(w + 32 * j + 16 + 4 * g);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            float y[8];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                y[r] = x[2 * j][c][r] * w0[r];
+                y[4 + r] = x[2 * j + 1][c][r] * w1[r];
+            }
+            split8(y, f[j][c]);
+        }
+    }
+}
+// O += T f, T a triangle's image.
+template <int C, int NC, bool LOWER, int PF>
+__device__ __forceinline__ void triangle(f32x4 (&O)[C / 16][NC], const u16 *img, const bf16x8 (&f)[C / 32][NC][PF], int lane) {
+#pragma unroll
+    for (int j = 0; j < C / 32; ++j) {
+        bf16x8 a[C / 16][kPlanes];
+#pragma unroll
+        for (int t = 0; t < C / 16; ++t)
+            if (has_frag<C, LOWER>(t, j))
+#pragma unroll
+                for (int p = 0; p < kPlanes; ++p) a[t][p] = image_frag(img, frag_at<C, LOWER>(t, j), p, lane);
+#pragma unroll
+        for (int p = 0; p < kPlanes; ++p)
+#pragma unroll
+            for (int q = 0; q < PF; ++q)
+                if (p + q < kPlanes)
+#pragma unroll
+                    for (int t = 0; t < C / 16; ++t)
+                        if (has_frag<C, LOWER>(t, j))
+#pragma unroll
+                            for (int c = 0; c < NC; ++c)
+                                O[t][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[t][p], f[j][c][q], O[t][c], 0, 0, 0);
+    }
+}
+// S += Y^T f, Y a tile of the inputs' rows.
+template <typename T, int C, int KD, int NC>
+__device__ __forceinline__ void add_rows(f32x4 (&S)[KD / 16][NC], const u16 *Y, const bf16x8 (&f)[C / 32][NC][kPlanes], int lane) {
+    constexpr int PL = kTile<C, KD>, PI = Cfg<T>::in, KB = PI > 1 ? 2 : 4;
+    const int g = lane >> 4, i = lane & 15;
+#pragma unroll
+    for (int j = 0; j < C / 32; ++j)
+#pragma unroll
+        for (int b = 0; b < KD / 16; b += KB) {
+            bf16x8 a[KB][PI];
+#pragma unroll
+            for (int k = 0; k < KB; ++k)
+#pragma unroll
+                for (int p = 0; p < PI; ++p) a[k][p] = frag_tr<KD>(Y + p * PL, 32 * j, 16 * (b + k), g, i);
+#pragma unroll
+            for (int p = 0; p < PI; ++p)
+#pragma unroll
+                for (int q = 0; q < kPlanes; ++q)
+                    if (p + q < kPlanes)
+#pragma unroll
+                        for (int k = 0; k < KB; ++k)
+#pragma unroll
+                            for (int c = 0; c < NC; ++c)
+                                S[b + k][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[k][p], f[j][c][q], S[b + k][c], 0, 0, 0);
+        }
+}
+// A tile of the inputs' rows in the accumulators' layout, from the wave's columns.
+template <typename T, int C, int NC, int LDV, typename F>
+__device__ __forceinline__ void tile_columns(const u16 *V, int col, int lane, F &&f) {
+    constexpr int PL = kTile<C, LDV>, PI = Cfg<T>::in;
+    const int g = lane >> 4, i = lane & 15;
+#pragma unroll
+    for (int j = 0; j < C / 32; ++j)
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            float x[8], y[8];
+            unpack_frag(frag_tr<LDV>(V + (PI - 1) * PL, 32 * j, col + 16 * c, g, i), x);
+#pragma unroll
+            for (int p = PI - 2; p >= 0; --p) {
+                unpack_frag(frag_tr<LDV>(V + p * PL, 32 * j, col + 16 * c, g, i), y);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] += y[e];
+            }
+            f(j, c, x);
+        }
+}
+
+// ---- P and M -------------------------------------------------------------------------------------
+
+// Row pitch of the float32 triangles in LDS: rows of one column lie 4 banks apart.
+template <int C> constexpr int kPitch = C + 4;
+
+// A triangle in `f` (row-major, pitch kPitch; 0 above the diagonal in the tiles on it, tiles above it not written) as operands, TR: its
+// transpose.
+template <int C, bool TR>
+__device__ __forceinline__ void write_image(char *dst, const float *f, int wave, int lane) {
+    const int g = lane >> 4, i = lane & 15;
+#pragma unroll
+    for (int t = 0; t < C / 16; ++t)
+#pragma unroll
+        for (int j = 0; j < C / 32; ++j)
+            if (has_frag<C, !TR>(t, j)) {
+                const int n = frag_at<C, !TR>(t, j);
+                if (n % kWaves != wave) continue;
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int o = 2 * j + e / 4, a = 16 * t + i, b = 16 * o + 4 * g + e % 4;   // tile o
+                    x[e] = (TR ? o >= t : o <= t) ? f[(TR ? b : a) * kPitch<C> + (TR ? a : b)] : 0.f;
+                }
+                bf16x8 p[kPlanes];
+                split8(x, p);
+#pragma unroll
+                for (int q = 0; q < kPlanes; ++q)
+                    *reinterpret_cast<bf16x8 *>(dst + ((n * kPlanes + q) * 64 + lane) * 16) = p[q];
+            }
+}
+
+// P (and M) of every chunk, as operand images; REV: P, P^T and M^T for the backward (P into img_a's first half... see the plan).
+// One workgroup per chunk. The triangles are made in float32: the diagonal tiles of P by substitution, row by row, those of a column
+// block below by 16 x 16 products on v_mfma_f32_16x16x4_f32, which keeps them float32.
+template <typename T, int KD, bool REV, bool VEC>
+__global__ void __launch_bounds__(kThreads) dr_prep(const Args) {
+    constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, CT = C / 16, LD = kPitch<C>;
+    typedef Stage<T, C, KD, kThreads, VEC> SX;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    u16 *K = reinterpret_cast<u16 *>(smem), *Q = K + PI * kTile<C, KD>;
+    float *N = reinterpret_cast<float *>(smem), *P = N + C * LD, *M = P + C * LD;   // over K and Q, once those are read
+    constexpr int kTiles = 2 * 2 * PI * kTile<C, KD>, kTri = 3 * C * LD * 4;
+    Chunk<C> *ck = reinterpret_cast<Chunk<C> *>(smem + (kTiles > kTri ? kTiles : kTri));
+    auto args = [] { return own_args<Args>(); };
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid & 63, g = lane >> 4, i = lane & 15;
+    const int64_t total = [&] { const Args a = args(); return a.batch * a.heads * a.chunks; }();
+    for (int64_t id = blockIdx.x; id < total; id += gridDim.x) {
+        // Heads next to each other: those of a group read the same rows of q and k.
+        int chunk;
+        Spot p;
+        {
+            const Args a = args();
+            const int64_t bc = id / a.heads;
+            chunk = afresh(int(bc % a.chunks));
+            p = spot_of(a, unsigned(bc / a.chunks * a.heads + id % a.heads));
+        }
+        const int t0 = chunk * C, end = int(args().seqlen), rows = min(C, end - t0);
+        __syncthreads();
+        {
+            const Args a = args();
+            SX sk, sq;
+            sk.load(rows_of<T>(a.k, p.b, p.h, a.dk), t0, rows, tid);
+            sq.load(rows_of<T>(a.q, p.b, p.h, a.dk), t0, rows, tid);
+            if (wave == kWaves - 1)
+                make_chunk<C>(*ck, load_gate<C>(gates_of(a.g, p), t0, end, lane), a.g.type, load_gate<C>(gates_of(a.beta, p), t0, end, lane), a.beta.type, a.scale, lane);
+            sk.store(K, tid);
+            sq.store(Q, tid);
+        }
+        __syncthreads();
+        f32x4 n[3], m[3];
+        each_tile<C>(wave, [&](auto Lc) {
+            typedef decltype(Lc) L;
+#pragma unroll
+            for (int j = 0; j < L::N; ++j) n[j] = m[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            tile_products<PI, PI, C, KD, L>(n, K, K, lane);
+            tile_products<PI, PI, C, KD, L>(m, Q, K, lane);
+        });
+        __syncthreads();
+        const float scale = args().scale;
+        each_tile<C>(wave, [&](auto Lc) {
+            typedef decltype(Lc) L;
+            static_for<0, L::N>([&](auto Jc) {
+                constexpr int j = decltype(Jc)::value, O = L::O(j), o = L::n(j);
+                const f32x4 f = tile_decay<C, false, O, o>(ck->d, 1.f, lane);
+                f32x4 x, y;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    x[r] = O != o || 4 * g + r < i ? n[j][r] * f[r] : 0.f;
+                    y[r] = O != o || 4 * g + r <= i ? m[j][r] * (f[r] * scale) : 0.f;
+                }
+                *reinterpret_cast<f32x4 *>(&N[(16 * O + i) * LD + 16 * o + 4 * g]) = x;
+                *reinterpret_cast<f32x4 *>(&M[(16 * O + i) * LD + 16 * o + 4 * g]) = y;
+            });
+        });
+        __syncthreads();
+        // Diagonal tiles, one per 16 lanes: a lane has a column.
+        if (wave == 0 && g < CT) {
+            float x[16];
+            const float *Nd = N + 16 * g * LD + 16 * g, *bt = ck->beta + 16 * g;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                float s = -Nd[r * LD + i];   // 0 from the diagonal on, as x then is
+#pragma unroll
+                for (int k = 0; k < r; ++k) s = __builtin_fmaf(-(Nd[r * LD + k] * bt[k]), x[k], s);
+                x[r] = s;
+                P[(16 * g + r) * LD + 16 * g + i] = s;
+            }
+        }
+        __syncthreads();
+        // The tiles below them, a wave its column block J: P_IJ = (1 + P_II B_I) Y, Y = -(N_IJ + sum over K of N_IK B_K P_KJ).
+        if (wave < CT - 1) {
+            const int J = wave;
+            f32x4 w[CT];   // B_K P_KJ
+#pragma unroll
+            for (int I = 0; I < CT; ++I) {
+                w[I] = f32x4{0.f, 0.f, 0.f, 0.f};
+                if (I < J) continue;
+                const f32x4 bt = *reinterpret_cast<const f32x4 *>(ck->beta + 16 * I + 4 * g);
+                f32x4 y;
+                if (I == J) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) y[r] = P[(16 * I + 4 * g + r) * LD + 16 * J + i];
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) y[r] = N[(16 * I + 4 * g + r) * LD + 16 * J + i];
+#pragma unroll
+                    for (int K2 = 0; K2 < I; ++K2) {
+                        if (K2 < J) continue;
+                        const f32x4 a = *reinterpret_cast<const f32x4 *>(&N[(16 * I + i) * LD + 16 * K2 + 4 * g]);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) y = __builtin_amdgcn_mfma_f32_16x16x4f32(a[r], w[K2][r], y, 0, 0, 0);
+                    }
+                    y = -y;
+                    const f32x4 a = *reinterpret_cast<const f32x4 *>(&P[(16 * I + i) * LD + 16 * I + 4 * g]);
+                    f32x4 z = y;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) z = __builtin_amdgcn_mfma_f32_16x16x4f32(a[r], bt[r] * y[r], z, 0, 0, 0);
+                    y = z;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) P[(16 * I + 4 * g + r) * LD + 16 * J + i] = y[r];
+                }
+#pragma unroll
+                for (int r = 0; r < 4; ++r) w[I][r] = bt[r] * y[r];
+            }
+        }
+        __syncthreads();
+        {
+            const Args a = args();
+            const int64_t at = p.bh * a.chunks + chunk;
+            char *ia = afresh(a.img_a) + at * (REV ? 1 : 2) * kImage<C> * 2;
+            write_image<C, false>(ia, P, wave, lane);
+            if constexpr (!REV) {
+                write_image<C, false>(ia + kImage<C> * 2, M, wave, lane);
+            } else {
+                char *ib = afresh(a.img_b) + at * 2 * kImage<C> * 2;
+                write_image<C, true>(ib, P, wave, lane);
+                write_image<C, true>(ib + kImage<C> * 2, M, wave, lane);
+            }
+        }
+    }
+}
+
+// ---- walks ---------------------------------------------------------------------------------------
+
+// An image on its way from memory to LDS.
+template <int BYTES>
+struct StageImage {
+    static constexpr int N = (BYTES / 16 + kThreads - 1) / kThreads;
+    uint4 r[N];
+    __device__ __forceinline__ void load(const char *src, int tid) {
+        const __amdgpu_buffer_rsrc_t buf = buffer(src);
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int at = (n * kThreads + tid) * 16;
+            r[n] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(buf, BYTES % (kThreads * 16) == 0 || at < BYTES ? uint32_t(at) : kNone, 0, 0));
+        }
+    }
+    __device__ __forceinline__ void store(char *dst, int tid) const {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int at = (n * kThreads + tid) * 16;
+            if (BYTES % (kThreads * 16) == 0 || at < BYTES) *reinterpret_cast<uint4 *>(dst + at) = r[n];
+        }
+    }
+};
+
+// The (pair, slice) of a workgroup. Slices of one pair read the same q, k and images: they are 8 ids apart, which is one XCD and its L2.
+struct Unit {
+    unsigned pair, slice;
+    bool live;
+};
+__device__ __forceinline__ Unit unit_of(const Args &a) {
+    const unsigned id = blockIdx.x, per = 8u * unsigned(a.slices), in = id % per;
+    Unit u;
+    u.pair = id / per * 8u + in % 8u;
+    u.slice = in / 8u;
+    u.live = u.pair < unsigned(a.batch * a.heads);
+    return u;
+}
+inline int64_t unit_grid(const Args &a) { return (a.batch * a.heads + 7) / 8 * 8 * a.slices; }
+
+// A chunk's tokens one by one, as the recurrence says, for what is not finite in it. out(t, c, the column's q S) in every lane.
+template <typename T, int C, int KD, int NC, int LDV, typename F>
+__device__ __forceinline__ void recur_delta(f32x4 (&S)[KD / 16][NC], const u16 *Q, const u16 *K, const u16 *V, const Steps<C> &ck, int rows, int kdim,
+                                            int col, int lane, F &&out) {
+#pragma unroll 1
+    for (int t = 0; t < rows; ++t) {
+        lane = afresh_lane(lane);
+        const int g = lane >> 4, i = lane & 15;
+        const float e = exp_f32(t ? (ck.hi[t] - ck.hi[t - 1]) + (ck.lo[t] - ck.lo[t - 1]) : ck.hi[0] + ck.lo[0]);
+        float z[NC], o[NC];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) z[c] = o[c] = 0.f;
+#pragma unroll
+        for (int k = 0; k < KD / 16; ++k) {
+            float y[4];
+            tile_row4<T, C, KD>(y, K, t, 16 * k + 4 * g);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const bool in = 16 * k + 4 * g + r < kdim;
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    S[k][c][r] = in ? e * S[k][c][r] : 0.f;
+                    z[c] += in ? y[r] * S[k][c][r] : 0.f;
+                }
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            z[c] += __shfl_xor(z[c], 16);
+            z[c] += __shfl_xor(z[c], 32);
+            z[c] = (tile_at<T, C, LDV>(V, t, col + 16 * c + i) - z[c]) * ck.beta[t];
+        }
+#pragma unroll
+        for (int k = 0; k < KD / 16; ++k) {
+            float y[4], x[4];
+            tile_row4<T, C, KD>(y, K, t, 16 * k + 4 * g);
+            tile_row4<T, C, KD>(x, Q, t, 16 * k + 4 * g);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const bool in = 16 * k + 4 * g + r < kdim;
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    S[k][c][r] = in ? __builtin_fmaf(y[r], z[c], S[k][c][r]) : 0.f;
+                    o[c] += in ? x[r] * S[k][c][r] : 0.f;
+                }
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            o[c] += __shfl_xor(o[c], 16);
+            o[c] += __shfl_xor(o[c], 32);
+            out(t, c, o[c]);
+        }
+    }
+}
+
+// The state's way through a row's chunks, a workgroup 64 columns of it, a wave 16. Forward: outputs and the last state. STATES (the
+// backward's): the state before every chunk and Z instead.
+template <typename T, int KD, bool STATES, bool VEC>
+__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) dr_walk(const Args) {
+    constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, W = 64, NC = 1, CT = C / 16;
+    constexpr int kImages = (STATES ? 1 : 2) * kImage<C> * 2;
+    typedef Stage<T, C, KD, kThreads, VEC> SX;
+    typedef Stage<T, C, W, kThreads, VEC> SV;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    u16 *K = reinterpret_cast<u16 *>(smem), *Q = K + PI * kTile<C, KD>, *V = STATES ? Q : Q + PI * kTile<C, KD>;
+    u16 *img = V + PI * kTile<C, W>;
+    Steps<C> *cks = reinterpret_cast<Steps<C> *>(img + kImages / 2);
+
+    int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid / 64), col = wave * 16 * NC;
+    auto fresh = [&] {
+        tid = afresh_lane(tid);
+        lane = tid & 63;
+    };
+    auto args = [] { return own_args<Args>(); };
+    const Unit u = unit_of(args());
+    if (!u.live) return;
+    const Spot p = spot_of(args(), u.pair);
+    const int col0 = afresh(int(u.slice) * W), end = afresh(int(args().seqlen));
+    f32x4 S[KD / 16][NC];
+    {
+        const Args a = args();
+        load_state<KD, NC>(S, Mat{const_cast<float *>(a.s0 ? a.s0 + int64_t(p.bh) * a.dk * a.dv + col0 : nullptr), a.dv, 1}, a.dk, a.dv - col0, col, lane);
+    }
+    auto tensor = [&](auto of) { const Args a = args(); return of(a); };
+    const Rows<T> rk = tensor([&](const Args &a) { return rows_of<T>(a.k, p.b, p.h, a.dk); });
+    const Rows<T> rq = STATES ? rk : tensor([&](const Args &a) { return rows_of<T>(a.q, p.b, p.h, a.dk); });
+    const Rows<T> rv = tensor([&](const Args &a) { return rows_of<T>(a.v, p.b, p.h, a.dv, col0); });
+    const Gates gg = tensor([&](const Args &a) { return gates_of(a.g, p); });
+    const Gates gb = tensor([&](const Args &a) { return gates_of(a.beta, p); });
+    const float scale = afresh(args().scale);
+    const char *images = tensor([&](const Args &a) { return afresh(a.img_a + int64_t(p.bh) * a.chunks * kImages); });
+    char *const out = tensor([&](const Args &a) {
+        return STATES ? nullptr : afresh(static_cast<char *>(a.out) + (p.b * a.out_batch + p.h * a.out_head + col0) * int64_t(sizeof(T)));
+    });
+    const uint32_t out_stride = uint32_t(afresh(int(args().out_seq)));
+
+    SX sk, sq;
+    SV sv;
+    StageImage<kImages> si;
+    uint32_t gnext = 0, bnext = 0;
+    auto load = [&](int t0) {
+        const int rows = min(C, end - t0);
+        sk.load(rk, t0, rows, tid);
+        si.load(images + int64_t(t0 / C) * kImages, tid);
+        if constexpr (!STATES) sq.load(rq, t0, rows, tid);
+        sv.load(rv, t0, rows, tid);
+    };
+    auto load_gates = [&](int t0) {
+        gnext = load_gate<C>(gg, t0, end, lane);
+        bnext = load_gate<C>(gb, t0, end, lane);
+    };
+    auto make = [&](int buf) { make_steps<C>(cks[buf], gnext, gg.type, bnext, gb.type, scale, lane); };
+    const bool dwave = wave == kWaves - 1;
+    load(0);
+    if (dwave) {
+        load_gates(0);
+        make(0);
+        if (C < end) load_gates(C);
+    }
+    int buf = 0;
+    for (int t0 = 0; t0 < end; t0 += C, buf ^= 1) {
+        const int rows = min(C, end - t0);
+        const bool more = t0 + C < end;
+        __syncthreads();
+        fresh();
+        sk.store(K, tid);
+        si.store(reinterpret_cast<char *>(img), tid);
+        if constexpr (!STATES) sq.store(Q, tid);
+        sv.store(V, tid);
+        if (more) load(t0 + C);
+        __syncthreads();
+        fresh();
+        const Steps<C> &ck = cks[buf];
+        if constexpr (STATES) {
+            const Args a = args();
+            const int vd = 64 * a.slices;
+            store_state<KD, NC>(S, Mat{a.states + (int64_t(p.bh) * a.chunks + t0 / C) * KD * vd + col0, vd, 1}, KD, W, col, lane);
+        }
+        f32x4 X[CT][NC], O[CT][NC];
+        inter<T, C, KD, NC>(X, S, K, ck.in, lane);
+        tile_columns<T, C, NC, W>(V, col, lane, [&](int j, int c, const float *v) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                X[2 * j][c][r] = v[r] - X[2 * j][c][r];
+                X[2 * j + 1][c][r] = v[4 + r] - X[2 * j + 1][c][r];
+            }
+        });
+        if constexpr (!STATES) inter<T, C, KD, NC>(O, S, Q, ck.inq, lane);
+        if (dwave && more) {
+            make(buf ^ 1);
+            if (t0 + 2 * C < end) load_gates(t0 + 2 * C);
+        }
+        fresh();
+        bf16x8 f[C / 32][NC][kPlanes];
+        split_rows<C, NC>(f, X, ck.beta, lane);
+        triangle<C, NC, true, kPlanes>(X, img, f, lane);   // Z
+        const int g = lane >> 4;
+        if constexpr (STATES) {
+            const Args a = args();
+            const int vd = 64 * a.slices;
+            const __amdgpu_buffer_rsrc_t to = buffer(a.z + (int64_t(p.bh) * a.chunks * C + t0) * vd + col0 + col);
+#pragma unroll
+            for (int t = 0; t < CT; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int c = 0; c < NC; ++c)
+                        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(X[t][c][r]), to, uint32_t((16 * t + 4 * g + r) * vd + 16 * c + (lane & 15)) * 4, 0, 0);
+        }
+        bool odd = false;
+        float U0[CT][4];
+#pragma unroll
+        for (int t = 0; t < CT; ++t) {
+            const f32x4 b = *reinterpret_cast<const f32x4 *>(ck.beta + 16 * t + 4 * g);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) U0[t][r] = b[r];
+        }
+#pragma unroll
+        for (int t = 0; t < CT; ++t)
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) X[t][c][r] *= U0[t][r];   // U
+        if constexpr (!STATES) {
+            bf16x8 w[C / 32][NC][kPlanes];
+#pragma unroll
+            for (int j = 0; j < C / 32; ++j)
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    float y[8];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        y[r] = X[2 * j][c][r];
+                        y[4 + r] = X[2 * j + 1][c][r];
+                    }
+                    split8(y, w[j][c]);
+                }
+            triangle<C, NC, true, kPlanes>(O, img + kImage<C>, w, lane);
+            // 0 times what is not finite is not 0.
+            float nan = 0.f;
+#pragma unroll
+            for (int t = 0; t < CT; ++t)
+#pragma unroll
+                for (int c = 0; c < NC; ++c)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        nan = __builtin_fmaf(X[t][c][r], 0.f, nan);
+                        nan = __builtin_fmaf(O[t][c][r], 0.f, nan);
+                    }
+            odd = __any(!(nan == 0.f));
+        }
+        if (STATES || !odd) {
+            split_rows<C, NC>(f, X, ck.out, lane);
+            const float all = ck.all;
+#pragma unroll
+            for (int k = 0; k < KD / 16; ++k)
+#pragma unroll
+                for (int c = 0; c < NC; ++c)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) S[k][c][r] *= all;
+            add_rows<T, C, KD, NC>(S, K, f, lane);
+            fresh();
+            if constexpr (!STATES) store_out<T, C, NC, W, VEC, false>(O, out, out_stride, t0, rows, rv.d, V, col, lane);
+        } else if constexpr (!STATES) {
+            const Args a = args();
+            const __amdgpu_buffer_rsrc_t to = buffer(out + uint64_t(unsigned(t0)) * out_stride * sizeof(T));
+            recur_delta<T, C, KD, NC, W>(S, Q, K, V, ck, rows, a.dk, col, lane, [&](int t, int c, float x) {
+                const int at = col + 16 * c + (lane & 15);
+                store_element<T, false>(x * scale, to, lane < 16 && at < rv.d ? uint32_t(t) * out_stride + uint32_t(at) : kNone);
+            });
+        }
+    }
+    if constexpr (!STATES) {
+        const Args a = args();
+        if (a.s1) store_state<KD, NC>(S, Mat{a.s1 + int64_t(p.bh) * a.dk * a.dv + col0, a.dv, 1}, a.dk, a.dv - col0, col, lane);
+    }
+}
+
+// The state's gradient R back through a row's chunks: dV, dbeta's shares, R at every chunk's end, and the first state's gradient.
+template <typename T, int KD, bool VEC>
+__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) dr_back(const Args) {
+    constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, W = 64, NC = 1, CT = C / 16;
+    constexpr int kImages = 2 * kImage<C> * 2;
+    typedef Stage<T, C, KD, kThreads, VEC> SX;
+    typedef Stage<T, C, W, kThreads, VEC> SV;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    u16 *K = reinterpret_cast<u16 *>(smem), *Q = K + PI * kTile<C, KD>, *V = Q + PI * kTile<C, KD>;
+    u16 *img = V + PI * kTile<C, W>;
+    Steps<C> *cks = reinterpret_cast<Steps<C> *>(img + kImages / 2);
+    float *part = reinterpret_cast<float *>(cks + 2);   // [wave][C]
+
+    int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid / 64), col = wave * 16 * NC;
+    auto fresh = [&] {
+        tid = afresh_lane(tid);
+        lane = tid & 63;
+    };
+    auto args = [] { return own_args<Args>(); };
+    const Unit u = unit_of(args());
+    if (!u.live) return;
+    const Spot p = spot_of(args(), u.pair);
+    const int col0 = afresh(int(u.slice) * W), end = afresh(int(args().seqlen)), chunks = (end + C - 1) / C;
+    f32x4 R[KD / 16][NC];
+    {
+        const Args a = args();
+        load_state<KD, NC>(R, Mat{const_cast<float *>(a.dlast ? a.dlast + int64_t(p.bh) * a.dk * a.dv + col0 : nullptr), a.dv, 1}, a.dk, a.dv - col0, col, lane);
+    }
+    auto tensor = [&](auto of) { const Args a = args(); return of(a); };
+    const Rows<T> rk = tensor([&](const Args &a) { return rows_of<T>(a.k, p.b, p.h, a.dk); });
+    const Rows<T> rq = tensor([&](const Args &a) { return rows_of<T>(a.q, p.b, p.h, a.dk); });
+    const Rows<T> rd = tensor([&](const Args &a) { return rows_of<T>(a.dout, p.b, p.h, a.dv, col0); });
+    const Gates gg = tensor([&](const Args &a) { return gates_of(a.g, p); });
+    const Gates gb = tensor([&](const Args &a) { return gates_of(a.beta, p); });
+    const float scale = afresh(args().scale);
+    const char *images = tensor([&](const Args &a) { return afresh(a.img_b + int64_t(p.bh) * a.chunks * kImages); });
+    char *const out = tensor([&](const Args &a) {
+        return afresh(static_cast<char *>(a.out) + (p.b * a.out_batch + p.h * a.out_head + col0) * int64_t(sizeof(T)));
+    });
+    const uint32_t out_stride = uint32_t(afresh(int(args().out_seq)));
+    SX sk, sq;
+    SV sd;
+    StageImage<kImages> si;
+    uint32_t gnext = 0, bnext = 0;
+    auto load = [&](int n) {
+        const int t0 = n * C, rows = min(C, end - t0);
+        sk.load(rk, t0, rows, tid);
+        si.load(images + int64_t(n) * kImages, tid);
+        sq.load(rq, t0, rows, tid);
+        sd.load(rd, t0, rows, tid);
+    };
+    auto load_gates = [&](int n) {
+        gnext = load_gate<C>(gg, n * C, end, lane);
+        bnext = load_gate<C>(gb, n * C, end, lane);
+    };
+    auto make = [&](int buf) { make_steps<C>(cks[buf], gnext, gg.type, bnext, gb.type, scale, lane); };
+    const bool dwave = wave == kWaves - 1;
+    load(chunks - 1);
+    if (dwave) {
+        load_gates(chunks - 1);
+        make(0);
+        if (chunks > 1) load_gates(chunks - 2);
+    }
+    int buf = 0;
+    for (int n = chunks - 1; n >= 0; --n, buf ^= 1) {
+        const int t0 = n * C, rows = min(C, end - t0);
+        const bool more = n > 0;
+        __syncthreads();
+        fresh();
+        sk.store(K, tid);
+        si.store(reinterpret_cast<char *>(img), tid);
+        sq.store(Q, tid);
+        sd.store(V, tid);
+        if (more) load(n - 1);
+        f32x4 Z[CT][NC];
+        const int g = lane >> 4;
+        {
+            const Args a = args();
+            const int vd = 64 * a.slices;
+            store_state<KD, NC>(R, Mat{a.r + (int64_t(p.bh) * a.chunks + n) * KD * vd + col0, vd, 1}, KD, W, col, lane);
+            const __amdgpu_buffer_rsrc_t from = buffer(a.z + (int64_t(p.bh) * a.chunks * C + t0) * vd + col0 + col);
+#pragma unroll
+            for (int t = 0; t < CT; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int c = 0; c < NC; ++c)
+                        Z[t][c][r] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(from, uint32_t((16 * t + 4 * g + r) * vd + 16 * c + (lane & 15)) * 4, 0, 0));
+        }
+        __syncthreads();
+        fresh();
+        const Steps<C> &ck = cks[buf];
+        f32x4 G[CT][NC];
+        inter<T, C, KD, NC>(G, R, K, ck.out, lane);
+        bf16x8 d[C / 32][NC][PI];
+        load_v<T, C, NC, W>(d, V, col, lane);
+        triangle<C, NC, false, PI>(G, img + kImage<C>, d, lane);   // dU
+        if (dwave && more) {
+            make(buf ^ 1);
+            if (n > 1) load_gates(n - 2);
+        }
+        fresh();
+        bf16x8 f[C / 32][NC][kPlanes];
+        split_rows<C, NC>(f, G, ck.beta, lane);
+        triangle<C, NC, false, kPlanes>(G, img, f, lane);          // G
+#pragma unroll
+        for (int t = 0; t < CT; ++t) {
+            const f32x4 b = *reinterpret_cast<const f32x4 *>(ck.beta + 16 * t + 4 * g);
+            f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    s[r] = __builtin_fmaf(G[t][c][r], Z[t][c][r], s[r]);
+                    G[t][c][r] *= b[r];   // dV
+                }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[r] = group_sum<16>(s[r]);
+            if ((lane & 15) == 0) *reinterpret_cast<f32x4 *>(part + wave * C + 16 * t + 4 * g) = s;
+        }
+        {
+            const Args a = args();
+            const int vd = 64 * a.slices;
+            const __amdgpu_buffer_rsrc_t to = buffer(a.dx + (int64_t(p.bh) * a.chunks * C + t0) * vd + col0 + col);
+#pragma unroll
+            for (int t = 0; t < CT; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int c = 0; c < NC; ++c)
+                        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(G[t][c][r]), to, uint32_t((16 * t + 4 * g + r) * vd + 16 * c + (lane & 15)) * 4, 0, 0);
+        }
+        // R = e^c_end R + Q^T (scale e^c dO) - K^T (e^c dV)
+        update<T, C, KD, NC>(R, d, Q, ck.inq, ck.all, lane);
+        {
+            f32x4 y[CT][NC];
+#pragma unroll
+            for (int t = 0; t < CT; ++t)
+#pragma unroll
+                for (int c = 0; c < NC; ++c) y[t][c] = -G[t][c];
+            split_rows<C, NC>(f, y, ck.in, lane);
+        }
+        add_rows<T, C, KD, NC>(R, K, f, lane);
+        fresh();
+        store_out<T, C, NC, W, VEC, false>(G, out, out_stride, t0, rows, rd.d, V, col, lane);
+        __syncthreads();
+        if (tid < C) {
+            float s = 0.f;
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) s += part[w * C + tid];
+            const Args a = args();
+            a.pbeta[(int64_t(u.slice) * a.batch * a.heads + p.bh) * a.chunks * C + t0 + tid] = s;
+        }
+    }
+    const Args a = args();
+    if (a.ds0) store_state<KD, NC>(R, Mat{a.ds0 + int64_t(p.bh) * a.dk * a.dv + col0, a.dv, 1}, a.dk, a.dv - col0, col, lane);
+}
+
+// ---- dQ, dK, dbeta and the decays' gradient ------------------------------------------------------
+
+// 64 columns of a chunk's float32 rows (pitch vd) times w into a tile's planes.
+template <int C>
+__device__ __forceinline__ void stage_f32(u16 *tile, const float *src, int vd, const float *w, int tid) {
+    constexpr int PL = kTile<C, 64>;
+#pragma unroll
+    for (int n = 0; n < C * 8 / kThreads; ++n) {
+        const int at = n * kThreads + tid, row = at / 8, x = at % 8 * 8;
+        const float4 a = *reinterpret_cast<const float4 *>(src + int64_t(row) * vd + x), b = *reinterpret_cast<const float4 *>(src + int64_t(row) * vd + x + 4);
+        const float s = w ? w[row] : 1.f;
+        const float y[8] = {a.x * s, a.y * s, a.z * s, a.w * s, b.x * s, b.y * s, b.z * s, b.w * s};
+        bf16x8 p[kPlanes];
+        split8(y, p);
+#pragma unroll
+        for (int q = 0; q < kPlanes; ++q) {
+            const u32x4 v = __builtin_bit_cast(u32x4, p[q]);
+            *reinterpret_cast<uint2 *>(tile + q * PL + la::at<64>(row, x)) = make_uint2(v.x, v.y);
+            *reinterpret_cast<uint2 *>(tile + q * PL + la::at<64>(row, x + 4)) = make_uint2(v.z, v.w);
+        }
+    }
+}
+
+// O[t] += A(t, k) f for one 32-wide step k of rows in PA planes (D-wide tile).
+template <int C, int D, int PA>
+__device__ __forceinline__ void row_products(f32x4 *O, int stride, const u16 *A, int k, const bf16x8 (&f)[kPlanes], int lane) {
+    constexpr int PL = kTile<C, D>;
+    const int g = lane >> 4, i = lane & 15;
+    bf16x8 a[C / 16][PA];
+#pragma unroll
+    for (int t = 0; t < C / 16; ++t)
+#pragma unroll
+        for (int p = 0; p < PA; ++p) a[t][p] = frag_row<D>(A + p * PL, 16 * t, k, g, i);
+#pragma unroll
+    for (int p = 0; p < PA; ++p)
+#pragma unroll
+        for (int q = 0; q < kPlanes; ++q)
+            if (p + q < kPlanes)
+#pragma unroll
+                for (int t = 0; t < C / 16; ++t) O[t * stride] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[t][p], f[q], O[t * stride], 0, 0, 0);
+}
+
+// part[n] = sum over the wave's columns of A[n][x] Y[n][x] + B[n][x] Z[n][x] (B may be NULL).
+template <typename T, int C, int NC, int LD, bool TWO>
+__device__ __forceinline__ void dot_two(const f32x4 (&A)[C / 16][NC], const u16 *Y, const f32x4 (&B)[C / 16][NC], const u16 *Z, int col, float *part, int lane) {
+    float s[C / 32][8] = {};
+    tile_columns<T, C, NC, LD>(Y, col, lane, [&](int j, int c, const float *y) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[j][e] = __builtin_fmaf(A[2 * j + e / 4][c][e % 4], y[e], s[j][e]);
+    });
+    if constexpr (TWO)
+        tile_columns<T, C, NC, LD>(Z, col, lane, [&](int j, int c, const float *y) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[j][e] = __builtin_fmaf(B[2 * j + e / 4][c][e % 4], y[e], s[j][e]);
+        });
+#pragma unroll
+    for (int j = 0; j < C / 32; ++j) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[j][e] = group_sum<16>(s[j][e]);
+        if ((lane & 15) == 0) {
+            *reinterpret_cast<f32x4 *>(part + 32 * j + 4 * (lane >> 4)) = f32x4{s[j][0], s[j][1], s[j][2], s[j][3]};
+            *reinterpret_cast<f32x4 *>(part + 32 * j + 16 + 4 * (lane >> 4)) = f32x4{s[j][4], s[j][5], s[j][6], s[j][7]};
+        }
+    }
+}
+
+__device__ __forceinline__ void store_gate(void *p, mm_dtype t, int64_t i, float x) {
+    switch (t) {
+        case MM_FLOAT32: reinterpret_cast<float *>(p)[i] = x; break;
+        case MM_FLOAT16: reinterpret_cast<f16_t *>(p)[i] = from_f32<f16_t>(x); break;
+        default: reinterpret_cast<bf16_t *>(p)[i] = from_f32<bf16_t>(x);
+    }
+}
+
+// One workgroup per chunk; waves split the columns of dQ and dK. dO, U and dV pass through LDS 64 columns at a time; S and R come
+// from memory as B operands, each wave its own rows of them.
+//
+// A log decay's gradient is the sum over the pairs (i, j) that it lies between, j < t <= i, of W_ij = A_ij (q_i . k_j) + E_ij (k_i . k_j),
+// of what enters the chunk (S) and of what leaves it (R). Row sums of W with the entering terms are q_i . dQ_i + k_i . dKr_i (dKr: dK's
+// terms with E and S), column sums with the leaving ones, f_j, are k_j . dKc_j. So, summed from t on to the chunk's end or to the next
+// forgotten state, which no pair crosses,
+//     dg_t = sum of (row sum - column sum without f) + sum over j < t of f_j + e^c_end <R, S>.
+template <typename T, int KD, bool VEC, bool F32>
+__global__ void __launch_bounds__(kThreads) dr_grad(const Args) {
+    constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, CT = C / 16, NC = KD / 64, PM = kTile<C, kScoreRow>;
+    typedef Stage<T, C, KD, kThreads, VEC> SX;
+    typedef Stage<T, C, 64, kThreads, VEC> SV;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    u16 *K = reinterpret_cast<u16 *>(smem), *Q = K + PI * kTile<C, KD>, *D = Q + PI * kTile<C, KD>;
+    u16 *U = D + PI * kTile<C, 64>, *X = U + kPlanes * kTile<C, 64>;
+    u16 *MA = U, *ME = X;   // the triangles, once U and dV are read (kTile<C, 64> is kTile<C, kScoreRow>)
+    Chunk<C> *ck = reinterpret_cast<Chunk<C> *>(X + kPlanes * kTile<C, 64>);
+    float *row = reinterpret_cast<float *>(ck + 1), *cols = row + kWaves * C, *fs = cols + kWaves * C, *rs = fs + kWaves * C;   // [wave][C]; rs [wave]
+    auto args = [] { return own_args<Args>(); };
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid & 63, g = lane >> 4, i = lane & 15, col = wave * 16 * NC;
+    const int64_t total = [&] { const Args a = args(); return a.batch * a.heads * a.chunks; }();
+    for (int64_t id = blockIdx.x; id < total; id += gridDim.x) {
+        int chunk;
+        Spot p;
+        {
+            const Args a = args();
+            const int64_t bc = id / a.heads;
+            chunk = afresh(int(bc % a.chunks));
+            p = spot_of(a, unsigned(bc / a.chunks * a.heads + id % a.heads));
+        }
+        const int t0 = chunk * C, end = afresh(int(args().seqlen)), rows = min(C, end - t0), vd = afresh(64 * args().slices);
+        const int64_t at = afresh(p.bh * args().chunks + chunk);
+        __syncthreads();
+        uint32_t gbits = 0;
+        {
+            const Args a = args();
+            SX sk, sq;
+            sk.load(rows_of<T>(a.k, p.b, p.h, a.dk), t0, rows, tid);
+            sq.load(rows_of<T>(a.q, p.b, p.h, a.dk), t0, rows, tid);
+            gbits = load_gate<C>(gates_of(a.g, p), t0, end, lane);
+            if (wave == kWaves - 1) make_chunk<C>(*ck, gbits, a.g.type, load_gate<C>(gates_of(a.beta, p), t0, end, lane), a.beta.type, a.scale, lane);
+            sk.store(K, tid);
+            sq.store(Q, tid);
+        }
+        f32x4 a1[3], a2[3], dq[CT][NC], dr[CT][NC], dc[CT][NC];
+        float rdots = 0.f;
+#pragma unroll
+        for (int j = 0; j < 3; ++j) a1[j] = a2[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int t = 0; t < CT; ++t)
+#pragma unroll
+            for (int c = 0; c < NC; ++c) dq[t][c] = dr[t][c] = dc[t][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int h0 = 0; h0 < vd; h0 += 64) {
+            __syncthreads();
+            {
+                const Args a = args();
+                SV sd;
+                sd.load(rows_of<T>(a.dout, p.b, p.h, a.dv, h0), t0, rows, tid);
+                stage_f32<C>(U, a.z + at * C * vd + h0, vd, ck->beta, tid);
+                stage_f32<C>(X, a.dx + at * C * vd + h0, vd, nullptr, tid);
+                sd.store(D, tid);
+            }
+            __syncthreads();
+            each_tile<C>(wave, [&](auto Lc) {
+                typedef decltype(Lc) L;
+                tile_products<PI, kPlanes, C, 64, L>(a1, D, U, lane);
+                tile_products<kPlanes, kPlanes, C, 64, L>(a2, X, U, lane);
+            });
+            const Args a = args();
+            const float *S = a.states + at * KD * vd + h0, *R = a.r + at * KD * vd + h0;
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    float s[8], r[8];
+                    const int64_t o = int64_t(col + 16 * c + i) * vd + 32 * k + 4 * g;
+                    *reinterpret_cast<float4 *>(s) = *reinterpret_cast<const float4 *>(S + o);
+                    *reinterpret_cast<float4 *>(s + 4) = *reinterpret_cast<const float4 *>(S + o + 16);
+                    *reinterpret_cast<float4 *>(r) = *reinterpret_cast<const float4 *>(R + o);
+                    *reinterpret_cast<float4 *>(r + 4) = *reinterpret_cast<const float4 *>(R + o + 16);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) rdots = __builtin_fmaf(s[e], r[e], rdots);
+                    bf16x8 f[kPlanes];
+                    split8(s, f);
+                    row_products<C, 64, PI>(&dq[0][c], NC, D, k, f, lane);
+                    row_products<C, 64, kPlanes>(&dr[0][c], NC, X, k, f, lane);
+                    split8(r, f);
+                    row_products<C, 64, kPlanes>(&dc[0][c], NC, U, k, f, lane);
+                }
+        }
+        // The state terms' row factors.
+#pragma unroll
+        for (int t = 0; t < CT; ++t) {
+            const f32x4 fq = *reinterpret_cast<const f32x4 *>(ck->inq + 16 * t + 4 * g), fi = *reinterpret_cast<const f32x4 *>(ck->d.in + 16 * t + 4 * g),
+                        fo = *reinterpret_cast<const f32x4 *>(ck->d.out + 16 * t + 4 * g);
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    dq[t][c][r] *= fq[r];
+                    dr[t][c][r] *= -fi[r];
+                    dc[t][c][r] *= fo[r];
+                }
+        }
+        const bool want_g = args().dg || args().dg_sum;
+        if (want_g) {
+            dot_two<T, C, NC, KD, false>(dc, K, dc, K, col, fs + wave * C, lane);
+            rdots = wave_sum(rdots);
+            if (lane == 0) rs[wave] = rdots;
+        }
+        __syncthreads();
+        // The triangles.
+        const float scale = args().scale;
+        each_tile<C>(wave, [&](auto Lc) {
+            typedef decltype(Lc) L;
+            static_for<0, L::N>([&](auto Jc) {
+                constexpr int j = decltype(Jc)::value, O = L::O(j), o = L::n(j);
+                const f32x4 f = tile_decay<C, false, O, o>(ck->d, 1.f, lane);
+                float x[4], y[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    x[r] = O != o || 4 * g + r <= i ? a1[j][r] * (f[r] * scale) : 0.f;
+                    y[r] = O != o || 4 * g + r < i ? -(a2[j][r] * f[r]) : 0.f;
+                }
+                store_scores<C>(MA, x, O, o, lane);
+                store_scores<C>(ME, y, O, o, lane);
+            });
+        });
+        zero_masked_scores<C>(MA, false, tid, kThreads);
+        zero_masked_scores<C>(ME, false, tid, kThreads);
+        __syncthreads();
+        // dQ += A K, dKr += E K
+#pragma unroll
+        for (int j = 0; j < C / 32; ++j)
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                bf16x8 k[PI], q[PI];
+#pragma unroll
+                for (int x = 0; x < PI; ++x) {
+                    k[x] = frag_tr<KD>(K + x * kTile<C, KD>, 32 * j, col + 16 * c, g, i);
+                    q[x] = frag_tr<KD>(Q + x * kTile<C, KD>, 32 * j, col + 16 * c, g, i);
+                }
+#pragma unroll
+                for (int t = 0; t < CT; ++t) {
+                    if (has_frag<C, true>(t, j)) {
+#pragma unroll
+                        for (int x = 0; x < kPlanes; ++x) {
+                            const bf16x8 ma = frag_row<kScoreRow>(MA + x * PM, 16 * t, j, g, i), me = frag_row<kScoreRow>(ME + x * PM, 16 * t, j, g, i);
+#pragma unroll
+                            for (int y = 0; y < PI; ++y)
+                                if (x + y < kPlanes) {
+                                    dq[t][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ma, k[y], dq[t][c], 0, 0, 0);
+                                    dr[t][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(me, k[y], dr[t][c], 0, 0, 0);
+                                }
+                        }
+                    }
+                    // dKc += A^T Q + E^T K
+                    if (has_frag<C, false>(t, j)) {
+#pragma unroll
+                        for (int x = 0; x < kPlanes; ++x) {
+                            const bf16x8 ma = frag_tr<kScoreRow>(MA + x * PM, 32 * j, 16 * t, g, i), me = frag_tr<kScoreRow>(ME + x * PM, 32 * j, 16 * t, g, i);
+#pragma unroll
+                            for (int y = 0; y < PI; ++y)
+                                if (x + y < kPlanes) {
+                                    dc[t][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ma, q[y], dc[t][c], 0, 0, 0);
+                                    dc[t][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(me, k[y], dc[t][c], 0, 0, 0);
+                                }
+                        }
+                    }
+                }
+            }
+        if (want_g) {
+            dot_two<T, C, NC, KD, true>(dq, Q, dr, K, col, row + wave * C, lane);
+            dot_two<T, C, NC, KD, false>(dc, K, dc, K, col, cols + wave * C, lane);
+        }
+#pragma unroll
+        for (int t = 0; t < CT; ++t)
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) dr[t][c][r] += dc[t][c][r];
+        {
+            const Args a = args();
+            const int64_t ob = (p.b * a.seqlen * a.heads + p.h) * a.dk * int64_t(F32 ? 4 : sizeof(T));
+            const uint32_t stride = uint32_t(a.heads * a.dk);
+            store_out<T, C, NC, KD, VEC, F32>(dq, static_cast<char *>(a.dq) + ob, stride, t0, rows, a.dk, Q, col, lane);
+            store_out<T, C, NC, KD, VEC, F32>(dr, static_cast<char *>(a.dk_out) + ob, stride, t0, rows, a.dk, K, col, lane);
+        }
+        __syncthreads();
+        if (wave == 0 && lane < C) {
+            const Args a = args();
+            if (lane < rows) {
+                float s = 0.f;
+                for (int x = 0; x < a.slices; ++x) s += a.pbeta[(int64_t(x) * a.batch * a.heads + p.bh) * a.chunks * C + t0 + lane];
+                store_gate(a.dbeta, a.beta.type, (p.b * a.seqlen + t0 + lane) * a.heads + p.h, s);
+            }
+        }
+        if (want_g && wave == 0) {
+            const mm_dtype gtype = mm_dtype(afresh(int(args().g.type)));
+            const bool forgets = lane < rows && decode_g(gbits, gtype) == -128.f;
+            const uint64_t all = __ballot(forgets);
+            if (lane < C) {
+                float e = 0.f, f = 0.f;
+#pragma unroll
+                for (int w = 0; w < kWaves; ++w) {
+                    e += row[w * C + lane] - (cols[w * C + lane] - fs[w * C + lane]);
+                    f += fs[w * C + lane];
+                }
+                row[lane] = e;
+                fs[lane] = f;
+            }
+            wave_fence();
+            if (lane < rows) {
+                float s = ck->d.all * ((rs[0] + rs[1]) + (rs[2] + rs[3]));
+                for (int n = 0; n < lane; ++n) s += fs[n];
+                const uint64_t behind = all >> lane >> 1;
+                const int last = min(rows, lane + 1 + (behind ? __builtin_ctzll(behind) : 64));
+                float sum = 0.f;
+                for (int n = last - 1; n >= lane; --n) sum += row[n];
+                s = forgets ? 0.f : s + sum;
+                const Args a = args();
+                if (a.dg_sum) a.dg_sum[p.bh * a.seqlen + t0 + lane] = s;
+                else store_gate(a.dg, gtype, (p.b * a.seqlen + t0 + lane) * a.heads + p.h, s);
+            }
+        }
+    }
+}
+
+// ---- launches ------------------------------------------------------------------------------------
+
+constexpr int64_t kMostGroups = int64_t(1) << 16;   // of a launch that loops over chunks
+
+template <typename T, int KD, bool REV, bool VEC>
+static int prep_t(const Args &a, hipStream_t s) {
+    constexpr int C = Cfg<T>::C, PI = Cfg<T>::in;
+    constexpr int tiles = 2 * 2 * PI * kTile<C, KD>, tri = 3 * C * kPitch<C> * 4, bytes = (tiles > tri ? tiles : tri) + int(sizeof(Chunk<C>));
+    static std::atomic<uint64_t> done{0};
+    return launch_kernel(dr_prep<T, KD, REV, VEC>, bytes, done, std::min<int64_t>(a.batch * a.heads * a.chunks, kMostGroups), kThreads, a, s, "dr_prep");
+}
+template <typename T, int KD, bool STATES, bool VEC>
+static int walk_t(const Args &a, hipStream_t s) {
+    constexpr int C = Cfg<T>::C, PI = Cfg<T>::in;
+    constexpr int bytes = 2 * ((STATES ? 1 : 2) * PI * kTile<C, KD> + PI * kTile<C, 64> + (STATES ? 1 : 2) * kImage<C>) + 2 * int(sizeof(Steps<C>));
+    static_assert(bytes <= 80 * 1024, "two workgroups on a CU");
+    static std::atomic<uint64_t> done{0};
+    return launch_kernel(dr_walk<T, KD, STATES, VEC>, bytes, done, unit_grid(a), kThreads, a, s, "dr_walk");
+}
+template <typename T, int KD, bool VEC>
+static int back_t(const Args &a, hipStream_t s) {
+    constexpr int C = Cfg<T>::C, PI = Cfg<T>::in;
+    constexpr int bytes = 2 * (2 * PI * kTile<C, KD> + PI * kTile<C, 64> + 2 * kImage<C>) + 2 * int(sizeof(Steps<C>)) + 4 * kWaves * C;
+    static_assert(bytes <= 160 * 1024, "LDS");
+    static std::atomic<uint64_t> done{0};
+    return launch_kernel(dr_back<T, KD, VEC>, bytes, done, unit_grid(a), kThreads, a, s, "dr_back");
+}
+template <typename T, int KD, bool VEC, bool F32>
+static int grad_t(const Args &a, hipStream_t s) {
+    constexpr int C = Cfg<T>::C, PI = Cfg<T>::in;
+    constexpr int bytes = 2 * (2 * PI * kTile<C, KD> + PI * kTile<C, 64> + 2 * kPlanes * kTile<C, 64>) + int(sizeof(Chunk<C>)) + 4 * (3 * kWaves * C + kWaves);
+    static_assert(bytes <= 160 * 1024, "LDS");
+    static std::atomic<uint64_t> done{0};
+    return launch_kernel(dr_grad<T, KD, VEC, F32>, bytes, done, std::min<int64_t>(a.batch * a.heads * a.chunks, kMostGroups), kThreads, a, s, "dr_grad");
+}
+
+template <typename T>
+int launch_prep(const Args &a, bool rev, hipStream_t s) {
+    const bool vec = a.q.vec && a.k.vec;
+    auto go = [&](auto kd, auto r) {
+        constexpr int KD = decltype(kd)::value;
+        constexpr bool REV = decltype(r)::value;
+        return vec ? prep_t<T, KD, REV, true>(a, s) : prep_t<T, KD, REV, false>(a, s);
+    };
+    typedef std::integral_constant<int, 64> K64;
+    typedef std::integral_constant<int, 128> K128;
+    if (rev) return a.dk <= 64 ? go(K64{}, std::true_type{}) : go(K128{}, std::true_type{});
+    return a.dk <= 64 ? go(K64{}, std::false_type{}) : go(K128{}, std::false_type{});
+}
+template <typename T>
+int launch_walk(const Args &a, bool states, hipStream_t s) {
+    const bool vec = a.k.vec && a.v.vec && (states || (a.q.vec && a.out_vec));
+    auto go = [&](auto kd, auto st) {
+        constexpr int KD = decltype(kd)::value;
+        constexpr bool ST = decltype(st)::value;
+        return vec ? walk_t<T, KD, ST, true>(a, s) : walk_t<T, KD, ST, false>(a, s);
+    };
+    typedef std::integral_constant<int, 64> K64;
+    typedef std::integral_constant<int, 128> K128;
+    if (states) return a.dk <= 64 ? go(K64{}, std::true_type{}) : go(K128{}, std::true_type{});
+    return a.dk <= 64 ? go(K64{}, std::false_type{}) : go(K128{}, std::false_type{});
+}
+template <typename T>
+int launch_back(const Args &a, hipStream_t s) {
+    const bool vec = a.q.vec && a.k.vec && a.dout.vec && a.out_vec;
+    if (a.dk <= 64) return vec ? back_t<T, 64, true>(a, s) : back_t<T, 64, false>(a, s);
+    return vec ? back_t<T, 128, true>(a, s) : back_t<T, 128, false>(a, s);
+}
+template <typename T>
+int launch_grad(const Args &a, hipStream_t s) {
+    const bool vec = a.q.vec && a.k.vec && a.dout.vec && a.dqk_vec;
+    auto go = [&](auto kd) {
+        constexpr int KD = decltype(kd)::value;
+        if constexpr (sizeof(T) == 2)
+            if (!a.dqk_f32) return vec ? grad_t<T, KD, true, false>(a, s) : grad_t<T, KD, false, false>(a, s);
+        return vec ? grad_t<T, KD, true, true>(a, s) : grad_t<T, KD, false, true>(a, s);
+    };
+    return a.dk <= 64 ? go(std::integral_constant<int, 64>{}) : go(std::integral_constant<int, 128>{});
+}
+
+template int launch_prep<MM_DELTA_TYPE>(const Args &, bool, hipStream_t);
+template int launch_walk<MM_DELTA_TYPE>(const Args &, bool, hipStream_t);
+template int launch_back<MM_DELTA_TYPE>(const Args &, hipStream_t);
+template int launch_grad<MM_DELTA_TYPE>(const Args &, hipStream_t);
+
+}  // namespace dr
+}  // namespace mm

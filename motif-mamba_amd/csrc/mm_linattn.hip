@@ -15,7 +15,6 @@
 #endif
 
 #include <algorithm>
-#include <atomic>
 
 #include "mm_linattn_dev.h"
 #include "mm_linattn_host.h"
@@ -25,22 +24,6 @@ namespace la {
 
 constexpr int kWaves = 4, kThreads = 64 * kWaves;
 
-// The kernel's only argument, read where this stands. A walk keeps the few numbers that every chunk needs (a tensor's first
-// row and stride, 3 scalars each) and reads the others when it needs them: all of them, some 60, do not fit the scalar registers, and a
-// build that spilled them lost the low word of an output's address (a tuple of arguments was overwritten in part before it was
-// spilled; one instance of 144 stored to wrong addresses).
-template <typename A>
-__device__ __forceinline__ A own_args() {
-    typedef const __attribute__((address_space(4))) A *Args;
-    Args args = (Args)__builtin_amdgcn_kernarg_segment_ptr();
-    asm volatile("" : "+s"(args));
-    return *(const A *)args;
-}
-
-template <typename T>
-__device__ __forceinline__ Rows<T> rows_of(const View &v, int b, int h, int d, int col0 = 0) {
-    return Rows<T>{afresh(reinterpret_cast<const T *>(v.p) + b * v.batch + int64_t(unsigned(h) / unsigned(v.share)) * v.head + col0), uint32_t(afresh(int(v.seq) * int(sizeof(T)))), afresh(d - col0)};
-}
 // A workgroup's place: its batch row, head and segment, and the segment's tokens.
 struct Place {
     int slice, seg, b, h, beg, end;
@@ -57,19 +40,6 @@ __device__ __forceinline__ Place place_of(const A &a, int slices) {
     p.end = afresh(min(int(a.seqlen), p.beg + int(a.seg_len)));
     return p;
 }
-// The log decays of a (batch row, head).
-struct Gates {
-    const char *p;
-    int64_t stride;   // bytes
-    mm_dtype type;
-
-    // A lane's token's bits in the chunk at t0, 0 past `end`; see decode_g.
-    template <int C>
-    __device__ __forceinline__ uint32_t load(int t0, int end, int lane) const {
-        const int t = t0 + lane;
-        return lane < C && t < end ? load_g_raw(p + t * stride, type, 0) : 0u;
-    }
-};
 template <typename A>
 __device__ __forceinline__ Gates gates_of(const A &a, const Place &p) {
     const int64_t size = a.gtype == MM_FLOAT32 ? 4 : 2;
@@ -608,22 +578,6 @@ __global__ void __launch_bounds__(2 * kThreads) __attribute__((amdgpu_waves_per_
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid & 63;
     if (wave < kWaves) bwd_walk<T, KD, VD, VEC, F32, false>(smem, tid, wave, lane);
     else bwd_walk<T, KD, VD, VEC, F32, true>(smem, tid, wave, lane);
-}
-
-// Launches with `bytes` of dynamic LDS, which a kernel is allowed once per device (`done`: a bit per device).
-template <typename K, typename A>
-static int launch_kernel(K kernel, int bytes, std::atomic<uint64_t> &done, int64_t grid, int threads, const A &a, hipStream_t s,
-                         const char *what) {
-    int dev = 0;
-    if (const hipError_t e = hipGetDevice(&dev)) return set_error(int(e), "linear attention: hipGetDevice failed");
-    const uint64_t bit = uint64_t(1) << (dev & 63);
-    if (!(done.load(std::memory_order_relaxed) & bit)) {
-        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-        if (e != hipSuccess) return set_error(int(e), "linear attention: hipFuncSetAttribute failed");
-        done.fetch_or(bit, std::memory_order_relaxed);
-    }
-    hipLaunchKernelGGL(kernel, dim3(unsigned(grid)), dim3(unsigned(threads)), bytes, s, a);
-    return launch_status(what);
 }
 
 template <typename T, int KD, int NC, bool DOT, bool VEC, bool F32>

@@ -27,9 +27,12 @@
 
 #include <hip/hip_runtime.h>
 
+#include <atomic>
+
 #include "mm_common.h"
 #include "mm_internal.h"
 #include "mm_linattn.h"
+#include "mm_linattn_host.h"
 
 namespace mm {
 namespace la {
@@ -1023,6 +1026,55 @@ __device__ __forceinline__ float wave_sum(float x) {
     x += __shfl_xor(x, 16);
     x += __shfl_xor(x, 32);
     return x;
+}
+
+// ---- a kernel's arguments, and its launch ---------------------------------------------------------
+
+// The kernel's only argument, read where this stands. A walk keeps the few numbers that every chunk needs (a tensor's first
+// row and stride, 3 scalars each) and reads the others when it needs them: all of them, some 60, do not fit the scalar registers, and a
+// build that spilled them lost the low word of an output's address (a tuple of arguments was overwritten in part before it was
+// spilled; one instance of 144 stored to wrong addresses).
+template <typename A>
+__device__ __forceinline__ A own_args() {
+    typedef const __attribute__((address_space(4))) A *Args;
+    Args args = (Args)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(args));
+    return *(const A *)args;
+}
+
+template <typename T>
+__device__ __forceinline__ Rows<T> rows_of(const View &v, int b, int h, int d, int col0 = 0) {
+    return Rows<T>{afresh(reinterpret_cast<const T *>(v.p) + b * v.batch + int64_t(unsigned(h) / unsigned(v.share)) * v.head + col0), uint32_t(afresh(int(v.seq) * int(sizeof(T)))), afresh(d - col0)};
+}
+
+// The log decays of a (batch row, head).
+struct Gates {
+    const char *p;
+    int64_t stride;   // bytes
+    mm_dtype type;
+
+    // A lane's token's bits in the chunk at t0, 0 past `end`; see decode_g.
+    template <int C>
+    __device__ __forceinline__ uint32_t load(int t0, int end, int lane) const {
+        const int t = t0 + lane;
+        return lane < C && t < end ? load_g_raw(p + t * stride, type, 0) : 0u;
+    }
+};
+
+// Launches with `bytes` of dynamic LDS, which a kernel is allowed once per device (`done`: a bit per device).
+template <typename K, typename A>
+static int launch_kernel(K kernel, int bytes, std::atomic<uint64_t> &done, int64_t grid, int threads, const A &a, hipStream_t s,
+                         const char *what) {
+    int dev = 0;
+    if (const hipError_t e = hipGetDevice(&dev)) return set_error(int(e), "hipGetDevice failed");
+    const uint64_t bit = uint64_t(1) << (dev & 63);
+    if (!(done.load(std::memory_order_relaxed) & bit)) {
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e != hipSuccess) return set_error(int(e), "hipFuncSetAttribute failed");
+        done.fetch_or(bit, std::memory_order_relaxed);
+    }
+    hipLaunchKernelGGL(kernel, dim3(unsigned(grid)), dim3(unsigned(threads)), bytes, s, a);
+    return launch_status(what);
 }
 
 }  // namespace la

@@ -20,7 +20,9 @@
 #include <vector>
 
 #include "mm_conv1d.h"
+#include "mm_delta.h"
 #include "mm_group_norm.h"
+#include "mm_layer_norm.h"
 #include "mm_linattn.h"
 #include "mm_norm.h"
 #include "mm_scan.h"
@@ -1017,6 +1019,260 @@ std::vector<c10::optional<at::Tensor>> group_norm_bwd(const at::Tensor &x, int64
     return res;
 }
 
+// ---- gated delta rule ----------------------------------------------------------------------------
+
+void check_beta(const at::Tensor &b, at::IntArrayRef sizes, const at::Tensor &v) {
+    TORCH_CHECK(b.is_cuda() && b.device() == v.device(), "beta must be on the device of v");
+    TORCH_CHECK(b.sizes() == sizes, "beta must have the shape of v without its last dimension");
+    float_dtype(b, "beta");
+}
+
+// The fields that the forward and backward have alike.
+template <typename P>
+void delta_common(P &p, const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &b, const c10::optional<at::Tensor> &g_, double scale) {
+    check_qkv(q, k, v, 4);
+    const int64_t batch = v.size(0), seqlen = v.size(1), heads = v.size(2);
+    check_beta(b, {batch, seqlen, heads}, v);
+    std::memset(&p, 0, sizeof(p));
+    p.batch = batch; p.seqlen = seqlen; p.n_groups = q.size(2); p.nheads = heads; p.dk = q.size(3); p.dv = v.size(3);
+    p.itype = to_mm(v.scalar_type());
+    p.btype = to_mm(b.scalar_type());
+    p.gtype = MM_FLOAT32;
+    p.scale = static_cast<float>(scale);
+    p.q = q.data_ptr(); p.k = k.data_ptr(); p.v = v.data_ptr(); p.beta = b.data_ptr();
+    p.q_batch_stride = q.stride(0); p.q_seq_stride = seq_stride(q); p.q_group_stride = q.stride(2);
+    p.k_batch_stride = k.stride(0); p.k_seq_stride = seq_stride(k); p.k_group_stride = k.stride(2);
+    p.v_batch_stride = v.stride(0); p.v_seq_stride = seq_stride(v); p.v_head_stride = v.stride(2);
+    p.b_batch_stride = b.stride(0); p.b_seq_stride = b.stride(1); p.b_head_stride = b.stride(2);
+    if (g_.has_value()) {
+        const at::Tensor &g = g_.value();
+        check_decay(g, {batch, seqlen, heads}, v);
+        p.gtype = to_mm(g.scalar_type());
+        p.log_decay = g.data_ptr();
+        p.g_batch_stride = g.stride(0); p.g_seq_stride = g.stride(1); p.g_head_stride = g.stride(2);
+    }
+}
+
+std::vector<at::Tensor> delta_fwd(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &b, const c10::optional<at::Tensor> &g,
+                                  double scale, const c10::optional<at::Tensor> &initial_, bool return_last_state) {
+    mm_delta_fwd_params p;
+    delta_common(p, q, k, v, b, g, scale);
+    at::Tensor initial;
+    if (initial_.has_value()) {
+        check_state(initial_.value(), v, p.batch, p.nheads, p.dk, p.dv, "initial_state");
+        initial = initial_.value().contiguous();
+    }
+    const c10::DeviceGuard device_guard{v.device()};
+    at::Tensor out = torch::empty({p.batch, p.seqlen, p.nheads, p.dv}, v.options());
+    at::Tensor last;
+    if (return_last_state) last = torch::empty({p.batch, p.nheads, p.dk, p.dv}, v.options().dtype(at::ScalarType::Float));
+    p.initial_state = initial.defined() ? initial.data_ptr<float>() : nullptr;
+    p.out = out.data_ptr();
+    p.last_state = last.defined() ? last.data_ptr<float>() : nullptr;
+    p.out_batch_stride = out.stride(0); p.out_seq_stride = seq_stride(out); p.out_head_stride = out.stride(2);
+    at::Tensor ws;
+    p.workspace_bytes = mm_delta_fwd_workspace_size(&p);
+    p.workspace = workspace_of(ws, p.workspace_bytes, v);
+    check_rc(mm_delta_fwd(&p, c10::hip::getCurrentHIPStream().stream()), "mm_delta_fwd");
+    std::vector<at::Tensor> res{out};
+    if (return_last_state) res.push_back(last);
+    return res;
+}
+
+// Gradients [dq, dk, dv, dbeta, dlog_decay | None, dinitial_state | None]; dlog_decay has the shape of log_decay, or (nheads,) with
+// decay_per_head.
+std::vector<c10::optional<at::Tensor>> delta_bwd(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &b,
+                                                 const c10::optional<at::Tensor> &g, double scale, const c10::optional<at::Tensor> &initial_,
+                                                 const at::Tensor &dout, const c10::optional<at::Tensor> &dlast_, bool decay_per_head,
+                                                 bool want_decay, bool want_initial) {
+    mm_delta_bwd_params p;
+    delta_common(p, q, k, v, b, g, scale);
+    TORCH_CHECK(dout.is_cuda() && dout.sizes() == v.sizes() && dout.scalar_type() == v.scalar_type(), "dout must have the shape and dtype of v");
+    TORCH_CHECK(dout.stride(-1) == 1 || dout.size(-1) == 1 || dout.numel() == 0, "dout must be contiguous along its last dimension");
+    at::Tensor initial, dlast;
+    if (initial_.has_value()) {
+        check_state(initial_.value(), v, p.batch, p.nheads, p.dk, p.dv, "initial_state");
+        initial = initial_.value().contiguous();
+    }
+    if (dlast_.has_value()) {
+        check_state(dlast_.value(), v, p.batch, p.nheads, p.dk, p.dv, "dlast_state");
+        dlast = dlast_.value().contiguous();
+    }
+    const c10::DeviceGuard device_guard{v.device()};
+    at::Tensor dq = torch::empty(q.sizes(), q.options()), dkk = torch::empty(k.sizes(), k.options()), dvv = torch::empty(v.sizes(), v.options());
+    at::Tensor db = torch::empty(b.sizes(), b.options()), dg, ds;
+    if (want_decay && g.has_value())
+        dg = decay_per_head ? torch::empty({p.nheads}, g.value().options()) : torch::empty({p.batch, p.seqlen, p.nheads}, g.value().options());
+    if (want_initial) ds = torch::empty({p.batch, p.nheads, p.dk, p.dv}, v.options().dtype(at::ScalarType::Float));
+    p.initial_state = initial.defined() ? initial.data_ptr<float>() : nullptr;
+    p.dout = dout.data_ptr();
+    p.dlast_state = dlast.defined() ? dlast.data_ptr<float>() : nullptr;
+    p.dq = dq.data_ptr(); p.dk_out = dkk.data_ptr(); p.dv_out = dvv.data_ptr(); p.dbeta = db.data_ptr();
+    p.dlog_decay = dg.defined() ? dg.data_ptr() : nullptr;
+    p.dinitial_state = ds.defined() ? ds.data_ptr<float>() : nullptr;
+    p.decay_per_head = decay_per_head;
+    p.do_batch_stride = dout.stride(0); p.do_seq_stride = seq_stride(dout); p.do_head_stride = dout.stride(2);
+    at::Tensor ws;
+    p.workspace_bytes = mm_delta_bwd_workspace_size(&p);
+    p.workspace = workspace_of(ws, p.workspace_bytes, v);
+    check_rc(mm_delta_bwd(&p, c10::hip::getCurrentHIPStream().stream()), "mm_delta_bwd");
+    std::vector<c10::optional<at::Tensor>> res{dq, dkk, dvv, db, c10::nullopt, c10::nullopt};
+    if (dg.defined()) res[4] = dg;
+    if (want_initial) res[5] = ds;
+    return res;
+}
+
+at::Tensor delta_update(const at::Tensor &state, const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &b,
+                        const c10::optional<at::Tensor> &g_, double scale) {
+    check_qkv(q, k, v, 3);
+    const int64_t batch = v.size(0), heads = v.size(1), dv = v.size(2), dk = q.size(2);
+    check_beta(b, {batch, heads}, v);
+    check_state(state, v, batch, heads, dk, dv, "state");
+    TORCH_CHECK(state.stride(-1) == 1 || dv == 1, "state must be contiguous along its last dimension");
+    auto no_derivative = [](const at::Tensor &t) {
+        TORCH_CHECK(!(at::GradMode::is_enabled() && t.requires_grad()) && !t._fw_grad(0).defined(),
+                    "delta_rule_update has no derivatives: call it under torch.no_grad() or on detached tensors");
+    };
+    for (const auto *t : {&state, &q, &k, &v, &b}) no_derivative(*t);
+    mm_delta_update_params p;
+    std::memset(&p, 0, sizeof(p));
+    p.gtype = MM_FLOAT32;
+    if (g_.has_value()) {
+        const at::Tensor &g = g_.value();
+        check_decay(g, {batch, heads}, v);
+        no_derivative(g);
+        p.gtype = to_mm(g.scalar_type());
+        p.log_decay = g.data_ptr();
+        p.g_batch_stride = g.stride(0); p.g_head_stride = g.stride(1);
+    }
+    const c10::DeviceGuard device_guard{v.device()};
+    at::Tensor out = torch::empty({batch, heads, dv}, v.options());
+    p.batch = batch; p.n_groups = q.size(1); p.nheads = heads; p.dk = dk; p.dv = dv;
+    p.itype = to_mm(v.scalar_type());
+    p.btype = to_mm(b.scalar_type());
+    p.scale = static_cast<float>(scale);
+    p.state = state.data_ptr<float>();
+    p.q = q.data_ptr(); p.k = k.data_ptr(); p.v = v.data_ptr(); p.beta = b.data_ptr();
+    p.out = out.data_ptr();
+    p.state_batch_stride = state.stride(0); p.state_head_stride = state.stride(1); p.state_dk_stride = state.stride(2);
+    p.q_batch_stride = q.stride(0); p.q_group_stride = q.stride(1);
+    p.k_batch_stride = k.stride(0); p.k_group_stride = k.stride(1);
+    p.v_batch_stride = v.stride(0); p.v_head_stride = v.stride(1);
+    p.b_batch_stride = b.stride(0); p.b_head_stride = b.stride(1);
+    check_rc(mm_delta_update(&p, c10::hip::getCurrentHIPStream().stream()), "mm_delta_update");
+    // The state is not what an autograd node may have saved any more.
+    if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();
+    return out;
+}
+
+// ---- layer norm ----------------------------------------------------------------------------------
+
+// x or residual (rows, channels); x None: residual is h already.
+mm_layer_norm_params layer_norm_params(const c10::optional<at::Tensor> &x_, const c10::optional<at::Tensor> &residual_, at::ScalarType rtype,
+                                       const c10::optional<at::Tensor> &weight_, const c10::optional<at::Tensor> &bias_, double eps, bool is_rms,
+                                       at::ScalarType itype) {
+    const at::Tensor &ref = x_.has_value() ? x_.value() : residual_.value();
+    TORCH_CHECK(ref.is_cuda() && ref.dim() == 2, "x must be a (rows, channels) tensor on the GPU");
+    const int64_t rows = ref.size(0), channels = ref.size(1);
+    TORCH_CHECK(itype == at::ScalarType::Float || itype == at::ScalarType::Half || itype == at::ScalarType::BFloat16, "x must be float32, float16 or bfloat16");
+    mm_layer_norm_params p;
+    std::memset(&p, 0, sizeof(p));
+    p.rows = rows; p.channels = channels;
+    p.itype = to_mm(itype);
+    TORCH_CHECK(rtype == itype || rtype == at::ScalarType::Float, "residual must have x's dtype or float32");
+    p.rtype = to_mm(rtype);
+    p.wtype = MM_FLOAT32;
+    p.eps = static_cast<float>(eps);
+    p.is_rms = is_rms;
+    for (const auto *t : {&x_, &residual_})
+        if (t->has_value()) {
+            const at::Tensor &r = t->value();
+            TORCH_CHECK(r.is_cuda() && r.device() == ref.device() && r.sizes() == ref.sizes(), "residual must have the shape and device of x");
+            TORCH_CHECK(r.scalar_type() == (t == &x_ ? itype : rtype), "residual has another dtype than stated");
+            TORCH_CHECK(r.stride(1) == 1 || channels == 1 || rows == 0, "x and residual must be contiguous along their channels");
+        }
+    if (x_.has_value()) {
+        p.x = x_.value().data_ptr();
+        p.x_row_stride = x_.value().stride(0);
+    }
+    if (residual_.has_value()) {
+        p.residual = residual_.value().data_ptr();
+        p.residual_row_stride = residual_.value().stride(0);
+    }
+    for (const auto *t : {&weight_, &bias_})
+        if (t->has_value()) {
+            const at::Tensor &w = t->value();
+            TORCH_CHECK(w.is_cuda() && w.device() == ref.device() && w.dim() == 1 && w.size(0) == channels && w.is_contiguous(),
+                        "weight and bias must be contiguous (channels,) tensors on the device of x");
+            p.wtype = float_dtype(w, "weight");
+        }
+    if (weight_.has_value() && bias_.has_value())
+        TORCH_CHECK(weight_.value().scalar_type() == bias_.value().scalar_type(), "weight and bias must have one dtype");
+    p.weight = weight_.has_value() ? weight_.value().data_ptr() : nullptr;
+    p.bias = bias_.has_value() ? bias_.value().data_ptr() : nullptr;
+    return p;
+}
+
+// [out, residual_out | None]; wide: residual_out in float32 where there is no residual that gives its dtype.
+std::vector<c10::optional<at::Tensor>> layer_norm_fwd(const at::Tensor &x, const c10::optional<at::Tensor> &residual, const c10::optional<at::Tensor> &weight,
+                                                      const c10::optional<at::Tensor> &bias, double eps, bool is_rms, bool want_residual, bool wide) {
+    const at::ScalarType rtype = residual.has_value() ? residual.value().scalar_type() : wide ? at::ScalarType::Float : x.scalar_type();
+    mm_layer_norm_params p = layer_norm_params(x, residual, rtype, weight, bias, eps, is_rms, x.scalar_type());
+    const c10::DeviceGuard device_guard{x.device()};
+    std::vector<c10::optional<at::Tensor>> res{torch::empty({p.rows, p.channels}, x.options()), c10::nullopt};
+    p.out = res[0].value().data_ptr();
+    if (want_residual) {
+        res[1] = torch::empty({p.rows, p.channels}, x.options().dtype(rtype));
+        p.residual_out = res[1].value().data_ptr();
+    }
+    check_rc(mm_layer_norm_fwd(&p, c10::hip::getCurrentHIPStream().stream()), "mm_layer_norm_fwd");
+    return res;
+}
+
+// [dx | None, dresidual | None, dweight | None, dbias | None]
+std::vector<c10::optional<at::Tensor>> layer_norm_bwd(const c10::optional<at::Tensor> &x, const c10::optional<at::Tensor> &residual,
+                                                      const c10::optional<at::Tensor> &weight, const c10::optional<at::Tensor> &bias, double eps, bool is_rms,
+                                                      const at::Tensor &dout, const c10::optional<at::Tensor> &dres, bool wide, bool want_dx, bool want_dres,
+                                                      bool want_weight, bool want_bias) {
+    const at::ScalarType rtype = wide ? at::ScalarType::Float : dout.scalar_type();
+    mm_layer_norm_params p = layer_norm_params(x, residual, rtype, weight, bias, eps, is_rms, dout.scalar_type());
+    const at::Tensor &ref = x.has_value() ? x.value() : residual.value();
+    TORCH_CHECK(dout.is_cuda() && dout.device() == ref.device() && dout.sizes() == ref.sizes(), "dout must have the shape and device of x");
+    TORCH_CHECK(dout.stride(1) == 1 || p.channels == 1 || p.rows == 0, "dout must be contiguous along its channels");
+    p.dout = dout.data_ptr();
+    p.dout_row_stride = dout.stride(0);
+    if (dres.has_value()) {
+        const at::Tensor &d = dres.value();
+        TORCH_CHECK(d.is_cuda() && d.device() == ref.device() && d.sizes() == ref.sizes() && d.scalar_type() == rtype, "dresidual_out must have the shape, dtype and device of residual_out");
+        TORCH_CHECK(d.stride(1) == 1 || p.channels == 1 || p.rows == 0, "dresidual_out must be contiguous along its channels");
+        p.dresidual_out = d.data_ptr();
+        p.dresidual_out_row_stride = d.stride(0);
+    }
+    const c10::DeviceGuard device_guard{ref.device()};
+    std::vector<c10::optional<at::Tensor>> res{c10::nullopt, c10::nullopt, c10::nullopt, c10::nullopt};
+    if (want_dx) {
+        res[0] = torch::empty({p.rows, p.channels}, dout.options());
+        p.dx = res[0].value().data_ptr();
+    }
+    if (want_dres) {
+        res[1] = torch::empty({p.rows, p.channels}, dout.options().dtype(rtype));
+        p.dresidual = res[1].value().data_ptr();
+    }
+    if (want_weight && weight.has_value()) {
+        res[2] = torch::empty_like(weight.value());
+        p.dweight = res[2].value().data_ptr();
+    }
+    if (want_bias && bias.has_value()) {
+        res[3] = torch::empty_like(bias.value());
+        p.dbias = res[3].value().data_ptr();
+    }
+    at::Tensor ws;
+    p.workspace_bytes = mm_layer_norm_bwd_workspace_size(&p);
+    p.workspace = workspace_of(ws, p.workspace_bytes, dout);
+    check_rc(mm_layer_norm_bwd(&p, c10::hip::getCurrentHIPStream().stream()), "mm_layer_norm_bwd");
+    return res;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -1072,5 +1328,20 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("group_norm_bwd", &group_norm_bwd, "Gated group norm backward [dx, dweight?, dbias?, dz?]", pybind11::arg("x"),
           pybind11::arg("n_groups"), pybind11::arg("weight"), pybind11::arg("bias"), pybind11::arg("z"), pybind11::arg("eps"),
           pybind11::arg("is_rms"), pybind11::arg("gate"), pybind11::arg("dout"), pybind11::arg("want_weights"));
+    m.def("delta_fwd", &delta_fwd, "Gated delta rule forward [out, last_state?]", pybind11::arg("q"), pybind11::arg("k"), pybind11::arg("v"),
+          pybind11::arg("beta"), pybind11::arg("log_decay"), pybind11::arg("scale"), pybind11::arg("initial_state"), pybind11::arg("return_last_state"));
+    m.def("delta_bwd", &delta_bwd, "Gated delta rule backward [dq, dk, dv, dbeta, dlog_decay?, dinitial_state?]", pybind11::arg("q"),
+          pybind11::arg("k"), pybind11::arg("v"), pybind11::arg("beta"), pybind11::arg("log_decay"), pybind11::arg("scale"),
+          pybind11::arg("initial_state"), pybind11::arg("dout"), pybind11::arg("dlast_state"), pybind11::arg("decay_per_head"),
+          pybind11::arg("want_decay"), pybind11::arg("want_initial"));
+    m.def("delta_update", &delta_update, "Gated delta rule, one token (in place on state)", pybind11::arg("state"), pybind11::arg("q"),
+          pybind11::arg("k"), pybind11::arg("v"), pybind11::arg("beta"), pybind11::arg("log_decay"), pybind11::arg("scale"));
+    m.def("layer_norm_fwd", &layer_norm_fwd, "Residual add and layer norm forward [out, residual_out?]", pybind11::arg("x"),
+          pybind11::arg("residual"), pybind11::arg("weight"), pybind11::arg("bias"), pybind11::arg("eps"), pybind11::arg("is_rms"),
+          pybind11::arg("want_residual"), pybind11::arg("wide"));
+    m.def("layer_norm_bwd", &layer_norm_bwd, "Residual add and layer norm backward [dx?, dresidual?, dweight?, dbias?]", pybind11::arg("x"),
+          pybind11::arg("residual"), pybind11::arg("weight"), pybind11::arg("bias"), pybind11::arg("eps"), pybind11::arg("is_rms"),
+          pybind11::arg("dout"), pybind11::arg("dresidual_out"), pybind11::arg("wide"), pybind11::arg("want_dx"), pybind11::arg("want_dresidual"),
+          pybind11::arg("want_weight"), pybind11::arg("want_bias"));
     m.def("abi_version", []() { return mm_abi_version(); });
 }
