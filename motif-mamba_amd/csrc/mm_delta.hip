@@ -121,27 +121,30 @@ template <int PX, int PY, int C, int D, typename L>
 __device__ __forceinline__ void tile_products(f32x4 *s, const u16 *X, const u16 *Y, int lane) {
     constexpr int PL = kTile<C, D>;
     const int g = lane >> 4, i = lane & 15;
+    constexpr int B = PY > 1 ? 3 : 4;   // tiles whose operands are held at once
 #pragma unroll
-    for (int k = 0; k < D / 32; ++k) {
-        bf16x8 a[L::N][PY], b[L::N][PX];
+    for (int k = 0; k < D / 32; ++k)
 #pragma unroll
-        for (int j = 0; j < L::N; ++j) {
+        for (int j0 = 0; j0 < L::N; j0 += B) {
+            bf16x8 a[B][PY], b[B][PX];
 #pragma unroll
-            for (int p = 0; p < PX; ++p) {
-                if (j > 0 && L::O(j) == L::O(j - 1)) b[j][p] = b[j - 1][p];
-                else b[j][p] = frag_row<D>(X + p * PL, 16 * L::O(j), k, g, i);
+            for (int j = 0; j < B && j0 + j < L::N; ++j) {
+#pragma unroll
+                for (int p = 0; p < PX; ++p) {
+                    if (j > 0 && L::O(j0 + j) == L::O(j0 + j - 1)) b[j][p] = b[j - 1][p];
+                    else b[j][p] = frag_row<D>(X + p * PL, 16 * L::O(j0 + j), k, g, i);
+                }
+#pragma unroll
+                for (int p = 0; p < PY; ++p) a[j][p] = frag_row<D>(Y + p * PL, 16 * L::n(j0 + j), k, g, i);
             }
 #pragma unroll
-            for (int p = 0; p < PY; ++p) a[j][p] = frag_row<D>(Y + p * PL, 16 * L::n(j), k, g, i);
+            for (int p = 0; p < PY; ++p)
+#pragma unroll
+                for (int q = 0; q < PX; ++q)
+                    if (p + q < kPlanes)
+#pragma unroll
+                        for (int j = 0; j < B && j0 + j < L::N; ++j) s[j0 + j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[j][p], b[j][q], s[j0 + j], 0, 0, 0);
         }
-#pragma unroll
-        for (int p = 0; p < PY; ++p)
-#pragma unroll
-            for (int q = 0; q < PX; ++q)
-                if (p + q < kPlanes)
-#pragma unroll
-                    for (int j = 0; j < L::N; ++j) s[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[j][p], b[j][q], s[j], 0, 0, 0);
-    }
 }
 // The waves' shares of a chunk's lower triangle of tiles.
 template <int C, typename F>
@@ -854,26 +857,43 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
 
 // ---- dQ, dK, dbeta and the decays' gradient ------------------------------------------------------
 
-// 64 columns of a chunk's float32 rows (pitch vd) times w into a tile's planes.
-template <int C>
-__device__ __forceinline__ void stage_f32(u16 *tile, const float *src, int vd, const float *w, int tid) {
-    constexpr int PL = kTile<C, 64>;
+// 64 columns of a chunk's float32 rows (pitch vd) on their way into a tile's planes, 8 of a row per thread and step.
+template <int C, int NT>
+struct StageF32 {
+    static constexpr int N = (C * 8 + NT - 1) / NT;
+    float4 r[N][2];
+
+    __device__ __forceinline__ void load(const float *src, int vd, int tid) {
 #pragma unroll
-    for (int n = 0; n < C * 8 / kThreads; ++n) {
-        const int at = n * kThreads + tid, row = at / 8, x = at % 8 * 8;
-        const float4 a = *reinterpret_cast<const float4 *>(src + int64_t(row) * vd + x), b = *reinterpret_cast<const float4 *>(src + int64_t(row) * vd + x + 4);
-        const float s = w ? w[row] : 1.f;
-        const float y[8] = {a.x * s, a.y * s, a.z * s, a.w * s, b.x * s, b.y * s, b.z * s, b.w * s};
-        bf16x8 p[kPlanes];
-        split8(y, p);
-#pragma unroll
-        for (int q = 0; q < kPlanes; ++q) {
-            const u32x4 v = __builtin_bit_cast(u32x4, p[q]);
-            *reinterpret_cast<uint2 *>(tile + q * PL + la::at<64>(row, x)) = make_uint2(v.x, v.y);
-            *reinterpret_cast<uint2 *>(tile + q * PL + la::at<64>(row, x + 4)) = make_uint2(v.z, v.w);
+        for (int n = 0; n < N; ++n) {
+            const int at = n * NT + tid;
+            if (C * 8 % NT != 0 && at >= C * 8) break;
+            const float *p = src + (at / 8) * vd + at % 8 * 8;
+            r[n][0] = *reinterpret_cast<const float4 *>(p);
+            r[n][1] = *reinterpret_cast<const float4 *>(p + 4);
         }
     }
-}
+    // Rows times w (NULL: 1).
+    __device__ __forceinline__ void store(u16 *tile, const float *w, int tid) const {
+        constexpr int PL = kTile<C, 64>;
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int at = n * NT + tid, row = at / 8, x = at % 8 * 8;
+            if (C * 8 % NT != 0 && at >= C * 8) break;
+            const float s = w ? w[row] : 1.f;
+            const float4 a = r[n][0], b = r[n][1];
+            const float y[8] = {a.x * s, a.y * s, a.z * s, a.w * s, b.x * s, b.y * s, b.z * s, b.w * s};
+            bf16x8 p[kPlanes];
+            split8(y, p);
+#pragma unroll
+            for (int q = 0; q < kPlanes; ++q) {
+                const u32x4 v = __builtin_bit_cast(u32x4, p[q]);
+                *reinterpret_cast<uint2 *>(tile + q * PL + la::at<64>(row, x)) = make_uint2(v.x, v.y);
+                *reinterpret_cast<uint2 *>(tile + q * PL + la::at<64>(row, x + 4)) = make_uint2(v.z, v.w);
+            }
+        }
+    }
+};
 
 // O[t] += A(t, k) f for one 32-wide step k of rows in PA planes (D-wide tile).
 template <int C, int D, int PA>
@@ -926,8 +946,50 @@ __device__ __forceinline__ void store_gate(void *p, mm_dtype t, int64_t i, float
     }
 }
 
-// One workgroup per chunk; waves split the columns of dQ and dK. dO, U and dV pass through LDS 64 columns at a time; S and R come
-// from memory as B operands, each wave its own rows of them.
+// The waves' shares of the lower triangles of tiles of dO U^T (f's first list; PI planes by 3) and of dV U^T (its second one; 3 by 3,
+// twice the products).
+template <int C, int NW, typename F>
+__device__ __forceinline__ void each_tile_of_two(int wave, F &&f) {
+    typedef Tiles<> None;
+    if constexpr (C == 64 && NW == 8) {
+        switch (wave) {
+            case 0: f(None{}, Tiles<3, 0, 3, 1>{}); break;
+            case 1: f(None{}, Tiles<3, 2, 3, 3>{}); break;
+            case 2: f(None{}, Tiles<2, 0, 2, 1>{}); break;
+            case 3: f(None{}, Tiles<2, 2, 1, 0>{}); break;
+            case 4: f(None{}, Tiles<1, 1, 0, 0>{}); break;
+            case 5: f(Tiles<3, 0, 3, 1, 3, 2, 3, 3>{}, None{}); break;
+            case 6: f(Tiles<2, 0, 2, 1, 2, 2>{}, None{}); break;
+            default: f(Tiles<1, 0, 1, 1, 0, 0>{}, None{});
+        }
+    } else if constexpr (C == 64) {
+        switch (wave) {
+            case 0: f(None{}, Tiles<3, 0, 3, 1, 3, 2, 3, 3>{}); break;
+            case 1: f(None{}, Tiles<2, 0, 2, 1, 2, 2, 1, 0>{}); break;
+            case 2: f(Tiles<3, 0, 3, 1, 3, 2, 3, 3>{}, Tiles<1, 1, 0, 0>{}); break;
+            default: f(Tiles<2, 0, 2, 1, 2, 2, 1, 0, 1, 1, 0, 0>{}, None{});
+        }
+    } else if constexpr (NW == 8) {
+        switch (wave) {
+            case 0: f(None{}, Tiles<1, 0>{}); break;
+            case 1: f(None{}, Tiles<1, 1>{}); break;
+            case 2: f(None{}, Tiles<0, 0>{}); break;
+            case 3: f(Tiles<1, 0>{}, None{}); break;
+            case 4: f(Tiles<1, 1>{}, None{}); break;
+            case 5: f(Tiles<0, 0>{}, None{});
+        }
+    } else {
+        switch (wave) {
+            case 0: f(None{}, Tiles<1, 0>{}); break;
+            case 1: f(None{}, Tiles<1, 1>{}); break;
+            case 2: f(None{}, Tiles<0, 0>{}); break;
+            default: f(Tiles<1, 0, 1, 1, 0, 0>{}, None{});
+        }
+    }
+}
+
+// One workgroup per chunk; its waves split the columns of dQ and dK, 16 each. dO, U and dV pass through LDS 64 columns at a time; S and
+// R come from memory as B operands, each wave its own rows of them.
 //
 // A log decay's gradient is the sum over the pairs (i, j) that it lies between, j < t <= i, of W_ij = A_ij (q_i . k_j) + E_ij (k_i . k_j),
 // of what enters the chunk (S) and of what leaves it (R). Row sums of W with the entering terms are q_i . dQ_i + k_i . dKr_i (dKr: dK's
@@ -935,18 +997,25 @@ __device__ __forceinline__ void store_gate(void *p, mm_dtype t, int64_t i, float
 // forgotten state, which no pair crosses,
 //     dg_t = sum of (row sum - column sum without f) + sum over j < t of f_j + e^c_end <R, S>.
 template <typename T, int KD, bool VEC, bool F32>
-__global__ void __launch_bounds__(kThreads) dr_grad(const Args) {
-    constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, CT = C / 16, NC = KD / 64, PM = kTile<C, kScoreRow>;
-    typedef Stage<T, C, KD, kThreads, VEC> SX;
-    typedef Stage<T, C, 64, kThreads, VEC> SV;
+__global__ void __launch_bounds__(KD * 4) __attribute__((amdgpu_waves_per_eu(2, 2))) dr_grad(const Args) {
+    constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, CT = C / 16, NC = 1, NW = KD / 16, NT = 64 * NW, PM = kTile<C, kScoreRow>;
+    typedef Stage<T, C, KD, NT, VEC> SX;
+    typedef Stage<T, C, 64, NT, VEC> SV;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     u16 *K = reinterpret_cast<u16 *>(smem), *Q = K + PI * kTile<C, KD>, *D = Q + PI * kTile<C, KD>;
     u16 *U = D + PI * kTile<C, 64>, *X = U + kPlanes * kTile<C, 64>;
     u16 *MA = U, *ME = X;   // the triangles, once U and dV are read (kTile<C, 64> is kTile<C, kScoreRow>)
     Chunk<C> *ck = reinterpret_cast<Chunk<C> *>(X + kPlanes * kTile<C, 64>);
-    float *row = reinterpret_cast<float *>(ck + 1), *cols = row + kWaves * C, *fs = cols + kWaves * C, *rs = fs + kWaves * C;   // [wave][C]; rs [wave]
+    float *row = reinterpret_cast<float *>(ck + 1), *cols = row + NW * C, *fs = cols + NW * C, *rs = fs + NW * C;   // [wave][C]; rs [wave]
     auto args = [] { return own_args<Args>(); };
-    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid & 63, g = lane >> 4, i = lane & 15, col = wave * 16 * NC;
+    int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, i = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(tid / 64), col = wave * 16;
+    auto fresh = [&] {
+        tid = afresh_lane(tid);
+        lane = tid & 63;
+        g = lane >> 4;
+        i = lane & 15;
+    };
     const int64_t total = [&] { const Args a = args(); return a.batch * a.heads * a.chunks; }();
     for (int64_t id = blockIdx.x; id < total; id += gridDim.x) {
         int chunk;
@@ -957,65 +1026,92 @@ __global__ void __launch_bounds__(kThreads) dr_grad(const Args) {
             chunk = afresh(int(bc % a.chunks));
             p = spot_of(a, unsigned(bc / a.chunks * a.heads + id % a.heads));
         }
-        const int t0 = chunk * C, end = afresh(int(args().seqlen)), rows = min(C, end - t0), vd = afresh(64 * args().slices);
+        const int t0 = chunk * C, rows = min(C, afresh(int(args().seqlen)) - t0), vd = afresh(64 * args().slices);
         const int64_t at = afresh(p.bh * args().chunks + chunk);
-        __syncthreads();
-        uint32_t gbits = 0;
-        {
+        SV sd;
+        StageF32<C, NT> su, sx;
+        float4 sr[2][2][2];   // [k][S, R][half of 8]
+        auto load = [&](int h0) {
             const Args a = args();
-            SX sk, sq;
-            sk.load(rows_of<T>(a.k, p.b, p.h, a.dk), t0, rows, tid);
-            sq.load(rows_of<T>(a.q, p.b, p.h, a.dk), t0, rows, tid);
-            gbits = load_gate<C>(gates_of(a.g, p), t0, end, lane);
-            if (wave == kWaves - 1) make_chunk<C>(*ck, gbits, a.g.type, load_gate<C>(gates_of(a.beta, p), t0, end, lane), a.beta.type, a.scale, lane);
-            sk.store(K, tid);
-            sq.store(Q, tid);
-        }
-        f32x4 a1[3], a2[3], dq[CT][NC], dr[CT][NC], dc[CT][NC];
-        float rdots = 0.f;
-#pragma unroll
-        for (int j = 0; j < 3; ++j) a1[j] = a2[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int t = 0; t < CT; ++t)
-#pragma unroll
-            for (int c = 0; c < NC; ++c) dq[t][c] = dr[t][c] = dc[t][c] = f32x4{0.f, 0.f, 0.f, 0.f};
-        for (int h0 = 0; h0 < vd; h0 += 64) {
-            __syncthreads();
-            {
-                const Args a = args();
-                SV sd;
-                sd.load(rows_of<T>(a.dout, p.b, p.h, a.dv, h0), t0, rows, tid);
-                stage_f32<C>(U, a.z + at * C * vd + h0, vd, ck->beta, tid);
-                stage_f32<C>(X, a.dx + at * C * vd + h0, vd, nullptr, tid);
-                sd.store(D, tid);
-            }
-            __syncthreads();
-            each_tile<C>(wave, [&](auto Lc) {
-                typedef decltype(Lc) L;
-                tile_products<PI, kPlanes, C, 64, L>(a1, D, U, lane);
-                tile_products<kPlanes, kPlanes, C, 64, L>(a2, X, U, lane);
-            });
+            sd.load(rows_of<T>(a.dout, p.b, p.h, a.dv, h0), t0, rows, tid);
+            su.load(a.z + at * C * vd + h0, vd, tid);
+            sx.load(a.dx + at * C * vd + h0, vd, tid);
+        };
+        auto load_states = [&](int h0) {
             const Args a = args();
             const float *S = a.states + at * KD * vd + h0, *R = a.r + at * KD * vd + h0;
 #pragma unroll
-            for (int k = 0; k < 2; ++k)
+            for (int k = 0; k < 2; ++k) {
+                const int o = (col + i) * vd + 32 * k + 4 * g;
+                sr[k][0][0] = *reinterpret_cast<const float4 *>(S + o);
+                sr[k][0][1] = *reinterpret_cast<const float4 *>(S + o + 16);
+                sr[k][1][0] = *reinterpret_cast<const float4 *>(R + o);
+                sr[k][1][1] = *reinterpret_cast<const float4 *>(R + o + 16);
+            }
+        };
+        __syncthreads();
+        {
+            const Args a = args();
+            const Gates gg = gates_of(a.g, p), gb = gates_of(a.beta, p);
+            const int end = int(a.seqlen);
+            SX sk, sq;
+            sk.load(rows_of<T>(a.k, p.b, p.h, a.dk), t0, rows, tid);
+            sq.load(rows_of<T>(a.q, p.b, p.h, a.dk), t0, rows, tid);
+            load(0);
+            load_states(0);
+            if (wave == NW - 1)
+                make_chunk<C>(*ck, load_gate<C>(gg, t0, end, lane), a.g.type, load_gate<C>(gb, t0, end, lane), a.beta.type, a.scale, lane);
+            sk.store(K, tid);
+            sq.store(Q, tid);
+        }
+        f32x4 a1[6], a2[4], dq[CT][NC], dr[CT][NC], dc[CT][NC];
+        float rdots = 0.f;
 #pragma unroll
-                for (int c = 0; c < NC; ++c) {
-                    float s[8], r[8];
-                    const int64_t o = int64_t(col + 16 * c + i) * vd + 32 * k + 4 * g;
-                    *reinterpret_cast<float4 *>(s) = *reinterpret_cast<const float4 *>(S + o);
-                    *reinterpret_cast<float4 *>(s + 4) = *reinterpret_cast<const float4 *>(S + o + 16);
-                    *reinterpret_cast<float4 *>(r) = *reinterpret_cast<const float4 *>(R + o);
-                    *reinterpret_cast<float4 *>(r + 4) = *reinterpret_cast<const float4 *>(R + o + 16);
+        for (int j = 0; j < 6; ++j) a1[j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) rdots = __builtin_fmaf(s[e], r[e], rdots);
-                    bf16x8 f[kPlanes];
-                    split8(s, f);
-                    row_products<C, 64, PI>(&dq[0][c], NC, D, k, f, lane);
-                    row_products<C, 64, kPlanes>(&dr[0][c], NC, X, k, f, lane);
-                    split8(r, f);
-                    row_products<C, 64, kPlanes>(&dc[0][c], NC, U, k, f, lane);
-                }
+        for (int j = 0; j < 4; ++j) a2[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int t = 0; t < CT; ++t) dq[t][0] = dr[t][0] = dc[t][0] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+        for (int h0 = 0; h0 < vd; h0 += 64) {
+            __syncthreads();
+            fresh();
+            sd.store(D, tid);
+            su.store(U, ck->beta, tid);
+            sx.store(X, nullptr, tid);
+            if (h0 + 64 < vd) load(h0 + 64);
+            __syncthreads();
+            fresh();
+            each_tile_of_two<C, NW>(wave, [&](auto L1, auto L2) {
+                if constexpr (decltype(L1)::N > 0) tile_products<PI, kPlanes, C, 64, decltype(L1)>(a1, D, U, lane);
+                if constexpr (decltype(L2)::N > 0) tile_products<kPlanes, kPlanes, C, 64, decltype(L2)>(a2, X, U, lane);
+            });
+            fresh();
+            bf16x8 f[2][2][kPlanes];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                float y[2][8];
+#pragma unroll
+                for (int m = 0; m < 2; ++m)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        y[m][4 * e] = sr[k][m][e].x;
+                        y[m][4 * e + 1] = sr[k][m][e].y;
+                        y[m][4 * e + 2] = sr[k][m][e].z;
+                        y[m][4 * e + 3] = sr[k][m][e].w;
+                    }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) rdots = __builtin_fmaf(y[0][e], y[1][e], rdots);
+                split8(y[0], f[k][0]);
+                split8(y[1], f[k][1]);
+            }
+            if (h0 + 64 < vd) load_states(h0 + 64);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                row_products<C, 64, PI>(&dq[0][0], NC, D, k, f[k][0], lane);
+                row_products<C, 64, kPlanes>(&dr[0][0], NC, X, k, f[k][0], lane);
+                row_products<C, 64, kPlanes>(&dc[0][0], NC, U, k, f[k][1], lane);
+            }
         }
         // The state terms' row factors.
 #pragma unroll
@@ -1023,13 +1119,11 @@ __global__ void __launch_bounds__(kThreads) dr_grad(const Args) {
             const f32x4 fq = *reinterpret_cast<const f32x4 *>(ck->inq + 16 * t + 4 * g), fi = *reinterpret_cast<const f32x4 *>(ck->d.in + 16 * t + 4 * g),
                         fo = *reinterpret_cast<const f32x4 *>(ck->d.out + 16 * t + 4 * g);
 #pragma unroll
-            for (int c = 0; c < NC; ++c)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    dq[t][c][r] *= fq[r];
-                    dr[t][c][r] *= -fi[r];
-                    dc[t][c][r] *= fo[r];
-                }
+            for (int r = 0; r < 4; ++r) {
+                dq[t][0][r] *= fq[r];
+                dr[t][0][r] *= -fi[r];
+                dc[t][0][r] *= fo[r];
+            }
         }
         const bool want_g = args().dg || args().dg_sum;
         if (want_g) {
@@ -1038,66 +1132,74 @@ __global__ void __launch_bounds__(kThreads) dr_grad(const Args) {
             if (lane == 0) rs[wave] = rdots;
         }
         __syncthreads();
+        fresh();
         // The triangles.
         const float scale = args().scale;
-        each_tile<C>(wave, [&](auto Lc) {
-            typedef decltype(Lc) L;
-            static_for<0, L::N>([&](auto Jc) {
-                constexpr int j = decltype(Jc)::value, O = L::O(j), o = L::n(j);
-                const f32x4 f = tile_decay<C, false, O, o>(ck->d, 1.f, lane);
-                float x[4], y[4];
+        each_tile_of_two<C, NW>(wave, [&](auto L1, auto L2) {
+            typedef decltype(L1) A;
+            typedef decltype(L2) E;
+            static_for<0, A::N>([&](auto Jc) {
+                constexpr int j = decltype(Jc)::value, O = A::O(j), o = A::n(j);
+                const f32x4 w = tile_decay<C, false, O, o>(ck->d, 1.f, lane);
+                float x[4];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    x[r] = O != o || 4 * g + r <= i ? a1[j][r] * (f[r] * scale) : 0.f;
-                    y[r] = O != o || 4 * g + r < i ? -(a2[j][r] * f[r]) : 0.f;
-                }
+                for (int r = 0; r < 4; ++r) x[r] = O != o || 4 * g + r <= i ? a1[j][r] * (w[r] * scale) : 0.f;
                 store_scores<C>(MA, x, O, o, lane);
-                store_scores<C>(ME, y, O, o, lane);
+            });
+            static_for<0, E::N>([&](auto Jc) {
+                constexpr int j = decltype(Jc)::value, O = E::O(j), o = E::n(j);
+                const f32x4 w = tile_decay<C, false, O, o>(ck->d, 1.f, lane);
+                float x[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) x[r] = O != o || 4 * g + r < i ? -(a2[j][r] * w[r]) : 0.f;
+                store_scores<C>(ME, x, O, o, lane);
             });
         });
-        zero_masked_scores<C>(MA, false, tid, kThreads);
-        zero_masked_scores<C>(ME, false, tid, kThreads);
+        zero_masked_scores<C>(MA, false, tid, NT);
+        zero_masked_scores<C>(ME, false, tid, NT);
         __syncthreads();
-        // dQ += A K, dKr += E K
+        fresh();
 #pragma unroll
-        for (int j = 0; j < C / 32; ++j)
+        for (int j = 0; j < C / 32; ++j) {
+            bf16x8 k[PI], q[PI];
 #pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                bf16x8 k[PI], q[PI];
+            for (int x = 0; x < PI; ++x) {
+                k[x] = frag_tr<KD>(K + x * kTile<C, KD>, 32 * j, col, g, i);
+                q[x] = frag_tr<KD>(Q + x * kTile<C, KD>, 32 * j, col, g, i);
+            }
+            // dQ += A K, dKr += E K, dKc += A^T Q + E^T K: a plane's products of all row tiles, then the next plane's.
 #pragma unroll
-                for (int x = 0; x < PI; ++x) {
-                    k[x] = frag_tr<KD>(K + x * kTile<C, KD>, 32 * j, col + 16 * c, g, i);
-                    q[x] = frag_tr<KD>(Q + x * kTile<C, KD>, 32 * j, col + 16 * c, g, i);
-                }
+            for (int x = 0; x < kPlanes; ++x) {
+                bf16x8 ma[CT], me[CT], ta[CT], te[CT];
 #pragma unroll
                 for (int t = 0; t < CT; ++t) {
                     if (has_frag<C, true>(t, j)) {
-#pragma unroll
-                        for (int x = 0; x < kPlanes; ++x) {
-                            const bf16x8 ma = frag_row<kScoreRow>(MA + x * PM, 16 * t, j, g, i), me = frag_row<kScoreRow>(ME + x * PM, 16 * t, j, g, i);
-#pragma unroll
-                            for (int y = 0; y < PI; ++y)
-                                if (x + y < kPlanes) {
-                                    dq[t][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ma, k[y], dq[t][c], 0, 0, 0);
-                                    dr[t][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(me, k[y], dr[t][c], 0, 0, 0);
-                                }
-                        }
+                        ma[t] = frag_row<kScoreRow>(MA + x * PM, 16 * t, j, g, i);
+                        me[t] = frag_row<kScoreRow>(ME + x * PM, 16 * t, j, g, i);
                     }
-                    // dKc += A^T Q + E^T K
                     if (has_frag<C, false>(t, j)) {
-#pragma unroll
-                        for (int x = 0; x < kPlanes; ++x) {
-                            const bf16x8 ma = frag_tr<kScoreRow>(MA + x * PM, 32 * j, 16 * t, g, i), me = frag_tr<kScoreRow>(ME + x * PM, 32 * j, 16 * t, g, i);
-#pragma unroll
-                            for (int y = 0; y < PI; ++y)
-                                if (x + y < kPlanes) {
-                                    dc[t][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ma, q[y], dc[t][c], 0, 0, 0);
-                                    dc[t][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(me, k[y], dc[t][c], 0, 0, 0);
-                                }
-                        }
+                        ta[t] = frag_tr<kScoreRow>(MA + x * PM, 32 * j, 16 * t, g, i);
+                        te[t] = frag_tr<kScoreRow>(ME + x * PM, 32 * j, 16 * t, g, i);
                     }
                 }
+#pragma unroll
+                for (int y = 0; y < PI; ++y)
+                    if (x + y < kPlanes) {
+#pragma unroll
+                        for (int t = 0; t < CT; ++t) {
+                            if (has_frag<C, true>(t, j)) {
+                                dq[t][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ma[t], k[y], dq[t][0], 0, 0, 0);
+                                dr[t][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(me[t], k[y], dr[t][0], 0, 0, 0);
+                            }
+                            if (has_frag<C, false>(t, j)) dc[t][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ta[t], q[y], dc[t][0], 0, 0, 0);
+                        }
+#pragma unroll
+                        for (int t = 0; t < CT; ++t)
+                            if (has_frag<C, false>(t, j)) dc[t][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(te[t], k[y], dc[t][0], 0, 0, 0);
+                    }
             }
+        }
+        fresh();
         if (want_g) {
             dot_two<T, C, NC, KD, true>(dq, Q, dr, K, col, row + wave * C, lane);
             dot_two<T, C, NC, KD, false>(dc, K, dc, K, col, cols + wave * C, lane);
@@ -1105,9 +1207,7 @@ __global__ void __launch_bounds__(kThreads) dr_grad(const Args) {
 #pragma unroll
         for (int t = 0; t < CT; ++t)
 #pragma unroll
-            for (int c = 0; c < NC; ++c)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) dr[t][c][r] += dc[t][c][r];
+            for (int r = 0; r < 4; ++r) dr[t][0][r] += dc[t][0][r];
         {
             const Args a = args();
             const int64_t ob = (p.b * a.seqlen * a.heads + p.h) * a.dk * int64_t(F32 ? 4 : sizeof(T));
@@ -1116,22 +1216,20 @@ __global__ void __launch_bounds__(kThreads) dr_grad(const Args) {
             store_out<T, C, NC, KD, VEC, F32>(dr, static_cast<char *>(a.dk_out) + ob, stride, t0, rows, a.dk, K, col, lane);
         }
         __syncthreads();
-        if (wave == 0 && lane < C) {
+        if (wave == 0 && lane < rows) {
             const Args a = args();
-            if (lane < rows) {
-                float s = 0.f;
-                for (int x = 0; x < a.slices; ++x) s += a.pbeta[(int64_t(x) * a.batch * a.heads + p.bh) * a.chunks * C + t0 + lane];
-                store_gate(a.dbeta, a.beta.type, (p.b * a.seqlen + t0 + lane) * a.heads + p.h, s);
-            }
+            float s = 0.f;
+            for (int x = 0; x < a.slices; ++x) s += a.pbeta[(int64_t(x) * a.batch * a.heads + p.bh) * a.chunks * C + t0 + lane];
+            store_gate(a.dbeta, a.beta.type, (p.b * a.seqlen + t0 + lane) * a.heads + p.h, s);
         }
-        if (want_g && wave == 0) {
-            const mm_dtype gtype = mm_dtype(afresh(int(args().g.type)));
-            const bool forgets = lane < rows && decode_g(gbits, gtype) == -128.f;
+        if (want_g && wave == 1) {
+            const Args a = args();
+            const bool forgets = lane < rows && decode_g(load_gate<C>(gates_of(a.g, p), t0, t0 + rows, lane), a.g.type) == -128.f;
             const uint64_t all = __ballot(forgets);
             if (lane < C) {
                 float e = 0.f, f = 0.f;
 #pragma unroll
-                for (int w = 0; w < kWaves; ++w) {
+                for (int w = 0; w < NW; ++w) {
                     e += row[w * C + lane] - (cols[w * C + lane] - fs[w * C + lane]);
                     f += fs[w * C + lane];
                 }
@@ -1140,16 +1238,18 @@ __global__ void __launch_bounds__(kThreads) dr_grad(const Args) {
             }
             wave_fence();
             if (lane < rows) {
-                float s = ck->d.all * ((rs[0] + rs[1]) + (rs[2] + rs[3]));
+                float s = 0.f;
+#pragma unroll
+                for (int w = 0; w < NW; ++w) s += rs[w];
+                s *= ck->d.all;
                 for (int n = 0; n < lane; ++n) s += fs[n];
                 const uint64_t behind = all >> lane >> 1;
                 const int last = min(rows, lane + 1 + (behind ? __builtin_ctzll(behind) : 64));
                 float sum = 0.f;
                 for (int n = last - 1; n >= lane; --n) sum += row[n];
                 s = forgets ? 0.f : s + sum;
-                const Args a = args();
                 if (a.dg_sum) a.dg_sum[p.bh * a.seqlen + t0 + lane] = s;
-                else store_gate(a.dg, gtype, (p.b * a.seqlen + t0 + lane) * a.heads + p.h, s);
+                else store_gate(a.dg, a.g.type, (p.b * a.seqlen + t0 + lane) * a.heads + p.h, s);
             }
         }
     }
@@ -1185,10 +1285,11 @@ static int back_t(const Args &a, hipStream_t s) {
 template <typename T, int KD, bool VEC, bool F32>
 static int grad_t(const Args &a, hipStream_t s) {
     constexpr int C = Cfg<T>::C, PI = Cfg<T>::in;
-    constexpr int bytes = 2 * (2 * PI * kTile<C, KD> + PI * kTile<C, 64> + 2 * kPlanes * kTile<C, 64>) + int(sizeof(Chunk<C>)) + 4 * (3 * kWaves * C + kWaves);
-    static_assert(bytes <= 160 * 1024, "LDS");
+    constexpr int NW = KD / 16;
+    constexpr int bytes = 2 * (2 * PI * kTile<C, KD> + PI * kTile<C, 64> + 2 * kPlanes * kTile<C, 64>) + int(sizeof(Chunk<C>)) + 4 * (3 * NW * C + NW);
+    static_assert(bytes <= (KD == 64 ? 80 : 160) * 1024, "two workgroups on a CU at KD 64, one at 128");
     static std::atomic<uint64_t> done{0};
-    return launch_kernel(dr_grad<T, KD, VEC, F32>, bytes, done, std::min<int64_t>(a.batch * a.heads * a.chunks, kMostGroups), kThreads, a, s, "dr_grad");
+    return launch_kernel(dr_grad<T, KD, VEC, F32>, bytes, done, std::min<int64_t>(a.batch * a.heads * a.chunks, kMostGroups), 64 * NW, a, s, "dr_grad");
 }
 
 template <typename T>
