@@ -274,9 +274,18 @@ __device__ __forceinline__ void write_image(char *dst, const float *f, int wave,
                 if (n % kWaves != wave) continue;
                 float x[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int o = 2 * j + e / 4, a = 16 * t + i, b = 16 * o + 4 * g + e % 4;   // tile o
-                    x[e] = (TR ? o >= t : o <= t) ? f[(TR ? b : a) * kPitch<C> + (TR ? a : b)] : 0.f;
+                for (int h = 0; h < 2; ++h) {
+                    const int o = 2 * j + h;   // tile o
+                    f32x4 y = {0.f, 0.f, 0.f, 0.f};
+                    if constexpr (TR) {
+                        if (o >= t)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) y[r] = f[(16 * o + 4 * g + r) * kPitch<C> + 16 * t + i];
+                    } else {
+                        if (o <= t) y = *reinterpret_cast<const f32x4 *>(&f[(16 * t + i) * kPitch<C> + 16 * o + 4 * g]);
+                    }
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) x[4 * h + r] = y[r];
                 }
                 bf16x8 p[kPlanes];
                 split8(x, p);
@@ -289,8 +298,9 @@ __device__ __forceinline__ void write_image(char *dst, const float *f, int wave,
 // P (and M) of every chunk, as operand images; REV: P, P^T and M^T for the backward (P into img_a's first half... see the plan).
 // One workgroup per chunk. The triangles are made in float32: the diagonal tiles of P by substitution, row by row, those of a column
 // block below by 16 x 16 products on v_mfma_f32_16x16x4_f32, which keeps them float32.
+template <typename T, int KD> constexpr int kPrepGroups = sizeof(T) == 2 || KD == 64 ? 3 : 2;   // on a CU
 template <typename T, int KD, bool REV, bool VEC>
-__global__ void __launch_bounds__(kThreads) dr_prep(const Args) {
+__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kPrepGroups<T, KD>, kPrepGroups<T, KD>))) dr_prep(const Args) {
     constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, CT = C / 16, LD = kPitch<C>;
     typedef Stage<T, C, KD, kThreads, VEC> SX;
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -311,15 +321,24 @@ __global__ void __launch_bounds__(kThreads) dr_prep(const Args) {
             chunk = afresh(int(bc % a.chunks));
             p = spot_of(a, unsigned(bc / a.chunks * a.heads + id % a.heads));
         }
-        const int t0 = chunk * C, end = int(args().seqlen), rows = min(C, end - t0);
+        const int t0 = chunk * C, rows = min(C, afresh(int(args().seqlen)) - t0);
+        uint32_t gbits = 0, bbits = 0;
         __syncthreads();
         {
-            const Args a = args();
             SX sk, sq;
-            sk.load(rows_of<T>(a.k, p.b, p.h, a.dk), t0, rows, tid);
-            sq.load(rows_of<T>(a.q, p.b, p.h, a.dk), t0, rows, tid);
-            if (wave == kWaves - 1)
-                make_chunk<C>(*ck, load_gate<C>(gates_of(a.g, p), t0, end, lane), a.g.type, load_gate<C>(gates_of(a.beta, p), t0, end, lane), a.beta.type, a.scale, lane);
+            {
+                const Args a = args();
+                sk.load(rows_of<T>(a.k, p.b, p.h, a.dk), t0, rows, tid);
+            }
+            {
+                const Args a = args();
+                sq.load(rows_of<T>(a.q, p.b, p.h, a.dk), t0, rows, tid);
+            }
+            if (wave == kWaves - 1) {
+                const Args a = args();
+                gbits = load_gate<C>(gates_of(a.g, p), t0, t0 + rows, lane);
+                bbits = load_gate<C>(gates_of(a.beta, p), t0, t0 + rows, lane);
+            }
             sk.store(K, tid);
             sq.store(Q, tid);
         }
@@ -332,6 +351,10 @@ __global__ void __launch_bounds__(kThreads) dr_prep(const Args) {
             tile_products<PI, PI, C, KD, L>(n, K, K, lane);
             tile_products<PI, PI, C, KD, L>(m, Q, K, lane);
         });
+        if (wave == kWaves - 1) {   // which has the fewest tiles
+            const Args a = args();
+            make_chunk<C>(*ck, gbits, a.g.type, bbits, a.beta.type, a.scale, lane);
+        }
         __syncthreads();
         const float scale = args().scale;
         each_tile<C>(wave, [&](auto Lc) {
@@ -350,55 +373,75 @@ __global__ void __launch_bounds__(kThreads) dr_prep(const Args) {
             });
         });
         __syncthreads();
-        // Diagonal tiles, one per 16 lanes: a lane has a column.
+        // Diagonal tiles, one per 16 lanes: a lane has a column. N is 0 from the diagonal on, and so is x.
         if (wave == 0 && g < CT) {
-            float x[16];
+            float x[16], w[16];   // P and B P
             const float *Nd = N + 16 * g * LD + 16 * g, *bt = ck->beta + 16 * g;
+            f32x4 n4[2][4];
+            float own[2], bs[2];
+            auto read = [&](int r) {
+#pragma unroll
+                for (int k = 0; k < (r + 3) / 4; ++k) n4[r % 2][k] = *reinterpret_cast<const f32x4 *>(Nd + r * LD + 4 * k);
+                own[r % 2] = Nd[r * LD + i];
+                bs[r % 2] = bt[r];
+            };
+            read(0);
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                float s = -Nd[r * LD + i];   // 0 from the diagonal on, as x then is
+                if (r < 15) read(r + 1);
+                __builtin_amdgcn_sched_barrier(0);
+                float s = -own[r % 2], s2 = 0.f;
 #pragma unroll
-                for (int k = 0; k < r; ++k) s = __builtin_fmaf(-(Nd[r * LD + k] * bt[k]), x[k], s);
-                x[r] = s;
-                P[(16 * g + r) * LD + 16 * g + i] = s;
+                for (int k = 0; k < r; ++k) {
+                    if (k % 2) s2 = __builtin_fmaf(-n4[r % 2][k / 4][k % 4], w[k], s2);
+                    else s = __builtin_fmaf(-n4[r % 2][k / 4][k % 4], w[k], s);
+                }
+                x[r] = s + s2;
+                w[r] = bs[r % 2] * x[r];
             }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) P[(16 * g + r) * LD + 16 * g + i] = x[r];
         }
         __syncthreads();
         // The tiles below them, a wave its column block J: P_IJ = (1 + P_II B_I) Y, Y = -(N_IJ + sum over K of N_IK B_K P_KJ).
-        if (wave < CT - 1) {
-            const int J = wave;
-            f32x4 w[CT];   // B_K P_KJ
+        auto column = [&](auto Jc) {
+            constexpr int J = decltype(Jc)::value;
+            auto rows4 = [&](const float *f, int I, int K2) { return *reinterpret_cast<const f32x4 *>(&f[(16 * I + i) * LD + 16 * K2 + 4 * g]); };   // as an A operand
+            auto tile = [&](const float *f, int I) {
+                f32x4 x;
 #pragma unroll
-            for (int I = 0; I < CT; ++I) {
-                w[I] = f32x4{0.f, 0.f, 0.f, 0.f};
-                if (I < J) continue;
-                const f32x4 bt = *reinterpret_cast<const f32x4 *>(ck->beta + 16 * I + 4 * g);
-                f32x4 y;
-                if (I == J) {
+                for (int r = 0; r < 4; ++r) x[r] = f[(16 * I + 4 * g + r) * LD + 16 * J + i];
+                return x;
+            };
+            f32x4 w[CT], bt[CT], y[CT], nn[CT][CT], pp[CT];   // w: B_K P_KJ
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) y[r] = P[(16 * I + 4 * g + r) * LD + 16 * J + i];
-                } else {
+            for (int I = J; I < CT; ++I) {
+                bt[I] = *reinterpret_cast<const f32x4 *>(ck->beta + 16 * I + 4 * g);
+                y[I] = tile(I == J ? P : N, I);
+                if (I > J) pp[I] = rows4(P, I, I);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) y[r] = N[(16 * I + 4 * g + r) * LD + 16 * J + i];
-#pragma unroll
-                    for (int K2 = 0; K2 < I; ++K2) {
-                        if (K2 < J) continue;
-                        const f32x4 a = *reinterpret_cast<const f32x4 *>(&N[(16 * I + i) * LD + 16 * K2 + 4 * g]);
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) y = __builtin_amdgcn_mfma_f32_16x16x4f32(a[r], w[K2][r], y, 0, 0, 0);
-                    }
-                    y = -y;
-                    const f32x4 a = *reinterpret_cast<const f32x4 *>(&P[(16 * I + i) * LD + 16 * I + 4 * g]);
-                    f32x4 z = y;
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) z = __builtin_amdgcn_mfma_f32_16x16x4f32(a[r], bt[r] * y[r], z, 0, 0, 0);
-                    y = z;
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) P[(16 * I + 4 * g + r) * LD + 16 * J + i] = y[r];
-                }
-#pragma unroll
-                for (int r = 0; r < 4; ++r) w[I][r] = bt[r] * y[r];
+                for (int K2 = J; K2 < I; ++K2) nn[I][K2] = rows4(N, I, K2);
             }
+            w[J] = bt[J] * y[J];
+#pragma unroll
+            for (int I = J + 1; I < CT; ++I) {
+#pragma unroll
+                for (int K2 = J; K2 < I; ++K2)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) y[I] = __builtin_amdgcn_mfma_f32_16x16x4f32(nn[I][K2][r], w[K2][r], y[I], 0, 0, 0);
+                f32x4 z = -y[I];
+                const f32x4 v = bt[I] * z;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) z = __builtin_amdgcn_mfma_f32_16x16x4f32(pp[I][r], v[r], z, 0, 0, 0);
+                w[I] = bt[I] * z;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) P[(16 * I + 4 * g + r) * LD + 16 * J + i] = z[r];
+            }
+        };
+        switch (wave) {
+            case 0: column(std::integral_constant<int, 0>{}); break;
+            case 1: if constexpr (CT > 2) column(std::integral_constant<int, 1>{}); break;
+            case 2: if constexpr (CT > 2) column(std::integral_constant<int, 2>{});
         }
         __syncthreads();
         {
@@ -1257,7 +1300,7 @@ __global__ void __launch_bounds__(KD * 4) __attribute__((amdgpu_waves_per_eu(2, 
 
 // ---- launches ------------------------------------------------------------------------------------
 
-constexpr int64_t kMostGroups = int64_t(1) << 16;   // of a launch that loops over chunks
+constexpr int64_t kMostGroups = int64_t(1) << 17;   // of a launch that loops over chunks
 
 template <typename T, int KD, bool REV, bool VEC>
 static int prep_t(const Args &a, hipStream_t s) {
