@@ -49,6 +49,7 @@ typedef struct mm_delta_fwd_params {
     const float *initial_state;  /* (batch, nheads, dk, dv) or NULL (zeros) */
     void *out;                   /* (batch, seqlen, nheads, dv) */
     float *last_state;           /* (batch, nheads, dk, dv) or NULL */
+    void *segment_states;        /* mm_delta_segment_states_size() bytes, 16-byte aligned, written for the backward; or NULL */
     void *workspace;             /* mm_delta_fwd_workspace_size() bytes, 16-byte aligned (required) */
     int64_t workspace_bytes;
     int64_t q_batch_stride, q_seq_stride, q_group_stride;
@@ -74,6 +75,8 @@ typedef struct mm_delta_bwd_params {
     void *dlog_decay;            /* contiguous (batch, seqlen, nheads), or (nheads,) with decay_per_head; or NULL */
     float *dinitial_state;       /* (batch, nheads, dk, dv) or NULL */
     int32_t decay_per_head;      /* log_decay is one value per head: dlog_decay is summed over batch and seqlen */
+    const void *segment_states;  /* what the forward left there, after a call with the same sizes, inputs and device, or NULL
+                                  * (computed again) */
     void *workspace;             /* mm_delta_bwd_workspace_size() bytes, 16-byte aligned (required) */
     int64_t workspace_bytes;
     int64_t q_batch_stride, q_seq_stride, q_group_stride;
@@ -104,9 +107,11 @@ typedef struct mm_delta_update_params {
     int64_t g_batch_stride, g_head_stride;
 } mm_delta_update_params;
 
-/* Workspace bytes (0: none needed). They depend on the sizes and on the current device's compute-unit count: query with
- * the device of the call current. The backward's also depend on whether dlog_decay is NULL. */
+/* Workspace bytes (0: none needed). They depend on the sizes and on the current device's compute-unit count: query with the device of
+ * the call current. They also depend on whether segment_states and the backward's dlog_decay are NULL: query with those pointers set
+ * as in the call. segment_states' own size is 0 where rows are not cut: leave it NULL then. */
 int64_t mm_delta_fwd_workspace_size(const mm_delta_fwd_params *params);
+int64_t mm_delta_segment_states_size(const mm_delta_fwd_params *params);
 int64_t mm_delta_bwd_workspace_size(const mm_delta_bwd_params *params);
 
 int mm_delta_fwd(const mm_delta_fwd_params *params, void *stream);

@@ -14,7 +14,8 @@
 //     dQ = scale diag(e^c) dO S^T + A K,                    A = the lower triangle of scale dO U^T . D
 //     dK = A^T Q + E K + E^T K - diag(e^c) dV S^T + diag(e^(c_end - c)) U R^T,   E = minus the strict one of dV U^T . D
 // P and M need no state: dr_prep makes them for all chunks at once, dr_walk carries the state through a row's chunks, dr_back the
-// state's gradient back, and dr_grad takes dQ and dK chunk by chunk from the kept S, R, Z and dV, again all chunks at once.
+// state's gradient back (rows of few heads in segments: a first walk finds what each adds to the state and what it makes of it, dr_join
+// the states that they start from), and dr_grad takes dQ and dK chunk by chunk from the kept S, R, Z and dV, again all chunks at once.
 //
 // Exactness: as in the linear attention, every float32 factor (S, R, P, M, U, dV and the decayed scores) enters its product as
 // three bfloat16 planes (2^-25), for every input type; 16-bit results are rounded once.
@@ -92,27 +93,24 @@ __device__ __forceinline__ void make_chunk(Chunk<C> &k, uint32_t g, mm_dtype gty
     }
 }
 
-// What a walk needs of it: no factors between two tokens.
+// What a walk needs of it: no factors between two tokens. It lies behind the chunk's images (dr_prep).
 template <int C>
 struct __attribute__((aligned(16))) Steps {
     float in[C], out[C], beta[C], inq[C];   // e^c, e^(c_end - c), beta, scale e^c
     float hi[C], lo[C];                     // c
     float all;                              // e^c_end
 };
+static_assert(sizeof(Steps<64>) == steps_bytes(64) && sizeof(Steps<32>) == steps_bytes(32), "the plan's bytes");
 template <int C>
-__device__ __forceinline__ void make_steps(Steps<C> &k, uint32_t g, mm_dtype gtype, uint32_t b, mm_dtype btype, float scale, int lane) {
-    const double c = prefix_f64(double(decode_g(g, gtype))), all = readlane_f64(c, C - 1);
-    const float hi = float(c), in = exp_f32(hi);
-    if (C == 64 || lane < C) {
-        k.in[lane] = in;
-        k.out[lane] = exp_f32(float(all - c));
-        k.beta[lane] = decode_beta(b, btype);
-        k.inq[lane] = in * scale;
-        k.hi[lane] = hi;
-        k.lo[lane] = float(c - double(hi));
-        if (lane == C - 1) k.all = in;
+__device__ __forceinline__ void write_steps(char *dst, const Chunk<C> &k, int tid) {
+    float *to = reinterpret_cast<float *>(dst);
+    for (int x = tid; x < 6 * C + 1; x += kThreads) {
+        const int n = x / C, t = x % C;
+        to[x] = n == 0 ? k.d.in[t] : n == 1 ? k.d.out[t] : n == 2 ? k.beta[t] : n == 3 ? k.inq[t] : n == 4 ? k.d.hi[t] : n == 5 ? k.d.lo[t] : k.d.all;
     }
 }
+// A chunk's record: N images, then its steps.
+template <int C, int N> constexpr int kRecord = N * kImage<C> * 2 + int(sizeof(Steps<C>));
 
 // ---- products ------------------------------------------------------------------------------------
 
@@ -295,8 +293,7 @@ __device__ __forceinline__ void write_image(char *dst, const float *f, int wave,
             }
 }
 
-// P (and M) of every chunk, as operand images; REV: P, P^T and M^T for the backward (P into img_a's first half... see the plan).
-// One workgroup per chunk. The triangles are made in float32: the diagonal tiles of P by substitution, row by row, those of a column
+// The records of every chunk: the images of P and M; REV, for the backward: that of P, and those of P^T and M^T. One workgroup per chunk. The triangles are made in float32: the diagonal tiles of P by substitution, row by row, those of a column
 // block below by 16 x 16 products on v_mfma_f32_16x16x4_f32, which keeps them float32.
 template <typename T, int KD> constexpr int kPrepGroups = sizeof(T) == 2 || KD == 64 ? 3 : 2;   // on a CU
 template <typename T, int KD, bool REV, bool VEC>
@@ -447,14 +444,17 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(k
         {
             const Args a = args();
             const int64_t at = p.bh * a.chunks + chunk;
-            char *ia = afresh(a.img_a) + at * (REV ? 1 : 2) * kImage<C> * 2;
-            write_image<C, false>(ia, P, wave, lane);
+            char *ra = afresh(a.rec_a) + at * kRecord<C, REV ? 1 : 2>;
+            write_image<C, false>(ra, P, wave, lane);
             if constexpr (!REV) {
-                write_image<C, false>(ia + kImage<C> * 2, M, wave, lane);
+                write_image<C, false>(ra + kImage<C> * 2, M, wave, lane);
+                write_steps<C>(ra + 2 * kImage<C> * 2, *ck, tid);
             } else {
-                char *ib = afresh(a.img_b) + at * 2 * kImage<C> * 2;
-                write_image<C, true>(ib, P, wave, lane);
-                write_image<C, true>(ib + kImage<C> * 2, M, wave, lane);
+                write_steps<C>(ra + kImage<C> * 2, *ck, tid);
+                char *rb = afresh(a.rec_b) + at * kRecord<C, 2>;
+                write_image<C, true>(rb, P, wave, lane);
+                write_image<C, true>(rb + kImage<C> * 2, M, wave, lane);
+                write_steps<C>(rb + 2 * kImage<C> * 2, *ck, tid);
             }
         }
     }
@@ -462,44 +462,186 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(k
 
 // ---- walks ---------------------------------------------------------------------------------------
 
-// An image on its way from memory to LDS.
+// A record on its way from memory to LDS.
 template <int BYTES>
-struct StageImage {
+struct StageRecord {
     static constexpr int N = (BYTES / 16 + kThreads - 1) / kThreads;
     uint4 r[N];
     __device__ __forceinline__ void load(const char *src, int tid) {
         const __amdgpu_buffer_rsrc_t buf = buffer(src);
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const int at = (n * kThreads + tid) * 16;
-            r[n] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(buf, BYTES % (kThreads * 16) == 0 || at < BYTES ? uint32_t(at) : kNone, 0, 0));
+            uint32_t at = uint32_t((n * kThreads + tid) * 16);
+            if ((n + 1) * kThreads * 16 > BYTES && at >= uint32_t(BYTES)) at = kNone;
+            asm("" : "+v"(at));
+            r[n] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(buf, at, 0, 0));
+        }
+    }
+    // The first image and the last `STEPS` bytes of a record of `size` bytes.
+    template <int STEPS>
+    __device__ __forceinline__ void load_ends(const char *src, int size, int tid) {
+        const __amdgpu_buffer_rsrc_t buf = buffer(src);
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            uint32_t at = uint32_t((n * kThreads + tid) * 16);
+            if ((n + 1) * kThreads * 16 > BYTES - STEPS) at = at < uint32_t(BYTES - STEPS) ? at : at < uint32_t(BYTES) ? at + uint32_t(size - BYTES) : kNone;
+            asm("" : "+v"(at));
+            r[n] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(buf, at, 0, 0));
         }
     }
     __device__ __forceinline__ void store(char *dst, int tid) const {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             const int at = (n * kThreads + tid) * 16;
-            if (BYTES % (kThreads * 16) == 0 || at < BYTES) *reinterpret_cast<uint4 *>(dst + at) = r[n];
+            if ((n + 1) * kThreads * 16 <= BYTES || at < BYTES) *reinterpret_cast<uint4 *>(dst + at) = r[n];
         }
     }
 };
 
-// The (pair, slice) of a workgroup. Slices of one pair read the same q, k and images: they are 8 ids apart, which is one XCD and its L2.
+// A workgroup's (pair, segment, slice). Slices of one segment read the same q, k and records: they are 8 ids apart, which is one XCD and
+// its L2.
 struct Unit {
-    unsigned pair, slice;
+    unsigned pair, seg, slice;
     bool live;
 };
-__device__ __forceinline__ Unit unit_of(const Args &a) {
-    const unsigned id = blockIdx.x, per = 8u * unsigned(a.slices), in = id % per;
+__device__ __forceinline__ Unit unit_of(const Args &a, unsigned slices) {
+    const unsigned id = blockIdx.x, per = 8u * slices, in = id % per, ps = id / per * 8u + in % 8u;
     Unit u;
-    u.pair = id / per * 8u + in % 8u;
+    u.pair = ps / unsigned(a.segs);
+    u.seg = ps % unsigned(a.segs);
     u.slice = in / 8u;
-    u.live = u.pair < unsigned(a.batch * a.heads);
+    u.live = ps < unsigned(a.batch * a.heads) * unsigned(a.segs);
     return u;
 }
-inline int64_t unit_grid(const Args &a) { return (a.batch * a.heads + 7) / 8 * 8 * a.slices; }
+inline int64_t unit_grid(const Args &a, int slices) { return (a.batch * a.heads * a.segs + 7) / 8 * 8 * slices; }
 
-// A chunk's tokens one by one, as the recurrence says, for what is not finite in it. out(t, c, the column's q S) in every lane.
+// The wave's outputs of a chunk. Whole 16-byte pieces leave by way of its own columns of V, which no other wave reads (see
+// store_out); they are held until the next chunk's rows are staged, so that those wait for no store.
+template <typename T, int C, int LDV, bool VEC>
+struct HeldOut {
+    static constexpr bool kPieces = VEC && sizeof(T) == 2;
+    static constexpr int CT = C / 16, NP = kPieces ? C * 2 / 64 : 1;
+    u32x4 w[NP];
+    f32x4 o[kPieces ? 1 : CT];
+    int rows;
+
+    __device__ __forceinline__ void take(const f32x4 (&O)[CT][1], u16 *tile, int r, int col, int lane) {
+        rows = r;
+        if constexpr (kPieces) {
+            const int g = lane >> 4, i = lane & 15;
+            wave_fence();
+#pragma unroll
+            for (int t = 0; t < CT; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; e += 2) {
+                    const uint32_t x = std::is_same_v<T, bf16_t> ? pack_bf16x2(O[t][0][e], O[t][0][e + 1]) : pack_f16x2(O[t][0][e], O[t][0][e + 1]);
+                    tile[block<LDV>(16 * t) + at<LDV>(4 * g + e, col + i)] = u16(x);
+                    tile[block<LDV>(16 * t) + at<LDV>(4 * g + e + 1, col + i)] = u16(x >> 16);
+                }
+            wave_fence();
+#pragma unroll
+            for (int n = 0; n < NP; ++n) {
+                const u16 *src = tile + block<LDV>(32 * n);
+                const int row = lane / 2, c = lane % 2 * 8;
+                const uint2 a = *reinterpret_cast<const uint2 *>(src + at<LDV>(row, col + c)), b = *reinterpret_cast<const uint2 *>(src + at<LDV>(row, col + c + 4));
+                w[n] = u32x4{a.x, a.y, b.x, b.y};
+            }
+        } else {
+#pragma unroll
+            for (int t = 0; t < CT; ++t) o[t] = O[t][0];
+        }
+    }
+    // The rows from token t0 on; stride in elements, `cols` of the row exist.
+    __device__ __forceinline__ void flush(char *out, uint32_t stride, int t0, int cols, int col, int lane) const {
+        const __amdgpu_buffer_rsrc_t buf = buffer(out + uint64_t(unsigned(t0)) * stride * sizeof(T));
+        if constexpr (kPieces) {
+#pragma unroll
+            for (int n = 0; n < NP; ++n) {
+                const int row = 32 * n + lane / 2, c = col + lane % 2 * 8;
+                __builtin_amdgcn_raw_buffer_store_b128(w[n], buf, row < rows && c < cols ? uint32_t(row) * stride * 2 + uint32_t(c) * 2 : kNone, 0, 0);
+            }
+        } else {
+            const int g = lane >> 4, x = col + (lane & 15);
+#pragma unroll
+            for (int t = 0; t < CT; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int n = 16 * t + 4 * g + r;
+                    store_element<T, false>(o[t][r], buf, n < rows && x < cols ? uint32_t(n) * stride + uint32_t(x) : kNone);
+                }
+        }
+    }
+};
+
+// X = diag(wx) A S and, with TWO, O = diag(wo) B S for the wave's columns; the state is split once for both.
+template <typename T, int C, int KD, bool TWO>
+__device__ __forceinline__ void state_products(f32x4 (&X)[C / 16][1], f32x4 (&O)[C / 16][1], const f32x4 (&S)[KD / 16][1], const u16 *A, const u16 *B,
+                                               const float *wx, const float *wo, int lane) {
+    constexpr int PL = kTile<C, KD>, PI = Cfg<T>::in, CT = C / 16, STEPS = KD / 32 * (TWO ? 2 : 1);
+    const int g = lane >> 4, i = lane & 15;
+#pragma unroll
+    for (int t = 0; t < CT; ++t) X[t][0] = O[t][0] = f32x4{0.f, 0.f, 0.f, 0.f};
+    // The next step's rows are read while the products of this one run.
+    bf16x8 a[2][CT][PI];
+    auto read = [&](int n) {
+        const u16 *tile = TWO && n % 2 ? B : A;
+        const int k = TWO ? n / 2 : n;
+#pragma unroll
+        for (int t = 0; t < CT; ++t)
+#pragma unroll
+            for (int p = 0; p < PI; ++p) a[n % 2][t][p] = frag_row<KD>(tile + p * PL, 16 * t, k, g, i);
+    };
+    auto split = [&](int k, bf16x8 (&s)[kPlanes]) {
+        float x[8];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            x[r] = S[2 * k][0][r];
+            x[4 + r] = S[2 * k + 1][0][r];
+        }
+        split8(x, s);
+    };
+    read(0);
+    bf16x8 s[2][kPlanes];
+    split(0, s[0]);
+#pragma unroll
+    for (int n = 0; n < STEPS; ++n) {
+        const int k = TWO ? n / 2 : n;
+        if (n + 1 < STEPS) read(n + 1);
+        const bool ahead = k + 1 < KD / 32 && (!TWO || n % 2 == 0);
+        if (ahead) split(k + 1, s[(k + 1) % 2]);
+#pragma unroll
+        for (int p = 0; p < PI; ++p)
+#pragma unroll
+            for (int q = 0; q < kPlanes; ++q)
+                if (p + q < kPlanes)
+#pragma unroll
+                    for (int t = 0; t < CT; ++t) {
+                        f32x4 &to = TWO && n % 2 ? O[t][0] : X[t][0];
+                        to = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[n % 2][t][p], s[k % 2][q], to, 0, 0, 0);
+                    }
+        // The next operands' reads first; then the products with the state's next split between them, a product's time each.
+        __builtin_amdgcn_sched_group_barrier(0x100, 4 * CT * PI, 0);
+#pragma unroll
+        for (int m = 0; m < CT * (PI == 1 ? 3 : PI == 2 ? 5 : 6); ++m) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int t = 0; t < CT; ++t) {
+        const f32x4 f = *reinterpret_cast<const f32x4 *>(wx + 16 * t + 4 * g);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) X[t][0][r] *= f[r];
+        if constexpr (TWO) {
+            const f32x4 h = *reinterpret_cast<const f32x4 *>(wo + 16 * t + 4 * g);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) O[t][0][r] *= h[r];
+        }
+    }
+}
+
+// A chunk's tokens one by one, as the recurrence says. out(t, c, the column's q S) in every lane.
 template <typename T, int C, int KD, int NC, int LDV, typename F>
 __device__ __forceinline__ void recur_delta(f32x4 (&S)[KD / 16][NC], const u16 *Q, const u16 *K, const u16 *V, const Steps<C> &ck, int rows, int kdim,
                                             int col, int lane, F &&out) {
@@ -531,6 +673,7 @@ __device__ __forceinline__ void recur_delta(f32x4 (&S)[KD / 16][NC], const u16 *
             z[c] += __shfl_xor(z[c], 32);
             z[c] = (tile_at<T, C, LDV>(V, t, col + 16 * c + i) - z[c]) * ck.beta[t];
         }
+        kdim = afresh(kdim);   // (no masks of all rows held from the loop above)
 #pragma unroll
         for (int k = 0; k < KD / 16; ++k) {
             float y[4], x[4];
@@ -555,18 +698,83 @@ __device__ __forceinline__ void recur_delta(f32x4 (&S)[KD / 16][NC], const u16 *
     }
 }
 
-// The state's way through a row's chunks, a workgroup 64 columns of it, a wave 16. Forward: outputs and the last state. STATES (the
-// backward's): the state before every chunk and Z instead.
-template <typename T, int KD, bool STATES, bool VEC>
+// The state that a unit starts from.
+template <int KD>
+__device__ __forceinline__ void start_state(f32x4 (&S)[KD / 16][1], const Args &a, const Spot &p, int seg, int col0, int col, int lane) {
+    if (a.segs > 1) {
+        const int vd = 64 * a.slices;
+        load_state<KD, 1>(S, Mat{a.starts + (int64_t(p.bh) * a.segs + seg) * KD * vd + col0, vd, 1}, KD, 64, col, lane);
+    } else {
+        load_state<KD, 1>(S, Mat{const_cast<float *>(a.s0 ? a.s0 + int64_t(p.bh) * a.dk * a.dv + col0 : nullptr), a.dv, 1}, a.dk, a.dv - col0, col, lane);
+    }
+}
+
+// What an infinity or NaN reaches is not what the chunks' products make of it (their planes and masked zeros make NaN of more). A walk
+// that met one is followed by this: the recurrence once more from its start, whose outputs from the wave's first such chunk on (`first`),
+// and state, take the others' place. Its arguments are read again, so that nothing of it takes registers while the products run.
+template <typename T, int KD, bool VEC>
+__device__ __forceinline__ void infinite_rows(f32x4 (&S)[KD / 16][1], char *smem, int seg, int beg, int end, int first) {
+    constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, W = 64;
+    auto args = [] { return own_args<Args>(); };
+    u16 *K = reinterpret_cast<u16 *>(smem), *Q = K + PI * kTile<C, KD>, *V = Q + PI * kTile<C, KD>;
+    Steps<C> &ck = *reinterpret_cast<Steps<C> *>(V + PI * kTile<C, W>);
+    const int tid = afresh_lane(threadIdx.x), wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid & 63, col = wave * 16;
+    const Unit u = unit_of(args(), args().slices);
+    const Spot p = spot_of(args(), u.pair);
+    const int col0 = int(u.slice) * W;
+    f32x4 R[KD / 16][1];
+    start_state<KD>(R, args(), p, seg, col0, col, lane);
+    __threadfence();   // the outputs that are stored once more
+#pragma unroll 1
+    for (int t0 = beg; t0 < end; t0 += C) {
+        const Args a = args();
+        const int rows = min(C, end - t0);
+        __syncthreads();
+        {
+            Stage<T, C, KD, kThreads, VEC> s;
+            s.load(rows_of<T>(a.k, p.b, p.h, a.dk), t0, rows, tid);
+            s.store(K, tid);
+            s.load(rows_of<T>(a.q, p.b, p.h, a.dk), t0, rows, tid);
+            s.store(Q, tid);
+        }
+        {
+            Stage<T, C, W, kThreads, VEC> s;
+            s.load(rows_of<T>(a.v, p.b, p.h, a.dv, col0), t0, rows, tid);
+            s.store(V, tid);
+        }
+        const float *steps = reinterpret_cast<const float *>(a.rec_a + (int64_t(p.bh) * a.chunks + t0 / C + 1) * kRecord<C, 2> - sizeof(Steps<C>));
+        for (int x = tid; x < int(sizeof(Steps<C>)) / 4; x += kThreads) reinterpret_cast<float *>(&ck)[x] = steps[x];
+        __syncthreads();
+        const __amdgpu_buffer_rsrc_t to = buffer(static_cast<char *>(a.out) + (p.b * a.out_batch + p.h * a.out_head + t0 * a.out_seq + col0) * int64_t(sizeof(T)));
+        recur_delta<T, C, KD, 1, W>(R, Q, K, V, ck, rows, a.dk, col, lane, [&](int t, int, float x) {
+            const int at = col + (lane & 15);
+            store_element<T, false>(x * a.scale, to, t0 >= first && lane < 16 && at < a.dv - col0 ? uint32_t(t) * uint32_t(a.out_seq) + uint32_t(at) : kNone);
+        });
+    }
+    if (first < end)
+#pragma unroll
+        for (int k = 0; k < KD / 16; ++k) S[k][0] = R[k][0];
+}
+
+// What a walk leaves.
+enum Leaves {
+    kOutputs,   // outputs, and the last state
+    kStates,    // the state before every chunk, and Z (the backward's)
+    kMaps       // of a segment: what it adds to the state (V's columns) and what it makes of it (as many columns as rows, from the identity)
+};
+
+// The state's way through a segment's chunks, a workgroup 64 columns of it, a wave 16.
+template <typename T, int KD, Leaves L, bool VEC>
 __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) dr_walk(const Args) {
     constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, W = 64, NC = 1, CT = C / 16;
-    constexpr int kImages = (STATES ? 1 : 2) * kImage<C> * 2;
+    constexpr bool kOut = L == kOutputs;
+    constexpr int kLoaded = kRecord<C, kOut ? 2 : 1>;
     typedef Stage<T, C, KD, kThreads, VEC> SX;
     typedef Stage<T, C, W, kThreads, VEC> SV;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    u16 *K = reinterpret_cast<u16 *>(smem), *Q = K + PI * kTile<C, KD>, *V = STATES ? Q : Q + PI * kTile<C, KD>;
+    u16 *K = reinterpret_cast<u16 *>(smem), *Q = K + PI * kTile<C, KD>, *V = kOut ? Q + PI * kTile<C, KD> : Q;
     u16 *img = V + PI * kTile<C, W>;
-    Steps<C> *cks = reinterpret_cast<Steps<C> *>(img + kImages / 2);
+    const Steps<C> &ck = *reinterpret_cast<const Steps<C> *>(img + (kOut ? 2 : 1) * kImage<C>);
 
     int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid / 64), col = wave * 16 * NC;
@@ -575,72 +783,87 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
         lane = tid & 63;
     };
     auto args = [] { return own_args<Args>(); };
-    const Unit u = unit_of(args());
+    const Unit u = unit_of(args(), L == kMaps ? args().slices + KD / 64 : args().slices);
     if (!u.live) return;
     const Spot p = spot_of(args(), u.pair);
-    const int col0 = afresh(int(u.slice) * W), end = afresh(int(args().seqlen));
+    const int col0 = afresh(int(u.slice) * W);
+    int beg, end;
+    {
+        const Args a = args();
+        beg = afresh(int(u.seg) * int(a.seg_len));
+        end = afresh(min(int(a.seqlen), beg + int(a.seg_len)));
+        if constexpr (kOut) {
+            // A state that is not finite goes through its row in one piece, as the recurrence does.
+            if (a.segs > 1 && a.flags[p.bh]) {
+                if (u.seg) return;
+                end = afresh(int(a.seqlen));
+            }
+        }
+        // What the last segment adds is nobody's start; what it makes of the state is, in the backward.
+        if (L == kMaps && u.seg + 1 == unsigned(a.segs) && (!a.last_map || int(u.slice) < a.slices)) return;
+    }
     f32x4 S[KD / 16][NC];
     {
         const Args a = args();
-        load_state<KD, NC>(S, Mat{const_cast<float *>(a.s0 ? a.s0 + int64_t(p.bh) * a.dk * a.dv + col0 : nullptr), a.dv, 1}, a.dk, a.dv - col0, col, lane);
+        if (L == kMaps) {
+            const int j0 = col0 - 64 * a.slices + col;
+#pragma unroll
+            for (int k = 0; k < KD / 16; ++k)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) S[k][0][r] = j0 >= 0 && 16 * k + 4 * (lane >> 4) + r == j0 + (lane & 15) ? 1.f : 0.f;
+        } else {
+            start_state<KD>(S, a, p, u.seg, col0, col, lane);
+        }
     }
     auto tensor = [&](auto of) { const Args a = args(); return of(a); };
     const Rows<T> rk = tensor([&](const Args &a) { return rows_of<T>(a.k, p.b, p.h, a.dk); });
-    const Rows<T> rq = STATES ? rk : tensor([&](const Args &a) { return rows_of<T>(a.q, p.b, p.h, a.dk); });
+    const Rows<T> rq = kOut ? tensor([&](const Args &a) { return rows_of<T>(a.q, p.b, p.h, a.dk); }) : rk;
     const Rows<T> rv = tensor([&](const Args &a) { return rows_of<T>(a.v, p.b, p.h, a.dv, col0); });
-    const Gates gg = tensor([&](const Args &a) { return gates_of(a.g, p); });
-    const Gates gb = tensor([&](const Args &a) { return gates_of(a.beta, p); });
-    const float scale = afresh(args().scale);
-    const char *images = tensor([&](const Args &a) { return afresh(a.img_a + int64_t(p.bh) * a.chunks * kImages); });
+    const int stride = afresh(args().rec_a_step);
+    const char *records = tensor([&](const Args &a) { return afresh(a.rec_a + int64_t(p.bh) * a.chunks * a.rec_a_step); });
     char *const out = tensor([&](const Args &a) {
-        return STATES ? nullptr : afresh(static_cast<char *>(a.out) + (p.b * a.out_batch + p.h * a.out_head + col0) * int64_t(sizeof(T)));
+        return kOut ? afresh(static_cast<char *>(a.out) + (p.b * a.out_batch + p.h * a.out_head + col0) * int64_t(sizeof(T))) : nullptr;
     });
     const uint32_t out_stride = uint32_t(afresh(int(args().out_seq)));
 
     SX sk, sq;
     SV sv;
-    StageImage<kImages> si;
-    uint32_t gnext = 0, bnext = 0;
-    auto load = [&](int t0) {
+    StageRecord<kLoaded> si;
+    auto load_rows = [&](int t0) {
         const int rows = min(C, end - t0);
         sk.load(rk, t0, rows, tid);
-        si.load(images + int64_t(t0 / C) * kImages, tid);
-        if constexpr (!STATES) sq.load(rq, t0, rows, tid);
+        if constexpr (kOut) sq.load(rq, t0, rows, tid);
         sv.load(rv, t0, rows, tid);
     };
-    auto load_gates = [&](int t0) {
-        gnext = load_gate<C>(gg, t0, end, lane);
-        bnext = load_gate<C>(gb, t0, end, lane);
+    auto load_record = [&](int t0) {
+        // P and the steps; in the forward's records M lies between.
+        if constexpr (kOut) si.load(records + int64_t(t0 / C) * stride, tid);
+        else si.template load_ends<int(sizeof(Steps<C>))>(records + int64_t(t0 / C) * stride, stride, tid);
     };
-    auto make = [&](int buf) { make_steps<C>(cks[buf], gnext, gg.type, bnext, gb.type, scale, lane); };
-    const bool dwave = wave == kWaves - 1;
-    load(0);
-    if (dwave) {
-        load_gates(0);
-        make(0);
-        if (C < end) load_gates(C);
-    }
-    int buf = 0;
-    for (int t0 = 0; t0 < end; t0 += C, buf ^= 1) {
+    load_record(beg);
+    load_rows(beg);
+    HeldOut<T, C, W, VEC> held;
+    int first_odd = 0x7fffffff;   // the first chunk with something not finite in it
+    for (int t0 = beg; t0 < end; t0 += C) {
         const int rows = min(C, end - t0);
-        const bool more = t0 + C < end;
         __syncthreads();
         fresh();
         sk.store(K, tid);
         si.store(reinterpret_cast<char *>(img), tid);
-        if constexpr (!STATES) sq.store(Q, tid);
+        if constexpr (kOut) sq.store(Q, tid);
         sv.store(V, tid);
-        if (more) load(t0 + C);
+        if constexpr (kOut)
+            if (t0 > beg) held.flush(out, out_stride, t0 - C, rv.d, col, lane);
+        if (t0 + C < end) load_rows(t0 + C);
         __syncthreads();
         fresh();
-        const Steps<C> &ck = cks[buf];
-        if constexpr (STATES) {
+        if constexpr (L == kStates) {
             const Args a = args();
             const int vd = 64 * a.slices;
             store_state<KD, NC>(S, Mat{a.states + (int64_t(p.bh) * a.chunks + t0 / C) * KD * vd + col0, vd, 1}, KD, W, col, lane);
         }
         f32x4 X[CT][NC], O[CT][NC];
-        inter<T, C, KD, NC>(X, S, K, ck.in, lane);
+        state_products<T, C, KD, kOut>(X, O, S, K, Q, ck.in, ck.inq, lane);
         tile_columns<T, C, NC, W>(V, col, lane, [&](int j, int c, const float *v) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
@@ -648,17 +871,12 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
                 X[2 * j + 1][c][r] = v[4 + r] - X[2 * j + 1][c][r];
             }
         });
-        if constexpr (!STATES) inter<T, C, KD, NC>(O, S, Q, ck.inq, lane);
-        if (dwave && more) {
-            make(buf ^ 1);
-            if (t0 + 2 * C < end) load_gates(t0 + 2 * C);
-        }
         fresh();
         bf16x8 f[C / 32][NC][kPlanes];
         split_rows<C, NC>(f, X, ck.beta, lane);
         triangle<C, NC, true, kPlanes>(X, img, f, lane);   // Z
         const int g = lane >> 4;
-        if constexpr (STATES) {
+        if constexpr (L == kStates) {
             const Args a = args();
             const int vd = 64 * a.slices;
             const __amdgpu_buffer_rsrc_t to = buffer(a.z + (int64_t(p.bh) * a.chunks * C + t0) * vd + col0 + col);
@@ -666,91 +884,74 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
             for (int t = 0; t < CT; ++t)
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-#pragma unroll
-                    for (int c = 0; c < NC; ++c)
-                        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(X[t][c][r]), to, uint32_t((16 * t + 4 * g + r) * vd + 16 * c + (lane & 15)) * 4, 0, 0);
+                    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(X[t][0][r]), to, uint32_t((16 * t + 4 * g + r) * vd + (lane & 15)) * 4, 0, 0);
         }
-        bool odd = false;
-        float U0[CT][4];
 #pragma unroll
         for (int t = 0; t < CT; ++t) {
             const f32x4 b = *reinterpret_cast<const f32x4 *>(ck.beta + 16 * t + 4 * g);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) U0[t][r] = b[r];
+            X[t][0] *= b;   // U
         }
-#pragma unroll
-        for (int t = 0; t < CT; ++t)
-#pragma unroll
-            for (int c = 0; c < NC; ++c)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) X[t][c][r] *= U0[t][r];   // U
-        if constexpr (!STATES) {
+        if constexpr (kOut) {
             bf16x8 w[C / 32][NC][kPlanes];
 #pragma unroll
-            for (int j = 0; j < C / 32; ++j)
+            for (int j = 0; j < C / 32; ++j) {
+                float y[8];
 #pragma unroll
-                for (int c = 0; c < NC; ++c) {
-                    float y[8];
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        y[r] = X[2 * j][c][r];
-                        y[4 + r] = X[2 * j + 1][c][r];
-                    }
-                    split8(y, w[j][c]);
+                for (int r = 0; r < 4; ++r) {
+                    y[r] = X[2 * j][0][r];
+                    y[4 + r] = X[2 * j + 1][0][r];
                 }
+                split8(y, w[j][0]);
+            }
             triangle<C, NC, true, kPlanes>(O, img + kImage<C>, w, lane);
             // 0 times what is not finite is not 0.
             float nan = 0.f;
 #pragma unroll
             for (int t = 0; t < CT; ++t)
 #pragma unroll
-                for (int c = 0; c < NC; ++c)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        nan = __builtin_fmaf(X[t][c][r], 0.f, nan);
-                        nan = __builtin_fmaf(O[t][c][r], 0.f, nan);
-                    }
-            odd = __any(!(nan == 0.f));
+                for (int r = 0; r < 4; ++r) {
+                    nan = __builtin_fmaf(X[t][0][r], 0.f, nan);
+                    nan = __builtin_fmaf(O[t][0][r], 0.f, nan);
+                }
+            if (first_odd > t0 && __any(!(nan == 0.f))) first_odd = t0;
         }
-        if (STATES || !odd) {
-            split_rows<C, NC>(f, X, ck.out, lane);
-            const float all = ck.all;
+        if (t0 + C < end) load_record(t0 + C);
+        split_rows<C, NC>(f, X, ck.out, lane);
+        const float all = ck.all;
 #pragma unroll
-            for (int k = 0; k < KD / 16; ++k)
-#pragma unroll
-                for (int c = 0; c < NC; ++c)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) S[k][c][r] *= all;
-            add_rows<T, C, KD, NC>(S, K, f, lane);
-            fresh();
-            if constexpr (!STATES) store_out<T, C, NC, W, VEC, false>(O, out, out_stride, t0, rows, rv.d, V, col, lane);
-        } else if constexpr (!STATES) {
-            const Args a = args();
-            const __amdgpu_buffer_rsrc_t to = buffer(out + uint64_t(unsigned(t0)) * out_stride * sizeof(T));
-            recur_delta<T, C, KD, NC, W>(S, Q, K, V, ck, rows, a.dk, col, lane, [&](int t, int c, float x) {
-                const int at = col + 16 * c + (lane & 15);
-                store_element<T, false>(x * scale, to, lane < 16 && at < rv.d ? uint32_t(t) * out_stride + uint32_t(at) : kNone);
-            });
-        }
+        for (int k = 0; k < KD / 16; ++k) S[k][0] *= all;
+        add_rows<T, C, KD, NC>(S, K, f, lane);
+        fresh();
+        if constexpr (kOut) held.take(O, V, rows, col, lane);
     }
-    if constexpr (!STATES) {
-        const Args a = args();
-        if (a.s1) store_state<KD, NC>(S, Mat{a.s1 + int64_t(p.bh) * a.dk * a.dv + col0, a.dv, 1}, a.dk, a.dv - col0, col, lane);
+    if constexpr (kOut) {
+        held.flush(out, out_stride, beg + (end - 1 - beg) / C * C, rv.d, col, lane);
+        if (__syncthreads_or(first_odd < end)) infinite_rows<T, KD, VEC>(S, smem, u.seg, beg, end, first_odd);
+    }
+    const Args a = args();
+    if constexpr (kOut) {
+        if (a.s1 && end == int(a.seqlen)) store_state<KD, NC>(S, Mat{a.s1 + int64_t(p.bh) * a.dk * a.dv + col0, a.dv, 1}, a.dk, a.dv - col0, col, lane);
+    }
+    if constexpr (L == kMaps) {
+        const int md = 64 * a.slices + KD;
+        store_state<KD, NC>(S, Mat{a.maps + (int64_t(p.bh) * a.segs + u.seg) * KD * md + col0, md, 1}, KD, W, col, lane);
+        if (u.seg == 0 && u.slice == 0 && tid == 0) a.flags[p.bh] = 0;
     }
 }
 
-// The state's gradient R back through a row's chunks: dV, dbeta's shares, R at every chunk's end, and the first state's gradient.
-template <typename T, int KD, bool VEC>
+// The state's gradient R back through a segment's chunks: dV, dbeta's shares, R at every chunk's end, and the first state's gradient.
+// MAPS: what a segment adds to R alone.
+template <typename T, int KD, bool MAPS, bool VEC>
 __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) dr_back(const Args) {
     constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, W = 64, NC = 1, CT = C / 16;
-    constexpr int kImages = 2 * kImage<C> * 2;
+    constexpr int kRec = kRecord<C, 2>;
     typedef Stage<T, C, KD, kThreads, VEC> SX;
     typedef Stage<T, C, W, kThreads, VEC> SV;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     u16 *K = reinterpret_cast<u16 *>(smem), *Q = K + PI * kTile<C, KD>, *V = Q + PI * kTile<C, KD>;
     u16 *img = V + PI * kTile<C, W>;
-    Steps<C> *cks = reinterpret_cast<Steps<C> *>(img + kImages / 2);
-    float *part = reinterpret_cast<float *>(cks + 2);   // [wave][C]
+    const Steps<C> &ck = *reinterpret_cast<const Steps<C> *>(img + 2 * kImage<C>);
+    float *part = reinterpret_cast<float *>(reinterpret_cast<char *>(img) + kRec);   // [wave][C]
 
     int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid / 64), col = wave * 16 * NC;
@@ -759,88 +960,80 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
         lane = tid & 63;
     };
     auto args = [] { return own_args<Args>(); };
-    const Unit u = unit_of(args());
-    if (!u.live) return;
+    const Unit u = unit_of(args(), args().slices);
+    if (!u.live || (MAPS && u.seg == 0)) return;
     const Spot p = spot_of(args(), u.pair);
-    const int col0 = afresh(int(u.slice) * W), end = afresh(int(args().seqlen)), chunks = (end + C - 1) / C;
+    const int col0 = afresh(int(u.slice) * W);
+    int beg, end;
+    {
+        const Args a = args();
+        beg = afresh(int(u.seg) * int(a.seg_len));
+        end = afresh(min(int(a.seqlen), beg + int(a.seg_len)));
+    }
+    const int first = beg / C, last = (end - 1) / C;
     f32x4 R[KD / 16][NC];
     {
         const Args a = args();
-        load_state<KD, NC>(R, Mat{const_cast<float *>(a.dlast ? a.dlast + int64_t(p.bh) * a.dk * a.dv + col0 : nullptr), a.dv, 1}, a.dk, a.dv - col0, col, lane);
+        if (MAPS) {
+            load_state<KD, NC>(R, Mat{nullptr, 0, 1}, 0, 0, col, lane);
+        } else if (a.segs > 1) {
+            const int vd = 64 * a.slices;
+            load_state<KD, NC>(R, Mat{a.back_starts + (int64_t(p.bh) * a.segs + u.seg) * KD * vd + col0, vd, 1}, KD, W, col, lane);
+        } else {
+            load_state<KD, NC>(R, Mat{const_cast<float *>(a.dlast ? a.dlast + int64_t(p.bh) * a.dk * a.dv + col0 : nullptr), a.dv, 1}, a.dk, a.dv - col0, col, lane);
+        }
     }
     auto tensor = [&](auto of) { const Args a = args(); return of(a); };
     const Rows<T> rk = tensor([&](const Args &a) { return rows_of<T>(a.k, p.b, p.h, a.dk); });
     const Rows<T> rq = tensor([&](const Args &a) { return rows_of<T>(a.q, p.b, p.h, a.dk); });
     const Rows<T> rd = tensor([&](const Args &a) { return rows_of<T>(a.dout, p.b, p.h, a.dv, col0); });
-    const Gates gg = tensor([&](const Args &a) { return gates_of(a.g, p); });
-    const Gates gb = tensor([&](const Args &a) { return gates_of(a.beta, p); });
-    const float scale = afresh(args().scale);
-    const char *images = tensor([&](const Args &a) { return afresh(a.img_b + int64_t(p.bh) * a.chunks * kImages); });
+    const char *records = tensor([&](const Args &a) { return afresh(a.rec_b + int64_t(p.bh) * a.chunks * kRec); });
     char *const out = tensor([&](const Args &a) {
         return afresh(static_cast<char *>(a.out) + (p.b * a.out_batch + p.h * a.out_head + col0) * int64_t(sizeof(T)));
     });
     const uint32_t out_stride = uint32_t(afresh(int(args().out_seq)));
     SX sk, sq;
     SV sd;
-    StageImage<kImages> si;
-    uint32_t gnext = 0, bnext = 0;
+    StageRecord<kRec> si;
     auto load = [&](int n) {
         const int t0 = n * C, rows = min(C, end - t0);
         sk.load(rk, t0, rows, tid);
-        si.load(images + int64_t(n) * kImages, tid);
+        si.load(records + int64_t(n) * kRec, tid);
         sq.load(rq, t0, rows, tid);
         sd.load(rd, t0, rows, tid);
     };
-    auto load_gates = [&](int n) {
-        gnext = load_gate<C>(gg, n * C, end, lane);
-        bnext = load_gate<C>(gb, n * C, end, lane);
-    };
-    auto make = [&](int buf) { make_steps<C>(cks[buf], gnext, gg.type, bnext, gb.type, scale, lane); };
-    const bool dwave = wave == kWaves - 1;
-    load(chunks - 1);
-    if (dwave) {
-        load_gates(chunks - 1);
-        make(0);
-        if (chunks > 1) load_gates(chunks - 2);
-    }
-    int buf = 0;
-    for (int n = chunks - 1; n >= 0; --n, buf ^= 1) {
+    load(last);
+    HeldOut<T, C, W, VEC> held;
+    for (int n = last; n >= first; --n) {
         const int t0 = n * C, rows = min(C, end - t0);
-        const bool more = n > 0;
         __syncthreads();
         fresh();
         sk.store(K, tid);
         si.store(reinterpret_cast<char *>(img), tid);
         sq.store(Q, tid);
         sd.store(V, tid);
-        if (more) load(n - 1);
         f32x4 Z[CT][NC];
         const int g = lane >> 4;
-        {
+        if constexpr (!MAPS) {
             const Args a = args();
             const int vd = 64 * a.slices;
-            store_state<KD, NC>(R, Mat{a.r + (int64_t(p.bh) * a.chunks + n) * KD * vd + col0, vd, 1}, KD, W, col, lane);
             const __amdgpu_buffer_rsrc_t from = buffer(a.z + (int64_t(p.bh) * a.chunks * C + t0) * vd + col0 + col);
 #pragma unroll
             for (int t = 0; t < CT; ++t)
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-#pragma unroll
-                    for (int c = 0; c < NC; ++c)
-                        Z[t][c][r] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(from, uint32_t((16 * t + 4 * g + r) * vd + 16 * c + (lane & 15)) * 4, 0, 0));
+                    Z[t][0][r] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(from, uint32_t((16 * t + 4 * g + r) * vd + (lane & 15)) * 4, 0, 0));
+            if (n < last) held.flush(out, out_stride, t0 + C, rd.d, col, lane);
+            store_state<KD, NC>(R, Mat{a.r + (int64_t(p.bh) * a.chunks + n) * KD * vd + col0, vd, 1}, KD, W, col, lane);
         }
+        if (n > first) load(n - 1);
         __syncthreads();
         fresh();
-        const Steps<C> &ck = cks[buf];
-        f32x4 G[CT][NC];
-        inter<T, C, KD, NC>(G, R, K, ck.out, lane);
+        f32x4 G[CT][NC], none[CT][NC];
+        state_products<T, C, KD, false>(G, none, R, K, K, ck.out, ck.out, lane);
         bf16x8 d[C / 32][NC][PI];
         load_v<T, C, NC, W>(d, V, col, lane);
         triangle<C, NC, false, PI>(G, img + kImage<C>, d, lane);   // dU
-        if (dwave && more) {
-            make(buf ^ 1);
-            if (n > 1) load_gates(n - 2);
-        }
         fresh();
         bf16x8 f[C / 32][NC][kPlanes];
         split_rows<C, NC>(f, G, ck.beta, lane);
@@ -848,19 +1041,15 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
 #pragma unroll
         for (int t = 0; t < CT; ++t) {
             const f32x4 b = *reinterpret_cast<const f32x4 *>(ck.beta + 16 * t + 4 * g);
-            f32x4 s = {0.f, 0.f, 0.f, 0.f};
+            if constexpr (!MAPS) {
+                f32x4 s = G[t][0] * Z[t][0];
 #pragma unroll
-            for (int c = 0; c < NC; ++c)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    s[r] = __builtin_fmaf(G[t][c][r], Z[t][c][r], s[r]);
-                    G[t][c][r] *= b[r];   // dV
-                }
-#pragma unroll
-            for (int r = 0; r < 4; ++r) s[r] = group_sum<16>(s[r]);
-            if ((lane & 15) == 0) *reinterpret_cast<f32x4 *>(part + wave * C + 16 * t + 4 * g) = s;
+                for (int r = 0; r < 4; ++r) s[r] = group_sum<16>(s[r]);
+                if ((lane & 15) == 0) *reinterpret_cast<f32x4 *>(part + wave * C + 16 * t + 4 * g) = s;
+            }
+            G[t][0] *= b;   // dV
         }
-        {
+        if constexpr (!MAPS) {
             const Args a = args();
             const int vd = 64 * a.slices;
             const __amdgpu_buffer_rsrc_t to = buffer(a.dx + (int64_t(p.bh) * a.chunks * C + t0) * vd + col0 + col);
@@ -868,34 +1057,125 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
             for (int t = 0; t < CT; ++t)
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-#pragma unroll
-                    for (int c = 0; c < NC; ++c)
-                        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(G[t][c][r]), to, uint32_t((16 * t + 4 * g + r) * vd + 16 * c + (lane & 15)) * 4, 0, 0);
+                    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(G[t][0][r]), to, uint32_t((16 * t + 4 * g + r) * vd + (lane & 15)) * 4, 0, 0);
         }
         // R = e^c_end R + Q^T (scale e^c dO) - K^T (e^c dV)
         update<T, C, KD, NC>(R, d, Q, ck.inq, ck.all, lane);
         {
             f32x4 y[CT][NC];
 #pragma unroll
-            for (int t = 0; t < CT; ++t)
-#pragma unroll
-                for (int c = 0; c < NC; ++c) y[t][c] = -G[t][c];
+            for (int t = 0; t < CT; ++t) y[t][0] = -G[t][0];
             split_rows<C, NC>(f, y, ck.in, lane);
         }
         add_rows<T, C, KD, NC>(R, K, f, lane);
         fresh();
-        store_out<T, C, NC, W, VEC, false>(G, out, out_stride, t0, rows, rd.d, V, col, lane);
-        __syncthreads();
-        if (tid < C) {
-            float s = 0.f;
+        if constexpr (!MAPS) {
+            held.take(G, V, rows, col, lane);
+            __syncthreads();
+            if (tid < C) {
+                float s = 0.f;
 #pragma unroll
-            for (int w = 0; w < kWaves; ++w) s += part[w * C + tid];
-            const Args a = args();
-            a.pbeta[(int64_t(u.slice) * a.batch * a.heads + p.bh) * a.chunks * C + t0 + tid] = s;
+                for (int w = 0; w < kWaves; ++w) s += part[w * C + tid];
+                const Args a = args();
+                a.pbeta[(int64_t(u.slice) * a.batch * a.heads + p.bh) * a.chunks * C + t0 + tid] = s;
+            }
         }
     }
     const Args a = args();
-    if (a.ds0) store_state<KD, NC>(R, Mat{a.ds0 + int64_t(p.bh) * a.dk * a.dv + col0, a.dv, 1}, a.dk, a.dv - col0, col, lane);
+    if constexpr (MAPS) {
+        const int vd = 64 * a.slices;
+        store_state<KD, NC>(R, Mat{a.back_maps + (int64_t(p.bh) * a.segs + u.seg) * KD * vd + col0, vd, 1}, KD, W, col, lane);
+    } else {
+        held.flush(out, out_stride, first * C, rd.d, col, lane);
+        if (a.ds0 && u.seg == 0) store_state<KD, NC>(R, Mat{a.ds0 + int64_t(p.bh) * a.dk * a.dv + col0, a.dv, 1}, a.dk, a.dv - col0, col, lane);
+    }
+}
+
+// The segments' maps (B | A: what they add, what they make of the state) into the states that they start from; BACK: into R at their ends,
+// by the transposes of A. One workgroup per 32 columns of a (batch row, head); its waves split the rows, in float32 on
+// v_mfma_f32_16x16x4_f32, the next segment's map on its way meanwhile. A row that holds something not finite is flagged.
+template <int KD, bool BACK>
+__global__ void __launch_bounds__(kThreads) dr_join(const Args) {
+    constexpr int NT = KD / 64, NC = 2;   // tiles of 16 rows, of 16 columns per wave
+    __shared__ float S[2][KD][16 * NC + 4];
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid & 63, g = lane >> 4, i = lane & 15;
+    const Args a = own_args<Args>();
+    const int vd = 64 * a.slices, md = vd + KD, segs = a.segs, groups = vd / (16 * NC), row0 = 16 * wave * NT;
+    const int64_t bh = blockIdx.x / groups;
+    const int col = int(blockIdx.x % groups) * 16 * NC;
+    const float *edge = BACK ? a.dlast : a.s0;
+    float *starts = (BACK ? a.back_starts : a.starts) + bh * segs * KD * vd;
+    const float *maps = a.maps + bh * segs * KD * md, *adds = BACK ? a.back_maps + bh * segs * KD * vd : maps;
+    const int ad = BACK ? vd : md;
+    float nan = 0.f;
+    f32x4 x[NT][NC], add[NT][NC], ma[NT][KD / 16];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int row = row0 + 16 * t + 4 * g + r, v = col + 16 * c + i;
+                x[t][c][r] = edge && row < a.dk && v < a.dv ? edge[bh * a.dk * a.dv + int64_t(row) * a.dv + v] : 0.f;
+            }
+    auto load = [&](int seg) {
+        const float *m = maps + int64_t(seg) * KD * md + vd, *b = adds + int64_t(seg) * KD * ad + col;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const int at = row0 + 16 * t;
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) add[t][c][r] = b[(at + 4 * g + r) * ad + 16 * c + i];
+#pragma unroll
+            for (int k = 0; k < KD / 16; ++k) {
+                if constexpr (BACK) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) ma[t][k][r] = m[(16 * k + 4 * g + r) * md + at + i];
+                } else {
+                    ma[t][k] = *reinterpret_cast<const f32x4 *>(m + (at + i) * md + 16 * k + 4 * g);
+                }
+            }
+        }
+    };
+    load(BACK ? segs - 1 : 0);
+    for (int n = 0; n < segs; ++n) {
+        const int seg = BACK ? segs - 1 - n : n;
+        auto s = S[n % 2];
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int row = row0 + 16 * t + 4 * g + r;
+                    s[row][16 * c + i] = x[t][c][r];
+                    starts[(int64_t(seg) * KD + row) * vd + col + 16 * c + i] = x[t][c][r];
+                    nan = __builtin_fmaf(x[t][c][r], 0.f, nan);
+                }
+        if (n + 1 == segs) break;
+        f32x4 m[NT][KD / 16];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+#pragma unroll
+            for (int c = 0; c < NC; ++c) x[t][c] = add[t][c];
+#pragma unroll
+            for (int k = 0; k < KD / 16; ++k) m[t][k] = ma[t][k];
+        }
+        if (n + 2 < segs) load(BACK ? seg - 1 : seg + 1);
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < KD / 16; ++k)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    const float b = s[16 * k + 4 * g + r][16 * c + i];
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) x[t][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(m[t][k][r], b, x[t][c], 0, 0, 0);
+                }
+    }
+    if (!BACK && !(nan == 0.f)) a.flags[bh] = 1;
 }
 
 // ---- dQ, dK, dbeta and the decays' gradient ------------------------------------------------------
@@ -1309,21 +1589,26 @@ static int prep_t(const Args &a, hipStream_t s) {
     static std::atomic<uint64_t> done{0};
     return launch_kernel(dr_prep<T, KD, REV, VEC>, bytes, done, std::min<int64_t>(a.batch * a.heads * a.chunks, kMostGroups), kThreads, a, s, "dr_prep");
 }
-template <typename T, int KD, bool STATES, bool VEC>
+template <typename T, int KD, Leaves L, bool VEC>
 static int walk_t(const Args &a, hipStream_t s) {
     constexpr int C = Cfg<T>::C, PI = Cfg<T>::in;
-    constexpr int bytes = 2 * ((STATES ? 1 : 2) * PI * kTile<C, KD> + PI * kTile<C, 64> + (STATES ? 1 : 2) * kImage<C>) + 2 * int(sizeof(Steps<C>));
+    constexpr int bytes = 2 * ((L == kOutputs ? 2 : 1) * PI * kTile<C, KD> + PI * kTile<C, 64>) + kRecord<C, L == kOutputs ? 2 : 1>;
     static_assert(bytes <= 80 * 1024, "two workgroups on a CU");
     static std::atomic<uint64_t> done{0};
-    return launch_kernel(dr_walk<T, KD, STATES, VEC>, bytes, done, unit_grid(a), kThreads, a, s, "dr_walk");
+    return launch_kernel(dr_walk<T, KD, L, VEC>, bytes, done, unit_grid(a, L == kMaps ? a.slices + KD / 64 : a.slices), kThreads, a, s, "dr_walk");
 }
-template <typename T, int KD, bool VEC>
+template <typename T, int KD, bool MAPS, bool VEC>
 static int back_t(const Args &a, hipStream_t s) {
     constexpr int C = Cfg<T>::C, PI = Cfg<T>::in;
-    constexpr int bytes = 2 * (2 * PI * kTile<C, KD> + PI * kTile<C, 64> + 2 * kImage<C>) + 2 * int(sizeof(Steps<C>)) + 4 * kWaves * C;
+    constexpr int bytes = 2 * (2 * PI * kTile<C, KD> + PI * kTile<C, 64>) + kRecord<C, 2> + 4 * kWaves * C;
     static_assert(bytes <= 160 * 1024, "LDS");
     static std::atomic<uint64_t> done{0};
-    return launch_kernel(dr_back<T, KD, VEC>, bytes, done, unit_grid(a), kThreads, a, s, "dr_back");
+    return launch_kernel(dr_back<T, KD, MAPS, VEC>, bytes, done, unit_grid(a, a.slices), kThreads, a, s, "dr_back");
+}
+template <int KD, bool BACK>
+static int join_t(const Args &a, hipStream_t s) {
+    hipLaunchKernelGGL((dr_join<KD, BACK>), dim3(unsigned(a.batch * a.heads * a.slices * 2)), dim3(kThreads), 0, s, a);
+    return launch_status("dr_join");
 }
 template <typename T, int KD, bool VEC, bool F32>
 static int grad_t(const Args &a, hipStream_t s) {
@@ -1350,22 +1635,30 @@ int launch_prep(const Args &a, bool rev, hipStream_t s) {
 }
 template <typename T>
 int launch_walk(const Args &a, bool states, hipStream_t s) {
-    const bool vec = a.k.vec && a.v.vec && (states || (a.q.vec && a.out_vec));
-    auto go = [&](auto kd, auto st) {
+    const bool maps = a.k.vec && a.v.vec, vec = maps && (states || (a.q.vec && a.out_vec));
+    auto go = [&](auto kd) {
         constexpr int KD = decltype(kd)::value;
-        constexpr bool ST = decltype(st)::value;
-        return vec ? walk_t<T, KD, ST, true>(a, s) : walk_t<T, KD, ST, false>(a, s);
+        if (a.segs > 1 && !a.kept_starts) {
+            if (const int rc = maps ? walk_t<T, KD, kMaps, true>(a, s) : walk_t<T, KD, kMaps, false>(a, s)) return rc;
+            if (const int rc = join_t<KD, false>(a, s)) return rc;
+        }
+        if (states) return vec ? walk_t<T, KD, kStates, true>(a, s) : walk_t<T, KD, kStates, false>(a, s);
+        return vec ? walk_t<T, KD, kOutputs, true>(a, s) : walk_t<T, KD, kOutputs, false>(a, s);
     };
-    typedef std::integral_constant<int, 64> K64;
-    typedef std::integral_constant<int, 128> K128;
-    if (states) return a.dk <= 64 ? go(K64{}, std::true_type{}) : go(K128{}, std::true_type{});
-    return a.dk <= 64 ? go(K64{}, std::false_type{}) : go(K128{}, std::false_type{});
+    return a.dk <= 64 ? go(std::integral_constant<int, 64>{}) : go(std::integral_constant<int, 128>{});
 }
 template <typename T>
 int launch_back(const Args &a, hipStream_t s) {
-    const bool vec = a.q.vec && a.k.vec && a.dout.vec && a.out_vec;
-    if (a.dk <= 64) return vec ? back_t<T, 64, true>(a, s) : back_t<T, 64, false>(a, s);
-    return vec ? back_t<T, 128, true>(a, s) : back_t<T, 128, false>(a, s);
+    const bool maps = a.q.vec && a.k.vec && a.dout.vec, vec = maps && a.out_vec;
+    auto go = [&](auto kd) {
+        constexpr int KD = decltype(kd)::value;
+        if (a.segs > 1) {
+            if (const int rc = maps ? back_t<T, KD, true, true>(a, s) : back_t<T, KD, true, false>(a, s)) return rc;
+            if (const int rc = join_t<KD, true>(a, s)) return rc;
+        }
+        return vec ? back_t<T, KD, false, true>(a, s) : back_t<T, KD, false, false>(a, s);
+    };
+    return a.dk <= 64 ? go(std::integral_constant<int, 64>{}) : go(std::integral_constant<int, 128>{});
 }
 template <typename T>
 int launch_grad(const Args &a, hipStream_t s) {

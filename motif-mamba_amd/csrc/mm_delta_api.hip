@@ -2,6 +2,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cstdlib>
 #include <initializer_list>
 
 #include "mm_common.h"
@@ -223,15 +224,98 @@ static Args common(const P &p) {
     return a;
 }
 
-static int64_t fwd_bytes(const mm_delta_fwd_params &p) {
-    const int C = chunk_tokens(p.itype);
-    return p.batch * p.nheads * ((p.seqlen + C - 1) / C) * 2 * image_bytes(C);
+// Segments of a row.
+struct Cut {
+    int segs;
+    int64_t len;   // tokens
+};
+// By the time that the passes over a row of n segments take, in chunks of one workgroup of dr_walk alone on its CU (two on a CU take
+// 1.85 of that for both): the first walk over all segments but the last (0.85 of a chunk; slices of V's columns and of the map's), the
+// join, and the walk itself. A training step (`train`) runs the backward's walks on the same segments: states (0.9) and R (1.6), R once
+// more before that (1.3), and another join.
+static Cut segments(int64_t pairs, int64_t seqlen, int64_t dk, int64_t dv, mm_dtype t, bool train) {
+    const int C = chunk_tokens(t);
+    const int64_t chunks = (seqlen + C - 1) / C, cus = device_simds() / 4, vs = pad64(dv) / 64, ks = pad64(dk) / 64;
+    auto cut = [&](int64_t n) {
+        const int64_t per = (chunks + n - 1) / n;
+        return Cut{int((chunks + per - 1) / per), per * C};
+    };
+    if (const char *e = std::getenv("MM_DELTA_SEGMENTS")) return cut(std::min<int64_t>(std::max<int64_t>(std::atoll(e), 1), chunks));
+    const double us = (ks == 2 ? 4.8 : 3.6), join = (ks == 2 ? 3.0 : 1.2) / us, launch = 6.0 / us;
+    auto rounds = [&](int64_t groups) {
+        const int64_t full = groups / (2 * cus), rest = groups % (2 * cus);
+        return 1.85 * double(full) + (rest == 0 ? 0.0 : rest <= cus ? 1.0 : 1.85);
+    };
+    Cut best = cut(1);
+    double least = 0.0;
+    for (int64_t n = 1; n <= std::min<int64_t>(chunks / 2 + 1, 64); ++n) {
+        const Cut c = cut(n);
+        if (c.segs != n) continue;
+        const double m = double(c.len / C), walk = rounds(pairs * n * vs);
+        double cost = m * walk * (train ? 1.0 + 0.9 + 1.6 : 1.0);
+        if (n > 1) {
+            cost += m * 0.85 * rounds(pairs * (n - 1) * vs + pairs * (train ? n : n - 1) * ks) + double(n) * join + 2.0 * launch;
+            if (train) cost += m * 1.3 * rounds(pairs * (n - 1) * vs) + double(n) * join + 2.0 * launch;
+        }
+        if (n == 1 || cost < least) {
+            least = cost;
+            best = c;
+        }
+    }
+    return best;
 }
+
+// Bytes taken from a workspace, one piece after the other.
+struct Take {
+    int64_t at = 0;
+    int64_t operator()(int64_t bytes) {
+        const int64_t o = at;
+        at += pad16(bytes);
+        return o;
+    }
+};
+
+// What a training step's forward leaves of its segments for the backward: maps, starts.
+struct Kept {
+    Cut cut;
+    int64_t maps, starts, flags, bytes;   // byte offsets
+};
+template <typename P>
+static Kept plan_kept(const P &p, bool train) {
+    Kept w = {};
+    const int64_t bh = p.batch * p.nheads, kd = pad64(p.dk), vd = pad64(p.dv);
+    w.cut = segments(bh, p.seqlen, p.dk, p.dv, p.itype, train);
+    if (w.cut.segs == 1) return w;
+    Take take;
+    w.maps = take(bh * w.cut.segs * kd * (vd + kd) * 4);
+    w.starts = take(bh * w.cut.segs * kd * vd * 4);
+    w.flags = take(bh * 4);
+    w.bytes = take.at;
+    return w;
+}
+static void set_kept(Args &a, const Kept &w, void *place) {
+    char *at = static_cast<char *>(place);
+    a.segs = w.cut.segs;
+    a.seg_len = w.cut.len;
+    a.maps = reinterpret_cast<float *>(at + w.maps);
+    a.starts = reinterpret_cast<float *>(at + w.starts);
+    a.flags = reinterpret_cast<int *>(at + w.flags);
+}
+
+static int64_t records(const mm_delta_fwd_params &p) {
+    const int C = chunk_tokens(p.itype);
+    return p.batch * p.nheads * ((p.seqlen + C - 1) / C) * record_bytes(C, 2);
+}
+static int64_t fwd_bytes(const mm_delta_fwd_params &p) { return records(p) + (p.segment_states ? 0 : plan_kept(p, false).bytes); }
 
 template <typename T>
 static int run_fwd(const mm_delta_fwd_params &p, hipStream_t s) {
     Args a = common(p);
-    a.img_a = static_cast<char *>(p.workspace);
+    a.rec_a = static_cast<char *>(p.workspace);
+    a.rec_a_step = int(record_bytes(chunk_tokens(p.itype), 2));
+    if (p.segment_states) set_kept(a, plan_kept(p, true), p.segment_states);
+    else set_kept(a, plan_kept(p, false), static_cast<char *>(p.workspace) + records(p));
+    a.last_map = p.segment_states != nullptr;
     a.s1 = p.last_state;
     a.out = p.out;
     a.out_vec = view(p.out, p.itype, p.out_batch_stride, p.out_seq_stride, p.out_head_stride, 1, p.dv).vec;
@@ -242,21 +326,18 @@ static int run_fwd(const mm_delta_fwd_params &p, hipStream_t s) {
 
 // The backward's workspace, in order.
 struct BwdPlan {
-    int64_t img_a, img_b, states, z, r, dx, pbeta, dq, dk, dg, bytes;   // byte offsets
+    Kept kept;
+    int64_t rec_a, rec_b, states, z, r, dx, pbeta, dq, dk, dg, segs, back_maps, back_starts, bytes;   // byte offsets
 };
 
 static BwdPlan plan_bwd(const mm_delta_bwd_params &p) {
     BwdPlan w = {};
     const int C = chunk_tokens(p.itype);
     const int64_t bh = p.batch * p.nheads, chunks = (p.seqlen + C - 1) / C, kd = pad64(p.dk), vd = pad64(p.dv);
-    int64_t at = 0;
-    auto take = [&](int64_t bytes) {
-        const int64_t o = at;
-        at += pad16(bytes);
-        return o;
-    };
-    w.img_a = take(bh * chunks * image_bytes(C));
-    w.img_b = take(bh * chunks * 2 * image_bytes(C));
+    w.kept = plan_kept(p, true);
+    Take take;
+    w.rec_a = take(bh * chunks * record_bytes(C, 1));
+    w.rec_b = take(bh * chunks * record_bytes(C, 2));
     w.states = take(bh * chunks * kd * vd * 4);
     w.z = take(bh * chunks * C * vd * 4);
     w.r = take(bh * chunks * kd * vd * 4);
@@ -267,7 +348,12 @@ static BwdPlan plan_bwd(const mm_delta_bwd_params &p) {
         w.dk = take(bh * p.seqlen * p.dk * 4);
     }
     if (p.dlog_decay && p.decay_per_head) w.dg = take(bh * p.seqlen * 4);
-    w.bytes = at;
+    if (w.kept.cut.segs > 1) {
+        w.back_maps = take(bh * w.kept.cut.segs * kd * vd * 4);
+        w.back_starts = take(bh * w.kept.cut.segs * kd * vd * 4);
+        if (!p.segment_states) w.segs = take(w.kept.bytes);
+    }
+    w.bytes = take.at;
     return w;
 }
 
@@ -280,8 +366,13 @@ static int run_bwd(const mm_delta_bwd_params &p, hipStream_t s) {
     const bool shared = share > 1;
     Args a = common(p);
     a.dout = view(p.dout, p.itype, p.do_batch_stride, p.do_seq_stride, p.do_head_stride, 1, p.dv);
-    a.img_a = ws + w.img_a;
-    a.img_b = ws + w.img_b;
+    a.rec_a = ws + w.rec_a;
+    a.rec_a_step = int(record_bytes(chunk_tokens(p.itype), 1));
+    a.rec_b = ws + w.rec_b;
+    set_kept(a, w.kept, p.segment_states ? const_cast<void *>(p.segment_states) : ws + w.segs);
+    a.kept_starts = p.segment_states != nullptr;
+    a.last_map = 1;
+    a.back_maps = f32(w.back_maps); a.back_starts = f32(w.back_starts);
     a.states = f32(w.states); a.z = f32(w.z); a.r = f32(w.r); a.dx = f32(w.dx); a.pbeta = f32(w.pbeta);
     a.dlast = p.dlast_state;
     a.ds0 = p.dinitial_state;
@@ -318,6 +409,11 @@ using namespace mm;
 extern "C" int64_t mm_delta_fwd_workspace_size(const mm_delta_fwd_params *p) {
     if (!p || p->batch <= 0 || p->seqlen <= 0 || p->nheads <= 0) return 0;
     return dr::fwd_bytes(*p);
+}
+
+extern "C" int64_t mm_delta_segment_states_size(const mm_delta_fwd_params *p) {
+    if (!p || p->batch <= 0 || p->seqlen <= 0 || p->nheads <= 0) return 0;
+    return dr::plan_kept(*p, true).bytes;
 }
 
 extern "C" int64_t mm_delta_bwd_workspace_size(const mm_delta_bwd_params *p) {

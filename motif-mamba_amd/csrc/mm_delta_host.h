@@ -24,6 +24,9 @@ inline int chunk_tokens(mm_dtype t) { return t == MM_BFLOAT16 ? 64 : 32; }
 inline int chunk_frags(int tokens) { return tokens == 64 ? 6 : 2; }
 // Bytes of a chunk's triangle as operands: three planes of 64 x 16 bytes each.
 inline int64_t image_bytes(int tokens) { return int64_t(chunk_frags(tokens)) * 3 * 1024; }
+// Of its decays and beta; of its record: images, then those.
+constexpr int64_t steps_bytes(int tokens) { return (6 * tokens + 1) * 4 + 12; }
+inline int64_t record_bytes(int tokens, int images) { return images * image_bytes(tokens) + steps_bytes(tokens); }
 
 // The argument block of every kernel; each reads what it needs.
 struct Args {
@@ -32,7 +35,16 @@ struct Args {
     int64_t batch, seqlen, heads, chunks;
     int dk, dv, slices;            // slices: workgroups over dv
     float scale;
-    char *img_a, *img_b;           // [bh][chunk] operand images of P and M (dr_prep), or of their transposes
+    char *rec_a, *rec_b;           // [bh][chunk] records (dr_prep): images of P and M, or, for the backward, of P in rec_a and of the
+                                   // transposes of both in rec_b
+    int rec_a_step;                // bytes of a record of rec_a
+    int segs;                      // segments of a row, seg_len tokens each (a multiple of the chunk)
+    int64_t seg_len;
+    float *maps, *starts;          // [bh][seg][KD][VD + KD], [bh][seg][KD][VD]
+    float *back_maps, *back_starts;   // the backward's: [bh][seg][KD][VD] both
+    int last_map;                  // the last segment's map too (the backward's)
+    int kept_starts;               // maps and starts are there already
+    int *flags;                    // [bh]: a row's states are not finite
     const float *s0;               // state before the first token, or NULL
     float *s1;                     // state after the last one, or NULL
     float *states, *z;             // the backward's: [bh][chunk][KD][VD], [bh][chunk * C][VD]

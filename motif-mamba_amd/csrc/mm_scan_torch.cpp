@@ -1054,7 +1054,7 @@ void delta_common(P &p, const at::Tensor &q, const at::Tensor &k, const at::Tens
 }
 
 std::vector<at::Tensor> delta_fwd(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &b, const c10::optional<at::Tensor> &g,
-                                  double scale, const c10::optional<at::Tensor> &initial_, bool return_last_state) {
+                                  double scale, const c10::optional<at::Tensor> &initial_, bool return_last_state, bool keep_states) {
     mm_delta_fwd_params p;
     delta_common(p, q, k, v, b, g, scale);
     at::Tensor initial;
@@ -1070,12 +1070,14 @@ std::vector<at::Tensor> delta_fwd(const at::Tensor &q, const at::Tensor &k, cons
     p.out = out.data_ptr();
     p.last_state = last.defined() ? last.data_ptr<float>() : nullptr;
     p.out_batch_stride = out.stride(0); p.out_seq_stride = seq_stride(out); p.out_head_stride = out.stride(2);
-    at::Tensor ws;
+    at::Tensor ws, kept;
+    if (keep_states) p.segment_states = workspace_of(kept, mm_delta_segment_states_size(&p), v);
     p.workspace_bytes = mm_delta_fwd_workspace_size(&p);
     p.workspace = workspace_of(ws, p.workspace_bytes, v);
     check_rc(mm_delta_fwd(&p, c10::hip::getCurrentHIPStream().stream()), "mm_delta_fwd");
     std::vector<at::Tensor> res{out};
     if (return_last_state) res.push_back(last);
+    if (keep_states) res.push_back(kept);   // undefined where a row is one segment
     return res;
 }
 
@@ -1083,8 +1085,8 @@ std::vector<at::Tensor> delta_fwd(const at::Tensor &q, const at::Tensor &k, cons
 // decay_per_head.
 std::vector<c10::optional<at::Tensor>> delta_bwd(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &b,
                                                  const c10::optional<at::Tensor> &g, double scale, const c10::optional<at::Tensor> &initial_,
-                                                 const at::Tensor &dout, const c10::optional<at::Tensor> &dlast_, bool decay_per_head,
-                                                 bool want_decay, bool want_initial) {
+                                                 const at::Tensor &dout, const c10::optional<at::Tensor> &dlast_, const c10::optional<at::Tensor> &states_,
+                                                 bool decay_per_head, bool want_decay, bool want_initial) {
     mm_delta_bwd_params p;
     delta_common(p, q, k, v, b, g, scale);
     TORCH_CHECK(dout.is_cuda() && dout.sizes() == v.sizes() && dout.scalar_type() == v.scalar_type(), "dout must have the shape and dtype of v");
@@ -1111,6 +1113,7 @@ std::vector<c10::optional<at::Tensor>> delta_bwd(const at::Tensor &q, const at::
     p.dlog_decay = dg.defined() ? dg.data_ptr() : nullptr;
     p.dinitial_state = ds.defined() ? ds.data_ptr<float>() : nullptr;
     p.decay_per_head = decay_per_head;
+    p.segment_states = states_.has_value() && states_.value().defined() ? states_.value().data_ptr() : nullptr;
     p.do_batch_stride = dout.stride(0); p.do_seq_stride = seq_stride(dout); p.do_head_stride = dout.stride(2);
     at::Tensor ws;
     p.workspace_bytes = mm_delta_bwd_workspace_size(&p);
@@ -1328,12 +1331,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("group_norm_bwd", &group_norm_bwd, "Gated group norm backward [dx, dweight?, dbias?, dz?]", pybind11::arg("x"),
           pybind11::arg("n_groups"), pybind11::arg("weight"), pybind11::arg("bias"), pybind11::arg("z"), pybind11::arg("eps"),
           pybind11::arg("is_rms"), pybind11::arg("gate"), pybind11::arg("dout"), pybind11::arg("want_weights"));
-    m.def("delta_fwd", &delta_fwd, "Gated delta rule forward [out, last_state?]", pybind11::arg("q"), pybind11::arg("k"), pybind11::arg("v"),
-          pybind11::arg("beta"), pybind11::arg("log_decay"), pybind11::arg("scale"), pybind11::arg("initial_state"), pybind11::arg("return_last_state"));
+    m.def("delta_fwd", &delta_fwd, "Gated delta rule forward [out, last_state?, states of the segments?]", pybind11::arg("q"), pybind11::arg("k"), pybind11::arg("v"),
+          pybind11::arg("beta"), pybind11::arg("log_decay"), pybind11::arg("scale"), pybind11::arg("initial_state"), pybind11::arg("return_last_state"),
+          pybind11::arg("keep_states"));
     m.def("delta_bwd", &delta_bwd, "Gated delta rule backward [dq, dk, dv, dbeta, dlog_decay?, dinitial_state?]", pybind11::arg("q"),
           pybind11::arg("k"), pybind11::arg("v"), pybind11::arg("beta"), pybind11::arg("log_decay"), pybind11::arg("scale"),
-          pybind11::arg("initial_state"), pybind11::arg("dout"), pybind11::arg("dlast_state"), pybind11::arg("decay_per_head"),
-          pybind11::arg("want_decay"), pybind11::arg("want_initial"));
+          pybind11::arg("initial_state"), pybind11::arg("dout"), pybind11::arg("dlast_state"), pybind11::arg("states"),
+          pybind11::arg("decay_per_head"), pybind11::arg("want_decay"), pybind11::arg("want_initial"));
     m.def("delta_update", &delta_update, "Gated delta rule, one token (in place on state)", pybind11::arg("state"), pybind11::arg("q"),
           pybind11::arg("k"), pybind11::arg("v"), pybind11::arg("beta"), pybind11::arg("log_decay"), pybind11::arg("scale"));
     m.def("layer_norm_fwd", &layer_norm_fwd, "Residual add and layer norm forward [out, residual_out?]", pybind11::arg("x"),

@@ -33,34 +33,36 @@ def _decays(log_decay, lead, v):
     return (None, False) if log_decay is None else _spread(log_decay, lead, v)
 
 
-def _forward(q, k, v, beta, log_decay, scale, initial_state, return_last_state):
+def _forward(q, k, v, beta, log_decay, scale, initial_state, return_last_state, keep_states=False):
     q, k, v = _rows(q), _rows(k), _rows(v)
     g, per_head = _decays(log_decay, v.shape[:2], v)
-    res = ext().delta_fwd(q, k, v, beta, g, scale, initial_state, return_last_state)
-    return q, k, v, per_head, tuple(res) if return_last_state else res[0]
+    res = ext().delta_fwd(q, k, v, beta, g, scale, initial_state, return_last_state, keep_states)
+    states = res.pop() if keep_states else None
+    return q, k, v, per_head, states, tuple(res) if return_last_state else res[0]
 
 
 class DeltaRuleFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, beta, log_decay, scale, initial_state, return_last_state):
-        q, k, v, ctx.per_head, out = _forward(q, k, v, beta, log_decay, scale, initial_state, return_last_state)
+        # Long rows of few heads run in segments; the states those start from, and what each makes of a state, serve the backward too.
+        q, k, v, ctx.per_head, states, out = _forward(q, k, v, beta, log_decay, scale, initial_state, return_last_state, True)
         ctx.scale = scale
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(q, k, v, beta, log_decay, initial_state)
+        ctx.save_for_backward(q, k, v, beta, log_decay, initial_state, states)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout, dlast=None):
-        q, k, v, beta, log_decay, initial_state = ctx.saved_tensors
+        q, k, v, beta, log_decay, initial_state, states = ctx.saved_tensors
         if dout is None:
             if dlast is None:
                 return (None,) * 8
             dout = torch.zeros_like(v, memory_format=torch.contiguous_format)
         g, _ = _decays(log_decay, v.shape[:2], v)
         want = ctx.needs_input_grad
-        dq, dk, dv, db, dg, ds = ext().delta_bwd(q, k, v, beta, g, ctx.scale, initial_state, _rows(dout), dlast, ctx.per_head, want[4],
+        dq, dk, dv, db, dg, ds = ext().delta_bwd(q, k, v, beta, g, ctx.scale, initial_state, _rows(dout), dlast, states, ctx.per_head, want[4],
                                                  want[6] and initial_state is not None)
         return dq, dk, dv, db, dg, None, ds, None
 
@@ -75,7 +77,7 @@ def delta_rule_fn(q, k, v, beta, log_decay=None, scale=None, initial_state=None,
     args = (q, k, v, beta, log_decay, _scale(scale, q), initial_state, return_last_state)
     if differentiated(q, k, v, beta, log_decay, initial_state):
         return DeltaRuleFn.apply(*args)
-    return _forward(*args)[4]
+    return _forward(*args)[5]
 
 
 def delta_rule_update(state, q, k, v, beta, log_decay=None, scale=None):

@@ -12,7 +12,8 @@ from torch.autograd import forward_ad
 
 from tests import capi
 
-HEADERS = {"mm_delta.h": ["mm_delta_fwd", "mm_delta_fwd_workspace_size", "mm_delta_bwd", "mm_delta_bwd_workspace_size", "mm_delta_update"],
+HEADERS = {"mm_delta.h": ["mm_delta_fwd", "mm_delta_fwd_workspace_size", "mm_delta_bwd", "mm_delta_bwd_workspace_size", "mm_delta_update",
+                          "mm_delta_segment_states_size"],
            "mm_layer_norm.h": ["mm_layer_norm_fwd", "mm_layer_norm_bwd", "mm_layer_norm_bwd_workspace_size"]}
 INC = os.path.join(capi.REPO, "include")
 
@@ -174,8 +175,9 @@ def test_python_refusals_without_a_gpu():
 class _Ext:
     """Outputs of the right shapes."""
 
-    def delta_fwd(self, q, k, v, beta, g, scale, initial, last):
-        return [torch.zeros_like(v), *([torch.zeros(v.shape[0], v.shape[2], q.shape[3], v.shape[3])] if last else [])]
+    def delta_fwd(self, q, k, v, beta, g, scale, initial, last, keep):
+        return [torch.zeros_like(v), *([torch.zeros(v.shape[0], v.shape[2], q.shape[3], v.shape[3])] if last else []),
+                *([None] if keep else [])]
 
     def layer_norm_fwd(self, x, residual, weight, bias, eps, rms, want, wide):
         return [torch.zeros_like(x), torch.zeros_like(x) if want else None]
