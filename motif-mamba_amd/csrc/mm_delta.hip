@@ -1340,53 +1340,88 @@ __global__ void __launch_bounds__(KD * 4) __attribute__((amdgpu_waves_per_eu(2, 
         i = lane & 15;
     };
     const int64_t total = [&] { const Args a = args(); return a.batch * a.heads * a.chunks; }();
-    for (int64_t id = blockIdx.x; id < total; id += gridDim.x) {
-        int chunk;
+    struct Where {
         Spot p;
+        int64_t at;
+        int t0, rows;
+    };
+    auto where = [&](int64_t id) {
+        const Args a = args();
+        const int64_t bc = id / a.heads;
+        const int chunk = int(bc % a.chunks);
+        Where w;
+        w.p = spot_of(a, unsigned(bc / a.chunks * a.heads + id % a.heads));
+        w.at = afresh(w.p.bh * a.chunks + chunk);
+        w.t0 = afresh(chunk * C);
+        w.rows = afresh(min(C, int(a.seqlen) - w.t0));
+        return w;
+    };
+    const int vd = afresh(64 * args().slices);
+    SX sk, sq;
+    SV sd;
+    StageF32<C, NT> su, sx;
+    float4 sr[2][2][2];   // [k][S, R][half of 8]
+    uint32_t gbits = 0, bbits = 0;
+    auto load = [&](const Where &w, int h0) {
         {
             const Args a = args();
-            const int64_t bc = id / a.heads;
-            chunk = afresh(int(bc % a.chunks));
-            p = spot_of(a, unsigned(bc / a.chunks * a.heads + id % a.heads));
+            sd.load(rows_of<T>(a.dout, w.p.b, w.p.h, a.dv, h0), w.t0, w.rows, tid);
         }
-        const int t0 = chunk * C, rows = min(C, afresh(int(args().seqlen)) - t0), vd = afresh(64 * args().slices);
-        const int64_t at = afresh(p.bh * args().chunks + chunk);
-        SV sd;
-        StageF32<C, NT> su, sx;
-        float4 sr[2][2][2];   // [k][S, R][half of 8]
-        auto load = [&](int h0) {
-            const Args a = args();
-            sd.load(rows_of<T>(a.dout, p.b, p.h, a.dv, h0), t0, rows, tid);
-            su.load(a.z + at * C * vd + h0, vd, tid);
-            sx.load(a.dx + at * C * vd + h0, vd, tid);
-        };
-        auto load_states = [&](int h0) {
-            const Args a = args();
-            const float *S = a.states + at * KD * vd + h0, *R = a.r + at * KD * vd + h0;
+        const Args a = args();
+        su.load(a.z + w.at * C * vd + h0, vd, tid);
+        sx.load(a.dx + w.at * C * vd + h0, vd, tid);
+    };
+    auto load_states = [&](const Where &w, int h0) {
+        const Args a = args();
+        const float *S = a.states + w.at * KD * vd + h0, *R = a.r + w.at * KD * vd + h0;
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const int o = (col + i) * vd + 32 * k + 4 * g;
-                sr[k][0][0] = *reinterpret_cast<const float4 *>(S + o);
-                sr[k][0][1] = *reinterpret_cast<const float4 *>(S + o + 16);
-                sr[k][1][0] = *reinterpret_cast<const float4 *>(R + o);
-                sr[k][1][1] = *reinterpret_cast<const float4 *>(R + o + 16);
-            }
-        };
-        __syncthreads();
+        for (int k = 0; k < 2; ++k) {
+            const int o = (col + i) * vd + 32 * k + 4 * g;
+            sr[k][0][0] = *reinterpret_cast<const float4 *>(S + o);
+            sr[k][0][1] = *reinterpret_cast<const float4 *>(S + o + 16);
+            sr[k][1][0] = *reinterpret_cast<const float4 *>(R + o);
+            sr[k][1][1] = *reinterpret_cast<const float4 *>(R + o + 16);
+        }
+    };
+    auto load_first = [&](const Where &w) {
+        if (wave == NW - 1) {
+            const Args a = args();
+            gbits = load_gate<C>(gates_of(a.g, w.p), w.t0, w.t0 + w.rows, lane);
+            bbits = load_gate<C>(gates_of(a.beta, w.p), w.t0, w.t0 + w.rows, lane);
+        }
         {
             const Args a = args();
-            const Gates gg = gates_of(a.g, p), gb = gates_of(a.beta, p);
-            const int end = int(a.seqlen);
-            SX sk, sq;
-            sk.load(rows_of<T>(a.k, p.b, p.h, a.dk), t0, rows, tid);
-            sq.load(rows_of<T>(a.q, p.b, p.h, a.dk), t0, rows, tid);
-            load(0);
-            load_states(0);
-            if (wave == NW - 1)
-                make_chunk<C>(*ck, load_gate<C>(gg, t0, end, lane), a.g.type, load_gate<C>(gb, t0, end, lane), a.beta.type, a.scale, lane);
-            sk.store(K, tid);
-            sq.store(Q, tid);
+            sk.load(rows_of<T>(a.k, w.p.b, w.p.h, a.dk), w.t0, w.rows, tid);
         }
+        {
+            const Args a = args();
+            sq.load(rows_of<T>(a.q, w.p.b, w.p.h, a.dk), w.t0, w.rows, tid);
+        }
+        load(w, 0);
+        load_states(w, 0);
+    };
+    // At dk 128 a group takes several chunks, the next one's first loads on their way while it ends one (465 us where a group for each
+    // took 508, 64 pairs, L 4,096, dv 128). At 64 two groups are on a CU, which do the same for each other and have no registers for it
+    // (312 and 363 us, 192 pairs, L 2,048, dv 64).
+    constexpr bool kAhead = KD == 128;
+    Where next = where(blockIdx.x);
+    if constexpr (kAhead) load_first(next);
+    for (int64_t id = blockIdx.x; id < total; id += gridDim.x) {
+        if constexpr (!kAhead) {
+            if (id != blockIdx.x) next = where(id);
+            load_first(next);
+        }
+        const Where w = next;
+        const Spot p = w.p;
+        const int t0 = w.t0, rows = w.rows;
+        __syncthreads();
+        fresh();
+        if (wave == NW - 1) {
+            const Args a = args();
+            make_chunk<C>(*ck, gbits, a.g.type, bbits, a.beta.type, a.scale, lane);
+        }
+        sk.store(K, tid);
+        sq.store(Q, tid);
         f32x4 a1[6], a2[4], dq[CT][NC], dr[CT][NC], dc[CT][NC];
         float rdots = 0.f;
 #pragma unroll
@@ -1402,7 +1437,7 @@ __global__ void __launch_bounds__(KD * 4) __attribute__((amdgpu_waves_per_eu(2, 
             sd.store(D, tid);
             su.store(U, ck->beta, tid);
             sx.store(X, nullptr, tid);
-            if (h0 + 64 < vd) load(h0 + 64);
+            if (h0 + 64 < vd) load(w, h0 + 64);
             __syncthreads();
             fresh();
             each_tile_of_two<C, NW>(wave, [&](auto L1, auto L2) {
@@ -1428,12 +1463,18 @@ __global__ void __launch_bounds__(KD * 4) __attribute__((amdgpu_waves_per_eu(2, 
                 split8(y[0], f[k][0]);
                 split8(y[1], f[k][1]);
             }
-            if (h0 + 64 < vd) load_states(h0 + 64);
+            if (h0 + 64 < vd) load_states(w, h0 + 64);
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 row_products<C, 64, PI>(&dq[0][0], NC, D, k, f[k][0], lane);
                 row_products<C, 64, kPlanes>(&dr[0][0], NC, X, k, f[k][0], lane);
                 row_products<C, 64, kPlanes>(&dc[0][0], NC, U, k, f[k][1], lane);
+            }
+        }
+        if constexpr (kAhead) {
+            if (id + gridDim.x < total) {
+                next = where(id + gridDim.x);
+                load_first(next);
             }
         }
         // The state terms' row factors.
@@ -1549,28 +1590,31 @@ __global__ void __launch_bounds__(KD * 4) __attribute__((amdgpu_waves_per_eu(2, 
             const Args a = args();
             const bool forgets = lane < rows && decode_g(load_gate<C>(gates_of(a.g, p), t0, t0 + rows, lane), a.g.type) == -128.f;
             const uint64_t all = __ballot(forgets);
+            float e = 0.f, f = 0.f;
             if (lane < C) {
-                float e = 0.f, f = 0.f;
 #pragma unroll
                 for (int w = 0; w < NW; ++w) {
-                    e += row[w * C + lane] - (cols[w * C + lane] - fs[w * C + lane]);
-                    f += fs[w * C + lane];
+                    const float left = fs[w * C + lane];
+                    e += row[w * C + lane] - (cols[w * C + lane] - left);
+                    f += left;
                 }
-                row[lane] = e;
-                fs[lane] = f;
             }
-            wave_fence();
+            // e from here to the chunk's end or the next forgotten state, f of the tokens before.
+            const uint64_t behind = all >> lane >> 1;
+            const int last = min(rows, lane + 1 + (behind ? __builtin_ctzll(behind) : 64));
+            float before = f;
+#pragma unroll
+            for (int d = 1; d < C; d *= 2) {
+                const float x = __shfl_down(e, d), y = __shfl_up(before, d);
+                if (lane + d < last) e += x;
+                if (lane >= d) before += y;
+            }
+            before = __shfl_up(before, 1);
             if (lane < rows) {
                 float s = 0.f;
 #pragma unroll
                 for (int w = 0; w < NW; ++w) s += rs[w];
-                s *= ck->d.all;
-                for (int n = 0; n < lane; ++n) s += fs[n];
-                const uint64_t behind = all >> lane >> 1;
-                const int last = min(rows, lane + 1 + (behind ? __builtin_ctzll(behind) : 64));
-                float sum = 0.f;
-                for (int n = last - 1; n >= lane; --n) sum += row[n];
-                s = forgets ? 0.f : s + sum;
+                s = forgets ? 0.f : ck->d.all * s + (lane ? before : 0.f) + e;
                 if (a.dg_sum) a.dg_sum[p.bh * a.seqlen + t0 + lane] = s;
                 else store_gate(a.dg, a.g.type, (p.b * a.seqlen + t0 + lane) * a.heads + p.h, s);
             }
@@ -1617,7 +1661,7 @@ static int grad_t(const Args &a, hipStream_t s) {
     constexpr int bytes = 2 * (2 * PI * kTile<C, KD> + PI * kTile<C, 64> + 2 * kPlanes * kTile<C, 64>) + int(sizeof(Chunk<C>)) + 4 * (3 * NW * C + NW);
     static_assert(bytes <= (KD == 64 ? 80 : 160) * 1024, "two workgroups on a CU at KD 64, one at 128");
     static std::atomic<uint64_t> done{0};
-    return launch_kernel(dr_grad<T, KD, VEC, F32>, bytes, done, std::min<int64_t>(a.batch * a.heads * a.chunks, kMostGroups), 64 * NW, a, s, "dr_grad");
+    return launch_kernel(dr_grad<T, KD, VEC, F32>, bytes, done, std::min<int64_t>(a.batch * a.heads * a.chunks, KD == 64 ? kMostGroups : device_simds() / 4), 64 * NW, a, s, "dr_grad");
 }
 
 template <typename T>
