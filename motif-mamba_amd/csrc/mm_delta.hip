@@ -295,7 +295,7 @@ __device__ __forceinline__ void write_image(char *dst, const float *f, int wave,
 
 // The records of every chunk: the images of P and M; REV, for the backward: that of P, and those of P^T and M^T. One workgroup per chunk. The triangles are made in float32: the diagonal tiles of P by substitution, row by row, those of a column
 // block below by 16 x 16 products on v_mfma_f32_16x16x4_f32, which keeps them float32.
-template <typename T, int KD> constexpr int kPrepGroups = sizeof(T) == 2 || KD == 64 ? 3 : 2;   // on a CU
+template <typename T, int KD> constexpr int kPrepGroups = Cfg<T>::C == 32 && KD == 64 ? 4 : sizeof(T) == 2 ? 3 : 2;   // on a CU, by registers
 template <typename T, int KD, bool REV, bool VEC>
 __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kPrepGroups<T, KD>, kPrepGroups<T, KD>))) dr_prep(const Args) {
     constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, CT = C / 16, LD = kPitch<C>;

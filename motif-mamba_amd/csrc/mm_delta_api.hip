@@ -42,13 +42,16 @@ __device__ __forceinline__ void row_sums(float (&x)[4], float4 (*part)[LPR]) {
 }
 
 // S' = exp(g) S, u = beta (v - S'^T k), S = S' + k u^T, o = scale S^T q. Bound by the state, read once and written once: a workgroup
-// holds one (batch row, head)'s state in registers between the two. LPR lanes cover a row's dv in 16-byte pieces, RPT rows each.
+// holds one (batch row, head)'s columns of it (4 LPR of them) in registers between the two. LPR lanes cover a row in 16-byte pieces, RPT
+// rows each. 256 x 40 heads of 128 x 128: 276 us, 1.34 GB at 4.9 TB/s (a large copy reaches 5.2); with twice the rows per lane and so half
+// the workgroups on a CU 304, with waves of 32 columns that meet no other 359.
 template <typename T, int LPR, int RPT>
-__global__ void __launch_bounds__(256) dr_update(const mm_delta_update_params p) {
-    constexpr int NT = 256, ROWS = NT / LPR;
+__global__ void __launch_bounds__(512) dr_update(const mm_delta_update_params p, int slices) {
+    constexpr int NT = LPR == 32 ? 512 : 256, ROWS = NT / LPR;
     __shared__ float4 part[2][NT / 64][LPR];
-    const int64_t bh = blockIdx.x, b = bh / p.nheads, h = bh % p.nheads, grp = h / (p.nheads / p.n_groups);
-    const int tid = threadIdx.x, x = 4 * (tid % LPR), row0 = tid / LPR;
+    __shared__ float kq[2][MM_DELTA_MAX_DIM];
+    const int64_t bh = blockIdx.x / unsigned(slices), b = bh / p.nheads, h = bh % p.nheads, grp = h / (p.nheads / p.n_groups);
+    const int tid = threadIdx.x, x = 4 * (tid % LPR + LPR * int(blockIdx.x % unsigned(slices))), row0 = tid / LPR;
     const int dk = int(p.dk), dv = int(p.dv);
     float *s = p.state + b * p.state_batch_stride + h * p.state_head_stride + x;
     const T *q = reinterpret_cast<const T *>(p.q) + b * p.q_batch_stride + grp * p.q_group_stride;
@@ -56,16 +59,16 @@ __global__ void __launch_bounds__(256) dr_update(const mm_delta_update_params p)
     const T *v = reinterpret_cast<const T *>(p.v) + b * p.v_batch_stride + h * p.v_head_stride + x;
     const int n = dv - x < 4 ? dv - x : 4;    // elements of this lane's piece
     const bool vec = n == 4 && (reinterpret_cast<uintptr_t>(p.state) | p.state_dk_stride * 4 | p.state_head_stride * 4 | p.state_batch_stride * 4) % 16 == 0;
-    float w[RPT][4], kk[RPT], qq[RPT];
+    // k and q first: their way through LDS does not wait for the state's rows then.
+    const int at = tid % MM_DELTA_MAX_DIM;
+    const float own = tid < 2 * MM_DELTA_MAX_DIM && at < dk ? to_f32((tid < MM_DELTA_MAX_DIM ? k : q)[at]) : 0.f;
+    float w[RPT][4];
 #pragma unroll
     for (int r = 0; r < RPT; ++r) {
         const int row = row0 + r * ROWS;
-        kk[r] = qq[r] = 0.f;
 #pragma unroll
         for (int e = 0; e < 4; ++e) w[r][e] = 0.f;
         if (row < dk) {
-            kk[r] = to_f32(k[row]);
-            qq[r] = to_f32(q[row]);
             const float *src = s + row * p.state_dk_stride;
             if (vec) {
                 const float4 y = *reinterpret_cast<const float4 *>(src);
@@ -83,13 +86,17 @@ __global__ void __launch_bounds__(256) dr_update(const mm_delta_update_params p)
     float g = p.log_decay ? read_gate(p.log_decay, p.gtype, b * p.g_batch_stride + h * p.g_head_stride) : 0.f;
     g = p.log_decay ? expf(g < -128.f ? -128.f : g) : 1.f;
     const float beta = read_gate(p.beta, p.btype, b * p.b_batch_stride + h * p.b_head_stride);
+    if (tid < 2 * MM_DELTA_MAX_DIM) kq[tid / MM_DELTA_MAX_DIM][at] = own;
+    __syncthreads();
 #pragma unroll
-    for (int r = 0; r < RPT; ++r)
+    for (int r = 0; r < RPT; ++r) {
+        const float kk = kq[0][row0 + r * ROWS];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             w[r][e] *= g;
-            z[e] = __builtin_fmaf(kk[r], w[r][e], z[e]);
+            z[e] = __builtin_fmaf(kk, w[r][e], z[e]);
         }
+    }
     row_sums<LPR, NT / 64>(z, part[0]);
 #pragma unroll
     for (int e = 0; e < 4; ++e) u[e] = beta * (u[e] - z[e]);
@@ -97,10 +104,11 @@ __global__ void __launch_bounds__(256) dr_update(const mm_delta_update_params p)
     for (int r = 0; r < RPT; ++r) {
         const int row = row0 + r * ROWS;
         if (row >= dk) continue;
+        const float kk = kq[0][row], qq = kq[1][row];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            w[r][e] = __builtin_fmaf(kk[r], u[e], w[r][e]);
-            o[e] = __builtin_fmaf(qq[r], w[r][e], o[e]);
+            w[r][e] = __builtin_fmaf(kk, u[e], w[r][e]);
+            o[e] = __builtin_fmaf(qq, w[r][e], o[e]);
         }
         float *dst = s + row * p.state_dk_stride;
         if (vec) {
@@ -122,15 +130,17 @@ __global__ void __launch_bounds__(256) dr_update(const mm_delta_update_params p)
 
 template <typename T>
 static int launch_update(const mm_delta_update_params &p, hipStream_t s) {
-    const dim3 grid(unsigned(p.batch * p.nheads));
     auto go = [&](auto lpr) {
-        constexpr int LPR = decltype(lpr)::value, RPT = LPR / 2;   // 128 rows
-        if (p.dk <= 64) hipLaunchKernelGGL((dr_update<T, LPR, RPT / 2>), grid, dim3(256), 0, s, p);
-        else hipLaunchKernelGGL((dr_update<T, LPR, RPT>), grid, dim3(256), 0, s, p);
+        constexpr int LPR = decltype(lpr)::value, NT = LPR == 32 ? 512 : 256, RPT = 128 * LPR / NT;
+        const int slices = int((p.dv + 4 * LPR - 1) / (4 * LPR));
+        const dim3 grid(unsigned(p.batch * p.nheads * slices));
+        if (p.dk <= 64) hipLaunchKernelGGL((dr_update<T, LPR, RPT / 2>), grid, dim3(NT), 0, s, p, slices);
+        else hipLaunchKernelGGL((dr_update<T, LPR, RPT>), grid, dim3(NT), 0, s, p, slices);
         return launch_status("dr_update");
     };
     if (p.dv <= 32) return go(std::integral_constant<int, 8>{});
-    if (p.dv <= 64) return go(std::integral_constant<int, 16>{});
+    // Whole rows, but halves of them where the pairs leave CUs without work (40 pairs of 128 x 128: 6.5 us, 7.4 whole).
+    if (p.dv <= 64 || p.batch * p.nheads * 2 <= device_simds() / 4) return go(std::integral_constant<int, 16>{});
     return go(std::integral_constant<int, 32>{});
 }
 
