@@ -32,33 +32,37 @@ __device__ __forceinline__ void store_w(void *p, mm_dtype dt, int64_t i, float x
     }
 }
 
-// VE elements of a row from column c on, of which `size` exist; 0 behind them.
+// A row's channels among its threads: `full` pieces of VE elements, one every 64 W pieces of a thread, and the few behind the last whole
+// piece (fewer than VE), one each of the first threads.
+template <int W, int VE>
+struct Split {
+    int lane, full, tail;   // tail: this thread's channel behind the pieces, or -1
+
+    __device__ __forceinline__ Split(int lane_, int size) : lane(lane_), full(unsigned(size) / VE), tail(-1) {
+        if (full * VE + lane < size) tail = full * VE + lane;
+        if (lane >= VE) tail = -1;
+    }
+    __device__ __forceinline__ bool has(int v) const { return v * 64 * W + lane < full; }
+    __device__ __forceinline__ int at(int v) const { return (v * 64 * W + lane) * VE; }
+};
+
 template <typename T, int VE>
-__device__ __forceinline__ RawVec<T, VE> load_piece(const T *row, int c, int size) {
-    RawVec<T, VE> r = {};
-    if (c + VE <= size) return load_any<T, VE>(reinterpret_cast<const char *>(row), uint32_t(c) * uint32_t(sizeof(T)));
-    if (c < size)
-#pragma unroll
-        for (int e = 0; e < VE - 1; ++e)
-            if (c + e < size) set_raw(r, e, load_elem<T>(reinterpret_cast<const char *>(row), uint32_t(c + e) * uint32_t(sizeof(T))));
-    return r;
+__device__ __forceinline__ RawVec<T, VE> load_piece(const T *row, int c) {
+    return load_any<T, VE>(reinterpret_cast<const char *>(row), uint32_t(c) * uint32_t(sizeof(T)));
 }
 template <typename T, int VE>
-__device__ __forceinline__ void store_piece(T *row, int c, int size, const float *x) {
-    if (c + VE <= size) store_any<T, VE>(reinterpret_cast<char *>(row), uint32_t(c) * uint32_t(sizeof(T)), x);
-    else if (c < size)
-#pragma unroll
-        for (int e = 0; e < VE - 1; ++e)
-            if (c + e < size) row[c + e] = from_f32<T>(x[e]);
+__device__ __forceinline__ void store_piece(T *row, int c, const float *x) {
+    store_any<T, VE>(reinterpret_cast<char *>(row), uint32_t(c) * uint32_t(sizeof(T)), x);
 }
+// Four or eight weights.
 template <int VE>
-__device__ __forceinline__ void weight_piece(const void *p, mm_dtype dt, int c, int size, float other, float *w) {
+__device__ __forceinline__ void weight_piece(const void *p, mm_dtype dt, int c, float other, float *w) {
 #pragma unroll
     for (int e = 0; e < VE; ++e) w[e] = other;
     if (!p) return;
-    if (dt == MM_FLOAT32) unpack_raw(load_piece<float, VE>(static_cast<const float *>(p), c, size), w);
-    else if (dt == MM_FLOAT16) unpack_raw(load_piece<f16_t, VE>(static_cast<const f16_t *>(p), c, size), w);
-    else unpack_raw(load_piece<bf16_t, VE>(static_cast<const bf16_t *>(p), c, size), w);
+    if (dt == MM_FLOAT32) unpack_raw(load_piece<float, VE>(static_cast<const float *>(p), c), w);
+    else if (dt == MM_FLOAT16) unpack_raw(load_piece<f16_t, VE>(static_cast<const f16_t *>(p), c), w);
+    else unpack_raw(load_piece<bf16_t, VE>(static_cast<const bf16_t *>(p), c), w);
 }
 
 // Sum over a row's threads: W waves, in the same order in every thread; `buf` alternates between two halves so that one barrier per
@@ -92,79 +96,86 @@ constexpr int kThreads = 256;
 // A thread's elements of h, and the row's mean and 1 / sqrt(var + eps).
 template <int W, int VE, int NV>
 struct Row {
-    float h[NV][VE];
+    float h[NV][VE], ht;
     float mean, rstd;
 
     template <typename T, typename R>
-    __device__ __forceinline__ void load(const T *x, const R *res, int lane, int size) {
-        RawVec<T, VE> rx[NV];
-        RawVec<R, VE> rr[NV];
+    __device__ __forceinline__ void load(const T *x, const R *res, const Split<W, VE> &s) {
+        RawVec<T, VE> rx[NV] = {};
+        RawVec<R, VE> rr[NV] = {};
 #pragma unroll
-        for (int v = 0; v < NV; ++v) {
-            const int c = (v * 64 * W + lane) * VE;
-            if (x) rx[v] = load_piece<T, VE>(x, c, size);
-            if (res) rr[v] = load_piece<R, VE>(res, c, size);
-        }
+        for (int v = 0; v < NV; ++v)
+            if (s.has(v)) {
+                if (x) rx[v] = load_piece<T, VE>(x, s.at(v));
+                if (res) rr[v] = load_piece<R, VE>(res, s.at(v));
+            }
+        ht = 0.f;
+        if (s.tail >= 0) ht = (x ? to_f32(x[s.tail]) : 0.f) + (res ? to_f32(res[s.tail]) : 0.f);
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
             float a[VE], b[VE];
-            if (x) unpack_raw(rx[v], a);
-            if (res) unpack_raw(rr[v], b);
+            unpack_raw(rx[v], a);
+            unpack_raw(rr[v], b);
 #pragma unroll
-            for (int e = 0; e < VE; ++e) h[v][e] = x ? res ? a[e] + b[e] : a[e] : b[e];
+            for (int e = 0; e < VE; ++e) h[v][e] = a[e] + b[e];
         }
     }
-    __device__ __forceinline__ void stats(bool rms, float eps, int lane, int size, float *buf, int &half) {
-        float s[1] = {0.f};
+    __device__ __forceinline__ void stats(bool rms, float eps, int size, const Split<W, VE> &s, float *buf, int &half) {
+        float sum[1] = {ht};
         mean = 0.f;
         if (!rms) {
 #pragma unroll
             for (int v = 0; v < NV; ++v)
 #pragma unroll
-                for (int e = 0; e < VE; ++e) s[0] += h[v][e];
-            row_sum<W>(s, buf, half);
-            mean = s[0] / float(size);
+                for (int e = 0; e < VE; ++e) sum[0] += h[v][e];
+            row_sum<W>(sum, buf, half);
+            mean = sum[0] / float(size);
         }
-        s[0] = 0.f;
+        sum[0] = s.tail >= 0 ? (ht - mean) * (ht - mean) : 0.f;
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            const int c = (v * 64 * W + lane) * VE;
+            float q = 0.f;
 #pragma unroll
-            for (int e = 0; e < VE; ++e) {
-                const float d = c + e < size ? h[v][e] - mean : 0.f;
-                s[0] = __builtin_fmaf(d, d, s[0]);
-            }
+            for (int e = 0; e < VE; ++e) q = __builtin_fmaf(h[v][e] - mean, h[v][e] - mean, q);
+            sum[0] += s.has(v) ? q : 0.f;
         }
-        row_sum<W>(s, buf, half);
-        rstd = 1.f / sqrtf(s[0] / float(size) + eps);
+        row_sum<W>(sum, buf, half);
+        rstd = 1.f / sqrtf(sum[0] / float(size) + eps);
     }
 };
 
 template <typename T, typename R, int W, int VE, int NV>
 __global__ void __launch_bounds__(kThreads) ln_fwd(const mm_layer_norm_params p) {
     __shared__ float buf[2 * W];
-    const int lane = threadIdx.x % (64 * W), size = int(p.channels);
+    const int size = int(p.channels);
     const int64_t row = int64_t(blockIdx.x) * (4 / W) + threadIdx.x / (64 * W);
     if (row >= p.rows) return;   // whole waves, and whole blocks where they meet at a barrier
+    const Split<W, VE> s(threadIdx.x % (64 * W), size);
     int half = 0;
     Row<W, VE, NV> r;
-    r.load(static_cast<const T *>(p.x) + row * p.x_row_stride, p.residual ? static_cast<const R *>(p.residual) + row * p.residual_row_stride : nullptr, lane, size);
+    r.load(static_cast<const T *>(p.x) + row * p.x_row_stride, p.residual ? static_cast<const R *>(p.residual) + row * p.residual_row_stride : nullptr, s);
     if (p.residual_out) {
         R *to = static_cast<R *>(p.residual_out) + row * p.channels;
 #pragma unroll
-        for (int v = 0; v < NV; ++v) store_piece<R, VE>(to, (v * 64 * W + lane) * VE, size, r.h[v]);
+        for (int v = 0; v < NV; ++v)
+            if (s.has(v)) store_piece<R, VE>(to, s.at(v), r.h[v]);
+        if (s.tail >= 0) to[s.tail] = from_f32<R>(r.ht);
     }
-    r.stats(p.is_rms, p.eps, lane, size, buf, half);
+    r.stats(p.is_rms, p.eps, size, s, buf, half);
     T *out = static_cast<T *>(p.out) + row * p.channels;
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-        const int c = (v * 64 * W + lane) * VE;
-        float w[VE], b[VE];
-        weight_piece<VE>(p.weight, p.wtype, c, size, 1.f, w);
-        weight_piece<VE>(p.bias, p.wtype, c, size, 0.f, b);
+    for (int v = 0; v < NV; ++v)
+        if (s.has(v)) {
+            float w[VE], b[VE];
+            weight_piece<VE>(p.weight, p.wtype, s.at(v), 1.f, w);
+            weight_piece<VE>(p.bias, p.wtype, s.at(v), 0.f, b);
 #pragma unroll
-        for (int e = 0; e < VE; ++e) w[e] = __builtin_fmaf((r.h[v][e] - r.mean) * r.rstd, w[e], b[e]);
-        store_piece<T, VE>(out, c, size, w);
+            for (int e = 0; e < VE; ++e) w[e] = __builtin_fmaf((r.h[v][e] - r.mean) * r.rstd, w[e], b[e]);
+            store_piece<T, VE>(out, s.at(v), w);
+        }
+    if (s.tail >= 0) {
+        const float w = p.weight ? load_w(p.weight, p.wtype, s.tail) : 1.f, b = p.bias ? load_w(p.bias, p.wtype, s.tail) : 0.f;
+        out[s.tail] = from_f32<T>(__builtin_fmaf((r.ht - r.mean) * r.rstd, w, b));
     }
 }
 
@@ -174,9 +185,10 @@ __global__ void __launch_bounds__(kThreads) ln_fwd(const mm_layer_norm_params p)
 template <typename T, typename R, int W, int VE, int NV, bool DB>
 __global__ void __launch_bounds__(kThreads) ln_bwd(const mm_layer_norm_params p, float *part) {
     __shared__ float buf[2 * 2 * W], sums[W == 1 ? 3 * 64 * VE : 1];
-    const int lane = threadIdx.x % (64 * W), size = int(p.channels);
+    const int size = int(p.channels);
+    const Split<W, VE> s(threadIdx.x % (64 * W), size);
     int half = 0;
-    float dw[NV][VE], db[DB ? NV : 1][VE];
+    float dw[NV][VE], db[DB ? NV : 1][VE], dwt = 0.f, dbt = 0.f;
 #pragma unroll
     for (int v = 0; v < NV; ++v)
 #pragma unroll
@@ -184,64 +196,78 @@ __global__ void __launch_bounds__(kThreads) ln_bwd(const mm_layer_norm_params p,
             dw[v][e] = 0.f;
             if constexpr (DB) db[v][e] = 0.f;
         }
+    const float wt = s.tail >= 0 && p.weight ? load_w(p.weight, p.wtype, s.tail) : 1.f;
+#pragma unroll 1
     for (int64_t row = int64_t(blockIdx.x) * (4 / W) + threadIdx.x / (64 * W); row < p.rows; row += int64_t(gridDim.x) * (4 / W)) {
         Row<W, VE, NV> r;
-        RawVec<T, VE> rd[NV];
+        RawVec<T, VE> rd[NV] = {};
         const T *dout = static_cast<const T *>(p.dout) + row * p.dout_row_stride;
 #pragma unroll
-        for (int v = 0; v < NV; ++v) rd[v] = load_piece<T, VE>(dout, (v * 64 * W + lane) * VE, size);
+        for (int v = 0; v < NV; ++v)
+            if (s.has(v)) rd[v] = load_piece<T, VE>(dout, s.at(v));
+        const float dt = s.tail >= 0 ? to_f32(dout[s.tail]) : 0.f;
         r.load(p.x ? static_cast<const T *>(p.x) + row * p.x_row_stride : nullptr,
-               p.residual ? static_cast<const R *>(p.residual) + row * p.residual_row_stride : nullptr, lane, size);
-        r.stats(p.is_rms, p.eps, lane, size, buf, half);
-        float dn[NV][VE], s[2] = {0.f, 0.f};
+               p.residual ? static_cast<const R *>(p.residual) + row * p.residual_row_stride : nullptr, s);
+        r.stats(p.is_rms, p.eps, size, s, buf, half);
+        const float yt = (r.ht - r.mean) * r.rstd;
+        dwt = __builtin_fmaf(dt, yt, dwt);
+        dbt += dt;
+        float sum[2] = {dt * wt * yt, dt * wt};
 #pragma unroll
-        for (int v = 0; v < NV; ++v) {
-            const int c = (v * 64 * W + lane) * VE;
-            float d[VE], w[VE];
-            unpack_raw(rd[v], d);
-            weight_piece<VE>(p.weight, p.wtype, c, size, 1.f, w);
+        for (int v = 0; v < NV; ++v)
+            if (s.has(v)) {
+                float d[VE], w[VE];
+                unpack_raw(rd[v], d);
+                weight_piece<VE>(p.weight, p.wtype, s.at(v), 1.f, w);
 #pragma unroll
-            for (int e = 0; e < VE; ++e) {   // behind the row d and so all of these are 0
-                const float y = (r.h[v][e] - r.mean) * r.rstd;
-                dw[v][e] = __builtin_fmaf(d[e], y, dw[v][e]);
-                if constexpr (DB) db[v][e] += d[e];
-                dn[v][e] = d[e] * w[e];
-                s[0] = __builtin_fmaf(dn[v][e], y, s[0]);
-                s[1] += dn[v][e];
+                for (int e = 0; e < VE; ++e) {
+                    const float y = (r.h[v][e] - r.mean) * r.rstd, dn = d[e] * w[e];
+                    dw[v][e] = __builtin_fmaf(d[e], y, dw[v][e]);
+                    if constexpr (DB) db[v][e] += d[e];
+                    sum[0] = __builtin_fmaf(dn, y, sum[0]);
+                    sum[1] += dn;
+                }
             }
-        }
-        row_sum<W>(s, buf, half);
-        const float m1 = s[0] / float(size), m0 = p.is_rms ? 0.f : s[1] / float(size);
+        row_sum<W>(sum, buf, half);
+        const float m1 = sum[0] / float(size), m0 = p.is_rms ? 0.f : sum[1] / float(size);
         const R *dres = p.dresidual_out ? static_cast<const R *>(p.dresidual_out) + row * p.dresidual_out_row_stride : nullptr;
+        T *dx = p.dx ? static_cast<T *>(p.dx) + row * p.channels : nullptr;
+        R *dr = p.dresidual ? static_cast<R *>(p.dresidual) + row * p.channels : nullptr;
 #pragma unroll
-        for (int v = 0; v < NV; ++v) {
-            const int c = (v * 64 * W + lane) * VE;
-            float dh[VE], a[VE];
-            if (dres) unpack_raw(load_piece<R, VE>(dres, c, size), a);
+        for (int v = 0; v < NV; ++v)
+            if (s.has(v)) {
+                float d[VE], w[VE], a[VE];
+                unpack_raw(rd[v], d);
+                weight_piece<VE>(p.weight, p.wtype, s.at(v), 1.f, w);   // once more, from the cache: held it would take too many registers
+                if (dres) unpack_raw(load_piece<R, VE>(dres, s.at(v)), a);
 #pragma unroll
-            for (int e = 0; e < VE; ++e) {
-                const float y = (r.h[v][e] - r.mean) * r.rstd;
-                dh[e] = r.rstd * (dn[v][e] - m0 - y * m1);
-                if (dres) dh[e] += a[e];
+                for (int e = 0; e < VE; ++e) {
+                    const float y = (r.h[v][e] - r.mean) * r.rstd;
+                    d[e] = r.rstd * (d[e] * w[e] - m0 - y * m1);
+                    if (dres) d[e] += a[e];
+                }
+                if (dx) store_piece<T, VE>(dx, s.at(v), d);
+                if (dr) store_piece<R, VE>(dr, s.at(v), d);
             }
-            if (p.dx) store_piece<T, VE>(static_cast<T *>(p.dx) + row * p.channels, c, size, dh);
-            if (p.dresidual) store_piece<R, VE>(static_cast<R *>(p.dresidual) + row * p.channels, c, size, dh);
+        if (s.tail >= 0) {
+            float d = r.rstd * (dt * wt - m0 - yt * m1);
+            if (dres) d += to_f32(dres[s.tail]);
+            if (dx) dx[s.tail] = from_f32<T>(d);
+            if (dr) dr[s.tail] = from_f32<R>(d);
         }
     }
     if (!part) return;
     float *pw = part + int64_t(blockIdx.x) * 2 * p.channels, *pb = pw + p.channels;
     // The four waves' rows of a block, in order.
-    auto add = [&](float (&x)[VE]) {
+    auto add = [&](float *x, int n) {
         if constexpr (W == 1) {
             const int l = threadIdx.x % 64, wave = threadIdx.x / 64;
             __syncthreads();
             if (wave > 0)
-#pragma unroll
-                for (int e = 0; e < VE; ++e) sums[((wave - 1) * VE + e) * 64 + l] = x[e];
+                for (int e = 0; e < n; ++e) sums[((wave - 1) * VE + e) * 64 + l] = x[e];
             __syncthreads();
             if (wave == 0)
-#pragma unroll
-                for (int e = 0; e < VE; ++e)
+                for (int e = 0; e < n; ++e)
 #pragma unroll
                     for (int w = 0; w < 3; ++w) x[e] += sums[(w * VE + e) * 64 + l];
             return wave == 0;
@@ -250,12 +276,16 @@ __global__ void __launch_bounds__(kThreads) ln_bwd(const mm_layer_norm_params p,
     };
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-        const int c = (v * 64 * W + lane) * VE;
-        if (v * 64 * W * VE >= size) break;
-        if (add(dw[v])) store_piece<float, VE>(pw, c, size, dw[v]);
-        if constexpr (DB)
-            if (add(db[v])) store_piece<float, VE>(pb, c, size, db[v]);
+        const bool mine = add(dw[v], VE) && s.has(v);
+        if (mine) store_piece<float, VE>(pw, s.at(v), dw[v]);
+        if constexpr (DB) {
+            const bool too = add(db[v], VE) && s.has(v);
+            if (too) store_piece<float, VE>(pb, s.at(v), db[v]);
+        }
     }
+    if (add(&dwt, 1) && s.tail >= 0) pw[s.tail] = dwt;
+    if constexpr (DB)
+        if (add(&dbt, 1) && s.tail >= 0) pb[s.tail] = dbt;
 }
 
 // dweight and dbias: the blocks' partial rows summed in order, 32 columns and 32 runs of rows per block.
@@ -293,11 +323,11 @@ struct Plan {
 };
 static Plan plan(const mm_layer_norm_params &p, bool bwd) {
     Plan k;
-    const int64_t ve = p.itype == MM_FLOAT32 ? 4 : 8, pieces = (p.channels + ve - 1) / ve, cus = device_simds() / 4;
+    const int64_t ve = p.itype == MM_FLOAT32 ? 4 : 8, pieces = p.channels / ve, cus = device_simds() / 4;
     // One wave per row while that takes at most 64 elements of a thread, but for forwards of so few rows that they do not fill the
     // card: there four waves shorten a row's time.
-    k.waves = pieces * ve > 4096 || (!bwd && p.rows <= cus * 4 && pieces > 64) ? 4 : 1;
-    k.nv = int((pieces + 64 * k.waves - 1) / (64 * k.waves));
+    k.waves = p.channels > 4096 || (!bwd && p.rows <= cus * 4 && pieces > 64) ? 4 : 1;
+    k.nv = std::max(1, int((pieces + 64 * k.waves - 1) / (64 * k.waves)));
     const int64_t per = 4 / k.waves;
     k.blocks = (p.rows + per - 1) / per;
     // Two blocks per CU, and a partial row for each.
@@ -334,7 +364,7 @@ static int run_r(const mm_layer_norm_params &p, bool bwd, hipStream_t s) {
     const Plan k = plan(p, bwd);
     constexpr int VE = 16 / sizeof(T);
     if constexpr (sizeof(T) == 2) return k.waves == 1 ? launch<T, R, 1, VE, 1, 2, 3, 4, 5, 6, 8>(p, k, bwd, s) : launch<T, R, 4, VE, 1, 2, 4, 8>(p, k, bwd, s);
-    else return k.waves == 1 ? launch<T, R, 1, VE, 1, 2, 4, 6, 8, 10, 12, 16>(p, k, bwd, s) : launch<T, R, 4, VE, 1, 2, 4, 8, 16>(p, k, bwd, s);
+    else return k.waves == 1 ? launch<T, R, 1, VE, 1, 2, 4, 6, 8, 12, 16>(p, k, bwd, s) : launch<T, R, 4, VE, 1, 2, 4, 8, 16>(p, k, bwd, s);
 }
 static int run(const mm_layer_norm_params &p, bool bwd, hipStream_t s) {
     const bool wide = p.rtype == MM_FLOAT32;

@@ -24,8 +24,9 @@ def _forward(x, weight, bias, residual, eps, prenorm, wide, is_rms_norm):
     weight = None if weight is None else weight.contiguous()
     bias = None if bias is None else bias.contiguous()
     out, res = ext().layer_norm_fwd(xf, rf, weight, bias, eps, is_rms_norm, prenorm, wide)
-    out = out.view(x.shape)
-    return xf, rf, weight, bias, res, (out, res.view(x.shape)) if prenorm else out
+    if x.dim() != 2:
+        out = out.view(x.shape)
+    return xf, rf, weight, bias, res, out if not prenorm else (out, res if x.dim() == 2 else res.view(x.shape))
 
 
 class LayerNormFn(torch.autograd.Function):
