@@ -21,7 +21,7 @@
  * allocated, 0 or a code of mm_scan.h is returned and mm_last_error() has the text. The innermost dimension (dk or dv) of q, k, v,
  * dout and of every output is contiguous; states are contiguous (batch, nheads, dk, dv). Sequence strides are 0 to 2^22 - 1
  * elements (nheads * dk and nheads * dv too in the backward), seqlen is at most 2^23, batch * nheads at most 2^20
- * (mm_delta_update: 2^24 - 1); else MM_ERR_UNSUPPORTED.
+ * (mm_delta_update: 2^23 - 1); else MM_ERR_UNSUPPORTED.
  */
 #ifndef MM_DELTA_H_
 #define MM_DELTA_H_

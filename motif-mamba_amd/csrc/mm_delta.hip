@@ -750,6 +750,14 @@ __device__ __forceinline__ void infinite_rows(f32x4 (&S)[KD / 16][1], char *smem
             const int at = col + (lane & 15);
             store_element<T, false>(x * a.scale, to, t0 >= first && lane < 16 && at < a.dv - col0 ? uint32_t(t) * uint32_t(a.out_seq) + uint32_t(at) : kNone);
         });
+        // A state that is NaN throughout stays so, and so did the walk's.
+        bool lost = true;
+        const int dk = afresh(a.dk), g = lane >> 4;
+#pragma unroll
+        for (int k = 0; k < KD / 16; ++k)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) lost &= R[k][0][r] != R[k][0][r] || 16 * k + 4 * g + r >= dk;
+        if (__syncthreads_and(lost || first >= end || col + (lane & 15) >= a.dv - col0)) break;
     }
     if (first < end)
 #pragma unroll
@@ -1180,6 +1188,29 @@ __global__ void __launch_bounds__(kThreads) dr_join(const Args) {
 
 // ---- dQ, dK, dbeta and the decays' gradient ------------------------------------------------------
 
+// A C x 64 tile whose rows are only ever read as operands lies in their order, 1,024 bytes for 16 rows and 32 columns of a plane: one
+// 16-byte read per lane without bank conflicts. Element (row, x), x a multiple of 4, of the first of P planes, 512 elements apart:
+template <int P>
+__device__ __forceinline__ int operand_at(int row, int x) {
+    return ((row >> 4) * 2 + (x >> 5)) * P * 512 + ((x >> 2 & 3) * 16 + (row & 15)) * 8 + (x >> 4 & 1) * 4;
+}
+template <int P>
+__device__ __forceinline__ bf16x8 operand(const u16 *img, int t, int k, int plane, int lane) {
+    return *reinterpret_cast<const bf16x8 *>(img + ((t * 2 + k) * P + plane) * 512 + lane * 8);
+}
+// Eight (four) consecutive elements of a row in P planes, each the nearest of what is left.
+template <int P, int N = 8>
+__device__ __forceinline__ void put_operand(u16 *img, int row, int x, const float (&y)[8]) {
+    bf16x8 p[kPlanes];
+    split8(y, p);
+#pragma unroll
+    for (int q = 0; q < P; ++q) {
+        const u32x4 v = __builtin_bit_cast(u32x4, p[q]);
+        *reinterpret_cast<uint2 *>(img + q * 512 + operand_at<P>(row, x)) = make_uint2(v.x, v.y);
+        if constexpr (N == 8) *reinterpret_cast<uint2 *>(img + q * 512 + operand_at<P>(row, x + 4)) = make_uint2(v.z, v.w);
+    }
+}
+
 // 64 columns of a chunk's float32 rows (pitch vd) on their way into a tile's planes, 8 of a row per thread and step.
 template <int C, int NT>
 struct StageF32 {
@@ -1197,8 +1228,7 @@ struct StageF32 {
         }
     }
     // Rows times w (NULL: 1).
-    __device__ __forceinline__ void store(u16 *tile, const float *w, int tid) const {
-        constexpr int PL = kTile<C, 64>;
+    __device__ __forceinline__ void store(u16 *img, const float *w, int tid) const {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             const int at = n * NT + tid, row = at / 8, x = at % 8 * 8;
@@ -1206,35 +1236,74 @@ struct StageF32 {
             const float s = w ? w[row] : 1.f;
             const float4 a = r[n][0], b = r[n][1];
             const float y[8] = {a.x * s, a.y * s, a.z * s, a.w * s, b.x * s, b.y * s, b.z * s, b.w * s};
-            bf16x8 p[kPlanes];
-            split8(y, p);
-#pragma unroll
-            for (int q = 0; q < kPlanes; ++q) {
-                const u32x4 v = __builtin_bit_cast(u32x4, p[q]);
-                *reinterpret_cast<uint2 *>(tile + q * PL + la::at<64>(row, x)) = make_uint2(v.x, v.y);
-                *reinterpret_cast<uint2 *>(tile + q * PL + la::at<64>(row, x + 4)) = make_uint2(v.z, v.w);
-            }
+            put_operand<kPlanes>(img, row, x, y);
         }
     }
 };
+// The same of a tensor's own rows (64 of their columns).
+template <typename T, int C, int NT, bool VEC>
+__device__ __forceinline__ void store_operand(const Stage<T, C, 64, NT, VEC> &s, u16 *img, int tid) {
+    typedef Stage<T, C, 64, NT, VEC> S;
+#pragma unroll
+    for (int n = 0; n < S::N; ++n) {
+        const int row = tid / S::VR + n * S::RS, x = tid % S::VR * S::VE;
+        if (!S::kEven && row >= C) break;
+        const uint32_t w[4] = {s.r[n].x, s.r[n].y, s.r[n].z, s.r[n].w};
+        if constexpr (std::is_same_v<T, bf16_t>) {
+            *reinterpret_cast<uint2 *>(img + operand_at<1>(row, x)) = make_uint2(w[0], w[1]);
+            *reinterpret_cast<uint2 *>(img + operand_at<1>(row, x + 4)) = make_uint2(w[2], w[3]);
+        } else {
+            float y[8] = {};
+#pragma unroll
+            for (int e = 0; e < S::VE; ++e) y[e] = elem_f32<T>(sizeof(T) == 4 ? w[e] : (w[e / 2] >> (16 * (e % 2))) & 0xffffu);
+            put_operand<Cfg<T>::in, S::VE>(img, row, x, y);
+        }
+    }
+}
 
-// O[t] += A(t, k) f for one 32-wide step k of rows in PA planes (D-wide tile).
-template <int C, int D, int PA>
-__device__ __forceinline__ void row_products(f32x4 *O, int stride, const u16 *A, int k, const bf16x8 (&f)[kPlanes], int lane) {
-    constexpr int PL = kTile<C, D>;
-    const int g = lane >> 4, i = lane & 15;
+// O[t] += A(t, k) f for one 32-wide step k of rows in PA planes.
+template <int C, int PA>
+__device__ __forceinline__ void row_products(f32x4 (&O)[C / 16][1], const u16 *A, int k, const bf16x8 (&f)[kPlanes], int lane) {
     bf16x8 a[C / 16][PA];
 #pragma unroll
     for (int t = 0; t < C / 16; ++t)
 #pragma unroll
-        for (int p = 0; p < PA; ++p) a[t][p] = frag_row<D>(A + p * PL, 16 * t, k, g, i);
+        for (int p = 0; p < PA; ++p) a[t][p] = operand<PA>(A, t, k, p, lane);
 #pragma unroll
     for (int p = 0; p < PA; ++p)
 #pragma unroll
         for (int q = 0; q < kPlanes; ++q)
             if (p + q < kPlanes)
 #pragma unroll
-                for (int t = 0; t < C / 16; ++t) O[t * stride] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[t][p], f[q], O[t * stride], 0, 0, 0);
+                for (int t = 0; t < C / 16; ++t) O[t][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[t][p], f[q], O[t][0], 0, 0, 0);
+}
+// tile_products of two such tiles.
+template <int PX, int PY, typename L>
+__device__ __forceinline__ void operand_products(f32x4 *s, const u16 *X, const u16 *Y, int lane) {
+    constexpr int B = PX > 1 ? 3 : 4;   // tiles whose operands are held at once
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int j0 = 0; j0 < L::N; j0 += B) {
+            bf16x8 a[B][PY], b[B][PX];
+#pragma unroll
+            for (int j = 0; j < B && j0 + j < L::N; ++j) {
+#pragma unroll
+                for (int p = 0; p < PX; ++p) {
+                    if (j > 0 && L::O(j0 + j) == L::O(j0 + j - 1)) b[j][p] = b[j - 1][p];
+                    else b[j][p] = operand<PX>(X, L::O(j0 + j), k, p, lane);
+                }
+#pragma unroll
+                for (int p = 0; p < PY; ++p) a[j][p] = operand<PY>(Y, L::n(j0 + j), k, p, lane);
+            }
+#pragma unroll
+            for (int p = 0; p < PY; ++p)
+#pragma unroll
+                for (int q = 0; q < PX; ++q)
+                    if (p + q < kPlanes)
+#pragma unroll
+                        for (int j = 0; j < B && j0 + j < L::N; ++j) s[j0 + j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[j][p], b[j][q], s[j0 + j], 0, 0, 0);
+        }
 }
 
 // part[n] = sum over the wave's columns of A[n][x] Y[n][x] + B[n][x] Z[n][x] (B may be NULL).
@@ -1319,6 +1388,7 @@ __device__ __forceinline__ void each_tile_of_two(int wave, F &&f) {
 // terms with E and S), column sums with the leaving ones, f_j, are k_j . dKc_j. So, summed from t on to the chunk's end or to the next
 // forgotten state, which no pair crosses,
 //     dg_t = sum of (row sum - column sum without f) + sum over j < t of f_j + e^c_end <R, S>.
+// A's diagonal would be in a row sum and in a column sum alike; it is added to dQ and dK behind them.
 template <typename T, int KD, bool VEC, bool F32>
 __global__ void __launch_bounds__(KD * 4) __attribute__((amdgpu_waves_per_eu(2, 2))) dr_grad(const Args) {
     constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, CT = C / 16, NC = 1, NW = KD / 16, NT = 64 * NW, PM = kTile<C, kScoreRow>;
@@ -1329,7 +1399,7 @@ __global__ void __launch_bounds__(KD * 4) __attribute__((amdgpu_waves_per_eu(2, 
     u16 *U = D + PI * kTile<C, 64>, *X = U + kPlanes * kTile<C, 64>;
     u16 *MA = U, *ME = X;   // the triangles, once U and dV are read (kTile<C, 64> is kTile<C, kScoreRow>)
     Chunk<C> *ck = reinterpret_cast<Chunk<C> *>(X + kPlanes * kTile<C, 64>);
-    float *row = reinterpret_cast<float *>(ck + 1), *cols = row + NW * C, *fs = cols + NW * C, *rs = fs + NW * C;   // [wave][C]; rs [wave]
+    float *row = reinterpret_cast<float *>(ck + 1), *cols = row + NW * C, *fs = cols + NW * C, *diag = fs + NW * C, *rs = diag + C;   // [wave][C]; diag [C], rs [wave]
     auto args = [] { return own_args<Args>(); };
     int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, i = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(tid / 64), col = wave * 16;
@@ -1422,27 +1492,26 @@ __global__ void __launch_bounds__(KD * 4) __attribute__((amdgpu_waves_per_eu(2, 
         }
         sk.store(K, tid);
         sq.store(Q, tid);
-        f32x4 a1[6], a2[4], dq[CT][NC], dr[CT][NC], dc[CT][NC];
+        constexpr int kScores = C == 64 && NW == 4 ? 6 : C == 64 ? 4 : 3;
+        f32x4 sc[kScores], dq[CT][NC], dr[CT][NC], dc[CT][NC];   // sc: the tiles of both lists
         float rdots = 0.f;
 #pragma unroll
-        for (int j = 0; j < 6; ++j) a1[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) a2[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int j = 0; j < kScores; ++j) sc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int t = 0; t < CT; ++t) dq[t][0] = dr[t][0] = dc[t][0] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
         for (int h0 = 0; h0 < vd; h0 += 64) {
             __syncthreads();
             fresh();
-            sd.store(D, tid);
+            store_operand<T, C, NT, VEC>(sd, D, tid);
             su.store(U, ck->beta, tid);
             sx.store(X, nullptr, tid);
             if (h0 + 64 < vd) load(w, h0 + 64);
             __syncthreads();
             fresh();
             each_tile_of_two<C, NW>(wave, [&](auto L1, auto L2) {
-                if constexpr (decltype(L1)::N > 0) tile_products<PI, kPlanes, C, 64, decltype(L1)>(a1, D, U, lane);
-                if constexpr (decltype(L2)::N > 0) tile_products<kPlanes, kPlanes, C, 64, decltype(L2)>(a2, X, U, lane);
+                if constexpr (decltype(L1)::N > 0) operand_products<PI, kPlanes, decltype(L1)>(sc, D, U, lane);
+                if constexpr (decltype(L2)::N > 0) operand_products<kPlanes, kPlanes, decltype(L2)>(sc + decltype(L1)::N, X, U, lane);
             });
             fresh();
             bf16x8 f[2][2][kPlanes];
@@ -1466,9 +1535,9 @@ __global__ void __launch_bounds__(KD * 4) __attribute__((amdgpu_waves_per_eu(2, 
             if (h0 + 64 < vd) load_states(w, h0 + 64);
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                row_products<C, 64, PI>(&dq[0][0], NC, D, k, f[k][0], lane);
-                row_products<C, 64, kPlanes>(&dr[0][0], NC, X, k, f[k][0], lane);
-                row_products<C, 64, kPlanes>(&dc[0][0], NC, U, k, f[k][1], lane);
+                row_products<C, PI>(dq, D, k, f[k][0], lane);
+                row_products<C, kPlanes>(dr, X, k, f[k][0], lane);
+                row_products<C, kPlanes>(dc, U, k, f[k][1], lane);
             }
         }
         if constexpr (kAhead) {
@@ -1507,7 +1576,13 @@ __global__ void __launch_bounds__(KD * 4) __attribute__((amdgpu_waves_per_eu(2, 
                 const f32x4 w = tile_decay<C, false, O, o>(ck->d, 1.f, lane);
                 float x[4];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) x[r] = O != o || 4 * g + r <= i ? a1[j][r] * (w[r] * scale) : 0.f;
+                for (int r = 0; r < 4; ++r) {
+                    x[r] = sc[j][r] * (w[r] * scale);
+                    if constexpr (O == o) {
+                        if (4 * g + r == i) diag[16 * O + i] = x[r];
+                        x[r] = 4 * g + r < i ? x[r] : 0.f;
+                    }
+                }
                 store_scores<C>(MA, x, O, o, lane);
             });
             static_for<0, E::N>([&](auto Jc) {
@@ -1515,7 +1590,7 @@ __global__ void __launch_bounds__(KD * 4) __attribute__((amdgpu_waves_per_eu(2, 
                 const f32x4 w = tile_decay<C, false, O, o>(ck->d, 1.f, lane);
                 float x[4];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) x[r] = O != o || 4 * g + r < i ? -(a2[j][r] * w[r]) : 0.f;
+                for (int r = 0; r < 4; ++r) x[r] = O != o || 4 * g + r < i ? -(sc[A::N + j][r] * w[r]) : 0.f;
                 store_scores<C>(ME, x, O, o, lane);
             });
         });
@@ -1568,10 +1643,21 @@ __global__ void __launch_bounds__(KD * 4) __attribute__((amdgpu_waves_per_eu(2, 
             dot_two<T, C, NC, KD, true>(dq, Q, dr, K, col, row + wave * C, lane);
             dot_two<T, C, NC, KD, false>(dc, K, dc, K, col, cols + wave * C, lane);
         }
+        // A's diagonal, which is in no decay's sum: dQ_i += A_ii k_i, dK_i += A_ii q_i.
+        auto add_diagonal = [&](f32x4 (&x)[CT][NC], const u16 *rows_) {
+            tile_columns<T, C, NC, KD>(rows_, col, lane, [&](int j, int, const float *y) {
 #pragma unroll
-        for (int t = 0; t < CT; ++t)
+                for (int h = 0; h < 2; ++h) {
+                    const f32x4 d = *reinterpret_cast<const f32x4 *>(diag + 32 * j + 16 * h + 4 * g);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) dr[t][0][r] += dc[t][0][r];
+                    for (int r = 0; r < 4; ++r) x[2 * j + h][0][r] = __builtin_fmaf(d[r], y[4 * h + r], x[2 * j + h][0][r]);
+                }
+            });
+        };
+#pragma unroll
+        for (int t = 0; t < CT; ++t) dr[t][0] += dc[t][0];
+        add_diagonal(dq, K);
+        add_diagonal(dr, Q);
         {
             const Args a = args();
             const int64_t ob = (p.b * a.seqlen * a.heads + p.h) * a.dk * int64_t(F32 ? 4 : sizeof(T));
@@ -1658,7 +1744,7 @@ template <typename T, int KD, bool VEC, bool F32>
 static int grad_t(const Args &a, hipStream_t s) {
     constexpr int C = Cfg<T>::C, PI = Cfg<T>::in;
     constexpr int NW = KD / 16;
-    constexpr int bytes = 2 * (2 * PI * kTile<C, KD> + PI * kTile<C, 64> + 2 * kPlanes * kTile<C, 64>) + int(sizeof(Chunk<C>)) + 4 * (3 * NW * C + NW);
+    constexpr int bytes = 2 * (2 * PI * kTile<C, KD> + PI * kTile<C, 64> + 2 * kPlanes * kTile<C, 64>) + int(sizeof(Chunk<C>)) + 4 * ((3 * NW + 1) * C + NW);
     static_assert(bytes <= (KD == 64 ? 80 : 160) * 1024, "two workgroups on a CU at KD 64, one at 128");
     static std::atomic<uint64_t> done{0};
     return launch_kernel(dr_grad<T, KD, VEC, F32>, bytes, done, std::min<int64_t>(a.batch * a.heads * a.chunks, KD == 64 ? kMostGroups : device_simds() / 4), 64 * NW, a, s, "dr_grad");

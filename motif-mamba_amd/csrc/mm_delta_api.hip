@@ -171,7 +171,7 @@ static bool known(mm_dtype t) { return t == MM_FLOAT32 || t == MM_FLOAT16 || t =
 static int64_t pad16(int64_t n) { return (n + 15) / 16 * 16; }
 static int64_t pad64(int64_t n) { return (n + 63) / 64 * 64; }
 
-constexpr int64_t kMostPairs = int64_t(1) << 20, kMostTokenPairs = (int64_t(1) << 24) - 1;
+constexpr int64_t kMostPairs = int64_t(1) << 20, kMostTokenPairs = (int64_t(1) << 23) - 1;   // a launch takes less than 2^32 threads, one token's up to 512 for each
 
 static View view(const void *p, mm_dtype t, int64_t b, int64_t s, int64_t h, int share, int64_t d) {
     const int64_t e = size_of(t);
@@ -187,7 +187,7 @@ static int check(const P &p, int64_t seqlen, int64_t pairs) {
     if (p.dk < 1 || p.dv < 1) return set_error(MM_ERR_INVALID_ARGUMENT, "delta rule: dk and dv must be at least 1");
     if (p.dk > MM_DELTA_MAX_DIM || p.dv > MM_DELTA_MAX_DIM) return set_error(MM_ERR_UNSUPPORTED, "delta rule: dk and dv must be <= 128");
     if (p.batch > pairs || p.nheads > pairs || p.batch * p.nheads > pairs)
-        return set_error(MM_ERR_UNSUPPORTED, "delta rule: batch * nheads is too large (at most 2^20, for one token 2^24 - 1)");
+        return set_error(MM_ERR_UNSUPPORTED, "delta rule: batch * nheads is too large (at most 2^20, for one token 2^23 - 1)");
     if (seqlen > (int64_t(1) << 23)) return set_error(MM_ERR_UNSUPPORTED, "delta rule: seqlen must be <= 2^23");
     return MM_OK;
 }
@@ -250,7 +250,7 @@ static Cut segments(int64_t pairs, int64_t seqlen, int64_t dk, int64_t dv, mm_dt
         const int64_t per = (chunks + n - 1) / n;
         return Cut{int((chunks + per - 1) / per), per * C};
     };
-    if (const char *e = std::getenv("MM_DELTA_SEGMENTS")) return cut(std::min<int64_t>(std::max<int64_t>(std::atoll(e), 1), chunks));
+    if (const char *e = std::getenv("MM_DELTA_SEGMENTS")) return cut(std::min<int64_t>({std::max<int64_t>(std::atoll(e), 1), chunks, kMostPairs / pairs}));
     const double us = (ks == 2 ? 4.8 : 3.6), join = (ks == 2 ? 3.0 : 1.2) / us, launch = 6.0 / us;
     auto rounds = [&](int64_t groups) {
         const int64_t full = groups / (2 * cus), rest = groups % (2 * cus);
@@ -258,7 +258,7 @@ static Cut segments(int64_t pairs, int64_t seqlen, int64_t dk, int64_t dv, mm_dt
     };
     Cut best = cut(1);
     double least = 0.0;
-    for (int64_t n = 1; n <= std::min<int64_t>(chunks / 2 + 1, 64); ++n) {
+    for (int64_t n = 1; n <= std::min<int64_t>({chunks / 2 + 1, 64, kMostPairs / pairs}); ++n) {
         const Cut c = cut(n);
         if (c.segs != n) continue;
         const double m = double(c.len / C), walk = rounds(pairs * n * vs);

@@ -103,7 +103,7 @@ def test_bwd_refusals(blocks, change, code, needle):
 
 
 @pytest.mark.parametrize("change,code,needle", [
-    (dict(itype=7), -1, "dtype"), (dict(dk=129), -2, "128"), (dict(batch=1 << 24, nheads=1), -2, "too large"), (dict(state=0), -1, "required"),
+    (dict(itype=7), -1, "dtype"), (dict(dk=129), -2, "128"), (dict(batch=1 << 23, nheads=1), -2, "too large"), (dict(state=0), -1, "required"),
     (dict(beta=0), -1, "required"), *((dict(zip(("state_batch_stride", "state_head_stride", "state_dk_stride"), s)), -1, "overlap") for s in (
         (0, 256, 16), (512, 0, 16), (512, 256, 0), (512, 256, 15), (512, 255, 16), (256, 512, 8), (500, 256, 16), (-256, 256, 16)))])
 def test_update_refusals(blocks, change, code, needle):
