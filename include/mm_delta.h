@@ -50,6 +50,7 @@ typedef struct mm_delta_fwd_params {
     void *out;                   /* (batch, seqlen, nheads, dv) */
     float *last_state;           /* (batch, nheads, dk, dv) or NULL */
     void *segment_states;        /* mm_delta_segment_states_size() bytes, 16-byte aligned, written for the backward; or NULL */
+    int64_t segment_states_bytes;
     void *workspace;             /* mm_delta_fwd_workspace_size() bytes, 16-byte aligned (required) */
     int64_t workspace_bytes;
     int64_t q_batch_stride, q_seq_stride, q_group_stride;
@@ -77,6 +78,7 @@ typedef struct mm_delta_bwd_params {
     int32_t decay_per_head;      /* log_decay is one value per head: dlog_decay is summed over batch and seqlen */
     const void *segment_states;  /* what the forward left there, after a call with the same sizes, inputs and device, or NULL
                                   * (computed again) */
+    int64_t segment_states_bytes;   /* as in that call */
     void *workspace;             /* mm_delta_bwd_workspace_size() bytes, 16-byte aligned (required) */
     int64_t workspace_bytes;
     int64_t q_batch_stride, q_seq_stride, q_group_stride;
@@ -109,7 +111,8 @@ typedef struct mm_delta_update_params {
 
 /* Workspace bytes (0: none needed). They depend on the sizes and on the current device's compute-unit count: query with the device of
  * the call current. They also depend on whether segment_states and the backward's dlog_decay are NULL: query with those pointers set
- * as in the call. segment_states' own size is 0 where rows are not cut: leave it NULL then. */
+ * as in the call. segment_states' own size is 0 where rows are not cut: leave it NULL then. A call refuses segment_states of any other
+ * size than the query's, as after a change of MM_DELTA_SEGMENTS (the number of segments, for measurements) between the two. */
 int64_t mm_delta_fwd_workspace_size(const mm_delta_fwd_params *params);
 int64_t mm_delta_segment_states_size(const mm_delta_fwd_params *params);
 int64_t mm_delta_bwd_workspace_size(const mm_delta_bwd_params *params);

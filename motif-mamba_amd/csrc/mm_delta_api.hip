@@ -23,7 +23,8 @@ __device__ __forceinline__ float read_gate(const void *p, mm_dtype t, int64_t i)
     }
 }
 
-// Sums over the rows of a workgroup of each lane's four columns: over those that a wave holds, then over the waves.
+// Sums over the rows of a workgroup of each lane's four columns: over those that a wave holds, then over the waves, eight in pairs:
+// what four of twice the rows add. So a pair's bits do not depend on how many pairs a call has (launch_update).
 template <int LPR, int NW>
 __device__ __forceinline__ void row_sums(float (&x)[4], float4 (*part)[LPR]) {
     const int tid = threadIdx.x;
@@ -35,8 +36,12 @@ __device__ __forceinline__ void row_sums(float (&x)[4], float4 (*part)[LPR]) {
     __syncthreads();
     x[0] = x[1] = x[2] = x[3] = 0.f;
 #pragma unroll
-    for (int w = 0; w < NW; ++w) {
-        const float4 y = part[w][tid % LPR];
+    for (int w = 0; w < NW; w += NW / 4) {
+        float4 y = part[w][tid % LPR];
+        if constexpr (NW == 8) {
+            const float4 y2 = part[w + 1][tid % LPR];
+            y.x += y2.x; y.y += y2.y; y.z += y2.z; y.w += y2.w;
+        }
         x[0] += y.x; x[1] += y.y; x[2] += y.z; x[3] += y.w;
     }
 }
@@ -303,6 +308,11 @@ static Kept plan_kept(const P &p, bool train) {
     w.bytes = take.at;
     return w;
 }
+template <typename P>
+static int check_kept(const P &p) {
+    if (!p.segment_states || p.segment_states_bytes == plan_kept(p, true).bytes) return MM_OK;
+    return set_error(MM_ERR_INVALID_ARGUMENT, "delta rule: segment_states is not of mm_delta_segment_states_size()");
+}
 static void set_kept(Args &a, const Kept &w, void *place) {
     char *at = static_cast<char *>(place);
     a.segs = w.cut.segs;
@@ -441,6 +451,7 @@ extern "C" int mm_delta_fwd(const mm_delta_fwd_params *params, void *stream) {
     if (p.seqlen == 0) return p.last_state ? la::launch_copy(p.last_state, p.initial_state, bh * p.dk * p.dv, s) : MM_OK;
     if (!p.q || !p.k || !p.v || !p.beta || !p.out)
         return set_error(MM_ERR_INVALID_ARGUMENT, "mm_delta_fwd: q, k, v, beta and out are required");
+    if (const int rc = dr::check_kept(p)) return rc;
     if (!p.workspace || p.workspace_bytes < dr::fwd_bytes(p))
         return set_error(MM_ERR_INVALID_ARGUMENT, "mm_delta_fwd: the workspace is smaller than mm_delta_fwd_workspace_size()");
     if (!dr::near({p.q_seq_stride, p.k_seq_stride, p.v_seq_stride, p.out_seq_stride}))
@@ -475,6 +486,7 @@ extern "C" int mm_delta_bwd(const mm_delta_bwd_params *params, void *stream) {
     }
     if (!p.q || !p.k || !p.v || !p.beta || !p.dout || !p.dq || !p.dk_out || !p.dv_out || !p.dbeta)
         return set_error(MM_ERR_INVALID_ARGUMENT, "mm_delta_bwd: q, k, v, beta, dout, dq, dk_out, dv_out and dbeta are required");
+    if (const int rc = dr::check_kept(p)) return rc;
     if (!p.workspace || p.workspace_bytes < dr::plan_bwd(p).bytes)
         return set_error(MM_ERR_INVALID_ARGUMENT, "mm_delta_bwd: the workspace is smaller than mm_delta_bwd_workspace_size()");
     if (!dr::near({p.q_seq_stride, p.k_seq_stride, p.v_seq_stride, p.do_seq_stride, p.nheads * p.dk, p.nheads * p.dv}))

@@ -1071,7 +1071,10 @@ std::vector<at::Tensor> delta_fwd(const at::Tensor &q, const at::Tensor &k, cons
     p.last_state = last.defined() ? last.data_ptr<float>() : nullptr;
     p.out_batch_stride = out.stride(0); p.out_seq_stride = seq_stride(out); p.out_head_stride = out.stride(2);
     at::Tensor ws, kept;
-    if (keep_states) p.segment_states = workspace_of(kept, mm_delta_segment_states_size(&p), v);
+    if (keep_states) {
+        p.segment_states_bytes = mm_delta_segment_states_size(&p);
+        p.segment_states = workspace_of(kept, p.segment_states_bytes, v);
+    }
     p.workspace_bytes = mm_delta_fwd_workspace_size(&p);
     p.workspace = workspace_of(ws, p.workspace_bytes, v);
     check_rc(mm_delta_fwd(&p, c10::hip::getCurrentHIPStream().stream()), "mm_delta_fwd");
@@ -1113,7 +1116,10 @@ std::vector<c10::optional<at::Tensor>> delta_bwd(const at::Tensor &q, const at::
     p.dlog_decay = dg.defined() ? dg.data_ptr() : nullptr;
     p.dinitial_state = ds.defined() ? ds.data_ptr<float>() : nullptr;
     p.decay_per_head = decay_per_head;
-    p.segment_states = states_.has_value() && states_.value().defined() ? states_.value().data_ptr() : nullptr;
+    if (states_.has_value() && states_.value().defined()) {
+        p.segment_states = states_.value().data_ptr();
+        p.segment_states_bytes = int64_t(states_.value().nbytes());
+    }
     p.do_batch_stride = dout.stride(0); p.do_seq_stride = seq_stride(dout); p.do_head_stride = dout.stride(2);
     at::Tensor ws;
     p.workspace_bytes = mm_delta_bwd_workspace_size(&p);

@@ -125,6 +125,31 @@ def test_workspaces_are_enough_by_a_byte(blocks):
             assert size(_fill(blocks, name + "_params", **{**block, "seqlen": 0})) == 0 == size(None)
 
 
+def test_segment_states_of_another_size_are_refused(blocks, monkeypatch):
+    """The forward's and backward's cuts of a row are the same, or the call is refused (MM_DELTA_SEGMENTS may change between the two)."""
+    monkeypatch.setenv("MM_DELTA_SEGMENTS", "3")
+    size = _lib().mm_delta_segment_states_size
+    size.restype = ctypes.c_int64
+    sizes = {t: size(_fill(blocks, "mm_delta_fwd_params", **{**FWD, "itype": t, "seqlen": 200})) for t in (0, 1, 2)}
+    assert all(sizes.values())
+    for name, base in (("mm_delta_fwd", FWD), ("mm_delta_bwd", BWD)):
+        for t, n in sizes.items():
+            block = {**base, "itype": t, "seqlen": 200, "segment_states": 4096}
+            work = getattr(_lib(), name + "_workspace_size")
+            work.restype = ctypes.c_int64
+            least = work(_fill(blocks, name + "_params", **{**block, "segment_states_bytes": n}))
+            assert least < work(_fill(blocks, name + "_params", **{**block, "segment_states": 0}))
+            for bytes_ in (0, n - 16, n + 16):
+                rc, msg = _call(name, _fill(blocks, name + "_params", **{**block, "segment_states_bytes": bytes_}))
+                assert rc == -1 and "segment_states" in msg, (rc, msg)
+            rc, msg = _call(name, _fill(blocks, name + "_params", **{**block, "segment_states_bytes": n, "workspace_bytes": least - 1}))
+            assert rc == -1 and "workspace" in msg, (rc, msg)
+            monkeypatch.setenv("MM_DELTA_SEGMENTS", "1")
+            rc, msg = _call(name, _fill(blocks, name + "_params", **{**block, "segment_states_bytes": n}))
+            assert rc == -1 and "segment_states" in msg, (rc, msg)
+            monkeypatch.setenv("MM_DELTA_SEGMENTS", "3")
+
+
 def test_nothing_to_do(blocks):
     assert _call("mm_delta_fwd", _fill(blocks, "mm_delta_fwd_params", **{**SIZES, "batch": 0}))[0] == 0
     assert _call("mm_delta_fwd", _fill(blocks, "mm_delta_fwd_params", **{**SIZES, "seqlen": 0}))[0] == 0
