@@ -201,6 +201,132 @@ def test_one_row_s_values_stay_in_it():
         assert torch.isnan(b[1]).any() or n in ("v", "initial_state")
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("segs", [1, 2, 3, 7])
+def test_segments(segs, dtype, monkeypatch):
+    """Rows cut into segments, the last one shorter or of one token: outputs, states and gradients as without; heads of a group, one
+    decay per head, no initial state."""
+    _say(f"delta segments {segs} {dtype}")
+    monkeypatch.setenv("MM_DELTA_SEGMENTS", str(segs))
+    for L, dk, dv in ((449, 64, 48), (300, 128, 128), (200, 100, 72), (33, 16, 16)):
+        _forward(case(segs, 1, L, 2, 1, dk, dv, dtype))
+        _backward(case(dk, 2, L, 2, 1, dk, dv, dtype), L)
+    t = case(44, 1, 257, 3, 3, 40, 40, dtype, decay="head", states=False)
+    _forward(t)
+    _backward(t, 45, dlast=False)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_segments_kept_and_computed_again(dtype, monkeypatch):
+    """The backward gives the same bits with the forward's segment states as without them."""
+    _say(f"delta kept segments {dtype}")
+    from motif_mamba_amd._native import ext
+    monkeypatch.setenv("MM_DELTA_SEGMENTS", "4")
+    d = _dev(case(46, 2, 300, 2, 2, 64, 64, dtype))
+    args = [d[n] for n in ref.NAMES[:5]] + [0.125, d["initial_state"]]
+    *_, kept = ext().delta_fwd(*args, True, True)
+    dout, dlast = torch.randn_like(d["v"]), torch.randn_like(d["initial_state"])
+    a, b = (ext().delta_bwd(*args, dout, dlast, s, False, True, True) for s in (kept, None))
+    for x, y in zip(a, b):
+        assert torch.equal(x, y)
+    monkeypatch.setenv("MM_DELTA_SEGMENTS", "5")
+    with pytest.raises(RuntimeError, match="segment_states"):
+        ext().delta_bwd(*args, dout, dlast, kept, False, True, True)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("segs", [2, 5])
+def test_segments_not_finite(segs, dtype, monkeypatch):
+    """As test_infinities_and_nan, in every segment, of one (batch row, head) beside others that stay as they were."""
+    _say(f"delta segments not finite {segs} {dtype}")
+    from motif_mamba_amd import delta_rule_fn
+    monkeypatch.setenv("MM_DELTA_SEGMENTS", str(segs))
+    inf, nan = float("inf"), float("nan")
+    plain = case(47, 1, 330, 2, 1, 32, 24, dtype)
+    before = delta_rule_fn(**_dev(plain), return_last_state=True)
+    for name, at, bad in (("v", (0, 3, 1, 7), inf), ("v", (0, 200, 1, 7), nan), ("v", (0, 329, 1, 7), inf), ("beta", (0, 170, 1), nan), ("beta", (0, 70, 1), inf),
+                          ("log_decay", (0, 100, 1), nan), ("log_decay", (0, 290, 1), inf), ("log_decay", (0, 2, 1), inf), ("initial_state", (0, 1, 4, 5), -inf),
+                          ("initial_state", (0, 1, 4, 5), nan)):
+        t = {n: x.clone() for n, x in plain.items()}
+        t[name][at] = bad
+        with torch.no_grad():
+            exact = ref.recurrence(*(t[n].double() for n in ref.NAMES[:5]), 32 ** -0.5, t["initial_state"].double())
+        got = delta_rule_fn(**_dev(t), return_last_state=True)
+        assert torch.equal(got[0][:, :, 0], before[0][:, :, 0]) and torch.equal(got[1][:, 0], before[1][:, 0]), name
+        for what, g, e in zip(("out", "last_state"), got, exact):
+            g = g.cpu().double()
+            fin = torch.isfinite(e)
+            assert torch.equal(torch.isnan(g), torch.isnan(e)), (name, what, torch.isnan(g).sum(), torch.isnan(e).sum())
+            assert torch.equal(g[~fin & ~torch.isnan(e)], e[~fin & ~torch.isnan(e)]), (name, what)
+            m = e[fin].abs().max() if fin.any() else 0.0
+            assert ((g - e)[fin].abs() <= ref.ROUND[got[0].dtype] * e[fin].abs() + 4 * 1024 * 2 ** -24 * m).all(), (name, what)
+
+
+def test_segments_in_a_graph(monkeypatch):
+    _say("delta segments graph")
+    from motif_mamba_amd import delta_rule_fn
+    monkeypatch.setenv("MM_DELTA_SEGMENTS", "3")
+    t = case(48, 1, 400, 2, 1, 64, 64, BF16)
+    d = _dev(t)
+    dout = torch.randn(t["v"].shape).to(BF16).to(DEV)
+
+    def go():
+        x = {n: y.detach().requires_grad_(True) for n, y in d.items()}
+        out, last = delta_rule_fn(**x, return_last_state=True)
+        return [out, last, *torch.autograd.grad([out, last], list(x.values()), [dout, d["initial_state"]])]
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        go()
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        res = go()
+    for i in range(3):
+        r = torch.Generator().manual_seed(50 + i)
+        d["v"].copy_(torch.randn(t["v"].shape, generator=r))
+        if i == 1:
+            d["v"][0, 5, 1] = float("inf")   # the row goes in one piece, and in segments again after that
+        g.replay()
+        torch.cuda.synchronize()
+        got = [x.clone() for x in res]
+        want = go()
+        torch.cuda.synchronize()
+        for x, y in zip(got, want):
+            assert torch.equal(torch.nan_to_num(x.float(), 7.0), torch.nan_to_num(y.float(), 7.0)), i
+
+
+def test_a_token_that_sees_no_other():
+    """Its decay has no gradient at all, and the state before it has none of what comes after a forgotten one."""
+    _say("delta lone token")
+    from motif_mamba_amd import delta_rule_fn
+    for dtype in (BF16, F16, F32):
+        d = _dev(case(49, 2, 1, 2, 1, 64, 64, dtype, states=False), True)
+        (g,) = torch.autograd.grad(delta_rule_fn(**d).float().sum(), [d["log_decay"]])
+        assert not g.any()
+        t = case(51, 1, 90, 2, 1, 64, 64, dtype)
+        t["log_decay"][:, 40] = float("-inf")
+        d = _dev(t, True)
+        out = delta_rule_fn(**d)
+        (s,) = torch.autograd.grad(out[:, 40:].float().sum(), [d["initial_state"]])
+        assert not s.any()
+
+
+def test_update_many_pairs():
+    """Pairs by the hundred thousand, more than fill the card several times over: each as alone."""
+    _say("delta update many pairs")
+    from motif_mamba_amd import delta_rule_update
+    for dk, dv in ((8, 16), (16, 40), (8, 72)):
+        t = {n: x[:, 0] if n != "initial_state" else x for n, x in _dev(case(52, 4, 1, 3, 1, dk, dv, F32)).items()}
+        one = t["initial_state"].clone()
+        out = delta_rule_update(one, *(t[n] for n in ref.NAMES[:5]))
+        many = t["initial_state"].repeat(20000, 1, 1, 1)
+        outs = delta_rule_update(many, *(t[n].repeat(20000, *[1] * (t[n].dim() - 1)) for n in ref.NAMES[:5]))
+        assert torch.equal(outs, out.repeat(20000, 1, 1)) and torch.equal(many, one.repeat(20000, 1, 1, 1))
+
+
 def test_layouts():
     """Slices of one projection, aligned and not, a transposed batch, one beta and decay for all tokens: the same values."""
     _say("delta layouts")
