@@ -295,9 +295,9 @@ __device__ __forceinline__ void write_image(char *dst, const float *f, int wave,
 
 // The records of every chunk: the images of P and M; REV, for the backward: that of P, and those of P^T and M^T. One workgroup per chunk. The triangles are made in float32: the diagonal tiles of P by substitution, row by row, those of a column
 // block below by 16 x 16 products on v_mfma_f32_16x16x4_f32, which keeps them float32.
-template <typename T, int KD> constexpr int kPrepGroups = Cfg<T>::C == 32 && KD == 64 ? 4 : sizeof(T) == 2 ? 3 : 2;   // on a CU, by registers
+template <typename T, int KD, bool VEC> constexpr int kPrepGroups = Cfg<T>::C == 32 && KD == 64 && VEC ? 4 : sizeof(T) == 2 && (VEC || KD == 64) ? 3 : 2;   // on a CU, by registers
 template <typename T, int KD, bool REV, bool VEC>
-__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kPrepGroups<T, KD>, kPrepGroups<T, KD>))) dr_prep(const Args) {
+__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kPrepGroups<T, KD, VEC>, kPrepGroups<T, KD, VEC>))) dr_prep(const Args) {
     constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, CT = C / 16, LD = kPitch<C>;
     typedef Stage<T, C, KD, kThreads, VEC> SX;
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -655,6 +655,7 @@ __device__ __forceinline__ void recur_delta(f32x4 (&S)[KD / 16][NC], const u16 *
         for (int c = 0; c < NC; ++c) z[c] = o[c] = 0.f;
 #pragma unroll
         for (int k = 0; k < KD / 16; ++k) {
+            kdim = afresh(kdim);   // (no masks of all rows held at once)
             float y[4];
             tile_row4<T, C, KD>(y, K, t, 16 * k + 4 * g);
 #pragma unroll
@@ -673,9 +674,9 @@ __device__ __forceinline__ void recur_delta(f32x4 (&S)[KD / 16][NC], const u16 *
             z[c] += __shfl_xor(z[c], 32);
             z[c] = (tile_at<T, C, LDV>(V, t, col + 16 * c + i) - z[c]) * ck.beta[t];
         }
-        kdim = afresh(kdim);   // (no masks of all rows held from the loop above)
 #pragma unroll
         for (int k = 0; k < KD / 16; ++k) {
+            kdim = afresh(kdim);
             float y[4], x[4];
             tile_row4<T, C, KD>(y, K, t, 16 * k + 4 * g);
             tile_row4<T, C, KD>(x, Q, t, 16 * k + 4 * g);
@@ -713,7 +714,7 @@ __device__ __forceinline__ void start_state(f32x4 (&S)[KD / 16][1], const Args &
 // that met one is followed by this: the recurrence once more from its start, whose outputs from the wave's first such chunk on (`first`),
 // and state, take the others' place. Its arguments are read again, so that nothing of it takes registers while the products run.
 template <typename T, int KD, bool VEC>
-__device__ __forceinline__ void infinite_rows(f32x4 (&S)[KD / 16][1], char *smem, int seg, int beg, int end, int first) {
+__device__ __forceinline__ void infinite_rows(f32x4 (&S)[KD / 16][1], char *smem, int beg, int end, int first) {
     constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, W = 64;
     auto args = [] { return own_args<Args>(); };
     u16 *K = reinterpret_cast<u16 *>(smem), *Q = K + PI * kTile<C, KD>, *V = Q + PI * kTile<C, KD>;
@@ -723,7 +724,7 @@ __device__ __forceinline__ void infinite_rows(f32x4 (&S)[KD / 16][1], char *smem
     const Spot p = spot_of(args(), u.pair);
     const int col0 = int(u.slice) * W;
     f32x4 R[KD / 16][1];
-    start_state<KD>(R, args(), p, seg, col0, col, lane);
+    start_state<KD>(R, args(), p, u.seg, col0, col, lane);
     __threadfence();   // the outputs that are stored once more
 #pragma unroll 1
     for (int t0 = beg; t0 < end; t0 += C) {
@@ -827,7 +828,7 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
     const Rows<T> rk = tensor([&](const Args &a) { return rows_of<T>(a.k, p.b, p.h, a.dk); });
     const Rows<T> rq = kOut ? tensor([&](const Args &a) { return rows_of<T>(a.q, p.b, p.h, a.dk); }) : rk;
     const Rows<T> rv = tensor([&](const Args &a) { return rows_of<T>(a.v, p.b, p.h, a.dv, col0); });
-    const int stride = afresh(args().rec_a_step);
+    const int stride = kOut ? kRecord<C, 2> : afresh(args().rec_a_step);
     const char *records = tensor([&](const Args &a) { return afresh(a.rec_a + int64_t(p.bh) * a.chunks * a.rec_a_step); });
     char *const out = tensor([&](const Args &a) {
         return kOut ? afresh(static_cast<char *>(a.out) + (p.b * a.out_batch + p.h * a.out_head + col0) * int64_t(sizeof(T))) : nullptr;
@@ -934,7 +935,7 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
     }
     if constexpr (kOut) {
         held.flush(out, out_stride, beg + (end - 1 - beg) / C * C, rv.d, col, lane);
-        if (__syncthreads_or(first_odd < end)) infinite_rows<T, KD, VEC>(S, smem, u.seg, beg, end, first_odd);
+        if (__syncthreads_or(first_odd < end)) infinite_rows<T, KD, VEC>(S, smem, beg, end, first_odd);
     }
     const Args a = args();
     if constexpr (kOut) {

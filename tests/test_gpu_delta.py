@@ -179,6 +179,33 @@ def test_infinities_and_nan(dtype):
             assert ((g - e)[fin].abs() <= ref.ROUND[got[0].dtype] * e[fin].abs() + 4 * 1024 * 2 ** -24 * m).all(), (name, what)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("dk,dv", [(128, 128), (100, 72), (66, 33), (64, 128)])
+def test_infinities_of_larger_heads(dk, dv, dtype):
+    """As above, several at once, in whole and broken 16-byte pieces, of rows beside others that stay as they were."""
+    _say(f"delta not finite {dk} {dv} {dtype}")
+    from motif_mamba_amd import delta_rule_fn
+    inf, nan = float("inf"), float("nan")
+    plain = case(53, 2, 150, 2, 1, dk, dv, dtype)
+    before = delta_rule_fn(**_dev(plain), return_last_state=True)
+    t = {n: x.clone() for n, x in plain.items()}
+    t["v"][0, 40, 1, 7] = inf
+    t["v"][0, 130, 1, dv - 1] = -inf
+    t["beta"][1, 149, 0] = nan
+    t["initial_state"][1, 1, dk - 1, dv - 1] = inf
+    with torch.no_grad():
+        exact = ref.recurrence(*(t[n].double() for n in ref.NAMES[:5]), dk ** -0.5, t["initial_state"].double())
+    got = delta_rule_fn(**_dev(t), return_last_state=True)
+    assert torch.equal(got[0][0, :, 0], before[0][0, :, 0]) and torch.equal(got[1][0, 0], before[1][0, 0])
+    assert torch.equal(got[0][1, :128, 0], before[0][1, :128, 0])   # (the chunks before its own, which goes token by token)
+    for what, g, e in zip(("out", "last_state"), got, exact):
+        g = g.cpu().double()
+        fin = torch.isfinite(e)
+        assert torch.equal(torch.isnan(g), torch.isnan(e)), (what, torch.isnan(g).sum(), torch.isnan(e).sum())
+        assert torch.equal(g[~fin & ~torch.isnan(e)], e[~fin & ~torch.isnan(e)]), what
+        assert ((g - e)[fin].abs() <= ref.ROUND[got[0].dtype] * e[fin].abs() + 4 * 1024 * 2 ** -24 * e[fin].abs().max()).all(), what
+
+
 def test_one_row_s_values_stay_in_it():
     """NaN in one (batch row, head) reaches no other's outputs or gradients."""
     _say("delta NaN of another row")
