@@ -462,6 +462,27 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(k
 
 // ---- walks ---------------------------------------------------------------------------------------
 
+// Stage with its pieces' halves swapped by selects, and one address and constants for all pieces of a thread (they are whole blocks of
+// 16 rows apart): 100 vector instructions of a walk's chunk less (bfloat16; the other types' stores are the base's).
+template <typename T, int C, int D, int NT, bool VEC>
+struct Staged : Stage<T, C, D, NT, VEC> {
+    typedef Stage<T, C, D, NT, VEC> S;
+    __device__ __forceinline__ void store(u16 *tile, int tid) const {
+        if constexpr (std::is_same_v<T, bf16_t> && S::RS % 16 == 0 && S::kEven) {
+            static_assert(S::VE == 8, "two units of four elements");
+            const int row = unsigned(tid) / S::VR, col = unsigned(tid) % S::VR * 8, sw = swizzle(row);
+            u16 *dst = tile + row * D + (row >> 4) * 8 + ((((col >> 2) ^ sw) & ~1) << 2);
+#pragma unroll
+            for (int n = 0; n < S::N; ++n) {
+                const uint4 r = S::r[n];
+                const uint64_t lo = uint64_t(r.y) << 32 | r.x, hi = uint64_t(r.w) << 32 | r.z, x = sw & 1 ? hi : lo, y = sw & 1 ? lo : hi;
+                *reinterpret_cast<uint4 *>(dst + n * (S::RS * D + S::RS / 16 * 8)) = make_uint4(uint32_t(x), uint32_t(x >> 32), uint32_t(y), uint32_t(y >> 32));
+            }
+        } else {
+            S::store(tile, tid);
+        }
+    }
+};
 // A record on its way from memory to LDS.
 template <int BYTES>
 struct StageRecord {
@@ -514,6 +535,24 @@ __device__ __forceinline__ Unit unit_of(const Args &a, unsigned slices) {
     return u;
 }
 inline int64_t unit_grid(const Args &a, int slices) { return (a.batch * a.heads * a.segs + 7) / 8 * 8 * slices; }
+
+// Two workgroups on a CU: of two waves that could issue the older one does, so that one workgroup runs ahead and leaves the other its CU
+// alone at the end. A wave gives way with every quarter of its chunks that it has done (of `n`): 64 pairs of 128 x 128 in four segments of
+// 1,024 tokens, two groups on every CU: 142 us where the older one's way took 153, prompts of 160 pairs in one piece 491 and 523.
+struct Turns {
+    int quarter, left;
+    __device__ __forceinline__ void start(int n) {
+        quarter = afresh((n + 3) / 4);
+        left = 4 * quarter;
+        __builtin_amdgcn_s_setprio(3);
+    }
+    __device__ __forceinline__ void step() {
+        --left;
+        if (left == 3 * quarter) __builtin_amdgcn_s_setprio(2);
+        if (left == 2 * quarter) __builtin_amdgcn_s_setprio(1);
+        if (left == quarter) __builtin_amdgcn_s_setprio(0);
+    }
+};
 
 // The wave's outputs of a chunk. Whole 16-byte pieces leave by way of its own columns of V, which no other wave reads (see
 // store_out); they are held until the next chunk's rows are staged, so that those wait for no store.
@@ -778,8 +817,8 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
     constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, W = 64, NC = 1, CT = C / 16;
     constexpr bool kOut = L == kOutputs;
     constexpr int kLoaded = kRecord<C, kOut ? 2 : 1>;
-    typedef Stage<T, C, KD, kThreads, VEC> SX;
-    typedef Stage<T, C, W, kThreads, VEC> SV;
+    typedef Staged<T, C, KD, kThreads, VEC> SX;
+    typedef Staged<T, C, W, kThreads, VEC> SV;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     u16 *K = reinterpret_cast<u16 *>(smem), *Q = K + PI * kTile<C, KD>, *V = kOut ? Q + PI * kTile<C, KD> : Q;
     u16 *img = V + PI * kTile<C, W>;
@@ -853,14 +892,17 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
     load_rows(beg);
     HeldOut<T, C, W, VEC> held;
     int first_odd = 0x7fffffff;   // the first chunk with something not finite in it
+    Turns turns;   // (of aligned rows: the element-wise loads have no scalars left for it)
+    if constexpr (VEC) turns.start((end - beg + C - 1) / C);
     for (int t0 = beg; t0 < end; t0 += C) {
         const int rows = min(C, end - t0);
+        if constexpr (VEC) turns.step();
         __syncthreads();
         fresh();
         sk.store(K, tid);
-        si.store(reinterpret_cast<char *>(img), tid);
         if constexpr (kOut) sq.store(Q, tid);
         sv.store(V, tid);
+        si.store(reinterpret_cast<char *>(img), tid);
         if constexpr (kOut)
             if (t0 > beg) held.flush(out, out_stride, t0 - C, rv.d, col, lane);
         if (t0 + C < end) load_rows(t0 + C);
@@ -913,15 +955,12 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
                 split8(y, w[j][0]);
             }
             triangle<C, NC, true, kPlanes>(O, img + kImage<C>, w, lane);
-            // 0 times what is not finite is not 0.
+            // 0 times what is not finite is not 0. (A row of U that is not finite is in its own row tile's products, and makes NaN of them.)
             float nan = 0.f;
 #pragma unroll
             for (int t = 0; t < CT; ++t)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    nan = __builtin_fmaf(X[t][0][r], 0.f, nan);
-                    nan = __builtin_fmaf(O[t][0][r], 0.f, nan);
-                }
+                for (int r = 0; r < 4; ++r) nan = __builtin_fmaf(O[t][0][r], 0.f, nan);
             if (first_odd > t0 && __any(!(nan == 0.f))) first_odd = t0;
         }
         if (t0 + C < end) load_record(t0 + C);
@@ -954,8 +993,8 @@ template <typename T, int KD, bool MAPS, bool VEC>
 __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) dr_back(const Args) {
     constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, W = 64, NC = 1, CT = C / 16;
     constexpr int kRec = kRecord<C, 2>;
-    typedef Stage<T, C, KD, kThreads, VEC> SX;
-    typedef Stage<T, C, W, kThreads, VEC> SV;
+    typedef Staged<T, C, KD, kThreads, VEC> SX;
+    typedef Staged<T, C, W, kThreads, VEC> SV;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     u16 *K = reinterpret_cast<u16 *>(smem), *Q = K + PI * kTile<C, KD>, *V = Q + PI * kTile<C, KD>;
     u16 *img = V + PI * kTile<C, W>;
@@ -1013,8 +1052,11 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
     };
     load(last);
     HeldOut<T, C, W, VEC> held;
+    Turns turns;
+    if constexpr (VEC) turns.start(last - first + 1);
     for (int n = last; n >= first; --n) {
         const int t0 = n * C, rows = min(C, end - t0);
+        if constexpr (VEC) turns.step();
         __syncthreads();
         fresh();
         sk.store(K, tid);
