@@ -14,11 +14,11 @@
 //     dQ = scale diag(e^c) dO S^T + A K,                    A = the lower triangle of scale dO U^T . D
 //     dK = A^T Q + E K + E^T K - diag(e^c) dV S^T + diag(e^(c_end - c)) U R^T,   E = minus the strict one of dV U^T . D
 // P and M need no state: dr_prep makes them for all chunks at once, dr_walk carries the state through a row's chunks, dr_back the
-// state's gradient back (rows of few heads in segments: a first walk finds what each adds to the state and what it makes of it, dr_join
-// the states that they start from), and dr_grad takes dQ and dK chunk by chunk from the kept S, R, Z and dV, again all chunks at once.
+// state's gradient back, and dr_grad takes dQ and dK chunk by chunk from the kept S, R, Z and dV, again all chunks at once. Rows of few heads
+// run in segments: a first walk finds what each adds to the state and what it makes of it, dr_join the states that they start from.
 //
-// Exactness: as in the linear attention, every float32 factor (S, R, P, M, U, dV and the decayed scores) enters its product as
-// three bfloat16 planes (2^-25), for every input type; 16-bit results are rounded once.
+// Exactness: every float32 factor (S, R, P, M, U, dV and the decayed scores) enters its product as three bfloat16 planes (2^-25), for
+// every input type: two would be 2^-17 per factor, and errors of the state add up over the chunks. 16-bit results are rounded once.
 //
 // Built once per input type: this file for float32, mm_delta_f16.hip / mm_delta_bf16.hip, which set MM_DELTA_TYPE.
 #ifndef MM_DELTA_TYPE
@@ -121,7 +121,7 @@ __device__ __forceinline__ void tile_products(f32x4 *s, const u16 *X, const u16 
     const int g = lane >> 4, i = lane & 15;
     constexpr int B = PY > 1 ? 3 : 4;   // tiles whose operands are held at once
 #pragma unroll
-    for (int k = 0; k < D / 32; ++k)
+    for (int k = 0; k < D / 32; ++k) {
 #pragma unroll
         for (int j0 = 0; j0 < L::N; j0 += B) {
             bf16x8 a[B][PY], b[B][PX];
@@ -143,6 +143,8 @@ __device__ __forceinline__ void tile_products(f32x4 *s, const u16 *X, const u16 
 #pragma unroll
                         for (int j = 0; j < B && j0 + j < L::N; ++j) s[j0 + j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[j][p], b[j][q], s[j0 + j], 0, 0, 0);
         }
+        if (k % 2) __builtin_amdgcn_sched_barrier(0);   // (no more than two steps' operands held)
+    }
 }
 // The waves' shares of a chunk's lower triangle of tiles.
 template <int C, typename F>
@@ -259,8 +261,8 @@ __device__ __forceinline__ void tile_columns(const u16 *V, int col, int lane, F 
 template <int C> constexpr int kPitch = C + 4;
 
 // A triangle in `f` (row-major, pitch kPitch; 0 above the diagonal in the tiles on it, tiles above it not written) as operands, TR: its
-// transpose.
-template <int C, bool TR>
+// transpose. NW waves share it.
+template <int C, bool TR, int NW = kWaves>
 __device__ __forceinline__ void write_image(char *dst, const float *f, int wave, int lane) {
     const int g = lane >> 4, i = lane & 15;
 #pragma unroll
@@ -269,7 +271,7 @@ __device__ __forceinline__ void write_image(char *dst, const float *f, int wave,
         for (int j = 0; j < C / 32; ++j)
             if (has_frag<C, !TR>(t, j)) {
                 const int n = frag_at<C, !TR>(t, j);
-                if (n % kWaves != wave) continue;
+                if (n % NW != wave) continue;
                 float x[8];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
@@ -293,20 +295,31 @@ __device__ __forceinline__ void write_image(char *dst, const float *f, int wave,
             }
 }
 
-// The records of every chunk: the images of P and M; REV, for the backward: that of P, and those of P^T and M^T. One workgroup per chunk. The triangles are made in float32: the diagonal tiles of P by substitution, row by row, those of a column
-// block below by 16 x 16 products on v_mfma_f32_16x16x4_f32, which keeps them float32.
-template <typename T, int KD, bool VEC> constexpr int kPrepGroups = Cfg<T>::C == 32 && KD == 64 && VEC ? 4 : sizeof(T) == 2 && (VEC || KD == 64) ? 3 : 2;   // on a CU, by registers
+// The records of every chunk: the images of P and M; REV, for the backward: that of P, and those of P^T and M^T. One workgroup per chunk. The
+// triangles are made in float32: the diagonal tiles of P by substitution, row by row, those of a column block below by 16 x 16 products on
+// v_mfma_f32_16x16x4_f32, which keeps them float32. Bound by what it stores (38 KB for a chunk of 64, 57 with REV) and by the substitution's
+// latency, which the workgroups on a CU hide for each other: 10,240 chunks at dk 128, 384 MB of operands, 134 us (2.9 TB/s). Two on a CU, as
+// with M in LDS of its own, took 180, and so did three with spills; M lies in P's place, and waves that do not substitute write its image.
+// A workgroup that takes several chunks and loads ahead was slower: the loads' wait is one for the stores before them too.
+template <typename T, int KD> constexpr int kPrepGroups = KD == 64 || sizeof(T) == 2 ? 4 : 3;   // on a CU, by registers
 template <typename T, int KD, bool REV, bool VEC>
-__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kPrepGroups<T, KD, VEC>, kPrepGroups<T, KD, VEC>))) dr_prep(const Args) {
+__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kPrepGroups<T, KD>, kPrepGroups<T, KD>))) dr_prep(const Args) {
     constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, CT = C / 16, LD = kPitch<C>;
     typedef Stage<T, C, KD, kThreads, VEC> SX;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     u16 *K = reinterpret_cast<u16 *>(smem), *Q = K + PI * kTile<C, KD>;
-    float *N = reinterpret_cast<float *>(smem), *P = N + C * LD, *M = P + C * LD;   // over K and Q, once those are read
-    constexpr int kTiles = 2 * 2 * PI * kTile<C, KD>, kTri = 3 * C * LD * 4;
+    float *N = reinterpret_cast<float *>(smem), *P = N + C * LD, *M = P;   // over K and Q, once those are read; P over M
+    constexpr int kTiles = 2 * 2 * PI * kTile<C, KD>, kTri = 2 * C * LD * 4;
     Chunk<C> *ck = reinterpret_cast<Chunk<C> *>(smem + (kTiles > kTri ? kTiles : kTri));
     auto args = [] { return own_args<Args>(); };
-    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid & 63, g = lane >> 4, i = lane & 15;
+    int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, i = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
+    auto fresh = [&] {   // (no addresses of later steps held from here)
+        tid = afresh_lane(tid);
+        lane = tid & 63;
+        g = lane >> 4;
+        i = lane & 15;
+    };
     const int64_t total = [&] { const Args a = args(); return a.batch * a.heads * a.chunks; }();
     for (int64_t id = blockIdx.x; id < total; id += gridDim.x) {
         // Heads next to each other: those of a group read the same rows of q and k.
@@ -321,6 +334,7 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(k
         const int t0 = chunk * C, rows = min(C, afresh(int(args().seqlen)) - t0);
         uint32_t gbits = 0, bbits = 0;
         __syncthreads();
+        fresh();
         {
             SX sk, sq;
             {
@@ -340,6 +354,7 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(k
             sq.store(Q, tid);
         }
         __syncthreads();
+        fresh();
         f32x4 n[3], m[3];
         each_tile<C>(wave, [&](auto Lc) {
             typedef decltype(Lc) L;
@@ -353,6 +368,7 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(k
             make_chunk<C>(*ck, gbits, a.g.type, bbits, a.beta.type, a.scale, lane);
         }
         __syncthreads();
+        fresh();
         const float scale = args().scale;
         each_tile<C>(wave, [&](auto Lc) {
             typedef decltype(Lc) L;
@@ -370,9 +386,20 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(k
             });
         });
         __syncthreads();
-        // Diagonal tiles, one per 16 lanes: a lane has a column. N is 0 from the diagonal on, and so is x.
-        if (wave == 0 && g < CT) {
-            float x[16], w[16];   // P and B P
+        fresh();
+        char *ra, *rb;
+        {
+            const Args a = args();
+            const int64_t at = p.bh * a.chunks + chunk;
+            ra = afresh(a.rec_a) + at * kRecord<C, REV ? 1 : 2>;
+            rb = REV ? afresh(a.rec_b) + at * kRecord<C, 2> : nullptr;
+        }
+        // Diagonal tiles, one per 16 lanes: a lane has a column. N is 0 from the diagonal on, and so is x. M's image by the other waves
+        // meanwhile.
+        float x[16], w[16];   // P and B P
+        if (wave > 0) {
+            write_image<C, REV, kWaves - 1>((REV ? rb : ra) + kImage<C> * 2, M, wave - 1, lane);
+        } else if (g < CT) {
             const float *Nd = N + 16 * g * LD + 16 * g, *bt = ck->beta + 16 * g;
             f32x4 n4[2][4];
             float own[2], bs[2];
@@ -396,10 +423,14 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(k
                 x[r] = s + s2;
                 w[r] = bs[r % 2] * x[r];
             }
-#pragma unroll
-            for (int r = 0; r < 16; ++r) P[(16 * g + r) * LD + 16 * g + i] = x[r];
         }
         __syncthreads();
+        fresh();
+        if (wave == 0 && g < CT)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) P[(16 * g + r) * LD + 16 * g + i] = x[r];
+        __syncthreads();
+        fresh();
         // The tiles below them, a wave its column block J: P_IJ = (1 + P_II B_I) Y, Y = -(N_IJ + sum over K of N_IK B_K P_KJ).
         auto column = [&](auto Jc) {
             constexpr int J = decltype(Jc)::value;
@@ -441,21 +472,12 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(k
             case 2: if constexpr (CT > 2) column(std::integral_constant<int, 2>{});
         }
         __syncthreads();
-        {
-            const Args a = args();
-            const int64_t at = p.bh * a.chunks + chunk;
-            char *ra = afresh(a.rec_a) + at * kRecord<C, REV ? 1 : 2>;
-            write_image<C, false>(ra, P, wave, lane);
-            if constexpr (!REV) {
-                write_image<C, false>(ra + kImage<C> * 2, M, wave, lane);
-                write_steps<C>(ra + 2 * kImage<C> * 2, *ck, tid);
-            } else {
-                write_steps<C>(ra + kImage<C> * 2, *ck, tid);
-                char *rb = afresh(a.rec_b) + at * kRecord<C, 2>;
-                write_image<C, true>(rb, P, wave, lane);
-                write_image<C, true>(rb + kImage<C> * 2, M, wave, lane);
-                write_steps<C>(rb + 2 * kImage<C> * 2, *ck, tid);
-            }
+        fresh();
+        write_image<C, false>(ra, P, wave, lane);
+        write_steps<C>(ra + (REV ? 1 : 2) * kImage<C> * 2, *ck, tid);
+        if constexpr (REV) {
+            write_image<C, true>(rb, P, wave, lane);
+            write_steps<C>(rb + 2 * kImage<C> * 2, *ck, tid);
         }
     }
 }
@@ -811,7 +833,10 @@ enum Leaves {
     kMaps       // of a segment: what it adds to the state (V's columns) and what it makes of it (as many columns as rows, from the identity)
 };
 
-// The state's way through a segment's chunks, a workgroup 64 columns of it, a wave 16.
+// The state's way through a segment's chunks, a workgroup 64 columns of it, a wave 16. A chunk's steps hang on each other (split the state,
+// K S and Q S, split, P, split, M, the update), so that latency bounds it: at dk 128 in bfloat16 4.6 us per chunk where a workgroup is alone on its
+// CU (10,300 cycles, the matrix cores busy for 3,456), 7.7 to 8.9 where two are; 160 pairs of 128 x 128, L 4,096: 491 us. Both
+// 64-column halves of a head in one workgroup of eight waves, with one staging: at most 8 % less, 2 % of a training step.
 template <typename T, int KD, Leaves L, bool VEC>
 __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) dr_walk(const Args) {
     constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, W = 64, NC = 1, CT = C / 16;
@@ -988,7 +1013,8 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
 }
 
 // The state's gradient R back through a segment's chunks: dV, dbeta's shares, R at every chunk's end, and the first state's gradient.
-// MAPS: what a segment adds to R alone.
+// MAPS: what a segment adds to R alone. Bound as dr_walk is, with the states' gradients and dV's float32 rows stored beside it: 64 pairs of
+// 128 x 128, L 4,096, four segments, bfloat16: 216 us, the maps 143.
 template <typename T, int KD, bool MAPS, bool VEC>
 __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) dr_back(const Args) {
     constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, W = 64, NC = 1, CT = C / 16;
@@ -1144,7 +1170,8 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
 
 // The segments' maps (B | A: what they add, what they make of the state) into the states that they start from; BACK: into R at their ends,
 // by the transposes of A. One workgroup per 32 columns of a (batch row, head); its waves split the rows, in float32 on
-// v_mfma_f32_16x16x4_f32, the next segment's map on its way meanwhile. A row that holds something not finite is flagged.
+// v_mfma_f32_16x16x4_f32, the next segment's map on its way meanwhile. A row that holds something not finite is flagged. A chain of one step per
+// segment, whatever the pairs: some 6 us a step at dk 128 (four segments of 64 pairs: 22 us), 2.3 at 64.
 template <int KD, bool BACK>
 __global__ void __launch_bounds__(kThreads) dr_join(const Args) {
     constexpr int NT = KD / 64, NC = 2;   // tiles of 16 rows, of 16 columns per wave
@@ -1432,6 +1459,10 @@ __device__ __forceinline__ void each_tile_of_two(int wave, F &&f) {
 // forgotten state, which no pair crosses,
 //     dg_t = sum of (row sum - column sum without f) + sum over j < t of f_j + e^c_end <R, S>.
 // A's diagonal would be in a row sum and in a column sum alike; it is added to dQ and dK behind them.
+//
+// Bound by the LDS's latency at two waves per SIMD (138 KB at dk 128, one workgroup on a CU): 64 pairs of 128 x 128, L 4,096, bfloat16, heads of
+// 4 sharing q and k: 420 us, matrix cores 21 % and vector units 40 % busy, a third of the LDS cycles conflicts, in the transposed
+// triangles' reads; 192 pairs of 64 x 64, L 2,048: 260 us. dO, U and dV in the order of their operands took 498 to 422 and 294 to 260.
 template <typename T, int KD, bool VEC, bool F32>
 __global__ void __launch_bounds__(KD * 4) __attribute__((amdgpu_waves_per_eu(2, 2))) dr_grad(const Args) {
     constexpr int C = Cfg<T>::C, PI = Cfg<T>::in, CT = C / 16, NC = 1, NW = KD / 16, NT = 64 * NW, PM = kTile<C, kScoreRow>;
@@ -1758,7 +1789,7 @@ constexpr int64_t kMostGroups = int64_t(1) << 17;   // of a launch that loops ov
 template <typename T, int KD, bool REV, bool VEC>
 static int prep_t(const Args &a, hipStream_t s) {
     constexpr int C = Cfg<T>::C, PI = Cfg<T>::in;
-    constexpr int tiles = 2 * 2 * PI * kTile<C, KD>, tri = 3 * C * kPitch<C> * 4, bytes = (tiles > tri ? tiles : tri) + int(sizeof(Chunk<C>));
+    constexpr int tiles = 2 * 2 * PI * kTile<C, KD>, tri = 2 * C * kPitch<C> * 4, bytes = (tiles > tri ? tiles : tri) + int(sizeof(Chunk<C>));
     static std::atomic<uint64_t> done{0};
     return launch_kernel(dr_prep<T, KD, REV, VEC>, bytes, done, std::min<int64_t>(a.batch * a.heads * a.chunks, kMostGroups), kThreads, a, s, "dr_prep");
 }

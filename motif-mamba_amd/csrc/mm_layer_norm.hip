@@ -6,6 +6,9 @@
 // results need no second read. Pieces of 16 bytes of x at any alignment; weight and bias come from the cache row by row. The backward
 // adds its rows' dweight and dbias in registers, one partial row per block, which a second kernel sums in order (no atomics: the same
 // bits on every call).
+//
+// 16,384 rows of 2,560, bfloat16 with a float32 residual: forward 89 us (5.6 TB/s, x and residual in part from the last-level cache; 96.5
+// in calls of their own, a large copy's rate), backward 145 (4.2 TB/s: the rows' sums, with two blocks per CU), ln_sum 5. 64 rows: 3.6 us.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
