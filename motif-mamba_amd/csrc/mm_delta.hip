@@ -1171,7 +1171,8 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
 // The segments' maps (B | A: what they add, what they make of the state) into the states that they start from; BACK: into R at their ends,
 // by the transposes of A. One workgroup per 32 columns of a (batch row, head); its waves split the rows, in float32 on
 // v_mfma_f32_16x16x4_f32, the next segment's map on its way meanwhile. A row that holds something not finite is flagged. A chain of one step per
-// segment, whatever the pairs: some 6 us a step at dk 128 (four segments of 64 pairs: 22 us), 2.3 at 64.
+// segment, whatever the pairs: some 6 us a step at dk 128 (four segments of 64 pairs: 22 us), 1.6 at 64 (21 segments of 24 pairs: 35 us);
+// three or five maps on their way took as long.
 template <int KD, bool BACK>
 __global__ void __launch_bounds__(kThreads) dr_join(const Args) {
     constexpr int NT = KD / 64, NC = 2;   // tiles of 16 rows, of 16 columns per wave

@@ -248,6 +248,8 @@ struct Cut {
 // 1.85 of that for both): the first walk over all segments but the last (0.85 of a chunk; slices of V's columns and of the map's), the
 // join, and the walk itself. A training step (`train`) runs the backward's walks on the same segments: states (0.9) and R (1.6), R once
 // more before that (1.3), and another join.
+// 24 pairs of 64 x 64, 32,768 tokens, float32: 709 us in segments, the walk alone 3,845 in one piece; 48 pairs, 1,777 tokens, bfloat16: 76,
+// the walk alone 121. 160 pairs of 4,096 tokens go in one piece, 546 us, and so do the 192 of a training step.
 static Cut segments(int64_t pairs, int64_t seqlen, int64_t dk, int64_t dv, mm_dtype t, bool train) {
     const int C = chunk_tokens(t);
     const int64_t chunks = (seqlen + C - 1) / C, cus = device_simds() / 4, vs = pad64(dv) / 64, ks = pad64(dk) / 64;
