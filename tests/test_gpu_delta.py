@@ -325,6 +325,38 @@ def test_segments_in_a_graph(monkeypatch):
             assert torch.equal(torch.nan_to_num(x.float(), 7.0), torch.nan_to_num(y.float(), 7.0)), i
 
 
+def test_backward_twice_and_two_streams(monkeypatch):
+    """A graph that is kept gives the same gradients again, and calls on two streams at once each their own."""
+    _say("delta backward twice")
+    from motif_mamba_amd import delta_rule_fn
+    monkeypatch.setenv("MM_DELTA_SEGMENTS", "3")
+    cases = [_dev(case(seed, 2, 500, 4, 2, 64, 128, BF16), True) for seed in (54, 55)]
+    dout = torch.randn(cases[0]["v"].shape).to(BF16).to(DEV)
+
+    def go(d):
+        out, last = delta_rule_fn(**d, return_last_state=True)
+        return [torch.autograd.grad([out, last], list(d.values()), [dout, d["initial_state"].detach()], retain_graph=True) for _ in range(2)]
+
+    alone = []
+    for d in cases:
+        one, two = go(d)
+        for x, y in zip(one, two):
+            assert torch.equal(x, y)
+        alone.append(one)
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = []
+    for s, d in zip(streams, cases):
+        with torch.cuda.stream(s):
+            got.append([go(d) for _ in range(3)])
+    torch.cuda.synchronize()
+    for runs, want in zip(got, alone):
+        for pair in runs:
+            for grads in pair:
+                for x, y in zip(grads, want):
+                    assert torch.equal(x, y)
+
+
 def test_a_token_that_sees_no_other():
     """Its decay has no gradient at all, and the state before it has none of what comes after a forgotten one."""
     _say("delta lone token")

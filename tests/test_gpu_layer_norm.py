@@ -250,6 +250,25 @@ def test_graph():
             assert torch.equal(x, y), i
 
 
+def test_backward_twice_and_a_changed_residual():
+    """A graph that is kept gives the same gradients again; the residual stream that it holds may not change before that."""
+    _say("layer norm backward twice")
+    from motif_mamba_amd import layer_norm_fn
+    r = torch.Generator().manual_seed(61)
+    x = torch.randn(70, 96, generator=r).to(torch.bfloat16).to(DEV).requires_grad_(True)
+    res = torch.randn(70, 96, generator=r).to(DEV).requires_grad_(True)
+    w = torch.randn(96, generator=r).to(DEV).requires_grad_(True)
+    y, h = layer_norm_fn(x, w, residual=res, prenorm=True, is_rms_norm=True)
+    dy, dh = torch.ones_like(y), torch.ones_like(h)
+    one, two = (torch.autograd.grad([y, h], [x, res, w], [dy, dh], retain_graph=True) for _ in range(2))
+    for a, b in zip(one, two):
+        assert torch.equal(a, b)
+    with torch.no_grad():
+        h.add_(1.0)
+    with pytest.raises(RuntimeError, match="inplace"):
+        torch.autograd.grad(y, [x], dy)
+
+
 def test_against_differences():
     _say("layer norm differences")
     from motif_mamba_amd import layer_norm_fn
