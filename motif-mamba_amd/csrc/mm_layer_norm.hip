@@ -68,10 +68,11 @@ __device__ __forceinline__ void weight_piece(const void *p, mm_dtype dt, int c, 
     else unpack_raw(load_piece<bf16_t, VE>(static_cast<const bf16_t *>(p), c), w);
 }
 
-// Sum over a row's threads: W waves, in the same order in every thread; `buf` alternates between two halves so that one barrier per
-// sum is enough.
+// Sums of one or two values over a row's threads: W waves, in the same order in every thread; `buf` (4 W floats) alternates between two
+// halves, which lie alike for one value and two: no wave writes where another may still read, with one barrier per sum.
 template <int W, int N>
 __device__ __forceinline__ void row_sum(float (&x)[N], float *buf, int &half) {
+    static_assert(N <= 2, "a half has 2 W floats");
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         x[i] = group_sum<16>(x[i]);
@@ -79,7 +80,7 @@ __device__ __forceinline__ void row_sum(float (&x)[N], float *buf, int &half) {
         x[i] += __shfl_xor(x[i], 32);
     }
     if constexpr (W > 1) {
-        float *b = buf + half * W * N;
+        float *b = buf + half * 2 * W;
         half ^= 1;
         if (threadIdx.x % 64 == 0)
 #pragma unroll
@@ -149,7 +150,7 @@ struct Row {
 
 template <typename T, typename R, int W, int VE, int NV>
 __global__ void __launch_bounds__(kThreads) ln_fwd(const mm_layer_norm_params p) {
-    __shared__ float buf[2 * W];
+    __shared__ float buf[4 * W];
     const int size = int(p.channels);
     const int64_t row = int64_t(blockIdx.x) * (4 / W) + threadIdx.x / (64 * W);
     if (row >= p.rows) return;   // whole waves, and whole blocks where they meet at a barrier
@@ -187,7 +188,7 @@ __global__ void __launch_bounds__(kThreads) ln_fwd(const mm_layer_norm_params p)
 // Waves (W = 4: blocks) take every gridDim.x-th row; part: [block][2][channels].
 template <typename T, typename R, int W, int VE, int NV, bool DB>
 __global__ void __launch_bounds__(kThreads) ln_bwd(const mm_layer_norm_params p, float *part) {
-    __shared__ float buf[2 * 2 * W], sums[W == 1 ? 3 * 64 * VE : 1];
+    __shared__ float buf[4 * W], sums[W == 1 ? 3 * 64 * VE : 1];
     const int size = int(p.channels);
     const Split<W, VE> s(threadIdx.x % (64 * W), size);
     int half = 0;

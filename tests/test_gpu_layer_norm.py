@@ -220,6 +220,29 @@ def test_same_bits_and_another_stream():
         assert torch.equal(x, y)
 
 
+@pytest.mark.parametrize("dtype,residual", [(BF16, F32), (F32, F32)])
+@pytest.mark.parametrize("rms", [False, True])
+@pytest.mark.parametrize("n", [4104, 5001])
+def test_rows_of_four_waves_many_to_a_block(n, rms, dtype, residual):
+    """Waves that exchange their sums through LDS, row after row: the formula's values, and the same bits on every call."""
+    _say(f"layer norm four waves {n} rms={rms} {dtype} {residual}")
+    from motif_mamba_amd import layer_norm_fn
+    t = _case(n, 1300, n, dtype, residual)
+    _check(t, rms, True)
+    dev = {k: x.to(DEV) for k, x in _case(n + 1, 2000, n, dtype, residual).items()}
+    douts = [torch.randn(2000, n, device=DEV).to(x) for x in (dtype, residual)]
+
+    def go():
+        d = {k: x.detach().requires_grad_(True) for k, x in dev.items()}
+        outs = layer_norm_fn(**d, prenorm=True, is_rms_norm=rms)
+        return [*outs, *torch.autograd.grad(outs, list(d.values()), douts)]
+
+    one = go()
+    for _ in range(3):
+        for i, (x, y) in enumerate(zip(one, go())):
+            assert torch.equal(x, y), i
+
+
 def test_graph():
     _say("layer norm graph")
     from motif_mamba_amd import layer_norm_fn
