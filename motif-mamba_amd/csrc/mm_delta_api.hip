@@ -95,10 +95,10 @@ __global__ void __launch_bounds__(512) dr_update(const mm_delta_update_params p,
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < RPT; ++r) {
-        const float kk = kq[0][row0 + r * ROWS];
+        const float kk = kq[0][row0 + r * ROWS], gr = row0 + r * ROWS < dk ? g : 0.f;   // rows past dk stay 0 whatever the growth
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            w[r][e] *= g;
+            w[r][e] *= gr;
             z[e] = __builtin_fmaf(kk, w[r][e], z[e]);
         }
     }

@@ -522,6 +522,32 @@ def test_update_infinities():
             assert torch.allclose(g.double(), x, rtol=1e-4, atol=1e-4, equal_nan=True), name
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("dk,dv", [(1, 1), (8, 64), (24, 32), (40, 80), (64, 64), (65, 16), (100, 128), (128, 128)])
+def test_infinite_growth(dk, dv, dtype):
+    """An infinite decay factor under a negative beta: the state, what it gives and what a further token reads of it are infinite, and NaN
+    only where the recurrence has one; rows that fill a head up to the kernel's size take no part."""
+    _say(f"delta infinite growth {dk} {dv} {dtype}")
+    from motif_mamba_amd import delta_rule_fn, delta_rule_update
+    t = case(36, 1, 2, 2, 1, dk, dv, dtype)
+    for n in ("q", "k", "initial_state"):
+        t[n] = t[n].abs() + 0.25
+    t["beta"] = -t["beta"] - 0.25
+    t["initial_state"][0, 1] *= -1
+    t["log_decay"][0, 0, 1] = t["log_decay"][0, 1, 0] = float("inf")
+    with torch.no_grad():
+        out, last = ref.recurrence(*(t[n].double() for n in ref.NAMES[:5]), dk ** -0.5, t["initial_state"].double())
+    fin = torch.isfinite(out)
+    assert torch.isinf(last).all() and fin[0, 0, 0].all() and fin.sum() == dv   # the first token of the head that grows at the second
+    t["log_decay"][0, 1, 0] = 129.0   # counts as infinite
+    d = _dev(t)
+    state = d["initial_state"].clone()
+    outs = [delta_rule_update(state, *(d[n][:, i] for n in ref.NAMES[:5])) for i in range(2)]
+    for what, (o, s) in (("update", (torch.stack(outs, 1), state)), ("prompt", delta_rule_fn(**d, return_last_state=True))):
+        o = o.cpu().double()
+        assert torch.equal(s.cpu().double(), last) and torch.isfinite(o[fin]).all() and torch.equal(o[~fin], out[~fin]), what
+
+
 def test_prompt_then_tokens():
     _say("delta prompt then tokens")
     from motif_mamba_amd import delta_rule_fn, delta_rule_update
