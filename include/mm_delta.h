@@ -109,10 +109,11 @@ typedef struct mm_delta_update_params {
     int64_t g_batch_stride, g_head_stride;
 } mm_delta_update_params;
 
-/* Workspace bytes (0: none needed). They depend on the sizes and on the current device's compute-unit count: query with the device of
- * the call current. They also depend on whether segment_states and the backward's dlog_decay are NULL: query with those pointers set
- * as in the call. segment_states' own size is 0 where rows are not cut: leave it NULL then. A call refuses segment_states of any other
- * size than the query's, as after a change of MM_DELTA_SEGMENTS (the number of segments, for measurements) between the two. */
+/* Workspace bytes (0: none needed, or sizes that the call refuses). They depend on the sizes and on the current device's
+ * compute-unit count: query with the device of the call current. They also depend on whether segment_states and the backward's
+ * dlog_decay are NULL: query with those pointers set as in the call. segment_states' own size is 0 where rows are not cut: leave it NULL
+ * then. A call refuses segment_states of any other size than the query's, as after a change of MM_DELTA_SEGMENTS (the number of
+ * segments, for measurements) between the two. */
 int64_t mm_delta_fwd_workspace_size(const mm_delta_fwd_params *params);
 int64_t mm_delta_segment_states_size(const mm_delta_fwd_params *params);
 int64_t mm_delta_bwd_workspace_size(const mm_delta_bwd_params *params);

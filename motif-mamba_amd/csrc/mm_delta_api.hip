@@ -197,6 +197,12 @@ static int check(const P &p, int64_t seqlen, int64_t pairs) {
     return MM_OK;
 }
 
+// A size query has something to count: the plan's arithmetic is for calls that are not refused.
+template <typename P>
+static bool asks(const P *p) {
+    return p && p->batch > 0 && p->seqlen > 0 && p->nheads > 0 && check(*p, p->seqlen, kMostPairs) == MM_OK;
+}
+
 // A tile's rows are addressed with 32-bit offsets.
 static bool near(std::initializer_list<int64_t> strides) {
     for (const int64_t s : strides)
@@ -429,17 +435,17 @@ static int run_bwd(const mm_delta_bwd_params &p, hipStream_t s) {
 using namespace mm;
 
 extern "C" int64_t mm_delta_fwd_workspace_size(const mm_delta_fwd_params *p) {
-    if (!p || p->batch <= 0 || p->seqlen <= 0 || p->nheads <= 0) return 0;
+    if (!dr::asks(p)) return 0;
     return dr::fwd_bytes(*p);
 }
 
 extern "C" int64_t mm_delta_segment_states_size(const mm_delta_fwd_params *p) {
-    if (!p || p->batch <= 0 || p->seqlen <= 0 || p->nheads <= 0) return 0;
+    if (!dr::asks(p)) return 0;
     return dr::plan_kept(*p, true).bytes;
 }
 
 extern "C" int64_t mm_delta_bwd_workspace_size(const mm_delta_bwd_params *p) {
-    if (!p || p->batch <= 0 || p->seqlen <= 0 || p->nheads <= 0) return 0;
+    if (!dr::asks(p)) return 0;
     return dr::plan_bwd(*p).bytes;
 }
 

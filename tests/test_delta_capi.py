@@ -5,6 +5,7 @@ import ctypes
 import os
 import re
 import subprocess
+import sys
 
 import pytest
 import torch
@@ -148,6 +149,31 @@ def test_segment_states_of_another_size_are_refused(blocks, monkeypatch):
             rc, msg = _call(name, _fill(blocks, name + "_params", **{**block, "segment_states_bytes": n}))
             assert rc == -1 and "segment_states" in msg, (rc, msg)
             monkeypatch.setenv("MM_DELTA_SEGMENTS", "3")
+
+
+@pytest.mark.parametrize("segments", [None, "1", "4"])
+@pytest.mark.parametrize("change", [dict(batch=1 << 20, nheads=2), dict(batch=1 << 62, nheads=8), dict(batch=1 << 32, nheads=1 << 32), dict(dk=129), dict(dv=0),
+                                    dict(seqlen=(1 << 23) + 1), dict(n_groups=0), dict(itype=7)])
+def test_sizes_of_refused_calls(blocks, change, segments):
+    """The size queries, which come before the call that refuses, need nothing for it and end as they should, with any number of segments
+    asked for. (In a process of its own, which a division by zero would end.)"""
+    work = []
+    for name, base in (("mm_delta_fwd", FWD), ("mm_delta_bwd", BWD)):
+        block = bytes(_fill(blocks, name + "_params", **{**base, "seqlen": 200, **change})).hex()
+        work += [(f, block) for f in ([name + "_workspace_size"] + (["mm_delta_segment_states_size"] if name == "mm_delta_fwd" else []))]
+    code = f"""
+import ctypes, sys
+lib = ctypes.CDLL({_lib()._name!r})
+for name, block in {work!r}:
+    f = getattr(lib, name)
+    f.restype = ctypes.c_int64
+    raw = bytes.fromhex(block)
+    print(name, f((ctypes.c_char * len(raw)).from_buffer_copy(raw)), flush=True)
+"""
+    env = {n: x for n, x in os.environ.items() if n != "MM_DELTA_SEGMENTS"}
+    res = subprocess.run([sys.executable, "-c", code], env={**env, **({"MM_DELTA_SEGMENTS": segments} if segments else {})}, stdout=subprocess.PIPE, timeout=120)
+    assert res.returncode == 0, (res.returncode, res.stdout)
+    assert res.stdout.decode().split("\n")[:-1] == [f"{f} 0" for f, _ in work]
 
 
 def test_nothing_to_do(blocks):
