@@ -46,7 +46,7 @@ class GatedDeltaBlock(nn.Module):
         """(conv_state, state) of an empty text."""
         w = self.conv_weight
         return (torch.zeros(batch_size, self.d_qkv, self.d_conv, device=w.device, dtype=w.dtype),
-                torch.zeros(batch_size, self.nheads, self.d_state, self.headdim, device=w.device))
+                torch.zeros(batch_size, self.nheads, self.d_state, self.headdim, device=w.device, dtype=torch.float32))
 
     def _enter(self, hidden, residual):
         x, residual = self.norm(hidden, residual, prenorm=True, residual_in_fp32=self.residual_in_fp32)

@@ -41,7 +41,7 @@ class LinearAttentionBlock(nn.Module):
         """(conv_state, state) of an empty text."""
         w = self.conv_weight
         return (torch.zeros(batch_size, self.d_xbc, self.d_conv, device=w.device, dtype=w.dtype),
-                torch.zeros(batch_size, self.nheads, self.d_state, self.headdim, device=w.device))
+                torch.zeros(batch_size, self.nheads, self.d_state, self.headdim, device=w.device, dtype=torch.float32))
 
     def _split(self, zxdt):
         return zxdt.split([self.d_inner, self.d_xbc, self.nheads], -1)
