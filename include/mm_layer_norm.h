@@ -50,8 +50,8 @@ typedef struct mm_layer_norm_params {
 } mm_layer_norm_params;
 
 int mm_layer_norm_fwd(const mm_layer_norm_params *params, void *stream);
-/* Workspace bytes (0: none needed). They depend on which pointers are set, on the tensors' alignment and row strides, and on the
- * current device's compute-unit count: query with the call's own parameters, its device current. */
+/* Workspace bytes (0: none needed). They depend on rows, channels and itype, on whether dweight or dbias is set, and on the current
+ * device's compute-unit count: query with the call's own parameters, its device current. */
 int64_t mm_layer_norm_bwd_workspace_size(const mm_layer_norm_params *params);
 int mm_layer_norm_bwd(const mm_layer_norm_params *params, void *stream);
 

@@ -48,8 +48,8 @@ __device__ __forceinline__ void row_sums(float (&x)[4], float4 (*part)[LPR]) {
 
 // S' = exp(g) S, u = beta (v - S'^T k), S = S' + k u^T, o = scale S^T q. Bound by the state, read once and written once: a workgroup
 // holds one (batch row, head)'s columns of it (4 LPR of them) in registers between the two. LPR lanes cover a row in 16-byte pieces, RPT
-// rows each. 256 x 40 heads of 128 x 128: 276 us, 1.34 GB at 4.9 TB/s (a large copy reaches 5.2); with twice the rows per lane and so half
-// the workgroups on a CU 304, with waves of 32 columns that meet no other 359.
+// rows each. 256 x 40 heads of 128 x 128: 269 us, 1.34 GB at 5.0 TB/s (a large copy reaches 5.2); with twice the rows per lane and so half
+// the workgroups on a CU 304, with waves of 32 columns that meet no other 359 (on a card where the first took 276).
 template <typename T, int LPR, int RPT>
 __global__ void __launch_bounds__(512) dr_update(const mm_delta_update_params p, int slices) {
     constexpr int NT = LPR == 32 ? 512 : 256, ROWS = NT / LPR;
@@ -253,7 +253,8 @@ struct Cut {
 // By the time that the passes over a row of n segments take, in chunks of one workgroup of dr_walk alone on its CU (two on a CU take
 // 1.85 of that for both): the first walk over all segments but the last (0.85 of a chunk; slices of V's columns and of the map's), the
 // join, and the walk itself. A training step (`train`) runs the backward's walks on the same segments: states (0.9) and R (1.6), R once
-// more before that (1.3), and another join.
+// more before that (1.3), and another join. The times are bfloat16's, of 64 tokens a chunk; the other types' chunks have 32 and up to twice
+// the products, and no ratios of their own were taken.
 // 24 pairs of 64 x 64, 32,768 tokens, float32: 709 us in segments, the walk alone 3,845 in one piece; 48 pairs, 1,777 tokens, bfloat16: 76,
 // the walk alone 121. 160 pairs of 4,096 tokens go in one piece, 546 us, and so do the 192 of a training step.
 static Cut segments(int64_t pairs, int64_t seqlen, int64_t dk, int64_t dv, mm_dtype t, bool train) {

@@ -8,7 +8,9 @@
 // bits on every call).
 //
 // 16,384 rows of 2,560, bfloat16 with a float32 residual: forward 89 us (5.6 TB/s, x and residual in part from the last-level cache; 96.5
-// in calls of their own, a large copy's rate), backward 145 (4.2 TB/s: the rows' sums, with two blocks per CU), ln_sum 5. 64 rows: 3.6 us.
+// in calls of their own, a large copy's rate), backward 145 (4.6 TB/s: the rows' sums, with two blocks per CU), ln_sum 5. 64 rows: 3.6 us.
+// Wider rows of as many elements: 10,240 of 4,096 backward 176 us (3.8 TB/s; eight pieces of a thread take 314 registers, with dbias 378, so
+// that a SIMD holds one wave and half the blocks wait for the other half), 8,192 of 5,120 146, 2,560 of 16,384 with mean and dbias 196.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
