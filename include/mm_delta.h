@@ -15,7 +15,8 @@
  * -128 count as -128, whose exponential is 0 in float32, values above 128 as 128, whose exponential is infinite. NaN stays NaN.
  *
  * Infinities and NaN: outputs and states of mm_delta_fwd and mm_delta_update are what the recurrence makes of them (chunks that one
- * reaches run token by token, many times slower). Gradients of a (batch row, head) that one reaches are NaN or infinite.
+ * reaches run token by token, many times slower). In the gradients of its (batch row, head) what one reaches is NaN or infinite, and
+ * other elements may be NaN.
  *
  * Conventions as in mm_scan.h: device pointers, element strides, outputs allocated by the caller, nothing is synchronised or
  * allocated, 0 or a code of mm_scan.h is returned and mm_last_error() has the text. The innermost dimension (dk or dv) of q, k, v,

@@ -14,8 +14,8 @@ group per head gives it) and beta to lie between 0 and 2. Without log_decay noth
 float32, float16 and bfloat16; beta and log_decay may have dtypes of their own (float32 is advised: a decay's error is raised to the
 power of its memory). Sums, scores and states are float32 from end to end; 16-bit outputs are rounded once. log_decay is meant to be
 at most 0; -inf forgets the state, so a packed batch marks each document's first token with it (below -128 counts as that, above 128
-as an infinite growth). Infinities and NaN in the inputs give the outputs and states of the recurrence, slowly; the gradients of a
-(batch row, head) that one reaches are NaN or infinite.
+as an infinite growth). Infinities and NaN in the inputs give the outputs and states of the recurrence, slowly; in the gradients of
+its (batch row, head) what one reaches is NaN or infinite, and other elements may be NaN.
 
 dk and dv up to 128 (else NotImplementedError).
 """
